@@ -158,12 +158,12 @@ def prepare(case, seed):
         s["k"], s["v"] = randn(B, n, Hkv, D), randn(B, n, Hkv, D)
         for x in ("k", "v"):
             if case["op"] == "fill":
-                s[x + "8"] = torch.zeros(B, T, Hkv, D, dtype=torch.int8, device="cuda")
-                s[x + "s"] = torch.zeros(B, nb, Hkv, device="cuda")
+                s[x + "8"] = torch.zeros(B, Hkv, T, D, dtype=torch.int8, device="cuda")
+                s[x + "s"] = torch.zeros(B, Hkv, nb, device="cuda")
             else:
-                s[x + "8"] = torch.randint(-127, 128, (B, T, Hkv, D), generator=g, device="cuda", dtype=torch.int8)
-                s[x + "s"] = (3.0 + torch.rand(B, nb, Hkv, generator=g, device="cuda")) / 127.0 / 2.0
-            s[x + "t"] = randn(B, block, Hkv, D)
+                s[x + "8"] = torch.randint(-127, 128, (B, Hkv, T, D), generator=g, device="cuda", dtype=torch.int8)
+                s[x + "s"] = (3.0 + torch.rand(B, Hkv, nb, generator=g, device="cuda")) / 127.0 / 2.0
+            s[x + "t"] = randn(B, Hkv, block, D)
         if case["op"] == "fill":
             s["start"] = torch.zeros(B, dtype=torch.int32, device="cuda")
             s["count"] = ints(n // 2, n + 1, B)
@@ -323,7 +323,8 @@ def _write_plain(s, x):
     """The new tokens of s[x] go into the cache's blocks (the complete ones) and its tail (the last, incomplete one)."""
     new, c8, cs, tail = s[x], s[x + "8"], s[x + "s"], s[x + "t"]
     B, n, Hkv, D = new.shape
-    T, block = c8.shape[1], tail.shape[1]
+    T, block = c8.shape[2], tail.shape[2]
+    tail = tail.transpose(1, 2)
     start, total = s["start"].long()[:, None], s["total"].long()[:, None]
     # the blocks that new tokens fall into, complete with the tail's tokens before them
     nb = (n + block - 1) // block + (0 if n % block == 0 and s["case"]["op"] == "fill" else 1)
@@ -340,21 +341,20 @@ def _write_plain(s, x):
     which = at[:, ::block] // block  # (B, nb)
     done = (which + 1) * block <= total
     b, j = done.nonzero(as_tuple=True)
-    c8.view(B, T // block, block, Hkv, D)[b, which[b, j]] = eight[b, j]
-    cs[b, which[b, j]] = scale[b, j]
+    c8.view(B, Hkv, T // block, block, D).permute(0, 2, 3, 1, 4)[b, which[b, j]] = eight[b, j]
+    cs.transpose(1, 2)[b, which[b, j]] = scale[b, j]
     b, j = ((at >= start) & (at < total) & (at >= total // block * block)).nonzero(as_tuple=True)
     tail[b, at[b, j] % block] = val[b, j].to(tail.dtype)
 
 
 def _read_plain(s, x):
-    """The cached states in fp32 (B, T, Hkv, D), zero past each sequence's length, and which are there."""
+    """The cached states in fp32 (B, Hkv, T, D), zero past each sequence's length, and which are there."""
     c8, cs, tail = s[x + "8"], s[x + "s"], s[x + "t"]
-    B, T = c8.shape[:2]
-    block = tail.shape[1]
+    T, block = c8.shape[2], tail.shape[2]
     at, total = torch.arange(T, device="cuda"), s["total"][:, None]
-    full = c8.float() * cs.repeat_interleave(block, 1)[..., None]
-    full = torch.where((at < total // block * block)[..., None, None], full, tail.float()[:, at % block])
-    return torch.where((at < total)[..., None, None], full, 0.0), at < total
+    full = c8.float() * cs.repeat_interleave(block, 2)[..., None]
+    full = torch.where((at < total // block * block)[:, None, :, None], full, tail.float()[:, :, at % block])
+    return torch.where((at < total)[:, None, :, None], full, 0.0), at < total
 
 
 @torch.no_grad()
@@ -366,8 +366,8 @@ def _kv8_plain(s):
     v, _ = _read_plain(s, "v")
     dt = s["kt"].dtype
     if c["op"] == "fill":
-        return {"k": k.to(dt), "v": v.to(dt), "kt": s["kt"], "vt": s["vt"]}
-    q, k, v = _heads(s["q"], c["Hkv"]), _heads(k, c["Hkv"]), _heads(v, c["Hkv"])
+        return {"k": k.transpose(1, 2).to(dt).contiguous(), "v": v.transpose(1, 2).to(dt).contiguous(), "kt": s["kt"], "vt": s["vt"]}
+    q = _heads(s["q"], c["Hkv"])
     p = _softmax((q * c["D"] ** -0.5) @ k.transpose(-1, -2), there[:, None, None])
     return {"o": _tokens(p @ v, c["n"], c["H"]).to(dt).contiguous(), "kt": s["kt"], "vt": s["vt"]}
 
@@ -466,9 +466,9 @@ def _kv8_exact(s):
         vals = {}
         for x in ("k", "v"):
             val = torch.zeros(T, c["Hkv"], c["D"], dtype=torch.float64, device="cuda")
-            val[:old * block] = (s[x + "8"][b, :old * block].double().unflatten(0, (-1, block))
-                                 * s[x + "s"][b, :old].double()[:, None, :, None]).flatten(0, 1)
-            val[old * block:st] = s[x + "t"][b, :st - old * block].double()
+            held = s[x + "8"][b, :, :old * block].transpose(0, 1).double().unflatten(0, (-1, block))
+            val[:old * block] = (held * s[x + "s"][b, :, :old].T.double()[:, None, :, None]).flatten(0, 1)
+            val[old * block:st] = s[x + "t"][b, :, :st - old * block].transpose(0, 1).double()
             val[st:total] = s[x][b, :total - st].double()
             if full > old:
                 blk = val[old * block:full * block].unflatten(0, (-1, block))
@@ -478,7 +478,7 @@ def _kv8_exact(s):
                 val[old * block:full * block] = (r.double() * sc.double()).flatten(0, 1)
             if total > full * block:
                 a = max(st, full * block)
-                tails[x][b, a - full * block:total - full * block] = s[x][b, a - st:total - st].double()
+                tails[x][b, :, a - full * block:total - full * block] = s[x][b, a - st:total - st].double().transpose(0, 1)
             vals[x] = val
         if c["op"] == "fill":
             outs["k"].append(vals["k"])
