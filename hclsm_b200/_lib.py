@@ -71,9 +71,47 @@ SIGNATURES = {
     "hclsm_relu_bwd": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _i64, _vp]),
     "hclsm_swiglu_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _i32, _vp]),
     "hclsm_event_mha_bwd": (ctypes.c_int, [_vp] * 4 + [_i32] * 4 + [ctypes.c_float, _i32, _vp]),
+    "hclsm_qk_norm_rope": (ctypes.c_int, [_vp] * 4 + [_i32, _i32, _i64, _i32, ctypes.c_float, _i32, _i32, _vp]),
+    "hclsm_qk_norm_rope_bwd_workspace_size": (_sz, [_i32]),
+    "hclsm_qk_norm_rope_bwd": (ctypes.c_int, [_vp] * 4 + [_i32, _i32, _i64, _i32, ctypes.c_float, _i32, _i32, _vp,
+                                                          _sz, _vp]),
+    "hclsm_xattn_fwd_workspace_size": (_sz, [_vp]),
+    "hclsm_xattn_fwd": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "hclsm_xattn_bwd_workspace_size": (_sz, [_vp]),
+    "hclsm_xattn_bwd": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "hclsm_kv8_write": (ctypes.c_int, [_vp] * 3 + [_i32] + [_vp] * 3),
+    "hclsm_kv8_read": (ctypes.c_int, [_vp] * 5),
+    "hclsm_kv8_attn_workspace_size": (_sz, [_vp, _i32, _i32]),
+    "hclsm_kv8_attn": (ctypes.c_int, [_vp] * 4 + [_i32, _i32, ctypes.c_float, _vp, _sz, _vp]),
     "hclsm_ssm_scan_bwd_noalloc_max_scratch": (_sz, []),
     "hclsm_ssm_scan_bwd_noalloc": (ctypes.c_int, [_vp] * 15 + [_i64, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
+
+
+class View(ctypes.Structure):
+    """hclsm_view: a (B, L, H, D) tensor whose last dim is dense."""
+    _fields_ = [("p", ctypes.c_void_p), ("sb", ctypes.c_int64), ("st", ctypes.c_int64), ("sh", ctypes.c_int64)]
+
+
+class RopeSide(ctypes.Structure):
+    """hclsm_rope_side."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "dy", "y", "w", "pos", "dw")] + \
+               [(n, ctypes.c_int64) for n in ("sb", "st", "sh")] + [("L", ctypes.c_int32), ("H", ctypes.c_int32)]
+
+
+class XattnArgs(ctypes.Structure):
+    """hclsm_xattn_args."""
+    _fields_ = [(n, View) for n in ("q", "k", "v", "dout")] + \
+               [(n, ctypes.c_void_p) for n in ("o", "dq", "dk", "dv", "lse2", "lens", "mask")] + \
+               [("mask_sb", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)]
+
+
+class Kv8(ctypes.Structure):
+    """hclsm_kv8_cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")] + \
+               [(n, ctypes.c_int32) for n in ("B", "Hkv", "T", "D", "block", "dtype")]
+
 
 class SlotIterWeights(ctypes.Structure):
     """hclsm_slot_iter_weights (include/hclsm_b200.h)."""
@@ -135,3 +173,36 @@ def require_cuda(*tensors) -> torch.device:
         elif t.device != dev:
             raise ValueError("hclsm_b200: all tensors must be on the same device")
     return dev
+
+
+def dense_last(t):
+    """t itself if its last dim is dense, else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def rows16(t):
+    """t itself if its last dim is dense and every row starts on 16 bytes, else an aligned contiguous copy."""
+    e = t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s * e % 16 for s in t.stride()[:-1]):
+        return t
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def view(t):
+    """hclsm_view of a (B, L, H, D) tensor."""
+    s = t.stride()
+    return View(t.data_ptr(), s[0], s[1], s[2])
+
+
+def index32(t, shape, name, device):
+    """An int32, contiguous index tensor of that shape on that device (int64 is converted), or None."""
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    return t.to(torch.int32).contiguous()

@@ -1,0 +1,527 @@
+// Attention of few query rows over long keys, the keys split over thread
+// blocks: the single-token form of the cross attention (states in fp32 or
+// bf16) and the attention over the 8-bit state cache.
+//
+// The rows that share a key head (tokens x query heads of the group) form the
+// M = 16 side of mma.sync m16n8k16 products; a warp takes 16 keys a step:
+//   S = Q K^T  ->  running max / sum  ->  P (fp32 accumulators become the A
+//   fragments of the next product in place)  ->  O += P V.
+// A contraction's index can run in any order, so fragments come straight from
+// global memory with 16-byte loads and no shared memory: for S a lane's four k
+// slots are four consecutive dims of its key's row; for P V a lane holds
+// consecutive dims of the four keys whose scores it has.  8-bit integers become
+// bf16 exactly, two at a time: 0x4300 | low 7 bits is 128 + those bits, and
+// 0x4300 | sign is 128, or 256 for a negative value, so one packed subtraction
+// gives the value.  The scale of a block of keys multiplies its scores (K) and
+// its weights (V).
+// fp32 operands are split into three bf16 pieces (8 bits each) and the products
+// of pieces whose order is at most 2 are summed: fp32 accuracy.
+// Bound: HBM (each key and value byte is read once); splits and warps are merged
+// in a fixed order.
+#include <type_traits>
+
+#include "xattn.cuh"
+
+namespace hclsm {
+namespace split {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;
+
+struct Params {
+  xattn::Params x;  // q, o, lse2, lens, mask, sizes; k and v where the states are dense
+  const int8_t *k8, *v8;      // (B, Hkv, T, D)
+  const float *ks, *vs;       // (B, Hkv, T / block)
+  const void *kt, *vt;        // (B, Hkv, block, D), the last incomplete block
+  int T, block;
+  int splits, rtiles;
+  float* part_o;   // (B * Hkv * rtiles, splits, 16, D)
+  float2* part_ml; // (B * Hkv * rtiles, splits, 16): max, sum
+};
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+      "%2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The N leading bf16 pieces of two fp32 values, packed.
+template <int N>
+__device__ __forceinline__ void pieces(float lo, float hi, uint32_t (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    out[i] = pack(lo, hi);
+    lo -= __uint_as_float(out[i] << 16);
+    hi -= __uint_as_float(out[i] & 0xffff0000u);
+  }
+}
+// Two signed bytes (bits 0-7 and 16-23; the others are ignored) as packed bf16.
+__device__ __forceinline__ uint32_t bytes2(uint32_t t) {
+  const uint32_t m = (t & 0x007f007fu) | 0x43004300u, s = (t & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 r =
+      __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&s));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// How one lane reads rows of D elements of type E: K as D / 4 elements (a quad
+// shares a row), V as D / 8 elements (eight lanes share a row) in runs of CV
+// consecutive dims.  CV fixes which dims an accumulator tile holds, so storage
+// types that meet in one accumulator use the same.
+constexpr int load_bytes(int bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : 4; }
+
+template <typename E, int D, int CV>
+struct Rows {
+  static constexpr int kES = (int)sizeof(E);
+  static constexpr int kPieces = kES == 4 ? 3 : 1;
+  static constexpr int kKB = D / 4 * kES, kVB = D / 8 * kES;  // bytes a lane reads of a row
+  static constexpr int kKC = load_bytes(kKB);                 // bytes of one load
+  static constexpr int kVC = load_bytes(CV * kES);
+  static constexpr int kKW = kKB / 4, kVW = kVB / 4;          // words
+  static constexpr int kCK = kKC / kES;                       // elements of one load of K
+
+  template <int CB>
+  static __device__ __forceinline__ void load(const char* p, uint32_t* w) {
+    if constexpr (CB == 16) {
+      const uint4 r = __ldcs(reinterpret_cast<const uint4*>(p));
+      w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else if constexpr (CB == 8) {
+      const uint2 r = __ldcs(reinterpret_cast<const uint2*>(p));
+      w[0] = r.x, w[1] = r.y;
+    } else {
+      w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    }
+  }
+  // row: address of the key's first element
+  static __device__ __forceinline__ void load_k(const char* row, int c, uint32_t (&w)[kKW]) {
+#pragma unroll
+    for (int i = 0; i < kKB / kKC; ++i) load<kKC>(row + (i * 4 + c) * kKC, w + i * (kKC / 4));
+  }
+  static __device__ __forceinline__ void load_v(const char* row, int g, uint32_t (&w)[kVW]) {
+#pragma unroll
+    for (int i = 0; i < D / 8 / CV; ++i)
+#pragma unroll
+      for (int k = 0; k < CV * kES / kVC; ++k)
+        load<kVC>(row + (i * 8 + g) * CV * kES + k * kVC, w + (i * CV * kES + k * kVC) / 4);
+  }
+  // the dim of lane quad-index c's element 0..3 of k step s
+  static __device__ __forceinline__ int k_dim(int s, int c) {
+    return s / (kCK / 4) * 4 * kCK + c * kCK + s % (kCK / 4) * 4;
+  }
+  // the dim of lane group g's element j
+  static __device__ __forceinline__ int v_dim(int j, int g) { return j / CV * 8 * CV + g * CV + j % CV; }
+
+  // B fragments of k step s
+  static __device__ __forceinline__ void k_frag(const uint32_t (&w)[kKW], int s, uint32_t (&b0)[kPieces],
+                                                uint32_t (&b1)[kPieces]) {
+    if constexpr (kES == 1) {
+      b0[0] = bytes2(__byte_perm(w[s], 0, 0x0100));
+      b1[0] = bytes2(__byte_perm(w[s], 0, 0x0302));
+    } else if constexpr (kES == 2) {
+      b0[0] = w[2 * s], b1[0] = w[2 * s + 1];
+    } else {
+      pieces<3>(__uint_as_float(w[4 * s]), __uint_as_float(w[4 * s + 1]), b0);
+      pieces<3>(__uint_as_float(w[4 * s + 2]), __uint_as_float(w[4 * s + 3]), b1);
+    }
+  }
+  // B fragments of n tile j from the rows of the lane's four keys
+  static __device__ __forceinline__ void v_frag(const uint32_t (&w)[4][kVW], int j, uint32_t (&b0)[kPieces],
+                                                uint32_t (&b1)[kPieces]) {
+    if constexpr (kES == 1) {
+      const uint32_t sel = (j & 3) | ((4 + (j & 3)) << 8);  // byte j of the first word, of the second at bit 16
+      b0[0] = bytes2(__byte_perm(w[0][j / 4], w[1][j / 4], sel));
+      b1[0] = bytes2(__byte_perm(w[2][j / 4], w[3][j / 4], sel));
+    } else if constexpr (kES == 2) {
+      const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
+      b0[0] = __byte_perm(w[0][j / 2], w[1][j / 2], sel);
+      b1[0] = __byte_perm(w[2][j / 2], w[3][j / 2], sel);
+    } else {
+      pieces<3>(__uint_as_float(w[0][j]), __uint_as_float(w[1][j]), b0);
+      pieces<3>(__uint_as_float(w[2][j]), __uint_as_float(w[3][j]), b1);
+    }
+  }
+};
+
+// A warp's running state over its keys.
+template <int D>
+struct State {
+  float o[D / 8][4];
+  float m[2], l[2];
+};
+
+// Queries of the tile in shared memory as fp32 [16][D + 4] (rows past the end are zeros).
+template <typename T, int D, int NQ, typename R>
+__device__ __forceinline__ void q_frag(const float* sq, int s, int g, int c, uint32_t (&a)[NQ][4]) {
+  const int d = R::k_dim(s, c);
+  const float4 x = *reinterpret_cast<const float4*>(sq + g * (D + 4) + d);
+  const float4 y = *reinterpret_cast<const float4*>(sq + (g + 8) * (D + 4) + d);
+  uint32_t t[NQ];
+  pieces<NQ>(x.x, x.y, t);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) a[i][0] = t[i];
+  pieces<NQ>(y.x, y.y, t);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) a[i][1] = t[i];
+  pieces<NQ>(x.z, x.w, t);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) a[i][2] = t[i];
+  pieces<NQ>(y.z, y.w, t);
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) a[i][3] = t[i];
+}
+
+// Steps first, first + stride, ... below last of 16 keys each.  addr_k / addr_v
+// (key) give a row's address; ok(key) says whether the key is allowed (false
+// past the end); nk > 0 keys have memory; all_ok(step) skips the per-key checks.
+template <typename T, typename E, int D, int CV, int NQ, typename AddrK, typename AddrV, typename Ok, typename AllOk,
+          typename Scale>
+__device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, int last, int stride, int nk, float c2,
+                                      AddrK addr_k, AddrV addr_v, Ok ok, AllOk all_ok, Scale scale) {
+  using R = Rows<E, D, CV>;
+  constexpr int NK = R::kPieces, kOrder = (NQ > NK ? NQ : NK) - 1;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  if (first >= last) return;
+  uint32_t kr[2][R::kKW], vr[4][R::kVW];
+  auto fetch_k = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) R::load_k(addr_k(min(step * 16 + t * 8 + g, nk - 1)), c, kr[t]);
+  };
+  auto fetch_v = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) R::load_v(addr_v(min(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1), nk - 1)), g, vr[t]);
+  };
+  float2 sc = scale(first);
+  fetch_k(first);
+  fetch_v(first);
+  for (int step = first; step < last; step += stride) {
+    const int next = step + stride < last ? step + stride : step;
+    float s[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      uint32_t a[NQ][4];
+      q_frag<T, D, NQ, R>(sq, ks, g, c, a);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        uint32_t b0[NK], b1[NK];
+        R::k_frag(kr[t], ks, b0, b1);
+#pragma unroll
+        for (int i = NQ - 1; i >= 0; --i)
+#pragma unroll
+          for (int j = NK - 1; j >= 0; --j)
+            if (i + j <= kOrder) mma(s[t], a[i], b0[j], b1[j]);
+      }
+    }
+    const float2 cur = sc;
+    sc = scale(next);
+    fetch_k(next);
+    // ---- running max and sum; a lane's scores: rows g, g + 8, keys 8 t + 2 c, + 1
+    const bool all = all_ok(step);
+    bool good[4] = {true, true, true, true};
+    if (!all) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) good[t] = ok(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1));
+    }
+    const float f = c2 * cur.x;
+    float mx[2] = {st.m[0], st.m[1]};
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[t][e] = good[2 * t + (e & 1)] ? s[t][e] * f : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+    }
+    if (__any_sync(0xffffffffu, mx[0] != st.m[0] || mx[1] != st.m[1])) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float w = mx[r] == -INFINITY ? 1.0f : ex2(st.m[r] - mx[r]);
+        st.m[r] = mx[r];
+        st.l[r] *= w;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) st.o[j][2 * r] *= w, st.o[j][2 * r + 1] *= w;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float base = st.m[e >> 1] == -INFINITY ? 0.0f : st.m[e >> 1];
+        s[t][e] = ex2(s[t][e] - base);
+        st.l[e >> 1] += s[t][e];
+        s[t][e] *= cur.y;
+        if (!all && !good[2 * t + (e & 1)]) s[t][e] = 0.0f;
+      }
+    uint32_t pa[NQ][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t t[NQ];
+      pieces<NQ>(s[k >> 1][2 * (k & 1)], s[k >> 1][2 * (k & 1) + 1], t);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) pa[i][k] = t[i];
+    }
+    if (!all) {  // what is not allowed is no operand: 0 * NaN is NaN
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (!good[t]) {
+#pragma unroll
+          for (int w = 0; w < R::kVW; ++w) vr[t][w] = 0;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      uint32_t b0[NK], b1[NK];
+      R::v_frag(vr, j, b0, b1);
+#pragma unroll
+      for (int i = NQ - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = NK - 1; k >= 0; --k)
+          if (i + k <= kOrder) mma(st.o[j], pa[i], b0[k], b1[k]);
+    }
+    fetch_v(next);
+  }
+}
+
+template <typename T, int D, bool CACHE>
+__global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__ Params p) {
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1;
+  constexpr int ES = CACHE ? 1 : (int)sizeof(T), CV = load_bytes(D / 8 * ES) / ES;
+  extern __shared__ float smem[];  // [16][D + 4] queries, then (merge) [kWarps][16][D]
+  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  pdl_wait();
+  pdl_trigger();
+  const int rt = (int)(blockIdx.x % p.rtiles);
+  const int sp = (int)(blockIdx.x / p.rtiles % p.splits);
+  const int64_t bh = blockIdx.x / p.rtiles / p.splits;
+  const int64_t b = bh / p.x.Hkv;
+  const int hk = (int)(bh % p.x.Hkv);
+  const int G = p.x.H / p.x.Hkv;
+  const int rows = p.x.Lq * G;  // row r: token r / G, head hk * G + r % G
+  const int n = p.x.lens ? min(max(p.x.lens[b], 0), CACHE ? p.T : p.x.Lk) : (CACHE ? p.T : p.x.Lk);
+  float* sq = smem;
+  for (int i = threadIdx.x; i < kRows * D; i += kThreads) {
+    const int r = rt * kRows + i / D, d = i % D;
+    float v = 0.0f;
+    if (r < rows)
+      v = io<T>::ld(static_cast<const T*>(p.x.q.p) + b * p.x.q.sb + (int64_t)(r / G) * p.x.q.st +
+                    (int64_t)(hk * G + r % G) * p.x.q.sh + d);
+    sq[i / D * (D + 4) + d] = v;
+  }
+  __syncthreads();
+  State<D> st;
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st.o[j][e] = 0.0f;
+  st.m[0] = st.m[1] = -INFINITY;
+  st.l[0] = st.l[1] = 0.0f;
+  const float c2 = p.x.scale * kLog2e;
+  // this block's share of the sequence's own steps
+  const int n8 = CACHE ? n / p.block * p.block : n;
+  const int steps = (n8 + 15) / 16, per = (steps + p.splits - 1) / p.splits;
+  const int first = min(steps, sp * per), last = min(steps, first + per);
+  if constexpr (CACHE) {
+    const char* k8 = reinterpret_cast<const char*>(p.k8) + bh * p.T * D;
+    const char* v8 = reinterpret_cast<const char*>(p.v8) + bh * p.T * D;
+    const int64_t s0 = bh * (p.T / p.block);
+    const int spb = p.block / 16;
+    sweep<T, int8_t, D, CV, NQ>(
+        st, sq, first + warp, last, kWarps, n8, c2, [&](int j) { return k8 + (int64_t)j * D; },
+        [&](int j) { return v8 + (int64_t)j * D; }, [](int) { return true; }, [](int) { return true; },
+        [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); });
+  } else {
+    const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.v.p) + b * p.x.v.sb + hk * p.x.v.sh);
+    const int64_t kst = p.x.k.st * (int64_t)sizeof(T), vst = p.x.v.st * (int64_t)sizeof(T);
+    sweep<T, T, D, CV, NQ>(
+        st, sq, first + warp, last, kWarps, n, c2, [&](int j) { return kb + j * kst; },
+        [&](int j) { return vb + j * vst; }, [&](int j) { return xattn::key_ok(p.x, b, n, j); },
+        [&](int step) { return !p.x.mask && step * 16 + 16 <= n; }, [](int) { return make_float2(1.0f, 1.0f); });
+  }
+  if constexpr (CACHE) {
+    if (sp == p.splits - 1 && n > n8) {  // the last, incomplete block, in the inputs' own type
+      const char* kt = reinterpret_cast<const char*>(static_cast<const T*>(p.kt) + bh * p.block * D);
+      const char* vt = reinterpret_cast<const char*>(static_cast<const T*>(p.vt) + bh * p.block * D);
+      const int nt = n - n8;
+      sweep<T, T, D, CV, NQ>(
+          st, sq, warp, (nt + 15) / 16, kWarps, nt, c2, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
+          [&](int j) { return vt + j * (int)(D * sizeof(T)); }, [&](int j) { return j < nt; },
+          [&](int step) { return step * 16 + 16 <= nt; }, [](int) { return make_float2(1.0f, 1.0f); });
+    }
+  }
+  // ---- merge the warps, in order -----------------------------------------------------
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
+    if (c == 0) s_m[warp][g + 8 * r] = st.m[r], s_l[warp][g + 8 * r] = st.l[r];
+  }
+  __syncthreads();  // the queries are done with
+  using R = Rows<T, D, CV>;
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      smem[(warp * kRows + g + 8 * (e >> 1)) * D + R::v_dim(j, 2 * c + (e & 1))] = st.o[j][e];
+  __shared__ float s_w[kWarps][kRows];
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    float m = -INFINITY, l = 0.0f;
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][r]);
+    for (int w = 0; w < kWarps; ++w) {
+      // a part without a maximum holds zeros, or NaN that has to stay
+      const float f = s_m[w][r] == -INFINITY ? 1.0f : ex2(s_m[w][r] - m);
+      s_w[w][r] = f;
+      l += f * s_l[w][r];
+    }
+    const int row = rt * kRows + r;
+    if (p.splits > 1) {
+      p.part_ml[((bh * p.rtiles + rt) * p.splits + sp) * kRows + r] = make_float2(m, l);
+    } else {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      for (int w = 0; w < kWarps; ++w) s_w[w][r] *= inv;
+      if (p.x.lse2 && row < rows)
+        p.x.lse2[(b * p.x.H + hk * G + row % G) * p.x.Lq + row / G] = l == 0.0f ? INFINITY : m + log2f(l);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kRows * D; i += kThreads) {
+    const int r = i / D, d = i % D, row = rt * kRows + r;
+    if (row >= rows) break;
+    float a = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) a += s_w[w][r] * smem[(w * kRows + r) * D + d];
+    if (p.splits > 1)
+      p.part_o[(((bh * p.rtiles + rt) * p.splits + sp) * kRows + r) * D + d] = a;
+    else
+      io<T>::st(static_cast<T*>(p.x.o) + ((b * p.x.Lq + row / G) * p.x.H + hk * G + row % G) * (int64_t)D + d, a);
+  }
+}
+
+// One warp a row: the splits' parts, in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31;
+  const int G = p.x.H / p.x.Hkv, rows = p.x.Lq * G;
+  const int64_t at = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (at >= (int64_t)p.x.B * p.x.Hkv * rows) return;
+  const int64_t bh = at / rows, b = bh / p.x.Hkv;
+  const int row = (int)(at % rows), h = (int)(bh % p.x.Hkv) * G + row % G;
+  const int64_t part = ((bh * p.rtiles + row / kRows) * p.splits) * kRows + row % kRows;
+  float m = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) m = fmaxf(m, p.part_ml[part + (int64_t)s * kRows].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.0f, acc[D / 32] = {};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[part + (int64_t)s * kRows];
+    const float f = ml.x == -INFINITY ? 1.0f : ex2(ml.x - m);
+    l += f * ml.y;
+    const float* o = p.part_o + (part + (int64_t)s * kRows) * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] += f * o[lane + 32 * i];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(p.x.o) + ((b * p.x.Lq + row / G) * p.x.H + h) * (int64_t)D;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) io<T>::st(out + lane + 32 * i, acc[i] * inv);
+  if (p.x.lse2 && lane == 0) p.x.lse2[(b * p.x.H + h) * p.x.Lq + row / G] = l == 0.0f ? INFINITY : m + log2f(l);
+}
+
+// Splits so that about four blocks an SM are in flight, and none shorter than
+// 256 keys (a split writes 16 rows of fp32, as many bytes as 32 to 64 of its keys).
+void plan(Params& p, int keys) {
+  const int64_t rows = (int64_t)p.x.Lq * (p.x.H / p.x.Hkv);
+  p.rtiles = (int)((rows + kRows - 1) / kRows);
+  const int64_t base = (int64_t)p.x.B * p.x.Hkv * p.rtiles, want = (int64_t)num_sms() * 4;
+  int64_t s = base > 0 ? (want + base - 1) / base : 1;
+  const int64_t most = (keys + 255) / 256;
+  if (s > most) s = most;
+  p.splits = s < 1 ? 1 : (int)s;
+}
+
+size_t workspace(const Params& p) {
+  if (p.splits <= 1) return 0;
+  const size_t n = (size_t)p.x.B * p.x.Hkv * p.rtiles * p.splits * kRows;
+  return n * (p.x.D * sizeof(float) + sizeof(float2));
+}
+
+template <typename T, int D, bool CACHE>
+int launch(Params& p, void* ws, cudaStream_t st) {
+  const int64_t grid = (int64_t)p.x.B * p.x.Hkv * p.rtiles * p.splits;
+  const int64_t rows = (int64_t)p.x.B * p.x.H * p.x.Lq;
+  if (grid > 0x7fffffff || rows / kWarps > 0x7ffffff0) return HCLSM_ERR_SHAPE;
+  if (p.splits > 1) {
+    p.part_ml = static_cast<float2*>(ws);
+    p.part_o = reinterpret_cast<float*>(p.part_ml + grid * kRows);
+  }
+  constexpr size_t smem = (size_t)kWarps * kRows * D * sizeof(float) + kRows * 16;
+  auto f = split_kernel<T, D, CACHE>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(f), smem)) return HCLSM_ERR_LAUNCH;
+  if (const int rc = launch_pdl(f, (unsigned)grid, kThreads, smem, st, p)) return rc;
+  if (p.splits <= 1) return HCLSM_OK;
+  return launch_pdl(join_kernel<T, D>, (unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st, p);
+}
+
+template <bool CACHE>
+int run(Params& p, int dtype, void* ws, cudaStream_t st) {
+  const bool f = dtype == HCLSM_F32;
+  switch (p.x.D) {
+    case 32: return f ? launch<float, 32, CACHE>(p, ws, st) : launch<__nv_bfloat16, 32, CACHE>(p, ws, st);
+    case 64: return f ? launch<float, 64, CACHE>(p, ws, st) : launch<__nv_bfloat16, 64, CACHE>(p, ws, st);
+    case 96: return f ? launch<float, 96, CACHE>(p, ws, st) : launch<__nv_bfloat16, 96, CACHE>(p, ws, st);
+    case 128: return f ? launch<float, 128, CACHE>(p, ws, st) : launch<__nv_bfloat16, 128, CACHE>(p, ws, st);
+  }
+  return HCLSM_ERR_UNSUPPORTED;
+}
+
+}  // namespace split
+
+namespace xattn {
+// The cross attention's forward in this form; 16-byte aligned rows of k and v, D 32, 64, 96 or 128.
+size_t split_workspace(const Params& x) {
+  split::Params p = {};
+  p.x = x;
+  split::plan(p, x.Lk);
+  return split::workspace(p);
+}
+int split_fwd(const Params& x, int dtype, void* ws, cudaStream_t st) {
+  split::Params p = {};
+  p.x = x;
+  split::plan(p, x.Lk);
+  return split::run<false>(p, dtype, ws, st);
+}
+}  // namespace xattn
+
+namespace kv8 {
+size_t attn_workspace(const hclsm_kv8_cache* c, int Lq, int H) {
+  split::Params p = {};
+  p.x.B = c->B, p.x.Lq = Lq, p.x.H = H, p.x.Hkv = c->Hkv, p.x.D = c->D;
+  split::plan(p, c->T);
+  return split::workspace(p);
+}
+int attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens, int Lq, int H, float scale,
+         void* ws, cudaStream_t st) {
+  split::Params p = {};
+  p.x.q = xattn::View{q->p, q->sb, q->st, q->sh};
+  p.x.o = o, p.x.lens = lens, p.x.scale = scale;
+  p.x.B = c->B, p.x.Lq = Lq, p.x.H = H, p.x.Hkv = c->Hkv, p.x.D = c->D;
+  p.k8 = c->k, p.v8 = c->v, p.ks = c->k_scale, p.vs = c->v_scale, p.kt = c->k_tail, p.vt = c->v_tail;
+  p.T = c->T, p.block = c->block;
+  split::plan(p, c->T);
+  return split::run<true>(p, c->dtype, ws, st);
+}
+}  // namespace kv8
+}  // namespace hclsm

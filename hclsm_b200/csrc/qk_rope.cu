@@ -1,0 +1,379 @@
+// Per-head norm of queries and keys with the position rotation in the same
+// pass, forward and backward.
+//
+//   xh = x * r,  r = rsqrt(mean(x^2) + eps)   over the D dims of one head
+//   z  = xh * w
+//   y  = R(pos) z: the first `rot` dims as rot/2 pairs (a, b), each turned by
+//        its angle: (a cos - b sin, b cos + a sin); the other dims pass
+// and with u = R(pos)^T dy, g = u * w:
+//   dw = sum over rows of u * xh
+//   dx = r * (g - xh * mean(g * xh))
+//
+// Every element is read once and written once, about 10 (forward) and 25
+// (backward) operations each, so the bound is HBM.  A lane holds 8 dims of a
+// head (16 bytes of bf16, two 16-byte loads of fp32) and D / 8 lanes (rounded
+// up to a power of two) a head, so a head's sums are a butterfly inside the
+// warp and the half layout's partner dims are a shuffle away.  A warp takes
+// the heads of ONE token, 32 / lanes-per-head at a time: the token's cos and
+// sin (64 bytes a lane) are read once and stay in registers for all its heads.
+// Queries and keys go in one launch, the first warps the queries'.
+#include "common.cuh"
+
+namespace hclsm {
+int* device_err_ptr();
+int num_sms();
+
+namespace rope {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+struct Side {
+  const void* x;
+  const void* dy;
+  void* y;  // forward: y, backward: dx
+  const float* w;
+  const int32_t* pos;
+  int64_t sb, st, sh;  // element strides of x (dy and y are dense)
+  int L, H;
+  int chunks;       // a token's heads are split over this many warps
+  int64_t tasks;    // B * L * chunks
+  int blocks;       // thread blocks that work on this side
+  float* partial;   // (blocks, D) column sums of u * xh, or null
+  float* dw;
+};
+
+struct Params {
+  Side s[2];
+  const float* cosv;
+  const float* sinv;
+  int P, rot, D, lph;  // lph: lanes per head
+  float eps;
+  int norm, inter;
+  int* err;
+};
+
+template <typename T> struct Vec8;
+template <> struct Vec8<__nv_bfloat16> {
+  static __device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ void st(__nv_bfloat16* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <> struct Vec8<float> {
+  static __device__ __forceinline__ void ld(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  static __device__ __forceinline__ void st(float* p, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+
+// The rotation of a lane's 8 dims, angle sign `sg` (+1 forward, -1 its
+// transpose).  c, s: the lane's cosines and sines (1 and 0 past the rotated
+// dims).  Half layout: c, s of the 8 dims; the partner dims sit `hop` lanes
+// away, up for the first half and down for the second.  Interleaved: c[0..3],
+// s[0..3] of the 4 pairs.
+__device__ __forceinline__ void rotate(float (&v)[8], const float (&c)[8], const float (&s)[8], float sg, bool inter,
+                                       int partner, bool second) {
+  if (inter) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = v[2 * i], b = v[2 * i + 1], t = sg * s[i];
+      v[2 * i] = a * c[i] - b * t;
+      v[2 * i + 1] = b * c[i] + a * t;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float o = __shfl_sync(0xffffffffu, v[i], partner);
+      const float t = second ? sg * s[i] : -sg * s[i];
+      v[i] = v[i] * c[i] + o * t;
+    }
+  }
+}
+
+__device__ __forceinline__ float head_sum(float v, int lph) {
+  for (int o = lph >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One warp-task: the heads [h0, h1) of token t of batch b.
+template <typename T, bool BWD>
+__device__ __forceinline__ void token(const Params& p, const Side& sd, int64_t task, int lane, const float (&w)[8],
+                                      float (&dw)[8]) {
+  const int chunk = (int)(task % sd.chunks);
+  const int64_t bt = task / sd.chunks;
+  const int64_t b = bt / sd.L;
+  const int t = (int)(bt - b * sd.L);
+  const int lph = p.lph, hpw = 32 / lph;
+  const int hl = lane / lph, d0 = (lane % lph) * 8;
+  const int per = (sd.H + sd.chunks - 1) / sd.chunks;
+  const int h0 = chunk * per, h1 = min(sd.H, h0 + per);
+  const bool dim_ok = d0 < p.D;
+  const bool in_rot = d0 < p.rot;
+  const int half = p.rot >> 1;
+  const bool second = d0 >= half;
+  const int hop = half >> 3;
+  const int partner = !p.inter && in_rot ? (second ? lane - hop : lane + hop) : lane;
+
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
+  if (p.rot > 0) {
+    int pos = sd.pos ? sd.pos[bt] : t;
+    const bool bad = pos < 0 || pos >= p.P;
+    if (bad) {
+      if (lane == 0) record_error(p.err, HCLSM_ERR_SHAPE);
+      pos = 0;
+    }
+    if (in_rot) {
+      const int64_t row = (int64_t)pos * half;
+      if (p.inter) {
+        const float4 a = *reinterpret_cast<const float4*>(p.cosv + row + (d0 >> 1));
+        const float4 e = *reinterpret_cast<const float4*>(p.sinv + row + (d0 >> 1));
+        c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w;
+        s[0] = e.x, s[1] = e.y, s[2] = e.z, s[3] = e.w;
+      } else {
+        Vec8<float>::ld(p.cosv + row + d0 - (second ? half : 0), c);
+        Vec8<float>::ld(p.sinv + row + d0 - (second ? half : 0), s);
+      }
+      if (bad) {  // a position outside the table: NaN, not another position's angle
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+      }
+    }
+  }
+  const T* x = static_cast<const T*>(sd.x) + b * sd.sb + (int64_t)t * sd.st;
+  const int64_t dense = bt * sd.H * p.D;
+  const float inv_d = 1.0f / (float)p.D;
+#pragma unroll 2
+  for (int hb = h0; hb < h1; hb += hpw) {  // warp-uniform trip count
+    const int h = hb + hl;
+    const bool ok = dim_ok && h < h1;
+    float v[8], u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f, u[i] = 0.0f;
+    if (ok) Vec8<T>::ld(x + h * sd.sh + d0, v);
+    if (BWD && ok) Vec8<T>::ld(static_cast<const T*>(sd.dy) + dense + (int64_t)h * p.D + d0, u);
+    float r = 1.0f;
+    if (p.norm) {
+      float q = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q += v[i] * v[i];
+      r = rsqrtf(head_sum(q, lph) * inv_d + p.eps);
+    }
+    if constexpr (!BWD) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
+      rotate(v, c, s, 1.0f, p.inter, partner, second);
+      if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, v);
+    } else {
+      rotate(u, c, s, -1.0f, p.inter, partner, second);
+      if (p.norm) {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[i] *= r;  // xh
+          dw[i] += u[i] * v[i];
+          u[i] *= w[i];
+          m += u[i] * v[i];
+        }
+        m = head_sum(m, lph) * inv_d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = r * (u[i] - v[i] * m);
+      }
+      if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, u);
+    }
+  }
+}
+
+template <typename T, bool BWD>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ Params p) {
+  __shared__ float red[BWD ? kWarps * 256 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool isk = blockIdx.x >= (unsigned)p.s[0].blocks;
+  const Side& sd = p.s[isk ? 1 : 0];
+  const int blk = (int)blockIdx.x - (isk ? p.s[0].blocks : 0);
+  pdl_wait();
+  pdl_trigger();
+  const int d0 = (lane % p.lph) * 8;
+  float w[8], dw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.0f, dw[i] = 0.0f;
+  if (sd.w && d0 < p.D) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = sd.w[d0 + i];
+  }
+  for (int64_t task = (int64_t)blk * kWarps + warp; task < sd.tasks; task += (int64_t)sd.blocks * kWarps)
+    token<T, BWD>(p, sd, task, lane, w, dw);
+  if constexpr (BWD) {
+    if (sd.partial) {
+      // the warp's heads, then the block's warps, both in a fixed order
+      for (int o = p.lph; o < 32; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+      }
+      if (lane < p.lph && d0 < p.D) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) red[warp * 256 + d0 + i] = dw[i];
+      }
+      __syncthreads();
+      for (int d = threadIdx.x; d < p.D; d += kThreads) {
+        float a = 0.0f;
+        for (int k = 0; k < kWarps; ++k) a += red[k * 256 + d];
+        sd.partial[(int64_t)blk * p.D + d] = a;
+      }
+    }
+  }
+}
+
+// The blocks' column sums, block blockIdx.x one side's; thread groups take every
+// G-th row and are added in order.
+__global__ void __launch_bounds__(1024) dw_kernel(const __grid_constant__ Params p) {
+  __shared__ float red[1024];
+  pdl_wait();
+  const Side& sd = p.s[blockIdx.x];
+  if (!sd.partial) return;
+  const int D = p.D, G = 1024 / D;
+  const int d = threadIdx.x % D, g = threadIdx.x / D;
+  float a = 0.0f;
+  if (g < G)
+    for (int r = g; r < sd.blocks; r += G) a += sd.partial[(int64_t)r * D + d];
+  red[threadIdx.x] = a;
+  __syncthreads();
+  if (g == 0) {
+    for (int k = 1; k < G; ++k) a += red[k * D + d];
+    sd.dw[d] = a;
+  }
+}
+
+int lanes_per_head(int D) {
+  int l = 1;
+  while (l * 8 < D) l <<= 1;
+  return l;
+}
+
+// Backward blocks of one side: bounded so that the column sums' second stage
+// stays short (4 blocks of 8 warps an SM hide the loads' latency).
+int bwd_blocks(int64_t tasks) {
+  const int64_t want = (tasks + kWarps - 1) / kWarps, most = (int64_t)num_sms() * 4;
+  return (int)(want < most ? want : most);
+}
+
+bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// A token's heads go to one warp unless there are too few tokens to fill the
+// GPU; then each warp takes as few as one pass over the lanes.
+void plan(Side& s, int64_t B, int lph) {
+  const int hpw = 32 / lph;
+  int passes = (s.H + hpw - 1) / hpw;
+  const int64_t tokens = B * s.L;
+  int chunks = 1;
+  while (chunks < passes && tokens * chunks < (int64_t)num_sms() * 64) chunks <<= 1;
+  if (chunks > passes) chunks = passes;
+  // whole passes to every chunk
+  const int per = (passes + chunks - 1) / chunks * hpw;
+  s.chunks = (s.H + per - 1) / per;
+  s.tasks = tokens * s.chunks;
+}
+
+int check(const hclsm_rope_side* s, int64_t B, int P, int rot, bool bwd) {
+  if (s->L < 0 || s->H < 1) return HCLSM_ERR_SHAPE;
+  if (B * s->L == 0) return HCLSM_OK;
+  if (!s->x || !s->y || (bwd && !s->dy)) return HCLSM_ERR_NULL;
+  if (rot > 0 && !s->pos && s->L > P) return HCLSM_ERR_SHAPE;
+  if (!aligned(s->x) || !aligned(s->y) || (bwd && !aligned(s->dy))) return HCLSM_ERR_ALIGN;
+  return HCLSM_OK;
+}
+
+int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, const float* sinv, int P, int rot,
+        int64_t B, int D, float eps, int dtype, int flags, bool bwd, void* ws, size_t ws_bytes, void* stream) {
+  if (dtype != HCLSM_F32 && dtype != HCLSM_BF16) return HCLSM_ERR_DTYPE;
+  if (!q) return HCLSM_ERR_NULL;
+  const bool inter = flags & HCLSM_ROPE_INTERLEAVED, norm = !(flags & HCLSM_ROPE_NO_NORM);
+  if (B < 0 || D < 8 || D > 256 || D % 8 || rot < 0 || rot > D || rot % (inter ? 8 : 16) || P < 0)
+    return HCLSM_ERR_SHAPE;
+  if (rot > 0 && (!cosv || !sinv)) return HCLSM_ERR_NULL;
+  if (rot > 0 && (!aligned(cosv) || !aligned(sinv))) return HCLSM_ERR_ALIGN;
+  Params p = {};
+  const hclsm_rope_side* in[2] = {q, k};
+  const int e = dtype == HCLSM_F32 ? 4 : 2;
+  p.lph = lanes_per_head(D);
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.s[i];
+    s.chunks = 1;
+    if (!in[i]) continue;
+    if (const int rc = check(in[i], B, P, rot, bwd)) return rc;
+    if (!norm && in[i]->w) return HCLSM_ERR_UNSUPPORTED;
+    if ((in[i]->sb * e) % 16 || (in[i]->st * e) % 16 || (in[i]->sh * e) % 16) return HCLSM_ERR_ALIGN;
+    s.x = in[i]->x, s.dy = in[i]->dy, s.y = in[i]->y, s.w = in[i]->w, s.pos = in[i]->pos;
+    s.sb = in[i]->sb, s.st = in[i]->st, s.sh = in[i]->sh;
+    s.L = in[i]->L, s.H = in[i]->H;
+    if (B * s.L > 0) plan(s, B, p.lph);
+    if (!bwd && (s.tasks + kWarps - 1) / kWarps > 0x3fffffff) return HCLSM_ERR_SHAPE;
+    s.blocks = bwd ? bwd_blocks(s.tasks) : (int)((s.tasks + kWarps - 1) / kWarps);
+    if (bwd && in[i]->dw) {
+      const size_t need = (size_t)s.blocks * D * sizeof(float);
+      const size_t used = i ? (p.s[0].partial ? (size_t)p.s[0].blocks * D * sizeof(float) : 0) : 0;
+      s.dw = in[i]->dw;
+      if (need) {
+        if (!ws || used + need > ws_bytes) return HCLSM_ERR_WORKSPACE;
+        s.partial = reinterpret_cast<float*>(static_cast<char*>(ws) + used);
+      }
+    }
+  }
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int i = 0; i < 2; ++i)  // no rows: the weight's gradient is zero
+    if (p.s[i].dw && p.s[i].blocks == 0 && cudaMemsetAsync(p.s[i].dw, 0, D * sizeof(float), st) != cudaSuccess)
+      return HCLSM_ERR_LAUNCH;
+  const int grid = p.s[0].blocks + p.s[1].blocks;
+  if (grid == 0) return HCLSM_OK;
+  p.cosv = cosv, p.sinv = sinv, p.P = P, p.rot = rot, p.D = D, p.eps = eps, p.norm = norm, p.inter = inter;
+  p.err = device_err_ptr();
+  int rc;
+  if (dtype == HCLSM_F32)
+    rc = bwd ? launch_pdl(rope_kernel<float, true>, grid, kThreads, 0, st, p)
+             : launch_pdl(rope_kernel<float, false>, grid, kThreads, 0, st, p);
+  else
+    rc = bwd ? launch_pdl(rope_kernel<__nv_bfloat16, true>, grid, kThreads, 0, st, p)
+             : launch_pdl(rope_kernel<__nv_bfloat16, false>, grid, kThreads, 0, st, p);
+  if (rc != HCLSM_OK || (!p.s[0].partial && !p.s[1].partial)) return rc;
+  return launch_pdl(dw_kernel, 2, 1024, 0, st, p);
+}
+
+}  // namespace rope
+}  // namespace hclsm
+
+extern "C" int hclsm_qk_norm_rope(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv,
+                                  const float* sinv, int32_t P, int32_t rot, int64_t B, int32_t D, float eps,
+                                  int32_t dtype, int32_t flags, void* stream) {
+  return hclsm::rope::run(q, k, cosv, sinv, P, rot, B, D, eps, dtype, flags, false, nullptr, 0, stream);
+}
+
+extern "C" size_t hclsm_qk_norm_rope_bwd_workspace_size(int32_t D) {
+  if (D < 8 || D > 256) return 0;
+  return (size_t)2 * 4 * hclsm::num_sms() * D * sizeof(float);
+}
+
+extern "C" int hclsm_qk_norm_rope_bwd(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv,
+                                      const float* sinv, int32_t P, int32_t rot, int64_t B, int32_t D, float eps,
+                                      int32_t dtype, int32_t flags, void* ws, size_t ws_bytes, void* stream) {
+  return hclsm::rope::run(q, k, cosv, sinv, P, rot, B, D, eps, dtype, flags, true, ws, ws_bytes, stream);
+}

@@ -1,0 +1,390 @@
+// Cross attention: the kernels that serve every type, head size, stride and
+// alignment (fp32 arithmetic throughout), and the C entry points.
+//
+// 64 x 64 score tiles, 256 threads, 4 x 4 scores a thread; operands are staged
+// in shared memory as fp32 rows of DP + 4 floats (the pad keeps the 16 lanes
+// that read different rows on different banks).  One pass over the keys with
+// the running maximum and sum of the softmax.  Bound: the FP32 pipes.
+#include "xattn.cuh"
+
+namespace hclsm {
+namespace xattn {
+
+constexpr int kT = 64;  // rows and keys of a tile
+constexpr int kThreads = 256;
+
+// Rows [r0, r0 + 64) of one head as fp32 rows of DP + 4; rows past n (and, with
+// KEYS, keys that are not allowed) and dims past D are zeros.
+template <typename T, int DP, bool KEYS>
+__device__ __forceinline__ void stage(float* dst, const View& x, const Params& p, int64_t b, int h, int r0, int n) {
+  const T* base = static_cast<const T*>(x.p) + b * x.sb + (int64_t)h * x.sh;
+  for (int i = threadIdx.x; i < kT * DP; i += kThreads) {
+    const int r = i / DP, d = i % DP, row = r0 + r;
+    bool ok = d < p.D && row < n;
+    if (KEYS) ok = ok && key_ok(p, b, n, row);
+    dst[r * (DP + 4) + d] = ok ? io<T>::ld(base + (int64_t)row * x.st + d) : 0.0f;
+  }
+}
+
+// acc[i][j] += sum_d a[4 ty + i][d] * b[tx + 16 j][d]
+template <int DP>
+__device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * (DP + 4) + d);
+      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * (DP + 4) + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
+  }
+}
+
+// out[i][n] += sum_c w(4 ty + i, c) * x[c][2 tx + 32 (n / 2) + n % 2]; w is [row][col] or, TRANS, [col][row].
+template <int DP, bool TRANS>
+__device__ __forceinline__ void gather_tile(float (&out)[4][DP / 16], const float* w, const float* x, int ty, int tx) {
+#pragma unroll 2
+  for (int c = 0; c < kT; ++c) {
+    float a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = TRANS ? w[c * (kT + 4) + 4 * ty + i] : w[(4 * ty + i) * (kT + 4) + c];
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n) {
+      const float2 y = *reinterpret_cast<const float2*>(x + c * (DP + 4) + 2 * tx + 32 * n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i][2 * n] += a[i] * y.x, out[i][2 * n + 1] += a[i] * y.y;
+    }
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[4][DP / 16], const float (&f)[4],
+                                           const Params& p, int64_t b, int L, int H, int h, int r0, int ty, int tx) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 4 * ty + i;
+    if (row >= L) continue;
+    T* out = static_cast<T*>(dst) + ((b * L + row) * H + h) * (int64_t)p.D;
+#pragma unroll
+    for (int n = 0; n < DP / 32; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = 2 * tx + 32 * n + e;
+        if (d < p.D) io<T>::st(out + d, acc[i][2 * n + e] * f[i]);
+      }
+  }
+}
+
+template <int DP> constexpr size_t op_floats() { return (size_t)kT * (DP + 4); }
+constexpr size_t kScoreFloats = (size_t)kT * (kT + 4);
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 smem4[];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sk = sq + op_floats<DP>();
+  float* sv = sk + op_floats<DP>();
+  float* sp = sv + op_floats<DP>();
+  __shared__ uint8_t okc[kT];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  pdl_wait();
+  pdl_trigger();
+  const int tiles = (p.Lq + kT - 1) / kT;
+  const int r0 = (int)(blockIdx.x % tiles) * kT;
+  const int h = (int)(blockIdx.x / tiles % p.H);
+  const int64_t b = blockIdx.x / tiles / p.H;
+  const int hk = h / (p.H / p.Hkv);
+  const int nk = key_count(p, b);
+  const float c2 = p.scale * kLog2e;
+  stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
+  float acc[4][DP / 16] = {}, m[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.0f;
+  for (int k0 = 0; k0 < nk; k0 += kT) {
+    __syncthreads();
+    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
+    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
+    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    __syncthreads();
+    float s[4][4] = {};
+    dot_tile<DP>(s, sq, sk, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = okc[tx + 16 * j] ? s[i][j] * c2 : -INFINITY;
+        mx = fmaxf(mx, s[i][j]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float base = mx == -INFINITY ? 0.0f : mx;  // no allowed key yet: every weight 0
+      const float f = exp2f(m[i] - base);
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = exp2f(s[i][j] - base);
+        sp[(4 * ty + i) * (kT + 4) + tx + 16 * j] = e;
+        sum += e;
+      }
+      m[i] = mx;
+      l[i] = l[i] * f + sum;
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) acc[i][n] *= f;
+    }
+    __syncthreads();
+    gather_tile<DP, false>(acc, sp, sv, ty, tx);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+    const bool empty = l[i] == 0.0f;  // a row with a key sums to at least 1
+    inv[i] = empty ? 0.0f : 1.0f / l[i];
+    const int row = r0 + 4 * ty + i;
+    if (p.lse2 && tx == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : m[i] + log2f(l[i]);
+  }
+  store_rows<T, DP>(p.o, acc, inv, p, b, p.Lq, p.H, h, r0, ty, tx);
+}
+
+// p and ds of one tile, left in sp and sds (row = query, column = key).
+template <int DP>
+__device__ __forceinline__ void grad_tile(float* sp, float* sds, const float* sq, const float* sk, const float* sdo,
+                                          const float* sv, const uint8_t* okc, const float (&lse)[4],
+                                          const float (&delta)[4], float c2, int ty, int tx) {
+  float s[4][4] = {}, dp[4][4] = {};
+  dot_tile<DP>(s, sq, sk, ty, tx);
+  dot_tile<DP>(dp, sdo, sv, ty, tx);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w = okc[tx + 16 * j] ? exp2f(s[i][j] * c2 - lse[i]) : 0.0f;
+      const int at = (4 * ty + i) * (kT + 4) + tx + 16 * j;
+      if (sp) sp[at] = w;
+      sds[at] = w * (dp[i][j] - delta[i]);
+    }
+}
+
+// lse2 and delta of the thread's 4 rows; rows past Lq weigh nothing.
+__device__ __forceinline__ void row_stats(float (&lse)[4], float (&delta)[4], const Params& p, int64_t b, int h, int r0,
+                                          int ty) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = r0 + 4 * ty + i;
+    const int64_t at = (b * p.H + h) * p.Lq + row;
+    lse[i] = row < p.Lq ? p.lse2[at] : INFINITY;
+    delta[i] = row < p.Lq ? p.delta[at] : 0.0f;
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 smem4[];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sdo = sq + op_floats<DP>();
+  float* sk = sdo + op_floats<DP>();
+  float* sv = sk + op_floats<DP>();
+  float* sds = sv + op_floats<DP>();
+  __shared__ uint8_t okc[kT];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  pdl_wait();
+  pdl_trigger();
+  const int tiles = (p.Lq + kT - 1) / kT;
+  const int r0 = (int)(blockIdx.x % tiles) * kT;
+  const int h = (int)(blockIdx.x / tiles % p.H);
+  const int64_t b = blockIdx.x / tiles / p.H;
+  const int hk = h / (p.H / p.Hkv);
+  const int nk = key_count(p, b);
+  stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
+  stage<T, DP, false>(sdo, p.dout, p, b, h, r0, p.Lq);
+  float acc[4][DP / 16] = {}, lse[4], delta[4];
+  row_stats(lse, delta, p, b, h, r0, ty);
+  for (int k0 = 0; k0 < nk; k0 += kT) {
+    __syncthreads();
+    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
+    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
+    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    __syncthreads();
+    grad_tile<DP>(nullptr, sds, sq, sk, sdo, sv, okc, lse, delta, p.scale * kLog2e, ty, tx);
+    __syncthreads();
+    gather_tile<DP, false>(acc, sds, sk, ty, tx);
+  }
+  const float f[4] = {p.scale, p.scale, p.scale, p.scale};
+  store_rows<T, DP>(p.dq, acc, f, p, b, p.Lq, p.H, h, r0, ty, tx);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads) dkv_kernel(const __grid_constant__ Params p) {
+  extern __shared__ float4 smem4[];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sdo = sq + op_floats<DP>();
+  float* sk = sdo + op_floats<DP>();
+  float* sv = sk + op_floats<DP>();
+  float* sp = sv + op_floats<DP>();
+  float* sds = sp + kScoreFloats;
+  __shared__ uint8_t okc[kT];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  pdl_wait();
+  pdl_trigger();
+  const int tiles = (p.Lk + kT - 1) / kT;
+  const int k0 = (int)(blockIdx.x % tiles) * kT;
+  const int hk = (int)(blockIdx.x / tiles % p.Hkv);
+  const int64_t b = blockIdx.x / tiles / p.Hkv;
+  const int G = p.H / p.Hkv;
+  const int nk = key_count(p, b);
+  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
+  if (k0 < nk) {
+    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
+    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
+    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    // the query heads that share this key head, one after another: a fixed order
+    for (int g = 0; g < G; ++g)
+      for (int r0 = 0; r0 < p.Lq; r0 += kT) {
+        const int h = hk * G + g;
+        __syncthreads();
+        stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
+        stage<T, DP, false>(sdo, p.dout, p, b, h, r0, p.Lq);
+        float lse[4], delta[4];
+        row_stats(lse, delta, p, b, h, r0, ty);
+        __syncthreads();
+        grad_tile<DP>(sp, sds, sq, sk, sdo, sv, okc, lse, delta, p.scale * kLog2e, ty, tx);
+        __syncthreads();
+        gather_tile<DP, true>(dv, sp, sdo, ty, tx);
+        gather_tile<DP, true>(dk, sds, sq, ty, tx);
+      }
+  }
+  const float one[4] = {1.0f, 1.0f, 1.0f, 1.0f}, f[4] = {p.scale, p.scale, p.scale, p.scale};
+  store_rows<T, DP>(p.dk, dk, f, p, b, p.Lk, p.Hkv, hk, k0, ty, tx);
+  store_rows<T, DP>(p.dv, dv, one, p, b, p.Lk, p.Hkv, hk, k0, ty, tx);
+}
+
+// delta_i = do_i . o_i, one warp a row.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__ Params p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= (int64_t)p.B * p.Lq * p.H) return;
+  const int h = (int)(row % p.H);
+  const int64_t bt = row / p.H, b = bt / p.Lq, t = bt % p.Lq;
+  const T* o = static_cast<const T*>(p.o) + row * p.D;
+  const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.sb + t * p.dout.st + h * p.dout.sh;
+  float a = 0.0f;
+  for (int d = lane; d < p.D; d += 32) a += io<T>::ld(o + d) * io<T>::ld(g + d);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) a += __shfl_xor_sync(0xffffffffu, a, s);
+  if (lane == 0) p.delta[(b * p.H + h) * p.Lq + t] = a;
+}
+
+template <typename T, int DP>
+int run(const Params& p, bool bwd, cudaStream_t st) {
+  const int64_t qt = (int64_t)((p.Lq + kT - 1) / kT) * p.H * p.B, kt = (int64_t)((p.Lk + kT - 1) / kT) * p.Hkv * p.B;
+  if (qt > 0x7fffffff || kt > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  const size_t s3 = (3 * op_floats<DP>() + kScoreFloats) * 4, s4 = (4 * op_floats<DP>() + kScoreFloats) * 4,
+               s5 = s4 + kScoreFloats * 4;
+  if (!bwd) {
+    auto f = fwd_kernel<T, DP>;
+    if (!set_smem_limit(reinterpret_cast<const void*>(f), s3)) return HCLSM_ERR_LAUNCH;
+    return launch_pdl(f, (unsigned)qt, kThreads, s3, st, p);
+  }
+  auto fq = dq_kernel<T, DP>;
+  auto fk = dkv_kernel<T, DP>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(fq), s4) || !set_smem_limit(reinterpret_cast<const void*>(fk), s5))
+    return HCLSM_ERR_LAUNCH;
+  if (qt > 0)
+    if (const int rc = launch_pdl(fq, (unsigned)qt, kThreads, s4, st, p)) return rc;
+  return kt > 0 ? launch_pdl(fk, (unsigned)kt, kThreads, s5, st, p) : HCLSM_OK;
+}
+
+template <typename T>
+int dispatch(const Params& p, bool bwd, cudaStream_t st) {
+  if (bwd && (int64_t)p.B * p.Lq > 0) {
+    const int64_t rows = (int64_t)p.B * p.Lq * p.H, grid = (rows + 7) / 8;
+    if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+    if (const int rc = launch_pdl(delta_kernel<T>, (unsigned)grid, kThreads, 0, st, p)) return rc;
+  }
+  if (p.D <= 32) return run<T, 32>(p, bwd, st);
+  if (p.D <= 64) return run<T, 64>(p, bwd, st);
+  return run<T, 128>(p, bwd, st);
+}
+
+int check(const hclsm_xattn_args* a) {
+  if (!a) return HCLSM_ERR_NULL;
+  if (a->dtype != HCLSM_F32 && a->dtype != HCLSM_BF16) return HCLSM_ERR_DTYPE;
+  if (a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv || a->D < 1 || a->D > 128 ||
+      !(a->scale > 0.0f) || a->scale > 3.0e38f)
+    return HCLSM_ERR_SHAPE;
+  return HCLSM_OK;
+}
+
+Params params(const hclsm_xattn_args* a) {
+  Params p = {};
+  auto view = [](const hclsm_view& v) { return View{v.p, v.sb, v.st, v.sh}; };
+  p.q = view(a->q), p.k = view(a->k), p.v = view(a->v), p.dout = view(a->dout);
+  p.o = a->o, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
+  p.lse2 = a->lse2;
+  p.lens = a->lens, p.mask = a->mask, p.mask_sb = a->mask_sb;
+  p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.Hkv = a->Hkv, p.D = a->D;
+  p.scale = a->scale;
+  p.err = device_err_ptr();
+  return p;
+}
+
+}  // namespace xattn
+}  // namespace hclsm
+
+using namespace hclsm;
+
+// Few enough rows a key head that the 16-row products of the split form carry
+// no padding to speak of, and operands it can read 16 bytes at a time.
+static bool use_split(const xattn::Params& p, int dtype) {
+  const int e = dtype == HCLSM_F32 ? 4 : 2;
+  auto ok = [&](const xattn::View& v) {
+    return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.sb * e % 16 == 0 && v.st * e % 16 == 0 && v.sh * e % 16 == 0;
+  };
+  return p.Lk > 0 && (int64_t)p.Lq * (p.H / p.Hkv) <= 16 && p.D % 32 == 0 && ok(p.k) && ok(p.v);
+}
+
+extern "C" size_t hclsm_xattn_fwd_workspace_size(const hclsm_xattn_args* a) {
+  if (xattn::check(a)) return 0;
+  const xattn::Params p = xattn::params(a);
+  return use_split(p, a->dtype) ? xattn::split_workspace(p) : 0;
+}
+
+extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = xattn::check(a)) return rc;
+  if ((int64_t)a->B * a->Lq == 0) return HCLSM_OK;
+  if (!a->q.p || !a->o || (a->Lk > 0 && (!a->k.p || !a->v.p))) return HCLSM_ERR_NULL;
+  const xattn::Params p = xattn::params(a);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (use_split(p, a->dtype)) {
+    const size_t need = xattn::split_workspace(p);
+    if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+    return xattn::split_fwd(p, a->dtype, ws, st);
+  }
+  return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
+}
+
+extern "C" size_t hclsm_xattn_bwd_workspace_size(const hclsm_xattn_args* a) {
+  if (xattn::check(a)) return 0;
+  return (size_t)a->B * a->H * a->Lq * sizeof(float);
+}
+
+extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
+  if (const int rc = xattn::check(a)) return rc;
+  if (a->B == 0) return HCLSM_OK;
+  if (a->Lq > 0 && (!a->q.p || !a->o || !a->dout.p || !a->dq || !a->lse2)) return HCLSM_ERR_NULL;
+  if (a->Lk > 0 && (!a->k.p || !a->v.p || !a->dk || !a->dv)) return HCLSM_ERR_NULL;
+  if (ws_bytes < hclsm_xattn_bwd_workspace_size(a) || (a->Lq > 0 && !ws)) return HCLSM_ERR_WORKSPACE;
+  xattn::Params p = xattn::params(a);
+  p.delta = static_cast<float*>(ws);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, true, st) : xattn::dispatch<__nv_bfloat16>(p, true, st);
+}

@@ -1,0 +1,141 @@
+"""A cache of keys and values in 8 bits, and the attention that reads it.
+
+Complete blocks of ``block`` tokens a head are int8 with one fp32 scale
+(max|x| / 127); the last, incomplete block of each sequence stays in the inputs'
+dtype, so every value is rounded to 8 bits once, when its block fills.  The
+caller owns the positions: ``start`` (tokens already there) and ``lens`` (tokens
+to attend to) are arguments, so a step captures into a CUDA graph and can be
+replayed with other positions.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass, field
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+
+__all__ = ["Kv8Cache", "kv8_write", "kv8_read", "kv8_attention"]
+
+
+@dataclass
+class Kv8Cache:
+    """The cache's tensors, all contiguous: k, v (B, Hkv, T, D) int8, k_scale,
+    v_scale (B, Hkv, T / block) fp32, k_tail, v_tail (B, Hkv, block, D) in the
+    inputs' dtype.  D is 32, 64, 96 or 128; block 16, 32, 64 or 128."""
+
+    k: Tensor
+    v: Tensor
+    k_scale: Tensor
+    v_scale: Tensor
+    k_tail: Tensor
+    v_tail: Tensor
+    _c: _lib.Kv8 = field(init=False, repr=False, compare=False, default=None)
+
+    def __post_init__(self):
+        _lib.require_cuda(self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
+        if self.k.dim() != 4 or self.k_tail.dim() != 4:
+            raise ValueError("k must be (B, Hkv, T, D), k_tail (B, Hkv, block, D)")
+        B, Hkv, T, D = self.k.shape
+        block, dtype = self.k_tail.shape[2], self.k_tail.dtype
+        if block not in (16, 32, 64, 128) or T % block:
+            raise ValueError(f"block must be 16, 32, 64 or 128 and divide the capacity {T}, got {block}")
+        if D not in (32, 64, 96, 128):
+            raise ValueError(f"head_dim must be 32, 64, 96 or 128, got {D}")
+        for name, t, shape, dt in (("k", self.k, (B, Hkv, T, D), torch.int8), ("v", self.v, (B, Hkv, T, D), torch.int8),
+                                   ("k_scale", self.k_scale, (B, Hkv, T // block), torch.float32),
+                                   ("v_scale", self.v_scale, (B, Hkv, T // block), torch.float32),
+                                   ("k_tail", self.k_tail, (B, Hkv, block, D), dtype),
+                                   ("v_tail", self.v_tail, (B, Hkv, block, D), dtype)):
+            if t.shape != shape or t.dtype != dt or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {shape} {dt}, got {tuple(t.shape)} {t.dtype}")
+        self._c = _lib.Kv8(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                           self.k_tail.data_ptr(), self.v_tail.data_ptr(), B, Hkv, T, D, block,
+                           _lib.dtype_code(dtype))
+
+    @classmethod
+    def empty(cls, batch: int, capacity: int, kv_heads: int, head_dim: int, *, block: int = 32, dtype=torch.bfloat16,
+              device="cuda") -> "Kv8Cache":
+        """A cache with room for ``capacity`` tokens (rounded up to whole blocks) a sequence."""
+        T = (capacity + block - 1) // block * block
+
+        def zeros(*shape, dt):
+            return torch.zeros(shape, dtype=dt, device=device)
+
+        return cls(*(zeros(batch, kv_heads, T, head_dim, dt=torch.int8) for _ in range(2)),
+                   *(zeros(batch, kv_heads, T // block, dt=torch.float32) for _ in range(2)),
+                   *(zeros(batch, kv_heads, block, head_dim, dt=dtype) for _ in range(2)))
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.k_tail.dtype
+
+    @property
+    def block(self) -> int:
+        return self.k_tail.shape[2]
+
+
+def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tensor | None = None) -> None:
+    """Append k, v (B, n, Hkv, D), in place: token i of entry b becomes token
+    ``start[b] + i`` of the cache, for the first ``count[b]`` tokens (default n).
+    ``start[b]`` is the number of tokens already there.  A request that does not
+    fit the capacity writes nothing and sets the device error word."""
+    dev = _lib.require_cuda(cache.k, k, v, start, count)
+    B, Hkv, _, D = cache.k.shape
+    if k.dim() != 4 or v.shape != k.shape or k.shape[0] != B or k.shape[2:] != (Hkv, D):
+        raise ValueError(f"k and v must be ({B}, tokens, {Hkv}, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.dtype != cache.dtype or v.dtype != cache.dtype:
+        raise TypeError(f"k and v must have the cache's dtype {cache.dtype}, got {k.dtype} and {v.dtype}")
+    start = _lib.index32(start, (B,), "start", dev)
+    if start is None:
+        raise ValueError("start is required")
+    count = _lib.index32(count, (B,), "count", dev)
+    k, v = _lib.rows16(k), _lib.rows16(v)
+    kv, vv = _lib.view(k), _lib.view(v)
+    _lib.check(_lib.load().hclsm_kv8_write(ctypes.addressof(cache._c), ctypes.addressof(kv), ctypes.addressof(vv),
+                                           k.shape[1], start.data_ptr(), _lib.ptr(count), _lib.stream_ptr(dev)),
+               "hclsm_kv8_write")
+
+
+def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
+    """(k, v), each (B, T, Hkv, D) in the cache's dtype: the first ``lens[b]``
+    tokens (default all) as the values they stand for, zeros after them."""
+    dev = _lib.require_cuda(cache.k, lens)
+    B, Hkv, T, D = cache.k.shape
+    lens = _lib.index32(lens, (B,), "lens", dev)
+    k, v = (torch.empty(B, T, Hkv, D, dtype=cache.dtype, device=dev) for _ in range(2))
+    _lib.check(_lib.load().hclsm_kv8_read(ctypes.addressof(cache._c), k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
+                                          _lib.stream_ptr(dev)), "hclsm_kv8_read")
+    return k, v
+
+
+def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, scale: float | None = None) -> Tensor:
+    """softmax(scale q k^T) v of q (B, Lq, H, D), in the cache's dtype, over the
+    first ``lens[b]`` tokens of the cache (default all; clamped to [0, T]); H is a
+    multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
+    dev = _lib.require_cuda(q, cache.k, lens)
+    B, Hkv, T, D = cache.k.shape
+    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
+        raise ValueError(f"q must be ({B}, tokens, heads, {D}), got {tuple(q.shape)}")
+    Lq, H = q.shape[1], q.shape[2]
+    if H < 1 or H % Hkv:
+        raise ValueError(f"query heads ({H}) must be a multiple of key heads ({Hkv})")
+    if q.dtype != cache.dtype:
+        raise TypeError(f"q must have the cache's dtype {cache.dtype}, got {q.dtype}")
+    if torch.is_grad_enabled() and q.requires_grad:
+        raise NotImplementedError("kv8_attention has no gradients: call it under torch.no_grad()")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    lens = _lib.index32(lens, (B,), "lens", dev)
+    q = _lib.dense_last(q)
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lib, c, qv = _lib.load(), ctypes.addressof(cache._c), _lib.view(q)
+    n = lib.hclsm_kv8_attn_workspace_size(c, Lq, H)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _lib.check(lib.hclsm_kv8_attn(c, ctypes.addressof(qv), o.data_ptr(), _lib.ptr(lens), Lq, H, scale, _lib.ptr(ws), n,
+                                  _lib.stream_ptr(dev)), "hclsm_kv8_attn")
+    return o

@@ -1,0 +1,165 @@
+"""Per-head norm of queries and keys and their position rotation, one launch.
+
+``qk_norm_rope(q, k, q_weight, k_weight, cos, sin)`` normalises every head of
+q (B, Lq, H, D) and k (B, Lk, Hkv, D) by its root mean square, multiplies by the
+weight and turns the first ``2 * cos.shape[1]`` dims by the angles of the token's
+position; forward and backward are one pass over the data each (plus a short
+reduction for the weights' gradients).  All arithmetic is fp32; outputs and
+gradients have their inputs' dtypes (float32 or bfloat16; weights fp32).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _lib
+
+__all__ = ["qk_norm_rope", "rope_tables"]
+
+_INTERLEAVED, _NO_NORM = 1, 2
+
+
+def rope_tables(positions: int, dim: int, base: float = 10000.0, *, scale: float = 1.0, device="cuda"):
+    """(cos, sin), each (positions, dim / 2) fp32: position p turns pair i by
+    ``p / scale * base ** (-2 i / dim)``; ``scale`` > 1 stretches the angles of
+    short training contexts over longer ones."""
+    if dim < 2 or dim % 2 or positions < 0 or not scale > 0 or not base > 0:
+        raise ValueError(f"rope_tables: positions {positions}, dim {dim}, base {base}, scale {scale}")
+    freq = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    ang = torch.arange(positions, dtype=torch.float64)[:, None] / float(scale) * freq
+    return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+def _check(q, k, q_weight, k_weight, cos, sin, eps):
+    dev = _lib.require_cuda(q, k, q_weight, k_weight, cos, sin)
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError("q and k must be (batch, tokens, heads, head_dim)")
+    B, D = q.shape[0], q.shape[3]
+    if k is not None and (k.shape[0] != B or k.shape[3] != D):
+        raise ValueError(f"k must share q's batch and head_dim {(B, D)}, got {tuple(k.shape)}")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"q and k must share one dtype, got {q.dtype} and {k.dtype}")
+    if k is None and k_weight is not None:
+        raise ValueError("k_weight without k")
+    _lib.dtype_code(q.dtype)
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"head_dim must be a multiple of 8 up to 256, got {D}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            continue
+        if eps is None:
+            raise ValueError(f"{name} without the norm (eps=None)")
+        if w.shape != (D,) or w.dtype != torch.float32:
+            raise ValueError(f"{name} must be ({D},) float32")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            raise ValueError("cos and sin must be (positions, rotary_dim / 2) float32")
+    return dev
+
+
+def _side(x, y, w, pos, dy=None, dw=None):
+    s = x.stride()
+    return _lib.RopeSide(x.data_ptr(), _lib.ptr(dy), y.data_ptr(), _lib.ptr(w), _lib.ptr(pos), _lib.ptr(dw),
+                         s[0], s[1], s[2], x.shape[1], x.shape[2])
+
+
+def _call(bwd, qs, ks, cos, sin, B, D, eps, dtype, interleaved, device):
+    lib = _lib.load()
+    flags = (_INTERLEAVED if interleaved else 0) | (_NO_NORM if eps is None else 0)
+    args = (ctypes.addressof(qs), None if ks is None else ctypes.addressof(ks), _lib.ptr(cos), _lib.ptr(sin),
+            0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1], B, D, eps or 0.0,
+            _lib.dtype_code(dtype), flags)
+    if not bwd:
+        _lib.check(lib.hclsm_qk_norm_rope(*args, _lib.stream_ptr(device)), "hclsm_qk_norm_rope")
+        return
+    ws, n = None, 0
+    if qs.dw or (ks is not None and ks.dw):
+        n = lib.hclsm_qk_norm_rope_bwd_workspace_size(D)
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+    _lib.check(lib.hclsm_qk_norm_rope_bwd(*args, _lib.ptr(ws), n, _lib.stream_ptr(device)), "hclsm_qk_norm_rope_bwd")
+
+
+def _forward(q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved):
+    q = _lib.rows16(q)
+    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    qs, ks, yk = _side(q, yq, qw, q_pos), None, None
+    if k is not None:
+        k = _lib.rows16(k)
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        ks = _side(k, yk, kw, k_pos)
+    _call(False, qs, ks, cos, sin, q.shape[0], q.shape[3], eps, q.dtype, interleaved, q.device)
+    return q, k, yq, yk
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved):
+        q, k, yq, yk = _forward(q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved)
+        ctx.save_for_backward(q, k, qw, kw, cos, sin, q_pos, k_pos)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return yq, yk
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, qw, kw, cos, sin, q_pos, k_pos = ctx.saved_tensors
+
+        def one(x, w, pos, g, want_w):
+            if x is None:
+                return None, None, None
+            g = _lib.rows16(g.to(x.dtype).contiguous())
+            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dw = torch.empty_like(w) if w is not None and want_w else None
+            return _side(x, dx, w, pos, g, dw), dx, dw, g
+
+        qs, dq, dqw, _gq = one(q, qw, q_pos, gq, ctx.needs_input_grad[2])
+        ks = dk = dkw = None
+        if k is not None:
+            ks, dk, dkw, _gk = one(k, kw, k_pos, gk, ctx.needs_input_grad[3])
+        _call(True, qs, ks, cos, sin, q.shape[0], q.shape[3], ctx.eps, q.dtype, ctx.interleaved, q.device)
+        return dq, dk, dqw, dkw, None, None, None, None, None, None
+
+
+def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, *, q_pos=None, k_pos=None, eps=1e-6,
+                 interleaved: bool = False):
+    """(q', k') with every head normalised by its root mean square, weighted and
+    rotated; k may be None (queries alone), and so may the weights and the tables.
+
+    ``q_pos`` (B, Lq) and ``k_pos`` (B, Lk): rows of ``cos`` / ``sin``
+    (positions, rotary_dim / 2), default 0, 1, 2, ...; a position outside the
+    tables gives NaN in that token's rotated dims and sets the device error word.
+    ``eps=None`` leaves the norm out.  Pairs are dims (i, i + rotary_dim / 2), or
+    (2 i, 2 i + 1) with ``interleaved``; rotary_dim is a multiple of 16 (8
+    interleaved).  Differentiable in q, k and the weights; rows of q and k may be
+    strided (each head dense).
+    """
+    dev = _check(q, k, q_weight, k_weight, cos, sin, eps)
+    if cos is not None:
+        cos, sin = _lib.rows16(cos.contiguous()), _lib.rows16(sin.contiguous())
+        rot = 2 * cos.shape[1]
+        if rot > q.shape[3] or rot % (8 if interleaved else 16):
+            raise ValueError(f"rotary_dim {rot} must be a multiple of {8 if interleaved else 16} up to head_dim")
+    B, Lq = q.shape[:2]
+    if cos is not None:
+        q_pos = _lib.index32(q_pos, (B, Lq), "q_pos", dev)
+        if q_pos is None and Lq > cos.shape[0]:
+            raise ValueError(f"{Lq} query positions, tables of {cos.shape[0]}")
+        if k is not None:
+            k_pos = _lib.index32(k_pos, (B, k.shape[1]), "k_pos", dev)
+            if k_pos is None and k.shape[1] > cos.shape[0]:
+                raise ValueError(f"{k.shape[1]} key positions, tables of {cos.shape[0]}")
+    else:
+        q_pos = k_pos = None
+    if k is None:
+        k_pos = None
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
+    args = (q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, None if eps is None else float(eps), bool(interleaved))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _QkNormRope.apply(*args)
+    return _forward(*args)[2:]

@@ -342,6 +342,96 @@ int hclsm_ssm_scan_bwd_noalloc(const void* x, const void* dt, const float* A_log
                                int64_t nseq, int32_t L, int32_t d_inner, int32_t d_state, int32_t dtype,
                                int32_t clamp, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention between sets of states of different lengths, the norm and rotation
+ * of its queries and keys, and an 8-bit cache of the states.  The reference has
+ * the cross attention of its goal transformer as a torch module
+ * (hclsm/dynamics/level2_goal.py:88-141) and no counterpart of the others.
+ *
+ * hclsm_view: a (B, L, H, D) tensor, D dense, the other strides in elements.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  const void* p;
+  int64_t sb, st, sh;
+} hclsm_view;
+
+/* One of the two tensors of hclsm_qk_norm_rope.  x may be strided (each stride
+ * a multiple of 16 bytes); y and dy are dense (B, L, H, D).  Backward: y is dx. */
+typedef struct {
+  const void* x;
+  const void* dy;      /* backward only */
+  void* y;
+  const float* w;      /* (D) or NULL: no weight */
+  const int32_t* pos;  /* (B, L) rows of the tables, or NULL: 0, 1, ... L - 1 */
+  float* dw;           /* backward: (D) or NULL */
+  int64_t sb, st, sh;
+  int32_t L, H;
+} hclsm_rope_side;
+
+typedef enum { HCLSM_ROPE_INTERLEAVED = 1, HCLSM_ROPE_NO_NORM = 2 } hclsm_rope_flags;
+
+/* y = R(pos) (x * rsqrt(mean(x^2) + eps) * w) for each head of q and of k (NULL:
+ * queries alone) in one launch.  R turns the first `rot` dims as rot / 2 pairs
+ * by the angles whose cosines and sines are row pos of cosv, sinv (P, rot / 2):
+ * dims (i, i + rot / 2), or (2 i, 2 i + 1) with HCLSM_ROPE_INTERLEAVED.
+ * HCLSM_ROPE_NO_NORM: the rotation alone.  D a multiple of 8 up to 256; rot a
+ * multiple of 16 (8 interleaved), 0 for none.  A position outside the tables
+ * gives NaN in the rotated dims and HCLSM_ERR_SHAPE in the error word. */
+int hclsm_qk_norm_rope(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv,
+                       const float* sinv, int32_t P, int32_t rot, int64_t B, int32_t D, float eps,
+                       int32_t dtype, int32_t flags, void* stream);
+size_t hclsm_qk_norm_rope_bwd_workspace_size(int32_t D);
+int hclsm_qk_norm_rope_bwd(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv,
+                           const float* sinv, int32_t P, int32_t rot, int64_t B, int32_t D,
+                           float eps, int32_t dtype, int32_t flags, void* ws, size_t ws_bytes,
+                           void* stream);
+
+/* Cross attention o = softmax(scale q k^T) v over the keys that lens (B) and
+ * mask (B, Lk; rows mask_sb bytes apart) allow; a row with none gives 0.
+ * H a multiple of Hkv: query head h reads key head h / (H / Hkv).  D <= 128.
+ * o and the gradients are dense.  lse2 (B, H, Lq): NULL when no backward
+ * follows; the backward reads what the forward wrote. */
+typedef struct {
+  hclsm_view q, k, v, dout;
+  void* o;
+  void *dq, *dk, *dv;  /* backward only */
+  float* lse2;
+  const int32_t* lens; /* or NULL */
+  const uint8_t* mask; /* or NULL */
+  int64_t mask_sb;
+  int32_t B, Lq, Lk, H, Hkv, D, dtype;
+  float scale;         /* positive */
+} hclsm_xattn_args;
+
+size_t hclsm_xattn_fwd_workspace_size(const hclsm_xattn_args* a);
+int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream);
+size_t hclsm_xattn_bwd_workspace_size(const hclsm_xattn_args* a);
+int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/* The 8-bit state cache.  Complete blocks of `block` tokens a head are 8-bit
+ * integers with one fp32 scale, max|x| / 127; the last, incomplete block of a
+ * sequence is held in `dtype` (the tail).  D 32, 64, 96 or 128; block 16, 32,
+ * 64 or 128; T a multiple of block. */
+typedef struct {
+  int8_t *k, *v;             /* (B, Hkv, T, D) */
+  float *k_scale, *v_scale;  /* (B, Hkv, T / block) */
+  void *k_tail, *v_tail;     /* (B, Hkv, block, D) dtype */
+  int32_t B, Hkv, T, D, block, dtype;
+} hclsm_kv8_cache;
+
+/* Tokens [0, count[b]) of k, v (B, n, Hkv, D; NULL count: n) become tokens
+ * start[b], start[b] + 1, ... of the cache.  A request that does not fit (start
+ * < 0, count outside [0, n], start + count > T) writes nothing and puts
+ * HCLSM_ERR_SHAPE in the error word. */
+int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, const hclsm_view* v, int32_t n,
+                    const int32_t* start, const int32_t* count, void* stream);
+/* The first lens[b] tokens (NULL: T) as dense (B, T, Hkv, D), zeros after them. */
+int hclsm_kv8_read(const hclsm_kv8_cache* c, void* k, void* v, const int32_t* lens, void* stream);
+/* Attention of q (B, Lq, H, D) over the first lens[b] tokens; o dense. */
+size_t hclsm_kv8_attn_workspace_size(const hclsm_kv8_cache* c, int32_t Lq, int32_t H);
+int hclsm_kv8_attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens,
+                   int32_t Lq, int32_t H, float scale, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
