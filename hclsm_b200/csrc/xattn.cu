@@ -355,7 +355,8 @@ static bool use_split(const xattn::Params& p, int dtype) {
 extern "C" size_t hclsm_xattn_fwd_workspace_size(const hclsm_xattn_args* a) {
   if (xattn::check(a)) return 0;
   const xattn::Params p = xattn::params(a);
-  return use_split(p, a->dtype) ? xattn::split_workspace(p) : 0;
+  if (use_split(p, a->dtype)) return xattn::split_workspace(p);
+  return a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false) ? xattn::tc_workspace(p) : 0;
 }
 
 extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -368,6 +369,11 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
     const size_t need = xattn::split_workspace(p);
     if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
     return xattn::split_fwd(p, a->dtype, ws, st);
+  }
+  if (a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false)) {
+    const size_t need = xattn::tc_workspace(p);
+    if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+    return xattn::tc_fwd(p, ws, st);
   }
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
 }

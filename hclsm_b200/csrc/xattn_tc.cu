@@ -1,0 +1,436 @@
+// Cross attention in bf16 on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
+//
+// Forward: a block takes QT tiles of 128 query rows of one head (QT 2: one block
+// an SM; QT 1: two), each with a softmax warpgroup (thread = row = TMEM lane), a
+// warp that issues TMA and a warp that issues MMA.  Per tile of 128 keys:
+//   S = Q K^T        128 x 128, fp32 in TMEM
+//   the row's thread reads its 128 scores, takes the running maximum, writes
+//   P = exp2(c s - m) as bf16 over S in TMEM, keeps the row sum in fp32
+//   O += P V         A from TMEM, V as the MN-major B operand; fp32 in TMEM
+// The maximum that O is scaled by is raised only when a row's new one exceeds it by
+// 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
+// with the same relative precision, and O is read back and rescaled rarely.
+// While one warpgroup takes its softmax the tensor cores run the other's products.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "tcgen05.cuh"
+#include "xattn.cuh"
+
+namespace hclsm {
+namespace xattn {
+
+using namespace ::hclsm::tc;
+
+constexpr int kTile = 128;            // query rows and keys of a forward tile
+constexpr uint32_t kRowBytes = 128;   // a 64-dim bf16 row of a swizzled block
+constexpr float kRaise = 8.0f;
+
+struct TcParams {
+  Params x;
+  const uint32_t* words;  // (B, word_sb) bits of the key mask, or null
+  int word_sb;
+  int qtiles;  // of QT * 128 rows
+};
+
+// The allowed keys of [k0, k0 + 128) as bits.
+__device__ __forceinline__ uint4 key_bits(const TcParams& p, int64_t b, int n, int k0) {
+  auto below = [&](int base) {
+    const int left = n - base;
+    return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+  };
+  uint4 r = make_uint4(below(k0), below(k0 + 32), below(k0 + 64), below(k0 + 96));
+  if (p.words) {
+    const uint4 w = *reinterpret_cast<const uint4*>(p.words + b * p.word_sb + k0 / 32);
+    r.x &= w.x, r.y &= w.y, r.z &= w.z, r.w &= w.w;
+  }
+  return r;
+}
+__device__ __forceinline__ bool all_bits(const uint4& w) { return (w.x & w.y & w.z & w.w) == 0xffffffffu; }
+
+// Zero the rows of a staged tile whose bit is off (a whole warp): an operand that
+// may be NaN or stale memory must not meet a zero weight.
+template <int DP, int ROWS>
+__device__ __forceinline__ void zero_rows(unsigned char* tile, const uint4& w, int lane) {
+  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < ROWS / 32; ++i)
+    if (!(word[i] >> lane & 1u)) {
+#pragma unroll
+      for (int kb = 0; kb < DP / 64; ++kb) {
+        uint4* row = reinterpret_cast<uint4*>(tile + ((size_t)kb * ROWS + i * 32 + lane) * kRowBytes);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) row[c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
+      " mov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+template <int DP, int QT> struct FwdShape {
+  static constexpr int kBlock = kTile * kRowBytes;        // 64 dims of a tile
+  static constexpr int kOp = DP / 64 * kBlock;            // a staged tile
+  static constexpr int kStages = DP == 64 ? (QT == 2 ? 3 : 2) : (QT == 2 ? 2 : 1);
+  static constexpr int kBars = 1 + 4 * kStages + 3 * QT;
+  static constexpr size_t kBytes = (size_t)(QT + 2 * kStages) * kOp + kBars * 8 + 1024;
+  static constexpr int kThreads = QT * 128 + 64;
+  static constexpr uint32_t kCols = QT == 2 ? 512 : 256;
+};
+
+template <int DP, int QT>
+__global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
+    tc_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                  const __grid_constant__ CUtensorMap mv, const __grid_constant__ TcParams p) {
+  using Sh = FwdShape<DP, QT>;
+  constexpr int ST = Sh::kStages;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  unsigned char *sQ = smem, *sK = sQ + QT * Sh::kOp, *sV = sK + ST * Sh::kOp;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::kOp);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST,
+           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  constexpr int kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"(Sh::kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    s_abort = 0;
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], &bars[i] >= p_full && &bars[i] < pv_done ? 128 : 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem = s_tmem;  // tile w: scores and weights in columns [w * 128, + 128), O in [QT * 128 + w * DP, + DP)
+  const Params& x = p.x;
+  const int q0 = (int)(blockIdx.x % p.qtiles) * (QT * kTile);
+  const int h = (int)(blockIdx.x / p.qtiles % x.H), hk = h / (x.H / x.Hkv);
+  const int64_t b = blockIdx.x / p.qtiles / x.H;
+  const int nk = key_count(x, b), tiles = (nk + kTile - 1) / kTile;
+  const int nq = QT == 2 && q0 + kTile >= x.Lq ? 1 : QT;  // tiles with rows
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, x.err); };
+
+  if (warp == kTmaWarp) {
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(q_full, nq * Sh::kOp);
+      for (int w = 0; w < nq; ++w)
+        for (int kb = 0; kb < DP / 64; ++kb)
+          tma_load_4d(sQ + w * Sh::kOp + kb * Sh::kBlock, &mq, kb * 64, q0 + w * kTile, h, (int)b, q_full);
+      for (int j = 0; j < tiles; ++j) {
+        const int s = j % ST;
+        const uint32_t ph = j / ST;
+        if (!wait(&k_empty[s], ph ^ 1)) break;
+        mbar_expect_tx(&k_full[s], Sh::kOp);
+        for (int kb = 0; kb < DP / 64; ++kb)
+          tma_load_4d(sK + s * Sh::kOp + kb * Sh::kBlock, &mk, kb * 64, j * kTile, hk, (int)b, &k_full[s]);
+        if (!wait(&v_empty[s], ph ^ 1)) break;
+        mbar_expect_tx(&v_full[s], Sh::kOp);
+        for (int kb = 0; kb < DP / 64; ++kb)
+          tma_load_4d(sV + s * Sh::kOp + kb * Sh::kBlock, &mv, kb * 64, j * kTile, hk, (int)b, &v_full[s]);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const uint32_t id_s = idesc_bf16(kTile, kTile, false, false);
+    const uint32_t id_o = idesc_bf16(kTile, (x.D + 15) / 16 * 16, false, true);
+    const int ksteps = (x.D + 15) / 16;
+    auto scores = [&](int w, int s) {
+      if (lane == 0) {
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t off = (k >> 2) * Sh::kBlock + (k & 3) * 32;
+          umma_bf16(tmem + w * 128, smem_desc_sw128(smem_u32(sQ + w * Sh::kOp) + off, 16, 1024),
+                    smem_desc_sw128(smem_u32(sK + s * Sh::kOp) + off, 16, 1024), id_s, k != 0);
+        }
+        umma_commit(&s_full[w]);
+      }
+      __syncwarp();
+    };
+    bool ok = tiles > 0 && wait(q_full, 0) && wait(&k_full[0], 0);
+    if (ok) {
+      tc_fence_after();
+      for (int w = 0; w < nq; ++w) scores(w, 0);
+      if (lane == 0) umma_commit(&k_empty[0]);
+      for (int j = 0; j < tiles && ok; ++j) {
+        const int s = j % ST, s1 = (j + 1) % ST;
+        const bool more = j + 1 < tiles;
+        if (!(ok = wait(&v_full[s], j / ST))) break;
+        const uint4 bits = key_bits(p, b, nk, j * kTile);
+        if (!all_bits(bits)) zero_rows<DP, kTile>(sV + s * Sh::kOp, bits, lane);
+        for (int w = 0; w < nq && ok; ++w) {
+          if (!(ok = wait(&p_full[w], j))) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)
+              umma_bf16_ts(tmem + QT * 128 + w * DP, tmem + w * 128 + k * 8,
+                           smem_desc_sw128(smem_u32(sV + s * Sh::kOp) + k * 16 * kRowBytes, Sh::kBlock, 1024), id_o,
+                           (j | k) != 0);
+            umma_commit(&pv_done[w]);
+            if (w == nq - 1) umma_commit(&v_empty[s]);
+          }
+          __syncwarp();
+          if (more) {
+            if (w == 0 && !(ok = wait(&k_full[s1], (j + 1) / ST))) break;
+            tc_fence_after();
+            scores(w, s1);
+            if (w == nq - 1 && lane == 0) umma_commit(&k_empty[s1]);
+          }
+        }
+      }
+    }
+  } else if (warp < QT * 4) {
+    const int w = warp >> 2;
+    const int row = q0 + w * kTile + (tid & 127);
+    const bool idle = q0 + w * kTile + (warp & 3) * 32 >= x.Lq;  // no row of this warp: it only keeps the phases
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + QT * 128 + w * DP;
+    const float c2 = x.scale * kLog2e;
+    float m = -INFINITY;  // the maximum O is scaled by, raw scores
+    float2 l = make_float2(0.0f, 0.0f);
+    bool ok = true;
+    if (w < nq) {
+      for (int j = 0; j < tiles; ++j) {
+        const uint4 bits = key_bits(p, b, nk, j * kTile);
+        if (!(ok = wait(&s_full[w], j))) break;
+        tc_fence_after();
+        if (idle) {
+          mbar_arrive(&p_full[w]);
+          continue;
+        }
+        // The scores are read twice, for the maximum and for the weights: a row of 128
+        // does not fit the registers beside the rest.
+        const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+        const bool all = all_bits(bits);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          float v[64];
+          tmem_ld32_nowait(tS + c * 32, v);
+          tmem_ld32_nowait(tS + c * 32 + 32, v + 32);
+          tmem_wait_ld();
+          tmem_pin<64>(v);
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i) v[i] = word[c + i / 32] >> (i & 31) & 1u ? v[i] : -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // the first keys of a row set its maximum; O is zero (j = 0: not yet written) till then
+        const bool raise = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
+        if (__any_sync(0xffffffffu, raise)) {
+          const float f = raise ? ex2((m - top) * c2) : 1.0f;  // 0 from -inf
+          if (raise) m = top;
+          l.x *= f, l.y *= f;
+          if (j > 0) {
+            if (!(ok = wait(&pv_done[w], j - 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < DP; c += 16) {
+              float o[16];
+              tmem_ld16_nowait(tO + c, o);
+              tmem_wait_ld();
+              tmem_pin<16>(o);
+              uint32_t r[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(o[i] * f);
+              tmem_st16(tO + c, r);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : -m * c2;
+        const float2 cc = make_float2(c2, c2), bb = make_float2(base, base);
+        float v[2][32];
+        tmem_ld32_nowait(tS, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld();
+          tmem_pin<32>(v[c & 1]);
+          if (c < 3) tmem_ld32_nowait(tS + c * 32 + 32, v[(c + 1) & 1]);
+          float* u = v[c & 1];
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) u[i] = word[c] >> i & 1u ? u[i] : -INFINITY;
+          }
+          uint32_t pw[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = fma2(make_float2(u[2 * i], u[2 * i + 1]), cc, bb);
+            e.x = ex2(e.x), e.y = ex2(e.y);
+            l = add2(l, e);
+            pw[i] = pack_bf16(e.x, e.y);
+          }
+          // over scores that have been read: columns [16 c, + 16) of [32 c, ...)
+          tmem_st16(tS + c * 16, pw);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+      }
+      if (ok && tiles > 0) ok = wait(&pv_done[w], tiles - 1);
+      tc_fence_after();
+      if (!idle) {
+        const float sum = l.x + l.y;
+        const float inv = tiles > 0 && sum != 0.0f ? 1.0f / sum : 0.0f;
+        if (row < x.Lq && x.lse2)
+          x.lse2[(b * x.H + h) * x.Lq + row] = sum == 0.0f ? INFINITY : m * c2 + log2f(sum);
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(x.o) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          float o[32];
+          if (tiles > 0) {
+            tmem_ld32_nowait(tO + c, o);
+            tmem_wait_ld();
+            tmem_pin<32>(o);
+          }
+          if (row < x.Lq) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+              if (c + i < x.D) {
+                uint32_t r[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // a row without keys: zero, whatever O holds
+                  r[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
+                *reinterpret_cast<uint4*>(out + c + i) = make_uint4(r[0], r[1], r[2], r[3]);
+              }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kCols) : "memory");
+}
+
+// ---- the key mask as bits ------------------------------------------------------------------
+__global__ void __launch_bounds__(256) bits_kernel(const __grid_constant__ Params p, uint32_t* words, int word_sb) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t b = i / ((int64_t)word_sb * 32);
+  const int j = (int)(i % ((int64_t)word_sb * 32));
+  const bool on = b < p.B && j < p.Lk && p.mask[b * p.mask_sb + j];
+  const uint32_t w = __ballot_sync(0xffffffffu, on);
+  if ((threadIdx.x & 31) == 0 && b < p.B) words[b * word_sb + j / 32] = w;
+}
+
+// ---- host ----------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(p);
+  });
+  return fn;
+}
+
+// (D, L, H, B) bf16, box (64, rows, 1, 1), 128-byte swizzle, zeros outside.
+static bool make_map(CUtensorMap* m, const View& v, int D, int L, int H, int B, int rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)v.st * 2, (cuuint64_t)v.sh * 2, (cuuint64_t)v.sb * 2};
+  for (int i = 0; i < 3; ++i)
+    if (dims[i + 1] == 1) strides[i] = (cuuint64_t)((D + 7) / 8 * 16);  // never stepped over
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(v.p), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a tensor map can describe: 16-byte aligned rows, positive strides.
+static bool mappable(const View& v, int L, int H, int B) {
+  auto ok = [](int n, int64_t s) { return n == 1 || (s > 0 && s % 8 == 0 && s < ((int64_t)1 << 38)); };
+  return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && ok(L, v.st) && ok(H, v.sh) && ok(B, v.sb);
+}
+
+bool tc_ok(const Params& p, bool bwd) {
+  return p.D % 8 == 0 && p.Lk > 0 && p.Lq > 0 && mappable(p.q, p.Lq, p.H, p.B) && mappable(p.k, p.Lk, p.Hkv, p.B) &&
+         mappable(p.v, p.Lk, p.Hkv, p.B) && (!bwd || mappable(p.dout, p.Lq, p.H, p.B)) &&
+         reinterpret_cast<uintptr_t>(p.o) % 16 == 0;
+}
+
+static int word_stride(const Params& p) { return (p.Lk + kTile - 1) / kTile * (kTile / 32); }
+
+size_t tc_workspace(const Params& p) { return p.mask ? (size_t)p.B * word_stride(p) * sizeof(uint32_t) : 0; }
+
+static int make_bits(TcParams& t, void* ws, cudaStream_t st) {
+  t.words = nullptr, t.word_sb = 0;
+  if (!t.x.mask) return HCLSM_OK;
+  t.word_sb = word_stride(t.x);
+  t.words = static_cast<uint32_t*>(ws);
+  const int64_t grid = ((int64_t)t.x.B * t.word_sb * 32 + 255) / 256;
+  if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  return launch_pdl(bits_kernel, (unsigned)grid, 256, 0, st, t.x, static_cast<uint32_t*>(ws), t.word_sb);
+}
+
+template <int DP, int QT>
+static int launch_fwd(TcParams& t, cudaStream_t st) {
+  using Sh = FwdShape<DP, QT>;
+  const Params& x = t.x;
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, x.q, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&mk, x.k, x.D, x.Lk, x.Hkv, x.B, kTile) ||
+      !make_map(&mv, x.v, x.D, x.Lk, x.Hkv, x.B, kTile))
+    return HCLSM_ERR_UNSUPPORTED;
+  t.qtiles = (x.Lq + QT * kTile - 1) / (QT * kTile);
+  const int64_t grid = (int64_t)t.qtiles * x.H * x.B;
+  if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  auto fn = tc_fwd_kernel<DP, QT>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(fn), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
+  return launch_pdl(fn, (unsigned)grid, Sh::kThreads, Sh::kBytes, st, mq, mk, mv, t);
+}
+
+int tc_fwd(const Params& p, void* ws, cudaStream_t st) {
+  TcParams t = {};
+  t.x = p;
+  if (const int rc = make_bits(t, ws, st)) return rc;
+  const bool two = p.Lq > kTile;
+  if (p.D <= 64) return two ? launch_fwd<64, 2>(t, st) : launch_fwd<64, 1>(t, st);
+  return two ? launch_fwd<128, 2>(t, st) : launch_fwd<128, 1>(t, st);
+}
+
+}  // namespace xattn
+}  // namespace hclsm
