@@ -305,15 +305,20 @@ int run(const Params& p, bool bwd, cudaStream_t st) {
 
 template <typename T>
 int dispatch(const Params& p, bool bwd, cudaStream_t st) {
-  if (bwd && (int64_t)p.B * p.Lq > 0) {
-    const int64_t rows = (int64_t)p.B * p.Lq * p.H, grid = (rows + 7) / 8;
-    if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
-    if (const int rc = launch_pdl(delta_kernel<T>, (unsigned)grid, kThreads, 0, st, p)) return rc;
-  }
   if (p.D <= 32) return run<T, 32>(p, bwd, st);
   if (p.D <= 64) return run<T, 64>(p, bwd, st);
   return run<T, 128>(p, bwd, st);
 }
+
+int launch_delta(const Params& p, int dtype, cudaStream_t st) {
+  const int64_t rows = (int64_t)p.B * p.Lq * p.H, grid = (rows + 7) / 8;
+  if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  if (grid == 0) return HCLSM_OK;
+  return dtype == HCLSM_F32 ? launch_pdl(delta_kernel<float>, (unsigned)grid, kThreads, 0, st, p)
+                            : launch_pdl(delta_kernel<__nv_bfloat16>, (unsigned)grid, kThreads, 0, st, p);
+}
+
+size_t delta_bytes(const Params& p) { return ((size_t)p.B * p.H * p.Lq * sizeof(float) + 15) / 16 * 16; }
 
 int check(const hclsm_xattn_args* a) {
   if (!a) return HCLSM_ERR_NULL;
@@ -378,9 +383,15 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
 }
 
+static bool use_tc_bwd(const xattn::Params& p, int dtype) {
+  auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  return dtype == HCLSM_BF16 && xattn::tc_ok(p, true) && al(p.dq) && al(p.dk) && al(p.dv);
+}
+
 extern "C" size_t hclsm_xattn_bwd_workspace_size(const hclsm_xattn_args* a) {
   if (xattn::check(a)) return 0;
-  return (size_t)a->B * a->H * a->Lq * sizeof(float);
+  const xattn::Params p = xattn::params(a);
+  return xattn::delta_bytes(p) + (a->dtype == HCLSM_BF16 ? xattn::tc_workspace(p) : 0);
 }
 
 extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -392,5 +403,7 @@ extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   xattn::Params p = xattn::params(a);
   p.delta = static_cast<float*>(ws);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (const int rc = xattn::launch_delta(p, a->dtype, st)) return rc;
+  if (use_tc_bwd(p, a->dtype)) return xattn::tc_bwd(p, static_cast<char*>(ws) + xattn::delta_bytes(p), st);
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, true, st) : xattn::dispatch<__nv_bfloat16>(p, true, st);
 }

@@ -52,6 +52,7 @@ __device__ __forceinline__ bool key_ok(const Params& p, int64_t b, int n, int j)
 bool tc_ok(const Params& p, bool bwd);
 size_t tc_workspace(const Params& p);
 int tc_fwd(const Params& p, void* ws, cudaStream_t st);
+int tc_bwd(const Params& p, void* ws, cudaStream_t st);
 // Few query rows, the keys split over blocks (attn_split.cu).
 size_t split_workspace(const Params& p);
 int split_fwd(const Params& p, int dtype, void* ws, cudaStream_t st);

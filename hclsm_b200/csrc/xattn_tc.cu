@@ -11,83 +11,12 @@
 // 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
 // with the same relative precision, and O is read back and rescaled rarely.
 // While one warpgroup takes its softmax the tensor cores run the other's products.
-#include <cuda.h>
-
-#include <mutex>
-
-#include "tcgen05.cuh"
-#include "xattn.cuh"
+#include "xattn_tc.cuh"
 
 namespace hclsm {
 namespace xattn {
 
-using namespace ::hclsm::tc;
-
-constexpr int kTile = 128;            // query rows and keys of a forward tile
-constexpr uint32_t kRowBytes = 128;   // a 64-dim bf16 row of a swizzled block
 constexpr float kRaise = 8.0f;
-
-struct TcParams {
-  Params x;
-  const uint32_t* words;  // (B, word_sb) bits of the key mask, or null
-  int word_sb;
-  int qtiles;  // of QT * 128 rows
-};
-
-// The allowed keys of [k0, k0 + 128) as bits.
-__device__ __forceinline__ uint4 key_bits(const TcParams& p, int64_t b, int n, int k0) {
-  auto below = [&](int base) {
-    const int left = n - base;
-    return left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
-  };
-  uint4 r = make_uint4(below(k0), below(k0 + 32), below(k0 + 64), below(k0 + 96));
-  if (p.words) {
-    const uint4 w = *reinterpret_cast<const uint4*>(p.words + b * p.word_sb + k0 / 32);
-    r.x &= w.x, r.y &= w.y, r.z &= w.z, r.w &= w.w;
-  }
-  return r;
-}
-__device__ __forceinline__ bool all_bits(const uint4& w) { return (w.x & w.y & w.z & w.w) == 0xffffffffu; }
-
-// Zero the rows of a staged tile whose bit is off (a whole warp): an operand that
-// may be NaN or stale memory must not meet a zero weight.
-template <int DP, int ROWS>
-__device__ __forceinline__ void zero_rows(unsigned char* tile, const uint4& w, int lane) {
-  const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < ROWS / 32; ++i)
-    if (!(word[i] >> lane & 1u)) {
-#pragma unroll
-      for (int kb = 0; kb < DP / 64; ++kb) {
-        uint4* row = reinterpret_cast<uint4*>(tile + ((size_t)kb * ROWS + i * 32 + lane) * kRowBytes);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) row[c] = make_uint4(0, 0, 0, 0);
-      }
-    }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
-      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n"
-      " mov.b64 {%0, %1}, x;\n}\n"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
 
 template <int DP, int QT> struct FwdShape {
   static constexpr int kBlock = kTile * kRowBytes;        // 64 dims of a tile
@@ -140,6 +69,8 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   const int nk = key_count(x, b), tiles = (nk + kTile - 1) / kTile;
   const int nq = QT == 2 && q0 + kTile >= x.Lq ? 1 : QT;  // tiles with rows
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, x.err); };
+  // the whole warp goes on or gives up together
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
   if (warp == kTmaWarp) {
     if (lane == 0 && tiles > 0) {
@@ -175,7 +106,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       }
       __syncwarp();
     };
-    bool ok = tiles > 0 && wait(q_full, 0) && wait(&k_full[0], 0);
+    bool ok = tiles > 0 && wait_all(q_full, 0) && wait_all(&k_full[0], 0);
     if (ok) {
       tc_fence_after();
       for (int w = 0; w < nq; ++w) scores(w, 0);
@@ -183,11 +114,11 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       for (int j = 0; j < tiles && ok; ++j) {
         const int s = j % ST, s1 = (j + 1) % ST;
         const bool more = j + 1 < tiles;
-        if (!(ok = wait(&v_full[s], j / ST))) break;
+        if (!(ok = wait_all(&v_full[s], j / ST))) break;
         const uint4 bits = key_bits(p, b, nk, j * kTile);
         if (!all_bits(bits)) zero_rows<DP, kTile>(sV + s * Sh::kOp, bits, lane);
         for (int w = 0; w < nq && ok; ++w) {
-          if (!(ok = wait(&p_full[w], j))) break;
+          if (!(ok = wait_all(&p_full[w], j))) break;
           tc_fence_after();
           if (lane == 0) {
 #pragma unroll
@@ -200,7 +131,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
           }
           __syncwarp();
           if (more) {
-            if (w == 0 && !(ok = wait(&k_full[s1], (j + 1) / ST))) break;
+            if (w == 0 && !(ok = wait_all(&k_full[s1], (j + 1) / ST))) break;
             tc_fence_after();
             scores(w, s1);
             if (w == nq - 1 && lane == 0) umma_commit(&k_empty[s1]);
@@ -221,7 +152,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
     if (w < nq) {
       for (int j = 0; j < tiles; ++j) {
         const uint4 bits = key_bits(p, b, nk, j * kTile);
-        if (!(ok = wait(&s_full[w], j))) break;
+        if (!(ok = wait_all(&s_full[w], j))) break;
         tc_fence_after();
         if (idle) {
           mbar_arrive(&p_full[w]);
@@ -254,7 +185,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
           if (raise) m = top;
           l.x *= f, l.y *= f;
           if (j > 0) {
-            if (!(ok = wait(&pv_done[w], j - 1))) break;
+            if (!(ok = wait_all(&pv_done[w], j - 1))) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < DP; c += 16) {
@@ -298,7 +229,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
         tc_fence_before();
         mbar_arrive(&p_full[w]);
       }
-      if (ok && tiles > 0) ok = wait(&pv_done[w], tiles - 1);
+      if (ok && tiles > 0) ok = wait_all(&pv_done[w], tiles - 1);
       tc_fence_after();
       if (!idle) {
         const float sum = l.x + l.y;
@@ -348,56 +279,15 @@ __global__ void __launch_bounds__(256) bits_kernel(const __grid_constant__ Param
   if ((threadIdx.x & 31) == 0 && b < p.B) words[b * word_sb + j / 32] = w;
 }
 
-// ---- host ----------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
-// (D, L, H, B) bf16, box (64, rows, 1, 1), 128-byte swizzle, zeros outside.
-static bool make_map(CUtensorMap* m, const View& v, int D, int L, int H, int B, int rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
-  cuuint64_t strides[3] = {(cuuint64_t)v.st * 2, (cuuint64_t)v.sh * 2, (cuuint64_t)v.sb * 2};
-  for (int i = 0; i < 3; ++i)
-    if (dims[i + 1] == 1) strides[i] = (cuuint64_t)((D + 7) / 8 * 16);  // never stepped over
-  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(v.p), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// What a tensor map can describe: 16-byte aligned rows, positive strides.
-static bool mappable(const View& v, int L, int H, int B) {
-  auto ok = [](int n, int64_t s) { return n == 1 || (s > 0 && s % 8 == 0 && s < ((int64_t)1 << 38)); };
-  return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && ok(L, v.st) && ok(H, v.sh) && ok(B, v.sb);
-}
-
 bool tc_ok(const Params& p, bool bwd) {
   return p.D % 8 == 0 && p.Lk > 0 && p.Lq > 0 && mappable(p.q, p.Lq, p.H, p.B) && mappable(p.k, p.Lk, p.Hkv, p.B) &&
          mappable(p.v, p.Lk, p.Hkv, p.B) && (!bwd || mappable(p.dout, p.Lq, p.H, p.B)) &&
          reinterpret_cast<uintptr_t>(p.o) % 16 == 0;
 }
 
-static int word_stride(const Params& p) { return (p.Lk + kTile - 1) / kTile * (kTile / 32); }
-
 size_t tc_workspace(const Params& p) { return p.mask ? (size_t)p.B * word_stride(p) * sizeof(uint32_t) : 0; }
 
-static int make_bits(TcParams& t, void* ws, cudaStream_t st) {
+int make_bits(TcParams& t, void* ws, cudaStream_t st) {
   t.words = nullptr, t.word_sb = 0;
   if (!t.x.mask) return HCLSM_OK;
   t.word_sb = word_stride(t.x);

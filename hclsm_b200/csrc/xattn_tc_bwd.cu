@@ -1,0 +1,412 @@
+// Cross attention backward in bf16 on the 5th-generation tensor cores.
+//
+// Two kernels, each with its own recomputation of the weights, so that every sum
+// has a fixed order (no atomics): 7 products instead of 5.
+//
+//   dq: a block takes 128 query rows and walks over tiles of 64 keys:
+//     S = Q K^T, dP = dO V^T  ->  dS = P (dP - delta), bf16 over S  ->  dQ += dS K
+//   dk, dv: a block takes 128 keys and walks over tiles of 64 query rows of every
+//   query head that shares them, transposed so that keys are the TMEM lanes:
+//     S^T = K Q^T, dP^T = V dO^T  ->  P^T over S^T, dS^T over dP^T  ->
+//     dV += P^T dO, dK += dS^T Q
+//
+// The weights and their gradients are A operands in TMEM; the same staged tile of
+// K (or Q, dO) is the K-major operand of one product and the MN-major operand of
+// another.  Two buffers of 64 + 64 columns: two warpgroups take alternate tiles, so
+// the tensor cores form one buffer's products while the other's weights are
+// computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
+// (128 or 256) do not fit TMEM's 512.
+#include "xattn_tc.cuh"
+
+namespace hclsm {
+namespace xattn {
+
+constexpr int kB = 64;  // keys (dq) or queries (dk, dv) of a streamed tile
+
+template <int DP> struct BwdShape {
+  static constexpr int kBlockA = kTile * kRowBytes, kBlockB = kB * kRowBytes;  // 64 dims
+  static constexpr int kOpA = DP / 64 * kBlockA, kOpB = DP / 64 * kBlockB;
+  static constexpr int kStages = 4;
+  static constexpr int kBars = 1 + 2 * kStages + 4 + 1;
+  static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
+  static constexpr int kThreads = 2 * 128 + 64;
+};
+
+// Shared by the two kernels: block layout, barriers, roles.
+template <int DP> struct Block {
+  using Sh = BwdShape<DP>;
+  unsigned char *a0, *a1, *b0, *b1;  // the block's own two operands, the streamed two
+  uint64_t *own, *full, *empty, *sd_full, *ds_full, *done;
+  __device__ __forceinline__ explicit Block(unsigned char* raw) {
+    a0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    a1 = a0 + Sh::kOpA, b0 = a1 + Sh::kOpA, b1 = b0 + Sh::kStages * Sh::kOpB;
+    own = reinterpret_cast<uint64_t*>(b1 + Sh::kStages * Sh::kOpB);
+    full = own + 1, empty = full + Sh::kStages, sd_full = empty + Sh::kStages, ds_full = sd_full + 2,
+    done = ds_full + 2;
+  }
+  __device__ __forceinline__ void init() const {
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 128 : 1);
+    fence_mbar_init();
+  }
+  // buffer w's two products of the streamed tile in stage s (one thread)
+  __device__ __forceinline__ void products(uint32_t tmem, int w, int s, int ksteps) const {
+    const uint32_t id = idesc_bf16(kTile, kB, false, false);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      for (int k = 0; k < ksteps; ++k) {
+        const uint32_t ka = (k >> 2) * Sh::kBlockA + (k & 3) * 32, kb = (k >> 2) * Sh::kBlockB + (k & 3) * 32;
+        umma_bf16(tmem + w * 128 + half * 64, smem_desc_sw128(smem_u32(half ? a1 : a0) + ka, 16, 1024),
+                  smem_desc_sw128(smem_u32((half ? b1 : b0) + s * Sh::kOpB) + kb, 16, 1024), id, k != 0);
+      }
+    umma_commit(&sd_full[w]);
+  }
+  // acc += (bf16 columns at a) x (streamed tile at b, as the MN-major operand) (one thread)
+  __device__ __forceinline__ void accumulate(uint32_t acc, uint32_t a, const unsigned char* b, int D, bool first) const {
+    const uint32_t id = idesc_bf16(kTile, (D + 15) / 16 * 16, false, true);
+#pragma unroll
+    for (int k = 0; k < kB / 16; ++k)
+      umma_bf16_ts(acc, a + k * 8, smem_desc_sw128(smem_u32(b) + k * 16 * kRowBytes, Sh::kBlockB, 1024), id,
+                   !(first && k == 0));
+  }
+};
+
+__device__ __forceinline__ void alloc_tmem(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void free_tmem(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// Columns [c0, c0 + n) of an accumulator's row to global memory, times f.
+template <int N>
+__device__ __forceinline__ void store_acc(uint32_t t, __nv_bfloat16* out, bool ok, bool zero, int c0, int D, float f) {
+#pragma unroll
+  for (int c = 0; c < N; c += 32) {
+    float o[32];
+    if (!zero) {
+      tmem_ld32_nowait(t + c0 + c, o);
+      tmem_wait_ld();
+      tmem_pin<32>(o);
+    }
+    if (!ok) continue;
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      if (c0 + c + i < D) {
+        uint32_t r[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = zero ? 0u : pack_bf16(o[i + 2 * e] * f, o[i + 2 * e + 1] * f);
+        *reinterpret_cast<uint4*>(out + c0 + c + i) = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+    tc_dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
+                 const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                 const __grid_constant__ TcParams p) {
+  using Sh = BwdShape<DP>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  const Block<DP> blk(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  if (warp == kMmaWarp) alloc_tmem(&s_tmem);
+  if (tid == 0) {
+    s_abort = 0;
+    blk.init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem = s_tmem, acc = tmem + 256;
+  const Params& x = p.x;
+  const int q0 = (int)(blockIdx.x % p.qtiles) * kTile;
+  const int h = (int)(blockIdx.x / p.qtiles % x.H), hk = h / (x.H / x.Hkv);
+  const int64_t b = blockIdx.x / p.qtiles / x.H;
+  const int nk = key_count(x, b), tiles = (nk + kB - 1) / kB;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, x.err); };
+  // the whole warp goes on or gives up together
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+  if (warp == kTmaWarp) {
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(blk.own, 2 * Sh::kOpA);
+      for (int kb = 0; kb < DP / 64; ++kb) {
+        tma_load_4d(blk.a0 + kb * Sh::kBlockA, &mq, kb * 64, q0, h, (int)b, blk.own);
+        tma_load_4d(blk.a1 + kb * Sh::kBlockA, &mdo, kb * 64, q0, h, (int)b, blk.own);
+      }
+      for (int j = 0; j < tiles; ++j) {
+        const int s = j % Sh::kStages;
+        if (!wait(&blk.empty[s], j / Sh::kStages ^ 1)) break;
+        mbar_expect_tx(&blk.full[s], 2 * Sh::kOpB);
+        for (int kb = 0; kb < DP / 64; ++kb) {
+          tma_load_4d(blk.b0 + s * Sh::kOpB + kb * Sh::kBlockB, &mk, kb * 64, j * kB, hk, (int)b, &blk.full[s]);
+          tma_load_4d(blk.b1 + s * Sh::kOpB + kb * Sh::kBlockB, &mv, kb * 64, j * kB, hk, (int)b, &blk.full[s]);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const int ksteps = (x.D + 15) / 16;
+    auto start = [&](int j) {  // the products of tile j into buffer j & 1
+      const int s = j % Sh::kStages;
+      if (!wait_all(&blk.full[s], j / Sh::kStages)) return false;
+      const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
+      const uint4 mine = j & 1 ? make_uint4(bits.z, bits.w, ~0u, ~0u) : make_uint4(bits.x, bits.y, ~0u, ~0u);
+      if (!all_bits(mine)) zero_rows<DP, kB>(blk.b0 + s * Sh::kOpB, mine, lane);  // dS 0 times K
+      tc_fence_after();
+      if (lane == 0) blk.products(tmem, j & 1, s, ksteps);
+      __syncwarp();
+      return true;
+    };
+    bool ok = tiles > 0 && wait_all(blk.own, 0) && start(0) && (tiles < 2 || start(1));
+    for (int j = 0; j < tiles && ok; ++j) {
+      if (!(ok = wait_all(&blk.ds_full[j & 1], j >> 1))) break;
+      tc_fence_after();
+      const int s = j % Sh::kStages;
+      if (lane == 0) {
+        blk.accumulate(acc, tmem + (j & 1) * 128, blk.b0 + s * Sh::kOpB, x.D, j == 0);
+        umma_commit(&blk.empty[s]);
+        if (j == tiles - 1) umma_commit(blk.done);
+      }
+      __syncwarp();
+      if (j + 2 < tiles) ok = start(j + 2);
+    }
+  } else {
+    const int w = warp >> 2;
+    const int row = q0 + (tid & 127);
+    const bool idle = q0 + (warp & 3) * 32 >= x.Lq;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + w * 128;
+    const int64_t at = (b * x.H + h) * x.Lq + row;
+    const float c2 = x.scale * kLog2e;
+    const float nl = row < x.Lq ? -x.lse2[at] : -INFINITY, delta = row < x.Lq ? x.delta[at] : 0.0f;
+    const float2 cc = make_float2(c2, c2), ll = make_float2(nl, nl), dd = make_float2(-delta, -delta);
+    bool ok = true;
+    for (int j = w; j < tiles; j += 2) {
+      const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
+      const uint32_t word[2] = {j & 1 ? bits.z : bits.x, j & 1 ? bits.w : bits.y};
+      if (!(ok = wait_all(&blk.sd_full[w], j >> 1))) break;
+      tc_fence_after();
+      if (!idle) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float s[32], g[32];
+          tmem_ld32_nowait(tS + c * 32, s);
+          tmem_ld32_nowait(tS + 64 + c * 32, g);
+          tmem_wait_ld();
+          tmem_pin<32>(s);
+          tmem_pin<32>(g);
+          uint32_t r[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
+            e.x = ex2(e.x), e.y = ex2(e.y);
+            const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
+            s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
+          }
+          if (word[c] != 0xffffffffu) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = word[c] >> i & 1u ? s[i] : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
+          tmem_st16(tS + c * 16, r);
+        }
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive(&blk.ds_full[w]);
+    }
+    if (ok && tiles > 0) wait_all(blk.done, 0);
+    tc_fence_after();
+    if (!idle)
+      store_acc<DP / 2>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
+                        row < x.Lq, tiles == 0, w * (DP / 2), x.D, x.scale);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) free_tmem(tmem);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+    tc_dkv_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                  const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
+                  const __grid_constant__ TcParams p) {
+  using Sh = BwdShape<DP>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_abort;
+  __shared__ float4 s_stat[2][2][2][kB / 4];  // warpgroup, slot, (-lse2, -delta)
+  const Block<DP> blk(smem_raw);
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  if (warp == kMmaWarp) alloc_tmem(&s_tmem);
+  if (tid == 0) {
+    s_abort = 0;
+    blk.init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t tmem = s_tmem, acc_v = tmem + 256, acc_k = acc_v + DP;
+  const Params& x = p.x;
+  const int ktiles = (x.Lk + kTile - 1) / kTile, qtiles = (x.Lq + kB - 1) / kB, G = x.H / x.Hkv;
+  const int k0 = (int)(blockIdx.x % ktiles) * kTile;
+  const int hk = (int)(blockIdx.x / ktiles % x.Hkv);
+  const int64_t b = blockIdx.x / ktiles / x.Hkv;
+  const int nk = key_count(x, b);
+  const int tiles = k0 < nk ? qtiles * G : 0;  // tile i: query head hk * G + i / qtiles, rows (i % qtiles) * 64 ...
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, x.err); };
+  // the whole warp goes on or gives up together
+  auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+  if (warp == kTmaWarp) {
+    if (lane == 0 && tiles > 0) {
+      mbar_expect_tx(blk.own, 2 * Sh::kOpA);
+      for (int kb = 0; kb < DP / 64; ++kb) {
+        tma_load_4d(blk.a0 + kb * Sh::kBlockA, &mk, kb * 64, k0, hk, (int)b, blk.own);
+        tma_load_4d(blk.a1 + kb * Sh::kBlockA, &mv, kb * 64, k0, hk, (int)b, blk.own);
+      }
+      for (int i = 0; i < tiles; ++i) {
+        const int s = i % Sh::kStages, h = hk * G + i / qtiles, r0 = i % qtiles * kB;
+        if (!wait(&blk.empty[s], i / Sh::kStages ^ 1)) break;
+        mbar_expect_tx(&blk.full[s], 2 * Sh::kOpB);
+        for (int kb = 0; kb < DP / 64; ++kb) {
+          tma_load_4d(blk.b0 + s * Sh::kOpB + kb * Sh::kBlockB, &mq, kb * 64, r0, h, (int)b, &blk.full[s]);
+          tma_load_4d(blk.b1 + s * Sh::kOpB + kb * Sh::kBlockB, &mdo, kb * 64, r0, h, (int)b, &blk.full[s]);
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    const int ksteps = (x.D + 15) / 16;
+    auto start = [&](int i) {
+      const int s = i % Sh::kStages;
+      if (!wait_all(&blk.full[s], i / Sh::kStages)) return false;
+      tc_fence_after();
+      if (lane == 0) blk.products(tmem, i & 1, s, ksteps);
+      __syncwarp();
+      return true;
+    };
+    bool ok = tiles > 0 && wait_all(blk.own, 0) && start(0) && (tiles < 2 || start(1));
+    for (int i = 0; i < tiles && ok; ++i) {
+      if (!(ok = wait_all(&blk.ds_full[i & 1], i >> 1))) break;
+      tc_fence_after();
+      const int s = i % Sh::kStages;
+      if (lane == 0) {
+        blk.accumulate(acc_v, tmem + (i & 1) * 128, blk.b1 + s * Sh::kOpB, x.D, i == 0);
+        blk.accumulate(acc_k, tmem + (i & 1) * 128 + 64, blk.b0 + s * Sh::kOpB, x.D, i == 0);
+        umma_commit(&blk.empty[s]);
+        if (i == tiles - 1) umma_commit(blk.done);
+      }
+      __syncwarp();
+      if (i + 2 < tiles) ok = start(i + 2);
+    }
+  } else {
+    const int w = warp >> 2, t = tid & 127;
+    const int key = k0 + t;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + w * 128;
+    const float c2 = x.scale * kLog2e;
+    const float2 cc = make_float2(c2, c2);
+    const bool allowed = key < x.Lk && key_ok(x, b, nk, key);
+    auto stat = [&](int i) {  // this thread's share of tile i's row statistics
+      const int r = i % qtiles * kB + (t & 63);
+      const int64_t at = (b * x.H + hk * G + i / qtiles) * x.Lq + r;
+      if (t < 64) return i < tiles && r < x.Lq ? -x.lse2[at] : -INFINITY;
+      return i < tiles && r < x.Lq ? -x.delta[at] : 0.0f;
+    };
+    float next = stat(w);
+    bool ok = true;
+    for (int i = w; i < tiles; i += 2) {
+      float4* st = s_stat[w][i >> 1 & 1][0];
+      reinterpret_cast<float*>(st)[t] = next;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+      next = stat(i + 2);
+      if (ok) ok = wait_all(&blk.sd_full[w], i >> 1);
+      if (!ok) continue;  // given up: the warpgroup still meets at its barrier
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float s[32], g[32];
+        tmem_ld32_nowait(tS + c * 32, s);
+        tmem_ld32_nowait(tS + 64 + c * 32, g);
+        tmem_wait_ld();
+        tmem_pin<32>(s);
+        tmem_pin<32>(g);
+        uint32_t pw[16], dw[16];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 l = st[c * 8 + q], d = st[kB / 4 + c * 8 + q];
+          float2 e0 = fma2(make_float2(s[4 * q], s[4 * q + 1]), cc, make_float2(l.x, l.y));
+          float2 e1 = fma2(make_float2(s[4 * q + 2], s[4 * q + 3]), cc, make_float2(l.z, l.w));
+          e0.x = ex2(e0.x), e0.y = ex2(e0.y), e1.x = ex2(e1.x), e1.y = ex2(e1.y);
+          const float2 d0 = add2(make_float2(g[4 * q], g[4 * q + 1]), make_float2(d.x, d.y));
+          const float2 d1 = add2(make_float2(g[4 * q + 2], g[4 * q + 3]), make_float2(d.z, d.w));
+          pw[2 * q] = pack_bf16(e0.x, e0.y), pw[2 * q + 1] = pack_bf16(e1.x, e1.y);
+          dw[2 * q] = pack_bf16(e0.x * d0.x, e0.y * d0.y), dw[2 * q + 1] = pack_bf16(e1.x * d1.x, e1.y * d1.y);
+        }
+        if (!allowed) {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) pw[q] = dw[q] = 0;
+        }
+        tmem_st16(tS + c * 16, pw);
+        tmem_st16(tS + 64 + c * 16, dw);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&blk.ds_full[w]);
+    }
+    if (ok && tiles > 0) wait_all(blk.done, 0);
+    tc_fence_after();
+    const int64_t at = ((b * x.Lk + key) * x.Hkv + hk) * (int64_t)x.D;
+    store_acc<DP>((w ? acc_k : acc_v) + lanes, static_cast<__nv_bfloat16*>(w ? x.dk : x.dv) + at, key < x.Lk,
+                  tiles == 0, 0, x.D, w ? x.scale : 1.0f);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) free_tmem(tmem);
+}
+
+// ---- host ----------------------------------------------------------------------------------
+template <int DP>
+static int launch_bwd(TcParams& t, cudaStream_t st) {
+  using Sh = BwdShape<DP>;
+  const Params& x = t.x;
+  CUtensorMap q128, q64, g128, g64, k128, k64, v128, v64;
+  if (!make_map(&q128, x.q, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&q64, x.q, x.D, x.Lq, x.H, x.B, kB) ||
+      !make_map(&g128, x.dout, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&g64, x.dout, x.D, x.Lq, x.H, x.B, kB) ||
+      !make_map(&k128, x.k, x.D, x.Lk, x.Hkv, x.B, kTile) || !make_map(&k64, x.k, x.D, x.Lk, x.Hkv, x.B, kB) ||
+      !make_map(&v128, x.v, x.D, x.Lk, x.Hkv, x.B, kTile) || !make_map(&v64, x.v, x.D, x.Lk, x.Hkv, x.B, kB))
+    return HCLSM_ERR_UNSUPPORTED;
+  t.qtiles = (x.Lq + kTile - 1) / kTile;
+  const int64_t gq = (int64_t)t.qtiles * x.H * x.B, gk = (int64_t)((x.Lk + kTile - 1) / kTile) * x.Hkv * x.B;
+  if (gq > 0x7fffffff || gk > 0x7fffffff || (int64_t)((x.Lq + kB - 1) / kB) * x.H > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  auto fq = tc_dq_kernel<DP>;
+  auto fk = tc_dkv_kernel<DP>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(fq), Sh::kBytes) ||
+      !set_smem_limit(reinterpret_cast<const void*>(fk), Sh::kBytes))
+    return HCLSM_ERR_LAUNCH;
+  if (const int rc = launch_pdl(fq, (unsigned)gq, Sh::kThreads, Sh::kBytes, st, q128, g128, k64, v64, t)) return rc;
+  return launch_pdl(fk, (unsigned)gk, Sh::kThreads, Sh::kBytes, st, k128, v128, q64, g64, t);
+}
+
+// x.delta is set; ws: tc_workspace bytes.
+int tc_bwd(const Params& p, void* ws, cudaStream_t st) {
+  TcParams t = {};
+  t.x = p;
+  if (const int rc = make_bits(t, ws, st)) return rc;
+  return p.D <= 64 ? launch_bwd<64>(t, st) : launch_bwd<128>(t, st);
+}
+
+}  // namespace xattn
+}  // namespace hclsm
