@@ -73,14 +73,43 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// A descriptor `bytes` further on.  The address field is the low 14 bits in units of 16 bytes, and all of shared
+// memory fits it, so a base descriptor is formed once and a step is one 32-bit add.
+__device__ __forceinline__ uint64_t desc_at(uint64_t base, uint32_t bytes) {
+  return (base & 0xffffffff00000000ull) | ((uint32_t)base + (bytes >> 4));
+}
+
 // ---- pieces of the attention kernels -------------------------------------------------------
-// A from TMEM (bf16 pairs, lane = row), B from shared memory.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                             uint32_t accumulate) {
+// MMA issue by a whole, converged warp with one elected lane: outside a divergent branch the descriptors stay in
+// uniform registers.  Under `if (lane == 0)` each MMA costs the issuing thread at least 52 cycles (moves into uniform
+// registers), more than a 128 x 64 x 16 product takes (35); issued this way it does not.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}\n" : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void umma_ss(uint32_t elect, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(elect)
+      : "memory");
+}
+// A from TMEM (bf16 pairs, lane = row), B from shared memory.
+__device__ __forceinline__ void umma_ts(uint32_t elect, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(elect)
+      : "memory");
+}
+__device__ __forceinline__ void umma_done(uint32_t elect, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(elect)
       : "memory");
 }
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,

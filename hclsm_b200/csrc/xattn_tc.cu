@@ -1,16 +1,18 @@
 // Cross attention in bf16 on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
 // Forward: a block takes QT tiles of 128 query rows of one head (QT 2: one block
-// an SM; QT 1: two), each with a softmax warpgroup (thread = row = TMEM lane), a
-// warp that issues TMA and a warp that issues MMA.  Per tile of 128 keys:
+// an SM; QT 1: two), each with two softmax warpgroups (thread = half a row, TMEM lane
+// = row), a warp that issues TMA and a warp that issues MMA.  Per tile of 128 keys:
 //   S = Q K^T        128 x 128, fp32 in TMEM
-//   the row's thread reads its 128 scores, takes the running maximum, writes
-//   P = exp2(c s - m) as bf16 over S in TMEM, keeps the row sum in fp32
+//   a row's two threads read 64 scores each, agree on the running maximum, write
+//   P = exp2(c s - m) as bf16 over S in TMEM, keep the row's sum in fp32
 //   O += P V         A from TMEM, V as the MN-major B operand; fp32 in TMEM
 // The maximum that O is scaled by is raised only when a row's new one exceeds it by
 // 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
-// with the same relative precision, and O is read back and rescaled rarely.
-// While one warpgroup takes its softmax the tensor cores run the other's products.
+// with the same relative precision, and O is read back and rescaled rarely.  The
+// threads of a tile meet once a tile at a barrier that says whether any row raises
+// its maximum (it also orders all reads of S before the writes of P over it).
+// While one tile takes its softmax the tensor cores run the other's products.
 #include "xattn_tc.cuh"
 
 namespace hclsm {
@@ -24,7 +26,7 @@ template <int DP, int QT> struct FwdShape {
   static constexpr int kStages = DP == 64 ? (QT == 2 ? 3 : 2) : (QT == 2 ? 2 : 1);
   static constexpr int kBars = 1 + 4 * kStages + 3 * QT;
   static constexpr size_t kBytes = (size_t)(QT + 2 * kStages) * kOp + kBars * 8 + 1024;
-  static constexpr int kThreads = QT * 128 + 64;
+  static constexpr int kThreads = QT * 256 + 64;
   static constexpr uint32_t kCols = QT == 2 ? 512 : 256;
 };
 
@@ -39,12 +41,13 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
+  __shared__ float s_row[QT][2][kTile];  // what a row's two threads tell each other
   unsigned char *sQ = smem, *sK = sQ + QT * Sh::kOp, *sV = sK + ST * Sh::kOp;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::kOp);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST,
            *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1;
+  constexpr int kTmaWarp = QT * 8, kMmaWarp = QT * 8 + 1;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(Sh::kCols)
@@ -53,7 +56,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   }
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], &bars[i] >= p_full && &bars[i] < pv_done ? 128 : 1);
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], &bars[i] >= p_full && &bars[i] < pv_done ? 256 : 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -95,22 +98,23 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
     const uint32_t id_s = idesc_bf16(kTile, kTile, false, false);
     const uint32_t id_o = idesc_bf16(kTile, (x.D + 15) / 16 * 16, false, true);
     const int ksteps = (x.D + 15) / 16;
+    const uint64_t d_q = smem_desc_sw128(smem_u32(sQ), 16, 1024), d_k = smem_desc_sw128(smem_u32(sK), 16, 1024),
+                   d_v = smem_desc_sw128(smem_u32(sV), Sh::kBlock, 1024);
+    const uint32_t one = elect_one();
     auto scores = [&](int w, int s) {
-      if (lane == 0) {
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t off = (k >> 2) * Sh::kBlock + (k & 3) * 32;
-          umma_bf16(tmem + w * 128, smem_desc_sw128(smem_u32(sQ + w * Sh::kOp) + off, 16, 1024),
-                    smem_desc_sw128(smem_u32(sK + s * Sh::kOp) + off, 16, 1024), id_s, k != 0);
-        }
-        umma_commit(&s_full[w]);
+      const uint64_t a = desc_at(d_q, w * Sh::kOp), bk = desc_at(d_k, s * Sh::kOp);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = (k >> 2) * Sh::kBlock + (k & 3) * 32;
+        if (k < ksteps) umma_ss(one, tmem + w * 128, desc_at(a, off), desc_at(bk, off), id_s, k != 0);
       }
-      __syncwarp();
+      umma_done(one, &s_full[w]);
     };
     bool ok = tiles > 0 && wait_all(q_full, 0) && wait_all(&k_full[0], 0);
     if (ok) {
       tc_fence_after();
       for (int w = 0; w < nq; ++w) scores(w, 0);
-      if (lane == 0) umma_commit(&k_empty[0]);
+      umma_done(one, &k_empty[0]);
       for (int j = 0; j < tiles && ok; ++j) {
         const int s = j % ST, s1 = (j + 1) % ST;
         const bool more = j + 1 < tiles;
@@ -120,31 +124,29 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
         for (int w = 0; w < nq && ok; ++w) {
           if (!(ok = wait_all(&p_full[w], j))) break;
           tc_fence_after();
-          if (lane == 0) {
+          const uint64_t bv = desc_at(d_v, s * Sh::kOp);
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              umma_bf16_ts(tmem + QT * 128 + w * DP, tmem + w * 128 + k * 8,
-                           smem_desc_sw128(smem_u32(sV + s * Sh::kOp) + k * 16 * kRowBytes, Sh::kBlock, 1024), id_o,
-                           (j | k) != 0);
-            umma_commit(&pv_done[w]);
-            if (w == nq - 1) umma_commit(&v_empty[s]);
-          }
-          __syncwarp();
+          for (int k = 0; k < kTile / 16; ++k)
+            umma_ts(one, tmem + QT * 128 + w * DP, tmem + w * 128 + k * 8, desc_at(bv, k * 16 * kRowBytes), id_o,
+                    (j | k) != 0);
+          umma_done(one, &pv_done[w]);
+          if (w == nq - 1) umma_done(one, &v_empty[s]);
           if (more) {
             if (w == 0 && !(ok = wait_all(&k_full[s1], (j + 1) / ST))) break;
             tc_fence_after();
             scores(w, s1);
-            if (w == nq - 1 && lane == 0) umma_commit(&k_empty[s1]);
+            if (w == nq - 1) umma_done(one, &k_empty[s1]);
           }
         }
       }
     }
-  } else if (warp < QT * 4) {
-    const int w = warp >> 2;
-    const int row = q0 + w * kTile + (tid & 127);
+  } else {
+    const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127;
+    const int row = q0 + w * kTile + r;
     const bool idle = q0 + w * kTile + (warp & 3) * 32 >= x.Lq;  // no row of this warp: it only keeps the phases
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + w * 128, tO = tmem + lanes + QT * 128 + w * DP;
+    const uint32_t tS = tmem + lanes + w * 128 + half * 64, tP = tmem + lanes + w * 128 + half * 32;
+    const uint32_t tO = tmem + lanes + QT * 128 + w * DP + half * (DP / 2);  // this thread's dims of O
     const float c2 = x.scale * kLog2e;
     float m = -INFINITY;  // the maximum O is scaled by, raw scores
     float2 l = make_float2(0.0f, 0.0f);
@@ -152,93 +154,88 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
     if (w < nq) {
       for (int j = 0; j < tiles; ++j) {
         const uint4 bits = key_bits(p, b, nk, j * kTile);
-        if (!(ok = wait_all(&s_full[w], j))) break;
+        const uint32_t word[2] = {half ? bits.z : bits.x, half ? bits.w : bits.y};
+        if (ok) ok = wait_all(&s_full[w], j);
         tc_fence_after();
-        if (idle) {
-          mbar_arrive(&p_full[w]);
-          continue;
-        }
-        // The scores are read twice, for the maximum and for the weights: a row of 128
-        // does not fit the registers beside the rest.
-        const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-        const bool all = all_bits(bits);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          float v[64];
-          tmem_ld32_nowait(tS + c * 32, v);
-          tmem_ld32_nowait(tS + c * 32 + 32, v + 32);
+        float v[64];
+        float top = -INFINITY;
+        bool raise = false;
+        if (ok && !idle) {
+          tmem_ld32_nowait(tS, v);
+          tmem_ld32_nowait(tS + 32, v + 32);
           tmem_wait_ld();
           tmem_pin<64>(v);
-          if (!all) {
+          if ((word[0] & word[1]) != 0xffffffffu) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = word[c + i / 32] >> (i & 31) & 1u ? v[i] : -INFINITY;
+            for (int i = 0; i < 64; ++i) v[i] = word[i / 32] >> (i & 31) & 1u ? v[i] : -INFINITY;
           }
+          float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int i = 0; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+          for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+          top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // the first keys of a row set its maximum; O is zero (j = 0: not yet written) till then
+          raise = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // the first keys of a row set its maximum; O is zero (j = 0: not yet written) till then
-        const bool raise = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
-        if (__any_sync(0xffffffffu, raise)) {
-          const float f = raise ? ex2((m - top) * c2) : 1.0f;  // 0 from -inf
-          if (raise) m = top;
+        if (bar_any(1 + w, raise)) {
+          s_row[w][half][r] = top;
+          bar_sync(1 + w);
+          const float both = fmaxf(top, s_row[w][half ^ 1][r]);
+          const bool up = (both - m) * c2 > kRaise;
+          const float f = up ? ex2((m - both) * c2) : 1.0f;  // 0 from -inf
+          if (up) m = both;
           l.x *= f, l.y *= f;
-          if (j > 0) {
-            if (!(ok = wait_all(&pv_done[w], j - 1))) break;
+          if (j > 0 && ok && !idle && __any_sync(0xffffffffu, up)) {
+            ok = wait_all(&pv_done[w], j - 1);
             tc_fence_after();
+            if (ok) {
 #pragma unroll
-            for (int c = 0; c < DP; c += 16) {
-              float o[16];
-              tmem_ld16_nowait(tO + c, o);
-              tmem_wait_ld();
-              tmem_pin<16>(o);
-              uint32_t r[16];
+              for (int c = 0; c < DP / 2; c += 16) {
+                float o[16];
+                tmem_ld16_nowait(tO + c, o);
+                tmem_wait_ld();
+                tmem_pin<16>(o);
+                uint32_t q[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(o[i] * f);
-              tmem_st16(tO + c, r);
+                for (int i = 0; i < 16; ++i) q[i] = __float_as_uint(o[i] * f);
+                tmem_st16(tO + c, q);
+              }
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : -m * c2;
-        const float2 cc = make_float2(c2, c2), bb = make_float2(base, base);
-        float v[2][32];
-        tmem_ld32_nowait(tS, v[0]);
+        if (ok && !idle) {
+          const float base = m == -INFINITY ? 0.0f : -m * c2;
+          const float2 cc = make_float2(c2, c2), bb = make_float2(base, base);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_ld();
-          tmem_pin<32>(v[c & 1]);
-          if (c < 3) tmem_ld32_nowait(tS + c * 32 + 32, v[(c + 1) & 1]);
-          float* u = v[c & 1];
-          if (!all) {
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pw[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = word[c] >> i & 1u ? u[i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) {
+              float2 e = fma2(make_float2(v[c * 32 + 2 * i], v[c * 32 + 2 * i + 1]), cc, bb);
+              e.x = ex2(e.x), e.y = ex2(e.y);
+              l = add2(l, e);
+              pw[i] = pack_bf16(e.x, e.y);
+            }
+            tmem_st16(tP + c * 16, pw);
           }
-          uint32_t pw[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(u[2 * i], u[2 * i + 1]), cc, bb);
-            e.x = ex2(e.x), e.y = ex2(e.y);
-            l = add2(l, e);
-            pw[i] = pack_bf16(e.x, e.y);
-          }
-          // over scores that have been read: columns [16 c, + 16) of [32 c, ...)
-          tmem_st16(tS + c * 16, pw);
+          tmem_wait_st();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&p_full[w]);
+        if (ok) {
+          tc_fence_before();
+          mbar_arrive(&p_full[w]);
+        }
       }
       if (ok && tiles > 0) ok = wait_all(&pv_done[w], tiles - 1);
       tc_fence_after();
+      s_row[w][half][r] = l.x + l.y;
+      bar_sync(1 + w);
       if (!idle) {
-        const float sum = l.x + l.y;
+        const float sum = s_row[w][0][r] + s_row[w][1][r];
         const float inv = tiles > 0 && sum != 0.0f ? 1.0f / sum : 0.0f;
-        if (row < x.Lq && x.lse2)
+        if (row < x.Lq && x.lse2 && half == 0)
           x.lse2[(b * x.H + h) * x.Lq + row] = sum == 0.0f ? INFINITY : m * c2 + log2f(sum);
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(x.o) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D;
 #pragma unroll
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = 0; c < DP / 2; c += 32) {
           float o[32];
           if (tiles > 0) {
             tmem_ld32_nowait(tO + c, o);
@@ -248,12 +245,12 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
           if (row < x.Lq) {
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
-              if (c + i < x.D) {
-                uint32_t r[4];
+              if (half * (DP / 2) + c + i < x.D) {
+                uint32_t q[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)  // a row without keys: zero, whatever O holds
-                  r[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
-                *reinterpret_cast<uint4*>(out + c + i) = make_uint4(r[0], r[1], r[2], r[3]);
+                  q[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
+                *reinterpret_cast<uint4*>(out + half * (DP / 2) + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
               }
           }
         }

@@ -12,8 +12,8 @@
 //
 // The weights and their gradients are A operands in TMEM; the same staged tile of
 // K (or Q, dO) is the K-major operand of one product and the MN-major operand of
-// another.  Two buffers of 64 + 64 columns: two warpgroups take alternate tiles, so
-// the tensor cores form one buffer's products while the other's weights are
+// another.  Two buffers of 64 + 64 columns, two warpgroups (thread = half a row) to
+// each: the tensor cores form one buffer's products while the other's weights are
 // computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
 // (128 or 256) do not fit TMEM's 512.
 #include "xattn_tc.cuh"
@@ -29,7 +29,7 @@ template <int DP> struct BwdShape {
   static constexpr int kStages = 4;
   static constexpr int kBars = 1 + 2 * kStages + 4 + 1;
   static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
-  static constexpr int kThreads = 2 * 128 + 64;
+  static constexpr int kThreads = 4 * 128 + 64;
 };
 
 // Shared by the two kernels: block layout, barriers, roles.
@@ -45,28 +45,47 @@ template <int DP> struct Block {
     done = ds_full + 2;
   }
   __device__ __forceinline__ void init() const {
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 128 : 1);
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 256 : 1);
     fence_mbar_init();
   }
-  // buffer w's two products of the streamed tile in stage s (one thread)
-  __device__ __forceinline__ void products(uint32_t tmem, int w, int s, int ksteps) const {
-    const uint32_t id = idesc_bf16(kTile, kB, false, false);
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-      for (int k = 0; k < ksteps; ++k) {
-        const uint32_t ka = (k >> 2) * Sh::kBlockA + (k & 3) * 32, kb = (k >> 2) * Sh::kBlockB + (k & 3) * 32;
-        umma_bf16(tmem + w * 128 + half * 64, smem_desc_sw128(smem_u32(half ? a1 : a0) + ka, 16, 1024),
-                  smem_desc_sw128(smem_u32((half ? b1 : b0) + s * Sh::kOpB) + kb, 16, 1024), id, k != 0);
-      }
-    umma_commit(&sd_full[w]);
+  // What the issuing thread computes once.
+  struct Issue {
+    uint64_t a0, a1, b0, b1, t0, t1;  // the operands K-major; the streamed two MN-major
+    uint32_t id_s, id_o, one;
+    int ksteps;
+  };
+  __device__ __forceinline__ Issue issue(int D) const {
+    Issue r;
+    r.one = elect_one();
+    r.a0 = smem_desc_sw128(smem_u32(a0), 16, 1024), r.a1 = smem_desc_sw128(smem_u32(a1), 16, 1024);
+    r.b0 = smem_desc_sw128(smem_u32(b0), 16, 1024), r.b1 = smem_desc_sw128(smem_u32(b1), 16, 1024);
+    r.t0 = smem_desc_sw128(smem_u32(b0), Sh::kBlockB, 1024), r.t1 = smem_desc_sw128(smem_u32(b1), Sh::kBlockB, 1024);
+    r.id_s = idesc_bf16(kTile, kB, false, false);
+    r.id_o = idesc_bf16(kTile, (D + 15) / 16 * 16, false, true);
+    r.ksteps = (D + 15) / 16;
+    return r;
   }
-  // acc += (bf16 columns at a) x (streamed tile at b, as the MN-major operand) (one thread)
-  __device__ __forceinline__ void accumulate(uint32_t acc, uint32_t a, const unsigned char* b, int D, bool first) const {
-    const uint32_t id = idesc_bf16(kTile, (D + 15) / 16 * 16, false, true);
+  // buffer w's two products of the streamed tile in stage s (a converged warp)
+  __device__ __forceinline__ void products(const Issue& r, uint32_t tmem, int w, int s) const {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint64_t b = desc_at(half ? r.b1 : r.b0, s * Sh::kOpB);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t ka = (k >> 2) * Sh::kBlockA + (k & 3) * 32, kb = (k >> 2) * Sh::kBlockB + (k & 3) * 32;
+        if (k < r.ksteps)
+          umma_ss(r.one, tmem + w * 128 + half * 64, desc_at(half ? r.a1 : r.a0, ka), desc_at(b, kb), r.id_s, k != 0);
+      }
+    }
+    umma_done(r.one, &sd_full[w]);
+  }
+  // acc += (bf16 columns at a) x (streamed tile in stage s, MN-major descriptor t) (a converged warp)
+  __device__ __forceinline__ void accumulate(const Issue& r, uint32_t acc, uint32_t a, uint64_t t, int s,
+                                             bool first) const {
+    const uint64_t b = desc_at(t, s * Sh::kOpB);
 #pragma unroll
     for (int k = 0; k < kB / 16; ++k)
-      umma_bf16_ts(acc, a + k * 8, smem_desc_sw128(smem_u32(b) + k * 16 * kRowBytes, Sh::kBlockB, 1024), id,
-                   !(first && k == 0));
+      umma_ts(r.one, acc, a + k * 8, desc_at(b, k * 16 * kRowBytes), r.id_o, !(first && k == 0));
   }
 };
 
@@ -82,16 +101,16 @@ __device__ __forceinline__ void free_tmem(uint32_t tmem) {
 template <int N>
 __device__ __forceinline__ void store_acc(uint32_t t, __nv_bfloat16* out, bool ok, bool zero, int c0, int D, float f) {
 #pragma unroll
-  for (int c = 0; c < N; c += 32) {
-    float o[32];
+  for (int c = 0; c < N; c += 16) {
+    float o[16];
     if (!zero) {
-      tmem_ld32_nowait(t + c0 + c, o);
+      tmem_ld16_nowait(t + c0 + c, o);
       tmem_wait_ld();
-      tmem_pin<32>(o);
+      tmem_pin<16>(o);
     }
     if (!ok) continue;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
+    for (int i = 0; i < 16; i += 8)
       if (c0 + c + i < D) {
         uint32_t r[4];
 #pragma unroll
@@ -112,7 +131,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   __shared__ volatile int s_abort;
   const Block<DP> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  constexpr int kTmaWarp = 16, kMmaWarp = 17;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
@@ -151,7 +170,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    const int ksteps = (x.D + 15) / 16;
+    const auto is = blk.issue(x.D);
     auto start = [&](int j) {  // the products of tile j into buffer j & 1
       const int s = j % Sh::kStages;
       if (!wait_all(&blk.full[s], j / Sh::kStages)) return false;
@@ -159,8 +178,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       const uint4 mine = j & 1 ? make_uint4(bits.z, bits.w, ~0u, ~0u) : make_uint4(bits.x, bits.y, ~0u, ~0u);
       if (!all_bits(mine)) zero_rows<DP, kB>(blk.b0 + s * Sh::kOpB, mine, lane);  // dS 0 times K
       tc_fence_after();
-      if (lane == 0) blk.products(tmem, j & 1, s, ksteps);
-      __syncwarp();
+      blk.products(is, tmem, j & 1, s);
       return true;
     };
     bool ok = tiles > 0 && wait_all(blk.own, 0) && start(0) && (tiles < 2 || start(1));
@@ -168,16 +186,13 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (!(ok = wait_all(&blk.ds_full[j & 1], j >> 1))) break;
       tc_fence_after();
       const int s = j % Sh::kStages;
-      if (lane == 0) {
-        blk.accumulate(acc, tmem + (j & 1) * 128, blk.b0 + s * Sh::kOpB, x.D, j == 0);
-        umma_commit(&blk.empty[s]);
-        if (j == tiles - 1) umma_commit(blk.done);
-      }
-      __syncwarp();
+      blk.accumulate(is, acc, tmem + (j & 1) * 128, is.t0, s, j == 0);
+      umma_done(is.one, &blk.empty[s]);
+      if (j == tiles - 1) umma_done(is.one, blk.done);
       if (j + 2 < tiles) ok = start(j + 2);
     }
   } else {
-    const int w = warp >> 2;
+    const int w = warp >> 3, half = warp >> 2 & 1;
     const int row = q0 + (tid & 127);
     const bool idle = q0 + (warp & 3) * 32 >= x.Lq;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -189,34 +204,35 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     bool ok = true;
     for (int j = w; j < tiles; j += 2) {
       const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
-      const uint32_t word[2] = {j & 1 ? bits.z : bits.x, j & 1 ? bits.w : bits.y};
-      if (!(ok = wait_all(&blk.sd_full[w], j >> 1))) break;
+      const uint32_t word = j & 1 ? (half ? bits.w : bits.z) : (half ? bits.y : bits.x);
+      if (ok) ok = wait_all(&blk.sd_full[w], j >> 1);
       tc_fence_after();
+      float s[32], g[32];
+      if (ok && !idle) {
+        tmem_ld32_nowait(tS + half * 32, s);
+        tmem_ld32_nowait(tS + 64 + half * 32, g);
+        tmem_wait_ld();
+        tmem_pin<32>(s);
+        tmem_pin<32>(g);
+      }
+      bar_sync(1 + w);  // both halves' scores are read before weights go over them
+      if (!ok) continue;
       if (!idle) {
+        uint32_t r[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float s[32], g[32];
-          tmem_ld32_nowait(tS + c * 32, s);
-          tmem_ld32_nowait(tS + 64 + c * 32, g);
-          tmem_wait_ld();
-          tmem_pin<32>(s);
-          tmem_pin<32>(g);
-          uint32_t r[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
-            e.x = ex2(e.x), e.y = ex2(e.y);
-            const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
-            s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
-          }
-          if (word[c] != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = word[c] >> i & 1u ? s[i] : 0.0f;
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
-          tmem_st16(tS + c * 16, r);
+        for (int i = 0; i < 16; ++i) {
+          float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
+          e.x = ex2(e.x), e.y = ex2(e.y);
+          const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
+          s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
         }
+        if (word != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = word >> i & 1u ? s[i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
+        tmem_st16(tS + half * 16, r);
         tmem_wait_st();
       }
       tc_fence_before();
@@ -225,8 +241,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     if (ok && tiles > 0) wait_all(blk.done, 0);
     tc_fence_after();
     if (!idle)
-      store_acc<DP / 2>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
-                        row < x.Lq, tiles == 0, w * (DP / 2), x.D, x.scale);
+      store_acc<DP / 4>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
+                        row < x.Lq, tiles == 0, (2 * w + half) * (DP / 4), x.D, x.scale);
   }
   tc_fence_before();
   __syncthreads();
@@ -246,7 +262,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   __shared__ float4 s_stat[2][2][2][kB / 4];  // warpgroup, slot, (-lse2, -delta)
   const Block<DP> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  constexpr int kTmaWarp = 16, kMmaWarp = 17;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
@@ -287,13 +303,12 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       }
     }
   } else if (warp == kMmaWarp) {
-    const int ksteps = (x.D + 15) / 16;
+    const auto is = blk.issue(x.D);
     auto start = [&](int i) {
       const int s = i % Sh::kStages;
       if (!wait_all(&blk.full[s], i / Sh::kStages)) return false;
       tc_fence_after();
-      if (lane == 0) blk.products(tmem, i & 1, s, ksteps);
-      __syncwarp();
+      blk.products(is, tmem, i & 1, s);
       return true;
     };
     bool ok = tiles > 0 && wait_all(blk.own, 0) && start(0) && (tiles < 2 || start(1));
@@ -301,17 +316,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (!(ok = wait_all(&blk.ds_full[i & 1], i >> 1))) break;
       tc_fence_after();
       const int s = i % Sh::kStages;
-      if (lane == 0) {
-        blk.accumulate(acc_v, tmem + (i & 1) * 128, blk.b1 + s * Sh::kOpB, x.D, i == 0);
-        blk.accumulate(acc_k, tmem + (i & 1) * 128 + 64, blk.b0 + s * Sh::kOpB, x.D, i == 0);
-        umma_commit(&blk.empty[s]);
-        if (i == tiles - 1) umma_commit(blk.done);
-      }
-      __syncwarp();
+      blk.accumulate(is, acc_v, tmem + (i & 1) * 128, is.t1, s, i == 0);
+      blk.accumulate(is, acc_k, tmem + (i & 1) * 128 + 64, is.t0, s, i == 0);
+      umma_done(is.one, &blk.empty[s]);
+      if (i == tiles - 1) umma_done(is.one, blk.done);
       if (i + 2 < tiles) ok = start(i + 2);
     }
   } else {
-    const int w = warp >> 2, t = tid & 127;
+    const int w = warp >> 3, half = warp >> 2 & 1, t = tid & 127;
     const int key = k0 + t;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128;
@@ -324,28 +336,32 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (t < 64) return i < tiles && r < x.Lq ? -x.lse2[at] : -INFINITY;
       return i < tiles && r < x.Lq ? -x.delta[at] : 0.0f;
     };
-    float next = stat(w);
+    float next = half ? 0.0f : stat(w);
     bool ok = true;
     for (int i = w; i < tiles; i += 2) {
       float4* st = s_stat[w][i >> 1 & 1][0];
-      reinterpret_cast<float*>(st)[t] = next;
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
-      next = stat(i + 2);
+      if (half == 0) {
+        reinterpret_cast<float*>(st)[t] = next;
+        next = stat(i + 2);
+      }
       if (ok) ok = wait_all(&blk.sd_full[w], i >> 1);
-      if (!ok) continue;  // given up: the warpgroup still meets at its barrier
       tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float s[32], g[32];
-        tmem_ld32_nowait(tS + c * 32, s);
-        tmem_ld32_nowait(tS + 64 + c * 32, g);
+      float s[32], g[32];
+      if (ok) {
+        tmem_ld32_nowait(tS + half * 32, s);
+        tmem_ld32_nowait(tS + 64 + half * 32, g);
         tmem_wait_ld();
         tmem_pin<32>(s);
         tmem_pin<32>(g);
+      }
+      // the statistics are there, and both halves' scores are read before weights go over them
+      bar_sync(1 + w);
+      if (!ok) continue;  // given up: the others still meet at the barrier
+      {
         uint32_t pw[16], dw[16];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float4 l = st[c * 8 + q], d = st[kB / 4 + c * 8 + q];
+          const float4 l = st[half * 8 + q], d = st[kB / 4 + half * 8 + q];
           float2 e0 = fma2(make_float2(s[4 * q], s[4 * q + 1]), cc, make_float2(l.x, l.y));
           float2 e1 = fma2(make_float2(s[4 * q + 2], s[4 * q + 3]), cc, make_float2(l.z, l.w));
           e0.x = ex2(e0.x), e0.y = ex2(e0.y), e1.x = ex2(e1.x), e1.y = ex2(e1.y);
@@ -358,8 +374,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
 #pragma unroll
           for (int q = 0; q < 16; ++q) pw[q] = dw[q] = 0;
         }
-        tmem_st16(tS + c * 16, pw);
-        tmem_st16(tS + 64 + c * 16, dw);
+        tmem_st16(tS + half * 16, pw);
+        tmem_st16(tS + 64 + half * 16, dw);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -368,8 +384,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     if (ok && tiles > 0) wait_all(blk.done, 0);
     tc_fence_after();
     const int64_t at = ((b * x.Lk + key) * x.Hkv + hk) * (int64_t)x.D;
-    store_acc<DP>((w ? acc_k : acc_v) + lanes, static_cast<__nv_bfloat16*>(w ? x.dk : x.dv) + at, key < x.Lk,
-                  tiles == 0, 0, x.D, w ? x.scale : 1.0f);
+    store_acc<DP / 2>((w ? acc_k : acc_v) + lanes, static_cast<__nv_bfloat16*>(w ? x.dk : x.dv) + at, key < x.Lk,
+                      tiles == 0, half * (DP / 2), x.D, w ? x.scale : 1.0f);
   }
   tc_fence_before();
   __syncthreads();
