@@ -1,18 +1,18 @@
 // Cross attention in bf16 on the 5th-generation tensor cores (tcgen05, TMEM, TMA).
 //
 // Forward: a block takes QT tiles of 128 query rows of one head (QT 2: one block
-// an SM; QT 1: two), each with two softmax warpgroups (thread = half a row, TMEM lane
-// = row), a warp that issues TMA and a warp that issues MMA.  Per tile of 128 keys:
+// an SM; QT 1: two), each with a softmax warpgroup (thread = row = TMEM lane), a warp
+// that issues TMA and one or two that issue MMA.  Per tile of 128 keys:
 //   S = Q K^T        128 x 128, fp32 in TMEM
-//   a row's two threads read 64 scores each, agree on the running maximum, write
-//   P = exp2(c s - m) as bf16 over S in TMEM, keep the row's sum in fp32
+//   the row's thread reads its scores, takes the running maximum, writes
+//   P = exp2(c s - m) as bf16 to TMEM, keeps the row's sum in fp32
 //   O += P V         A from TMEM, V as the MN-major B operand; fp32 in TMEM
 // The maximum that O is scaled by is raised only when a row's new one exceeds it by
 // 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
-// with the same relative precision, and O is read back and rescaled rarely.  The
-// threads of a tile meet once a tile at a barrier that says whether any row raises
-// its maximum (it also orders all reads of S before the writes of P over it).
+// with the same relative precision, and O is read back and rescaled rarely.
 // While one tile takes its softmax the tensor cores run the other's products.
+#include <type_traits>
+
 #include "xattn_tc.cuh"
 
 namespace hclsm {
@@ -24,9 +24,15 @@ template <int DP, int QT> struct FwdShape {
   static constexpr int kBlock = kTile * kRowBytes;        // 64 dims of a tile
   static constexpr int kOp = DP / 64 * kBlock;            // a staged tile
   static constexpr int kStages = DP == 64 ? (QT == 2 ? 3 : 2) : (QT == 2 ? 2 : 1);
-  static constexpr int kBars = 1 + 4 * kStages + 3 * QT;
+  // D <= 64 leaves TMEM columns for the weights beside the scores: then the next tile's
+  // scores are formed as soon as this tile's have been read, and the softmax threads
+  // never wait for a product.  D > 64: the weights go over the scores.
+  static constexpr bool kApart = DP == 64;
+  static constexpr int kBars = 1 + 4 * kStages + 4 * QT;
+  static constexpr int kColP = kApart ? QT * 128 : 0, kColO = QT * (kApart ? 192 : 128);
+  static constexpr int kStepP = kApart ? 64 : 128;  // columns from one tile's weights to the next's
   static constexpr size_t kBytes = (size_t)(QT + 2 * kStages) * kOp + kBars * 8 + 1024;
-  static constexpr int kThreads = QT * 256 + 64;
+  static constexpr int kThreads = QT * 128 + 96;
   static constexpr uint32_t kCols = QT == 2 ? 512 : 256;
 };
 
@@ -41,13 +47,12 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ float s_row[QT][2][kTile];  // what a row's two threads tell each other
   unsigned char *sQ = smem, *sK = sQ + QT * Sh::kOp, *sV = sK + ST * Sh::kOp;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::kOp);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST,
-           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT;
+           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT, *s_free = pv_done + QT;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = QT * 8, kMmaWarp = QT * 8 + 1;
+  constexpr int kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1, kWeighWarp = QT * 4 + 2;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(Sh::kCols)
@@ -56,7 +61,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   }
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], &bars[i] >= p_full && &bars[i] < pv_done ? 256 : 1);
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], (&bars[i] >= p_full && &bars[i] < pv_done) || &bars[i] >= s_free ? 128 : 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -64,7 +69,8 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   tc_fence_after();
   pdl_wait();
   pdl_trigger();
-  const uint32_t tmem = s_tmem;  // tile w: scores and weights in columns [w * 128, + 128), O in [QT * 128 + w * DP, + DP)
+  // tile w: scores in columns [w * 128, + 128), weights in [kColP + w * kStepP, + 64), O in [kColO + w * DP, + DP)
+  const uint32_t tmem = s_tmem;
   const Params& x = p.x;
   const int q0 = (int)(blockIdx.x % p.qtiles) * (QT * kTile);
   const int h = (int)(blockIdx.x / p.qtiles % x.H), hk = h / (x.H / x.Hkv);
@@ -94,7 +100,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
           tma_load_4d(sV + s * Sh::kOp + kb * Sh::kBlock, &mv, kb * 64, j * kTile, hk, (int)b, &v_full[s]);
       }
     }
-  } else if (warp == kMmaWarp) {
+  } else if (warp == kMmaWarp || warp == kWeighWarp) {
     const uint32_t id_s = idesc_bf16(kTile, kTile, false, false);
     const uint32_t id_o = idesc_bf16(kTile, (x.D + 15) / 16 * 16, false, true);
     const int ksteps = (x.D + 15) / 16;
@@ -110,28 +116,62 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       }
       umma_done(one, &s_full[w]);
     };
-    bool ok = tiles > 0 && wait_all(q_full, 0) && wait_all(&k_full[0], 0);
-    if (ok) {
-      tc_fence_after();
-      for (int w = 0; w < nq; ++w) scores(w, 0);
-      umma_done(one, &k_empty[0]);
+    auto weigh = [&](int w, int j) {  // O of tile w += its weights of keys j times V
+      const uint64_t bv = desc_at(d_v, j % ST * Sh::kOp);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        umma_ts(one, tmem + Sh::kColO + w * DP, tmem + Sh::kColP + w * Sh::kStepP + k * 8,
+                desc_at(bv, k * 16 * kRowBytes), id_o, (j | k) != 0);
+      umma_done(one, &pv_done[w]);
+      if (w == nq - 1) umma_done(one, &v_empty[j % ST]);
+    };
+    auto values = [&](int j) {  // V of keys j is there, and zero where it is not allowed
+      if (!wait_all(&v_full[j % ST], j / ST)) return false;
+      const uint4 bits = key_bits(p, b, nk, j * kTile);
+      if (!all_bits(bits)) zero_rows<DP, kTile>(sV + j % ST * Sh::kOp, bits, lane);
+      return true;
+    };
+    bool ok = tiles > 0;
+    if constexpr (Sh::kApart) {
+      // Scores and weighted sums wait for different threads: a warp issues each, so that
+      // neither waits behind the other.
+      if (warp == kMmaWarp) {
+        ok = ok && wait_all(q_full, 0);
+        for (int j = 0; j < tiles && ok; ++j) {
+          const int s = j % ST;
+          if (!(ok = wait_all(&k_full[s], j / ST))) break;
+          for (int w = 0; w < nq && ok; ++w) {
+            if (j > 0 && !(ok = wait_all(&s_free[w], j - 1))) break;
+            tc_fence_after();
+            scores(w, s);
+          }
+          if (ok) umma_done(one, &k_empty[s]);
+        }
+      } else {
+        for (int j = 0; j < tiles && ok; ++j) {
+          if (!(ok = values(j))) break;
+          for (int w = 0; w < nq && ok; ++w) {
+            if (!(ok = wait_all(&p_full[w], j))) break;
+            tc_fence_after();
+            weigh(w, j);
+          }
+        }
+      }
+    } else if (warp == kMmaWarp) {
+      ok = ok && wait_all(q_full, 0) && wait_all(&k_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        for (int w = 0; w < nq; ++w) scores(w, 0);
+        umma_done(one, &k_empty[0]);
+      }
       for (int j = 0; j < tiles && ok; ++j) {
-        const int s = j % ST, s1 = (j + 1) % ST;
-        const bool more = j + 1 < tiles;
-        if (!(ok = wait_all(&v_full[s], j / ST))) break;
-        const uint4 bits = key_bits(p, b, nk, j * kTile);
-        if (!all_bits(bits)) zero_rows<DP, kTile>(sV + s * Sh::kOp, bits, lane);
+        const int s1 = (j + 1) % ST;
+        if (!(ok = values(j))) break;
         for (int w = 0; w < nq && ok; ++w) {
           if (!(ok = wait_all(&p_full[w], j))) break;
           tc_fence_after();
-          const uint64_t bv = desc_at(d_v, s * Sh::kOp);
-#pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            umma_ts(one, tmem + QT * 128 + w * DP, tmem + w * 128 + k * 8, desc_at(bv, k * 16 * kRowBytes), id_o,
-                    (j | k) != 0);
-          umma_done(one, &pv_done[w]);
-          if (w == nq - 1) umma_done(one, &v_empty[s]);
-          if (more) {
+          weigh(w, j);
+          if (j + 1 < tiles) {
             if (w == 0 && !(ok = wait_all(&k_full[s1], (j + 1) / ST))) break;
             tc_fence_after();
             scores(w, s1);
@@ -141,118 +181,176 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       }
     }
   } else {
-    const int w = warp >> 3, half = warp >> 2 & 1, r = tid & 127;
-    const int row = q0 + w * kTile + r;
+    const int w = warp >> 2;
+    const int row = q0 + w * kTile + (tid & 127);
     const bool idle = q0 + w * kTile + (warp & 3) * 32 >= x.Lq;  // no row of this warp: it only keeps the phases
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes + w * 128 + half * 64, tP = tmem + lanes + w * 128 + half * 32;
-    const uint32_t tO = tmem + lanes + QT * 128 + w * DP + half * (DP / 2);  // this thread's dims of O
+    const uint32_t tS = tmem + lanes + w * 128, tP = tmem + lanes + Sh::kColP + w * Sh::kStepP,
+                   tO = tmem + lanes + Sh::kColO + w * DP;
     const float c2 = x.scale * kLog2e;
     float m = -INFINITY;  // the maximum O is scaled by, raw scores
     float2 l = make_float2(0.0f, 0.0f);
-    bool ok = true;
-    if (w < nq) {
-      for (int j = 0; j < tiles; ++j) {
-        const uint4 bits = key_bits(p, b, nk, j * kTile);
-        const uint32_t word[2] = {half ? bits.z : bits.x, half ? bits.w : bits.y};
-        if (ok) ok = wait_all(&s_full[w], j);
-        tc_fence_after();
-        float v[64];
-        float top = -INFINITY;
-        bool raise = false;
-        if (ok && !idle) {
-          tmem_ld32_nowait(tS, v);
-          tmem_ld32_nowait(tS + 32, v + 32);
-          tmem_wait_ld();
-          tmem_pin<64>(v);
-          if ((word[0] & word[1]) != 0xffffffffu) {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = word[i / 32] >> (i & 31) & 1u ? v[i] : -INFINITY;
-          }
-          float mx[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-          for (int i = 4; i < 64; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
-          top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          // the first keys of a row set its maximum; O is zero (j = 0: not yet written) till then
-          raise = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
-        }
-        if (bar_any(1 + w, raise)) {
-          s_row[w][half][r] = top;
-          bar_sync(1 + w);
-          const float both = fmaxf(top, s_row[w][half ^ 1][r]);
-          const bool up = (both - m) * c2 > kRaise;
-          const float f = up ? ex2((m - both) * c2) : 1.0f;  // 0 from -inf
-          if (up) m = both;
-          l.x *= f, l.y *= f;
-          if (j > 0 && ok && !idle && __any_sync(0xffffffffu, up)) {
-            ok = wait_all(&pv_done[w], j - 1);
-            tc_fence_after();
-            if (ok) {
-#pragma unroll
-              for (int c = 0; c < DP / 2; c += 16) {
-                float o[16];
-                tmem_ld16_nowait(tO + c, o);
-                tmem_wait_ld();
-                tmem_pin<16>(o);
-                uint32_t q[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) q[i] = __float_as_uint(o[i] * f);
-                tmem_st16(tO + c, q);
-              }
-            }
-          }
-        }
-        if (ok && !idle) {
-          const float base = m == -INFINITY ? 0.0f : -m * c2;
-          const float2 cc = make_float2(c2, c2), bb = make_float2(base, base);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pw[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float2 e = fma2(make_float2(v[c * 32 + 2 * i], v[c * 32 + 2 * i + 1]), cc, bb);
-              e.x = ex2(e.x), e.y = ex2(e.y);
-              l = add2(l, e);
-              pw[i] = pack_bf16(e.x, e.y);
-            }
-            tmem_st16(tP + c * 16, pw);
-          }
-          tmem_wait_st();
-        }
-        if (ok) {
-          tc_fence_before();
-          mbar_arrive(&p_full[w]);
-        }
-      }
-      if (ok && tiles > 0) ok = wait_all(&pv_done[w], tiles - 1);
+    bool ok = w < nq;
+    for (int j = 0; j < tiles && ok; ++j) {
+      const uint4 bits = key_bits(p, b, nk, j * kTile);
+      const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
+      const bool all = all_bits(bits);
+      if (!(ok = wait_all(&s_full[w], j))) break;
       tc_fence_after();
-      s_row[w][half][r] = l.x + l.y;
-      bar_sync(1 + w);
-      if (!idle) {
-        const float sum = s_row[w][0][r] + s_row[w][1][r];
-        const float inv = tiles > 0 && sum != 0.0f ? 1.0f / sum : 0.0f;
-        if (row < x.Lq && x.lse2 && half == 0)
-          x.lse2[(b * x.H + h) * x.Lq + row] = sum == 0.0f ? INFINITY : m * c2 + log2f(sum);
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(x.o) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D;
+      if (idle) {
+        if constexpr (Sh::kApart) mbar_arrive(&s_free[w]);
+        mbar_arrive(&p_full[w]);
+        continue;
+      }
+      auto highest = [&](float (&mx)[4], const float (&v)[32]) {
 #pragma unroll
-        for (int c = 0; c < DP / 2; c += 32) {
-          float o[32];
-          if (tiles > 0) {
-            tmem_ld32_nowait(tO + c, o);
+        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], v[i + q], v[i + q + 4]);
+      };
+      // a row's maximum is now `top`: O, kept by the old one, is scaled to it where it is too low
+      auto raise = [&](float top) {
+        const bool up = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
+        if (!__any_sync(0xffffffffu, up)) return false;
+        const float f = up ? ex2((m - top) * c2) : 1.0f;  // 0 from -inf: O is zero, or (j = 0) not yet written
+        if (up) m = top;
+        l.x *= f, l.y *= f;
+        if (j > 0) {
+          ok = wait_all(&pv_done[w], j - 1);
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP && ok; c += 16) {
+            float o[16];
+            tmem_ld16_nowait(tO + c, o);
             tmem_wait_ld();
-            tmem_pin<32>(o);
-          }
-          if (row < x.Lq) {
+            tmem_pin<16>(o);
+            uint32_t q[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              if (half * (DP / 2) + c + i < x.D) {
-                uint32_t q[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)  // a row without keys: zero, whatever O holds
-                  q[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
-                *reinterpret_cast<uint4*>(out + half * (DP / 2) + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
-              }
+            for (int i = 0; i < 16; ++i) q[i] = __float_as_uint(o[i] * f);
+            tmem_st16(tO + c, q);
           }
+        }
+        return true;
+      };
+      // 32 scores to weights; three pairs in eight on the FMA pipe, because the MUFU's 16 a clock
+      // would be the bound (measured for a 128 x 128 tile of two warpgroups: 1196 clocks with
+      // none there, 1071 with two in eight, 1003 with three, 1061 with four)
+      auto weights = [&](const float (&v)[32], uint32_t* pw, float2& sum) {
+        const float base = m == -INFINITY ? 0.0f : -m * c2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float2 e = fma2(make_float2(v[2 * i], v[2 * i + 1]), make_float2(c2, c2), make_float2(base, base));
+          if (0xa8 >> (i & 7) & 1) e = ex2_fma(e);
+          else e.x = ex2(e.x), e.y = ex2(e.y);
+          sum = add2(sum, e);
+          pw[i] = pack_bf16(e.x, e.y);
+        }
+      };
+      // The whole tile without a branch on the mask inside, so that the chunks' instructions interleave.
+      auto tile = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+        // fn(chunk, its 32 scores), each chunk's load in flight during the one before
+        auto chunks = [&](auto fn) {
+          float v[2][32];
+          tmem_ld32_nowait(tS, v[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_wait_ld();
+            tmem_pin<32>(v[c & 1]);
+            if (c < 3) tmem_ld32_nowait(tS + (c + 1) * 32, v[(c + 1) & 1]);
+            if constexpr (MASKED) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[c & 1][i] = word[c] >> i & 1u ? v[c & 1][i] : -INFINITY;
+            }
+            fn(c, v[c & 1]);
+          }
+        };
+        if constexpr (Sh::kApart) {
+          // The maximum first, then the weights, so that the scores are free for the next tile's
+          // while their last quarter is still being weighed.
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          chunks([&](int, const float (&v)[32]) { highest(mx, v); });
+          raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]));
+          if (ok && j > 0) ok = wait_all(&pv_done[w], j - 1);  // the last weights have been used
+          tc_fence_after();
+          if (!ok) return;
+          float2 sum = make_float2(0.0f, 0.0f);
+          chunks([&](int c, const float (&v)[32]) {
+            if (c == 3) {
+              tc_fence_before();
+              mbar_arrive(&s_free[w]);
+            }
+            uint32_t pw[16];
+            weights(v, pw, sum);
+            tmem_st16(tP + c * 16, pw);
+          });
+          l = add2(l, sum);
+        } else {
+          // The weights by the maximum as it stands, kept in registers, and again where it has
+          // to be raised: the scores' maximum is off the chain that the products wait for.
+          // (A masked tile takes its maximum first: its code would not fit the registers.)
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float2 sum = make_float2(0.0f, 0.0f);
+          auto over = [&](int c, const float (&v)[32]) {  // over scores that have been read
+            uint32_t pw[16];
+            weights(v, pw, sum);
+            tmem_st16(tP + c * 16, pw);
+          };
+          if constexpr (MASKED) {
+            chunks([&](int, const float (&v)[32]) { highest(mx, v); });
+            raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]));
+            if (!ok) return;
+            chunks(over);
+          } else {
+            uint32_t pw[64];
+            chunks([&](int c, const float (&v)[32]) {
+              highest(mx, v);
+              weights(v, pw + c * 16, sum);
+            });
+            if (raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]))) {
+              if (!ok) return;
+              sum = make_float2(0.0f, 0.0f);
+              chunks(over);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) tmem_st16(tP + c * 16, pw + c * 16);
+            }
+          }
+          l = add2(l, sum);
+        }
+      };
+      if (all) tile(std::false_type{});
+      else tile(std::true_type{});
+      if (!ok) break;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&p_full[w]);
+    }
+    if (ok && tiles > 0) ok = wait_all(&pv_done[w], tiles - 1);
+    tc_fence_after();
+    if (w < nq && !idle) {
+      const float sum = l.x + l.y;
+      const float inv = tiles > 0 && sum != 0.0f ? 1.0f / sum : 0.0f;
+      if (row < x.Lq && x.lse2) x.lse2[(b * x.H + h) * x.Lq + row] = sum == 0.0f ? INFINITY : m * c2 + log2f(sum);
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(x.o) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (tiles > 0) {
+          tmem_ld32_nowait(tO + c, o);
+          tmem_wait_ld();
+          tmem_pin<32>(o);
+        }
+        if (row < x.Lq) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (c + i < x.D) {
+              uint32_t q[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)  // a row without keys: zero, whatever O holds
+                q[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
+              *reinterpret_cast<uint4*>(out + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
+            }
         }
       }
     }
