@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -88,29 +89,12 @@ SIGNATURES = {
 }
 
 
-class View(ctypes.Structure):
-    """hclsm_view: a (B, L, H, D) tensor whose last dim is dense."""
-    _fields_ = [("p", ctypes.c_void_p), ("sb", ctypes.c_int64), ("st", ctypes.c_int64), ("sh", ctypes.c_int64)]
-
-
-class RopeSide(ctypes.Structure):
-    """hclsm_rope_side."""
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "dy", "y", "w", "pos", "dw")] + \
-               [(n, ctypes.c_int64) for n in ("sb", "st", "sh")] + [("L", ctypes.c_int32), ("H", ctypes.c_int32)]
-
-
-class XattnArgs(ctypes.Structure):
-    """hclsm_xattn_args."""
-    _fields_ = [(n, View) for n in ("q", "k", "v", "dout")] + \
-               [(n, ctypes.c_void_p) for n in ("o", "dq", "dk", "dv", "lse2", "lens", "mask")] + \
-               [("mask_sb", ctypes.c_int64)] + \
-               [(n, ctypes.c_int32) for n in ("B", "Lq", "Lk", "H", "Hkv", "D", "dtype")] + [("scale", ctypes.c_float)]
-
-
-class Kv8(ctypes.Structure):
-    """hclsm_kv8_cache."""
-    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")] + \
-               [(n, ctypes.c_int32) for n in ("B", "Hkv", "T", "D", "block", "dtype")]
+# The argument structs of include/hclsm_b200.h, packed with the C layout (a bytes object
+# passes as a pointer; several times cheaper to make than a ctypes.Structure).
+VIEW = struct.Struct("@Pqqq")                     # hclsm_view
+ROPE_SIDE = struct.Struct("@6P3q2i")              # hclsm_rope_side
+XATTN_ARGS = struct.Struct("@" + 4 * "Pqqq" + "7Pq7if")  # hclsm_xattn_args
+KV8_CACHE = struct.Struct("@6P6i")                # hclsm_kv8_cache
 
 
 class SlotIterWeights(ctypes.Structure):
@@ -149,7 +133,14 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
 def stream_ptr(device) -> int:
+    """The current stream of a CUDA device as an integer (a tensor's device has an index; the
+    raw query skips the Stream object, about 3 us a call)."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -181,28 +172,37 @@ def dense_last(t):
 
 
 def rows16(t):
-    """t itself if its last dim is dense and every row starts on 16 bytes, else an aligned contiguous copy."""
-    e = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s * e % 16 for s in t.stride()[:-1]):
+    """The (B, L, H, D) tensor itself if its last dim is dense and every row starts on 16
+    bytes, else an aligned contiguous copy."""
+    sb, st, sh, sd = t.stride()
+    if sd == 1 and t.data_ptr() % 16 == 0 and (sb | st | sh) * t.element_size() % 16 == 0:
         return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 
 
-def view(t):
-    """hclsm_view of a (B, L, H, D) tensor."""
-    s = t.stride()
-    return View(t.data_ptr(), s[0], s[1], s[2])
+def view_args(t):
+    """The fields of hclsm_view for a (B, L, H, D) tensor."""
+    sb, st, sh, _ = t.stride()
+    return t.data_ptr(), sb, st, sh
 
 
 def index32(t, shape, name, device):
     """An int32, contiguous index tensor of that shape on that device (int64 is converted), or None."""
     if t is None:
         return None
-    if t.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.dtype != torch.int32:
+        if t.dtype != torch.int64:
+            raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
+        t = t.to(torch.int32)
+    if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
-    return t.to(torch.int32).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def no_double_backward():
+    """A backward made of this library's kernels has no graph of its own."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("hclsm_b200: this operator has no second derivative (create_graph=True)")

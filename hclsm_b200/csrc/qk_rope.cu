@@ -53,10 +53,13 @@ struct Params {
   int* err;
 };
 
+// 8 elements as loaded, and as fp32.
 template <typename T> struct Vec8;
 template <> struct Vec8<__nv_bfloat16> {
-  static __device__ __forceinline__ void ld(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
+  uint4 r;
+  __device__ __forceinline__ void ld(const __nv_bfloat16* p) { r = __ldcs(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -75,8 +78,12 @@ template <> struct Vec8<__nv_bfloat16> {
   }
 };
 template <> struct Vec8<float> {
-  static __device__ __forceinline__ void ld(const float* p, float (&v)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  float4 a, b;
+  __device__ __forceinline__ void ld(const float* p) {
+    a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p + 4));
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   }
   static __device__ __forceinline__ void st(float* p, const float (&v)[8]) {
@@ -84,6 +91,10 @@ template <> struct Vec8<float> {
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
   }
 };
+__device__ __forceinline__ void table8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
 
 // The rotation of a lane's 8 dims, angle sign `sg` (+1 forward, -1 its
 // transpose).  c, s: the lane's cosines and sines (1 and 0 past the rotated
@@ -116,12 +127,12 @@ __device__ __forceinline__ float head_sum(float v, int lph) {
 
 // One warp-task: the heads [h0, h1) of token t of batch b.
 template <typename T, bool BWD>
-__device__ __forceinline__ void token(const Params& p, const Side& sd, int64_t task, int lane, const float (&w)[8],
+__device__ __forceinline__ void token(const Params& p, const Side& sd, uint32_t task, int lane, const float (&w)[8],
                                       float (&dw)[8]) {
-  const int chunk = (int)(task % sd.chunks);
-  const int64_t bt = task / sd.chunks;
-  const int64_t b = bt / sd.L;
-  const int t = (int)(bt - b * sd.L);
+  constexpr int U = sizeof(T) == 2 && !BWD ? 4 : 2;  // passes whose loads are in flight together
+  const uint32_t bt32 = task / (uint32_t)sd.chunks, b32 = bt32 / (uint32_t)sd.L;
+  const int chunk = (int)(task - bt32 * (uint32_t)sd.chunks), t = (int)(bt32 - b32 * (uint32_t)sd.L);
+  const int64_t bt = bt32, b = b32;
   const int lph = p.lph, hpw = 32 / lph;
   const int hl = lane / lph, d0 = (lane % lph) * 8;
   const int per = (sd.H + sd.chunks - 1) / sd.chunks;
@@ -151,8 +162,8 @@ __device__ __forceinline__ void token(const Params& p, const Side& sd, int64_t t
         c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w;
         s[0] = e.x, s[1] = e.y, s[2] = e.z, s[3] = e.w;
       } else {
-        Vec8<float>::ld(p.cosv + row + d0 - (second ? half : 0), c);
-        Vec8<float>::ld(p.sinv + row + d0 - (second ? half : 0), s);
+        table8(p.cosv + row + d0 - (second ? half : 0), c);
+        table8(p.sinv + row + d0 - (second ? half : 0), s);
       }
       if (bad) {  // a position outside the table: NaN, not another position's angle
 #pragma unroll
@@ -163,43 +174,56 @@ __device__ __forceinline__ void token(const Params& p, const Side& sd, int64_t t
   const T* x = static_cast<const T*>(sd.x) + b * sd.sb + (int64_t)t * sd.st;
   const int64_t dense = bt * sd.H * p.D;
   const float inv_d = 1.0f / (float)p.D;
-#pragma unroll 2
-  for (int hb = h0; hb < h1; hb += hpw) {  // warp-uniform trip count
-    const int h = hb + hl;
-    const bool ok = dim_ok && h < h1;
-    float v[8], u[8];
+  for (int hb = h0; hb < h1; hb += hpw * U) {  // warp-uniform trip count
+    Vec8<T> xr[U], gr[BWD ? U : 1];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f, u[i] = 0.0f;
-    if (ok) Vec8<T>::ld(x + h * sd.sh + d0, v);
-    if (BWD && ok) Vec8<T>::ld(static_cast<const T*>(sd.dy) + dense + (int64_t)h * p.D + d0, u);
-    float r = 1.0f;
-    if (p.norm) {
-      float q = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q += v[i] * v[i];
-      r = rsqrtf(head_sum(q, lph) * inv_d + p.eps);
-    }
-    if constexpr (!BWD) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i];
-      rotate(v, c, s, 1.0f, p.inter, partner, second);
-      if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, v);
-    } else {
-      rotate(u, c, s, -1.0f, p.inter, partner, second);
-      if (p.norm) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          v[i] *= r;  // xh
-          dw[i] += u[i] * v[i];
-          u[i] *= w[i];
-          m += u[i] * v[i];
-        }
-        m = head_sum(m, lph) * inv_d;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = r * (u[i] - v[i] * m);
+    for (int i = 0; i < U; ++i) {
+      const int h = hb + i * hpw + hl;
+      xr[i].zero();
+      if (BWD) gr[BWD ? i : 0].zero();
+      if (dim_ok && h < h1) {
+        xr[i].ld(x + h * sd.sh + d0);
+        if (BWD) gr[BWD ? i : 0].ld(static_cast<const T*>(sd.dy) + dense + (int64_t)h * p.D + d0);
       }
-      if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, u);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (hb + i * hpw >= h1) break;  // warp-uniform
+      const int h = hb + i * hpw + hl;
+      const bool ok = dim_ok && h < h1;
+      float v[8];
+      xr[i].get(v);
+      float r = 1.0f;
+      if (p.norm) {
+        float q = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q += v[e] * v[e];
+        r = rsqrtf(head_sum(q, lph) * inv_d + p.eps);
+      }
+      if constexpr (!BWD) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
+        rotate(v, c, s, 1.0f, p.inter, partner, second);
+        if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, v);
+      } else {
+        float u[8];
+        gr[i].get(u);
+        rotate(u, c, s, -1.0f, p.inter, partner, second);
+        if (p.norm) {
+          float m = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[e] *= r;  // xh
+            dw[e] += u[e] * v[e];
+            u[e] *= w[e];
+            m += u[e] * v[e];
+          }
+          m = head_sum(m, lph) * inv_d;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e] = r * (u[e] - v[e] * m);
+        }
+        if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, u);
+      }
     }
   }
 }
@@ -222,7 +246,7 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
     for (int i = 0; i < 8; ++i) w[i] = sd.w[d0 + i];
   }
   for (int64_t task = (int64_t)blk * kWarps + warp; task < sd.tasks; task += (int64_t)sd.blocks * kWarps)
-    token<T, BWD>(p, sd, task, lane, w, dw);
+    token<T, BWD>(p, sd, (uint32_t)task, lane, w, dw);
   if constexpr (BWD) {
     if (sd.partial) {
       // the warp's heads, then the block's warps, both in a fixed order
@@ -271,7 +295,7 @@ int lanes_per_head(int D) {
 }
 
 // Backward blocks of one side: bounded so that the column sums' second stage
-// stays short (4 blocks of 8 warps an SM hide the loads' latency).
+// stays short.
 int bwd_blocks(int64_t tasks) {
   const int64_t want = (tasks + kWarps - 1) / kWarps, most = (int64_t)num_sms() * 4;
   return (int)(want < most ? want : most);
@@ -327,7 +351,7 @@ int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, c
     s.sb = in[i]->sb, s.st = in[i]->st, s.sh = in[i]->sh;
     s.L = in[i]->L, s.H = in[i]->H;
     if (B * s.L > 0) plan(s, B, p.lph);
-    if (!bwd && (s.tasks + kWarps - 1) / kWarps > 0x3fffffff) return HCLSM_ERR_SHAPE;
+    if (s.tasks > 0x7fffffff) return HCLSM_ERR_SHAPE;
     s.blocks = bwd ? bwd_blocks(s.tasks) : (int)((s.tasks + kWarps - 1) / kWarps);
     if (bwd && in[i]->dw) {
       const size_t need = (size_t)s.blocks * D * sizeof(float);

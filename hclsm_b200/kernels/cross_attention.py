@@ -8,7 +8,6 @@ query heads, and is differentiable in q, k and v (bit-reproducible gradients).
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -18,31 +17,35 @@ from .. import _lib
 __all__ = ["cross_attention"]
 
 
-def _args(q, k, v, o, lse, lens, mask, scale):
-    a = _lib.XattnArgs()
-    a.q, a.k, a.v = _lib.view(q), _lib.view(k), _lib.view(v)
-    a.o, a.lse2, a.lens = o.data_ptr(), _lib.ptr(lse), _lib.ptr(lens)
-    if mask is not None:
-        a.mask, a.mask_sb = mask.data_ptr(), mask.stride(0)
-    a.B, a.Lq, a.H, a.D = q.shape
-    a.Lk, a.Hkv = k.shape[1], k.shape[2]
-    a.dtype, a.scale = _lib.dtype_code(q.dtype), scale
-    return a
-
-
-def _workspace(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def _args(q, k, v, o, lse, lens, mask, scale, do=None, dq=None, dk=None, dv=None):
+    B, Lq, H, D = q.shape
+    qb, qt, qh, _ = q.stride()
+    kb, kt, kh, _ = k.stride()
+    vb, vt, vh, _ = v.stride()
+    gp = gb = gt = gh = dqp = dkp = dvp = 0
+    if do is not None:
+        gp, gb, gt, gh = _lib.view_args(do)
+        dqp, dkp, dvp = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    return _lib.XATTN_ARGS.pack(
+        q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, gp, gb, gt, gh, o.data_ptr(),
+        dqp, dkp, dvp, 0 if lse is None else lse.data_ptr(), 0 if lens is None else lens.data_ptr(),
+        0 if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), B, Lq, k.shape[1], H, k.shape[2],
+        D, _lib.dtype_code(q.dtype), scale)
 
 
 def _forward(q, k, v, lens, mask, scale, keep):
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    B, Lq, H, _ = q.shape
-    lse = torch.empty(B, H, Lq, dtype=torch.float32, device=q.device) if keep else None
+    o = q.new_empty(q.shape)
+    lse = None
+    if keep:
+        B, Lq, H, _ = q.shape
+        lse = q.new_empty((B, H, Lq), dtype=torch.float32)
     a = _args(q, k, v, o, lse, lens, mask, scale)
-    lib, at = _lib.load(), ctypes.addressof(a)
-    n = lib.hclsm_xattn_fwd_workspace_size(at)
-    ws = _workspace(n, q.device)
-    _lib.check(lib.hclsm_xattn_fwd(at, _lib.ptr(ws), n, _lib.stream_ptr(q.device)), "hclsm_xattn_fwd")
+    lib, ws = _lib.load(), None
+    n = lib.hclsm_xattn_fwd_workspace_size(a)
+    if n:
+        ws = q.new_empty(n, dtype=torch.uint8)
+    _lib.check(lib.hclsm_xattn_fwd(a, None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(q.device)),
+               "hclsm_xattn_fwd")
     return o, lse
 
 
@@ -55,18 +58,16 @@ class _CrossAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
+        _lib.no_double_backward()
         q, k, v, o, lse, lens, mask = ctx.saved_tensors
-        do = _lib.dense_last(do.to(q.dtype))
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        a = _args(q, k, v, o, lse, lens, mask, ctx.scale)
-        a.dout = _lib.view(do)
-        a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        lib, at = _lib.load(), ctypes.addressof(a)
-        n = lib.hclsm_xattn_bwd_workspace_size(at)
-        ws = _workspace(n, q.device)
-        _lib.check(lib.hclsm_xattn_bwd(at, _lib.ptr(ws), n, _lib.stream_ptr(q.device)), "hclsm_xattn_bwd")
+        do = _lib.dense_last(do)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        a = _args(q, k, v, o, lse, lens, mask, ctx.scale, do, dq, dk, dv)
+        lib = _lib.load()
+        n = lib.hclsm_xattn_bwd_workspace_size(a)
+        ws = q.new_empty(n, dtype=torch.uint8)
+        _lib.check(lib.hclsm_xattn_bwd(a, ws.data_ptr(), n, _lib.stream_ptr(q.device)), "hclsm_xattn_bwd")
         return dq, dk, dv, None, None, None
 
 

@@ -9,7 +9,6 @@ replayed with other positions.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass, field
 
@@ -33,7 +32,7 @@ class Kv8Cache:
     v_scale: Tensor
     k_tail: Tensor
     v_tail: Tensor
-    _c: _lib.Kv8 = field(init=False, repr=False, compare=False, default=None)
+    _c: bytes = field(init=False, repr=False, compare=False, default=b"")  # hclsm_kv8_cache
 
     def __post_init__(self):
         _lib.require_cuda(self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
@@ -52,9 +51,9 @@ class Kv8Cache:
                                    ("v_tail", self.v_tail, (B, Hkv, block, D), dtype)):
             if t.shape != shape or t.dtype != dt or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous {shape} {dt}, got {tuple(t.shape)} {t.dtype}")
-        self._c = _lib.Kv8(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                           self.k_tail.data_ptr(), self.v_tail.data_ptr(), B, Hkv, T, D, block,
-                           _lib.dtype_code(dtype))
+        self._c = _lib.KV8_CACHE.pack(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
+                                      self.v_scale.data_ptr(), self.k_tail.data_ptr(), self.v_tail.data_ptr(), B, Hkv,
+                                      T, D, block, _lib.dtype_code(dtype))
 
     @classmethod
     def empty(cls, batch: int, capacity: int, kv_heads: int, head_dim: int, *, block: int = 32, dtype=torch.bfloat16,
@@ -94,10 +93,9 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
         raise ValueError("start is required")
     count = _lib.index32(count, (B,), "count", dev)
     k, v = _lib.rows16(k), _lib.rows16(v)
-    kv, vv = _lib.view(k), _lib.view(v)
-    _lib.check(_lib.load().hclsm_kv8_write(ctypes.addressof(cache._c), ctypes.addressof(kv), ctypes.addressof(vv),
-                                           k.shape[1], start.data_ptr(), _lib.ptr(count), _lib.stream_ptr(dev)),
-               "hclsm_kv8_write")
+    _lib.check(_lib.load().hclsm_kv8_write(cache._c, _lib.VIEW.pack(*_lib.view_args(k)),
+                                           _lib.VIEW.pack(*_lib.view_args(v)), k.shape[1], start.data_ptr(),
+                                           _lib.ptr(count), _lib.stream_ptr(dev)), "hclsm_kv8_write")
 
 
 def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
@@ -107,7 +105,7 @@ def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
     B, Hkv, T, D = cache.k.shape
     lens = _lib.index32(lens, (B,), "lens", dev)
     k, v = (torch.empty(B, T, Hkv, D, dtype=cache.dtype, device=dev) for _ in range(2))
-    _lib.check(_lib.load().hclsm_kv8_read(ctypes.addressof(cache._c), k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
+    _lib.check(_lib.load().hclsm_kv8_read(cache._c, k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
                                           _lib.stream_ptr(dev)), "hclsm_kv8_read")
     return k, v
 
@@ -132,10 +130,12 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
         raise ValueError(f"scale must be positive and finite, got {scale}")
     lens = _lib.index32(lens, (B,), "lens", dev)
     q = _lib.dense_last(q)
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lib, c, qv = _lib.load(), ctypes.addressof(cache._c), _lib.view(q)
-    n = lib.hclsm_kv8_attn_workspace_size(c, Lq, H)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(lib.hclsm_kv8_attn(c, ctypes.addressof(qv), o.data_ptr(), _lib.ptr(lens), Lq, H, scale, _lib.ptr(ws), n,
-                                  _lib.stream_ptr(dev)), "hclsm_kv8_attn")
+    o = q.new_empty(q.shape)
+    lib, ws = _lib.load(), None
+    n = lib.hclsm_kv8_attn_workspace_size(cache._c, Lq, H)
+    if n:
+        ws = q.new_empty(n, dtype=torch.uint8)
+    _lib.check(lib.hclsm_kv8_attn(cache._c, _lib.VIEW.pack(*_lib.view_args(q)), o.data_ptr(), _lib.ptr(lens), Lq, H,
+                                  scale, None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(dev)),
+               "hclsm_kv8_attn")
     return o

@@ -9,8 +9,6 @@ gradients have their inputs' dtypes (float32 or bfloat16; weights fp32).
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from .. import _lib
@@ -29,6 +27,12 @@ def rope_tables(positions: int, dim: int, base: float = 10000.0, *, scale: float
     freq = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
     ang = torch.arange(positions, dtype=torch.float64)[:, None] / float(scale) * freq
     return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+def _dense16(t):
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
@@ -61,36 +65,32 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
 
 
 def _side(x, y, w, pos, dy=None, dw=None):
-    s = x.stride()
-    return _lib.RopeSide(x.data_ptr(), _lib.ptr(dy), y.data_ptr(), _lib.ptr(w), _lib.ptr(pos), _lib.ptr(dw),
-                         s[0], s[1], s[2], x.shape[1], x.shape[2])
+    sb, st, sh, _ = x.stride()
+    return _lib.ROPE_SIDE.pack(x.data_ptr(), 0 if dy is None else dy.data_ptr(), y.data_ptr(),
+                               0 if w is None else w.data_ptr(), 0 if pos is None else pos.data_ptr(),
+                               0 if dw is None else dw.data_ptr(), sb, st, sh, x.shape[1], x.shape[2])
 
 
-def _call(bwd, qs, ks, cos, sin, B, D, eps, dtype, interleaved, device):
-    lib = _lib.load()
+def _tables(q, cos, sin, eps, interleaved):
+    """The arguments after the two sides."""
     flags = (_INTERLEAVED if interleaved else 0) | (_NO_NORM if eps is None else 0)
-    args = (ctypes.addressof(qs), None if ks is None else ctypes.addressof(ks), _lib.ptr(cos), _lib.ptr(sin),
-            0 if cos is None else cos.shape[0], 0 if cos is None else 2 * cos.shape[1], B, D, eps or 0.0,
-            _lib.dtype_code(dtype), flags)
-    if not bwd:
-        _lib.check(lib.hclsm_qk_norm_rope(*args, _lib.stream_ptr(device)), "hclsm_qk_norm_rope")
-        return
-    ws, n = None, 0
-    if qs.dw or (ks is not None and ks.dw):
-        n = lib.hclsm_qk_norm_rope_bwd_workspace_size(D)
-        ws = torch.empty(n, dtype=torch.uint8, device=device)
-    _lib.check(lib.hclsm_qk_norm_rope_bwd(*args, _lib.ptr(ws), n, _lib.stream_ptr(device)), "hclsm_qk_norm_rope_bwd")
+    B, _, _, D = q.shape
+    if cos is None:
+        return None, None, 0, 0, B, D, eps or 0.0, _lib.dtype_code(q.dtype), flags
+    P, half = cos.shape
+    return cos.data_ptr(), sin.data_ptr(), P, 2 * half, B, D, eps or 0.0, _lib.dtype_code(q.dtype), flags
 
 
 def _forward(q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved):
     q = _lib.rows16(q)
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    yq = q.new_empty(q.shape)
     qs, ks, yk = _side(q, yq, qw, q_pos), None, None
     if k is not None:
         k = _lib.rows16(k)
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        yk = k.new_empty(k.shape)
         ks = _side(k, yk, kw, k_pos)
-    _call(False, qs, ks, cos, sin, q.shape[0], q.shape[3], eps, q.dtype, interleaved, q.device)
+    _lib.check(_lib.load().hclsm_qk_norm_rope(qs, ks, *_tables(q, cos, sin, eps, interleaved),
+                                              _lib.stream_ptr(q.device)), "hclsm_qk_norm_rope")
     return q, k, yq, yk
 
 
@@ -103,23 +103,32 @@ class _QkNormRope(torch.autograd.Function):
         return yq, yk
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
+        _lib.no_double_backward()
         q, k, qw, kw, cos, sin, q_pos, k_pos = ctx.saved_tensors
-
-        def one(x, w, pos, g, want_w):
-            if x is None:
-                return None, None, None
-            g = _lib.rows16(g.to(x.dtype).contiguous())
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            dw = torch.empty_like(w) if w is not None and want_w else None
-            return _side(x, dx, w, pos, g, dw), dx, dw, g
-
-        qs, dq, dqw, _gq = one(q, qw, q_pos, gq, ctx.needs_input_grad[2])
-        ks = dk = dkw = None
+        dev = q.device
+        want = ctx.needs_input_grad
+        dq = dk = dqw = dkw = ks = ws = None
+        # the gradients arrive dense or are made so
+        gq = gq if gq.is_contiguous() and gq.data_ptr() % 16 == 0 else gq.clone(memory_format=torch.contiguous_format)
+        dq = q.new_empty(q.shape)
+        if qw is not None and want[2]:
+            dqw = qw.new_empty(qw.shape)
+        qs = _side(q, dq, qw, q_pos, gq, dqw)
         if k is not None:
-            ks, dk, dkw, _gk = one(k, kw, k_pos, gk, ctx.needs_input_grad[3])
-        _call(True, qs, ks, cos, sin, q.shape[0], q.shape[3], ctx.eps, q.dtype, ctx.interleaved, q.device)
+            gk = gk if gk.is_contiguous() and gk.data_ptr() % 16 == 0 else \
+                gk.clone(memory_format=torch.contiguous_format)
+            dk = k.new_empty(k.shape)
+            if kw is not None and want[3]:
+                dkw = kw.new_empty(kw.shape)
+            ks = _side(k, dk, kw, k_pos, gk, dkw)
+        lib, n = _lib.load(), 0
+        if dqw is not None or dkw is not None:
+            n = lib.hclsm_qk_norm_rope_bwd_workspace_size(q.shape[3])
+            ws = q.new_empty(n, dtype=torch.uint8)
+        _lib.check(lib.hclsm_qk_norm_rope_bwd(qs, ks, *_tables(q, cos, sin, ctx.eps, ctx.interleaved),
+                                              None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(dev)),
+                   "hclsm_qk_norm_rope_bwd")
         return dq, dk, dqw, dkw, None, None, None, None, None, None
 
 
@@ -138,7 +147,7 @@ def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, *,
     """
     dev = _check(q, k, q_weight, k_weight, cos, sin, eps)
     if cos is not None:
-        cos, sin = _lib.rows16(cos.contiguous()), _lib.rows16(sin.contiguous())
+        cos, sin = _dense16(cos), _dense16(sin)
         rot = 2 * cos.shape[1]
         if rot > q.shape[3] or rot % (8 if interleaved else 16):
             raise ValueError(f"rotary_dim {rot} must be a multiple of {8 if interleaved else 16} up to head_dim")
