@@ -27,6 +27,7 @@ namespace rope {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kBwdPerSm = 3;  // resident blocks of the backward kernel
 
 struct Side {
   const void* x;
@@ -59,19 +60,29 @@ template <> struct Vec8<__nv_bfloat16> {
   uint4 r;
   __device__ __forceinline__ void ld(const __nv_bfloat16* p) { r = __ldcs(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ void st(__nv_bfloat16* p, const float (&v)[8]) {
+  // another lane's elements, or zeros
+  __device__ __forceinline__ Vec8 from(int lane, bool some) const {
+    Vec8 o;
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[i] = __shfl_sync(0xffffffffu, w[i], lane);
+      q[i] = some ? q[i] : 0u;
+    }
+    o.r = make_uint4(q[0], q[1], q[2], q[3]);
+    return o;
+  }
+  static __device__ __forceinline__ void st(__nv_bfloat16* p, const float2 (&v)[4]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[i].x, v[i].y);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -83,12 +94,24 @@ template <> struct Vec8<float> {
     a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p + 4));
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  __device__ __forceinline__ void get(float2 (&v)[4]) const {
+    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
   }
-  static __device__ __forceinline__ void st(float* p, const float (&v)[8]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+  __device__ __forceinline__ Vec8 from(int lane, bool some) const {
+    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[i] = __shfl_sync(0xffffffffu, w[i], lane);
+      q[i] = some ? q[i] : 0.0f;
+    }
+    Vec8 o;
+    o.a = make_float4(q[0], q[1], q[2], q[3]), o.b = make_float4(q[4], q[5], q[6], q[7]);
+    return o;
+  }
+  static __device__ __forceinline__ void st(float* p, const float2 (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
   }
 };
 __device__ __forceinline__ void table8(const float* p, float (&v)[8]) {
@@ -96,57 +119,59 @@ __device__ __forceinline__ void table8(const float* p, float (&v)[8]) {
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// The rotation of a lane's 8 dims, angle sign `sg` (+1 forward, -1 its
-// transpose).  c, s: the lane's cosines and sines (1 and 0 past the rotated
-// dims).  Half layout: c, s of the 8 dims; the partner dims sit `hop` lanes
-// away, up for the first half and down for the second.  Interleaved: c[0..3],
-// s[0..3] of the 4 pairs.
-__device__ __forceinline__ void rotate(float (&v)[8], const float (&c)[8], const float (&s)[8], float sg, bool inter,
-                                       int partner, bool second) {
-  if (inter) {
+// The sum over a head's lanes.
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float a = v[2 * i], b = v[2 * i + 1], t = sg * s[i];
-      v[2 * i] = a * c[i] - b * t;
-      v[2 * i + 1] = b * c[i] + a * t;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float o = __shfl_sync(0xffffffffu, v[i], partner);
-      const float t = second ? sg * s[i] : -sg * s[i];
-      v[i] = v[i] * c[i] + o * t;
-    }
-  }
-}
-
-__device__ __forceinline__ float head_sum(float v, int lph) {
-  for (int o = lph >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = LPH >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+__device__ __forceinline__ float2 swap(float2 v) { return make_float2(v.y, v.x); }
 
 // One warp-task: the heads [h0, h1) of token t of batch b.
-template <typename T, bool BWD>
-__device__ __forceinline__ void token(const Params& p, const Side& sd, uint32_t task, int lane, const float (&w)[8],
-                                      float (&dw)[8]) {
+//
+// With c and s the cosines and signed sines of the lane's dims, the rotation is
+// y_i = c_i z_i + s_i z_p(i), p(i) the pair's other dim: in the same lane's pair
+// (INTER) or, for the half layout, at the same place `hop` lanes away.  Forward:
+// z = r w x, so w is folded into the angles once a token and r follows.  Backward:
+// the transpose, with the sines' signs turned.
+template <typename T, int LPH, bool INTER, bool BWD>
+__device__ __forceinline__ void token(const Params& p, const Side& sd, uint32_t task, int lane, const float2 (&w)[4],
+                                      float2 (&dw)[4]) {
   constexpr int U = sizeof(T) == 2 && !BWD ? 4 : 2;  // passes whose loads are in flight together
+  constexpr int HPW = 32 / LPH;
   const uint32_t bt32 = task / (uint32_t)sd.chunks, b32 = bt32 / (uint32_t)sd.L;
   const int chunk = (int)(task - bt32 * (uint32_t)sd.chunks), t = (int)(bt32 - b32 * (uint32_t)sd.L);
   const int64_t bt = bt32, b = b32;
-  const int lph = p.lph, hpw = 32 / lph;
-  const int hl = lane / lph, d0 = (lane % lph) * 8;
+  const int hl = lane / LPH, d0 = (lane % LPH) * 8;
   const int per = (sd.H + sd.chunks - 1) / sd.chunks;
   const int h0 = chunk * per, h1 = min(sd.H, h0 + per);
-  const bool dim_ok = d0 < p.D;
-  const bool in_rot = d0 < p.rot;
-  const int half = p.rot >> 1;
+  const bool dim_ok = d0 < p.D, in_rot = d0 < p.rot;
+  const int half = p.rot >> 1, hop = half >> 3;
   const bool second = d0 >= half;
-  const int hop = half >> 3;
-  const int partner = !p.inter && in_rot ? (second ? lane - hop : lane + hop) : lane;
-
-  float c[8], s[8];
+  const int partner = !INTER && in_rot ? (second ? lane - hop : lane + hop) : lane;
+  const T* x = static_cast<const T*>(sd.x) + b * sd.sb + (int64_t)t * sd.st + (int64_t)hl * sd.sh + d0;
+  const int64_t at = (bt * sd.H + hl) * p.D + d0;  // of the dense tensors
+  const T* dy = static_cast<const T*>(sd.dy) + at;
+  T* y = static_cast<T*>(sd.y) + at;
+  Vec8<T> xr[U], gr[BWD ? U : 1];
+  auto fetch = [&](int hb) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = 1.0f, s[i] = 0.0f;
+    for (int i = 0; i < U; ++i) {
+      const int h = hb + i * HPW;
+      xr[i].zero();
+      if (BWD) gr[BWD ? i : 0].zero();
+      if (dim_ok && h + hl < h1) {
+        xr[i].ld(x + h * sd.sh);
+        if (BWD) gr[BWD ? i : 0].ld(dy + (int64_t)h * p.D);
+      }
+    }
+  };
+  fetch(h0);  // in flight while the position and then its angles arrive
+
+  float2 c[4], s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i] = make_float2(1.0f, 1.0f), s[i] = make_float2(0.0f, 0.0f);
   if (p.rot > 0) {
     int pos = sd.pos ? sd.pos[bt] : t;
     const bool bad = pos < 0 || pos >= p.P;
@@ -156,80 +181,99 @@ __device__ __forceinline__ void token(const Params& p, const Side& sd, uint32_t 
     }
     if (in_rot) {
       const int64_t row = (int64_t)pos * half;
-      if (p.inter) {
-        const float4 a = *reinterpret_cast<const float4*>(p.cosv + row + (d0 >> 1));
-        const float4 e = *reinterpret_cast<const float4*>(p.sinv + row + (d0 >> 1));
-        c[0] = a.x, c[1] = a.y, c[2] = a.z, c[3] = a.w;
-        s[0] = e.x, s[1] = e.y, s[2] = e.z, s[3] = e.w;
+      const float sg = BWD ? -1.0f : 1.0f;
+      if constexpr (INTER) {
+        const float4 ca = *reinterpret_cast<const float4*>(p.cosv + row + (d0 >> 1));
+        const float4 sa = *reinterpret_cast<const float4*>(p.sinv + row + (d0 >> 1));
+        const float cv[4] = {ca.x, ca.y, ca.z, ca.w}, sv[4] = {sa.x, sa.y, sa.z, sa.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = make_float2(cv[i], cv[i]), s[i] = make_float2(-sg * sv[i], sg * sv[i]);
       } else {
-        table8(p.cosv + row + d0 - (second ? half : 0), c);
-        table8(p.sinv + row + d0 - (second ? half : 0), s);
+        float cv[8], sv[8];
+        table8(p.cosv + row + d0 - (second ? half : 0), cv);
+        table8(p.sinv + row + d0 - (second ? half : 0), sv);
+        const float f = second ? sg : -sg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          c[i] = make_float2(cv[2 * i], cv[2 * i + 1]), s[i] = make_float2(f * sv[2 * i], f * sv[2 * i + 1]);
       }
       if (bad) {  // a position outside the table: NaN, not another position's angle
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
+        for (int i = 0; i < 4; ++i) c[i] = s[i] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
       }
     }
   }
-  const T* x = static_cast<const T*>(sd.x) + b * sd.sb + (int64_t)t * sd.st;
-  const int64_t dense = bt * sd.H * p.D;
-  const float inv_d = 1.0f / (float)p.D;
-  for (int hb = h0; hb < h1; hb += hpw * U) {  // warp-uniform trip count
-    Vec8<T> xr[U], gr[BWD ? U : 1];
+  if constexpr (!BWD) {
+    if (sd.w) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int h = hb + i * hpw + hl;
-      xr[i].zero();
-      if (BWD) gr[BWD ? i : 0].zero();
-      if (dim_ok && h < h1) {
-        xr[i].ld(x + h * sd.sh + d0);
-        if (BWD) gr[BWD ? i : 0].ld(static_cast<const T*>(sd.dy) + dense + (int64_t)h * p.D + d0);
+      for (int i = 0; i < 4; ++i) {
+        float2 o = swap(w[i]);
+        if (!INTER)
+          o = make_float2(__shfl_sync(0xffffffffu, w[i].x, partner), __shfl_sync(0xffffffffu, w[i].y, partner));
+        c[i] = mul2(c[i], w[i]), s[i] = mul2(s[i], o);
       }
     }
+  }
+  const float inv_d = 1.0f / (float)p.D;
+  for (int hb = h0; hb < h1; hb += HPW * U) {  // warp-uniform trip count
+    if (hb != h0) fetch(hb);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      if (hb + i * hpw >= h1) break;  // warp-uniform
-      const int h = hb + i * hpw + hl;
-      const bool ok = dim_ok && h < h1;
-      float v[8];
+      if (hb + i * HPW >= h1) break;  // warp-uniform
+      const int h = hb + i * HPW;
+      const bool ok = dim_ok && h + hl < h1;
+      float2 v[4], o[4];
       xr[i].get(v);
       float r = 1.0f;
       if (p.norm) {
-        float q = 0.0f;
+        float2 q = mul2(v[0], v[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q += v[e] * v[e];
-        r = rsqrtf(head_sum(q, lph) * inv_d + p.eps);
+        for (int e = 1; e < 4; ++e) q = fma2(v[e], v[e], q);
+        r = rsqrtf(head_sum<LPH>(q.x + q.y) * inv_d + p.eps);
       }
+      const float2 rr = make_float2(r, r);
       if constexpr (!BWD) {
+        if constexpr (INTER) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
-        rotate(v, c, s, 1.0f, p.inter, partner, second);
-        if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, v);
-      } else {
-        float u[8];
-        gr[i].get(u);
-        rotate(u, c, s, -1.0f, p.inter, partner, second);
-        if (p.norm) {
-          float m = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[e] *= r;  // xh
-            dw[e] += u[e] * v[e];
-            u[e] *= w[e];
-            m += u[e] * v[e];
-          }
-          m = head_sum(m, lph) * inv_d;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = r * (u[e] - v[e] * m);
+          for (int e = 0; e < 4; ++e) o[e] = in_rot ? swap(v[e]) : make_float2(0.0f, 0.0f);
+        } else {
+          xr[i].from(partner, in_rot).get(o);
         }
-        if (ok) Vec8<T>::st(static_cast<T*>(sd.y) + dense + (int64_t)h * p.D + d0, u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = mul2(fma2(o[e], s[e], mul2(v[e], c[e])), rr);
+        if (ok) Vec8<T>::st(y + (int64_t)h * p.D, v);
+      } else {
+        float2 u[4];
+        gr[i].get(u);
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = in_rot ? swap(u[e]) : make_float2(0.0f, 0.0f);
+        } else {
+          gr[i].from(partner, in_rot).get(o);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = fma2(o[e], s[e], mul2(u[e], c[e]));
+        if (p.norm) {
+          float2 m = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] = mul2(v[e], rr);  // xh
+            dw[e] = fma2(u[e], v[e], dw[e]);
+            u[e] = mul2(u[e], w[e]);
+            m = fma2(u[e], v[e], m);
+          }
+          const float mean = -head_sum<LPH>(m.x + m.y) * inv_d;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = mul2(fma2(v[e], make_float2(mean, mean), u[e]), rr);
+        }
+        if (ok) Vec8<T>::st(y + (int64_t)h * p.D, u);
       }
     }
   }
 }
 
-template <typename T, bool BWD>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ Params p) {
+template <typename T, int LPH, bool INTER, bool BWD>
+__global__ void __launch_bounds__(kThreads, BWD ? kBwdPerSm : 4) rope_kernel(const __grid_constant__ Params p) {
   __shared__ float red[BWD ? kWarps * 256 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool isk = blockIdx.x >= (unsigned)p.s[0].blocks;
@@ -237,26 +281,29 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const __grid_constant__ 
   const int blk = (int)blockIdx.x - (isk ? p.s[0].blocks : 0);
   pdl_wait();
   pdl_trigger();
-  const int d0 = (lane % p.lph) * 8;
-  float w[8], dw[8];
+  const int d0 = (lane % LPH) * 8;
+  float2 w[4], dw[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 1.0f, dw[i] = 0.0f;
-  if (sd.w && d0 < p.D) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = sd.w[d0 + i];
+  for (int i = 0; i < 4; ++i) {
+    w[i] = make_float2(1.0f, 1.0f), dw[i] = make_float2(0.0f, 0.0f);
+    if (sd.w && d0 < p.D) w[i] = make_float2(sd.w[d0 + 2 * i], sd.w[d0 + 2 * i + 1]);
   }
   for (int64_t task = (int64_t)blk * kWarps + warp; task < sd.tasks; task += (int64_t)sd.blocks * kWarps)
-    token<T, BWD>(p, sd, (uint32_t)task, lane, w, dw);
+    token<T, LPH, INTER, BWD>(p, sd, (uint32_t)task, lane, w, dw);
   if constexpr (BWD) {
     if (sd.partial) {
       // the warp's heads, then the block's warps, both in a fixed order
-      for (int o = p.lph; o < 32; o <<= 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
+      for (int o = LPH; o < 32; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          dw[i].x += __shfl_xor_sync(0xffffffffu, dw[i].x, o);
+          dw[i].y += __shfl_xor_sync(0xffffffffu, dw[i].y, o);
+        }
       }
-      if (lane < p.lph && d0 < p.D) {
+      if (lane < LPH && d0 < p.D) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) red[warp * 256 + d0 + i] = dw[i];
+        for (int i = 0; i < 4; ++i) red[warp * 256 + d0 + 2 * i] = dw[i].x, red[warp * 256 + d0 + 2 * i + 1] = dw[i].y;
       }
       __syncthreads();
       for (int d = threadIdx.x; d < p.D; d += kThreads) {
@@ -289,16 +336,9 @@ __global__ void __launch_bounds__(1024) dw_kernel(const __grid_constant__ Params
 }
 
 int lanes_per_head(int D) {
-  int l = 1;
+  int l = 4;
   while (l * 8 < D) l <<= 1;
   return l;
-}
-
-// Backward blocks of one side: bounded so that the column sums' second stage
-// stays short.
-int bwd_blocks(int64_t tasks) {
-  const int64_t want = (tasks + kWarps - 1) / kWarps, most = (int64_t)num_sms() * 4;
-  return (int)(want < most ? want : most);
 }
 
 bool aligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -327,6 +367,24 @@ int check(const hclsm_rope_side* s, int64_t B, int P, int rot, bool bwd) {
   return HCLSM_OK;
 }
 
+template <typename T, int LPH>
+int launch(const Params& p, int grid, bool inter, bool bwd, cudaStream_t st) {
+  if (bwd)
+    return inter ? launch_pdl(rope_kernel<T, LPH, true, true>, grid, kThreads, 0, st, p)
+                 : launch_pdl(rope_kernel<T, LPH, false, true>, grid, kThreads, 0, st, p);
+  return inter ? launch_pdl(rope_kernel<T, LPH, true, false>, grid, kThreads, 0, st, p)
+               : launch_pdl(rope_kernel<T, LPH, false, false>, grid, kThreads, 0, st, p);
+}
+template <typename T>
+int launch(const Params& p, int grid, bool inter, bool bwd, cudaStream_t st) {
+  switch (p.lph) {
+    case 4: return launch<T, 4>(p, grid, inter, bwd, st);
+    case 8: return launch<T, 8>(p, grid, inter, bwd, st);
+    case 16: return launch<T, 16>(p, grid, inter, bwd, st);
+    default: return launch<T, 32>(p, grid, inter, bwd, st);
+  }
+}
+
 int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, const float* sinv, int P, int rot,
         int64_t B, int D, float eps, int dtype, int flags, bool bwd, void* ws, size_t ws_bytes, void* stream) {
   if (dtype != HCLSM_F32 && dtype != HCLSM_BF16) return HCLSM_ERR_DTYPE;
@@ -352,7 +410,20 @@ int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, c
     s.L = in[i]->L, s.H = in[i]->H;
     if (B * s.L > 0) plan(s, B, p.lph);
     if (s.tasks > 0x7fffffff) return HCLSM_ERR_SHAPE;
-    s.blocks = bwd ? bwd_blocks(s.tasks) : (int)((s.tasks + kWarps - 1) / kWarps);
+    s.blocks = (int)((s.tasks + kWarps - 1) / kWarps);
+  }
+  if (bwd) {  // as many blocks as are resident, shared out by the heads of the two sides
+    const int most = num_sms() * kBwdPerSm;
+    const double work[2] = {(double)B * p.s[0].L * p.s[0].H, (double)B * p.s[1].L * p.s[1].H};
+    int share = (int)(most * (work[1] / (work[0] + work[1] + 1e-9)) + 0.5);
+    if (share < 1) share = 1;
+    if (share > most - 1) share = most - 1;
+    if (p.s[1].blocks > share) p.s[1].blocks = share;
+    if (p.s[0].blocks > most - share) p.s[0].blocks = most - share;
+  }
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.s[i];
+    if (!in[i]) continue;
     if (bwd && in[i]->dw) {
       const size_t need = (size_t)s.blocks * D * sizeof(float);
       const size_t used = i ? (p.s[0].partial ? (size_t)p.s[0].blocks * D * sizeof(float) : 0) : 0;
@@ -371,13 +442,7 @@ int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, c
   if (grid == 0) return HCLSM_OK;
   p.cosv = cosv, p.sinv = sinv, p.P = P, p.rot = rot, p.D = D, p.eps = eps, p.norm = norm, p.inter = inter;
   p.err = device_err_ptr();
-  int rc;
-  if (dtype == HCLSM_F32)
-    rc = bwd ? launch_pdl(rope_kernel<float, true>, grid, kThreads, 0, st, p)
-             : launch_pdl(rope_kernel<float, false>, grid, kThreads, 0, st, p);
-  else
-    rc = bwd ? launch_pdl(rope_kernel<__nv_bfloat16, true>, grid, kThreads, 0, st, p)
-             : launch_pdl(rope_kernel<__nv_bfloat16, false>, grid, kThreads, 0, st, p);
+  const int rc = dtype == HCLSM_F32 ? launch<float>(p, grid, inter, bwd, st) : launch<__nv_bfloat16>(p, grid, inter, bwd, st);
   if (rc != HCLSM_OK || (!p.s[0].partial && !p.s[1].partial)) return rc;
   return launch_pdl(dw_kernel, 2, 1024, 0, st, p);
 }
@@ -393,7 +458,7 @@ extern "C" int hclsm_qk_norm_rope(const hclsm_rope_side* q, const hclsm_rope_sid
 
 extern "C" size_t hclsm_qk_norm_rope_bwd_workspace_size(int32_t D) {
   if (D < 8 || D > 256) return 0;
-  return (size_t)2 * 4 * hclsm::num_sms() * D * sizeof(float);
+  return ((size_t)hclsm::num_sms() * hclsm::rope::kBwdPerSm) * D * sizeof(float);
 }
 
 extern "C" int hclsm_qk_norm_rope_bwd(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv,
