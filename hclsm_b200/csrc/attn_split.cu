@@ -9,15 +9,20 @@
 // A contraction's index can run in any order, so fragments come straight from
 // global memory with 16-byte loads and no shared memory: for S a lane's four k
 // slots are four consecutive dims of its key's row; for P V a lane holds
-// consecutive dims of the four keys whose scores it has.  8-bit integers become
-// bf16 exactly, two at a time: 0x4300 | low 7 bits is 128 + those bits, and
-// 0x4300 | sign is 128, or 256 for a negative value, so one packed subtraction
-// gives the value.  The scale of a block of keys multiplies its scores (K) and
-// its weights (V).
+// consecutive dims of the four keys whose scores it has.
+// 8-bit integers become fp16 two at a time: 0x6400 | (x + 128) is 1152 + x.  For K
+// the 1152 stays in: S is off by 1152 times the row's sum of q, one subtraction a
+// score.  For V it is taken off (the sum over a long history would lose the
+// difference).  Queries are scaled by a power of two to a largest value below 1, and
+// the weights to at most 2^12, both exact, for fp16's range; with 11 bits they carry
+// less rounding than bf16's 8.  The scale of a block of keys multiplies its scores
+// (K); that of its values, over the largest so far, its weights (V).
 // fp32 operands are split into three bf16 pieces (8 bits each) and the products
 // of pieces whose order is at most 2 are summed: fp32 accuracy.
 // Bound: HBM (each key and value byte is read once); splits and warps are merged
 // in a fixed order.
+#include <cuda_fp16.h>
+
 #include <type_traits>
 
 #include "xattn.cuh"
@@ -28,6 +33,7 @@ namespace split {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;
+constexpr int kWaves = 4, kMinKeys = 1024;
 
 struct Params {
   xattn::Params x;  // q, o, lse2, lens, mask, sizes; k and v where the states are dense
@@ -40,12 +46,20 @@ struct Params {
   float2* part_ml; // (B * Hkv * rtiles, splits, 16): max, sum
 };
 
+template <bool F16>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
-      "%2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+        "%2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -61,8 +75,19 @@ __device__ __forceinline__ void pieces(float lo, float hi, uint32_t (&out)[N]) {
     hi -= __uint_as_float(out[i] & 0xffff0000u);
   }
 }
-// Two signed bytes (bits 0-7 and 16-23; the others are ignored) as packed bf16.
-__device__ __forceinline__ uint32_t bytes2(uint32_t t) {
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two signed bytes (bits 0-7 and 16-23; the others are ignored): 1152 + x as packed fp16, and x as packed bf16
+// (0x4300 | low 7 bits is 128 + those bits, 0x4300 | sign 128, or 256 for a negative value).
+__device__ __forceinline__ uint32_t bytes_f16(uint32_t t) { return (t & 0x00ff00ffu) ^ 0x64806480u; }
+__device__ __forceinline__ uint32_t minus1152(uint32_t t) {
+  const uint32_t k = 0x64806480u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t bytes_bf16(uint32_t t) {
   const uint32_t m = (t & 0x007f007fu) | 0x43004300u, s = (t & 0x00800080u) | 0x43004300u;
   const __nv_bfloat162 r =
       __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&s));
@@ -116,12 +141,17 @@ struct Rows {
   // the dim of lane group g's element j
   static __device__ __forceinline__ int v_dim(int j, int g) { return j / CV * 8 * CV + g * CV + j % CV; }
 
-  // B fragments of k step s
+  // B fragments of k step s (F16: 1152 + x)
+  template <bool F16>
   static __device__ __forceinline__ void k_frag(const uint32_t (&w)[kKW], int s, uint32_t (&b0)[kPieces],
                                                 uint32_t (&b1)[kPieces]) {
     if constexpr (kES == 1) {
-      b0[0] = bytes2(__byte_perm(w[s], 0, 0x0100));
-      b1[0] = bytes2(__byte_perm(w[s], 0, 0x0302));
+      if constexpr (F16) {
+        const uint32_t u = w[s] ^ 0x80808080u;
+        b0[0] = __byte_perm(u, 0x64646464u, 0x4140), b1[0] = __byte_perm(u, 0x64646464u, 0x4342);
+      } else {
+        b0[0] = bytes_bf16(__byte_perm(w[s], 0, 0x0100)), b1[0] = bytes_bf16(__byte_perm(w[s], 0, 0x0302));
+      }
     } else if constexpr (kES == 2) {
       b0[0] = w[2 * s], b1[0] = w[2 * s + 1];
     } else {
@@ -130,12 +160,14 @@ struct Rows {
     }
   }
   // B fragments of n tile j from the rows of the lane's four keys
+  template <bool F16>
   static __device__ __forceinline__ void v_frag(const uint32_t (&w)[4][kVW], int j, uint32_t (&b0)[kPieces],
                                                 uint32_t (&b1)[kPieces]) {
     if constexpr (kES == 1) {
       const uint32_t sel = (j & 3) | ((4 + (j & 3)) << 8);  // byte j of the first word, of the second at bit 16
-      b0[0] = bytes2(__byte_perm(w[0][j / 4], w[1][j / 4], sel));
-      b1[0] = bytes2(__byte_perm(w[2][j / 4], w[3][j / 4], sel));
+      const uint32_t t0 = __byte_perm(w[0][j / 4], w[1][j / 4], sel), t1 = __byte_perm(w[2][j / 4], w[3][j / 4], sel);
+      b0[0] = F16 ? minus1152(bytes_f16(t0)) : bytes_bf16(t0);
+      b1[0] = F16 ? minus1152(bytes_f16(t1)) : bytes_bf16(t1);
     } else if constexpr (kES == 2) {
       const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
       b0[0] = __byte_perm(w[0][j / 2], w[1][j / 2], sel);
@@ -154,33 +186,56 @@ struct State {
   float m[2], l[2];
 };
 
-// Queries of the tile in shared memory as fp32 [16][D + 4] (rows past the end are zeros).
-template <typename T, int D, int NQ, typename R>
-__device__ __forceinline__ void q_frag(const float* sq, int s, int g, int c, uint32_t (&a)[NQ][4]) {
-  const int d = R::k_dim(s, c);
-  const float4 x = *reinterpret_cast<const float4*>(sq + g * (D + 4) + d);
-  const float4 y = *reinterpret_cast<const float4*>(sq + (g + 8) * (D + 4) + d);
-  uint32_t t[NQ];
-  pieces<NQ>(x.x, x.y, t);
+// Blocks an SM: what the registers of a row's accumulators and one step's keys and values leave room for.
+template <typename T, int D> constexpr int kPerSm = sizeof(T) == 4 ? (D <= 64 ? 3 : 2) : (D <= 64 ? 4 : 3);
+
+// The A fragments of all k steps and pieces, as each lane reads them: [k step][piece][lane][2 NR words].
+template <int D, int NQ, int NR> constexpr int frag_words() { return D / 16 * NQ * 32 * 2 * NR; }
+
+// Packs them from fp32 queries [16][D + 4] (rows past the end are zeros); warps take k steps in turn.
+template <int D, int NQ, int NR, bool F16, typename R>
+__device__ __forceinline__ void pack_q(uint32_t* qf, const float* sq, const float* inv, int warp, int g, int c) {
+  for (int s = warp; s < D / 16; s += kWarps) {
+    const int d = R::k_dim(s, c);
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) a[i][0] = t[i];
-  pieces<NQ>(y.x, y.y, t);
+    for (int r = 0; r < NR; ++r) {
+      const float4 x = *reinterpret_cast<const float4*>(sq + (g + 8 * r) * (D + 4) + d);
+      uint32_t lo[NQ], hi[NQ];
+      if constexpr (F16) {
+        const float f = inv[g + 8 * r];
+        lo[0] = pack_f16(x.x * f, x.y * f), hi[0] = pack_f16(x.z * f, x.w * f);
+      } else {
+        pieces<NQ>(x.x, x.y, lo);
+        pieces<NQ>(x.z, x.w, hi);
+      }
 #pragma unroll
-  for (int i = 0; i < NQ; ++i) a[i][1] = t[i];
-  pieces<NQ>(x.z, x.w, t);
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) a[i][2] = t[i];
-  pieces<NQ>(y.z, y.w, t);
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) a[i][3] = t[i];
+      for (int i = 0; i < NQ; ++i) {  // words: (row g, low k), (row g, high k), then row g + 8
+        uint32_t* w = qf + ((s * NQ + i) * 32 + g * 4 + c) * 2 * NR + 2 * r;
+        w[0] = lo[i], w[1] = hi[i];
+      }
+    }
+  }
+}
+template <int NR>
+__device__ __forceinline__ void load_a(const uint32_t* w, uint32_t (&a)[4]) {
+  if constexpr (NR == 1) {
+    const uint2 v = *reinterpret_cast<const uint2*>(w);
+    a[0] = v.x, a[1] = 0, a[2] = v.y, a[3] = 0;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(w);
+    a[0] = v.x, a[1] = v.z, a[2] = v.y, a[3] = v.w;
+  }
 }
 
+// NR 1: at most 8 rows, so rows g + 8 are padding that takes no softmax.
 // Steps first, first + stride, ... below last of 16 keys each.  addr_k / addr_v
 // (key) give a row's address; ok(key) says whether the key is allowed (false
 // past the end); nk > 0 keys have memory; all_ok(step) skips the per-key checks.
-template <typename T, typename E, int D, int CV, int NQ, typename AddrK, typename AddrV, typename Ok, typename AllOk,
-          typename Scale>
-__device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, int last, int stride, int nk, float c2,
+// fs, off: factor and offset of rows g and g + 8's raw scores.
+template <typename E, int D, int CV, int NQ, int NR, bool F16, typename AddrK, typename AddrV, typename Ok,
+          typename AllOk, typename Scale>
+__device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const float (&fs)[2], const float (&off)[2],
+                                      int first, int last, int stride, int nk,
                                       AddrK addr_k, AddrV addr_v, Ok ok, AllOk all_ok, Scale scale) {
   using R = Rows<E, D, CV>;
   constexpr int NK = R::kPieces, kOrder = (NQ > NK ? NQ : NK) - 1;
@@ -195,6 +250,7 @@ __device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, 
 #pragma unroll
     for (int t = 0; t < 4; ++t) R::load_v(addr_v(min(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1), nk - 1)), g, vr[t]);
   };
+  float vref = 0.0f;  // F16: the largest value scale so far; O is held over it, times 2^12
   float2 sc = scale(first);
   fetch_k(first);
   fetch_v(first);
@@ -204,16 +260,17 @@ __device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, 
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
       uint32_t a[NQ][4];
-      q_frag<T, D, NQ, R>(sq, ks, g, c, a);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) load_a<NR>(qf + ((ks * NQ + i) * 32 + lane) * 2 * NR, a[i]);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         uint32_t b0[NK], b1[NK];
-        R::k_frag(kr[t], ks, b0, b1);
+        R::template k_frag<F16>(kr[t], ks, b0, b1);
 #pragma unroll
         for (int i = NQ - 1; i >= 0; --i)
 #pragma unroll
           for (int j = NK - 1; j >= 0; --j)
-            if (i + j <= kOrder) mma(s[t], a[i], b0[j], b1[j]);
+            if (i + j <= kOrder) mma<F16>(s[t], a[i], b0[j], b1[j]);
       }
     }
     const float2 cur = sc;
@@ -226,23 +283,24 @@ __device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, 
 #pragma unroll
       for (int t = 0; t < 4; ++t) good[t] = ok(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1));
     }
-    const float f = c2 * cur.x;
+    const float f[2] = {fs[0] * cur.x, fs[1] * cur.x};
     float mx[2] = {st.m[0], st.m[1]};
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[t][e] = good[2 * t + (e & 1)] ? s[t][e] * f : -INFINITY;
+      for (int e = 0; e < 2 * NR; ++e) {
+        if constexpr (F16) s[t][e] -= off[e >> 1];
+        s[t][e] = good[2 * t + (e & 1)] ? s[t][e] * f[e >> 1] : -INFINITY;
         mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
       }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < NR; ++r) {
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
     if (__any_sync(0xffffffffu, mx[0] != st.m[0] || mx[1] != st.m[1])) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
+      for (int r = 0; r < NR; ++r) {
         const float w = mx[r] == -INFINITY ? 1.0f : ex2(st.m[r] - mx[r]);
         st.m[r] = mx[r];
         st.l[r] *= w;
@@ -250,21 +308,39 @@ __device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, 
         for (int j = 0; j < D / 8; ++j) st.o[j][2 * r] *= w, st.o[j][2 * r + 1] *= w;
       }
     }
+    float pv = cur.y;
+    if constexpr (F16) {
+      if (cur.y > vref) {  // the same for the whole warp
+        const float w = vref / cur.y;
+        vref = cur.y;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
+      }
+      pv = cur.y > 0.0f ? cur.y / vref * 4096.0f : cur.y;  // 0 or NaN stay
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
+        if (e >= 2 * NR) {
+          s[t][e] = 0.0f;
+          continue;
+        }
         const float base = st.m[e >> 1] == -INFINITY ? 0.0f : st.m[e >> 1];
         s[t][e] = ex2(s[t][e] - base);
         st.l[e >> 1] += s[t][e];
-        s[t][e] *= cur.y;
+        s[t][e] *= pv;
         if (!all && !good[2 * t + (e & 1)]) s[t][e] = 0.0f;
       }
     uint32_t pa[NQ][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      const float lo = s[k >> 1][2 * (k & 1)], hi = s[k >> 1][2 * (k & 1) + 1];
       uint32_t t[NQ];
-      pieces<NQ>(s[k >> 1][2 * (k & 1)], s[k >> 1][2 * (k & 1) + 1], t);
+      if constexpr (F16) t[0] = pack_f16(lo, hi);
+      else pieces<NQ>(lo, hi, t);
 #pragma unroll
       for (int i = 0; i < NQ; ++i) pa[i][k] = t[i];
     }
@@ -279,22 +355,31 @@ __device__ __forceinline__ void sweep(State<D>& st, const float* sq, int first, 
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
       uint32_t b0[NK], b1[NK];
-      R::v_frag(vr, j, b0, b1);
+      R::template v_frag<F16>(vr, j, b0, b1);
 #pragma unroll
       for (int i = NQ - 1; i >= 0; --i)
 #pragma unroll
         for (int k = NK - 1; k >= 0; --k)
-          if (i + k <= kOrder) mma(st.o[j], pa[i], b0[k], b1[k]);
+          if (i + k <= kOrder) mma<F16>(st.o[j], pa[i], b0[k], b1[k]);
     }
     fetch_v(next);
   }
+  if constexpr (F16) {
+    const float w = vref * (1.0f / 4096.0f);
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
+  }
 }
 
-template <typename T, int D, bool CACHE>
-__global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__ Params p) {
+template <typename T, int D, bool CACHE, int NR>
+__global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __grid_constant__ Params p) {
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;
   constexpr int ES = CACHE ? 1 : (int)sizeof(T), CV = load_bytes(D / 8 * ES) / ES;
-  extern __shared__ float smem[];  // [16][D + 4] queries, then (merge) [kWarps][16][D]
+  constexpr bool F16 = CACHE && NQ == 1;
+  extern __shared__ float smem[];  // [16][D + 4] queries and the A fragments, then (merge) [kWarps][16][D]
+  __shared__ float s_inv[kRows], s_sum[kRows];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   pdl_wait();
@@ -317,6 +402,33 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
     sq[i / D * (D + 4) + d] = v;
   }
   __syncthreads();
+  uint32_t* qf = reinterpret_cast<uint32_t*>(sq + kRows * (D + 4));  // as the sweep over dense states reads them
+  uint32_t* qh = qf + frag_words<D, NQ, NR>();                       // fp16, for the 8-bit blocks
+  using RT = Rows<T, D, CV>;
+  if constexpr (F16) {  // each row times a power of two, to a largest value in [1/2, 1), and its sum
+    for (int r = warp; r < kRows; r += kWarps) {
+      float m = 0.0f;
+      for (int d = lane; d < D; d += 32) m = fmaxf(m, fabsf(sq[r * (D + 4) + d]));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const int e = min(max((int)(__float_as_uint(m) >> 23) - 126, -126), 126);
+      const float f = m == 0.0f ? 1.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+      float sum = 0.0f;
+      for (int d = lane; d < D; d += 32) sum += __half2float(__float2half_rn(sq[r * (D + 4) + d] * f));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_inv[r] = f, s_sum[r] = sum;
+    }
+    __syncthreads();
+    pack_q<D, 1, NR, true, Rows<int8_t, D, CV>>(qh, sq, s_inv, warp, g, c);
+    pack_q<D, 1, NR, false, RT>(qf, sq, s_inv, warp, g, c);
+  } else if constexpr (CACHE) {
+    pack_q<D, NQ, NR, false, Rows<int8_t, D, CV>>(qh, sq, s_inv, warp, g, c);
+    pack_q<D, NQ, NR, false, RT>(qf, sq, s_inv, warp, g, c);
+  } else {
+    pack_q<D, NQ, NR, false, RT>(qf, sq, s_inv, warp, g, c);
+  }
+  __syncthreads();
   State<D> st;
 #pragma unroll
   for (int j = 0; j < D / 8; ++j)
@@ -325,6 +437,7 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
   st.m[0] = st.m[1] = -INFINITY;
   st.l[0] = st.l[1] = 0.0f;
   const float c2 = p.x.scale * kLog2e;
+  const float fs[2] = {c2, c2}, off[2] = {0.0f, 0.0f};
   // this block's share of the sequence's own steps
   const int n8 = CACHE ? n / p.block * p.block : n;
   const int steps = (n8 + 15) / 16, per = (steps + p.splits - 1) / p.splits;
@@ -334,16 +447,21 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
     const char* v8 = reinterpret_cast<const char*>(p.v8) + bh * p.T * D;
     const int64_t s0 = bh * (p.T / p.block);
     const int spb = p.block / 16;
-    sweep<T, int8_t, D, CV, NQ>(
-        st, sq, first + warp, last, kWarps, n8, c2, [&](int j) { return k8 + (int64_t)j * D; },
+    float fs8[2] = {c2, c2}, off8[2] = {0.0f, 0.0f};
+    if constexpr (F16) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) fs8[r] = c2 / s_inv[g + 8 * r], off8[r] = 1152.0f * s_sum[g + 8 * r];
+    }
+    sweep<int8_t, D, CV, NQ, NR, F16>(
+        st, qh, fs8, off8, first + warp, last, kWarps, n8, [&](int j) { return k8 + (int64_t)j * D; },
         [&](int j) { return v8 + (int64_t)j * D; }, [](int) { return true; }, [](int) { return true; },
         [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); });
   } else {
     const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);
     const char* vb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.v.p) + b * p.x.v.sb + hk * p.x.v.sh);
     const int64_t kst = p.x.k.st * (int64_t)sizeof(T), vst = p.x.v.st * (int64_t)sizeof(T);
-    sweep<T, T, D, CV, NQ>(
-        st, sq, first + warp, last, kWarps, n, c2, [&](int j) { return kb + j * kst; },
+    sweep<T, D, CV, NQ, NR, false>(
+        st, qf, fs, off, first + warp, last, kWarps, n, [&](int j) { return kb + j * kst; },
         [&](int j) { return vb + j * vst; }, [&](int j) { return xattn::key_ok(p.x, b, n, j); },
         [&](int step) { return !p.x.mask && step * 16 + 16 <= n; }, [](int) { return make_float2(1.0f, 1.0f); });
   }
@@ -352,8 +470,8 @@ __global__ void __launch_bounds__(kThreads) split_kernel(const __grid_constant__
       const char* kt = reinterpret_cast<const char*>(static_cast<const T*>(p.kt) + bh * p.block * D);
       const char* vt = reinterpret_cast<const char*>(static_cast<const T*>(p.vt) + bh * p.block * D);
       const int nt = n - n8;
-      sweep<T, T, D, CV, NQ>(
-          st, sq, warp, (nt + 15) / 16, kWarps, nt, c2, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
+      sweep<T, D, CV, NQ, NR, false>(
+          st, qf, fs, off, warp, (nt + 15) / 16, kWarps, nt, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
           [&](int j) { return vt + j * (int)(D * sizeof(T)); }, [&](int j) { return j < nt; },
           [&](int step) { return step * 16 + 16 <= nt; }, [](int) { return make_float2(1.0f, 1.0f); });
     }
@@ -440,14 +558,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   if (p.x.lse2 && lane == 0) p.x.lse2[(b * p.x.H + h) * p.x.Lq + row / G] = l == 0.0f ? INFINITY : m + log2f(l);
 }
 
-// Splits so that about four blocks an SM are in flight, and none shorter than
-// 256 keys (a split writes 16 rows of fp32, as many bytes as 32 to 64 of its keys).
-void plan(Params& p, int keys) {
+// Whole waves of resident blocks.  Sequences have their own lengths and a block's
+// share is its own sequence's, so more waves even the blocks out, down to 1024 keys a
+// block (a block writes up to 16 rows of fp32 for the join).
+void plan(Params& p, int keys, int dtype) {
   const int64_t rows = (int64_t)p.x.Lq * (p.x.H / p.x.Hkv);
   p.rtiles = (int)((rows + kRows - 1) / kRows);
-  const int64_t base = (int64_t)p.x.B * p.x.Hkv * p.rtiles, want = (int64_t)num_sms() * 4;
-  int64_t s = base > 0 ? (want + base - 1) / base : 1;
-  const int64_t most = (keys + 255) / 256;
+  const int64_t base = (int64_t)p.x.B * p.x.Hkv * p.rtiles;
+  const int per_sm = dtype == HCLSM_F32 ? (p.x.D <= 64 ? 3 : 2) : (p.x.D <= 64 ? 4 : 3);
+  int64_t s = 1;
+  for (int waves = 1; waves <= kWaves; ++waves) {
+    const int64_t n = base > 0 ? (int64_t)num_sms() * per_sm * waves / base : 1;
+    if (n > 1 && (waves == 1 || keys / n >= kMinKeys)) s = n;
+  }
+  const int64_t most = (keys + 127) / 128;
   if (s > most) s = most;
   p.splits = s < 1 ? 1 : (int)s;
 }
@@ -467,8 +591,13 @@ int launch(Params& p, void* ws, cudaStream_t st) {
     p.part_ml = static_cast<float2*>(ws);
     p.part_o = reinterpret_cast<float*>(p.part_ml + grid * kRows);
   }
-  constexpr size_t smem = (size_t)kWarps * kRows * D * sizeof(float) + kRows * 16;
-  auto f = split_kernel<T, D, CACHE>;
+  const bool rows1 = (int64_t)p.x.Lq * (p.x.H / p.x.Hkv) <= 8;
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1;
+  const size_t merge = (size_t)kWarps * kRows * D * sizeof(float);
+  const size_t front = (size_t)kRows * (D + 4) * sizeof(float) +
+                       (size_t)(CACHE ? 2 : 1) * 4 * (rows1 ? frag_words<D, NQ, 1>() : frag_words<D, NQ, 2>());
+  const size_t smem = merge > front ? merge : front;
+  auto f = rows1 ? split_kernel<T, D, CACHE, 1> : split_kernel<T, D, CACHE, 2>;
   if (!set_smem_limit(reinterpret_cast<const void*>(f), smem)) return HCLSM_ERR_LAUNCH;
   if (const int rc = launch_pdl(f, (unsigned)grid, kThreads, smem, st, p)) return rc;
   if (p.splits <= 1) return HCLSM_OK;
@@ -491,16 +620,16 @@ int run(Params& p, int dtype, void* ws, cudaStream_t st) {
 
 namespace xattn {
 // The cross attention's forward in this form; 16-byte aligned rows of k and v, D 32, 64, 96 or 128.
-size_t split_workspace(const Params& x) {
+size_t split_workspace(const Params& x, int dtype) {
   split::Params p = {};
   p.x = x;
-  split::plan(p, x.Lk);
+  split::plan(p, x.Lk, dtype);
   return split::workspace(p);
 }
 int split_fwd(const Params& x, int dtype, void* ws, cudaStream_t st) {
   split::Params p = {};
   p.x = x;
-  split::plan(p, x.Lk);
+  split::plan(p, x.Lk, dtype);
   return split::run<false>(p, dtype, ws, st);
 }
 }  // namespace xattn
@@ -509,7 +638,7 @@ namespace kv8 {
 size_t attn_workspace(const hclsm_kv8_cache* c, int Lq, int H) {
   split::Params p = {};
   p.x.B = c->B, p.x.Lq = Lq, p.x.H = H, p.x.Hkv = c->Hkv, p.x.D = c->D;
-  split::plan(p, c->T);
+  split::plan(p, c->T, c->dtype);
   return split::workspace(p);
 }
 int attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens, int Lq, int H, float scale,
@@ -520,7 +649,7 @@ int attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* 
   p.x.B = c->B, p.x.Lq = Lq, p.x.H = H, p.x.Hkv = c->Hkv, p.x.D = c->D;
   p.k8 = c->k, p.v8 = c->v, p.ks = c->k_scale, p.vs = c->v_scale, p.kt = c->k_tail, p.vt = c->v_tail;
   p.T = c->T, p.block = c->block;
-  split::plan(p, c->T);
+  split::plan(p, c->T, c->dtype);
   return split::run<true>(p, c->dtype, ws, st);
 }
 }  // namespace kv8

@@ -360,7 +360,7 @@ static bool use_split(const xattn::Params& p, int dtype) {
 extern "C" size_t hclsm_xattn_fwd_workspace_size(const hclsm_xattn_args* a) {
   if (xattn::check(a)) return 0;
   const xattn::Params p = xattn::params(a);
-  if (use_split(p, a->dtype)) return xattn::split_workspace(p);
+  if (use_split(p, a->dtype)) return xattn::split_workspace(p, a->dtype);
   return a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false) ? xattn::tc_workspace(p) : 0;
 }
 
@@ -371,7 +371,7 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   const xattn::Params p = xattn::params(a);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (use_split(p, a->dtype)) {
-    const size_t need = xattn::split_workspace(p);
+    const size_t need = xattn::split_workspace(p, a->dtype);
     if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
     return xattn::split_fwd(p, a->dtype, ws, st);
   }

@@ -54,7 +54,7 @@ size_t tc_workspace(const Params& p);
 int tc_fwd(const Params& p, void* ws, cudaStream_t st);
 int tc_bwd(const Params& p, void* ws, cudaStream_t st);
 // Few query rows, the keys split over blocks (attn_split.cu).
-size_t split_workspace(const Params& p);
+size_t split_workspace(const Params& p, int dtype);
 int split_fwd(const Params& p, int dtype, void* ws, cudaStream_t st);
 
 }  // namespace xattn
