@@ -8,8 +8,7 @@
 // again when later tokens raise the block's maximum.  A block with a value that is
 // not finite gets a NaN scale: what is read from it is NaN, not a wrong number.
 //
-// Both kernels move every byte once (writing re-reads a block from L1 after its
-// maximum): the bound is HBM, at small sizes the launch.
+// Both kernels move every byte once: the bound is HBM, at small sizes the launch.
 #include "xattn.cuh"
 
 namespace hclsm {
@@ -28,53 +27,86 @@ struct Params {
   int* err;
 };
 
-template <typename T>
-__device__ __forceinline__ void ld8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 r = *reinterpret_cast<const uint4*>(p);
+// 8 elements as loaded, and as fp32.
+template <typename T> struct Raw;
+template <> struct Raw<__nv_bfloat16> {
+  uint4 r;
+  __device__ __forceinline__ void ld(const __nv_bfloat16* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void st(__nv_bfloat16* p) const { *reinterpret_cast<uint4*>(p) = r; }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = __uint_as_float(w[i] << 16);
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-  } else {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   }
-}
-template <typename T>
-__device__ __forceinline__ void st8(T* p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
+  __device__ __forceinline__ void set(const float (&v)[8]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    r = make_uint4(w[0], w[1], w[2], w[3]);
   }
+};
+template <> struct Raw<float> {
+  float4 a, b;
+  __device__ __forceinline__ void ld(const float* p) {
+    a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void st(float* p) const {
+    *reinterpret_cast<float4*>(p) = a, *reinterpret_cast<float4*>(p + 4) = b;
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  }
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
+  }
+};
+
+// The largest |x|; INFINITY for a value that is not finite, and it stays.
+__device__ __forceinline__ float largest(float m, const float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float a = fabsf(v[e]);
+    m = a <= 3.402823466e38f ? fmaxf(m, a) : INFINITY;
+  }
+  return m;
+}
+// 8 values over the scale, to the nearest integer (half to even); zeros where the scale is zero or NaN.
+__device__ __forceinline__ uint2 eight(const float (&v)[8], float s) {
+  uint32_t w[2] = {0, 0};
+  if (s > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // |x / scale| can round past 127 where the scale is subnormal
+      w[e >> 2] |= (uint32_t)(min(max(__float2int_rn(__fdiv_rn(v[e], s)), -127), 127) & 0xff) << (8 * (e & 3));
+  }
+  return make_uint2(w[0], w[1]);
 }
 
-// One block of threads a touched cache block and head, blockIdx.y keys or values.
-// The first one of a sequence also writes the tail, after it has read it.
+// One warp a touched cache block of a head, keys or values: no barrier, and a block of
+// up to 32 x 64 stays in registers between its maximum and its rounding.  The first
+// one of a sequence also writes the tail, after it has read it.
+constexpr int kHeld = 8;  // vectors of 8 a lane holds
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Params p) {
-  __shared__ float red[kThreads / 32];
-  __shared__ float s_max;
   pdl_wait();
   pdl_trigger();
-  const int j = (int)(blockIdx.x % p.touched);
-  const int64_t bh = blockIdx.x / p.touched;
+  const int lane = threadIdx.x & 31, kv = blockIdx.y;
+  const int64_t task = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t bh = task / p.touched;
+  const int j = (int)(task - bh * p.touched);
   const int64_t b = bh / p.Hkv;
-  const int hk = (int)(bh % p.Hkv), kv = blockIdx.y;
+  const int hk = (int)(bh - b * p.Hkv);
+  if (b >= p.B) return;
   const int start = p.start[b], count = p.count ? p.count[b] : p.n;
   // a request outside the cache or the new tokens writes nothing
   if (start < 0 || count < 0 || count > p.n || start > p.T - count) {
-    if (threadIdx.x == 0) record_error(p.err, HCLSM_ERR_SHAPE);
+    if (lane == 0) record_error(p.err, HCLSM_ERR_SHAPE);
     return;
   }
   if (count == 0) return;
@@ -84,83 +116,98 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
   const xattn::View& xv = p.x[kv];
   const T* x = static_cast<const T*>(xv.p) + b * xv.sb + hk * xv.sh;
   T* tail = static_cast<T*>(p.tail[kv]) + bh * block * D;
-  auto row = [&](int tok) { return tok >= start ? x + (int64_t)(tok - start) * xv.st : tail + (tok % block) * D; };
+  auto at = [&](int i) {  // vector i of the cache block: among the new tokens, or in the tail
+    const int tok = blk * block + i * 8 / D, d = i * 8 % D;
+    return tok >= start ? x + (int64_t)(tok - start) * xv.st + d : tail + (tok % block) * D + d;
+  };
   if ((blk + 1) * block <= end) {
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < vecs; i += kThreads) {
-      float v[8];
-      ld8(row(blk * block + i * 8 / D) + i * 8 % D, v);
+    float m = 0.0f, v[8];
+    Raw<T> r[kHeld];
+    const bool held = vecs <= 32 * kHeld;
+    if (held) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float a = fabsf(v[e]);
-        m = a <= 3.402823466e38f ? fmaxf(m, a) : INFINITY;  // INFINITY stays: fmaxf(inf, a) = inf
+      for (int k = 0; k < kHeld; ++k)
+        if (k * 32 + lane < vecs) r[k].ld(at(k * 32 + lane));
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if (k * 32 + lane < vecs) {
+          r[k].get(v);
+          m = largest(m, v);
+        }
+    } else {
+#pragma unroll 4
+      for (int i = lane; i < vecs; i += 32) {
+        Raw<T> t;
+        t.ld(at(i));
+        t.get(v);
+        m = largest(m, v);
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < kThreads / 32; ++w) m = fmaxf(m, red[w]);
-      const float s = m == INFINITY ? __int_as_float(0x7fc00000) : __fdiv_rn(m, 127.0f);
-      s_max = s;
-      p.scale[kv][bh * (p.T / block) + blk] = s;
-    }
-    __syncthreads();
-    const float s = s_max;
-    const bool fine = s > 0.0f;  // neither zero nor NaN
+    const float s = m == INFINITY ? __int_as_float(0x7fc00000) : __fdiv_rn(m, 127.0f);
+    if (lane == 0) p.scale[kv][bh * (p.T / block) + blk] = s;
     int8_t* q = p.q[kv] + (bh * p.T + (int64_t)blk * block) * D;
-    for (int i = threadIdx.x; i < vecs; i += kThreads) {
-      float v[8];
-      ld8(row(blk * block + i * 8 / D) + i * 8 % D, v);
-      uint32_t w[2] = {0, 0};
-      if (fine) {
+    if (held) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)  // |x / scale| can round past 127 where the scale is subnormal
-          w[e >> 2] |= (uint32_t)(min(max(__float2int_rn(__fdiv_rn(v[e], s)), -127), 127) & 0xff) << (8 * (e & 3));
+      for (int k = 0; k < kHeld; ++k)
+        if (k * 32 + lane < vecs) {
+          r[k].get(v);
+          *reinterpret_cast<uint2*>(q + (k * 32 + lane) * 8) = eight(v, s);
+        }
+    } else {
+#pragma unroll 4
+      for (int i = lane; i < vecs; i += 32) {
+        Raw<T> t;
+        t.ld(at(i));
+        t.get(v);
+        *reinterpret_cast<uint2*>(q + i * 8) = eight(v, s);
       }
-      *reinterpret_cast<uint2*>(q + i * 8) = make_uint2(w[0], w[1]);
     }
   }
   if (j == 0 && end % block) {
-    __syncthreads();  // the tail has been read
+    __syncwarp();  // the tail has been read
     const int t0 = max(start, lastb * block);
-    for (int i = threadIdx.x; i < (end - t0) * D / 8; i += kThreads) {
-      float v[8];
+    for (int i = lane; i < (end - t0) * D / 8; i += 32) {
       const int tok = t0 + i * 8 / D, d = i * 8 % D;
-      ld8(x + (int64_t)(tok - start) * xv.st + d, v);
-      st8(tail + (tok % block) * D + d, v);
+      Raw<T> t;
+      t.ld(x + (int64_t)(tok - start) * xv.st + d);
+      t.st(tail + (tok % block) * D + d);
     }
   }
 }
 
-// 8 dims a thread, in the output's order.
+// 8 dims a thread and item, in the output's order; blockIdx.y keys or values.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Params p) {
   pdl_wait();
   pdl_trigger();
-  const int kv = blockIdx.y, vd = p.D / 8;
-  const int64_t total = (int64_t)p.B * p.T * p.Hkv * vd;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int d = (int)(i % vd) * 8;
-    int64_t r = i / vd;
-    const int hk = (int)(r % p.Hkv);
-    r /= p.Hkv;
-    const int t = (int)(r % p.T);
-    const int64_t b = r / p.T, bh = b * p.Hkv + hk;
-    const int n = p.count ? min(max(p.count[b], 0), p.T) : p.T;
+  const int kv = blockIdx.y;
+  const uint32_t vd = p.D / 8, row = vd * p.Hkv;  // vectors of a token
+  const int64_t b = blockIdx.z;
+  const int n = p.count ? min(max(p.count[b], 0), p.T) : p.T;
+  const int n8 = n / p.block * p.block;
+  const uint32_t total = row * (uint32_t)p.T;  // of this sequence
+  T* out = static_cast<T*>(p.out[kv]) + b * (int64_t)total * 8;
+  for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+    const uint32_t t = i / row, h = (i - t * row) / vd, d = (i - t * row - h * vd) * 8;
+    const int64_t bh = b * p.Hkv + h;
     float v[8];
+    Raw<T> r;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if (t < n / p.block * p.block) {
-      const float s = p.scale[kv][bh * (p.T / p.block) + t / p.block];
+    if ((int)t < n8) {
+      const float s = p.scale[kv][bh * (p.T / p.block) + t / (uint32_t)p.block];
       const uint2 w = *reinterpret_cast<const uint2*>(p.q[kv] + (bh * p.T + t) * p.D + d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = s * (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
-    } else if (t < n) {
-      ld8(static_cast<const T*>(p.tail[kv]) + (bh * p.block + t % p.block) * p.D + d, v);
+      r.set(v);
+    } else if ((int)t < n) {
+      r.ld(static_cast<const T*>(p.tail[kv]) + (bh * p.block + (t - n8)) * p.D + d);
+    } else {
+      r.set(v);
     }
-    st8(static_cast<T*>(p.out[kv]) + i * 8, v);
+    r.st(out + (int64_t)i * 8);
   }
 }
 
@@ -216,7 +263,7 @@ extern "C" int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, co
   p.x[1] = xattn::View{v->p, v->sb, v->st, v->sh};
   p.n = n, p.start = start, p.count = count;
   p.touched = (int)(((int64_t)n + c->block - 2) / c->block + 1);
-  const int64_t grid = (int64_t)c->B * c->Hkv * p.touched;
+  const int64_t grid = ((int64_t)c->B * c->Hkv * p.touched + kv8::kThreads / 32 - 1) / (kv8::kThreads / 32);
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 g((unsigned)grid, 2);
@@ -231,9 +278,10 @@ extern "C" int hclsm_kv8_read(const hclsm_kv8_cache* c, void* k, void* v, const 
   if (!kv8::al16(k) || !kv8::al16(v)) return HCLSM_ERR_ALIGN;
   kv8::Params p = kv8::params(c);
   p.out[0] = k, p.out[1] = v, p.count = lens;
-  const int64_t blocks = ((int64_t)c->B * c->T * c->Hkv * (c->D / 8) + kv8::kThreads - 1) / kv8::kThreads;
-  const int64_t most = (int64_t)num_sms() * 32;
-  const dim3 g((unsigned)(blocks < most ? blocks : most), 2);
+  const int64_t total = (int64_t)c->T * c->Hkv * (c->D / 8);  // vectors of a sequence
+  if (total > 0x7fffffff || c->B > 65535) return HCLSM_ERR_SHAPE;
+  const int64_t blocks = (total + kv8::kThreads - 1) / kv8::kThreads, most = (int64_t)num_sms() * 32 / c->B + 1;
+  const dim3 g((unsigned)(blocks < most ? blocks : most), 2, (unsigned)c->B);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return c->dtype == HCLSM_F32 ? launch_pdl(kv8::read_kernel<float>, g, kv8::kThreads, 0, st, p)
                                : launch_pdl(kv8::read_kernel<__nv_bfloat16>, g, kv8::kThreads, 0, st, p);
