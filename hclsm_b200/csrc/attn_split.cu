@@ -238,6 +238,9 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
                                       int first, int last, int stride, int nk,
                                       AddrK addr_k, AddrV addr_v, Ok ok, AllOk all_ok, Scale scale) {
   using R = Rows<E, D, CV>;
+  // fp32: a product is formed from zero and added here, because the tensor core's own
+  // sum over steps is not rounded to nearest (1.2e-6 instead of 5e-7 off at 5000 keys)
+  constexpr bool kFull = NQ == 3;
   constexpr int NK = R::kPieces, kOrder = (NQ > NK ? NQ : NK) - 1;
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   if (first >= last) return;
@@ -266,11 +269,16 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
       for (int t = 0; t < 2; ++t) {
         uint32_t b0[NK], b1[NK];
         R::template k_frag<F16>(kr[t], ks, b0, b1);
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = NQ - 1; i >= 0; --i)
 #pragma unroll
           for (int j = NK - 1; j >= 0; --j)
-            if (i + j <= kOrder) mma<F16>(s[t], a[i], b0[j], b1[j]);
+            if (i + j <= kOrder) mma<F16>(kFull ? part : s[t], a[i], b0[j], b1[j]);
+        if constexpr (kFull) {
+#pragma unroll
+          for (int e = 0; e < 2 * NR; ++e) s[t][e] += part[e];
+        }
       }
     }
     const float2 cur = sc;
@@ -356,11 +364,16 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
     for (int j = 0; j < D / 8; ++j) {
       uint32_t b0[NK], b1[NK];
       R::template v_frag<F16>(vr, j, b0, b1);
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = NQ - 1; i >= 0; --i)
 #pragma unroll
         for (int k = NK - 1; k >= 0; --k)
-          if (i + k <= kOrder) mma<F16>(st.o[j], pa[i], b0[k], b1[k]);
+          if (i + k <= kOrder) mma<F16>(kFull ? part : st.o[j], pa[i], b0[k], b1[k]);
+      if constexpr (kFull) {
+#pragma unroll
+        for (int e = 0; e < 2 * NR; ++e) st.o[j][e] += part[e];
+      }
     }
     fetch_v(next);
   }

@@ -14,21 +14,47 @@ constexpr int kT = 64;  // rows and keys of a tile
 constexpr int kThreads = 256;
 
 // Rows [r0, r0 + 64) of one head as fp32 rows of DP + 4; rows past n (and, with
-// KEYS, keys that are not allowed) and dims past D are zeros.
-template <typename T, int DP, bool KEYS>
-__device__ __forceinline__ void stage(float* dst, const View& x, const Params& p, int64_t b, int h, int r0, int n) {
+// KEYS, keys that are not allowed) and dims past D are zeros.  VEC: D a multiple
+// of 4 and aligned rows, four elements a load, all loads in flight first.
+template <typename T, int DP, bool KEYS, bool VEC>
+__device__ __forceinline__ void stage(float* dst, const View& x, const Params& p, int64_t b, int h, int r0, int n,
+                                      const uint8_t* okc) {
   const T* base = static_cast<const T*>(x.p) + b * x.sb + (int64_t)h * x.sh;
-  for (int i = threadIdx.x; i < kT * DP; i += kThreads) {
-    const int r = i / DP, d = i % DP, row = r0 + r;
-    bool ok = d < p.D && row < n;
-    if (KEYS) ok = ok && key_ok(p, b, n, row);
-    dst[r * (DP + 4) + d] = ok ? io<T>::ld(base + (int64_t)row * x.st + d) : 0.0f;
+  if constexpr (VEC) {
+    constexpr int N = kT * DP / 4 / kThreads;
+    float4 v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + i * kThreads, r = at / (DP / 4), d = at % (DP / 4) * 4, row = r0 + r;
+      v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (d < p.D && row < n && (!KEYS || okc[r])) {
+        const T* src = base + (int64_t)row * x.st + d;
+        if constexpr (sizeof(T) == 4) {
+          v[i] = *reinterpret_cast<const float4*>(src);
+        } else {
+          const float2 lo = io<T>::ld2(src), hi = io<T>::ld2(src + 2);
+          v[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + i * kThreads, r = at / (DP / 4), d = at % (DP / 4) * 4;
+      *reinterpret_cast<float4*>(dst + r * (DP + 4) + d) = v[i];
+    }
+  } else {
+    for (int i = threadIdx.x; i < kT * DP; i += kThreads) {
+      const int r = i / DP, d = i % DP, row = r0 + r;
+      const bool ok = d < p.D && row < n && (!KEYS || okc[r]);
+      dst[r * (DP + 4) + d] = ok ? io<T>::ld(base + (int64_t)row * x.st + d) : 0.0f;
+    }
   }
 }
 
 // acc[i][j] += sum_d a[4 ty + i][d] * b[tx + 16 j][d]
 template <int DP>
 __device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
+#pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
     float4 x[4], y[4];
 #pragma unroll
@@ -39,25 +65,54 @@ __device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, con
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        acc[i][j] += x[i].x * y[j].x + x[i].y * y[j].y + x[i].z * y[j].z + x[i].w * y[j].w;
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
+        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
+        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
+        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
+      }
   }
 }
 
-// out[i][n] += sum_c w(4 ty + i, c) * x[c][2 tx + 32 (n / 2) + n % 2]; w is [row][col] or, TRANS, [col][row].
+// Dims of a thread: 4 tx ... + 3 of each 64, or 2 tx, + 1 of 32.
+template <int DP> constexpr int kRun = DP == 32 ? 2 : 4;
+template <int DP>
+__device__ __forceinline__ int dim_of(int n, int tx) {
+  return n / kRun<DP> * 16 * kRun<DP> + tx * kRun<DP> + n % kRun<DP>;
+}
+
+// out[i][n] += sum_c w(4 ty + i, c) * x[c][dim_of(n)]; w is [row][col] or, TRANS, [col][row].
 template <int DP, bool TRANS>
 __device__ __forceinline__ void gather_tile(float (&out)[4][DP / 16], const float* w, const float* x, int ty, int tx) {
 #pragma unroll 2
-  for (int c = 0; c < kT; ++c) {
-    float a[4];
+  for (int c = 0; c < kT; c += 4) {
+    float a[4][4];  // [row][c]
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = TRANS ? w[c * (kT + 4) + 4 * ty + i] : w[(4 * ty + i) * (kT + 4) + c];
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(TRANS ? w + (c + i) * (kT + 4) + 4 * ty
+                                                              : w + (4 * ty + i) * (kT + 4) + c);
+      const float e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n) {
-      const float2 y = *reinterpret_cast<const float2*>(x + c * (DP + 4) + 2 * tx + 32 * n);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[i][2 * n] += a[i] * y.x, out[i][2 * n + 1] += a[i] * y.y;
+      for (int k = 0; k < 4; ++k) a[TRANS ? k : i][TRANS ? i : k] = e[k];
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int n = 0; n < DP / 16; n += kRun<DP>) {
+        float y[kRun<DP>];
+        const float* src = x + (c + k) * (DP + 4) + dim_of<DP>(n, tx);
+        if constexpr (kRun<DP> == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src);
+          y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(src);
+          y[0] = v.x, y[1] = v.y;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < kRun<DP>; ++e) out[i][n + e] = fmaf(a[i][k], y[e], out[i][n + e]);
+      }
   }
 }
 
@@ -70,19 +125,17 @@ __device__ __forceinline__ void store_rows(void* dst, const float (&acc)[4][DP /
     if (row >= L) continue;
     T* out = static_cast<T*>(dst) + ((b * L + row) * H + h) * (int64_t)p.D;
 #pragma unroll
-    for (int n = 0; n < DP / 32; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int d = 2 * tx + 32 * n + e;
-        if (d < p.D) io<T>::st(out + d, acc[i][2 * n + e] * f[i]);
-      }
+    for (int n = 0; n < DP / 16; ++n) {
+      const int d = dim_of<DP>(n, tx);
+      if (d < p.D) io<T>::st(out + d, acc[i][n] * f[i]);
+    }
   }
 }
 
 template <int DP> constexpr size_t op_floats() { return (size_t)kT * (DP + 4); }
 constexpr size_t kScoreFloats = (size_t)kT * (kT + 4);
 
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
@@ -100,15 +153,16 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ P
   const int hk = h / (p.H / p.Hkv);
   const int nk = key_count(p, b);
   const float c2 = p.scale * kLog2e;
-  stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
+  stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
   float acc[4][DP / 16] = {}, m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.0f;
   for (int k0 = 0; k0 < nk; k0 += kT) {
     __syncthreads();
-    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
-    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
     if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    __syncthreads();
+    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
     float s[4][4] = {};
     dot_tile<DP>(s, sq, sk, ty, tx);
@@ -183,7 +237,7 @@ __device__ __forceinline__ void row_stats(float (&lse)[4], float (&delta)[4], co
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
@@ -201,15 +255,16 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Pa
   const int64_t b = blockIdx.x / tiles / p.H;
   const int hk = h / (p.H / p.Hkv);
   const int nk = key_count(p, b);
-  stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
-  stage<T, DP, false>(sdo, p.dout, p, b, h, r0, p.Lq);
+  stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
+  stage<T, DP, false, VEC>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
   float acc[4][DP / 16] = {}, lse[4], delta[4];
   row_stats(lse, delta, p, b, h, r0, ty);
   for (int k0 = 0; k0 < nk; k0 += kT) {
     __syncthreads();
-    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
-    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
     if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    __syncthreads();
+    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
     grad_tile<DP>(nullptr, sds, sq, sk, sdo, sv, okc, lse, delta, p.scale * kLog2e, ty, tx);
     __syncthreads();
@@ -219,7 +274,7 @@ __global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Pa
   store_rows<T, DP>(p.dq, acc, f, p, b, p.Lq, p.H, h, r0, ty, tx);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 __global__ void __launch_bounds__(kThreads) dkv_kernel(const __grid_constant__ Params p) {
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
@@ -240,16 +295,17 @@ __global__ void __launch_bounds__(kThreads) dkv_kernel(const __grid_constant__ P
   const int nk = key_count(p, b);
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   if (k0 < nk) {
-    stage<T, DP, true>(sk, p.k, p, b, hk, k0, nk);
-    stage<T, DP, true>(sv, p.v, p, b, hk, k0, nk);
     if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    __syncthreads();
+    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
     // the query heads that share this key head, one after another: a fixed order
     for (int g = 0; g < G; ++g)
       for (int r0 = 0; r0 < p.Lq; r0 += kT) {
         const int h = hk * G + g;
         __syncthreads();
-        stage<T, DP, false>(sq, p.q, p, b, h, r0, p.Lq);
-        stage<T, DP, false>(sdo, p.dout, p, b, h, r0, p.Lq);
+        stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
+        stage<T, DP, false, VEC>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
         float lse[4], delta[4];
         row_stats(lse, delta, p, b, h, r0, ty);
         __syncthreads();
@@ -283,19 +339,19 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__
   if (lane == 0) p.delta[(b * p.H + h) * p.Lq + t] = a;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool VEC>
 int run(const Params& p, bool bwd, cudaStream_t st) {
   const int64_t qt = (int64_t)((p.Lq + kT - 1) / kT) * p.H * p.B, kt = (int64_t)((p.Lk + kT - 1) / kT) * p.Hkv * p.B;
   if (qt > 0x7fffffff || kt > 0x7fffffff) return HCLSM_ERR_SHAPE;
   const size_t s3 = (3 * op_floats<DP>() + kScoreFloats) * 4, s4 = (4 * op_floats<DP>() + kScoreFloats) * 4,
                s5 = s4 + kScoreFloats * 4;
   if (!bwd) {
-    auto f = fwd_kernel<T, DP>;
+    auto f = fwd_kernel<T, DP, VEC>;
     if (!set_smem_limit(reinterpret_cast<const void*>(f), s3)) return HCLSM_ERR_LAUNCH;
     return launch_pdl(f, (unsigned)qt, kThreads, s3, st, p);
   }
-  auto fq = dq_kernel<T, DP>;
-  auto fk = dkv_kernel<T, DP>;
+  auto fq = dq_kernel<T, DP, VEC>;
+  auto fk = dkv_kernel<T, DP, VEC>;
   if (!set_smem_limit(reinterpret_cast<const void*>(fq), s4) || !set_smem_limit(reinterpret_cast<const void*>(fk), s5))
     return HCLSM_ERR_LAUNCH;
   if (qt > 0)
@@ -304,10 +360,20 @@ int run(const Params& p, bool bwd, cudaStream_t st) {
 }
 
 template <typename T>
+bool rows4(const View& v) {  // four elements at a time
+  const int64_t e = 16 / sizeof(T) / (sizeof(T) == 2 ? 2 : 1);
+  return reinterpret_cast<uintptr_t>(v.p) % (e * sizeof(T)) == 0 && v.sb % e == 0 && v.st % e == 0 && v.sh % e == 0;
+}
+template <typename T, int DP>
+int run_any(const Params& p, bool bwd, cudaStream_t st) {
+  const bool vec = p.D % 4 == 0 && rows4<T>(p.q) && rows4<T>(p.k) && rows4<T>(p.v) && (!bwd || rows4<T>(p.dout));
+  return vec ? run<T, DP, true>(p, bwd, st) : run<T, DP, false>(p, bwd, st);
+}
+template <typename T>
 int dispatch(const Params& p, bool bwd, cudaStream_t st) {
-  if (p.D <= 32) return run<T, 32>(p, bwd, st);
-  if (p.D <= 64) return run<T, 64>(p, bwd, st);
-  return run<T, 128>(p, bwd, st);
+  if (p.D <= 32) return run_any<T, 32>(p, bwd, st);
+  if (p.D <= 64) return run_any<T, 64>(p, bwd, st);
+  return run_any<T, 128>(p, bwd, st);
 }
 
 int launch_delta(const Params& p, int dtype, cudaStream_t st) {
