@@ -1,31 +1,34 @@
 // Cross attention: the kernels that serve every type, head size, stride and
 // alignment (fp32 arithmetic throughout), and the C entry points.
 //
-// 64 x 64 score tiles, 256 threads, 4 x 4 scores a thread; operands are staged
-// in shared memory as fp32 rows of DP + 4 floats (the pad keeps the 16 lanes
-// that read different rows on different banks).  One pass over the keys with
-// the running maximum and sum of the softmax.  Bound: the FP32 pipes.
+// A block keeps TM rows (queries; keys for dk and dv) and walks over tiles of 64 of the
+// other side: TM x 64 scores, 4 x 4 a thread; operands are staged in shared memory as
+// fp32 rows of DP + 4 floats (the pad keeps the 16 lanes that read different rows on
+// different banks).  One pass over the keys with the running maximum and sum of the
+// softmax.  Bound: the FP32 pipes.  TM 64 reads the least; TM 32 where 64 would leave
+// SMs without a block.
 #include "xattn.cuh"
 
 namespace hclsm {
 namespace xattn {
 
-constexpr int kT = 64;  // rows and keys of a tile
-constexpr int kThreads = 256;
+constexpr int kT = 64;  // rows of a streamed tile
+constexpr int kThreads = 256;  // of the row-wise kernel
+template <int TM> constexpr int kTileThreads = TM * 4;
 
-// Rows [r0, r0 + 64) of one head as fp32 rows of DP + 4; rows past n (and, with
+// Rows [r0, r0 + ROWS) of one head as fp32 rows of DP + 4; rows past n (and, with
 // KEYS, keys that are not allowed) and dims past D are zeros.  VEC: D a multiple
 // of 4 and aligned rows, four elements a load, all loads in flight first.
-template <typename T, int DP, bool KEYS, bool VEC>
+template <typename T, int DP, bool KEYS, bool VEC, int ROWS, int NT>
 __device__ __forceinline__ void stage(float* dst, const View& x, const Params& p, int64_t b, int h, int r0, int n,
                                       const uint8_t* okc) {
   const T* base = static_cast<const T*>(x.p) + b * x.sb + (int64_t)h * x.sh;
   if constexpr (VEC) {
-    constexpr int N = kT * DP / 4 / kThreads;
+    constexpr int N = ROWS * DP / 4 / NT;
     float4 v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * kThreads, r = at / (DP / 4), d = at % (DP / 4) * 4, row = r0 + r;
+      const int at = threadIdx.x + i * NT, r = at / (DP / 4), d = at % (DP / 4) * 4, row = r0 + r;
       v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (d < p.D && row < n && (!KEYS || okc[r])) {
         const T* src = base + (int64_t)row * x.st + d;
@@ -39,11 +42,11 @@ __device__ __forceinline__ void stage(float* dst, const View& x, const Params& p
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * kThreads, r = at / (DP / 4), d = at % (DP / 4) * 4;
+      const int at = threadIdx.x + i * NT, r = at / (DP / 4), d = at % (DP / 4) * 4;
       *reinterpret_cast<float4*>(dst + r * (DP + 4) + d) = v[i];
     }
   } else {
-    for (int i = threadIdx.x; i < kT * DP; i += kThreads) {
+    for (int i = threadIdx.x; i < ROWS * DP; i += NT) {
       const int r = i / DP, d = i % DP, row = r0 + r;
       const bool ok = d < p.D && row < n && (!KEYS || okc[r]);
       dst[r * (DP + 4) + d] = ok ? io<T>::ld(base + (int64_t)row * x.st + d) : 0.0f;
@@ -81,19 +84,16 @@ __device__ __forceinline__ int dim_of(int n, int tx) {
   return n / kRun<DP> * 16 * kRun<DP> + tx * kRun<DP> + n % kRun<DP>;
 }
 
-// out[i][n] += sum_c w(4 ty + i, c) * x[c][dim_of(n)]; w is [row][col] or, TRANS, [col][row].
-template <int DP, bool TRANS>
+// out[i][n] += sum_c w[4 ty + i][c] * x[c][dim_of(n)]
+template <int DP>
 __device__ __forceinline__ void gather_tile(float (&out)[4][DP / 16], const float* w, const float* x, int ty, int tx) {
 #pragma unroll 2
   for (int c = 0; c < kT; c += 4) {
     float a[4][4];  // [row][c]
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(TRANS ? w + (c + i) * (kT + 4) + 4 * ty
-                                                              : w + (4 * ty + i) * (kT + 4) + c);
-      const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) a[TRANS ? k : i][TRANS ? i : k] = e[k];
+      const float4 v = *reinterpret_cast<const float4*>(w + (4 * ty + i) * (kT + 4) + c);
+      a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -132,28 +132,33 @@ __device__ __forceinline__ void store_rows(void* dst, const float (&acc)[4][DP /
   }
 }
 
-template <int DP> constexpr size_t op_floats() { return (size_t)kT * (DP + 4); }
-constexpr size_t kScoreFloats = (size_t)kT * (kT + 4);
+template <int DP> constexpr size_t row_floats = DP + 4;
 
-template <typename T, int DP, bool VEC>
-__global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ Params p) {
+// Shared memory of a block: NA operands of TM rows, NB of 64, NS score tiles.
+template <int DP, int TM, int NA, int NB, int NS> constexpr size_t smem_bytes() {
+  return 4 * ((NA * TM + NB * kT) * row_floats<DP> + (size_t)NS * TM * (kT + 4));
+}
+
+template <typename T, int DP, bool VEC, int TM>
+__global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_constant__ Params p) {
+  constexpr int NT = kTileThreads<TM>;
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
-  float* sk = sq + op_floats<DP>();
-  float* sv = sk + op_floats<DP>();
-  float* sp = sv + op_floats<DP>();
+  float* sk = sq + TM * row_floats<DP>;
+  float* sv = sk + kT * row_floats<DP>;
+  float* sp = sv + kT * row_floats<DP>;
   __shared__ uint8_t okc[kT];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   pdl_wait();
   pdl_trigger();
-  const int tiles = (p.Lq + kT - 1) / kT;
-  const int r0 = (int)(blockIdx.x % tiles) * kT;
+  const int tiles = (p.Lq + TM - 1) / TM;
+  const int r0 = (int)(blockIdx.x % tiles) * TM;
   const int h = (int)(blockIdx.x / tiles % p.H);
   const int64_t b = blockIdx.x / tiles / p.H;
   const int hk = h / (p.H / p.Hkv);
   const int nk = key_count(p, b);
   const float c2 = p.scale * kLog2e;
-  stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
+  stage<T, DP, false, VEC, TM, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
   float acc[4][DP / 16] = {}, m[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.0f;
@@ -161,8 +166,8 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ P
     __syncthreads();
     if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
     __syncthreads();
-    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
-    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, kT, NT>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, kT, NT>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
     float s[4][4] = {};
     dot_tile<DP>(s, sq, sk, ty, tx);
@@ -190,8 +195,8 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ P
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) acc[i][n] *= f;
     }
-    __syncthreads();
-    gather_tile<DP, false>(acc, sp, sv, ty, tx);
+    __syncwarp();  // a warp's rows of weights are its own
+    gather_tile<DP>(acc, sp, sv, ty, tx);
   }
   float inv[4];
 #pragma unroll
@@ -206,113 +211,120 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const __grid_constant__ P
   store_rows<T, DP>(p.o, acc, inv, p, b, p.Lq, p.H, h, r0, ty, tx);
 }
 
-// p and ds of one tile, left in sp and sds (row = query, column = key).
-template <int DP>
-__device__ __forceinline__ void grad_tile(float* sp, float* sds, const float* sq, const float* sk, const float* sdo,
-                                          const float* sv, const uint8_t* okc, const float (&lse)[4],
-                                          const float (&delta)[4], float c2, int ty, int tx) {
-  float s[4][4] = {}, dp[4][4] = {};
-  dot_tile<DP>(s, sq, sk, ty, tx);
-  dot_tile<DP>(dp, sdo, sv, ty, tx);
+template <typename T, int DP, bool VEC, int TM>
+__global__ void __launch_bounds__(kTileThreads<TM>) dq_kernel(const __grid_constant__ Params p) {
+  constexpr int NT = kTileThreads<TM>;
+  extern __shared__ float4 smem4[];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sdo = sq + TM * row_floats<DP>;
+  float* sk = sdo + TM * row_floats<DP>;
+  float* sv = sk + kT * row_floats<DP>;
+  float* sds = sv + kT * row_floats<DP>;
+  __shared__ uint8_t okc[kT];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  pdl_wait();
+  pdl_trigger();
+  const int tiles = (p.Lq + TM - 1) / TM;
+  const int r0 = (int)(blockIdx.x % tiles) * TM;
+  const int h = (int)(blockIdx.x / tiles % p.H);
+  const int64_t b = blockIdx.x / tiles / p.H;
+  const int hk = h / (p.H / p.Hkv);
+  const int nk = key_count(p, b);
+  const float c2 = p.scale * kLog2e;
+  stage<T, DP, false, VEC, TM, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
+  stage<T, DP, false, VEC, TM, NT>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
+  float acc[4][DP / 16] = {}, lse[4], delta[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float w = okc[tx + 16 * j] ? exp2f(s[i][j] * c2 - lse[i]) : 0.0f;
-      const int at = (4 * ty + i) * (kT + 4) + tx + 16 * j;
-      if (sp) sp[at] = w;
-      sds[at] = w * (dp[i][j] - delta[i]);
-    }
-}
-
-// lse2 and delta of the thread's 4 rows; rows past Lq weigh nothing.
-__device__ __forceinline__ void row_stats(float (&lse)[4], float (&delta)[4], const Params& p, int64_t b, int h, int r0,
-                                          int ty) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i) {  // rows past the end weigh nothing
     const int row = r0 + 4 * ty + i;
     const int64_t at = (b * p.H + h) * p.Lq + row;
     lse[i] = row < p.Lq ? p.lse2[at] : INFINITY;
     delta[i] = row < p.Lq ? p.delta[at] : 0.0f;
   }
-}
-
-template <typename T, int DP, bool VEC>
-__global__ void __launch_bounds__(kThreads) dq_kernel(const __grid_constant__ Params p) {
-  extern __shared__ float4 smem4[];
-  float* sq = reinterpret_cast<float*>(smem4);
-  float* sdo = sq + op_floats<DP>();
-  float* sk = sdo + op_floats<DP>();
-  float* sv = sk + op_floats<DP>();
-  float* sds = sv + op_floats<DP>();
-  __shared__ uint8_t okc[kT];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  pdl_wait();
-  pdl_trigger();
-  const int tiles = (p.Lq + kT - 1) / kT;
-  const int r0 = (int)(blockIdx.x % tiles) * kT;
-  const int h = (int)(blockIdx.x / tiles % p.H);
-  const int64_t b = blockIdx.x / tiles / p.H;
-  const int hk = h / (p.H / p.Hkv);
-  const int nk = key_count(p, b);
-  stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
-  stage<T, DP, false, VEC>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
-  float acc[4][DP / 16] = {}, lse[4], delta[4];
-  row_stats(lse, delta, p, b, h, r0, ty);
   for (int k0 = 0; k0 < nk; k0 += kT) {
     __syncthreads();
     if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
     __syncthreads();
-    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
-    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, kT, NT>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, kT, NT>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
-    grad_tile<DP>(nullptr, sds, sq, sk, sdo, sv, okc, lse, delta, p.scale * kLog2e, ty, tx);
-    __syncthreads();
-    gather_tile<DP, false>(acc, sds, sk, ty, tx);
+    float s[4][4] = {}, dp[4][4] = {};
+    dot_tile<DP>(s, sq, sk, ty, tx);
+    dot_tile<DP>(dp, sdo, sv, ty, tx);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = okc[tx + 16 * j] ? exp2f(s[i][j] * c2 - lse[i]) : 0.0f;
+        sds[(4 * ty + i) * (kT + 4) + tx + 16 * j] = w * (dp[i][j] - delta[i]);
+      }
+    __syncwarp();
+    gather_tile<DP>(acc, sds, sk, ty, tx);
   }
   const float f[4] = {p.scale, p.scale, p.scale, p.scale};
   store_rows<T, DP>(p.dq, acc, f, p, b, p.Lq, p.H, h, r0, ty, tx);
 }
 
-template <typename T, int DP, bool VEC>
-__global__ void __launch_bounds__(kThreads) dkv_kernel(const __grid_constant__ Params p) {
+// Rows are keys, columns queries: the scores are formed transposed.
+template <typename T, int DP, bool VEC, int TM>
+__global__ void __launch_bounds__(kTileThreads<TM>) dkv_kernel(const __grid_constant__ Params p) {
+  constexpr int NT = kTileThreads<TM>;
   extern __shared__ float4 smem4[];
-  float* sq = reinterpret_cast<float*>(smem4);
-  float* sdo = sq + op_floats<DP>();
-  float* sk = sdo + op_floats<DP>();
-  float* sv = sk + op_floats<DP>();
-  float* sp = sv + op_floats<DP>();
-  float* sds = sp + kScoreFloats;
-  __shared__ uint8_t okc[kT];
+  float* sk = reinterpret_cast<float*>(smem4);
+  float* sv = sk + TM * row_floats<DP>;
+  float* sq = sv + TM * row_floats<DP>;
+  float* sdo = sq + kT * row_floats<DP>;
+  float* sp = sdo + kT * row_floats<DP>;
+  float* sds = sp + TM * (kT + 4);
+  __shared__ uint8_t okc[TM];
+  __shared__ float s_lse[kT], s_delta[kT];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   pdl_wait();
   pdl_trigger();
-  const int tiles = (p.Lk + kT - 1) / kT;
-  const int k0 = (int)(blockIdx.x % tiles) * kT;
+  const int tiles = (p.Lk + TM - 1) / TM;
+  const int k0 = (int)(blockIdx.x % tiles) * TM;
   const int hk = (int)(blockIdx.x / tiles % p.Hkv);
   const int64_t b = blockIdx.x / tiles / p.Hkv;
   const int G = p.H / p.Hkv;
   const int nk = key_count(p, b);
+  const float c2 = p.scale * kLog2e;
   float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
   if (k0 < nk) {
-    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    if (threadIdx.x < TM) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
     __syncthreads();
-    stage<T, DP, true, VEC>(sk, p.k, p, b, hk, k0, nk, okc);
-    stage<T, DP, true, VEC>(sv, p.v, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, TM, NT>(sk, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, TM, NT>(sv, p.v, p, b, hk, k0, nk, okc);
     // the query heads that share this key head, one after another: a fixed order
     for (int g = 0; g < G; ++g)
       for (int r0 = 0; r0 < p.Lq; r0 += kT) {
         const int h = hk * G + g;
         __syncthreads();
-        stage<T, DP, false, VEC>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
-        stage<T, DP, false, VEC>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
-        float lse[4], delta[4];
-        row_stats(lse, delta, p, b, h, r0, ty);
+        stage<T, DP, false, VEC, kT, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
+        stage<T, DP, false, VEC, kT, NT>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
+        if (threadIdx.x < kT) {  // rows past the end weigh nothing
+          const int row = r0 + threadIdx.x;
+          const int64_t at = (b * p.H + h) * p.Lq + row;
+          s_lse[threadIdx.x] = row < p.Lq ? p.lse2[at] : INFINITY;
+          s_delta[threadIdx.x] = row < p.Lq ? p.delta[at] : 0.0f;
+        }
         __syncthreads();
-        grad_tile<DP>(sp, sds, sq, sk, sdo, sv, okc, lse, delta, p.scale * kLog2e, ty, tx);
-        __syncthreads();
-        gather_tile<DP, true>(dv, sp, sdo, ty, tx);
-        gather_tile<DP, true>(dk, sds, sq, ty, tx);
+        float s[4][4] = {}, dp[4][4] = {};
+        dot_tile<DP>(s, sk, sq, ty, tx);
+        dot_tile<DP>(dp, sv, sdo, ty, tx);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lse = s_lse[tx + 16 * j], delta = s_delta[tx + 16 * j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float w = okc[4 * ty + i] ? exp2f(s[i][j] * c2 - lse) : 0.0f;
+            const int at = (4 * ty + i) * (kT + 4) + tx + 16 * j;
+            sp[at] = w;
+            sds[at] = w * (dp[i][j] - delta);
+          }
+        }
+        __syncwarp();
+        gather_tile<DP>(dv, sp, sdo, ty, tx);
+        gather_tile<DP>(dk, sds, sq, ty, tx);
       }
   }
   const float one[4] = {1.0f, 1.0f, 1.0f, 1.0f}, f[4] = {p.scale, p.scale, p.scale, p.scale};
@@ -339,24 +351,30 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__
   if (lane == 0) p.delta[(b * p.H + h) * p.Lq + t] = a;
 }
 
+template <typename T, int DP, bool VEC, int TM>
+int launch_rows(const Params& p, int which, cudaStream_t st) {  // 0 forward, 1 dq, 2 dk and dv
+  constexpr int NT = kTileThreads<TM>;
+  const int64_t rows = which == 2 ? p.Lk : p.Lq, heads = which == 2 ? p.Hkv : p.H;
+  const int64_t grid = (rows + TM - 1) / TM * heads * p.B;
+  if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  if (grid == 0) return HCLSM_OK;
+  const size_t bytes = which == 0   ? smem_bytes<DP, TM, 1, 2, 1>()
+                       : which == 1 ? smem_bytes<DP, TM, 2, 2, 1>()
+                                    : smem_bytes<DP, TM, 2, 2, 2>();
+  auto f = which == 0 ? fwd_kernel<T, DP, VEC, TM> : which == 1 ? dq_kernel<T, DP, VEC, TM> : dkv_kernel<T, DP, VEC, TM>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(f), bytes)) return HCLSM_ERR_LAUNCH;
+  return launch_pdl(f, (unsigned)grid, NT, bytes, st, p);
+}
+
 template <typename T, int DP, bool VEC>
 int run(const Params& p, bool bwd, cudaStream_t st) {
-  const int64_t qt = (int64_t)((p.Lq + kT - 1) / kT) * p.H * p.B, kt = (int64_t)((p.Lk + kT - 1) / kT) * p.Hkv * p.B;
-  if (qt > 0x7fffffff || kt > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  const size_t s3 = (3 * op_floats<DP>() + kScoreFloats) * 4, s4 = (4 * op_floats<DP>() + kScoreFloats) * 4,
-               s5 = s4 + kScoreFloats * 4;
-  if (!bwd) {
-    auto f = fwd_kernel<T, DP, VEC>;
-    if (!set_smem_limit(reinterpret_cast<const void*>(f), s3)) return HCLSM_ERR_LAUNCH;
-    return launch_pdl(f, (unsigned)qt, kThreads, s3, st, p);
+  for (int which = bwd ? 1 : 0; which < (bwd ? 3 : 1); ++which) {
+    const int64_t rows = which == 2 ? p.Lk : p.Lq, heads = which == 2 ? p.Hkv : p.H;
+    const bool small = (rows + 63) / 64 * heads * p.B < 2 * (int64_t)num_sms();
+    const int rc = small ? launch_rows<T, DP, VEC, 32>(p, which, st) : launch_rows<T, DP, VEC, 64>(p, which, st);
+    if (rc) return rc;
   }
-  auto fq = dq_kernel<T, DP, VEC>;
-  auto fk = dkv_kernel<T, DP, VEC>;
-  if (!set_smem_limit(reinterpret_cast<const void*>(fq), s4) || !set_smem_limit(reinterpret_cast<const void*>(fk), s5))
-    return HCLSM_ERR_LAUNCH;
-  if (qt > 0)
-    if (const int rc = launch_pdl(fq, (unsigned)qt, kThreads, s4, st, p)) return rc;
-  return kt > 0 ? launch_pdl(fk, (unsigned)kt, kThreads, s5, st, p) : HCLSM_OK;
+  return HCLSM_OK;
 }
 
 template <typename T>
