@@ -1,12 +1,16 @@
 // Cross attention: the kernels that serve every type, head size, stride and
-// alignment (fp32 arithmetic throughout), and the C entry points.
+// alignment, and the C entry points.
 //
-// A block keeps TM rows (queries; keys for dk and dv) and walks over tiles of 64 of the
-// other side: TM x 64 scores, 4 x 4 a thread; operands are staged in shared memory as
-// fp32 rows of DP + 4 floats (the pad keeps the 16 lanes that read different rows on
-// different banks).  One pass over the keys with the running maximum and sum of the
-// softmax.  Bound: the FP32 pipes.  TM 64 reads the least; TM 32 where 64 would leave
-// SMs without a block.
+// A block keeps TM rows (queries; keys for dk and dv), 16 a warp, and walks over tiles
+// of 64 of the other side with mma.sync m16n8k16 products.  An fp32 operand is split
+// into three bf16 pieces (8 bits each) when it is staged, one shared-memory plane a
+// piece, and the six products of pieces whose order is at most 2 are formed from zero
+// and added in fp32: the result is as exact as fp32 arithmetic, at a sixth of the bf16
+// rate (170 multiply-adds a clock and SM, 128 on the FP32 pipes) and with a tenth of
+// the instructions, which is what counts where few warps are resident.  Rows of planes
+// are DP + 8 elements, so that ldmatrix reads every bank once.  One pass over the keys
+// with the running maximum and sum of the softmax.  TM 32 where 64 would leave SMs
+// without a block.
 #include "xattn.cuh"
 
 namespace hclsm {
@@ -14,141 +18,193 @@ namespace xattn {
 
 constexpr int kT = 64;  // rows of a streamed tile
 constexpr int kThreads = 256;  // of the row-wise kernel
-template <int TM> constexpr int kTileThreads = TM * 4;
+template <int TM> constexpr int kTileThreads = TM * 2;
+template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
+template <int DP> constexpr int kLd = DP + 8;
 
-// Rows [r0, r0 + ROWS) of one head as fp32 rows of DP + 4; rows past n (and, with
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, "
+      "%2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const __nv_bfloat16* p) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p))
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p))
+                 : "memory");
+}
+// The N leading bf16 pieces of two fp32 values, packed.
+template <int N>
+__device__ __forceinline__ void pieces(float lo, float hi, uint32_t (&out)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    out[i] = *reinterpret_cast<const uint32_t*>(&h);
+    lo -= __uint_as_float(out[i] << 16);
+    hi -= __uint_as_float(out[i] & 0xffff0000u);
+  }
+}
+
+// Rows [r0, r0 + ROWS) of one head as planes of bf16 pieces; rows past n (and, with
 // KEYS, keys that are not allowed) and dims past D are zeros.  VEC: D a multiple
 // of 4 and aligned rows, four elements a load, all loads in flight first.
 template <typename T, int DP, bool KEYS, bool VEC, int ROWS, int NT>
-__device__ __forceinline__ void stage(float* dst, const View& x, const Params& p, int64_t b, int h, int r0, int n,
-                                      const uint8_t* okc) {
+__device__ __forceinline__ void stage(__nv_bfloat16* dst, const View& x, const Params& p, int64_t b, int h, int r0,
+                                      int n, const uint8_t* okc) {
+  constexpr int N = ROWS * DP / 4 / NT, NP = kPieces<T>, U = N < 8 ? N : 8;
   const T* base = static_cast<const T*>(x.p) + b * x.sb + (int64_t)h * x.sh;
-  if constexpr (VEC) {
-    constexpr int N = ROWS * DP / 4 / NT;
-    float4 v[N];
+#pragma unroll 1
+  for (int i0 = 0; i0 < N; i0 += U) {
+    float v[U][4];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * NT, r = at / (DP / 4), d = at % (DP / 4) * 4, row = r0 + r;
-      v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (d < p.D && row < n && (!KEYS || okc[r])) {
+    for (int i = 0; i < U; ++i) {
+      const int at = threadIdx.x + (i0 + i) * NT, r = at / (DP / 4), d = at % (DP / 4) * 4, row = r0 + r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i][e] = 0.0f;
+      if (row < n && (!KEYS || okc[r])) {
         const T* src = base + (int64_t)row * x.st + d;
-        if constexpr (sizeof(T) == 4) {
-          v[i] = *reinterpret_cast<const float4*>(src);
+        if constexpr (VEC) {
+          if (d < p.D) {
+            if constexpr (sizeof(T) == 4) {
+              const float4 f = *reinterpret_cast<const float4*>(src);
+              v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+            } else {
+              const float2 lo = io<T>::ld2(src), hi = io<T>::ld2(src + 2);
+              v[i][0] = lo.x, v[i][1] = lo.y, v[i][2] = hi.x, v[i][3] = hi.y;
+            }
+          }
         } else {
-          const float2 lo = io<T>::ld2(src), hi = io<T>::ld2(src + 2);
-          v[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < p.D) v[i][e] = io<T>::ld(src + e);
         }
       }
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * NT, r = at / (DP / 4), d = at % (DP / 4) * 4;
-      *reinterpret_cast<float4*>(dst + r * (DP + 4) + d) = v[i];
+    for (int i = 0; i < U; ++i) {
+      const int at = threadIdx.x + (i0 + i) * NT, r = at / (DP / 4), d = at % (DP / 4) * 4;
+      uint32_t lo[NP], hi[NP];
+      pieces<NP>(v[i][0], v[i][1], lo);
+      pieces<NP>(v[i][2], v[i][3], hi);
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        *reinterpret_cast<uint2*>(dst + ((size_t)k * ROWS + r) * kLd<DP> + d) = make_uint2(lo[k], hi[k]);
     }
+  }
+}
+
+// acc += the products of the pieces a[i] and b[j], order i + j at most NP - 1, smallest first.
+template <int NP>
+__device__ __forceinline__ void product(float (&acc)[4], const uint32_t (&a)[NP][4], const uint32_t (&b)[NP][4], int t) {
+  if constexpr (NP == 1) {
+    mma(acc, a[0], b[0][2 * t], b[0][2 * t + 1]);
   } else {
-    for (int i = threadIdx.x; i < ROWS * DP; i += NT) {
-      const int r = i / DP, d = i % DP, row = r0 + r;
-      const bool ok = d < p.D && row < n && (!KEYS || okc[r]);
-      dst[r * (DP + 4) + d] = ok ? io<T>::ld(base + (int64_t)row * x.st + d) : 0.0f;
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = NP - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = NP - 1 - i; j >= 0; --j) mma(part, a[i], b[j][2 * t], b[j][2 * t + 1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += part[e];
+  }
+}
+
+// s (the warp's 16 rows x 64) = own rows . streamed rows: a at the warp's first row, b the tile.
+template <int DP, int NP, int ROWS>
+__device__ __forceinline__ void dot_tile(float (&s)[8][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int ksteps,
+                                         int lane) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+#pragma unroll 1
+  for (int k = 0; k < ksteps; ++k) {
+    uint32_t fa[NP][4];
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      ldmatrix4<false>(fa[i], a + (size_t)i * ROWS * kLd<DP> + (lane & 15) * kLd<DP> + k * 16 + (lane >> 4) * 8);
+#pragma unroll
+    for (int t = 0; t < 8; t += 2) {
+      uint32_t fb[NP][4];
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        ldmatrix4<false>(fb[i], b + ((size_t)i * kT + t * 8 + (lane >> 4) * 8 + (lane & 7)) * kLd<DP> + k * 16 +
+                                    (lane >> 3 & 1) * 8);
+      product<NP>(s[t], fa, fb, 0);
+      product<NP>(s[t + 1], fa, fb, 1);
     }
   }
 }
 
-// acc[i][j] += sum_d a[4 ty + i][d] * b[tx + 16 j][d]
-template <int DP>
-__device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
-#pragma unroll 4
-  for (int d = 0; d < DP; d += 4) {
-    float4 x[4], y[4];
+// acc (16 rows x DP) += w (16 x 64, as dot_tile leaves its products) x the streamed tile.
+template <int DP, int NP>
+__device__ __forceinline__ void gather_tile(float (&acc)[DP / 8][4], const float (&w)[8][4], const __nv_bfloat16* x,
+                                            int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = *reinterpret_cast<const float4*>(a + (4 * ty + i) * (DP + 4) + d);
-      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * (DP + 4) + d);
+  for (int u = 0; u < 4; ++u) {
+    uint32_t fa[NP][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint32_t t[NP];
+      pieces<NP>(w[2 * u + (e >> 1)][2 * (e & 1)], w[2 * u + (e >> 1)][2 * (e & 1) + 1], t);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) fa[i][e] = t[i];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < DP / 8; j += 2) {
+      uint32_t fb[NP][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[i][j] = fmaf(x[i].x, y[j].x, acc[i][j]);
-        acc[i][j] = fmaf(x[i].y, y[j].y, acc[i][j]);
-        acc[i][j] = fmaf(x[i].z, y[j].z, acc[i][j]);
-        acc[i][j] = fmaf(x[i].w, y[j].w, acc[i][j]);
-      }
-  }
-}
-
-// Dims of a thread: 4 tx ... + 3 of each 64, or 2 tx, + 1 of 32.
-template <int DP> constexpr int kRun = DP == 32 ? 2 : 4;
-template <int DP>
-__device__ __forceinline__ int dim_of(int n, int tx) {
-  return n / kRun<DP> * 16 * kRun<DP> + tx * kRun<DP> + n % kRun<DP>;
-}
-
-// out[i][n] += sum_c w[4 ty + i][c] * x[c][dim_of(n)]
-template <int DP>
-__device__ __forceinline__ void gather_tile(float (&out)[4][DP / 16], const float* w, const float* x, int ty, int tx) {
-#pragma unroll 2
-  for (int c = 0; c < kT; c += 4) {
-    float a[4][4];  // [row][c]
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 v = *reinterpret_cast<const float4*>(w + (4 * ty + i) * (kT + 4) + c);
-      a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
+      for (int i = 0; i < NP; ++i)
+        ldmatrix4<true>(fb[i], x + ((size_t)i * kT + u * 16 + (lane & 15)) * kLd<DP> + j * 8 + (lane >> 4) * 8);
+      product<NP>(acc[j], fa, fb, 0);
+      product<NP>(acc[j + 1], fa, fb, 1);
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int n = 0; n < DP / 16; n += kRun<DP>) {
-        float y[kRun<DP>];
-        const float* src = x + (c + k) * (DP + 4) + dim_of<DP>(n, tx);
-        if constexpr (kRun<DP> == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-        } else {
-          const float2 v = *reinterpret_cast<const float2*>(src);
-          y[0] = v.x, y[1] = v.y;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < kRun<DP>; ++e) out[i][n + e] = fmaf(a[i][k], y[e], out[i][n + e]);
-      }
   }
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[4][DP / 16], const float (&f)[4],
-                                           const Params& p, int64_t b, int L, int H, int h, int r0, int ty, int tx) {
+__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8][4], float f0, float f1,
+                                           const Params& p, int64_t b, int L, int H, int h, int r0, int lane) {
+  const int g = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = r0 + 4 * ty + i;
+  for (int r = 0; r < 2; ++r) {
+    const int row = r0 + g + 8 * r;
     if (row >= L) continue;
     T* out = static_cast<T*>(dst) + ((b * L + row) * H + h) * (int64_t)p.D;
+    const float f = r ? f1 : f0;
 #pragma unroll
-    for (int n = 0; n < DP / 16; ++n) {
-      const int d = dim_of<DP>(n, tx);
-      if (d < p.D) io<T>::st(out + d, acc[i][n] * f[i]);
-    }
+    for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = j * 8 + 2 * c + e;
+        if (d < p.D) io<T>::st(out + d, acc[j][2 * r + e] * f);
+      }
   }
 }
 
-template <int DP> constexpr size_t row_floats = DP + 4;
-
-// Shared memory of a block: NA operands of TM rows, NB of 64, NS score tiles.
-template <int DP, int TM, int NA, int NB, int NS> constexpr size_t smem_bytes() {
-  return 4 * ((NA * TM + NB * kT) * row_floats<DP> + (size_t)NS * TM * (kT + 4));
+// Shared memory of a block: NA operands of TM rows and two of 64.
+template <typename T, int DP, int TM, int NA> constexpr size_t smem_bytes() {
+  return (size_t)kPieces<T> * (NA * TM + 2 * kT) * kLd<DP> * sizeof(__nv_bfloat16);
 }
 
 template <typename T, int DP, bool VEC, int TM>
 __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_constant__ Params p) {
-  constexpr int NT = kTileThreads<TM>;
-  extern __shared__ float4 smem4[];
-  float* sq = reinterpret_cast<float*>(smem4);
-  float* sk = sq + TM * row_floats<DP>;
-  float* sv = sk + kT * row_floats<DP>;
-  float* sp = sv + kT * row_floats<DP>;
+  constexpr int NT = kTileThreads<TM>, NP = kPieces<T>;
+  extern __shared__ uint4 smem4[];
+  __nv_bfloat16* sq = reinterpret_cast<__nv_bfloat16*>(smem4);
+  __nv_bfloat16* sk = sq + (size_t)NP * TM * kLd<DP>;
+  __nv_bfloat16* sv = sk + (size_t)NP * kT * kLd<DP>;
   __shared__ uint8_t okc[kT];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
   pdl_wait();
   pdl_trigger();
   const int tiles = (p.Lq + TM - 1) / TM;
@@ -156,180 +212,134 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
   const int h = (int)(blockIdx.x / tiles % p.H);
   const int64_t b = blockIdx.x / tiles / p.H;
   const int hk = h / (p.H / p.Hkv);
-  const int nk = key_count(p, b);
+  const int nk = key_count(p, b), ksteps = (p.D + 15) / 16;
   const float c2 = p.scale * kLog2e;
   stage<T, DP, false, VEC, TM, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
-  float acc[4][DP / 16] = {}, m[4], l[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.0f;
+  float acc[DP / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   for (int k0 = 0; k0 < nk; k0 += kT) {
     __syncthreads();
-    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
+    for (int i = threadIdx.x; i < kT; i += NT) okc[i] = key_ok(p, b, nk, k0 + i);
     __syncthreads();
     stage<T, DP, true, VEC, kT, NT>(sk, p.k, p, b, hk, k0, nk, okc);
     stage<T, DP, true, VEC, kT, NT>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
-    float s[4][4] = {};
-    dot_tile<DP>(s, sq, sk, ty, tx);
+    float s[8][4];
+    dot_tile<DP, NP, TM>(s, sq + warp * 16 * kLd<DP>, sk, ksteps, lane);
+    float mx[2] = {m[0], m[1]};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float mx = m[i];
+    for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] = okc[tx + 16 * j] ? s[i][j] * c2 : -INFINITY;
-        mx = fmaxf(mx, s[i][j]);
+      for (int e = 0; e < 4; ++e) {
+        s[t][e] = okc[t * 8 + 2 * c + (e & 1)] ? s[t][e] * c2 : -INFINITY;
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
       }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float base = mx == -INFINITY ? 0.0f : mx;  // no allowed key yet: every weight 0
-      const float f = exp2f(m[i] - base);
-      float sum = 0.0f;
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      const float base = mx[r] == -INFINITY ? 0.0f : mx[r];  // no allowed key yet: every weight 0
+      const float f = ex2(m[r] - base);
+      m[r] = mx[r];
+      l[r] *= f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = exp2f(s[i][j] - base);
-        sp[(4 * ty + i) * (kT + 4) + tx + 16 * j] = e;
-        sum += e;
-      }
-      m[i] = mx;
-      l[i] = l[i] * f + sum;
+      for (int j = 0; j < DP / 8; ++j) acc[j][2 * r] *= f, acc[j][2 * r + 1] *= f;
 #pragma unroll
-      for (int n = 0; n < DP / 16; ++n) acc[i][n] *= f;
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[t][2 * r + e] = ex2(s[t][2 * r + e] - base);
+          l[r] += s[t][2 * r + e];
+        }
     }
-    __syncwarp();  // a warp's rows of weights are its own
-    gather_tile<DP>(acc, sp, sv, ty, tx);
+    gather_tile<DP, NP>(acc, s, sv, lane);
   }
-  float inv[4];
+  float inv[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
-    const bool empty = l[i] == 0.0f;  // a row with a key sums to at least 1
-    inv[i] = empty ? 0.0f : 1.0f / l[i];
-    const int row = r0 + 4 * ty + i;
-    if (p.lse2 && tx == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : m[i] + log2f(l[i]);
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    const bool empty = l[r] == 0.0f;  // a row with a key sums to at least 1
+    inv[r] = empty ? 0.0f : 1.0f / l[r];
+    const int row = r0 + warp * 16 + (lane >> 2) + 8 * r;
+    if (p.lse2 && c == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : m[r] + log2f(l[r]);
   }
-  store_rows<T, DP>(p.o, acc, inv, p, b, p.Lq, p.H, h, r0, ty, tx);
+  store_rows<T, DP>(p.o, acc, inv[0], inv[1], p, b, p.Lq, p.H, h, r0 + warp * 16, lane);
 }
 
-template <typename T, int DP, bool VEC, int TM>
-__global__ void __launch_bounds__(kTileThreads<TM>) dq_kernel(const __grid_constant__ Params p) {
-  constexpr int NT = kTileThreads<TM>;
-  extern __shared__ float4 smem4[];
-  float* sq = reinterpret_cast<float*>(smem4);
-  float* sdo = sq + TM * row_floats<DP>;
-  float* sk = sdo + TM * row_floats<DP>;
-  float* sv = sk + kT * row_floats<DP>;
-  float* sds = sv + kT * row_floats<DP>;
-  __shared__ uint8_t okc[kT];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+// dq (KEYROWS false): rows are queries, columns keys, acc += ds k.
+// dk, dv (KEYROWS): rows are keys, columns queries, so the scores are formed transposed;
+// acc (dk) += ds^T q and acc2 (dv) += p^T do, over the query heads that share the key head one after another.
+template <typename T, int DP, bool VEC, int TM, bool KEYROWS>
+__global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_constant__ Params p) {
+  constexpr int NT = kTileThreads<TM>, NP = kPieces<T>;
+  extern __shared__ uint4 smem4[];
+  __nv_bfloat16* a0 = reinterpret_cast<__nv_bfloat16*>(smem4);  // q, do or k, v
+  __nv_bfloat16* a1 = a0 + (size_t)NP * TM * kLd<DP>;
+  __nv_bfloat16* b0 = a1 + (size_t)NP * TM * kLd<DP>;           // k, v or q, do
+  __nv_bfloat16* b1 = b0 + (size_t)NP * kT * kLd<DP>;
+  __shared__ uint8_t okc[kT];                  // of the keys
+  __shared__ float s_lse[kT], s_delta[kT];     // of the queries
+  constexpr int KROWS = KEYROWS ? TM : kT, QROWS = KEYROWS ? kT : TM;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3, g = lane >> 2;
   pdl_wait();
   pdl_trigger();
-  const int tiles = (p.Lq + TM - 1) / TM;
+  const int own = KEYROWS ? p.Lk : p.Lq, heads = KEYROWS ? p.Hkv : p.H, G = p.H / p.Hkv;
+  const int tiles = (own + TM - 1) / TM;
   const int r0 = (int)(blockIdx.x % tiles) * TM;
-  const int h = (int)(blockIdx.x / tiles % p.H);
-  const int64_t b = blockIdx.x / tiles / p.H;
-  const int hk = h / (p.H / p.Hkv);
-  const int nk = key_count(p, b);
+  const int h = (int)(blockIdx.x / tiles % heads);
+  const int64_t b = blockIdx.x / tiles / heads;
+  const int nk = key_count(p, b), ksteps = (p.D + 15) / 16;
   const float c2 = p.scale * kLog2e;
-  stage<T, DP, false, VEC, TM, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
-  stage<T, DP, false, VEC, TM, NT>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
-  float acc[4][DP / 16] = {}, lse[4], delta[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {  // rows past the end weigh nothing
-    const int row = r0 + 4 * ty + i;
-    const int64_t at = (b * p.H + h) * p.Lq + row;
-    lse[i] = row < p.Lq ? p.lse2[at] : INFINITY;
-    delta[i] = row < p.Lq ? p.delta[at] : 0.0f;
+  auto keys = [&](__nv_bfloat16* k, __nv_bfloat16* v, int hk, int k0) {
+    for (int i = threadIdx.x; i < KROWS; i += NT) okc[i] = key_ok(p, b, nk, k0 + i);
+    __syncthreads();
+    stage<T, DP, true, VEC, KROWS, NT>(k, p.k, p, b, hk, k0, nk, okc);
+    stage<T, DP, true, VEC, KROWS, NT>(v, p.v, p, b, hk, k0, nk, okc);
+  };
+  auto queries = [&](__nv_bfloat16* q, __nv_bfloat16* d, int hq, int q0) {
+    stage<T, DP, false, VEC, QROWS, NT>(q, p.q, p, b, hq, q0, p.Lq, nullptr);
+    stage<T, DP, false, VEC, QROWS, NT>(d, p.dout, p, b, hq, q0, p.Lq, nullptr);
+    for (int i = threadIdx.x; i < QROWS; i += NT) {  // rows past the end weigh nothing
+      const int64_t at = (b * p.H + hq) * p.Lq + q0 + i;
+      s_lse[i] = q0 + i < p.Lq ? p.lse2[at] : INFINITY;
+      s_delta[i] = q0 + i < p.Lq ? p.delta[at] : 0.0f;
+    }
+  };
+  float acc[DP / 8][4] = {}, acc2[KEYROWS ? DP / 8 : 1][4] = {};
+  const int n = KEYROWS ? p.Lq : nk;  // streamed rows of a head
+  const int loops = KEYROWS ? (r0 < nk ? G : 0) : 1;
+  if (loops > 0) {
+    if constexpr (KEYROWS) keys(a0, a1, h, r0);
+    else queries(a0, a1, h, r0);
   }
-  for (int k0 = 0; k0 < nk; k0 += kT) {
-    __syncthreads();
-    if (threadIdx.x < kT) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
-    __syncthreads();
-    stage<T, DP, true, VEC, kT, NT>(sk, p.k, p, b, hk, k0, nk, okc);
-    stage<T, DP, true, VEC, kT, NT>(sv, p.v, p, b, hk, k0, nk, okc);
-    __syncthreads();
-    float s[4][4] = {}, dp[4][4] = {};
-    dot_tile<DP>(s, sq, sk, ty, tx);
-    dot_tile<DP>(dp, sdo, sv, ty, tx);
+  for (int q = 0; q < loops; ++q)
+    for (int s0 = 0; s0 < n; s0 += kT) {
+      __syncthreads();
+      if constexpr (KEYROWS) queries(b0, b1, h * G + q, s0);
+      else keys(b0, b1, h / G, s0);
+      __syncthreads();
+      float s[8][4], d[8][4];
+      dot_tile<DP, NP, TM>(s, a0 + warp * 16 * kLd<DP>, b0, ksteps, lane);
+      dot_tile<DP, NP, TM>(d, a1 + warp * 16 * kLd<DP>, b1, ksteps, lane);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int t = 0; t < 8; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w = okc[tx + 16 * j] ? exp2f(s[i][j] * c2 - lse[i]) : 0.0f;
-        sds[(4 * ty + i) * (kT + 4) + tx + 16 * j] = w * (dp[i][j] - delta[i]);
-      }
-    __syncwarp();
-    gather_tile<DP>(acc, sds, sk, ty, tx);
-  }
-  const float f[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_rows<T, DP>(p.dq, acc, f, p, b, p.Lq, p.H, h, r0, ty, tx);
-}
-
-// Rows are keys, columns queries: the scores are formed transposed.
-template <typename T, int DP, bool VEC, int TM>
-__global__ void __launch_bounds__(kTileThreads<TM>) dkv_kernel(const __grid_constant__ Params p) {
-  constexpr int NT = kTileThreads<TM>;
-  extern __shared__ float4 smem4[];
-  float* sk = reinterpret_cast<float*>(smem4);
-  float* sv = sk + TM * row_floats<DP>;
-  float* sq = sv + TM * row_floats<DP>;
-  float* sdo = sq + kT * row_floats<DP>;
-  float* sp = sdo + kT * row_floats<DP>;
-  float* sds = sp + TM * (kT + 4);
-  __shared__ uint8_t okc[TM];
-  __shared__ float s_lse[kT], s_delta[kT];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  pdl_wait();
-  pdl_trigger();
-  const int tiles = (p.Lk + TM - 1) / TM;
-  const int k0 = (int)(blockIdx.x % tiles) * TM;
-  const int hk = (int)(blockIdx.x / tiles % p.Hkv);
-  const int64_t b = blockIdx.x / tiles / p.Hkv;
-  const int G = p.H / p.Hkv;
-  const int nk = key_count(p, b);
-  const float c2 = p.scale * kLog2e;
-  float dk[4][DP / 16] = {}, dv[4][DP / 16] = {};
-  if (k0 < nk) {
-    if (threadIdx.x < TM) okc[threadIdx.x] = key_ok(p, b, nk, k0 + threadIdx.x);
-    __syncthreads();
-    stage<T, DP, true, VEC, TM, NT>(sk, p.k, p, b, hk, k0, nk, okc);
-    stage<T, DP, true, VEC, TM, NT>(sv, p.v, p, b, hk, k0, nk, okc);
-    // the query heads that share this key head, one after another: a fixed order
-    for (int g = 0; g < G; ++g)
-      for (int r0 = 0; r0 < p.Lq; r0 += kT) {
-        const int h = hk * G + g;
-        __syncthreads();
-        stage<T, DP, false, VEC, kT, NT>(sq, p.q, p, b, h, r0, p.Lq, nullptr);
-        stage<T, DP, false, VEC, kT, NT>(sdo, p.dout, p, b, h, r0, p.Lq, nullptr);
-        if (threadIdx.x < kT) {  // rows past the end weigh nothing
-          const int row = r0 + threadIdx.x;
-          const int64_t at = (b * p.H + h) * p.Lq + row;
-          s_lse[threadIdx.x] = row < p.Lq ? p.lse2[at] : INFINITY;
-          s_delta[threadIdx.x] = row < p.Lq ? p.delta[at] : 0.0f;
+        for (int e = 0; e < 4; ++e) {
+          const int row = warp * 16 + g + 8 * (e >> 1), col = t * 8 + 2 * c + (e & 1);
+          const int key = KEYROWS ? row : col, query = KEYROWS ? col : row;
+          s[t][e] = okc[key] ? ex2(s[t][e] * c2 - s_lse[query]) : 0.0f;
+          d[t][e] = okc[key] ? s[t][e] * (d[t][e] - s_delta[query]) : 0.0f;
         }
-        __syncthreads();
-        float s[4][4] = {}, dp[4][4] = {};
-        dot_tile<DP>(s, sk, sq, ty, tx);
-        dot_tile<DP>(dp, sv, sdo, ty, tx);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lse = s_lse[tx + 16 * j], delta = s_delta[tx + 16 * j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float w = okc[4 * ty + i] ? exp2f(s[i][j] * c2 - lse) : 0.0f;
-            const int at = (4 * ty + i) * (kT + 4) + tx + 16 * j;
-            sp[at] = w;
-            sds[at] = w * (dp[i][j] - delta);
-          }
-        }
-        __syncwarp();
-        gather_tile<DP>(dv, sp, sdo, ty, tx);
-        gather_tile<DP>(dk, sds, sq, ty, tx);
-      }
+      gather_tile<DP, NP>(acc, d, b0, lane);
+      if constexpr (KEYROWS) gather_tile<DP, NP>(acc2, s, b1, lane);
+    }
+  const int row = r0 + warp * 16;
+  if constexpr (KEYROWS) {
+    store_rows<T, DP>(p.dk, acc, p.scale, p.scale, p, b, p.Lk, p.Hkv, h, row, lane);
+    store_rows<T, DP>(p.dv, acc2, 1.0f, 1.0f, p, b, p.Lk, p.Hkv, h, row, lane);
+  } else {
+    store_rows<T, DP>(p.dq, acc, p.scale, p.scale, p, b, p.Lq, p.H, h, row, lane);
   }
-  const float one[4] = {1.0f, 1.0f, 1.0f, 1.0f}, f[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_rows<T, DP>(p.dk, dk, f, p, b, p.Lk, p.Hkv, hk, k0, ty, tx);
-  store_rows<T, DP>(p.dv, dv, one, p, b, p.Lk, p.Hkv, hk, k0, ty, tx);
 }
 
 // delta_i = do_i . o_i, one warp a row.
@@ -353,17 +363,16 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__
 
 template <typename T, int DP, bool VEC, int TM>
 int launch_rows(const Params& p, int which, cudaStream_t st) {  // 0 forward, 1 dq, 2 dk and dv
-  constexpr int NT = kTileThreads<TM>;
   const int64_t rows = which == 2 ? p.Lk : p.Lq, heads = which == 2 ? p.Hkv : p.H;
   const int64_t grid = (rows + TM - 1) / TM * heads * p.B;
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
   if (grid == 0) return HCLSM_OK;
-  const size_t bytes = which == 0   ? smem_bytes<DP, TM, 1, 2, 1>()
-                       : which == 1 ? smem_bytes<DP, TM, 2, 2, 1>()
-                                    : smem_bytes<DP, TM, 2, 2, 2>();
-  auto f = which == 0 ? fwd_kernel<T, DP, VEC, TM> : which == 1 ? dq_kernel<T, DP, VEC, TM> : dkv_kernel<T, DP, VEC, TM>;
+  const size_t bytes = which == 0 ? smem_bytes<T, DP, TM, 1>() : smem_bytes<T, DP, TM, 2>();
+  auto f = which == 0   ? fwd_kernel<T, DP, VEC, TM>
+           : which == 1 ? bwd_kernel<T, DP, VEC, TM, false>
+                        : bwd_kernel<T, DP, VEC, TM, true>;
   if (!set_smem_limit(reinterpret_cast<const void*>(f), bytes)) return HCLSM_ERR_LAUNCH;
-  return launch_pdl(f, (unsigned)grid, NT, bytes, st, p);
+  return launch_pdl(f, (unsigned)grid, kTileThreads<TM>, bytes, st, p);
 }
 
 template <typename T, int DP, bool VEC>
