@@ -1,8 +1,9 @@
 // Cross attention: the kernels that serve every type, head size, stride and
 // alignment, and the C entry points.
 //
-// A block keeps TM rows (queries; keys for dk and dv), 16 a warp, and walks over tiles
-// of 64 of the other side with mma.sync m16n8k16 products.  An fp32 operand is split
+// A block keeps TM rows (queries; keys for dk and dv) and walks over tiles of 64 of the
+// other side with mma.sync m16n8k16 products; a warp takes 16 rows and half of each
+// tile, and the halves are added in order at the end.  An fp32 operand is split
 // into three bf16 pieces (8 bits each) when it is staged, one shared-memory plane a
 // piece, and the six products of pieces whose order is at most 2 are formed from zero
 // and added in fp32: the result is as exact as fp32 arithmetic, at a sixth of the bf16
@@ -18,7 +19,8 @@ namespace xattn {
 
 constexpr int kT = 64;  // rows of a streamed tile
 constexpr int kThreads = 256;  // of the row-wise kernel
-template <int TM> constexpr int kTileThreads = TM * 2;
+constexpr int kHalf = kT / 2;  // of it a warp takes
+template <int TM> constexpr int kTileThreads = TM * 4;
 template <typename T> constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
 template <int DP> constexpr int kLd = DP + 8;
 
@@ -102,55 +104,57 @@ __device__ __forceinline__ void stage(__nv_bfloat16* dst, const View& x, const P
   }
 }
 
-// acc += the products of the pieces a[i] and b[j], order i + j at most NP - 1, smallest first.
+// Four tiles' acc += the products of the pieces a[i] and b[j], order i + j at most NP - 1, smallest first.  b: of two
+// pairs of tiles.  The tiles go side by side, because one tile's products wait for each other.
 template <int NP>
-__device__ __forceinline__ void product(float (&acc)[4], const uint32_t (&a)[NP][4], const uint32_t (&b)[NP][4], int t) {
+__device__ __forceinline__ void product4(float (*acc)[4], const uint32_t (&a)[NP][4], const uint32_t (&b)[2][NP][4]) {
   if constexpr (NP == 1) {
-    mma(acc, a[0], b[0][2 * t], b[0][2 * t + 1]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) mma(acc[t], a[0], b[t >> 1][0][2 * (t & 1)], b[t >> 1][0][2 * (t & 1) + 1]);
   } else {
-    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float part[4][4] = {};
 #pragma unroll
     for (int i = NP - 1; i >= 0; --i)
 #pragma unroll
-      for (int j = NP - 1 - i; j >= 0; --j) mma(part, a[i], b[j][2 * t], b[j][2 * t + 1]);
+      for (int j = NP - 1 - i; j >= 0; --j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += part[e];
+        for (int t = 0; t < 4; ++t) mma(part[t], a[i], b[t >> 1][j][2 * (t & 1)], b[t >> 1][j][2 * (t & 1) + 1]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] += part[t][e];
   }
 }
 
-// s (the warp's 16 rows x 64) = own rows . streamed rows: a at the warp's first row, b the tile.
+// s (the warp's 16 rows x 32) = own rows . streamed rows: a at the warp's first row, b at its first streamed one.
 template <int DP, int NP, int ROWS>
-__device__ __forceinline__ void dot_tile(float (&s)[8][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int ksteps,
+__device__ __forceinline__ void dot_tile(float (&s)[4][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int ksteps,
                                          int lane) {
 #pragma unroll
-  for (int t = 0; t < 8; ++t)
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
-#pragma unroll 1
+#pragma unroll 2
   for (int k = 0; k < ksteps; ++k) {
-    uint32_t fa[NP][4];
+    uint32_t fa[NP][4], fb[2][NP][4];
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
+    for (int i = 0; i < NP; ++i) {
       ldmatrix4<false>(fa[i], a + (size_t)i * ROWS * kLd<DP> + (lane & 15) * kLd<DP> + k * 16 + (lane >> 4) * 8);
 #pragma unroll
-    for (int t = 0; t < 8; t += 2) {
-      uint32_t fb[NP][4];
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        ldmatrix4<false>(fb[i], b + ((size_t)i * kT + t * 8 + (lane >> 4) * 8 + (lane & 7)) * kLd<DP> + k * 16 +
-                                    (lane >> 3 & 1) * 8);
-      product<NP>(s[t], fa, fb, 0);
-      product<NP>(s[t + 1], fa, fb, 1);
+      for (int t = 0; t < 2; ++t)
+        ldmatrix4<false>(fb[t][i], b + ((size_t)i * kT + t * 16 + (lane >> 4) * 8 + (lane & 7)) * kLd<DP> + k * 16 +
+                                       (lane >> 3 & 1) * 8);
     }
+    product4<NP>(s, fa, fb);
   }
 }
 
-// acc (16 rows x DP) += w (16 x 64, as dot_tile leaves its products) x the streamed tile.
+// acc (16 rows x DP) += w (16 x 32, as dot_tile leaves its products) x the streamed rows at x.
 template <int DP, int NP>
-__device__ __forceinline__ void gather_tile(float (&acc)[DP / 8][4], const float (&w)[8][4], const __nv_bfloat16* x,
+__device__ __forceinline__ void gather_tile(float (&acc)[DP / 8][4], const float (&w)[4][4], const __nv_bfloat16* x,
                                             int lane) {
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
+  for (int u = 0; u < 2; ++u) {
     uint32_t fa[NP][4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -160,27 +164,51 @@ __device__ __forceinline__ void gather_tile(float (&acc)[DP / 8][4], const float
       for (int i = 0; i < NP; ++i) fa[i][e] = t[i];
     }
 #pragma unroll
-    for (int j = 0; j < DP / 8; j += 2) {
-      uint32_t fb[NP][4];
+    for (int j = 0; j < DP / 8; j += 4) {
+      uint32_t fb[2][NP][4];
 #pragma unroll
       for (int i = 0; i < NP; ++i)
-        ldmatrix4<true>(fb[i], x + ((size_t)i * kT + u * 16 + (lane & 15)) * kLd<DP> + j * 8 + (lane >> 4) * 8);
-      product<NP>(acc[j], fa, fb, 0);
-      product<NP>(acc[j + 1], fa, fb, 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          ldmatrix4<true>(fb[t][i], x + ((size_t)i * kT + u * 16 + (lane & 15)) * kLd<DP> + j * 8 + t * 16 + (lane >> 4) * 8);
+      product4<NP>(acc + j, fa, fb);
     }
   }
 }
 
+// The second half's accumulator rows through shared memory (fp32 [rows][DP]): put, then the first half's warps add.
+template <int DP>
+__device__ __forceinline__ void put_rows(float* dst, const float (&acc)[DP / 8][4], int lane) {
+#pragma unroll
+  for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      *reinterpret_cast<float2*>(dst + ((lane >> 2) + 8 * r) * DP + j * 8 + 2 * (lane & 3)) =
+          make_float2(acc[j][2 * r], acc[j][2 * r + 1]);
+}
+// acc = acc * f[row] + src * g[row]
+template <int DP>
+__device__ __forceinline__ void join_rows(float (&acc)[DP / 8][4], const float* src, const float (&f)[2],
+                                          const float (&g)[2], int lane) {
+#pragma unroll
+  for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float2 v =
+          *reinterpret_cast<const float2*>(src + ((lane >> 2) + 8 * r) * DP + j * 8 + 2 * (lane & 3));
+      acc[j][2 * r] = acc[j][2 * r] * f[r] + v.x * g[r];
+      acc[j][2 * r + 1] = acc[j][2 * r + 1] * f[r] + v.y * g[r];
+    }
+}
+
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8][4], float f0, float f1,
-                                           const Params& p, int64_t b, int L, int H, int h, int r0, int lane) {
+__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8][4], float f, const Params& p, int64_t b, int L, int H, int h, int r0, int lane) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int row = r0 + g + 8 * r;
     if (row >= L) continue;
     T* out = static_cast<T*>(dst) + ((b * L + row) * H + h) * (int64_t)p.D;
-    const float f = r ? f1 : f0;
 #pragma unroll
     for (int j = 0; j < DP / 8; ++j)
 #pragma unroll
@@ -193,7 +221,9 @@ __device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8]
 
 // Shared memory of a block: NA operands of TM rows and two of 64.
 template <typename T, int DP, int TM, int NA> constexpr size_t smem_bytes() {
-  return (size_t)kPieces<T> * (NA * TM + 2 * kT) * kLd<DP> * sizeof(__nv_bfloat16);
+  const size_t planes = (size_t)kPieces<T> * (NA * TM + 2 * kT) * kLd<DP> * sizeof(__nv_bfloat16);
+  const size_t halves = (size_t)NA * TM * DP * sizeof(float);
+  return planes > halves ? planes : halves;
 }
 
 template <typename T, int DP, bool VEC, int TM>
@@ -204,7 +234,9 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
   __nv_bfloat16* sk = sq + (size_t)NP * TM * kLd<DP>;
   __nv_bfloat16* sv = sk + (size_t)NP * kT * kLd<DP>;
   __shared__ uint8_t okc[kT];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3;
+  __shared__ float s_m[TM], s_l[TM];
+  const int lane = threadIdx.x & 31, c = lane & 3, g = lane >> 2;
+  const int rw = (threadIdx.x >> 5) % (TM / 16) * 16, half = (threadIdx.x >> 5) / (TM / 16);  // the warp's rows, keys
   pdl_wait();
   pdl_trigger();
   const int tiles = (p.Lq + TM - 1) / TM;
@@ -223,14 +255,14 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
     stage<T, DP, true, VEC, kT, NT>(sk, p.k, p, b, hk, k0, nk, okc);
     stage<T, DP, true, VEC, kT, NT>(sv, p.v, p, b, hk, k0, nk, okc);
     __syncthreads();
-    float s[8][4];
-    dot_tile<DP, NP, TM>(s, sq + warp * 16 * kLd<DP>, sk, ksteps, lane);
+    float s[4][4];
+    dot_tile<DP, NP, TM>(s, sq + rw * kLd<DP>, sk + half * kHalf * kLd<DP>, ksteps, lane);
     float mx[2] = {m[0], m[1]};
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[t][e] = okc[t * 8 + 2 * c + (e & 1)] ? s[t][e] * c2 : -INFINITY;
+        s[t][e] = okc[half * kHalf + t * 8 + 2 * c + (e & 1)] ? s[t][e] * c2 : -INFINITY;
         mx[e >> 1] = fmaxf(mx[e >> 1], s[t][e]);
       }
 #pragma unroll
@@ -244,26 +276,42 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < DP / 8; ++j) acc[j][2 * r] *= f, acc[j][2 * r + 1] *= f;
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           s[t][2 * r + e] = ex2(s[t][2 * r + e] - base);
           l[r] += s[t][2 * r + e];
         }
     }
-    gather_tile<DP, NP>(acc, s, sv, lane);
+    gather_tile<DP, NP>(acc, s, sv + half * kHalf * kLd<DP>, lane);
   }
-  float inv[2];
+  __syncthreads();  // the tiles are done with
+  float* other = reinterpret_cast<float*>(smem4) + (size_t)rw * DP;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const bool empty = l[r] == 0.0f;  // a row with a key sums to at least 1
-    inv[r] = empty ? 0.0f : 1.0f / l[r];
-    const int row = r0 + warp * 16 + (lane >> 2) + 8 * r;
-    if (p.lse2 && c == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : m[r] + log2f(l[r]);
+    if (half && c == 0) s_m[rw + g + 8 * r] = m[r], s_l[rw + g + 8 * r] = l[r];
   }
-  store_rows<T, DP>(p.o, acc, inv[0], inv[1], p, b, p.Lq, p.H, h, r0 + warp * 16, lane);
+  if (half) put_rows<DP>(other, acc, lane);
+  __syncthreads();
+  if (half) return;
+  float f0[2], f1[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float m1 = s_m[rw + g + 8 * r], l1 = s_l[rw + g + 8 * r], mx = fmaxf(m[r], m1);
+    // a half without a maximum holds zeros, or NaN that has to stay
+    f0[r] = m[r] == -INFINITY ? 1.0f : ex2(m[r] - mx);
+    f1[r] = m1 == -INFINITY ? 1.0f : ex2(m1 - mx);
+    const float sum = l[r] * f0[r] + l1 * f1[r];
+    const bool empty = sum == 0.0f;  // a row with a key sums to at least 1
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    f0[r] *= inv, f1[r] *= inv;
+    const int row = r0 + rw + g + 8 * r;
+    if (p.lse2 && c == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : mx + log2f(sum);
+  }
+  join_rows<DP>(acc, other, f0, f1, lane);
+  store_rows<T, DP>(p.o, acc, 1.0f, p, b, p.Lq, p.H, h, r0 + rw, lane);
 }
 
 // dq (KEYROWS false): rows are queries, columns keys, acc += ds k.
@@ -280,7 +328,8 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
   __shared__ uint8_t okc[kT];                  // of the keys
   __shared__ float s_lse[kT], s_delta[kT];     // of the queries
   constexpr int KROWS = KEYROWS ? TM : kT, QROWS = KEYROWS ? kT : TM;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane & 3, g = lane >> 2;
+  const int lane = threadIdx.x & 31, c = lane & 3, g = lane >> 2;
+  const int rw = (threadIdx.x >> 5) % (TM / 16) * 16, half = (threadIdx.x >> 5) / (TM / 16);
   pdl_wait();
   pdl_trigger();
   const int own = KEYROWS ? p.Lk : p.Lq, heads = KEYROWS ? p.Hkv : p.H, G = p.H / p.Hkv;
@@ -318,27 +367,38 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
       if constexpr (KEYROWS) queries(b0, b1, h * G + q, s0);
       else keys(b0, b1, h / G, s0);
       __syncthreads();
-      float s[8][4], d[8][4];
-      dot_tile<DP, NP, TM>(s, a0 + warp * 16 * kLd<DP>, b0, ksteps, lane);
-      dot_tile<DP, NP, TM>(d, a1 + warp * 16 * kLd<DP>, b1, ksteps, lane);
+      float s[4][4], d[4][4];
+      const int at = half * kHalf * kLd<DP>;
+      dot_tile<DP, NP, TM>(s, a0 + rw * kLd<DP>, b0 + at, ksteps, lane);
+      dot_tile<DP, NP, TM>(d, a1 + rw * kLd<DP>, b1 + at, ksteps, lane);
 #pragma unroll
-      for (int t = 0; t < 8; ++t)
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = warp * 16 + g + 8 * (e >> 1), col = t * 8 + 2 * c + (e & 1);
+          const int row = rw + g + 8 * (e >> 1), col = half * kHalf + t * 8 + 2 * c + (e & 1);
           const int key = KEYROWS ? row : col, query = KEYROWS ? col : row;
           s[t][e] = okc[key] ? ex2(s[t][e] * c2 - s_lse[query]) : 0.0f;
           d[t][e] = okc[key] ? s[t][e] * (d[t][e] - s_delta[query]) : 0.0f;
         }
-      gather_tile<DP, NP>(acc, d, b0, lane);
-      if constexpr (KEYROWS) gather_tile<DP, NP>(acc2, s, b1, lane);
+      gather_tile<DP, NP>(acc, d, b0 + at, lane);
+      if constexpr (KEYROWS) gather_tile<DP, NP>(acc2, s, b1 + at, lane);
     }
-  const int row = r0 + warp * 16;
+  __syncthreads();  // the tiles are done with
+  float* other = reinterpret_cast<float*>(smem4) + (size_t)rw * DP;
+  if (half) {
+    put_rows<DP>(other, acc, lane);
+    if constexpr (KEYROWS) put_rows<DP>(other + TM * DP, acc2, lane);
+  }
+  __syncthreads();
+  if (half) return;
+  const float one[2] = {1.0f, 1.0f};
+  join_rows<DP>(acc, other, one, one, lane);
   if constexpr (KEYROWS) {
-    store_rows<T, DP>(p.dk, acc, p.scale, p.scale, p, b, p.Lk, p.Hkv, h, row, lane);
-    store_rows<T, DP>(p.dv, acc2, 1.0f, 1.0f, p, b, p.Lk, p.Hkv, h, row, lane);
+    join_rows<DP>(acc2, other + TM * DP, one, one, lane);
+    store_rows<T, DP>(p.dk, acc, p.scale, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
+    store_rows<T, DP>(p.dv, acc2, 1.0f, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
   } else {
-    store_rows<T, DP>(p.dq, acc, p.scale, p.scale, p, b, p.Lq, p.H, h, row, lane);
+    store_rows<T, DP>(p.dq, acc, p.scale, p, b, p.Lq, p.H, h, r0 + rw, lane);
   }
 }
 
