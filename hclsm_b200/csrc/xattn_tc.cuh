@@ -57,19 +57,6 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, const uint4& w, i
   __syncwarp();
 }
 
-// The 256 threads of a tile (two warpgroups): a barrier, and one that says whether any of them asks.
-__device__ __forceinline__ void bar_sync(int id) { asm volatile("bar.sync %0, 256;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool bar_any(int id, bool ask) {
-  uint32_t r;
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred.aligned q, %1, 256, p;\n selp.u32 %0, 1, 0, "
-      "q;\n}\n"
-      : "=r"(r)
-      : "r"(id), "r"((uint32_t)ask)
-      : "memory");
-  return r != 0;
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

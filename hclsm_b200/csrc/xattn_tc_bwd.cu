@@ -12,9 +12,8 @@
 //
 // The weights and their gradients are A operands in TMEM; the same staged tile of
 // K (or Q, dO) is the K-major operand of one product and the MN-major operand of
-// another.  Two buffers of 64 + 64 columns, two warpgroups (thread = half a row) to
-// each: the tensor cores form one buffer's products while the other's weights are
-// computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
+// another.  Two buffers of 64 + 64 columns, a warpgroup (thread = row) to each: the
+// tensor cores form one buffer's products while the other's weights are computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
 // (128 or 256) do not fit TMEM's 512.
 #include "xattn_tc.cuh"
 
@@ -29,7 +28,7 @@ template <int DP> struct BwdShape {
   static constexpr int kStages = 4;
   static constexpr int kBars = 1 + 2 * kStages + 4 + 1;
   static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
-  static constexpr int kThreads = 4 * 128 + 64;
+  static constexpr int kThreads = 2 * 128 + 64;
 };
 
 // Shared by the two kernels: block layout, barriers, roles.
@@ -45,7 +44,7 @@ template <int DP> struct Block {
     done = ds_full + 2;
   }
   __device__ __forceinline__ void init() const {
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 256 : 1);
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 128 : 1);
     fence_mbar_init();
   }
   // What the issuing thread computes once.
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   __shared__ volatile int s_abort;
   const Block<DP> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 16, kMmaWarp = 17;
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (j + 2 < tiles) ok = start(j + 2);
     }
   } else {
-    const int w = warp >> 3, half = warp >> 2 & 1;
+    const int w = warp >> 2;
     const int row = q0 + (tid & 127);
     const bool idle = q0 + (warp & 3) * 32 >= x.Lq;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -204,35 +203,36 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     bool ok = true;
     for (int j = w; j < tiles; j += 2) {
       const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
-      const uint32_t word = j & 1 ? (half ? bits.w : bits.z) : (half ? bits.y : bits.x);
-      if (ok) ok = wait_all(&blk.sd_full[w], j >> 1);
+      const uint32_t word[2] = {j & 1 ? bits.z : bits.x, j & 1 ? bits.w : bits.y};
+      if (!(ok = wait_all(&blk.sd_full[w], j >> 1))) break;
       tc_fence_after();
-      float s[32], g[32];
-      if (ok && !idle) {
-        tmem_ld32_nowait(tS + half * 32, s);
-        tmem_ld32_nowait(tS + 64 + half * 32, g);
-        tmem_wait_ld();
-        tmem_pin<32>(s);
-        tmem_pin<32>(g);
-      }
-      bar_sync(1 + w);  // both halves' scores are read before weights go over them
-      if (!ok) continue;
       if (!idle) {
-        uint32_t r[16];
+        float s[2][32], g[2][32];
+        tmem_ld32_nowait(tS, s[0]);
+        tmem_ld32_nowait(tS + 64, g[0]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
-          e.x = ex2(e.x), e.y = ex2(e.y);
-          const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
-          s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
+        for (int c = 0; c < 2; ++c) {
+          tmem_wait_ld();
+          tmem_pin<32>(s[c]);
+          tmem_pin<32>(g[c]);
+          if (c == 0) {
+            tmem_ld32_nowait(tS + 32, s[1]);
+            tmem_ld32_nowait(tS + 96, g[1]);
+          }
+          uint32_t r[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float2 e = fma2(make_float2(s[c][2 * i], s[c][2 * i + 1]), cc, ll);
+            e.x = ex2(e.x), e.y = ex2(e.y);
+            e = mul2(e, add2(make_float2(g[c][2 * i], g[c][2 * i + 1]), dd));
+            if (word[c] != 0xffffffffu) {
+              e.x = word[c] >> (2 * i) & 1u ? e.x : 0.0f;
+              e.y = word[c] >> (2 * i + 1) & 1u ? e.y : 0.0f;
+            }
+            r[i] = pack_bf16(e.x, e.y);
+          }
+          tmem_st16(tS + c * 16, r);
         }
-        if (word != 0xffffffffu) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = word >> i & 1u ? s[i] : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
-        tmem_st16(tS + half * 16, r);
         tmem_wait_st();
       }
       tc_fence_before();
@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     if (ok && tiles > 0) wait_all(blk.done, 0);
     tc_fence_after();
     if (!idle)
-      store_acc<DP / 4>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
-                        row < x.Lq, tiles == 0, (2 * w + half) * (DP / 4), x.D, x.scale);
+      store_acc<DP / 2>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
+                        row < x.Lq, tiles == 0, w * (DP / 2), x.D, x.scale);
   }
   tc_fence_before();
   __syncthreads();
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   __shared__ float4 s_stat[2][2][2][kB / 4];  // warpgroup, slot, (-lse2, -delta)
   const Block<DP> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 16, kMmaWarp = 17;
+  constexpr int kTmaWarp = 8, kMmaWarp = 9;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (i + 2 < tiles) ok = start(i + 2);
     }
   } else {
-    const int w = warp >> 3, half = warp >> 2 & 1, t = tid & 127;
+    const int w = warp >> 2, t = tid & 127;
     const int key = k0 + t;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128;
@@ -336,46 +336,42 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (t < 64) return i < tiles && r < x.Lq ? -x.lse2[at] : -INFINITY;
       return i < tiles && r < x.Lq ? -x.delta[at] : 0.0f;
     };
-    float next = half ? 0.0f : stat(w);
+    float next = stat(w);
     bool ok = true;
     for (int i = w; i < tiles; i += 2) {
       float4* st = s_stat[w][i >> 1 & 1][0];
-      if (half == 0) {
-        reinterpret_cast<float*>(st)[t] = next;
-        next = stat(i + 2);
-      }
+      reinterpret_cast<float*>(st)[t] = next;
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + w) : "memory");
+      next = stat(i + 2);
       if (ok) ok = wait_all(&blk.sd_full[w], i >> 1);
-      tc_fence_after();
-      float s[32], g[32];
-      if (ok) {
-        tmem_ld32_nowait(tS + half * 32, s);
-        tmem_ld32_nowait(tS + 64 + half * 32, g);
-        tmem_wait_ld();
-        tmem_pin<32>(s);
-        tmem_pin<32>(g);
-      }
-      // the statistics are there, and both halves' scores are read before weights go over them
-      bar_sync(1 + w);
       if (!ok) continue;  // given up: the others still meet at the barrier
-      {
+      tc_fence_after();
+      float s[2][32], g[2][32];
+      tmem_ld32_nowait(tS, s[0]);
+      tmem_ld32_nowait(tS + 64, g[0]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tmem_wait_ld();
+        tmem_pin<32>(s[c]);
+        tmem_pin<32>(g[c]);
+        if (c == 0) {
+          tmem_ld32_nowait(tS + 32, s[1]);
+          tmem_ld32_nowait(tS + 96, g[1]);
+        }
         uint32_t pw[16], dw[16];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const float4 l = st[half * 8 + q], d = st[kB / 4 + half * 8 + q];
-          float2 e0 = fma2(make_float2(s[4 * q], s[4 * q + 1]), cc, make_float2(l.x, l.y));
-          float2 e1 = fma2(make_float2(s[4 * q + 2], s[4 * q + 3]), cc, make_float2(l.z, l.w));
+          const float4 l = st[c * 8 + q], d = st[kB / 4 + c * 8 + q];
+          float2 e0 = fma2(make_float2(s[c][4 * q], s[c][4 * q + 1]), cc, make_float2(l.x, l.y));
+          float2 e1 = fma2(make_float2(s[c][4 * q + 2], s[c][4 * q + 3]), cc, make_float2(l.z, l.w));
           e0.x = ex2(e0.x), e0.y = ex2(e0.y), e1.x = ex2(e1.x), e1.y = ex2(e1.y);
-          const float2 d0 = add2(make_float2(g[4 * q], g[4 * q + 1]), make_float2(d.x, d.y));
-          const float2 d1 = add2(make_float2(g[4 * q + 2], g[4 * q + 3]), make_float2(d.z, d.w));
-          pw[2 * q] = pack_bf16(e0.x, e0.y), pw[2 * q + 1] = pack_bf16(e1.x, e1.y);
-          dw[2 * q] = pack_bf16(e0.x * d0.x, e0.y * d0.y), dw[2 * q + 1] = pack_bf16(e1.x * d1.x, e1.y * d1.y);
+          const float2 d0 = mul2(e0, add2(make_float2(g[c][4 * q], g[c][4 * q + 1]), make_float2(d.x, d.y)));
+          const float2 d1 = mul2(e1, add2(make_float2(g[c][4 * q + 2], g[c][4 * q + 3]), make_float2(d.z, d.w)));
+          pw[2 * q] = allowed ? pack_bf16(e0.x, e0.y) : 0u, pw[2 * q + 1] = allowed ? pack_bf16(e1.x, e1.y) : 0u;
+          dw[2 * q] = allowed ? pack_bf16(d0.x, d0.y) : 0u, dw[2 * q + 1] = allowed ? pack_bf16(d1.x, d1.y) : 0u;
         }
-        if (!allowed) {
-#pragma unroll
-          for (int q = 0; q < 16; ++q) pw[q] = dw[q] = 0;
-        }
-        tmem_st16(tS + half * 16, pw);
-        tmem_st16(tS + 64 + half * 16, dw);
+        tmem_st16(tS + c * 16, pw);
+        tmem_st16(tS + 64 + c * 16, dw);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -384,8 +380,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     if (ok && tiles > 0) wait_all(blk.done, 0);
     tc_fence_after();
     const int64_t at = ((b * x.Lk + key) * x.Hkv + hk) * (int64_t)x.D;
-    store_acc<DP / 2>((w ? acc_k : acc_v) + lanes, static_cast<__nv_bfloat16*>(w ? x.dk : x.dv) + at, key < x.Lk,
-                      tiles == 0, half * (DP / 2), x.D, w ? x.scale : 1.0f);
+    store_acc<DP>((w ? acc_k : acc_v) + lanes, static_cast<__nv_bfloat16*>(w ? x.dk : x.dv) + at, key < x.Lk,
+                  tiles == 0, 0, x.D, w ? x.scale : 1.0f);
   }
   tc_fence_before();
   __syncthreads();
