@@ -12,8 +12,8 @@
 //
 // The weights and their gradients are A operands in TMEM; the same staged tile of
 // K (or Q, dO) is the K-major operand of one product and the MN-major operand of
-// another.  Two buffers of 64 + 64 columns, a warpgroup (thread = row) to each: the
-// tensor cores form one buffer's products while the other's weights are computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
+// another.  Two buffers of 64 + 64 columns with warpgroups of their own: the tensor
+// cores form one buffer's products while the other's weights are computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
 // (128 or 256) do not fit TMEM's 512.
 #include "xattn_tc.cuh"
 
@@ -28,7 +28,11 @@ template <int DP> struct BwdShape {
   static constexpr int kStages = 4;
   static constexpr int kBars = 1 + 2 * kStages + 4 + 1;
   static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
-  static constexpr int kThreads = 2 * 128 + 64;
+  // Warpgroups a buffer: dq two (thread = half a row), dk and dv one (thread = row, whose
+  // two results of 64 columns would spill the 96 registers that four warpgroups have).
+  // 8 x 2048 x 4096, 16 heads of 128: dq 864 us with one, 740 with two; dk, dv 840 with
+  // one, 1150 with two.
+  static constexpr int kDqThreads = 4 * 128 + 64, kDkvThreads = 2 * 128 + 64;
 };
 
 // Shared by the two kernels: block layout, barriers, roles.
@@ -43,8 +47,8 @@ template <int DP> struct Block {
     full = own + 1, empty = full + Sh::kStages, sd_full = empty + Sh::kStages, ds_full = sd_full + 2,
     done = ds_full + 2;
   }
-  __device__ __forceinline__ void init() const {
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? 128 : 1);
+  __device__ __forceinline__ void init(int threads) const {  // of a buffer
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? threads : 1);
     fence_mbar_init();
   }
   // What the issuing thread computes once.
@@ -120,7 +124,7 @@ __device__ __forceinline__ void store_acc(uint32_t t, __nv_bfloat16* out, bool o
 }
 
 template <int DP>
-__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
     tc_dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
                  const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                  const __grid_constant__ TcParams p) {
@@ -130,11 +134,11 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   __shared__ volatile int s_abort;
   const Block<DP> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 8, kMmaWarp = 9;
+  constexpr int kTmaWarp = 16, kMmaWarp = 17;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
-    blk.init();
+    blk.init(256);
   }
   tc_fence_before();
   __syncthreads();
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
       if (j + 2 < tiles) ok = start(j + 2);
     }
   } else {
-    const int w = warp >> 2;
+    const int w = warp >> 3, half = warp >> 2 & 1;
     const int row = q0 + (tid & 127);
     const bool idle = q0 + (warp & 3) * 32 >= x.Lq;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -203,36 +207,35 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     bool ok = true;
     for (int j = w; j < tiles; j += 2) {
       const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
-      const uint32_t word[2] = {j & 1 ? bits.z : bits.x, j & 1 ? bits.w : bits.y};
-      if (!(ok = wait_all(&blk.sd_full[w], j >> 1))) break;
+      const uint32_t word = j & 1 ? (half ? bits.w : bits.z) : (half ? bits.y : bits.x);
+      if (ok) ok = wait_all(&blk.sd_full[w], j >> 1);
       tc_fence_after();
+      float s[32], g[32];
+      if (ok && !idle) {
+        tmem_ld32_nowait(tS + half * 32, s);
+        tmem_ld32_nowait(tS + 64 + half * 32, g);
+        tmem_wait_ld();
+        tmem_pin<32>(s);
+        tmem_pin<32>(g);
+      }
+      asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory");  // both halves' scores are read before weights go over them
+      if (!ok) continue;
       if (!idle) {
-        float s[2][32], g[2][32];
-        tmem_ld32_nowait(tS, s[0]);
-        tmem_ld32_nowait(tS + 64, g[0]);
+        uint32_t r[16];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          tmem_wait_ld();
-          tmem_pin<32>(s[c]);
-          tmem_pin<32>(g[c]);
-          if (c == 0) {
-            tmem_ld32_nowait(tS + 32, s[1]);
-            tmem_ld32_nowait(tS + 96, g[1]);
-          }
-          uint32_t r[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = fma2(make_float2(s[c][2 * i], s[c][2 * i + 1]), cc, ll);
-            e.x = ex2(e.x), e.y = ex2(e.y);
-            e = mul2(e, add2(make_float2(g[c][2 * i], g[c][2 * i + 1]), dd));
-            if (word[c] != 0xffffffffu) {
-              e.x = word[c] >> (2 * i) & 1u ? e.x : 0.0f;
-              e.y = word[c] >> (2 * i + 1) & 1u ? e.y : 0.0f;
-            }
-            r[i] = pack_bf16(e.x, e.y);
-          }
-          tmem_st16(tS + c * 16, r);
+        for (int i = 0; i < 16; ++i) {
+          float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
+          e.x = ex2(e.x), e.y = ex2(e.y);
+          const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
+          s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
         }
+        if (word != 0xffffffffu) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = word >> i & 1u ? s[i] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
+        tmem_st16(tS + half * 16, r);
         tmem_wait_st();
       }
       tc_fence_before();
@@ -241,8 +244,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
     if (ok && tiles > 0) wait_all(blk.done, 0);
     tc_fence_after();
     if (!idle)
-      store_acc<DP / 2>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
-                        row < x.Lq, tiles == 0, w * (DP / 2), x.D, x.scale);
+      store_acc<DP / 4>(acc + lanes, static_cast<__nv_bfloat16*>(x.dq) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D,
+                        row < x.Lq, tiles == 0, (2 * w + half) * (DP / 4), x.D, x.scale);
   }
   tc_fence_before();
   __syncthreads();
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
 }
 
 template <int DP>
-__global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
     tc_dkv_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                   const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
                   const __grid_constant__ TcParams p) {
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, 1)
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
   if (tid == 0) {
     s_abort = 0;
-    blk.init();
+    blk.init(128);
   }
   tc_fence_before();
   __syncthreads();
@@ -408,8 +411,8 @@ static int launch_bwd(TcParams& t, cudaStream_t st) {
   if (!set_smem_limit(reinterpret_cast<const void*>(fq), Sh::kBytes) ||
       !set_smem_limit(reinterpret_cast<const void*>(fk), Sh::kBytes))
     return HCLSM_ERR_LAUNCH;
-  if (const int rc = launch_pdl(fq, (unsigned)gq, Sh::kThreads, Sh::kBytes, st, q128, g128, k64, v64, t)) return rc;
-  return launch_pdl(fk, (unsigned)gk, Sh::kThreads, Sh::kBytes, st, k128, v128, q64, g64, t);
+  if (const int rc = launch_pdl(fq, (unsigned)gq, Sh::kDqThreads, Sh::kBytes, st, q128, g128, k64, v64, t)) return rc;
+  return launch_pdl(fk, (unsigned)gk, Sh::kDkvThreads, Sh::kBytes, st, k128, v128, q64, g64, t);
 }
 
 // x.delta is set; ws: tc_workspace bytes.
