@@ -49,6 +49,17 @@ def _forward(q, k, v, lens, mask, scale, keep):
     return o, lse
 
 
+def _backward(q, k, v, o, lse, lens, mask, scale, do):
+    do = _lib.dense_last(do)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    a = _args(q, k, v, o, lse, lens, mask, scale, do, dq, dk, dv)
+    lib = _lib.load()
+    n = lib.hclsm_xattn_bwd_workspace_size(a)
+    ws = q.new_empty(n, dtype=torch.uint8)
+    _lib.check(lib.hclsm_xattn_bwd(a, ws.data_ptr(), n, _lib.stream_ptr(q.device)), "hclsm_xattn_bwd")
+    return dq, dk, dv
+
+
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lens, mask, scale):
@@ -61,27 +72,11 @@ class _CrossAttention(torch.autograd.Function):
     def backward(ctx, do):
         _lib.no_double_backward()
         q, k, v, o, lse, lens, mask = ctx.saved_tensors
-        do = _lib.dense_last(do)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-        a = _args(q, k, v, o, lse, lens, mask, ctx.scale, do, dq, dk, dv)
-        lib = _lib.load()
-        n = lib.hclsm_xattn_bwd_workspace_size(a)
-        ws = q.new_empty(n, dtype=torch.uint8)
-        _lib.check(lib.hclsm_xattn_bwd(a, ws.data_ptr(), n, _lib.stream_ptr(q.device)), "hclsm_xattn_bwd")
-        return dq, dk, dv, None, None, None
+        return (*_backward(q, k, v, o, lse, lens, mask, ctx.scale, do), None, None, None)
 
 
-def cross_attention(q, k, v, *, kv_lens=None, key_mask=None, scale=None):
-    """softmax(scale q k^T) v for q (B, Lq, H, D) and k, v (B, Lk, Hkv, D).
-
-    H is a multiple of Hkv: query head h reads key head h // (H // Hkv).
-    ``kv_lens`` (B,) int: entry b's first kv_lens[b] states count (clamped to
-    [0, Lk]); ``key_mask`` (B, Lk) bool: False states do not count.  What does not
-    count is never read as an operand (it may be NaN), and its gradients are zero;
-    a query with no state gives zeros.  ``scale`` > 0, default D ** -0.5.
-    float32 or bfloat16, head_dim up to 128; softmax and sums in fp32.  Heads are
-    dense, the other strides are free.
-    """
+def _prepare(q, k, v, kv_lens, key_mask, scale):
+    """The checked arguments of the kernels."""
     dev = _lib.require_cuda(q, k, v, kv_lens, key_mask)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError("q must be (B, Lq, H, D); k and v (B, Lk, Hkv, D)")
@@ -103,7 +98,32 @@ def cross_attention(q, k, v, *, kv_lens=None, key_mask=None, scale=None):
         if key_mask.dtype != torch.bool or tuple(key_mask.shape) != (B, k.shape[1]):
             raise ValueError(f"key_mask must be {(B, k.shape[1])} bool")
         key_mask = _lib.dense_last(key_mask)
-    q, k, v = _lib.dense_last(q), _lib.dense_last(k), _lib.dense_last(v)
+    return _lib.dense_last(q), _lib.dense_last(k), _lib.dense_last(v), lens, key_mask, scale
+
+
+def attention_fwd(q, k, v, kv_lens, key_mask, scale):
+    """(o, lse2): the forward and what its backward needs, without autograd."""
+    return _forward(*_prepare(q, k, v, kv_lens, key_mask, scale), True)
+
+
+def attention_bwd(q, k, v, o, lse, do, kv_lens, key_mask, scale):
+    """(dq, dk, dv) from attention_fwd's results."""
+    q, k, v, lens, key_mask, scale = _prepare(q, k, v, kv_lens, key_mask, scale)
+    return _backward(q, k, v, o, lse, lens, key_mask, scale, do)
+
+
+def cross_attention(q, k, v, *, kv_lens=None, key_mask=None, scale=None):
+    """softmax(scale q k^T) v for q (B, Lq, H, D) and k, v (B, Lk, Hkv, D).
+
+    H is a multiple of Hkv: query head h reads key head h // (H // Hkv).
+    ``kv_lens`` (B,) int: entry b's first kv_lens[b] states count (clamped to
+    [0, Lk]); ``key_mask`` (B, Lk) bool: False states do not count.  What does not
+    count is never read as an operand (it may be NaN), and its gradients are zero;
+    a query with no state gives zeros.  ``scale`` > 0, default D ** -0.5.
+    float32 or bfloat16, head_dim up to 128; softmax and sums in fp32.  Heads are
+    dense, the other strides are free.
+    """
+    q, k, v, lens, key_mask, scale = _prepare(q, k, v, kv_lens, key_mask, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _CrossAttention.apply(q, k, v, lens, key_mask, scale)
     return _forward(q, k, v, lens, key_mask, scale, False)[0]

@@ -94,6 +94,31 @@ def _forward(q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved):
     return q, k, yq, yk
 
 
+def _dense_grad(g):
+    return g if g.is_contiguous() and g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
+
+
+def _backward(q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk, want_qw, want_kw):
+    dk = dqw = dkw = ks = ws = None
+    gq, dq = _dense_grad(gq), q.new_empty(q.shape)
+    if qw is not None and want_qw:
+        dqw = qw.new_empty(qw.shape)
+    qs = _side(q, dq, qw, q_pos, gq, dqw)
+    if k is not None:
+        gk, dk = _dense_grad(gk), k.new_empty(k.shape)
+        if kw is not None and want_kw:
+            dkw = kw.new_empty(kw.shape)
+        ks = _side(k, dk, kw, k_pos, gk, dkw)
+    lib, n = _lib.load(), 0
+    if dqw is not None or dkw is not None:
+        n = lib.hclsm_qk_norm_rope_bwd_workspace_size(q.shape[3])
+        ws = q.new_empty(n, dtype=torch.uint8)
+    _lib.check(lib.hclsm_qk_norm_rope_bwd(qs, ks, *_tables(q, cos, sin, eps, interleaved),
+                                          None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(q.device)),
+               "hclsm_qk_norm_rope_bwd")
+    return dq, dk, dqw, dkw
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, cos, sin, q_pos, k_pos, eps, interleaved):
@@ -105,46 +130,13 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gq, gk):
         _lib.no_double_backward()
-        q, k, qw, kw, cos, sin, q_pos, k_pos = ctx.saved_tensors
-        dev = q.device
         want = ctx.needs_input_grad
-        dq = dk = dqw = dkw = ks = ws = None
-        # the gradients arrive dense or are made so
-        gq = gq if gq.is_contiguous() and gq.data_ptr() % 16 == 0 else gq.clone(memory_format=torch.contiguous_format)
-        dq = q.new_empty(q.shape)
-        if qw is not None and want[2]:
-            dqw = qw.new_empty(qw.shape)
-        qs = _side(q, dq, qw, q_pos, gq, dqw)
-        if k is not None:
-            gk = gk if gk.is_contiguous() and gk.data_ptr() % 16 == 0 else \
-                gk.clone(memory_format=torch.contiguous_format)
-            dk = k.new_empty(k.shape)
-            if kw is not None and want[3]:
-                dkw = kw.new_empty(kw.shape)
-            ks = _side(k, dk, kw, k_pos, gk, dkw)
-        lib, n = _lib.load(), 0
-        if dqw is not None or dkw is not None:
-            n = lib.hclsm_qk_norm_rope_bwd_workspace_size(q.shape[3])
-            ws = q.new_empty(n, dtype=torch.uint8)
-        _lib.check(lib.hclsm_qk_norm_rope_bwd(qs, ks, *_tables(q, cos, sin, ctx.eps, ctx.interleaved),
-                                              None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(dev)),
-                   "hclsm_qk_norm_rope_bwd")
-        return dq, dk, dqw, dkw, None, None, None, None, None, None
+        return (*_backward(*ctx.saved_tensors, ctx.eps, ctx.interleaved, gq, gk, want[2], want[3]), None, None, None,
+                None, None, None)
 
 
-def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, *, q_pos=None, k_pos=None, eps=1e-6,
-                 interleaved: bool = False):
-    """(q', k') with every head normalised by its root mean square, weighted and
-    rotated; k may be None (queries alone), and so may the weights and the tables.
-
-    ``q_pos`` (B, Lq) and ``k_pos`` (B, Lk): rows of ``cos`` / ``sin``
-    (positions, rotary_dim / 2), default 0, 1, 2, ...; a position outside the
-    tables gives NaN in that token's rotated dims and sets the device error word.
-    ``eps=None`` leaves the norm out.  Pairs are dims (i, i + rotary_dim / 2), or
-    (2 i, 2 i + 1) with ``interleaved``; rotary_dim is a multiple of 16 (8
-    interleaved).  Differentiable in q, k and the weights; rows of q and k may be
-    strided (each head dense).
-    """
+def _prepare(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved):
+    """The checked arguments of the kernels."""
     dev = _check(q, k, q_weight, k_weight, cos, sin, eps)
     if cos is not None:
         cos, sin = _dense16(cos), _dense16(sin)
@@ -168,7 +160,35 @@ def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, *,
         q_weight = q_weight.contiguous()
     if k_weight is not None:
         k_weight = k_weight.contiguous()
-    args = (q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, None if eps is None else float(eps), bool(interleaved))
+    return q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, None if eps is None else float(eps), bool(interleaved)
+
+
+def rope_fwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved):
+    """(q', k') without autograd."""
+    return _forward(*_prepare(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved))[2:]
+
+
+def rope_bwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk):
+    """(dq, dk, dq_weight, dk_weight), None for weights that are not there."""
+    args = list(_prepare(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved))
+    args[:2] = [None if t is None else _lib.rows16(t) for t in args[:2]]
+    return _backward(*args, gq, gk, True, True)
+
+
+def qk_norm_rope(q, k=None, q_weight=None, k_weight=None, cos=None, sin=None, *, q_pos=None, k_pos=None, eps=1e-6,
+                 interleaved: bool = False):
+    """(q', k') with every head normalised by its root mean square, weighted and
+    rotated; k may be None (queries alone), and so may the weights and the tables.
+
+    ``q_pos`` (B, Lq) and ``k_pos`` (B, Lk): rows of ``cos`` / ``sin``
+    (positions, rotary_dim / 2), default 0, 1, 2, ...; a position outside the
+    tables gives NaN in that token's rotated dims and sets the device error word.
+    ``eps=None`` leaves the norm out.  Pairs are dims (i, i + rotary_dim / 2), or
+    (2 i, 2 i + 1) with ``interleaved``; rotary_dim is a multiple of 16 (8
+    interleaved).  Differentiable in q, k and the weights; rows of q and k may be
+    strided (each head dense).
+    """
+    args = _prepare(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
         return _QkNormRope.apply(*args)
     return _forward(*args)[2:]

@@ -20,7 +20,11 @@ CUDA tensors only (no CPU kernel is registered).  Every op has a fake
   ``event_gather(states, idx, counts, meta, n_frames, pad_k)``,
   ``event_scatter(states, upd, pos, counts, pad_k)``,
   ``event_mha(qkv, key_pad, frames, T, H, HD, scale)``
-  (sparse_event_attn.py:93-188, level1_event.py:33-54).
+  (sparse_event_attn.py:93-188, level1_event.py:33-54);
+* ``qk_norm_rope_fwd`` / ``qk_norm_rope_bwd`` and ``cross_attention_fwd`` /
+  ``cross_attention_bwd`` (both forwards with registered autograd formulas), and
+  ``kv8_write`` / ``kv8_attention`` on the tensors of a ``Kv8Cache``
+  (``kv8_write`` mutates them).
 
 Scan inputs must already share one dtype (fp32 or bf16: x, dt, B, C, z) with
 A_log and D in fp32, and be contiguous; ``hclsm_b200.kernels.ssm_scan`` does
@@ -34,12 +38,18 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .kernels import kv8_cache as _kv8
 from .kernels import sparse_event_attn as _ev
 from .kernels import ssm_scan_kernel as _scan
+from .kernels.cross_attention import attention_bwd as _xattn_bwd
+from .kernels.cross_attention import attention_fwd as _xattn_fwd
+from .kernels.qk_norm_rope import rope_bwd as _rope_bwd
+from .kernels.qk_norm_rope import rope_fwd as _rope_fwd
 from .kernels.slot_attention_kernel import slot_attention_core as _slot_core
 
 __all__ = ["ssm_scan_fwd", "ssm_scan_bwd", "slot_attn_core", "event_compact", "event_gather", "event_scatter",
-           "event_mha"]
+           "event_mha", "qk_norm_rope_fwd", "qk_norm_rope_bwd", "cross_attention_fwd", "cross_attention_bwd",
+           "kv8_write", "kv8_attention"]
 
 _NS = "hclsm_b200"
 
@@ -185,3 +195,106 @@ def event_mha(qkv: Tensor, key_pad: Optional[Tensor], frames: int, T: int, H: in
 @event_mha.register_fake
 def _(qkv, key_pad, frames, T, H, HD, scale):
     return qkv.new_empty((frames * T, H * HD))
+
+
+# ---- attention between sets of states ------------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_fwd", mutates_args=())
+def qk_norm_rope_fwd(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor],
+                     cos: Optional[Tensor], sin: Optional[Tensor], q_pos: Optional[Tensor], k_pos: Optional[Tensor],
+                     eps: float, interleaved: bool) -> Tuple[Tensor, Tensor]:
+    return _rope_fwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved)
+
+
+@qk_norm_rope_fwd.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rope_bwd", mutates_args=())
+def qk_norm_rope_bwd(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor],
+                     cos: Optional[Tensor], sin: Optional[Tensor], q_pos: Optional[Tensor], k_pos: Optional[Tensor],
+                     eps: float, interleaved: bool, gq: Tensor, gk: Tensor) -> List[Tensor]:
+    g = _rope_bwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk)
+    return [q.new_empty(0, dtype=torch.float32) if t is None else t for t in g]
+
+
+@qk_norm_rope_bwd.register_fake
+def _(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk):
+    def w(t):
+        return q.new_empty(0 if t is None else t.shape[0], dtype=torch.float32)
+
+    return [q.new_empty(q.shape), k.new_empty(k.shape), w(q_weight), w(k_weight)]
+
+
+def _rope_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:8])
+    ctx.eps, ctx.interleaved = inputs[8:]
+
+
+def _rope_backward(ctx, gq, gk):
+    t = ctx.saved_tensors
+    dq, dk, dqw, dkw = qk_norm_rope_bwd(*t, ctx.eps, ctx.interleaved, gq, gk)
+    return (dq, dk, None if t[2] is None else dqw, None if t[3] is None else dkw) + (None,) * 6
+
+
+torch.library.register_autograd(f"{_NS}::qk_norm_rope_fwd", _rope_backward, setup_context=_rope_setup)
+
+
+@torch.library.custom_op(f"{_NS}::cross_attention_fwd", mutates_args=())
+def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Tensor], key_mask: Optional[Tensor],
+                        scale: float) -> Tuple[Tensor, Tensor]:
+    return _xattn_fwd(q, k, v, kv_lens, key_mask, scale)
+
+
+@cross_attention_fwd.register_fake
+def _(q, k, v, kv_lens, key_mask, scale):
+    B, Lq, H, _ = q.shape
+    return q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::cross_attention_bwd", mutates_args=())
+def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, do: Tensor,
+                        kv_lens: Optional[Tensor], key_mask: Optional[Tensor], scale: float) -> List[Tensor]:
+    return list(_xattn_bwd(q, k, v, o, lse, do, kv_lens, key_mask, scale))
+
+
+@cross_attention_bwd.register_fake
+def _(q, k, v, o, lse, do, kv_lens, key_mask, scale):
+    return [t.new_empty(t.shape) for t in (q, k, v)]
+
+
+def _xattn_setup(ctx, inputs, output):
+    q, k, v, kv_lens, key_mask, scale = inputs
+    ctx.save_for_backward(q, k, v, *output, kv_lens, key_mask)
+    ctx.scale = scale
+
+
+def _xattn_backward(ctx, go, glse):
+    q, k, v, o, lse, kv_lens, key_mask = ctx.saved_tensors
+    return (*cross_attention_bwd(q, k, v, o, lse, go, kv_lens, key_mask, ctx.scale), None, None, None)
+
+
+torch.library.register_autograd(f"{_NS}::cross_attention_fwd", _xattn_backward, setup_context=_xattn_setup)
+
+
+@torch.library.custom_op(f"{_NS}::kv8_write",
+                         mutates_args=("ck", "cv", "k_scale", "v_scale", "k_tail", "v_tail"))
+def kv8_write(ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor, v_tail: Tensor, k: Tensor,
+              v: Tensor, start: Tensor, count: Optional[Tensor]) -> None:
+    _kv8.kv8_write(_kv8.Kv8Cache(ck, cv, k_scale, v_scale, k_tail, v_tail), k, v, start, count)
+
+
+@kv8_write.register_fake
+def _(ck, cv, k_scale, v_scale, k_tail, v_tail, k, v, start, count):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::kv8_attention", mutates_args=())
+def kv8_attention(q: Tensor, ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor, v_tail: Tensor,
+                  lens: Optional[Tensor], scale: float) -> Tensor:
+    return _kv8.kv8_attention(q, _kv8.Kv8Cache(ck, cv, k_scale, v_scale, k_tail, v_tail), lens, scale=scale)
+
+
+@kv8_attention.register_fake
+def _(q, ck, cv, k_scale, v_scale, k_tail, v_tail, lens, scale):
+    return q.new_empty(q.shape)
