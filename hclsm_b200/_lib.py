@@ -194,7 +194,7 @@ def index32(t, shape, name, device):
     if t.dtype != torch.int32:
         if t.dtype != torch.int64:
             raise TypeError(f"{name} must be int32 or int64, got {t.dtype}")
-        t = t.to(torch.int32)
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)  # out of range stays out of range
     if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
     if t.device != device:

@@ -301,5 +301,6 @@ extern "C" int hclsm_kv8_attn(const hclsm_kv8_cache* c, const hclsm_view* q, voi
   if (!q || !q->p || !o) return HCLSM_ERR_NULL;
   const size_t need = kv8::attn_workspace(c, Lq, H);
   if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
   return kv8::attn(c, q, o, lens, Lq, H, scale, ws, static_cast<cudaStream_t>(stream));
 }

@@ -187,5 +187,16 @@ __device__ __forceinline__ bool mbar_wait_or(uint64_t* bar, uint32_t parity, vol
   return false;
 }
 
+// After a wait ran out: the (converged) warp's own products in flight end, or the limit does, before TMEM and shared
+// memory are given back.  bar: unused till now, count 1.
+__device__ __forceinline__ void drain_umma(uint64_t* bar) {
+  umma_done(elect_one(), bar);
+  mbar_wait(bar, 0);
+}
+// The same for copies: `issued` of them went round a ring of `stages` barriers.
+__device__ __forceinline__ void drain_copies(uint64_t* full, int issued, int stages) {
+  for (int i = issued > stages ? issued - stages : 0; i < issued; ++i) mbar_wait(&full[i % stages], i / stages & 1);
+}
+
 }  // namespace tc
 }  // namespace hclsm

@@ -526,11 +526,13 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (use_split(p, a->dtype)) {
     const size_t need = xattn::split_workspace(p, a->dtype);
     if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
     return xattn::split_fwd(p, a->dtype, ws, st);
   }
   if (a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false)) {
     const size_t need = xattn::tc_workspace(p);
     if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
     return xattn::tc_fwd(p, ws, st);
   }
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
@@ -553,6 +555,7 @@ extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (a->Lq > 0 && (!a->q.p || !a->o || !a->dout.p || !a->dq || !a->lse2)) return HCLSM_ERR_NULL;
   if (a->Lk > 0 && (!a->k.p || !a->v.p || !a->dk || !a->dv)) return HCLSM_ERR_NULL;
   if (ws_bytes < hclsm_xattn_bwd_workspace_size(a) || (a->Lq > 0 && !ws)) return HCLSM_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
   xattn::Params p = xattn::params(a);
   p.delta = static_cast<float*>(ws);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

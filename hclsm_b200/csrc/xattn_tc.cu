@@ -28,7 +28,7 @@ template <int DP, int QT> struct FwdShape {
   // scores are formed as soon as this tile's have been read, and the softmax threads
   // never wait for a product.  D > 64: the weights go over the scores.
   static constexpr bool kApart = DP == 64;
-  static constexpr int kBars = 1 + 4 * kStages + 4 * QT;
+  static constexpr int kBars = 1 + 4 * kStages + 4 * QT + 2;
   static constexpr int kColP = kApart ? QT * 128 : 0, kColO = QT * (kApart ? 192 : 128);
   static constexpr int kStepP = kApart ? 64 : 128;  // columns from one tile's weights to the next's
   static constexpr size_t kBytes = (size_t)(QT + 2 * kStages) * kOp + kBars * 8 + 1024;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   unsigned char *sQ = smem, *sK = sQ + QT * Sh::kOp, *sV = sK + ST * Sh::kOp;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::kOp);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST,
-           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT, *s_free = pv_done + QT;
+           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT, *s_free = pv_done + QT, *drain = s_free + QT;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1, kWeighWarp = QT * 4 + 2;
   if (warp == kMmaWarp) {
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   }
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], (&bars[i] >= p_full && &bars[i] < pv_done) || &bars[i] >= s_free ? 128 : 1);
+    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], (&bars[i] >= p_full && &bars[i] < pv_done) || (&bars[i] >= s_free && &bars[i] < drain) ? 128 : 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   // the whole warp goes on or gives up together
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
+  int issued = 0;  // copies of K and of V (lane 0 of the TMA warp)
   if (warp == kTmaWarp) {
     if (lane == 0 && tiles > 0) {
       mbar_expect_tx(q_full, nq * Sh::kOp);
@@ -94,10 +95,14 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
         mbar_expect_tx(&k_full[s], Sh::kOp);
         for (int kb = 0; kb < DP / 64; ++kb)
           tma_load_4d(sK + s * Sh::kOp + kb * Sh::kBlock, &mk, kb * 64, j * kTile, hk, (int)b, &k_full[s]);
-        if (!wait(&v_empty[s], ph ^ 1)) break;
+        if (!wait(&v_empty[s], ph ^ 1)) {
+          mbar_wait(&k_full[s], ph & 1);  // given up: the K just asked for arrives first
+          break;
+        }
         mbar_expect_tx(&v_full[s], Sh::kOp);
         for (int kb = 0; kb < DP / 64; ++kb)
           tma_load_4d(sV + s * Sh::kOp + kb * Sh::kBlock, &mv, kb * 64, j * kTile, hk, (int)b, &v_full[s]);
+        issued = j + 1;
       }
     }
   } else if (warp == kMmaWarp || warp == kWeighWarp) {
@@ -358,6 +363,15 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (s_abort) {  // the same for all: nothing writes it after the barrier
+    if (warp == kMmaWarp || warp == kWeighWarp) drain_umma(&drain[warp - kMmaWarp]);
+    if (warp == kTmaWarp && lane == 0 && tiles > 0) {
+      mbar_wait(q_full, 0);
+      drain_copies(k_full, issued, ST);
+      drain_copies(v_full, issued, ST);
+    }
+    __syncthreads();
+  }
   if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kCols) : "memory");
 }

@@ -26,7 +26,7 @@ template <int DP> struct BwdShape {
   static constexpr int kBlockA = kTile * kRowBytes, kBlockB = kB * kRowBytes;  // 64 dims
   static constexpr int kOpA = DP / 64 * kBlockA, kOpB = DP / 64 * kBlockB;
   static constexpr int kStages = 4;
-  static constexpr int kBars = 1 + 2 * kStages + 4 + 1;
+  static constexpr int kBars = 1 + 2 * kStages + 4 + 2;
   static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
   // Warpgroups a buffer: dq two (thread = half a row), dk and dv one (thread = row, whose
   // two results of 64 columns would spill the 96 registers that four warpgroups have).
@@ -39,13 +39,13 @@ template <int DP> struct BwdShape {
 template <int DP> struct Block {
   using Sh = BwdShape<DP>;
   unsigned char *a0, *a1, *b0, *b1;  // the block's own two operands, the streamed two
-  uint64_t *own, *full, *empty, *sd_full, *ds_full, *done;
+  uint64_t *own, *full, *empty, *sd_full, *ds_full, *done, *drain;
   __device__ __forceinline__ explicit Block(unsigned char* raw) {
     a0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     a1 = a0 + Sh::kOpA, b0 = a1 + Sh::kOpA, b1 = b0 + Sh::kStages * Sh::kOpB;
     own = reinterpret_cast<uint64_t*>(b1 + Sh::kStages * Sh::kOpB);
     full = own + 1, empty = full + Sh::kStages, sd_full = empty + Sh::kStages, ds_full = sd_full + 2,
-    done = ds_full + 2;
+    done = ds_full + 2, drain = done + 1;
   }
   __device__ __forceinline__ void init(int threads) const {  // of a buffer
     for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? threads : 1);
@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
   // the whole warp goes on or gives up together
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
+  int issued = 0;  // streamed tiles asked for (lane 0 of the TMA warp)
   if (warp == kTmaWarp) {
     if (lane == 0 && tiles > 0) {
       mbar_expect_tx(blk.own, 2 * Sh::kOpA);
@@ -170,6 +171,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
           tma_load_4d(blk.b0 + s * Sh::kOpB + kb * Sh::kBlockB, &mk, kb * 64, j * kB, hk, (int)b, &blk.full[s]);
           tma_load_4d(blk.b1 + s * Sh::kOpB + kb * Sh::kBlockB, &mv, kb * 64, j * kB, hk, (int)b, &blk.full[s]);
         }
+        issued = j + 1;
       }
     }
   } else if (warp == kMmaWarp) {
@@ -250,6 +252,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (s_abort) {  // the same for all: nothing writes it after the barrier
+    if (warp == kMmaWarp) drain_umma(blk.drain);
+    if (warp == kTmaWarp && lane == 0 && tiles > 0) {
+      mbar_wait(blk.own, 0);
+      drain_copies(blk.full, issued, Sh::kStages);
+    }
+    __syncthreads();
+  }
   if (warp == kMmaWarp) free_tmem(tmem);
 }
 
@@ -288,6 +298,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
   // the whole warp goes on or gives up together
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
+  int issued = 0;  // streamed tiles asked for (lane 0 of the TMA warp)
   if (warp == kTmaWarp) {
     if (lane == 0 && tiles > 0) {
       mbar_expect_tx(blk.own, 2 * Sh::kOpA);
@@ -303,6 +314,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
           tma_load_4d(blk.b0 + s * Sh::kOpB + kb * Sh::kBlockB, &mq, kb * 64, r0, h, (int)b, &blk.full[s]);
           tma_load_4d(blk.b1 + s * Sh::kOpB + kb * Sh::kBlockB, &mdo, kb * 64, r0, h, (int)b, &blk.full[s]);
         }
+        issued = i + 1;
       }
     }
   } else if (warp == kMmaWarp) {
@@ -389,6 +401,14 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (s_abort) {  // the same for all: nothing writes it after the barrier
+    if (warp == kMmaWarp) drain_umma(blk.drain);
+    if (warp == kTmaWarp && lane == 0 && tiles > 0) {
+      mbar_wait(blk.own, 0);
+      drain_copies(blk.full, issued, Sh::kStages);
+    }
+    __syncthreads();
+  }
   if (warp == kMmaWarp) free_tmem(tmem);
 }
 
