@@ -500,21 +500,46 @@ Params params(const hclsm_xattn_args* a) {
 
 using namespace hclsm;
 
-// Few enough rows a key head that the 16-row products of the split form carry
-// no padding to speak of, and operands it can read 16 bytes at a time.
-static bool use_split(const xattn::Params& p, int dtype) {
-  const int e = dtype == HCLSM_F32 ? 4 : 2;
+// The split form or the tiles, by the time that each takes on a B200 (us).  The split form: a start, and the keys'
+// and values read once for every 16 rows of a key head (bytes a us; more than one reading comes from L2).  The
+// tiles: a start, and a time a tile of keys (128 on the tensor cores, 64 otherwise) of each wave of blocks.  Fitted
+// to 521 shapes (1 to 64 entries, 1 to 64 heads, 1 to 256 queries over 200 to 16384 keys, heads of 64 and 128, both
+// types): picking by it costs 1.7 % over picking the faster one, always the split form for up to 16 rows and never
+// else 46 %.
+static bool use_split(const xattn::Params& p, int dtype, bool tc) {
+  const bool f32 = dtype == HCLSM_F32, small = p.D <= 64;
+  const int e = f32 ? 4 : 2;
   auto ok = [&](const xattn::View& v) {
     return reinterpret_cast<uintptr_t>(v.p) % 16 == 0 && v.sb * e % 16 == 0 && v.st * e % 16 == 0 && v.sh * e % 16 == 0;
   };
-  return p.Lk > 0 && (int64_t)p.Lq * (p.H / p.Hkv) <= 16 && p.D % 32 == 0 && ok(p.k) && ok(p.v);
+  if (p.Lk == 0 || p.D % 32 || !ok(p.k) || !ok(p.v)) return false;
+  const double rows16 = ((int64_t)p.Lq * (p.H / p.Hkv) + 15) / 16;
+  const double bytes = (double)p.B * p.Hkv * rows16 * p.Lk * p.D * 2 * e;
+  const double rate = f32 ? (small ? 5.2e6 : 4.3e6) : (rows16 == 1 ? 4.4e6 : 6.5e6);
+  const double split = (rows16 == 1 ? (small ? 6.0 : 7.5) : (small ? 8.0 : 11.0)) + bytes / rate;
+  double tiles;
+  if (tc) {
+    const int qt = p.Lq <= 128 ? 1 : 2, resident = num_sms() * (qt == 1 ? 2 : 1);
+    const int64_t blocks = (int64_t)((p.Lq + 128 * qt - 1) / (128 * qt)) * p.H * p.B;
+    tiles = 4.0 + (double)((blocks + resident - 1) / resident) * ((p.Lk + 127) / 128) * (small ? 1.3 : 1.7);
+  } else {
+    const double waves = (double)((p.Lq + 31) / 32) * p.H * p.B / num_sms();
+    tiles = 4.0 + (waves > 1.0 ? waves : 1.0) * ((p.Lk + 63) / 64) * (small ? 4.0 : 8.5);
+  }
+  return split < tiles;
+}
+// Which kernels serve a forward call.
+enum Path { kTiles, kTensor, kSplit };
+static Path fwd_path(const xattn::Params& p, int dtype) {
+  const bool tc = dtype == HCLSM_BF16 && xattn::tc_ok(p, false);
+  return use_split(p, dtype, tc) ? kSplit : tc ? kTensor : kTiles;
 }
 
 extern "C" size_t hclsm_xattn_fwd_workspace_size(const hclsm_xattn_args* a) {
   if (xattn::check(a)) return 0;
   const xattn::Params p = xattn::params(a);
-  if (use_split(p, a->dtype)) return xattn::split_workspace(p, a->dtype);
-  return a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false) ? xattn::tc_workspace(p) : 0;
+  const Path path = fwd_path(p, a->dtype);
+  return path == kSplit ? xattn::split_workspace(p, a->dtype) : path == kTensor ? xattn::tc_workspace(p) : 0;
 }
 
 extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -523,19 +548,13 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (!a->q.p || !a->o || (a->Lk > 0 && (!a->k.p || !a->v.p))) return HCLSM_ERR_NULL;
   const xattn::Params p = xattn::params(a);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (use_split(p, a->dtype)) {
-    const size_t need = xattn::split_workspace(p, a->dtype);
-    if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
-    return xattn::split_fwd(p, a->dtype, ws, st);
-  }
-  if (a->dtype == HCLSM_BF16 && xattn::tc_ok(p, false)) {
-    const size_t need = xattn::tc_workspace(p);
-    if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
-    if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
-    return xattn::tc_fwd(p, ws, st);
-  }
-  return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
+  const Path path = fwd_path(p, a->dtype);
+  if (path == kTiles)
+    return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, false, st) : xattn::dispatch<__nv_bfloat16>(p, false, st);
+  const size_t need = path == kSplit ? xattn::split_workspace(p, a->dtype) : xattn::tc_workspace(p);
+  if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
+  return path == kSplit ? xattn::split_fwd(p, a->dtype, ws, st) : xattn::tc_fwd(p, ws, st);
 }
 
 static bool use_tc_bwd(const xattn::Params& p, int dtype) {
