@@ -452,7 +452,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
   const float c2 = p.x.scale * kLog2e;
   const float fs[2] = {c2, c2}, off[2] = {0.0f, 0.0f};
   // this block's share of the sequence's own steps
-  const int n8 = CACHE ? n / p.block * p.block : n;
+  // the cache: tokens in 8 bits; a length inside the block that the tail holds (scale -1) ends before it
+  int n8 = n;
+  if (CACHE && n % p.block && p.ks[bh * (p.T / p.block) + n / p.block] < 0.0f) n8 = n / p.block * p.block;
   const int steps = (n8 + 15) / 16, per = (steps + p.splits - 1) / p.splits;
   const int first = min(steps, sp * per), last = min(steps, first + per);
   if constexpr (CACHE) {
@@ -467,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
     }
     sweep<int8_t, D, CV, NQ, NR, F16>(
         st, qh, fs8, off8, first + warp, last, kWarps, n8, [&](int j) { return k8 + (int64_t)j * D; },
-        [&](int j) { return v8 + (int64_t)j * D; }, [](int) { return true; }, [](int) { return true; },
+        [&](int j) { return v8 + (int64_t)j * D; }, [&](int j) { return j < n8; },
+        [&](int step) { return step * 16 + 16 <= n8; },
         [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); });
   } else {
     const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);

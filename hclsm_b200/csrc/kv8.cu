@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
   if (j == 0 && end % block) {
     __syncwarp();  // the tail has been read
     const int t0 = max(start, lastb * block);
+    if (lane == 0) p.scale[kv][bh * (p.T / block) + lastb] = -1.0f;  // this block is in the tail
     for (int i = lane; i < (end - t0) * D / 8; i += 32) {
       const int tok = t0 + i * 8 / D, d = i * 8 % D;
       Raw<T> t;
@@ -186,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
   const uint32_t vd = p.D / 8, row = vd * p.Hkv;  // vectors of a token
   const int64_t b = blockIdx.z;
   const int n = p.count ? min(max(p.count[b], 0), p.T) : p.T;
-  const int n8 = n / p.block * p.block;
+  const int n8 = n / p.block * p.block;  // whole blocks below the length
   const uint32_t total = row * (uint32_t)p.T;  // of this sequence
   T* out = static_cast<T*>(p.out[kv]) + b * (int64_t)total * 8;
   for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
@@ -196,8 +197,8 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
     Raw<T> r;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    if ((int)t < n8) {
-      const float s = p.scale[kv][bh * (p.T / p.block) + t / (uint32_t)p.block];
+    const float s = (int)t < n ? p.scale[kv][bh * (p.T / p.block) + t / (uint32_t)p.block] : 0.0f;
+    if ((int)t < n8 || ((int)t < n && !(s < 0.0f))) {
       const uint2 w = *reinterpret_cast<const uint2*>(p.q[kv] + (bh * p.T + t) * p.D + d);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = s * (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));

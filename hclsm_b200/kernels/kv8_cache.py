@@ -2,7 +2,8 @@
 
 Complete blocks of ``block`` tokens a head are int8 with one fp32 scale
 (max|x| / 127); the last, incomplete block of each sequence stays in the inputs'
-dtype, so every value is rounded to 8 bits once, when its block fills.  The
+dtype (its scale is -1), so every value is rounded to 8 bits once, when its block
+fills.  The
 caller owns the positions: ``start`` (tokens already there) and ``lens`` (tokens
 to attend to) are arguments, so a step captures into a CUDA graph and can be
 replayed with other positions.
@@ -61,12 +62,12 @@ class Kv8Cache:
         """A cache with room for ``capacity`` tokens (rounded up to whole blocks) a sequence."""
         T = (capacity + block - 1) // block * block
 
-        def zeros(*shape, dt):
-            return torch.zeros(shape, dtype=dt, device=device)
+        def full(value, *shape, dt):
+            return torch.full(shape, value, dtype=dt, device=device)
 
-        return cls(*(zeros(batch, kv_heads, T, head_dim, dt=torch.int8) for _ in range(2)),
-                   *(zeros(batch, kv_heads, T // block, dt=torch.float32) for _ in range(2)),
-                   *(zeros(batch, kv_heads, block, head_dim, dt=dtype) for _ in range(2)))
+        return cls(*(full(0, batch, kv_heads, T, head_dim, dt=torch.int8) for _ in range(2)),
+                   *(full(-1.0, batch, kv_heads, T // block, dt=torch.float32) for _ in range(2)),
+                   *(full(0, batch, kv_heads, block, head_dim, dt=dtype) for _ in range(2)))
 
     @property
     def dtype(self) -> torch.dtype:
@@ -80,7 +81,8 @@ class Kv8Cache:
 def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tensor | None = None) -> None:
     """Append k, v (B, n, Hkv, D), in place: token i of entry b becomes token
     ``start[b] + i`` of the cache, for the first ``count[b]`` tokens (default n).
-    ``start[b]`` is the number of tokens already there.  A request that does not
+    ``start[b]`` is the number of tokens already there (or, to write anew from there, a
+    multiple of the block: what was behind it is gone).  A request that does not
     fit the capacity writes nothing and sets the device error word."""
     dev = _lib.require_cuda(cache.k, k, v, start, count)
     B, Hkv, _, D = cache.k.shape
@@ -100,7 +102,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
 
 def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
     """(k, v), each (B, T, Hkv, D) in the cache's dtype: the first ``lens[b]``
-    tokens (default all) as the values they stand for, zeros after them."""
+    tokens written (default all) as the values they stand for, zeros after them."""
     dev = _lib.require_cuda(cache.k, lens)
     B, Hkv, T, D = cache.k.shape
     lens = _lib.index32(lens, (B,), "lens", dev)
@@ -112,8 +114,8 @@ def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
 
 def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, scale: float | None = None) -> Tensor:
     """softmax(scale q k^T) v of q (B, Lq, H, D), in the cache's dtype, over the
-    first ``lens[b]`` tokens of the cache (default all; clamped to [0, T]); H is a
-    multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
+    first ``lens[b]`` tokens written (default all of the capacity; clamped to [0, T]); H
+    is a multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
     dev = _lib.require_cuda(q, cache.k, lens)
     B, Hkv, T, D = cache.k.shape
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:

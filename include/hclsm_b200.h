@@ -410,7 +410,7 @@ int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* 
 
 /* The 8-bit state cache.  Complete blocks of `block` tokens a head are 8-bit
  * integers with one fp32 scale, max|x| / 127; the last, incomplete block of a
- * sequence is held in `dtype` (the tail).  D 32, 64, 96 or 128; block 16, 32,
+ * sequence is held in `dtype` (the tail), and -1 stands in its scale.  D 32, 64, 96 or 128; block 16, 32,
  * 64 or 128; T a multiple of block. */
 typedef struct {
   int8_t *k, *v;             /* (B, Hkv, T, D) */
@@ -420,7 +420,8 @@ typedef struct {
 } hclsm_kv8_cache;
 
 /* Tokens [0, count[b]) of k, v (B, n, Hkv, D; NULL count: n) become tokens
- * start[b], start[b] + 1, ... of the cache.  A request that does not fit (start
+ * start[b], start[b] + 1, ... of the cache; start[b] is the number of tokens there,
+ * or a multiple of block.  A request that does not fit (start
  * < 0, count outside [0, n], start + count > T) writes nothing and puts
  * HCLSM_ERR_SHAPE in the error word. */
 int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, const hclsm_view* v, int32_t n,

@@ -132,6 +132,34 @@ def test_rope_alone_strided_and_on_another_stream():
     assert _err(qk_norm_rope(wide)[0], _rope_ref(wide, None, None, None, None, 1e-6, False)) < U
 
 
+def test_rope_weights_of_one_side_and_positions_in_64_bits():
+    g = _gen(16)
+    q, k = _randn(g, 2, 5, 4, 64).requires_grad_(), _randn(g, 2, 9, 2, 64).requires_grad_()
+    w = (1 + 0.1 * _randn(g, 64)).requires_grad_()
+    cos, sin = rope_tables(16, 64)
+    pos = torch.randint(0, 16, (2, 9), generator=g, device="cuda")  # int64
+    gq, gk = _randn(g, *q.shape), _randn(g, *k.shape)
+    ref = [t.detach().double().requires_grad_() for t in (q, k, w)]
+    at = torch.arange(5, device="cuda").expand(2, 5)
+    for qw, kw in ((w, None), (None, w), (w, w)):
+        y = qk_norm_rope(q, k, qw, kw, cos, sin, k_pos=pos)
+        got = torch.autograd.grad(y, (q, k, w), (gq, gk))
+        r = (_rope_ref(ref[0], None if qw is None else ref[2], cos, sin, at, 1e-6, False),
+             _rope_ref(ref[1], None if kw is None else ref[2], cos, sin, pos, 1e-6, False))
+        for a, b in zip((*y, *got), (*r, *torch.autograd.grad(r, ref, (gq.double(), gk.double())))):
+            assert _err(a, b) < 1e-5
+    # a position of 2^32 is outside, not position 0
+    y, _ = qk_norm_rope(q[:, :1], None, cos=cos, sin=sin, q_pos=torch.full((2, 1), 1 << 32, device="cuda"))
+    assert hclsm_b200.device_error() == 1 and torch.isnan(y).all()
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(1, 4, 2, 64, device="cuda", requires_grad=True)
+    for f in (lambda: cross_attention(x, x, x), lambda: qk_norm_rope(x)[0]):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(f().sum(), x, create_graph=True)
+
+
 def test_rope_empty_and_outside_positions():
     q = torch.empty(2, 0, 4, 64, device="cuda", requires_grad=True)
     w = torch.ones(64, device="cuda", requires_grad=True)
@@ -314,6 +342,24 @@ def test_cross_attention_large_scores_and_empty_sizes(dtype):
             assert not a.any()
 
 
+@pytest.mark.parametrize("Lq", [1, 150])
+def test_offsets_past_32_bits(Lq):
+    """Batch entries 2^31 elements apart, with nothing but stale memory between them."""
+    g = _gen(15)
+    far = torch.empty((1 << 31) + 300 * 64, device="cuda", dtype=BF16)
+    k = far.as_strided((2, 300, 1, 64), (1 << 31, 64, 64, 1))
+    k.copy_(_randn(g, 2, 300, 1, 64, dtype=BF16))
+    q = _randn(g, 2, Lq, 1, 64, dtype=BF16).requires_grad_()
+    ok, do = _allowed(2, 300, None, None), _randn(g, 2, Lq, 1, 64, dtype=BF16)
+    kk = k.requires_grad_()
+    o = cross_attention(q, kk, kk.detach())
+    ref = [t.detach().double().requires_grad_() for t in (q, k)]
+    ro = _attn_ref(ref[0], ref[1], ref[1].detach(), ok)
+    assert _err(o, ro) < 2 * U
+    for a, b in zip(torch.autograd.grad(o, (q, kk), do), torch.autograd.grad(ro, ref, do.double())):
+        assert _err(a, b) < 3 * U
+
+
 def test_cross_attention_refusals():
     q, k = torch.zeros(2, 3, 4, 64, device="cuda"), torch.zeros(2, 5, 2, 64, device="cuda")
     lens = torch.zeros(2, device="cuda", dtype=torch.int32)
@@ -379,6 +425,11 @@ def test_cache_write_read_attend(dtype, D, block, Hkv, G):
         plain.write(kv, start, counts)
         start = [a + c for a, c in zip(start, counts)]
         lens = _i32(*start)
+        # and from the middle of what is there: inside a complete block, or inside the tail
+        part = _i32(*(max(0, v - 1 - i) for i, v in enumerate(start)))
+        q = _randn(g, B, 1, Hkv * G, D, dtype=dtype)
+        ref = _attn_ref(q, plain.x[0], plain.x[1], _allowed(B, T, part, None))
+        assert _err(kv8_attention(q, cache, part), ref) < _tol(dtype, 2)
         for got, want in zip(kv8_read(cache, lens), plain.x):
             assert got.dtype == dtype and _err(got, want) < (U if dtype == BF16 else 1e-6)
         ok = _allowed(B, T, lens, None)
@@ -398,8 +449,12 @@ def test_cache_long_and_shorter_views_of_it():
     kv8_write(cache, *kv, _i32(0, 0))
     plain.write(kv, [0, 0], [T, T])
     q = _randn(g, B, 2, 8, D, dtype=BF16)
-    # lengths at a block's end (what is past it is not read), past the capacity, and all of it
-    for lens in (_i32(T, 4096), _i32(T + 50, 0), None):
+    # lengths at a block's end, inside complete blocks, past the capacity, and all of it
+    for lens in (_i32(T, 4096), _i32(4100, 17), _i32(T - 1, 1), _i32(T + 50, 0), None):
+        if lens is not None:
+            for got, want in zip(kv8_read(cache, lens), plain.x):
+                keep = _allowed(B, T, lens.clamp(0, T), None)[:, :, None, None]
+                assert _err(got, torch.where(keep, want, 0.0)) < U
         ok = _allowed(B, T, None if lens is None else lens.clamp(0, T), None)
         assert _err(kv8_attention(q, cache, lens, scale=0.2), _attn_ref(q, *plain.x, ok, 0.2)) < 2 * U
 
@@ -437,13 +492,26 @@ def test_cache_values_that_are_zero_or_not_finite_and_step_replay():
         assert _err(o, _attn_ref(q, *plain.x, _allowed(2, 96, lens, None))) < 2 * U, t
 
 
+def test_cache_offsets_past_32_bits():
+    """The second sequence's states start 2^31 bytes into the cache."""
+    g = _gen(14)
+    cache, plain = Kv8Cache.empty(2, 1 << 24, 1, 128), _Plain(2, 96, 1, 128, 32)
+    kv = [_randn(g, 2, 90, 1, 128, dtype=BF16) for _ in range(2)]
+    kv8_write(cache, *kv, _i32(0, 0))
+    plain.write(kv, [0, 0], [90, 90])
+    q = _randn(g, 2, 1, 2, 128, dtype=BF16)
+    lens = _i32(17, 90)
+    assert _err(kv8_attention(q, cache, lens), _attn_ref(q, *plain.x, _allowed(2, 96, lens, None))) < 2 * U
+    assert cache.k[1, 0, :64].any() and not cache.k[0, 0, 64:].any()
+
+
 def test_cache_requests_that_do_not_fit_write_nothing():
     cache = Kv8Cache.empty(1, 32, 1, 32, dtype=F32)
     x = torch.ones(1, 8, 1, 32, device="cuda")
     for start, count in ((25, 8), (-1, 8), (0, 9), (0, -1), (2 ** 31 - 4, 8)):
         kv8_write(cache, x, x, _i32(start), _i32(count))
         assert hclsm_b200.device_error() == 1
-        assert not cache.k.any() and not cache.k_tail.any() and not cache.k_scale.any()
+        assert not cache.k.any() and not cache.k_tail.any() and (cache.k_scale == -1).all()
 
 
 def test_cache_refusals():
