@@ -10,6 +10,9 @@
 // The maximum that O is scaled by is raised only when a row's new one exceeds it by
 // 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
 // with the same relative precision, and O is read back and rescaled rarely.
+// The bound is the softmax's issue and its chain with the products: 4 x 2048 queries
+// over 8192 states, 32 heads of 64, 690 us (797 TFLOP/s), 8 x 2048 over 4096, 16 heads
+// of 128, 500 us (1100 TFLOP/s); tensor pipe 28 and 42 % busy (2 x 2048 over 4096).
 // While one tile takes its softmax the tensor cores run the other's products.
 #include <type_traits>
 
@@ -25,14 +28,15 @@ template <int DP, int QT> struct FwdShape {
   static constexpr int kOp = DP / 64 * kBlock;            // a staged tile
   static constexpr int kStages = DP == 64 ? (QT == 2 ? 3 : 2) : (QT == 2 ? 2 : 1);
   // D <= 64 leaves TMEM columns for the weights beside the scores: then the next tile's
-  // scores are formed as soon as this tile's have been read, and the softmax threads
-  // never wait for a product.  D > 64: the weights go over the scores.
-  static constexpr bool kApart = DP == 64;
+  // scores are formed as soon as this tile's have been read.  Else the weights go over
+  // the scores; so with QT 1, whose second block an SM hides the wait, and where a third
+  // warp of issue would cost the softmax threads 40 registers (spills).
+  static constexpr bool kApart = DP == 64 && QT == 2;
   static constexpr int kBars = 1 + 4 * kStages + 4 * QT + 2;
   static constexpr int kColP = kApart ? QT * 128 : 0, kColO = QT * (kApart ? 192 : 128);
   static constexpr int kStepP = kApart ? 64 : 128;  // columns from one tile's weights to the next's
   static constexpr size_t kBytes = (size_t)(QT + 2 * kStages) * kOp + kBars * 8 + 1024;
-  static constexpr int kThreads = QT * 128 + 96;
+  static constexpr int kThreads = QT * 128 + (kApart ? 96 : 64);
   static constexpr uint32_t kCols = QT == 2 ? 512 : 256;
 };
 
