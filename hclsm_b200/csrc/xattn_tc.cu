@@ -12,10 +12,8 @@
 // with the same relative precision, and O is read back and rescaled rarely.
 // The bound is the softmax's issue and its chain with the products: 4 x 2048 queries
 // over 8192 states, 32 heads of 64, 690 us (797 TFLOP/s), 8 x 2048 over 4096, 16 heads
-// of 128, 500 us (1100 TFLOP/s); tensor pipe 28 and 42 % busy (2 x 2048 over 4096).
+// of 128, 435 us (1264 TFLOP/s); tensor pipe 28 and 42 % busy (2 x 2048 over 4096).
 // While one tile takes its softmax the tensor cores run the other's products.
-#include <type_traits>
-
 #include "xattn_tc.cuh"
 
 namespace hclsm {
@@ -202,14 +200,27 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
     bool ok = w < nq;
     for (int j = 0; j < tiles && ok; ++j) {
       const uint4 bits = key_bits(p, b, nk, j * kTile);
-      const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-      const bool all = all_bits(bits);
       if (!(ok = wait_all(&s_full[w], j))) break;
       tc_fence_after();
       if (idle) {
         if constexpr (Sh::kApart) mbar_arrive(&s_free[w]);
         mbar_arrive(&p_full[w]);
         continue;
+      }
+      if (!all_bits(bits)) {  // -inf over the scores that do not count; the rest of the code has no mask
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t word = (c < 4 ? (c < 2 ? bits.x : bits.y) : (c < 6 ? bits.z : bits.w)) >> (16 * (c & 1));
+          float v[16];
+          tmem_ld16_nowait(tS + c * 16, v);
+          tmem_wait_ld();
+          tmem_pin<16>(v);
+          uint32_t q[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) q[i] = word >> i & 1u ? __float_as_uint(v[i]) : 0xff800000u;
+          tmem_st16(tS + c * 16, q);
+        }
+        tmem_wait_st();
       }
       auto highest = [&](float (&mx)[4], const float (&v)[32]) {
 #pragma unroll
@@ -220,7 +231,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
       // a row's maximum is now `top`: O, kept by the old one, is scaled to it where it is too low
       auto raise = [&](float top) {
         const bool up = (top - m) * c2 > kRaise;  // false where both are -inf (NaN)
-        if (!__any_sync(0xffffffffu, up)) return false;
+        if (!__any_sync(0xffffffffu, up)) return;
         const float f = up ? ex2((m - top) * c2) : 1.0f;  // 0 from -inf: O is zero, or (j = 0) not yet written
         if (up) m = top;
         l.x *= f, l.y *= f;
@@ -239,7 +250,6 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
             tmem_st16(tO + c, q);
           }
         }
-        return true;
       };
       // 32 scores to weights; three pairs in eight on the FMA pipe, because the MUFU's 16 a clock
       // would be the bound (measured for a 128 x 128 tile of two warpgroups: 1196 clocks with
@@ -255,82 +265,40 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
           pw[i] = pack_bf16(e.x, e.y);
         }
       };
-      // The whole tile without a branch on the mask inside, so that the chunks' instructions interleave.
-      auto tile = [&](auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
-        // fn(chunk, its 32 scores), each chunk's load in flight during the one before
-        auto chunks = [&](auto fn) {
-          float v[2][32];
-          tmem_ld32_nowait(tS, v[0]);
+      // fn(chunk, its 32 scores), each chunk's load in flight during the one before
+      auto chunks = [&](auto fn) {
+        float v[2][32];
+        tmem_ld32_nowait(tS, v[0]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld();
-            tmem_pin<32>(v[c & 1]);
-            if (c < 3) tmem_ld32_nowait(tS + (c + 1) * 32, v[(c + 1) & 1]);
-            if constexpr (MASKED) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[c & 1][i] = word[c] >> i & 1u ? v[c & 1][i] : -INFINITY;
-            }
-            fn(c, v[c & 1]);
-          }
-        };
-        if constexpr (Sh::kApart) {
-          // The maximum first, then the weights, so that the scores are free for the next tile's
-          // while their last quarter is still being weighed.
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          chunks([&](int, const float (&v)[32]) { highest(mx, v); });
-          raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]));
-          if (ok && j > 0) ok = wait_all(&pv_done[w], j - 1);  // the last weights have been used
-          tc_fence_after();
-          if (!ok) return;
-          float2 sum = make_float2(0.0f, 0.0f);
-          chunks([&](int c, const float (&v)[32]) {
-            if (c == 3) {
-              tc_fence_before();
-              mbar_arrive(&s_free[w]);
-            }
-            uint32_t pw[16];
-            weights(v, pw, sum);
-            tmem_st16(tP + c * 16, pw);
-          });
-          l = add2(l, sum);
-        } else {
-          // The weights by the maximum as it stands, kept in registers, and again where it has
-          // to be raised: the scores' maximum is off the chain that the products wait for.
-          // (A masked tile takes its maximum first: its code would not fit the registers.)
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          float2 sum = make_float2(0.0f, 0.0f);
-          auto over = [&](int c, const float (&v)[32]) {  // over scores that have been read
-            uint32_t pw[16];
-            weights(v, pw, sum);
-            tmem_st16(tP + c * 16, pw);
-          };
-          if constexpr (MASKED) {
-            chunks([&](int, const float (&v)[32]) { highest(mx, v); });
-            raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]));
-            if (!ok) return;
-            chunks(over);
-          } else {
-            uint32_t pw[64];
-            chunks([&](int c, const float (&v)[32]) {
-              highest(mx, v);
-              weights(v, pw + c * 16, sum);
-            });
-            if (raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]))) {
-              if (!ok) return;
-              sum = make_float2(0.0f, 0.0f);
-              chunks(over);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) tmem_st16(tP + c * 16, pw + c * 16);
-            }
-          }
-          l = add2(l, sum);
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld();
+          tmem_pin<32>(v[c & 1]);
+          if (c < 3) tmem_ld32_nowait(tS + (c + 1) * 32, v[(c + 1) & 1]);
+          fn(c, v[c & 1]);
         }
       };
-      if (all) tile(std::false_type{});
-      else tile(std::true_type{});
+      // The maximum first, then the weights from a second reading: a row's scores and weights
+      // together do not fit the registers (weights by the old maximum, kept until the new one
+      // is known, took 481 against 435 us with heads of 128, spills included).
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      chunks([&](int, const float (&v)[32]) { highest(mx, v); });
+      raise(max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]));
+      if constexpr (Sh::kApart) {
+        if (ok && j > 0) ok = wait_all(&pv_done[w], j - 1);  // the last weights have been used
+        tc_fence_after();
+      }
       if (!ok) break;
+      float2 sum = make_float2(0.0f, 0.0f);
+      chunks([&](int c, const float (&v)[32]) {
+        if (Sh::kApart && c == 3) {  // the scores are free while their last quarter is still being weighed
+          tc_fence_before();
+          mbar_arrive(&s_free[w]);
+        }
+        uint32_t pw[16];
+        weights(v, pw, sum);
+        tmem_st16(tP + c * 16, pw);  // where over the scores: over ones that have been read
+      });
+      l = add2(l, sum);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&p_full[w]);
