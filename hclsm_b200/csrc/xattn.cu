@@ -578,7 +578,7 @@ extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   xattn::Params p = xattn::params(a);
   p.delta = static_cast<float*>(ws);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (const int rc = xattn::launch_delta(p, a->dtype, st)) return rc;
   if (use_tc_bwd(p, a->dtype)) return xattn::tc_bwd(p, static_cast<char*>(ws) + xattn::delta_bytes(p), st);
+  if (const int rc = xattn::launch_delta(p, a->dtype, st)) return rc;
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, true, st) : xattn::dispatch<__nv_bfloat16>(p, true, st);
 }

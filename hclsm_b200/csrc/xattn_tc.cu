@@ -382,6 +382,9 @@ template <int DP, int QT>
 static int launch_fwd(TcParams& t, cudaStream_t st) {
   using Sh = FwdShape<DP, QT>;
   const Params& x = t.x;
+  // before the maps: encoding one needs the device's context, which this call makes current in a new thread
+  auto fn = tc_fwd_kernel<DP, QT>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(fn), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
   CUtensorMap mq, mk, mv;
   if (!make_map(&mq, x.q, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&mk, x.k, x.D, x.Lk, x.Hkv, x.B, kTile) ||
       !make_map(&mv, x.v, x.D, x.Lk, x.Hkv, x.B, kTile))
@@ -389,8 +392,6 @@ static int launch_fwd(TcParams& t, cudaStream_t st) {
   t.qtiles = (x.Lq + QT * kTile - 1) / (QT * kTile);
   const int64_t grid = (int64_t)t.qtiles * x.H * x.B;
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  auto fn = tc_fwd_kernel<DP, QT>;
-  if (!set_smem_limit(reinterpret_cast<const void*>(fn), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
   return launch_pdl(fn, (unsigned)grid, Sh::kThreads, Sh::kBytes, st, mq, mk, mv, t);
 }
 

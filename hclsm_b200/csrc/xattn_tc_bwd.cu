@@ -3,7 +3,8 @@
 // Two kernels, each with its own recomputation of the weights, so that every sum
 // has a fixed order (no atomics): 7 products instead of 5.
 //
-//   dq: a block takes 128 query rows and walks over tiles of 64 keys:
+//   dq: a block takes 128 query rows (q and do as A operands in TMEM; delta on the way)
+//   and walks over tiles of 64 keys:
 //     S = Q K^T, dP = dO V^T  ->  dS = P (dP - delta), bf16 over S  ->  dQ += dS K
 //   dk, dv: a block takes 128 keys and walks over tiles of 64 query rows of every
 //   query head that shares them, transposed so that keys are the TMEM lanes:
@@ -27,7 +28,8 @@ template <int DP> struct BwdShape {
   static constexpr int kOpA = DP / 64 * kBlockA, kOpB = DP / 64 * kBlockB;
   static constexpr int kStages = 4;
   static constexpr int kBars = 1 + 2 * kStages + 4 + 2;
-  static constexpr size_t kBytes = 2 * kOpA + 2 * kStages * (size_t)kOpB + kBars * 8 + 1024;
+  // shared memory: dq has no own operands there
+  static constexpr size_t kDqBytes = 2 * kStages * (size_t)kOpB + kBars * 8 + 1024, kDkvBytes = kDqBytes + 2 * kOpA;
   // Warpgroups a buffer: dq two (thread = half a row), dk and dv one (thread = row, whose
   // two results of 64 columns would spill the 96 registers that four warpgroups have).
   // 8 x 2048 x 4096, 16 heads of 128: dq 864 us with one, 740 with two; dk, dv 840 with
@@ -35,20 +37,21 @@ template <int DP> struct BwdShape {
   static constexpr int kDqThreads = 4 * 128 + 64, kDkvThreads = 2 * 128 + 64;
 };
 
-// Shared by the two kernels: block layout, barriers, roles.
-template <int DP> struct Block {
+// Shared by the two kernels: block layout, barriers, roles.  OWN: the block's own operands are in shared memory.
+template <int DP, bool OWN> struct Block {
   using Sh = BwdShape<DP>;
   unsigned char *a0, *a1, *b0, *b1;  // the block's own two operands, the streamed two
   uint64_t *own, *full, *empty, *sd_full, *ds_full, *done, *drain;
   __device__ __forceinline__ explicit Block(unsigned char* raw) {
     a0 = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    a1 = a0 + Sh::kOpA, b0 = a1 + Sh::kOpA, b1 = b0 + Sh::kStages * Sh::kOpB;
+    a1 = a0 + (OWN ? Sh::kOpA : 0), b0 = a1 + (OWN ? Sh::kOpA : 0), b1 = b0 + Sh::kStages * Sh::kOpB;
     own = reinterpret_cast<uint64_t*>(b1 + Sh::kStages * Sh::kOpB);
     full = own + 1, empty = full + Sh::kStages, sd_full = empty + Sh::kStages, ds_full = sd_full + 2,
     done = ds_full + 2, drain = done + 1;
   }
   __device__ __forceinline__ void init(int threads) const {  // of a buffer
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(own + i, own + i >= ds_full && own + i < done ? threads : 1);
+    for (int i = 0; i < Sh::kBars; ++i)
+      mbar_init(own + i, own + i >= ds_full && own + i < done ? threads : !OWN && i == 0 ? 2 * threads : 1);
     fence_mbar_init();
   }
   // What the issuing thread computes once.
@@ -82,13 +85,27 @@ template <int DP> struct Block {
     }
     umma_done(r.one, &sd_full[w]);
   }
-  // acc += (bf16 columns at a) x (streamed tile in stage s, MN-major descriptor t) (a converged warp)
+  // the same with the own operands in TMEM columns t0 and t1
+  __device__ __forceinline__ void products_ts(const Issue& r, uint32_t tmem, uint32_t t0, uint32_t t1, int w, int s) const {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint64_t b = desc_at(half ? r.b1 : r.b0, s * Sh::kOpB);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < r.ksteps)
+          umma_ts(r.one, tmem + w * 128 + half * 64, (half ? t1 : t0) + k * 8,
+                  desc_at(b, (k >> 2) * Sh::kBlockB + (k & 3) * 32), r.id_s, k != 0);
+    }
+    umma_done(r.one, &sd_full[w]);
+  }
+  // acc += (bf16 columns at a, the second 32 rows' STEP further) x (streamed tile in stage s, MN-major descriptor t) (a converged warp)
+  template <int STEP>
   __device__ __forceinline__ void accumulate(const Issue& r, uint32_t acc, uint32_t a, uint64_t t, int s,
                                              bool first) const {
     const uint64_t b = desc_at(t, s * Sh::kOpB);
 #pragma unroll
     for (int k = 0; k < kB / 16; ++k)
-      umma_ts(r.one, acc, a + k * 8, desc_at(b, k * 16 * kRowBytes), r.id_o, !(first && k == 0));
+      umma_ts(r.one, acc, a + (k & 1) * 8 + (k >> 1) * STEP, desc_at(b, k * 16 * kRowBytes), r.id_o, !(first && k == 0));
   }
 };
 
@@ -125,14 +142,14 @@ __device__ __forceinline__ void store_acc(uint32_t t, __nv_bfloat16* out, bool o
 
 template <int DP>
 __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
-    tc_dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mdo,
-                 const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+    tc_dq_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                  const __grid_constant__ TcParams p) {
   using Sh = BwdShape<DP>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  const Block<DP> blk(smem_raw);
+  __shared__ float s_delta[2][kTile];
+  const Block<DP, false> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = 16, kMmaWarp = 17;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
@@ -145,7 +162,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
   tc_fence_after();
   pdl_wait();
   pdl_trigger();
-  const uint32_t tmem = s_tmem, acc = tmem + 256;
+  const uint32_t tmem = s_tmem, acc = tmem + 256, t_q = acc + DP, t_do = t_q + DP / 2;
   const Params& x = p.x;
   const int q0 = (int)(blockIdx.x % p.qtiles) * kTile;
   const int h = (int)(blockIdx.x / p.qtiles % x.H), hk = h / (x.H / x.Hkv);
@@ -158,11 +175,6 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
   int issued = 0;  // streamed tiles asked for (lane 0 of the TMA warp)
   if (warp == kTmaWarp) {
     if (lane == 0 && tiles > 0) {
-      mbar_expect_tx(blk.own, 2 * Sh::kOpA);
-      for (int kb = 0; kb < DP / 64; ++kb) {
-        tma_load_4d(blk.a0 + kb * Sh::kBlockA, &mq, kb * 64, q0, h, (int)b, blk.own);
-        tma_load_4d(blk.a1 + kb * Sh::kBlockA, &mdo, kb * 64, q0, h, (int)b, blk.own);
-      }
       for (int j = 0; j < tiles; ++j) {
         const int s = j % Sh::kStages;
         if (!wait(&blk.empty[s], j / Sh::kStages ^ 1)) break;
@@ -183,7 +195,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
       const uint4 mine = j & 1 ? make_uint4(bits.z, bits.w, ~0u, ~0u) : make_uint4(bits.x, bits.y, ~0u, ~0u);
       if (!all_bits(mine)) zero_rows<DP, kB>(blk.b0 + s * Sh::kOpB, mine, lane);  // dS 0 times K
       tc_fence_after();
-      blk.products(is, tmem, j & 1, s);
+      blk.products_ts(is, tmem, t_q, t_do, j & 1, s);
       return true;
     };
     bool ok = tiles > 0 && wait_all(blk.own, 0) && start(0) && (tiles < 2 || start(1));
@@ -191,7 +203,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
       if (!(ok = wait_all(&blk.ds_full[j & 1], j >> 1))) break;
       tc_fence_after();
       const int s = j % Sh::kStages;
-      blk.accumulate(is, acc, tmem + (j & 1) * 128, is.t0, s, j == 0);
+      blk.template accumulate<32>(is, acc, tmem + (j & 1) * 128, is.t0, s, j == 0);
       umma_done(is.one, &blk.empty[s]);
       if (j == tiles - 1) umma_done(is.one, blk.done);
       if (j + 2 < tiles) ok = start(j + 2);
@@ -204,32 +216,64 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
     const uint32_t tS = tmem + lanes + w * 128;
     const int64_t at = (b * x.H + h) * x.Lq + row;
     const float c2 = x.scale * kLog2e;
-    const float nl = row < x.Lq ? -x.lse2[at] : -INFINITY, delta = row < x.Lq ? x.delta[at] : 0.0f;
+    // The block's own operands: buffer 0's threads bring q to TMEM, buffer 1's do, half a row each (zeros past the
+    // ends), and take delta = do . o from it.
+    {
+      const View& src = w ? x.dout : x.q;
+      const __nv_bfloat16* from =
+          static_cast<const __nv_bfloat16*>(src.p) + b * src.sb + (int64_t)row * src.st + (int64_t)h * src.sh;
+      const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(x.o) + ((b * x.Lq + row) * x.H + h) * (int64_t)x.D;
+      float2 dot = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int c = 0; c < DP / 2; c += 32) {
+        uint32_t r[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = half * (DP / 2) + c + i * 8;
+          uint4 v = make_uint4(0, 0, 0, 0), u = v;
+          if (row < x.Lq && d < x.D) {
+            v = *reinterpret_cast<const uint4*>(from + d);
+            if (w) u = *reinterpret_cast<const uint4*>(o + d);
+          }
+          r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
+          const uint32_t ow[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            dot = fma2(make_float2(__uint_as_float(r[4 * i + e] << 16), __uint_as_float(r[4 * i + e] & 0xffff0000u)),
+                       make_float2(__uint_as_float(ow[e] << 16), __uint_as_float(ow[e] & 0xffff0000u)), dot);
+        }
+        tmem_st16((w ? t_do : t_q) + lanes + half * (DP / 4) + c / 2, r);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(blk.own);
+      if (w) s_delta[half][tid & 127] = dot.x + dot.y;
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+    }
+    const float nl = row < x.Lq ? -x.lse2[at] : -INFINITY;
+    const float delta = s_delta[0][tid & 127] + s_delta[1][tid & 127];
+    if (w && half == 0 && row < x.Lq) x.delta[at] = delta;  // for dk and dv
     const float2 cc = make_float2(c2, c2), ll = make_float2(nl, nl), dd = make_float2(-delta, -delta);
     bool ok = true;
     for (int j = w; j < tiles; j += 2) {
       const uint4 bits = key_bits(p, b, nk, j * kB & ~127);
       const uint32_t word = j & 1 ? (half ? bits.w : bits.z) : (half ? bits.y : bits.x);
-      if (ok) ok = wait_all(&blk.sd_full[w], j >> 1);
+      if (!(ok = wait_all(&blk.sd_full[w], j >> 1))) break;
       tc_fence_after();
-      float s[32], g[32];
-      if (ok && !idle) {
+      if (!idle) {
+        float s[32], g[32];
         tmem_ld32_nowait(tS + half * 32, s);
         tmem_ld32_nowait(tS + 64 + half * 32, g);
         tmem_wait_ld();
         tmem_pin<32>(s);
         tmem_pin<32>(g);
-      }
-      asm volatile("bar.sync %0, 256;" ::"r"(1 + w) : "memory");  // both halves' scores are read before weights go over them
-      if (!ok) continue;
-      if (!idle) {
         uint32_t r[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float2 e = fma2(make_float2(s[2 * i], s[2 * i + 1]), cc, ll);
           e.x = ex2(e.x), e.y = ex2(e.y);
-          const float2 d = add2(make_float2(g[2 * i], g[2 * i + 1]), dd);
-          s[2 * i] = e.x * d.x, s[2 * i + 1] = e.y * d.y;
+          e = mul2(e, add2(make_float2(g[2 * i], g[2 * i + 1]), dd));
+          s[2 * i] = e.x, s[2 * i + 1] = e.y;
         }
         if (word != 0xffffffffu) {
 #pragma unroll
@@ -237,7 +281,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[i] = pack_bf16(s[2 * i], s[2 * i + 1]);
-        tmem_st16(tS + half * 16, r);
+        tmem_st16(tS + half * 32, r);  // over scores of this thread's own
         tmem_wait_st();
       }
       tc_fence_before();
@@ -255,7 +299,6 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
   if (s_abort) {  // the same for all: nothing writes it after the barrier
     if (warp == kMmaWarp) drain_umma(blk.drain);
     if (warp == kTmaWarp && lane == 0 && tiles > 0) {
-      mbar_wait(blk.own, 0);
       drain_copies(blk.full, issued, Sh::kStages);
     }
     __syncthreads();
@@ -273,7 +316,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ float4 s_stat[2][2][2][kB / 4];  // warpgroup, slot, (-lse2, -delta)
-  const Block<DP> blk(smem_raw);
+  const Block<DP, true> blk(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = 8, kMmaWarp = 9;
   if (warp == kMmaWarp) alloc_tmem(&s_tmem);
@@ -331,8 +374,8 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDkvThreads, 1)
       if (!(ok = wait_all(&blk.ds_full[i & 1], i >> 1))) break;
       tc_fence_after();
       const int s = i % Sh::kStages;
-      blk.accumulate(is, acc_v, tmem + (i & 1) * 128, is.t1, s, i == 0);
-      blk.accumulate(is, acc_k, tmem + (i & 1) * 128 + 64, is.t0, s, i == 0);
+      blk.template accumulate<16>(is, acc_v, tmem + (i & 1) * 128, is.t1, s, i == 0);
+      blk.template accumulate<16>(is, acc_k, tmem + (i & 1) * 128 + 64, is.t0, s, i == 0);
       umma_done(is.one, &blk.empty[s]);
       if (i == tiles - 1) umma_done(is.one, blk.done);
       if (i + 2 < tiles) ok = start(i + 2);
@@ -417,25 +460,25 @@ template <int DP>
 static int launch_bwd(TcParams& t, cudaStream_t st) {
   using Sh = BwdShape<DP>;
   const Params& x = t.x;
-  CUtensorMap q128, q64, g128, g64, k128, k64, v128, v64;
-  if (!make_map(&q128, x.q, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&q64, x.q, x.D, x.Lq, x.H, x.B, kB) ||
-      !make_map(&g128, x.dout, x.D, x.Lq, x.H, x.B, kTile) || !make_map(&g64, x.dout, x.D, x.Lq, x.H, x.B, kB) ||
+  // before the maps: encoding one needs the device's context, which these calls make current in a new thread
+  auto fq = tc_dq_kernel<DP>;
+  auto fk = tc_dkv_kernel<DP>;
+  if (!set_smem_limit(reinterpret_cast<const void*>(fq), Sh::kDqBytes) ||
+      !set_smem_limit(reinterpret_cast<const void*>(fk), Sh::kDkvBytes))
+    return HCLSM_ERR_LAUNCH;
+  CUtensorMap q64, g64, k128, k64, v128, v64;
+  if (!make_map(&q64, x.q, x.D, x.Lq, x.H, x.B, kB) || !make_map(&g64, x.dout, x.D, x.Lq, x.H, x.B, kB) ||
       !make_map(&k128, x.k, x.D, x.Lk, x.Hkv, x.B, kTile) || !make_map(&k64, x.k, x.D, x.Lk, x.Hkv, x.B, kB) ||
       !make_map(&v128, x.v, x.D, x.Lk, x.Hkv, x.B, kTile) || !make_map(&v64, x.v, x.D, x.Lk, x.Hkv, x.B, kB))
     return HCLSM_ERR_UNSUPPORTED;
   t.qtiles = (x.Lq + kTile - 1) / kTile;
   const int64_t gq = (int64_t)t.qtiles * x.H * x.B, gk = (int64_t)((x.Lk + kTile - 1) / kTile) * x.Hkv * x.B;
   if (gq > 0x7fffffff || gk > 0x7fffffff || (int64_t)((x.Lq + kB - 1) / kB) * x.H > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  auto fq = tc_dq_kernel<DP>;
-  auto fk = tc_dkv_kernel<DP>;
-  if (!set_smem_limit(reinterpret_cast<const void*>(fq), Sh::kBytes) ||
-      !set_smem_limit(reinterpret_cast<const void*>(fk), Sh::kBytes))
-    return HCLSM_ERR_LAUNCH;
-  if (const int rc = launch_pdl(fq, (unsigned)gq, Sh::kDqThreads, Sh::kBytes, st, q128, g128, k64, v64, t)) return rc;
-  return launch_pdl(fk, (unsigned)gk, Sh::kDkvThreads, Sh::kBytes, st, k128, v128, q64, g64, t);
+  if (const int rc = launch_pdl(fq, (unsigned)gq, Sh::kDqThreads, Sh::kDqBytes, st, k64, v64, t)) return rc;
+  return launch_pdl(fk, (unsigned)gk, Sh::kDkvThreads, Sh::kDkvBytes, st, k128, v128, q64, g64, t);
 }
 
-// x.delta is set; ws: tc_workspace bytes.
+// x.delta is room for the row sums; ws: tc_workspace bytes.
 int tc_bwd(const Params& p, void* ws, cudaStream_t st) {
   TcParams t = {};
   t.x = p;

@@ -9,6 +9,9 @@ forward output's rounding inside delta (3 u).  fp32 results carry sums of at mos
 a few thousand terms at 2^-24 each and hardware exp2 (2 ulp): 1e-5.
 """
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -340,6 +343,22 @@ def test_cross_attention_large_scores_and_empty_sizes(dtype):
         assert o.shape == q.shape and not o.any()
         for a in torch.autograd.grad(o, (q, k, v), torch.ones_like(o)):
             assert not a.any()
+
+
+def test_first_call_of_a_thread():
+    """A thread without a current context: the forward and the backward (autograd's own thread) bind it themselves."""
+    code = """
+import threading, torch
+from hclsm_b200.kernels import cross_attention
+x = [torch.randn(2, 150, 2, 64, device="cuda").bfloat16().requires_grad_() for _ in range(3)]
+out = []
+t = threading.Thread(target=lambda: out.append(cross_attention(*x)))
+t.start(), t.join()
+g = torch.autograd.grad(out[0], x, torch.ones_like(out[0]))
+assert all(torch.isfinite(v).all() for v in (out[0], *g))
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=root, timeout=300)
 
 
 @pytest.mark.parametrize("Lq", [1, 150])
