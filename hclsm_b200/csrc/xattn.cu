@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
 
 // dq (KEYROWS false): rows are queries, columns keys, acc += ds k.
 // dk, dv (KEYROWS): rows are keys, columns queries, so the scores are formed transposed;
-// acc (dk) += ds^T q and acc2 (dv) += p^T do, over the query heads that share the key head one after another.
+// acc (dk) += ds^T q and acc2 (dv) += p^T do, over the query heads that share the key head one after another, or
+// (p.part) over one of them, whose sums join_heads_kernel adds.
 template <typename T, int DP, bool VEC, int TM, bool KEYROWS>
 __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_constant__ Params p) {
   constexpr int NT = kTileThreads<TM>, NP = kPieces<T>;
@@ -334,9 +335,12 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
   pdl_trigger();
   const int own = KEYROWS ? p.Lk : p.Lq, heads = KEYROWS ? p.Hkv : p.H, G = p.H / p.Hkv;
   const int tiles = (own + TM - 1) / TM;
-  const int r0 = (int)(blockIdx.x % tiles) * TM;
-  const int h = (int)(blockIdx.x / tiles % heads);
-  const int64_t b = blockIdx.x / tiles / heads;
+  const bool apart = KEYROWS && p.part;
+  const int only = apart ? (int)(blockIdx.x % G) : 0;  // the query head of this block
+  const unsigned int block = apart ? blockIdx.x / G : blockIdx.x;
+  const int r0 = (int)(block % tiles) * TM;
+  const int h = (int)(block / tiles % heads);
+  const int64_t b = block / tiles / heads;
   const int nk = key_count(p, b), ksteps = (p.D + 15) / 16;
   const float c2 = p.scale * kLog2e;
   auto keys = [&](__nv_bfloat16* k, __nv_bfloat16* v, int hk, int k0) {
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
   };
   float acc[DP / 8][4] = {}, acc2[KEYROWS ? DP / 8 : 1][4] = {};
   const int n = KEYROWS ? p.Lq : nk;  // streamed rows of a head
-  const int loops = KEYROWS ? (r0 < nk ? G : 0) : 1;
+  const int loops = KEYROWS ? (r0 < nk ? (apart ? 1 : G) : 0) : 1;
   if (loops > 0) {
     if constexpr (KEYROWS) keys(a0, a1, h, r0);
     else queries(a0, a1, h, r0);
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
   for (int q = 0; q < loops; ++q)
     for (int s0 = 0; s0 < n; s0 += kT) {
       __syncthreads();
-      if constexpr (KEYROWS) queries(b0, b1, h * G + q, s0);
+      if constexpr (KEYROWS) queries(b0, b1, h * G + only + q, s0);
       else keys(b0, b1, h / G, s0);
       __syncthreads();
       float s[4][4], d[4][4];
@@ -395,11 +399,39 @@ __global__ void __launch_bounds__(kTileThreads<TM>) bwd_kernel(const __grid_cons
   join_rows<DP>(acc, other, one, one, lane);
   if constexpr (KEYROWS) {
     join_rows<DP>(acc2, other + TM * DP, one, one, lane);
+    if (apart) {
+      const int64_t n = (int64_t)p.B * p.Lk * p.Hkv * p.D;
+      store_rows<float, DP>(p.part + only * n, acc, p.scale, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
+      store_rows<float, DP>(p.part + (G + only) * n, acc2, 1.0f, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
+      return;
+    }
     store_rows<T, DP>(p.dk, acc, p.scale, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
     store_rows<T, DP>(p.dv, acc2, 1.0f, p, b, p.Lk, p.Hkv, h, r0 + rw, lane);
   } else {
     store_rows<T, DP>(p.dq, acc, p.scale, p, b, p.Lq, p.H, h, r0 + rw, lane);
   }
+}
+
+// dk (blockIdx.y 0) and dv (1) from the query heads' parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_heads_kernel(const __grid_constant__ Params p) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t n = (int64_t)p.B * p.Lk * p.Hkv * p.D, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= n) return;
+  const int G = p.H / p.Hkv;
+  const float* part = p.part + blockIdx.y * G * n + i;
+  float a = 0.0f;
+  for (int g = 0; g < G; ++g) a += part[g * n];
+  io<T>::st(static_cast<T*>(blockIdx.y ? p.dv : p.dk) + i, a);
+}
+
+// Whether dk and dv take a block a query head: shared key heads, and too few blocks for the SMs otherwise.
+bool heads_apart(const Params& p) {
+  return p.H > p.Hkv && (int64_t)((p.Lk + 31) / 32) * p.Hkv * p.B < 2 * (int64_t)num_sms();
+}
+size_t part_bytes(const Params& p) {
+  return heads_apart(p) ? (size_t)2 * p.B * p.Lk * p.H * p.D * sizeof(float) : 0;
 }
 
 // delta_i = do_i . o_i, one warp a row.
@@ -424,7 +456,8 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__
 template <typename T, int DP, bool VEC, int TM>
 int launch_rows(const Params& p, int which, cudaStream_t st) {  // 0 forward, 1 dq, 2 dk and dv
   const int64_t rows = which == 2 ? p.Lk : p.Lq, heads = which == 2 ? p.Hkv : p.H;
-  const int64_t grid = (rows + TM - 1) / TM * heads * p.B;
+  const bool apart = which == 2 && p.part;
+  const int64_t grid = (rows + TM - 1) / TM * heads * p.B * (apart ? p.H / p.Hkv : 1);
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
   if (grid == 0) return HCLSM_OK;
   const size_t bytes = which == 0 ? smem_bytes<T, DP, TM, 1>() : smem_bytes<T, DP, TM, 2>();
@@ -432,7 +465,10 @@ int launch_rows(const Params& p, int which, cudaStream_t st) {  // 0 forward, 1 
            : which == 1 ? bwd_kernel<T, DP, VEC, TM, false>
                         : bwd_kernel<T, DP, VEC, TM, true>;
   if (!set_smem_limit(reinterpret_cast<const void*>(f), bytes)) return HCLSM_ERR_LAUNCH;
-  return launch_pdl(f, (unsigned)grid, kTileThreads<TM>, bytes, st, p);
+  const int rc = launch_pdl(f, (unsigned)grid, kTileThreads<TM>, bytes, st, p);
+  if (rc || !apart) return rc;
+  const int64_t n = (int64_t)p.B * p.Lk * p.Hkv * p.D;
+  return launch_pdl(join_heads_kernel<T>, dim3((unsigned)((n + kThreads - 1) / kThreads), 2), kThreads, 0, st, p);
 }
 
 template <typename T, int DP, bool VEC>
@@ -565,7 +601,7 @@ static bool use_tc_bwd(const xattn::Params& p, int dtype) {
 extern "C" size_t hclsm_xattn_bwd_workspace_size(const hclsm_xattn_args* a) {
   if (xattn::check(a)) return 0;
   const xattn::Params p = xattn::params(a);
-  return xattn::delta_bytes(p) + (a->dtype == HCLSM_BF16 ? xattn::tc_workspace(p) : 0);
+  return xattn::delta_bytes(p) + (use_tc_bwd(p, a->dtype) ? xattn::tc_workspace(p) : xattn::part_bytes(p));
 }
 
 extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -573,12 +609,15 @@ extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (a->B == 0) return HCLSM_OK;
   if (a->Lq > 0 && (!a->q.p || !a->o || !a->dout.p || !a->dq || !a->lse2)) return HCLSM_ERR_NULL;
   if (a->Lk > 0 && (!a->k.p || !a->v.p || !a->dk || !a->dv)) return HCLSM_ERR_NULL;
-  if (ws_bytes < hclsm_xattn_bwd_workspace_size(a) || (a->Lq > 0 && !ws)) return HCLSM_ERR_WORKSPACE;
+  const size_t need = hclsm_xattn_bwd_workspace_size(a);
+  if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
   xattn::Params p = xattn::params(a);
   p.delta = static_cast<float*>(ws);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (use_tc_bwd(p, a->dtype)) return xattn::tc_bwd(p, static_cast<char*>(ws) + xattn::delta_bytes(p), st);
+  void* more = static_cast<char*>(ws) + xattn::delta_bytes(p);
+  if (use_tc_bwd(p, a->dtype)) return xattn::tc_bwd(p, more, st);
+  if (xattn::heads_apart(p)) p.part = static_cast<float*>(more);
   if (const int rc = xattn::launch_delta(p, a->dtype, st)) return rc;
   return a->dtype == HCLSM_F32 ? xattn::dispatch<float>(p, true, st) : xattn::dispatch<__nv_bfloat16>(p, true, st);
 }

@@ -32,6 +32,7 @@ struct Params {
   void *o, *dq, *dk, *dv;      // dense (B, L, H, D)
   float* lse2;                 // (B, H, Lq)
   float* delta;                // (B, H, Lq)
+  float* part;                 // the mma.sync dk, dv kernel: (2, G, B, Lk, Hkv, D) of each query head, or null
   const int32_t* lens;         // (B) or null
   const uint8_t* mask;         // (B, Lk) rows mask_sb apart, or null
   int64_t mask_sb;
