@@ -231,11 +231,12 @@ __device__ __forceinline__ void load_a(const uint32_t* w, uint32_t (&a)[4]) {
 // Steps first, first + stride, ... below last of 16 keys each.  addr_k / addr_v
 // (key) give a row's address; ok(key) says whether the key is allowed (false
 // past the end); nk > 0 keys have memory; all_ok(step) skips the per-key checks.
-// fs, off: factor and offset of rows g and g + 8's raw scores.
+// fs, off: factor and offset of rows g and g + 8's raw scores.  vref (F16): the largest value scale so far; O is held
+// over it, times 2^12.
 template <typename E, int D, int CV, int NQ, int NR, bool F16, typename AddrK, typename AddrV, typename Ok,
           typename AllOk, typename Scale>
 __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const float (&fs)[2], const float (&off)[2],
-                                      int first, int last, int stride, int nk,
+                                      float& vref, int first, int last, int stride, int nk,
                                       AddrK addr_k, AddrV addr_v, Ok ok, AllOk all_ok, Scale scale) {
   using R = Rows<E, D, CV>;
   // fp32: a product is formed from zero and added here, because the tensor core's own
@@ -253,12 +254,20 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
 #pragma unroll
     for (int t = 0; t < 4; ++t) R::load_v(addr_v(min(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1), nk - 1)), g, vr[t]);
   };
-  float vref = 0.0f;  // F16: the largest value scale so far; O is held over it, times 2^12
   float2 sc = scale(first);
   fetch_k(first);
   fetch_v(first);
   for (int step = first; step < last; step += stride) {
     const int next = step + stride < last ? step + stride : step;
+    if (const int far = step + 2 * stride; far < last) {  // the step after the next from DRAM to L2
+      constexpr int kLines = D * R::kES >= 128 ? D * R::kES / 128 : 1;  // of a row
+#pragma unroll
+      for (int at = lane; at < 16 * kLines; at += 32) {
+        const int j = min(far * 16 + at / kLines, nk - 1);
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(addr_k(j) + at % kLines * 128));
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(addr_v(j) + at % kLines * 128));
+      }
+    }
     float s[2][4] = {};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
@@ -377,13 +386,6 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
     }
     fetch_v(next);
   }
-  if constexpr (F16) {
-    const float w = vref * (1.0f / 4096.0f);
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
-  }
 }
 
 template <typename T, int D, bool CACHE, int NR>
@@ -452,9 +454,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
   const float c2 = p.x.scale * kLog2e;
   const float fs[2] = {c2, c2}, off[2] = {0.0f, 0.0f};
   // this block's share of the sequence's own steps
-  // the cache: tokens in 8 bits; a length inside the block that the tail holds (scale -1) ends before it
-  int n8 = n;
-  if (CACHE && n % p.block && p.ks[bh * (p.T / p.block) + n / p.block] < 0.0f) n8 = n / p.block * p.block;
+  const int n8 = CACHE ? n / p.block * p.block : n;
   const int steps = (n8 + 15) / 16, per = (steps + p.splits - 1) / p.splits;
   const int first = min(steps, sp * per), last = min(steps, first + per);
   if constexpr (CACHE) {
@@ -467,30 +467,45 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
 #pragma unroll
       for (int r = 0; r < 2; ++r) fs8[r] = c2 / s_inv[g + 8 * r], off8[r] = 1152.0f * s_sum[g + 8 * r];
     }
+    float vref = 0.0f;
+    auto scale = [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); };
+    auto key = [&](int j) { return k8 + (int64_t)j * D; };
+    auto value = [&](int j) { return v8 + (int64_t)j * D; };
     sweep<int8_t, D, CV, NQ, NR, F16>(
-        st, qh, fs8, off8, first + warp, last, kWarps, n8, [&](int j) { return k8 + (int64_t)j * D; },
-        [&](int j) { return v8 + (int64_t)j * D; }, [&](int j) { return j < n8; },
-        [&](int step) { return step * 16 + 16 <= n8; },
-        [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); });
-  } else {
-    const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);
-    const char* vb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.v.p) + b * p.x.v.sb + hk * p.x.v.sh);
-    const int64_t kst = p.x.k.st * (int64_t)sizeof(T), vst = p.x.v.st * (int64_t)sizeof(T);
-    sweep<T, D, CV, NQ, NR, false>(
-        st, qf, fs, off, first + warp, last, kWarps, n, [&](int j) { return kb + j * kst; },
-        [&](int j) { return vb + j * vst; }, [&](int j) { return xattn::key_ok(p.x, b, n, j); },
-        [&](int step) { return !p.x.mask && step * 16 + 16 <= n; }, [](int) { return make_float2(1.0f, 1.0f); });
-  }
-  if constexpr (CACHE) {
-    if (sp == p.splits - 1 && n > n8) {  // the last, incomplete block, in the inputs' own type
+        st, qh, fs8, off8, vref, first + warp, last, kWarps, n8, key, value, [](int) { return true; },
+        [](int) { return true; }, scale);
+    // a length inside a block: a complete one (8 bits), or the one that the tail holds (scale -1)
+    const bool more = sp == p.splits - 1 && n > n8;
+    const bool tail = more && p.ks[s0 + n8 / p.block] < 0.0f;
+    if (more && !tail)
+      sweep<int8_t, D, CV, NQ, NR, F16>(
+          st, qh, fs8, off8, vref, steps + warp, (n + 15) / 16, kWarps, n, key, value, [&](int j) { return j < n; },
+          [&](int step) { return step * 16 + 16 <= n; }, scale);
+    if constexpr (F16) {
+      const float w = vref * (1.0f / 4096.0f);
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
+    }
+    if (tail) {
       const char* kt = reinterpret_cast<const char*>(static_cast<const T*>(p.kt) + bh * p.block * D);
       const char* vt = reinterpret_cast<const char*>(static_cast<const T*>(p.vt) + bh * p.block * D);
       const int nt = n - n8;
       sweep<T, D, CV, NQ, NR, false>(
-          st, qf, fs, off, warp, (nt + 15) / 16, kWarps, nt, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
+          st, qf, fs, off, vref, warp, (nt + 15) / 16, kWarps, nt, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
           [&](int j) { return vt + j * (int)(D * sizeof(T)); }, [&](int j) { return j < nt; },
           [&](int step) { return step * 16 + 16 <= nt; }, [](int) { return make_float2(1.0f, 1.0f); });
     }
+  } else {
+    float vref = 0.0f;
+    const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.v.p) + b * p.x.v.sb + hk * p.x.v.sh);
+    const int64_t kst = p.x.k.st * (int64_t)sizeof(T), vst = p.x.v.st * (int64_t)sizeof(T);
+    sweep<T, D, CV, NQ, NR, false>(
+        st, qf, fs, off, vref, first + warp, last, kWarps, n, [&](int j) { return kb + j * kst; },
+        [&](int j) { return vb + j * vst; }, [&](int j) { return xattn::key_ok(p.x, b, n, j); },
+        [&](int step) { return !p.x.mask && step * 16 + 16 <= n; }, [](int) { return make_float2(1.0f, 1.0f); });
   }
   // ---- merge the warps, in order -----------------------------------------------------
 #pragma unroll
