@@ -93,7 +93,7 @@ SIGNATURES = {
 # passes as a pointer; several times cheaper to make than a ctypes.Structure).
 VIEW = struct.Struct("@Pqqq")                     # hclsm_view
 ROPE_SIDE = struct.Struct("@6P3q2i")              # hclsm_rope_side
-XATTN_ARGS = struct.Struct("@" + 4 * "Pqqq" + "7Pq7if")  # hclsm_xattn_args
+XATTN_ARGS = struct.Struct("@" + 4 * "Pqqq" + "8Pq7if")  # hclsm_xattn_args
 KV8_CACHE = struct.Struct("@6P6i")                # hclsm_kv8_cache
 
 

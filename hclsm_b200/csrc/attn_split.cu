@@ -388,6 +388,12 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
   }
 }
 
+template <typename T>
+__device__ __forceinline__ void store_o(const xattn::Params& x, int64_t at, float v) {
+  io<T>::st(static_cast<T*>(x.o) + at, v);
+  if (sizeof(T) == 2 && x.lo) x.lo[at] = __float2bfloat16_rn(xattn::rounding(v));
+}
+
 template <typename T, int D, bool CACHE, int NR>
 __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __grid_constant__ Params p) {
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1;
@@ -552,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
     if (p.splits > 1)
       p.part_o[(((bh * p.rtiles + rt) * p.splits + sp) * kRows + r) * D + d] = a;
     else
-      io<T>::st(static_cast<T*>(p.x.o) + ((b * p.x.Lq + row / G) * p.x.H + hk * G + row % G) * (int64_t)D + d, a);
+      store_o<T>(p.x, ((b * p.x.Lq + row / G) * p.x.H + hk * G + row % G) * (int64_t)D + d, a);
   }
 }
 
@@ -583,9 +589,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
     for (int i = 0; i < D / 32; ++i) acc[i] += f * o[lane + 32 * i];
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(p.x.o) + ((b * p.x.Lq + row / G) * p.x.H + h) * (int64_t)D;
+  const int64_t out = ((b * p.x.Lq + row / G) * p.x.H + h) * (int64_t)D;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) io<T>::st(out + lane + 32 * i, acc[i] * inv);
+  for (int i = 0; i < D / 32; ++i) store_o<T>(p.x, out + lane + 32 * i, acc[i] * inv);
   if (p.x.lse2 && lane == 0) p.x.lse2[(b * p.x.H + h) * p.x.Lq + row / G] = l == 0.0f ? INFINITY : m + log2f(l);
 }
 

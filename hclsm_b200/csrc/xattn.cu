@@ -202,7 +202,7 @@ __device__ __forceinline__ void join_rows(float (&acc)[DP / 8][4], const float* 
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8][4], float f, const Params& p, int64_t b, int L, int H, int h, int r0, int lane) {
+__device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8][4], float f, const Params& p, int64_t b, int L, int H, int h, int r0, int lane, __nv_bfloat16* lo = nullptr) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -214,7 +214,11 @@ __device__ __forceinline__ void store_rows(void* dst, const float (&acc)[DP / 8]
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int d = j * 8 + 2 * c + e;
-        if (d < p.D) io<T>::st(out + d, acc[j][2 * r + e] * f);
+        if (d < p.D) {
+          io<T>::st(out + d, acc[j][2 * r + e] * f);
+          if (sizeof(T) == 2 && lo)
+            lo[out - static_cast<T*>(dst) + d] = __float2bfloat16_rn(rounding(acc[j][2 * r + e] * f));
+        }
       }
   }
 }
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(kTileThreads<TM>) fwd_kernel(const __grid_cons
     if (p.lse2 && c == 0 && row < p.Lq) p.lse2[(b * p.H + h) * p.Lq + row] = empty ? INFINITY : mx + log2f(sum);
   }
   join_rows<DP>(acc, other, f0, f1, lane);
-  store_rows<T, DP>(p.o, acc, 1.0f, p, b, p.Lq, p.H, h, r0 + rw, lane);
+  store_rows<T, DP>(p.o, acc, 1.0f, p, b, p.Lq, p.H, h, r0 + rw, lane, p.lo);
 }
 
 // dq (KEYROWS false): rows are queries, columns keys, acc += ds k.
@@ -447,7 +451,11 @@ __global__ void __launch_bounds__(kThreads) delta_kernel(const __grid_constant__
   const T* o = static_cast<const T*>(p.o) + row * p.D;
   const T* g = static_cast<const T*>(p.dout.p) + b * p.dout.sb + t * p.dout.st + h * p.dout.sh;
   float a = 0.0f;
-  for (int d = lane; d < p.D; d += 32) a += io<T>::ld(o + d) * io<T>::ld(g + d);
+  for (int d = lane; d < p.D; d += 32) {
+    float v = io<T>::ld(o + d);
+    if (sizeof(T) == 2 && p.lo) v += __bfloat162float(p.lo[row * p.D + d]);
+    a += v * io<T>::ld(g + d);
+  }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) a += __shfl_xor_sync(0xffffffffu, a, s);
   if (lane == 0) p.delta[(b * p.H + h) * p.Lq + t] = a;
@@ -524,6 +532,7 @@ Params params(const hclsm_xattn_args* a) {
   p.q = view(a->q), p.k = view(a->k), p.v = view(a->v), p.dout = view(a->dout);
   p.o = a->o, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
   p.lse2 = a->lse2;
+  p.lo = a->dtype == HCLSM_BF16 ? static_cast<__nv_bfloat16*>(a->lo) : nullptr;
   p.lens = a->lens, p.mask = a->mask, p.mask_sb = a->mask_sb;
   p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.Hkv = a->Hkv, p.D = a->D;
   p.scale = a->scale;
@@ -582,6 +591,7 @@ extern "C" int hclsm_xattn_fwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (const int rc = xattn::check(a)) return rc;
   if ((int64_t)a->B * a->Lq == 0) return HCLSM_OK;
   if (!a->q.p || !a->o || (a->Lk > 0 && (!a->k.p || !a->v.p))) return HCLSM_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->lo) % 16) return HCLSM_ERR_ALIGN;
   const xattn::Params p = xattn::params(a);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Path path = fwd_path(p, a->dtype);
@@ -609,6 +619,7 @@ extern "C" int hclsm_xattn_bwd(const hclsm_xattn_args* a, void* ws, size_t ws_by
   if (a->B == 0) return HCLSM_OK;
   if (a->Lq > 0 && (!a->q.p || !a->o || !a->dout.p || !a->dq || !a->lse2)) return HCLSM_ERR_NULL;
   if (a->Lk > 0 && (!a->k.p || !a->v.p || !a->dk || !a->dv)) return HCLSM_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->lo) % 16) return HCLSM_ERR_ALIGN;
   const size_t need = hclsm_xattn_bwd_workspace_size(a);
   if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;

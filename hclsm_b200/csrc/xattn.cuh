@@ -31,6 +31,7 @@ struct Params {
   View q, k, v, dout;          // (B, L, H, D), innermost dense
   void *o, *dq, *dk, *dv;      // dense (B, L, H, D)
   float* lse2;                 // (B, H, Lq)
+  __nv_bfloat16* lo;           // bf16 calls, (B, Lq, H, D) or null: o before rounding minus o
   float* delta;                // (B, H, Lq)
   float* part;                 // the mma.sync dk, dv kernel: (2, G, B, Lk, Hkv, D) of each query head, or null
   const int32_t* lens;         // (B) or null
@@ -45,6 +46,8 @@ struct Params {
 __device__ __forceinline__ int key_count(const Params& p, int64_t b) {
   return p.lens ? min(max(p.lens[b], 0), p.Lk) : p.Lk;
 }
+// What rounding to bf16 takes from v.
+__device__ __forceinline__ float rounding(float v) { return v - __bfloat162float(__float2bfloat16_rn(v)); }
 __device__ __forceinline__ bool key_ok(const Params& p, int64_t b, int n, int j) {
   return j < n && (!p.mask || p.mask[b * p.mask_sb + j]);
 }

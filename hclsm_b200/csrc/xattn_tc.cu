@@ -327,6 +327,13 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
               for (int e = 0; e < 4; ++e)  // a row without keys: zero, whatever O holds
                 q[e] = inv == 0.0f ? 0u : pack_bf16(o[i + 2 * e] * inv, o[i + 2 * e + 1] * inv);
               *reinterpret_cast<uint4*>(out + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
+              if (x.lo) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  q[e] = inv == 0.0f ? 0u : pack_bf16(rounding(o[i + 2 * e] * inv), rounding(o[i + 2 * e + 1] * inv));
+                *reinterpret_cast<uint4*>(x.lo + (out - static_cast<__nv_bfloat16*>(x.o)) + c + i) =
+                    make_uint4(q[0], q[1], q[2], q[3]);
+              }
             }
         }
       }

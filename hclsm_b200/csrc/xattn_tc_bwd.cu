@@ -236,11 +236,13 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
             if (w) u = *reinterpret_cast<const uint4*>(o + d);
           }
           r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
-          const uint32_t ow[4] = {u.x, u.y, u.z, u.w};
+          uint4 lo = make_uint4(0, 0, 0, 0);
+          if (w && x.lo && row < x.Lq && d < x.D)
+            lo = *reinterpret_cast<const uint4*>(x.lo + (o - static_cast<const __nv_bfloat16*>(x.o)) + d);
+          const uint32_t ow[4] = {u.x, u.y, u.z, u.w}, lw[4] = {lo.x, lo.y, lo.z, lo.w};
+          auto both = [](uint32_t t) { return make_float2(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u)); };
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dot = fma2(make_float2(__uint_as_float(r[4 * i + e] << 16), __uint_as_float(r[4 * i + e] & 0xffff0000u)),
-                       make_float2(__uint_as_float(ow[e] << 16), __uint_as_float(ow[e] & 0xffff0000u)), dot);
+          for (int e = 0; e < 4; ++e) dot = fma2(both(r[4 * i + e]), add2(both(ow[e]), both(lw[e])), dot);
         }
         tmem_st16((w ? t_do : t_q) + lanes + half * (DP / 4) + c / 2, r);
       }

@@ -17,7 +17,7 @@ from .. import _lib
 __all__ = ["cross_attention"]
 
 
-def _args(q, k, v, o, lse, lens, mask, scale, do=None, dq=None, dk=None, dv=None):
+def _args(q, k, v, o, lse, lo, lens, mask, scale, do=None, dq=None, dk=None, dv=None):
     B, Lq, H, D = q.shape
     qb, qt, qh, _ = q.stride()
     kb, kt, kh, _ = k.stride()
@@ -28,31 +28,34 @@ def _args(q, k, v, o, lse, lens, mask, scale, do=None, dq=None, dk=None, dv=None
         dqp, dkp, dvp = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     return _lib.XATTN_ARGS.pack(
         q.data_ptr(), qb, qt, qh, k.data_ptr(), kb, kt, kh, v.data_ptr(), vb, vt, vh, gp, gb, gt, gh, o.data_ptr(),
-        dqp, dkp, dvp, 0 if lse is None else lse.data_ptr(), 0 if lens is None else lens.data_ptr(),
+        dqp, dkp, dvp, 0 if lse is None else lse.data_ptr(), 0 if lo is None else lo.data_ptr(),
+        0 if lens is None else lens.data_ptr(),
         0 if mask is None else mask.data_ptr(), 0 if mask is None else mask.stride(0), B, Lq, k.shape[1], H, k.shape[2],
         D, _lib.dtype_code(q.dtype), scale)
 
 
 def _forward(q, k, v, lens, mask, scale, keep):
     o = q.new_empty(q.shape)
-    lse = None
+    lse = lo = None
     if keep:
         B, Lq, H, _ = q.shape
         lse = q.new_empty((B, H, Lq), dtype=torch.float32)
-    a = _args(q, k, v, o, lse, lens, mask, scale)
+        if q.dtype == torch.bfloat16:
+            lo = q.new_empty(q.shape)  # what rounding takes from o: the backward's row sums do . o are then fp32's
+    a = _args(q, k, v, o, lse, lo, lens, mask, scale)
     lib, ws = _lib.load(), None
     n = lib.hclsm_xattn_fwd_workspace_size(a)
     if n:
         ws = q.new_empty(n, dtype=torch.uint8)
     _lib.check(lib.hclsm_xattn_fwd(a, None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(q.device)),
                "hclsm_xattn_fwd")
-    return o, lse
+    return o, lse, lo
 
 
-def _backward(q, k, v, o, lse, lens, mask, scale, do):
+def _backward(q, k, v, o, lse, lo, lens, mask, scale, do):
     do = _lib.dense_last(do)
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
-    a = _args(q, k, v, o, lse, lens, mask, scale, do, dq, dk, dv)
+    a = _args(q, k, v, o, lse, lo, lens, mask, scale, do, dq, dk, dv)
     lib = _lib.load()
     n = lib.hclsm_xattn_bwd_workspace_size(a)
     ws = q.new_empty(n, dtype=torch.uint8)
@@ -63,16 +66,15 @@ def _backward(q, k, v, o, lse, lens, mask, scale, do):
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lens, mask, scale):
-        o, lse = _forward(q, k, v, lens, mask, scale, True)
-        ctx.save_for_backward(q, k, v, o, lse, lens, mask)
+        o, lse, lo = _forward(q, k, v, lens, mask, scale, True)
+        ctx.save_for_backward(q, k, v, o, lse, lo, lens, mask)
         ctx.scale = scale
         return o
 
     @staticmethod
     def backward(ctx, do):
         _lib.no_double_backward()
-        q, k, v, o, lse, lens, mask = ctx.saved_tensors
-        return (*_backward(q, k, v, o, lse, lens, mask, ctx.scale, do), None, None, None)
+        return (*_backward(*ctx.saved_tensors, ctx.scale, do), None, None, None)
 
 
 def _prepare(q, k, v, kv_lens, key_mask, scale):
@@ -102,14 +104,14 @@ def _prepare(q, k, v, kv_lens, key_mask, scale):
 
 
 def attention_fwd(q, k, v, kv_lens, key_mask, scale):
-    """(o, lse2): the forward and what its backward needs, without autograd."""
+    """(o, lse2, lo): the forward and what its backward needs (lo: None in fp32), without autograd."""
     return _forward(*_prepare(q, k, v, kv_lens, key_mask, scale), True)
 
 
-def attention_bwd(q, k, v, o, lse, do, kv_lens, key_mask, scale):
+def attention_bwd(q, k, v, o, lse, lo, do, kv_lens, key_mask, scale):
     """(dq, dk, dv) from attention_fwd's results."""
     q, k, v, lens, key_mask, scale = _prepare(q, k, v, kv_lens, key_mask, scale)
-    return _backward(q, k, v, o, lse, lens, key_mask, scale, do)
+    return _backward(q, k, v, o, lse, lo, lens, key_mask, scale, do)
 
 
 def cross_attention(q, k, v, *, kv_lens=None, key_mask=None, scale=None):

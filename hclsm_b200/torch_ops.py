@@ -242,24 +242,26 @@ torch.library.register_autograd(f"{_NS}::qk_norm_rope_fwd", _rope_backward, setu
 
 @torch.library.custom_op(f"{_NS}::cross_attention_fwd", mutates_args=())
 def cross_attention_fwd(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Tensor], key_mask: Optional[Tensor],
-                        scale: float) -> Tuple[Tensor, Tensor]:
-    return _xattn_fwd(q, k, v, kv_lens, key_mask, scale)
+                        scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    o, lse, lo = _xattn_fwd(q, k, v, kv_lens, key_mask, scale)
+    return o, lse, q.new_empty(0) if lo is None else lo
 
 
 @cross_attention_fwd.register_fake
 def _(q, k, v, kv_lens, key_mask, scale):
     B, Lq, H, _ = q.shape
-    return q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32)
+    return (q.new_empty(q.shape), q.new_empty((B, H, Lq), dtype=torch.float32),
+            q.new_empty(q.shape if q.dtype == torch.bfloat16 else 0))
 
 
 @torch.library.custom_op(f"{_NS}::cross_attention_bwd", mutates_args=())
-def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, do: Tensor,
+def cross_attention_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, lo: Tensor, do: Tensor,
                         kv_lens: Optional[Tensor], key_mask: Optional[Tensor], scale: float) -> List[Tensor]:
-    return list(_xattn_bwd(q, k, v, o, lse, do, kv_lens, key_mask, scale))
+    return list(_xattn_bwd(q, k, v, o, lse, lo if lo.numel() else None, do, kv_lens, key_mask, scale))
 
 
 @cross_attention_bwd.register_fake
-def _(q, k, v, o, lse, do, kv_lens, key_mask, scale):
+def _(q, k, v, o, lse, lo, do, kv_lens, key_mask, scale):
     return [t.new_empty(t.shape) for t in (q, k, v)]
 
 
@@ -269,9 +271,9 @@ def _xattn_setup(ctx, inputs, output):
     ctx.scale = scale
 
 
-def _xattn_backward(ctx, go, glse):
-    q, k, v, o, lse, kv_lens, key_mask = ctx.saved_tensors
-    return (*cross_attention_bwd(q, k, v, o, lse, go, kv_lens, key_mask, ctx.scale), None, None, None)
+def _xattn_backward(ctx, go, glse, glo):
+    q, k, v, o, lse, lo, kv_lens, key_mask = ctx.saved_tensors
+    return (*cross_attention_bwd(q, k, v, o, lse, lo, go, kv_lens, key_mask, ctx.scale), None, None, None)
 
 
 torch.library.register_autograd(f"{_NS}::cross_attention_fwd", _xattn_backward, setup_context=_xattn_setup)

@@ -389,13 +389,15 @@ int hclsm_qk_norm_rope_bwd(const hclsm_rope_side* q, const hclsm_rope_side* k, c
 /* Cross attention o = softmax(scale q k^T) v over the keys that lens (B) and
  * mask (B, Lk; rows mask_sb bytes apart) allow; a row with none gives 0.
  * H a multiple of Hkv: query head h reads key head h / (H / Hkv).  D <= 128.
- * o and the gradients are dense.  lse2 (B, H, Lq): NULL when no backward
- * follows; the backward reads what the forward wrote. */
+ * o and the gradients are dense.  lse2 (B, H, Lq) and, for bf16, lo: NULL when no
+ * backward follows; the backward reads what the forward wrote (without lo its row
+ * sums do . o carry o's rounding). */
 typedef struct {
   hclsm_view q, k, v, dout;
   void* o;
   void *dq, *dk, *dv;  /* backward only */
   float* lse2;
+  void* lo;            /* bf16, like o, or NULL: what rounding took from o */
   const int32_t* lens; /* or NULL */
   const uint8_t* mask; /* or NULL */
   int64_t mask_sb;

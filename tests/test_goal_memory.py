@@ -42,13 +42,13 @@ def test_c_entries_refuse_without_a_gpu():
 
     def xattn(**kw):
         a = dict(q=(16, 0, 0, 0), k=(16, 0, 0, 0), v=(16, 0, 0, 0), do=(0, 0, 0, 0), o=16, B=1, Lq=1, Lk=1, H=1, Hkv=1,
-                 D=64, dtype=0, scale=1.0)
+                 D=64, dtype=0, scale=1.0, lo=0)
         a.update(kw)
-        return _lib.XATTN_ARGS.pack(*a["q"], *a["k"], *a["v"], *a["do"], a["o"], 0, 0, 0, 0, 0, 0, 0, a["B"], a["Lq"],
+        return _lib.XATTN_ARGS.pack(*a["q"], *a["k"], *a["v"], *a["do"], a["o"], 0, 0, 0, 0, a["lo"], 0, 0, 0, a["B"], a["Lq"],
                                     a["Lk"], a["H"], a["Hkv"], a["D"], a["dtype"], a["scale"])
 
     for want, kw in ((2, dict(dtype=7)), (1, dict(D=129)), (1, dict(D=0)), (1, dict(H=3, Hkv=2)), (1, dict(B=-1)),
-                     (1, dict(scale=0.0)), (1, dict(scale=float("nan"))), (8, dict(o=0)), (8, dict(k=(0, 0, 0, 0)))):
+                     (1, dict(scale=0.0)), (1, dict(scale=float("nan"))), (3, dict(lo=8)), (8, dict(o=0)), (8, dict(k=(0, 0, 0, 0)))):
         assert lib.hclsm_xattn_fwd(xattn(**kw), None, 0, None) == want, kw
     assert lib.hclsm_xattn_fwd(xattn(B=0), None, 0, None) == 0
     assert lib.hclsm_xattn_bwd(xattn(), None, 0, None) == 8
@@ -86,9 +86,11 @@ def test_ops_registered_and_fake_shapes():
     with FakeTensorMode():
         q = torch.empty(2, 5, 6, 64, dtype=torch.bfloat16, device="cuda")
         k = torch.empty(2, 9, 3, 64, dtype=torch.bfloat16, device="cuda")
-        o, lse = OPS.cross_attention_fwd(q, k, k, None, None, 0.1)
+        o, lse, lo = OPS.cross_attention_fwd(q, k, k, None, None, 0.1)
         assert o.shape == q.shape and o.dtype == q.dtype and lse.shape == (2, 6, 5) and lse.dtype == torch.float32
-        assert [t.shape for t in OPS.cross_attention_bwd(q, k, k, o, lse, o, None, None, 0.1)] == [q.shape, k.shape,
+        assert lo.shape == q.shape and OPS.cross_attention_fwd(q.float(), k.float(), k.float(), None, None,
+                                                               0.1)[2].numel() == 0
+        assert [t.shape for t in OPS.cross_attention_bwd(q, k, k, o, lse, lo, o, None, None, 0.1)] == [q.shape, k.shape,
                                                                                                k.shape]
         yq, yk = OPS.qk_norm_rope_fwd(q, k, None, None, None, None, None, None, 1e-6, False)
         assert yq.shape == q.shape and yk.shape == k.shape
