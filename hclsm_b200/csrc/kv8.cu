@@ -14,7 +14,7 @@
 namespace hclsm {
 namespace kv8 {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct Params {
   xattn::View x[2];  // new keys and values (B, n, Hkv, D)
@@ -76,13 +76,26 @@ __device__ __forceinline__ float largest(float m, const float (&v)[8]) {
   }
   return m;
 }
-// 8 values over the scale, to the nearest integer (half to even); zeros where the scale is zero or NaN.
-__device__ __forceinline__ uint2 eight(const float (&v)[8], float s) {
+// 8 values over the scale, to the nearest integer (half to even); zeros where the scale is zero or NaN.  inv is the
+// fp32 reciprocal of the scale: x * inv is within 3e-5 of the quotient, so only a value that lies nearer than 1e-4 to
+// halfway between two integers needs the division itself (as do scales whose reciprocal is not exact enough).
+__device__ __forceinline__ uint2 eight(const float (&v)[8], float s, float inv) {
   uint32_t w[2] = {0, 0};
   if (s > 0.0f) {
+    float q[8];
+    bool near = s < 1e-30f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[e] = v[e] * inv;
+      near |= fabsf(q[e] - rintf(q[e])) > 0.4999f;
+    }
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = __fdiv_rn(v[e], s);
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e)  // |x / scale| can round past 127 where the scale is subnormal
-      w[e >> 2] |= (uint32_t)(min(max(__float2int_rn(__fdiv_rn(v[e], s)), -127), 127) & 0xff) << (8 * (e & 3));
+      w[e >> 2] |= (uint32_t)(min(max(__float2int_rn(q[e]), -127), 127) & 0xff) << (8 * (e & 3));
   }
   return make_uint2(w[0], w[1]);
 }
@@ -92,7 +105,7 @@ __device__ __forceinline__ uint2 eight(const float (&v)[8], float s) {
 // one of a sequence also writes the tail, after it has read it.
 constexpr int kHeld = 8;  // vectors of 8 a lane holds
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Params p) {
   pdl_wait();
   pdl_trigger();
@@ -110,15 +123,15 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
     return;
   }
   if (count == 0) return;
-  const int end = start + count, D = p.D, block = p.block, vecs = block * D / 8;
-  const int blk = start / block + j, lastb = (end - 1) / block;
+  const int end = start + count, block = p.block, vecs = block * D / 8, mask = block - 1;  // block: a power of 2
+  const int log = 31 - __clz(block), blk = (start >> log) + j, lastb = (end - 1) >> log;
   if (blk > lastb) return;
   const xattn::View& xv = p.x[kv];
   const T* x = static_cast<const T*>(xv.p) + b * xv.sb + hk * xv.sh;
   T* tail = static_cast<T*>(p.tail[kv]) + bh * block * D;
   auto at = [&](int i) {  // vector i of the cache block: among the new tokens, or in the tail
     const int tok = blk * block + i * 8 / D, d = i * 8 % D;
-    return tok >= start ? x + (int64_t)(tok - start) * xv.st + d : tail + (tok % block) * D + d;
+    return tok >= start ? x + (int64_t)(tok - start) * xv.st + d : tail + (tok & mask) * D + d;
   };
   if ((blk + 1) * block <= end) {
     float m = 0.0f, v[8];
@@ -146,14 +159,15 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float s = m == INFINITY ? __int_as_float(0x7fc00000) : __fdiv_rn(m, 127.0f);
-    if (lane == 0) p.scale[kv][bh * (p.T / block) + blk] = s;
+    const float inv = 1.0f / s;
+    if (lane == 0) p.scale[kv][bh * (p.T >> log) + blk] = s;
     int8_t* q = p.q[kv] + (bh * p.T + (int64_t)blk * block) * D;
     if (held) {
 #pragma unroll
       for (int k = 0; k < kHeld; ++k)
         if (k * 32 + lane < vecs) {
           r[k].get(v);
-          *reinterpret_cast<uint2*>(q + (k * 32 + lane) * 8) = eight(v, s);
+          *reinterpret_cast<uint2*>(q + (k * 32 + lane) * 8) = eight(v, s, inv);
         }
     } else {
 #pragma unroll 4
@@ -161,19 +175,19 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
         Raw<T> t;
         t.ld(at(i));
         t.get(v);
-        *reinterpret_cast<uint2*>(q + i * 8) = eight(v, s);
+        *reinterpret_cast<uint2*>(q + i * 8) = eight(v, s, inv);
       }
     }
   }
-  if (j == 0 && end % block) {
+  if (j == 0 && (end & mask)) {
     __syncwarp();  // the tail has been read
     const int t0 = max(start, lastb * block);
-    if (lane == 0) p.scale[kv][bh * (p.T / block) + lastb] = -1.0f;  // this block is in the tail
+    if (lane == 0) p.scale[kv][bh * (p.T >> log) + lastb] = -1.0f;  // this block is in the tail
     for (int i = lane; i < (end - t0) * D / 8; i += 32) {
       const int tok = t0 + i * 8 / D, d = i * 8 % D;
       Raw<T> t;
       t.ld(x + (int64_t)(tok - start) * xv.st + d);
-      t.st(tail + (tok % block) * D + d);
+      t.st(tail + (tok & mask) * D + d);
     }
   }
 }
@@ -215,6 +229,16 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ 
 size_t attn_workspace(const hclsm_kv8_cache* c, int Lq, int H);
 int attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens, int Lq, int H, float scale,
          void* ws, cudaStream_t st);
+
+template <typename T>
+int launch_write(const Params& p, dim3 g, cudaStream_t st) {
+  switch (p.D) {
+    case 32: return launch_pdl(write_kernel<T, 32>, g, kThreads, 0, st, p);
+    case 64: return launch_pdl(write_kernel<T, 64>, g, kThreads, 0, st, p);
+    case 96: return launch_pdl(write_kernel<T, 96>, g, kThreads, 0, st, p);
+    default: return launch_pdl(write_kernel<T, 128>, g, kThreads, 0, st, p);
+  }
+}
 
 bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -268,8 +292,7 @@ extern "C" int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, co
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 g((unsigned)grid, 2);
-  return c->dtype == HCLSM_F32 ? launch_pdl(kv8::write_kernel<float>, g, kv8::kThreads, 0, st, p)
-                               : launch_pdl(kv8::write_kernel<__nv_bfloat16>, g, kv8::kThreads, 0, st, p);
+  return c->dtype == HCLSM_F32 ? kv8::launch_write<float>(p, g, st) : kv8::launch_write<__nv_bfloat16>(p, g, st);
 }
 
 extern "C" int hclsm_kv8_read(const hclsm_kv8_cache* c, void* k, void* v, const int32_t* lens, void* stream) {
@@ -281,7 +304,7 @@ extern "C" int hclsm_kv8_read(const hclsm_kv8_cache* c, void* k, void* v, const 
   p.out[0] = k, p.out[1] = v, p.count = lens;
   const int64_t total = (int64_t)c->T * c->Hkv * (c->D / 8);  // vectors of a sequence
   if (total > 0x7fffffff || c->B > 65535) return HCLSM_ERR_SHAPE;
-  const int64_t blocks = (total + kv8::kThreads - 1) / kv8::kThreads, most = (int64_t)num_sms() * 32 / c->B + 1;
+  const int64_t blocks = (total + kv8::kThreads - 1) / kv8::kThreads, most = (int64_t)num_sms() * 16 / c->B + 1;
   const dim3 g((unsigned)(blocks < most ? blocks : most), 2, (unsigned)c->B);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return c->dtype == HCLSM_F32 ? launch_pdl(kv8::read_kernel<float>, g, kv8::kThreads, 0, st, p)
