@@ -18,8 +18,8 @@ from .sparse_event_attn import (  # noqa: F401
     sparse_event_attn_fn,
 )
 from .level0 import level0_epilogue, level0_forward, masked_mean_pool  # noqa: F401
-from .qk_norm_rope import qk_norm_rope, rope_tables  # noqa: F401
-from .cross_attention import cross_attention  # noqa: F401
+from .qk_rope import qk_norm_rope, rope_tables  # noqa: F401
+from .cross_attn import cross_attention  # noqa: F401
 from .kv8_cache import Kv8Cache, kv8_attention, kv8_read, kv8_write  # noqa: F401
 
 __all__ = ["sparse_event_attn_fn", "EventTransformer", "sparse_event_attention_fused", "event_detect", "ssm_scan_fn",

@@ -41,10 +41,10 @@ from . import _lib
 from .kernels import kv8_cache as _kv8
 from .kernels import sparse_event_attn as _ev
 from .kernels import ssm_scan_kernel as _scan
-from .kernels.cross_attention import attention_bwd as _xattn_bwd
-from .kernels.cross_attention import attention_fwd as _xattn_fwd
-from .kernels.qk_norm_rope import rope_bwd as _rope_bwd
-from .kernels.qk_norm_rope import rope_fwd as _rope_fwd
+from .kernels.cross_attn import attention_bwd as _xattn_bwd
+from .kernels.cross_attn import attention_fwd as _xattn_fwd
+from .kernels.qk_rope import rope_bwd as _rope_bwd
+from .kernels.qk_rope import rope_fwd as _rope_fwd
 from .kernels.slot_attention_kernel import slot_attention_core as _slot_core
 
 __all__ = ["ssm_scan_fwd", "ssm_scan_bwd", "slot_attn_core", "event_compact", "event_gather", "event_scatter",
