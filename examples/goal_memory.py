@@ -91,7 +91,7 @@ def main(steps=30, B=8, K=24, N=32, G=4, d=384):
             want = model(goals, states[:, :t + 1], at)
         far.append((got.float() - want.float()).norm() / want.float().norm())
     far = float(torch.stack(far).max())
-    print(f"loss {losses[0]:.5f} -> {losses[-1]:.5f}; rollout from the 8-bit cache is {far:.4f} from the full attention")
+    print(f"loss {losses[0]:.5f} -> {losses[-1]:.5f}; rollout from the 8-bit cache: {far:.4f} from full attention")
     return losses, far
 
 

@@ -13,14 +13,17 @@
 // 8-bit integers become fp16 two at a time: 0x6400 | (x + 128) is 1152 + x.  For K
 // the 1152 stays in: S is off by 1152 times the row's sum of q, one subtraction a
 // score.  For V it is taken off (the sum over a long history would lose the
-// difference).  Queries are scaled by a power of two to a largest value below 1, and
-// the weights to at most 2^12, both exact, for fp16's range; with 11 bits they carry
-// less rounding than bf16's 8.  The scale of a block of keys multiplies its scores
-// (K); that of its values, over the largest so far, its weights (V).
+// difference).  For fp16's range queries are scaled by a power of two to a largest value
+// below 1 (exact, but for values 2^-14 of the largest and below, which lose what is below
+// 2^-24 of it) and weights to at most 2^12; fp16's 11 bits round them less than bf16's 8.
+// The scale of a block of keys multiplies its scores (K); that of its values, over the largest so far, its weights (V).
 // fp32 operands are split into three bf16 pieces (8 bits each) and the products
 // of pieces whose order is at most 2 are summed: fp32 accuracy.
 // Bound: HBM (each key and value byte is read once); splits and warps are merged
-// in a fixed order.
+// in a fixed order.  One query over 8 x 16384 ragged bf16 states, 16 heads over 4 of
+// 128: 48 us (floor 31); over 16 x 65536 cached states, 32 heads over 8 of 128: 371 us,
+// 4.3 TB/s, 41 % of the issue slots (conversions and softmax).  Three blocks an SM: four
+// spill (415 us against 380); four waves of blocks: eight are slower (480 against 450).
 #include <cuda_fp16.h>
 
 #include <type_traits>

@@ -17,6 +17,9 @@
 // the heads of ONE token, 32 / lanes-per-head at a time: the token's cos and
 // sin (64 bytes a lane) are read once and stay in registers for all its heads.
 // Queries and keys go in one launch, the first warps the queries'.
+// 64 x 2048 tokens, 32 + 8 heads of 64, bf16: 293 us forward (4.6 TB/s; 69 % of the
+// issue slots), 487 us backward (4.1 TB/s; 24 warps an SM keep too few loads in
+// flight; 16 warps: 561 us).
 #include "common.cuh"
 
 namespace hclsm {
@@ -95,7 +98,8 @@ template <> struct Vec8<float> {
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float2 (&v)[4]) const {
-    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w), v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
+    v[0] = make_float2(a.x, a.y), v[1] = make_float2(a.z, a.w);
+    v[2] = make_float2(b.x, b.y), v[3] = make_float2(b.z, b.w);
   }
   __device__ __forceinline__ Vec8 from(int lane, bool some) const {
     const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -442,7 +446,8 @@ int run(const hclsm_rope_side* q, const hclsm_rope_side* k, const float* cosv, c
   if (grid == 0) return HCLSM_OK;
   p.cosv = cosv, p.sinv = sinv, p.P = P, p.rot = rot, p.D = D, p.eps = eps, p.norm = norm, p.inter = inter;
   p.err = device_err_ptr();
-  const int rc = dtype == HCLSM_F32 ? launch<float>(p, grid, inter, bwd, st) : launch<__nv_bfloat16>(p, grid, inter, bwd, st);
+  const int rc = dtype == HCLSM_F32 ? launch<float>(p, grid, inter, bwd, st)
+                                    : launch<__nv_bfloat16>(p, grid, inter, bwd, st);
   if (rc != HCLSM_OK || (!p.s[0].partial && !p.s[1].partial)) return rc;
   return launch_pdl(dw_kernel, 2, 1024, 0, st, p);
 }

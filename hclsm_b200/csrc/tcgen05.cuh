@@ -97,8 +97,8 @@ __device__ __forceinline__ void umma_ss(uint32_t elect, uint32_t tmem_d, uint64_
       : "memory");
 }
 // A from TMEM (bf16 pairs, lane = row), B from shared memory.
-__device__ __forceinline__ void umma_ts(uint32_t elect, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t elect, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
       " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),

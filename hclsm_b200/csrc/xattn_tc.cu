@@ -12,7 +12,8 @@
 // with the same relative precision, and O is read back and rescaled rarely.
 // The bound is the softmax's issue and its chain with the products: 4 x 2048 queries
 // over 8192 states, 32 heads of 64, 690 us (797 TFLOP/s), 8 x 2048 over 4096, 16 heads
-// of 128, 435 us (1264 TFLOP/s); tensor pipe 28 and 42 % busy (2 x 2048 over 4096).
+// of 128, 435 to 462 us (1190 to 1264 TFLOP/s); tensor pipe 28 and 44 % busy (2 x 2048
+// over 4096).
 // While one tile takes its softmax the tensor cores run the other's products.
 #include "xattn_tc.cuh"
 
@@ -52,7 +53,8 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   unsigned char *sQ = smem, *sK = sQ + QT * Sh::kOp, *sV = sK + ST * Sh::kOp;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::kOp);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST,
-           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT, *s_free = pv_done + QT, *drain = s_free + QT;
+           *s_full = v_empty + ST, *p_full = s_full + QT, *pv_done = p_full + QT, *s_free = pv_done + QT,
+           *drain = s_free + QT;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = QT * 4, kMmaWarp = QT * 4 + 1, kWeighWarp = QT * 4 + 2;
   if (warp == kMmaWarp) {
@@ -63,7 +65,10 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   }
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < Sh::kBars; ++i) mbar_init(&bars[i], (&bars[i] >= p_full && &bars[i] < pv_done) || (&bars[i] >= s_free && &bars[i] < drain) ? 128 : 1);
+    for (uint64_t* bar = bars; bar < bars + Sh::kBars; ++bar) {
+      const bool by_rows = (bar >= p_full && bar < pv_done) || (bar >= s_free && bar < drain);
+      mbar_init(bar, by_rows ? 128 : 1);
+    }
     fence_mbar_init();
   }
   tc_fence_before();

@@ -14,8 +14,13 @@
 // The weights and their gradients are A operands in TMEM; the same staged tile of
 // K (or Q, dO) is the K-major operand of one product and the MN-major operand of
 // another.  Two buffers of 64 + 64 columns with warpgroups of their own: the tensor
-// cores form one buffer's products while the other's weights are computed.  A tile of 64 and not 128: 2 x (128 + 128) columns and the accumulators
-// (128 or 256) do not fit TMEM's 512.
+// cores form one buffer's products while the other's weights are computed.  A tile of
+// 64 and not 128: 2 x (128 + 128) columns and the accumulators (128 or 256) do not fit
+// TMEM's 512.  8 x 2048 queries over 4096 states, 16 heads of 128 over 4: 1525 to
+// 1560 us, of it 46 % for dq (3 products: 1150 TFLOP/s) and 54 % for dk and dv (4: 1300);
+// the tensor pipe is 45 and 56 % busy (2 x 2048 over 4096).  What bounds it is the chain
+// of products, weights and products; and in the second kernel 128 x 64 products with both
+// operands in shared memory, 51 cycles a step of 16 instead of 35.
 #include "xattn_tc.cuh"
 
 namespace hclsm {
@@ -86,7 +91,8 @@ template <int DP, bool OWN> struct Block {
     umma_done(r.one, &sd_full[w]);
   }
   // the same with the own operands in TMEM columns t0 and t1
-  __device__ __forceinline__ void products_ts(const Issue& r, uint32_t tmem, uint32_t t0, uint32_t t1, int w, int s) const {
+  __device__ __forceinline__ void products_ts(const Issue& r, uint32_t tmem, uint32_t t0, uint32_t t1, int w,
+                                              int s) const {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const uint64_t b = desc_at(half ? r.b1 : r.b0, s * Sh::kOpB);
@@ -98,14 +104,16 @@ template <int DP, bool OWN> struct Block {
     }
     umma_done(r.one, &sd_full[w]);
   }
-  // acc += (bf16 columns at a, the second 32 rows' STEP further) x (streamed tile in stage s, MN-major descriptor t) (a converged warp)
+  // acc += (bf16 columns at a, the second 32 rows' STEP further) x (streamed tile in stage s, MN-major descriptor t)
+  // (a converged warp)
   template <int STEP>
   __device__ __forceinline__ void accumulate(const Issue& r, uint32_t acc, uint32_t a, uint64_t t, int s,
                                              bool first) const {
     const uint64_t b = desc_at(t, s * Sh::kOpB);
 #pragma unroll
     for (int k = 0; k < kB / 16; ++k)
-      umma_ts(r.one, acc, a + (k & 1) * 8 + (k >> 1) * STEP, desc_at(b, k * 16 * kRowBytes), r.id_o, !(first && k == 0));
+      umma_ts(r.one, acc, a + (k & 1) * 8 + (k >> 1) * STEP, desc_at(b, k * 16 * kRowBytes), r.id_o,
+              !(first && k == 0));
   }
 };
 
@@ -240,7 +248,9 @@ __global__ void __launch_bounds__(BwdShape<DP>::kDqThreads, 1)
           if (w && x.lo && row < x.Lq && d < x.D)
             lo = *reinterpret_cast<const uint4*>(x.lo + (o - static_cast<const __nv_bfloat16*>(x.o)) + d);
           const uint32_t ow[4] = {u.x, u.y, u.z, u.w}, lw[4] = {lo.x, lo.y, lo.z, lo.w};
-          auto both = [](uint32_t t) { return make_float2(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u)); };
+          auto both = [](uint32_t t) {
+            return make_float2(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
+          };
 #pragma unroll
           for (int e = 0; e < 4; ++e) dot = fma2(both(r[4 * i + e]), add2(both(ow[e]), both(lw[e])), dot);
         }

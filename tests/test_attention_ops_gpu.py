@@ -5,7 +5,8 @@ wrong, and their refusals.
 Errors are 2-norms relative to the result's.  Tolerances: bf16 rounds to nearest
 with unit roundoff u = 2^-8.  A norm's output is rounded once (u).  An attention
 output sees the weights' rounding and its own (2 u); its gradients three at most:
-the weights' (or their gradients'), their own, and the output's where it enters do . o.  fp32 results carry sums of at most
+the weights' (or their gradients'), their own, and the output's where it enters do . o.  fp32 results carry
+sums of at most
 a few thousand terms at 2^-24 each and hardware exp2 (2 ulp): 1e-5.
 """
 import math

@@ -44,11 +44,13 @@ def test_c_entries_refuse_without_a_gpu():
         a = dict(q=(16, 0, 0, 0), k=(16, 0, 0, 0), v=(16, 0, 0, 0), do=(0, 0, 0, 0), o=16, B=1, Lq=1, Lk=1, H=1, Hkv=1,
                  D=64, dtype=0, scale=1.0, lo=0)
         a.update(kw)
-        return _lib.XATTN_ARGS.pack(*a["q"], *a["k"], *a["v"], *a["do"], a["o"], 0, 0, 0, 0, a["lo"], 0, 0, 0, a["B"], a["Lq"],
+        return _lib.XATTN_ARGS.pack(*a["q"], *a["k"], *a["v"], *a["do"], a["o"], 0, 0, 0, 0, a["lo"], 0, 0, 0, a["B"],
+                                    a["Lq"],
                                     a["Lk"], a["H"], a["Hkv"], a["D"], a["dtype"], a["scale"])
 
     for want, kw in ((2, dict(dtype=7)), (1, dict(D=129)), (1, dict(D=0)), (1, dict(H=3, Hkv=2)), (1, dict(B=-1)),
-                     (1, dict(scale=0.0)), (1, dict(scale=float("nan"))), (3, dict(lo=8)), (8, dict(o=0)), (8, dict(k=(0, 0, 0, 0)))):
+                     (1, dict(scale=0.0)), (1, dict(scale=float("nan"))), (3, dict(lo=8)), (8, dict(o=0)),
+                     (8, dict(k=(0, 0, 0, 0)))):
         assert lib.hclsm_xattn_fwd(xattn(**kw), None, 0, None) == want, kw
     assert lib.hclsm_xattn_fwd(xattn(B=0), None, 0, None) == 0
     assert lib.hclsm_xattn_bwd(xattn(), None, 0, None) == 8
@@ -114,7 +116,7 @@ def test_training_step_captures_as_a_graph():
 
     torch.manual_seed(1)
     model = _example().GoalMemory(256, heads=4, kv_heads=2)
-    goals, states = torch.randn(2, 3, 256, device="cuda").bfloat16(), torch.randn(2, 6, 8, 256, device="cuda").bfloat16()
+    goals, states = (torch.randn(*s, device="cuda").bfloat16() for s in ((2, 3, 256), (2, 6, 8, 256)))
     counts = torch.tensor([6, 3], device="cuda", dtype=torch.int32)
     alive = torch.rand(2, 8, device="cuda") > 0.2
 
