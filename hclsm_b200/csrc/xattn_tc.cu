@@ -63,11 +63,20 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  const int q0 = (int)(blockIdx.x % p.qtiles) * (QT * kTile);
   if (tid == 0) {
     s_abort = 0;
+    // Warps without a row take no part in the tiles' phases: with the weights apart from the scores, one that only
+    // arrived could be a whole tile ahead of a warp still at its last weights and end that warp's phase for it.
+    auto rows = [&](int w) {  // threads of query tile w's warps that have a row (a count is at least 1)
+      const int n = p.x.Lq - q0 - w * kTile;
+      return n >= kTile ? kTile : n > 0 ? (n + 31) / 32 * 32 : 1;
+    };
     for (uint64_t* bar = bars; bar < bars + Sh::kBars; ++bar) {
-      const bool by_rows = (bar >= p_full && bar < pv_done) || (bar >= s_free && bar < drain);
-      mbar_init(bar, by_rows ? 128 : 1);
+      const int w = bar >= p_full && bar < pv_done ? (int)(bar - p_full)
+                    : bar >= s_free && bar < drain ? (int)(bar - s_free)
+                                                   : -1;
+      mbar_init(bar, w >= 0 ? rows(w) : 1);
     }
     fence_mbar_init();
   }
@@ -79,7 +88,6 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   // tile w: scores in columns [w * 128, + 128), weights in [kColP + w * kStepP, + 64), O in [kColO + w * DP, + DP)
   const uint32_t tmem = s_tmem;
   const Params& x = p.x;
-  const int q0 = (int)(blockIdx.x % p.qtiles) * (QT * kTile);
   const int h = (int)(blockIdx.x / p.qtiles % x.H), hk = h / (x.H / x.Hkv);
   const int64_t b = blockIdx.x / p.qtiles / x.H;
   const int nk = key_count(x, b), tiles = (nk + kTile - 1) / kTile;
@@ -195,23 +203,18 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
   } else {
     const int w = warp >> 2;
     const int row = q0 + w * kTile + (tid & 127);
-    const bool idle = q0 + w * kTile + (warp & 3) * 32 >= x.Lq;  // no row of this warp: it only keeps the phases
+    const bool idle = q0 + w * kTile + (warp & 3) * 32 >= x.Lq;  // no row of this warp
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + w * 128, tP = tmem + lanes + Sh::kColP + w * Sh::kStepP,
                    tO = tmem + lanes + Sh::kColO + w * DP;
     const float c2 = x.scale * kLog2e;
     float m = -INFINITY;  // the maximum O is scaled by, raw scores
     float2 l = make_float2(0.0f, 0.0f);
-    bool ok = w < nq;
+    bool ok = !idle;
     for (int j = 0; j < tiles && ok; ++j) {
       const uint4 bits = key_bits(p, b, nk, j * kTile);
       if (!(ok = wait_all(&s_full[w], j))) break;
       tc_fence_after();
-      if (idle) {
-        if constexpr (Sh::kApart) mbar_arrive(&s_free[w]);
-        mbar_arrive(&p_full[w]);
-        continue;
-      }
       if (!all_bits(bits)) {  // -inf over the scores that do not count; the rest of the code has no mask
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(FwdShape<DP, QT>::kThreads, QT == 1 ? 2 : 1)
     }
     if (ok && tiles > 0) ok = wait_all(&pv_done[w], tiles - 1);
     tc_fence_after();
-    if (w < nq && !idle) {
+    if (!idle) {
       const float sum = l.x + l.y;
       const float inv = tiles > 0 && sum != 0.0f ? 1.0f / sum : 0.0f;
       if (row < x.Lq && x.lse2) x.lse2[(b * x.H + h) * x.Lq + row] = sum == 0.0f ? INFINITY : m * c2 + log2f(sum);
