@@ -33,9 +33,31 @@ class Kv8Cache:
     v_scale: Tensor
     k_tail: Tensor
     v_tail: Tensor
-    _c: bytes = field(init=False, repr=False, compare=False, default=b"")  # hclsm_kv8_cache
+    # (addresses, hclsm_kv8_cache, (B, Hkv, T, D)) of the tensors as last checked, or None
+    _packed: tuple | None = field(init=False, repr=False, compare=False, default=None)
 
     def __post_init__(self):
+        self._args()
+
+    def __setattr__(self, name, value):
+        self.__dict__[name] = value
+        if name != "_packed":  # another tensor: checked and packed at the next call
+            self.__dict__["_packed"] = None
+
+    def __getstate__(self):
+        return {**self.__dict__, "_packed": None}  # a copy's tensors are elsewhere
+
+    def _args(self):
+        """(hclsm_kv8_cache, (B, Hkv, T, D)) for a call.  A tensor that was assigned, copied or given other memory since
+        the last call is checked and its address taken anew: a kernel only ever sees the memory of the present tensors."""
+        at = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+              self.k_tail.data_ptr(), self.v_tail.data_ptr())
+        packed = self._packed
+        if packed is None or packed[0] != at:
+            packed = self._packed = (at, *self._check(at))
+        return packed[1:]
+
+    def _check(self, at):
         _lib.require_cuda(self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
         if self.k.dim() != 4 or self.k_tail.dim() != 4:
             raise ValueError("k must be (B, Hkv, T, D), k_tail (B, Hkv, block, D)")
@@ -52,9 +74,7 @@ class Kv8Cache:
                                    ("v_tail", self.v_tail, (B, Hkv, block, D), dtype)):
             if t.shape != shape or t.dtype != dt or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous {shape} {dt}, got {tuple(t.shape)} {t.dtype}")
-        self._c = _lib.KV8_CACHE.pack(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(),
-                                      self.v_scale.data_ptr(), self.k_tail.data_ptr(), self.v_tail.data_ptr(), B, Hkv,
-                                      T, D, block, _lib.dtype_code(dtype))
+        return _lib.KV8_CACHE.pack(*at, B, Hkv, T, D, block, _lib.dtype_code(dtype)), (B, Hkv, T, D)
 
     @classmethod
     def empty(cls, batch: int, capacity: int, kv_heads: int, head_dim: int, *, block: int = 32, dtype=torch.bfloat16,
@@ -85,7 +105,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
     multiple of the block: what was behind it is gone).  A request that does not
     fit the capacity writes nothing and sets the device error word."""
     dev = _lib.require_cuda(cache.k, k, v, start, count)
-    B, Hkv, _, D = cache.k.shape
+    c, (B, Hkv, _, D) = cache._args()
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != B or k.shape[2:] != (Hkv, D):
         raise ValueError(f"k and v must be ({B}, tokens, {Hkv}, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
@@ -95,7 +115,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
         raise ValueError("start is required")
     count = _lib.index32(count, (B,), "count", dev)
     k, v = _lib.rows16(k), _lib.rows16(v)
-    _lib.check(_lib.load().hclsm_kv8_write(cache._c, _lib.VIEW.pack(*_lib.view_args(k)),
+    _lib.check(_lib.load().hclsm_kv8_write(c, _lib.VIEW.pack(*_lib.view_args(k)),
                                            _lib.VIEW.pack(*_lib.view_args(v)), k.shape[1], start.data_ptr(),
                                            _lib.ptr(count), _lib.stream_ptr(dev)), "hclsm_kv8_write")
 
@@ -104,10 +124,10 @@ def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
     """(k, v), each (B, T, Hkv, D) in the cache's dtype: the first ``lens[b]``
     tokens written (default all) as the values they stand for, zeros after them."""
     dev = _lib.require_cuda(cache.k, lens)
-    B, Hkv, T, D = cache.k.shape
+    c, (B, Hkv, T, D) = cache._args()
     lens = _lib.index32(lens, (B,), "lens", dev)
     k, v = (torch.empty(B, T, Hkv, D, dtype=cache.dtype, device=dev) for _ in range(2))
-    _lib.check(_lib.load().hclsm_kv8_read(cache._c, k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
+    _lib.check(_lib.load().hclsm_kv8_read(c, k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
                                           _lib.stream_ptr(dev)), "hclsm_kv8_read")
     return k, v
 
@@ -117,7 +137,7 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
     first ``lens[b]`` tokens written (default all of the capacity; clamped to [0, T]); H
     is a multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
     dev = _lib.require_cuda(q, cache.k, lens)
-    B, Hkv, T, D = cache.k.shape
+    c, (B, Hkv, _, D) = cache._args()
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
         raise ValueError(f"q must be ({B}, tokens, heads, {D}), got {tuple(q.shape)}")
     Lq, H = q.shape[1], q.shape[2]
@@ -134,10 +154,10 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
     q = _lib.dense_last(q)
     o = q.new_empty(q.shape)
     lib, ws = _lib.load(), None
-    n = lib.hclsm_kv8_attn_workspace_size(cache._c, Lq, H)
+    n = lib.hclsm_kv8_attn_workspace_size(c, Lq, H)
     if n:
         ws = q.new_empty(n, dtype=torch.uint8)
-    _lib.check(lib.hclsm_kv8_attn(cache._c, _lib.VIEW.pack(*_lib.view_args(q)), o.data_ptr(), _lib.ptr(lens), Lq, H,
+    _lib.check(lib.hclsm_kv8_attn(c, _lib.VIEW.pack(*_lib.view_args(q)), o.data_ptr(), _lib.ptr(lens), Lq, H,
                                   scale, None if ws is None else ws.data_ptr(), n, _lib.stream_ptr(dev)),
                "hclsm_kv8_attn")
     return o

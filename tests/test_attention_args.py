@@ -1,0 +1,106 @@
+"""What the attention operators hand to the library, and what they refuse, seen on the CPU: the device check is stubbed
+and the library replaced by one that records its arguments."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+from hclsm_b200 import _lib
+from hclsm_b200.kernels import Kv8Cache, kv8_attention, kv8_read, kv8_write
+
+
+class _Library:
+    """Records each call's arguments; workspace queries give 0."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    rec = _Library()
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda dev: 0)
+    return rec
+
+
+NAMES = ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")
+
+
+def _cache(**kw):
+    return Kv8Cache.empty(2, 64, 1, 32, device="cpu", **kw)
+
+
+def _addresses(cache):
+    return [getattr(cache, n).data_ptr() for n in NAMES]
+
+
+def _uses_its_own(lib, cache):
+    """Every call on the cache gets the addresses of the tensors that it has now."""
+    B, Hkv, T, D = cache.k.shape
+    x = torch.zeros(B, 3, Hkv, D, dtype=cache.dtype)
+    at = torch.zeros(B, dtype=torch.int32)
+    lib.calls.clear()
+    kv8_write(cache, x, x, at)
+    kv8_read(cache, at)
+    o = kv8_attention(x, cache, at)
+    assert o.shape[0] == B
+    seen = {n: _lib.KV8_CACHE.unpack(a[0]) for n, a in lib.calls}
+    assert {"hclsm_kv8_write", "hclsm_kv8_read", "hclsm_kv8_attn"} <= set(seen)
+    for n, c in seen.items():
+        assert list(c[:6]) == _addresses(cache), n
+        assert c[6:] == (B, Hkv, T, D, cache.block, _lib.BF16), n
+
+
+def test_cache_copies_use_their_own_memory(lib):
+    cache = _cache()
+    _uses_its_own(lib, cache)
+    file = io.BytesIO()
+    torch.save(cache, file)
+    file.seek(0)
+    copies = [copy.deepcopy(cache), pickle.loads(pickle.dumps(cache)), torch.load(file, weights_only=False)]
+    for c in copies:
+        assert not set(_addresses(c)) & set(_addresses(cache))
+        _uses_its_own(lib, c)
+    shallow = copy.copy(cache)  # the same tensors
+    assert _addresses(shallow) == _addresses(cache)
+    _uses_its_own(lib, shallow)
+    shallow.k = shallow.k.clone()
+    _uses_its_own(lib, shallow)
+    _uses_its_own(lib, cache)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_cache_tensors_that_are_assigned_or_moved(lib, name):
+    cache = _cache()
+    setattr(cache, name, getattr(cache, name).clone())
+    _uses_its_own(lib, cache)
+    t = getattr(cache, name)
+    t.data = t.data.clone()  # the same tensor object over other memory
+    _uses_its_own(lib, cache)
+    t.set_(t.clone())
+    _uses_its_own(lib, cache)
+
+
+def test_cache_tensors_that_no_longer_fit_are_refused(lib):
+    x, at = torch.zeros(2, 3, 1, 32, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    for name, bad in (("v", lambda t: t[:, :, :32]), ("k", lambda t: t[:1]), ("k_scale", lambda t: t.double()),
+                      ("v_tail", lambda t: t.float()), ("k_tail", lambda t: t.transpose(0, 1))):
+        cache = _cache()
+        setattr(cache, name, bad(getattr(cache, name)))
+        lib.calls.clear()
+        for call in (lambda: kv8_write(cache, x, x, at), lambda: kv8_read(cache, at),
+                     lambda: kv8_attention(x, cache, at)):
+            with pytest.raises(ValueError):
+                call()
+        assert not lib.calls
