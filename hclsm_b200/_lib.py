@@ -173,10 +173,13 @@ def dense_last(t):
 
 def rows16(t):
     """The (B, L, H, D) tensor itself if its last dim is dense and every row starts on 16
-    bytes, else an aligned contiguous copy."""
+    bytes, else an aligned contiguous copy.  The stride of a dim of one says nothing (the
+    kernels do not use it): torch keeps any there, through contiguous() and clone() too."""
     sb, st, sh, sd = t.stride()
-    if sd == 1 and t.data_ptr() % 16 == 0 and (sb | st | sh) * t.element_size() % 16 == 0:
-        return t
+    if sd == 1 and t.data_ptr() % 16 == 0:
+        e = t.element_size()
+        if (sb | st | sh) * e % 16 == 0 or all(n == 1 or s * e % 16 == 0 for n, s in zip(t.shape[:3], (sb, st, sh))):
+            return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
 

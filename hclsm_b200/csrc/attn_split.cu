@@ -684,7 +684,7 @@ size_t attn_workspace(const hclsm_kv8_cache* c, int Lq, int H) {
 int attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens, int Lq, int H, float scale,
          void* ws, cudaStream_t st) {
   split::Params p = {};
-  p.x.q = xattn::View{q->p, q->sb, q->st, q->sh};
+  p.x.q = xattn::view(*q, c->B, Lq, H);
   p.x.o = o, p.x.lens = lens, p.x.scale = scale;
   p.x.B = c->B, p.x.Lq = Lq, p.x.H = H, p.x.Hkv = c->Hkv, p.x.D = c->D;
   p.k8 = c->k, p.v8 = c->v, p.ks = c->k_scale, p.vs = c->v_scale, p.kt = c->k_tail, p.vt = c->v_tail;

@@ -257,9 +257,9 @@ int check(const hclsm_kv8_cache* c) {
   return HCLSM_OK;
 }
 
-bool row16(const hclsm_view* v, int dtype) {
+bool row16(const xattn::View& v, int dtype) {
   const int e = dtype == HCLSM_F32 ? 4 : 2;
-  return al16(v->p) && v->sb * e % 16 == 0 && v->st * e % 16 == 0 && v->sh * e % 16 == 0;
+  return al16(v.p) && v.sb * e % 16 == 0 && v.st * e % 16 == 0 && v.sh * e % 16 == 0;
 }
 
 Params params(const hclsm_kv8_cache* c) {
@@ -284,10 +284,9 @@ extern "C" int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, co
   if ((int64_t)c->B * n == 0) return HCLSM_OK;
   if (!k || !v || !k->p || !v->p || !start) return HCLSM_ERR_NULL;
   if (c->T == 0) return HCLSM_ERR_SHAPE;
-  if (!kv8::row16(k, c->dtype) || !kv8::row16(v, c->dtype)) return HCLSM_ERR_ALIGN;
   kv8::Params p = kv8::params(c);
-  p.x[0] = xattn::View{k->p, k->sb, k->st, k->sh};
-  p.x[1] = xattn::View{v->p, v->sb, v->st, v->sh};
+  p.x[0] = xattn::view(*k, c->B, n, c->Hkv), p.x[1] = xattn::view(*v, c->B, n, c->Hkv);
+  if (!kv8::row16(p.x[0], c->dtype) || !kv8::row16(p.x[1], c->dtype)) return HCLSM_ERR_ALIGN;
   p.n = n, p.start = start, p.count = count;
   p.touched = (int)(((int64_t)n + c->block - 2) / c->block + 1);
   const int64_t grid = ((int64_t)c->B * c->Hkv * p.touched + kv8::kThreads / 32 - 1) / (kv8::kThreads / 32);

@@ -532,8 +532,8 @@ int check(const hclsm_xattn_args* a) {
 
 Params params(const hclsm_xattn_args* a) {
   Params p = {};
-  auto view = [](const hclsm_view& v) { return View{v.p, v.sb, v.st, v.sh}; };
-  p.q = view(a->q), p.k = view(a->k), p.v = view(a->v), p.dout = view(a->dout);
+  p.q = view(a->q, a->B, a->Lq, a->H), p.dout = view(a->dout, a->B, a->Lq, a->H);
+  p.k = view(a->k, a->B, a->Lk, a->Hkv), p.v = view(a->v, a->B, a->Lk, a->Hkv);
   p.o = a->o, p.dq = a->dq, p.dk = a->dk, p.dv = a->dv;
   p.lse2 = a->lse2;
   p.lo = a->dtype == HCLSM_BF16 ? static_cast<__nv_bfloat16*>(a->lo) : nullptr;

@@ -26,6 +26,10 @@ struct View {
   const void* p;
   int64_t sb, st, sh;  // elements
 };
+// A caller's (B, L, H, D) tensor; a dim of one is never stepped over, whatever its stride.
+inline View view(const hclsm_view& v, int B, int L, int H) {
+  return View{v.p, B > 1 ? v.sb : 0, L > 1 ? v.st : 0, H > 1 ? v.sh : 0};
+}
 
 struct Params {
   View q, k, v, dout;          // (B, L, H, D), innermost dense

@@ -66,9 +66,11 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
 
 def _side(x, y, w, pos, dy=None, dw=None):
     sb, st, sh, _ = x.stride()
+    B, L, H, _ = x.shape  # the library wants strides of whole 16 bytes; one of a dim of one is not used
+    sb, st, sh = sb if B > 1 else 0, st if L > 1 else 0, sh if H > 1 else 0
     return _lib.ROPE_SIDE.pack(x.data_ptr(), 0 if dy is None else dy.data_ptr(), y.data_ptr(),
                                0 if w is None else w.data_ptr(), 0 if pos is None else pos.data_ptr(),
-                               0 if dw is None else dw.data_ptr(), sb, st, sh, x.shape[1], x.shape[2])
+                               0 if dw is None else dw.data_ptr(), sb, st, sh, L, H)
 
 
 def _tables(q, cos, sin, eps, interleaved):

@@ -348,7 +348,8 @@ int hclsm_ssm_scan_bwd_noalloc(const void* x, const void* dt, const float* A_log
  * the cross attention of its goal transformer as a torch module
  * (hclsm/dynamics/level2_goal.py:88-141) and no counterpart of the others.
  *
- * hclsm_view: a (B, L, H, D) tensor, D dense, the other strides in elements.
+ * hclsm_view: a (B, L, H, D) tensor, D dense, the other strides in elements (that
+ * of a dim of one is not used).
  * ------------------------------------------------------------------------- */
 typedef struct {
   const void* p;
@@ -423,7 +424,7 @@ typedef struct {
 
 /* Tokens [0, count[b]) of k, v (B, n, Hkv, D; NULL count: n) become tokens
  * start[b], start[b] + 1, ... of the cache; start[b] is the number of tokens there,
- * or a multiple of block.  A request that does not fit (start
+ * or a multiple of block.  Rows of k and v start on 16 bytes.  A request that does not fit (start
  * < 0, count outside [0, n], start + count > T) writes nothing and puts
  * HCLSM_ERR_SHAPE in the error word. */
 int hclsm_kv8_write(const hclsm_kv8_cache* c, const hclsm_view* k, const hclsm_view* v, int32_t n,

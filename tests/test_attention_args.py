@@ -104,3 +104,19 @@ def test_cache_tensors_that_no_longer_fit_are_refused(lib):
             with pytest.raises(ValueError):
                 call()
         assert not lib.calls
+
+
+def test_rows_of_16_bytes_ignore_dims_of_one():
+    """Only a dim that is stepped over needs a stride of whole 16 bytes; what is returned always satisfies that."""
+    big = torch.zeros(3, 8, 4 * 64 + 4, dtype=torch.bfloat16)
+    token = big[:1, :1, :256].unflatten(-1, (4, 64))        # strides (2080, 260, 64, 1)
+    head = torch.zeros(2, 5, 1, 68, dtype=torch.bfloat16)[..., :64]
+    for t, same in ((token, True), (big[:, :, :256].unflatten(-1, (4, 64)), False), (token[..., 1:33], False),
+                    (head, False), (head[:1, :1], True),
+                    (big.as_strided((1, 3, 4, 64), (2083, 264, 64, 1)), True), (torch.zeros(2, 3, 4, 64), True),
+                    (torch.zeros(64 * 12 + 1)[1:].view(1, 3, 4, 64), False),
+                    (torch.zeros(2, 3, 64, 4).transpose(2, 3), False)):
+        r = _lib.rows16(t)
+        assert torch.equal(r, t) and (r is t) == same
+        assert r.stride(3) == 1 and r.data_ptr() % 16 == 0
+        assert all(n == 1 or s * r.element_size() % 16 == 0 for n, s in zip(r.shape[:3], r.stride()))

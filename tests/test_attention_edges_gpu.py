@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import hclsm_b200
-from hclsm_b200.kernels import cross_attention
-from test_attention_ops_gpu import BF16, U, _allowed, _attn_ref, _err, _gen, _randn
+from hclsm_b200.kernels import Kv8Cache, cross_attention, kv8_read, kv8_write, qk_norm_rope
+from test_attention_ops_gpu import BF16, F32, U, _allowed, _attn_ref, _err, _gen, _i32, _randn, _rope_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,42 @@ def test_long_sweeps_with_part_filled_query_tiles(D, Lq, Lk, masked):
         runs = [cross_attention(qq, kk, vv, kv_lens=lens, key_mask=mask) for _ in range(3)]
         assert _err(runs[0], _attn_ref(qq, kk, vv, ok)) < 2 * U
         assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+
+
+def _single(g, dtype, L, odd):
+    """(1, L, 4, 64) whose strides of size-1 dims are no multiple of 16 bytes: one entry of a padded buffer (odd batch
+    stride), or for L = 1 the first token of a padded projection (odd batch and token strides)."""
+    if L == 1:
+        return _randn(g, 1, 8, 4 * 64 + odd, dtype=dtype)[..., :256].unflatten(-1, (4, 64))[:, :1]
+    flat = _randn(g, 3 * (L * 256 + odd), dtype=dtype)
+    return flat.as_strided((1, L, 4, 64), (L * 256 + odd, 256, 64, 1), 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("L", [1, 70])
+@pytest.mark.parametrize("odd", [1, 4])
+def test_strides_of_dims_of_one_do_not_count(dtype, L, odd):
+    """A dim of one is never stepped over, so its stride is no reason to refuse, copy or take a slower form: results are
+    those of dense tensors to the bit."""
+    g = _gen(L + odd)
+    x, y = _single(g, dtype, L, odd), _single(g, dtype, L, odd)
+    dense = [t.new_empty(t.shape).copy_(t) for t in (x, y)]
+    runs = []
+    for q, k in ((x, y), dense):
+        q, k = (t.detach().requires_grad_() for t in (q, k))
+        out = qk_norm_rope(q, k)
+        runs.append([*out, *torch.autograd.grad(out, (q, k), dense)])
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
+    assert _err(runs[0][0], _rope_ref(x, None, None, None, None, 1e-6, False)) < (U if dtype == BF16 else 1e-5)
+    caches = [Kv8Cache.empty(1, 96, 4, 64, dtype=dtype) for _ in range(2)]
+    for c, (k, v) in zip(caches, ((x, y), dense)):
+        kv8_write(c, k, v, _i32(0))
+    for a, b in zip(*(kv8_read(c, _i32(L)) for c in caches)):
+        assert torch.equal(a, b)
+    # one query over 2000 keys of one batch entry: the form that splits the keys
+    k, v = _single(g, dtype, 2000, odd), _single(g, dtype, 2000, odd)
+    for Lq in (1, 150):
+        q = _randn(g, 1, Lq, 4, 64, dtype=dtype)
+        kd, vd = (t.new_empty(t.shape).copy_(t) for t in (k, v))
+        assert torch.equal(cross_attention(q, k, v), cross_attention(q, kd, vd))
