@@ -205,6 +205,17 @@ def index32(t, shape, name, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def like(t, shape, dtype, name, device):
+    """t, which a kernel takes to be a tensor of that shape, dtype and device; dense."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def no_double_backward():
     """A backward made of this library's kernels has no graph of its own."""
     if torch.is_grad_enabled():

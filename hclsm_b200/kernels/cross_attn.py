@@ -111,6 +111,12 @@ def attention_fwd(q, k, v, kv_lens, key_mask, scale):
 def attention_bwd(q, k, v, o, lse, lo, do, kv_lens, key_mask, scale):
     """(dq, dk, dv) from attention_fwd's results."""
     q, k, v, lens, key_mask, scale = _prepare(q, k, v, kv_lens, key_mask, scale)
+    o, do = (_lib.like(t, q.shape, q.dtype, n, q.device) for t, n in ((o, "o"), (do, "do")))
+    lse = _lib.like(lse, (q.shape[0], q.shape[2], q.shape[1]), torch.float32, "lse", q.device)
+    if lo is not None:
+        if q.dtype != torch.bfloat16:
+            raise TypeError("lo goes with bfloat16")
+        lo = _lib.like(lo, q.shape, q.dtype, "lo", q.device)
     return _backward(q, k, v, o, lse, lo, lens, key_mask, scale, do)
 
 

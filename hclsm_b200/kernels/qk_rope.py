@@ -173,6 +173,9 @@ def rope_fwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved)
 def rope_bwd(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk):
     """(dq, dk, dq_weight, dk_weight), None for weights that are not there."""
     args = list(_prepare(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved))
+    gq = _lib.like(gq, q.shape, q.dtype, "gq", q.device)
+    if k is not None:
+        gk = _lib.like(gk, k.shape, k.dtype, "gk", k.device)
     args[:2] = [None if t is None else _lib.rows16(t) for t in args[:2]]
     return _backward(*args, gq, gk, True, True)
 

@@ -7,8 +7,10 @@ import pickle
 import pytest
 import torch
 
+import hclsm_b200.torch_ops  # noqa: F401  (registers the ops)
 from hclsm_b200 import _lib
 from hclsm_b200.kernels import Kv8Cache, kv8_attention, kv8_read, kv8_write
+from hclsm_b200.kernels.cross_attn import attention_bwd
 
 
 class _Library:
@@ -120,3 +122,42 @@ def test_rows_of_16_bytes_ignore_dims_of_one():
         assert torch.equal(r, t) and (r is t) == same
         assert r.stride(3) == 1 and r.data_ptr() % 16 == 0
         assert all(n == 1 or s * r.element_size() % 16 == 0 for n, s in zip(r.shape[:3], r.stride()))
+
+
+def test_backward_operators_refuse_tensors_that_do_not_belong(lib):
+    """The kernels read o, lse, lo and the gradients at the sizes of q and k: another size, type or device is refused."""
+    ops = torch.ops.hclsm_b200
+    bf, f32 = torch.bfloat16, torch.float32
+    q, k = torch.zeros(2, 5, 4, 64, dtype=bf), torch.zeros(2, 9, 2, 64, dtype=bf)
+    good = dict(o=torch.zeros_like(q), lse=torch.zeros(2, 4, 5), lo=torch.zeros_like(q), do=torch.zeros_like(q))
+
+    def xattn(q=q, k=k, **kw):
+        a = {**good, **kw}
+        return ops.cross_attention_bwd(q, k, k, a["o"], a["lse"], a["lo"], a["do"], None, None, 0.125)
+
+    for name, bad, exc in (("o", q[:, :4], ValueError), ("o", q.float(), TypeError), ("do", q[:1], ValueError),
+                           ("do", q.float(), TypeError), ("do", q[..., :32], ValueError),
+                           ("lse", torch.zeros(2, 5, 4), ValueError), ("lse", torch.zeros(2, 4, 5, dtype=bf), TypeError),
+                           ("lo", q[:, :1], ValueError), ("lo", torch.zeros(2, 5, 4, 64), TypeError)):
+        with pytest.raises(exc):
+            xattn(**{name: bad})
+    with pytest.raises(ValueError):
+        attention_bwd(q, k, k, good["o"].to("meta"), good["lse"], good["lo"], good["do"], None, None, 0.125)
+    f = {n: t.float() for n, t in good.items()}
+    with pytest.raises(TypeError):
+        xattn(q.float(), k.float(), **{**f, "lo": good["lo"]})
+
+    def rope(gq=q, gk=k):
+        return ops.qk_norm_rope_bwd(q, k, None, None, None, None, None, None, 1e-6, False, gq, gk)
+
+    for kw, exc in ((dict(gq=q[:, :4]), ValueError), (dict(gq=q.float()), TypeError), (dict(gk=q), ValueError),
+                    (dict(gk=k.to(torch.float16)), TypeError)):
+        with pytest.raises(exc):
+            rope(**kw)
+    assert not lib.calls
+    # what belongs goes through, an o that is not dense as a dense copy
+    xattn(), rope()
+    xattn(o=torch.zeros(2, 4, 5, 64, dtype=bf).transpose(1, 2))
+    assert [n for n, _ in lib.calls if n.endswith("bwd")] == ["hclsm_xattn_bwd", "hclsm_qk_norm_rope_bwd",
+                                                              "hclsm_xattn_bwd"]
+    xattn(q.float(), k.float(), **{**f, "lo": torch.empty(0)})
