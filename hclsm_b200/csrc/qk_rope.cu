@@ -366,7 +366,8 @@ int check(const hclsm_rope_side* s, int64_t B, int P, int rot, bool bwd) {
   if (s->L < 0 || s->H < 1) return HCLSM_ERR_SHAPE;
   if (B * s->L == 0) return HCLSM_OK;
   if (!s->x || !s->y || (bwd && !s->dy)) return HCLSM_ERR_NULL;
-  if (rot > 0 && !s->pos && s->L > P) return HCLSM_ERR_SHAPE;
+  // an empty table has no row 0 either, which a position outside the table reads in its place
+  if (rot > 0 && (P < 1 || (!s->pos && s->L > P))) return HCLSM_ERR_SHAPE;
   if (!aligned(s->x) || !aligned(s->y) || (bwd && !aligned(s->dy))) return HCLSM_ERR_ALIGN;
   return HCLSM_OK;
 }

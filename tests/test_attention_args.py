@@ -161,3 +161,13 @@ def test_backward_operators_refuse_tensors_that_do_not_belong(lib):
     assert [n for n, _ in lib.calls if n.endswith("bwd")] == ["hclsm_xattn_bwd", "hclsm_qk_norm_rope_bwd",
                                                               "hclsm_xattn_bwd"]
     xattn(q.float(), k.float(), **{**f, "lo": torch.empty(0)})
+
+
+def test_rotation_by_an_empty_table_is_refused():
+    """Before anything is launched, positions given or not: there is no row to read."""
+    native = _lib.load()
+    for pos in (0, 16):
+        side = _lib.ROPE_SIDE.pack(16, 0, 16, 0, pos, 0, 64, 64, 64, 1, 1)
+        assert native.hclsm_qk_norm_rope(side, None, 16, 16, 0, 32, 1, 64, 1e-6, _lib.F32, 0, None) == 1
+        side = _lib.ROPE_SIDE.pack(16, 16, 16, 0, pos, 0, 64, 64, 64, 1, 1)
+        assert native.hclsm_qk_norm_rope_bwd(side, None, 16, 16, 0, 32, 1, 64, 1e-6, _lib.F32, 0, None, 0, None) == 1
