@@ -10,6 +10,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhclsm_b200.so")
@@ -214,6 +215,15 @@ def like(t, shape, dtype, name, device):
     if t.device != device:
         raise ValueError(f"{name} must be on {device}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def no_tangents(*tensors):
+    """A forward-mode derivative (torch.autograd.forward_ad) is refused: the kernels would drop the tangents."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside a dual level no tensor has one
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("hclsm_b200: this operator has no forward-mode derivative")
 
 
 def no_double_backward():

@@ -104,6 +104,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
     ``start[b]`` is the number of tokens already there (or, to write anew from there, a
     multiple of the block: what was behind it is gone).  A request that does not
     fit the capacity writes nothing and sets the device error word."""
+    _lib.no_tangents(k, v)
     dev = _lib.require_cuda(cache.k, k, v, start, count)
     c, (B, Hkv, _, D) = cache._args()
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != B or k.shape[2:] != (Hkv, D):
@@ -123,6 +124,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
 def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
     """(k, v), each (B, T, Hkv, D) in the cache's dtype: the first ``lens[b]``
     tokens written (default all) as the values they stand for, zeros after them."""
+    _lib.no_tangents(cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
     dev = _lib.require_cuda(cache.k, lens)
     c, (B, Hkv, T, D) = cache._args()
     lens = _lib.index32(lens, (B,), "lens", dev)
@@ -136,6 +138,7 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
     """softmax(scale q k^T) v of q (B, Lq, H, D), in the cache's dtype, over the
     first ``lens[b]`` tokens written (default all of the capacity; clamped to [0, T]); H
     is a multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
+    _lib.no_tangents(q, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
     dev = _lib.require_cuda(q, cache.k, lens)
     c, (B, Hkv, _, D) = cache._args()
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:

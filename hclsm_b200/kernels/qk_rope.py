@@ -36,6 +36,7 @@ def _dense16(t):
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
+    _lib.no_tangents(q, k, q_weight, k_weight, cos, sin)
     dev = _lib.require_cuda(q, k, q_weight, k_weight, cos, sin)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be (batch, tokens, heads, head_dim)")

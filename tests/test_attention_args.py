@@ -6,10 +6,11 @@ import pickle
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import hclsm_b200.torch_ops  # noqa: F401  (registers the ops)
 from hclsm_b200 import _lib
-from hclsm_b200.kernels import Kv8Cache, kv8_attention, kv8_read, kv8_write
+from hclsm_b200.kernels import Kv8Cache, cross_attention, kv8_attention, kv8_read, kv8_write, qk_norm_rope
 from hclsm_b200.kernels.cross_attn import attention_bwd
 
 
@@ -171,3 +172,25 @@ def test_rotation_by_an_empty_table_is_refused():
         assert native.hclsm_qk_norm_rope(side, None, 16, 16, 0, 32, 1, 64, 1e-6, _lib.F32, 0, None) == 1
         side = _lib.ROPE_SIDE.pack(16, 16, 16, 0, pos, 0, 64, 64, 64, 1, 1)
         assert native.hclsm_qk_norm_rope_bwd(side, None, 16, 16, 0, 32, 1, 64, 1e-6, _lib.F32, 0, None, 0, None) == 1
+
+
+def test_forward_mode_derivatives_are_refused_not_dropped(lib):
+    ops, at = torch.ops.hclsm_b200, torch.zeros(2, dtype=torch.int32)
+    x, w = torch.zeros(2, 3, 1, 32, dtype=torch.bfloat16), torch.ones(32)
+    cos, sin = torch.ones(8, 16), torch.zeros(8, 16)
+    cache, other = _cache(), _cache()
+    with forward_ad.dual_level():
+        d, dw, dc = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, cos))
+        other.k_tail = forward_ad.make_dual(other.k_tail, torch.ones_like(other.k_tail))
+        for call in (lambda: cross_attention(d, x, x), lambda: cross_attention(x, x, d), lambda: qk_norm_rope(d),
+                     lambda: qk_norm_rope(x, d), lambda: qk_norm_rope(x, None, dw),
+                     lambda: qk_norm_rope(x, cos=dc, sin=sin), lambda: kv8_write(cache, d, x, at),
+                     lambda: kv8_write(cache, x, d, at), lambda: kv8_attention(d, cache, at),
+                     lambda: kv8_attention(x, other, at), lambda: kv8_read(other, at),
+                     lambda: ops.cross_attention_fwd(x, d, x, None, None, 0.1),
+                     lambda: ops.qk_norm_rope_fwd(d, x, None, None, None, None, None, None, 1e-6, False)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not lib.calls
+        cross_attention(x, x, x), qk_norm_rope(x), kv8_attention(x, cache, at)  # no tangents
+        assert forward_ad.unpack_dual(d).tangent is not None
