@@ -98,12 +98,20 @@ class Kv8Cache:
         return self.k_tail.shape[2]
 
 
+def _no_gradients(what, cache, *tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors, cache.k_scale, cache.v_scale, cache.k_tail,
+                                                                 cache.v_tail)):
+        raise NotImplementedError(f"{what} has no gradients: call it under torch.no_grad()")
+
+
 def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tensor | None = None) -> None:
     """Append k, v (B, n, Hkv, D), in place: token i of entry b becomes token
     ``start[b] + i`` of the cache, for the first ``count[b]`` tokens (default n).
     ``start[b]`` is the number of tokens already there (or, to write anew from there, a
     multiple of the block: what was behind it is gone).  A request that does not
-    fit the capacity writes nothing and sets the device error word."""
+    fit the capacity writes nothing and sets the device error word.  No gradients:
+    k and v that require them are refused."""
+    _no_gradients("kv8_write", cache, k, v)
     _lib.no_tangents(k, v)
     dev = _lib.require_cuda(cache.k, k, v, start, count)
     c, (B, Hkv, _, D) = cache._args()
@@ -124,6 +132,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
 def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):
     """(k, v), each (B, T, Hkv, D) in the cache's dtype: the first ``lens[b]``
     tokens written (default all) as the values they stand for, zeros after them."""
+    _no_gradients("kv8_read", cache)
     _lib.no_tangents(cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
     dev = _lib.require_cuda(cache.k, lens)
     c, (B, Hkv, T, D) = cache._args()
@@ -138,6 +147,7 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
     """softmax(scale q k^T) v of q (B, Lq, H, D), in the cache's dtype, over the
     first ``lens[b]`` tokens written (default all of the capacity; clamped to [0, T]); H
     is a multiple of Hkv.  An entry without tokens gives zeros.  No gradients."""
+    _no_gradients("kv8_attention", cache, q)
     _lib.no_tangents(q, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
     dev = _lib.require_cuda(q, cache.k, lens)
     c, (B, Hkv, _, D) = cache._args()
@@ -148,8 +158,6 @@ def kv8_attention(q: Tensor, cache: Kv8Cache, lens: Tensor | None = None, *, sca
         raise ValueError(f"query heads ({H}) must be a multiple of key heads ({Hkv})")
     if q.dtype != cache.dtype:
         raise TypeError(f"q must have the cache's dtype {cache.dtype}, got {q.dtype}")
-    if torch.is_grad_enabled() and q.requires_grad:
-        raise NotImplementedError("kv8_attention has no gradients: call it under torch.no_grad()")
     scale = D ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"scale must be positive and finite, got {scale}")

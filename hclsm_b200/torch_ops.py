@@ -24,7 +24,7 @@ CUDA tensors only (no CPU kernel is registered).  Every op has a fake
 * ``qk_norm_rope_fwd`` / ``qk_norm_rope_bwd`` and ``cross_attention_fwd`` /
   ``cross_attention_bwd`` (both forwards with registered autograd formulas), and
   ``kv8_write`` / ``kv8_attention`` on the tensors of a ``Kv8Cache``
-  (``kv8_write`` mutates them).
+  (``kv8_write`` mutates them, and wants detached keys and values).
 
 Scan inputs must already share one dtype (fp32 or bf16: x, dt, B, C, z) with
 A_log and D in fp32, and be contiguous; ``hclsm_b200.kernels.ssm_scan`` does
@@ -283,6 +283,8 @@ torch.library.register_autograd(f"{_NS}::cross_attention_fwd", _xattn_backward, 
                          mutates_args=("ck", "cv", "k_scale", "v_scale", "k_tail", "v_tail"))
 def kv8_write(ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor, v_tail: Tensor, k: Tensor,
               v: Tensor, start: Tensor, count: Optional[Tensor]) -> None:
+    if k.requires_grad or v.requires_grad:  # an operator that mutates has no autograd formula, and grad mode is off here
+        raise NotImplementedError("kv8_write has no gradients: detach k and v")
     _kv8.kv8_write(_kv8.Kv8Cache(ck, cv, k_scale, v_scale, k_tail, v_tail), k, v, start, count)
 
 

@@ -194,3 +194,25 @@ def test_forward_mode_derivatives_are_refused_not_dropped(lib):
         assert not lib.calls
         cross_attention(x, x, x), qk_norm_rope(x), kv8_attention(x, cache, at)  # no tangents
         assert forward_ad.unpack_dual(d).tangent is not None
+
+
+def test_cache_calls_refuse_to_cut_a_graph(lib):
+    x, at = torch.zeros(2, 3, 1, 32, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    g = x.clone().requires_grad_()
+    cache, other = _cache(), _cache()
+    other.v_tail.requires_grad_()
+    c = (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
+    calls = (lambda: kv8_write(cache, g, x, at), lambda: kv8_write(cache, x, g, at), lambda: kv8_attention(g, cache, at),
+             lambda: kv8_write(cache, (g * 2), x, at), lambda: kv8_write(other, x, x, at), lambda: kv8_read(other, at),
+             lambda: kv8_attention(x, other, at))
+    for call in calls:
+        with pytest.raises(NotImplementedError, match="no gradients"):
+            call()
+    for k, v in ((g, x), (x, g)):
+        with pytest.raises(NotImplementedError, match="no gradients"):
+            torch.ops.hclsm_b200.kv8_write(*c, k, v, at, None)
+    assert not lib.calls
+    with torch.no_grad():
+        for call in calls:
+            call()
+    assert lib.calls
