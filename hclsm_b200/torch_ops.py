@@ -22,7 +22,8 @@ CUDA tensors only (no CPU kernel is registered).  Every op has a fake
   ``event_mha(qkv, key_pad, frames, T, H, HD, scale)``
   (sparse_event_attn.py:93-188, level1_event.py:33-54);
 * ``qk_norm_rope_fwd`` / ``qk_norm_rope_bwd`` and ``cross_attention_fwd`` /
-  ``cross_attention_bwd`` (both forwards with registered autograd formulas), and
+  ``cross_attention_bwd`` (both forwards with registered autograd formulas; of the
+  cross attention's outputs o alone has gradients), and
   ``kv8_write`` / ``kv8_attention`` on the tensors of a ``Kv8Cache``
   (``kv8_write`` mutates them, and wants detached keys and values).
 
@@ -269,9 +270,14 @@ def _xattn_setup(ctx, inputs, output):
     q, k, v, kv_lens, key_mask, scale = inputs
     ctx.save_for_backward(q, k, v, *output, kv_lens, key_mask)
     ctx.scale = scale
+    ctx.set_materialize_grads(False)
 
 
 def _xattn_backward(ctx, go, glse, glo):
+    if glse is not None or glo is not None:
+        raise NotImplementedError("cross_attention_fwd: only o has gradients; detach lse and lo")
+    if go is None:
+        return (None,) * 6
     q, k, v, o, lse, lo, kv_lens, key_mask = ctx.saved_tensors
     return (*cross_attention_bwd(q, k, v, o, lse, lo, go, kv_lens, key_mask, ctx.scale), None, None, None)
 

@@ -216,3 +216,17 @@ def test_cache_calls_refuse_to_cut_a_graph(lib):
         for call in calls:
             call()
     assert lib.calls
+
+
+def test_gradients_of_lse_and_lo_are_refused_not_dropped(lib):
+    q, k = torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 9, 2, 64, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (q, k, k.clone())]
+    for use in (lambda o, lse, lo: o.float().sum() + lse.sum(), lambda o, lse, lo: lse.sum(),
+                lambda o, lse, lo: o.float().sum() + lo.float().sum()):
+        out = torch.ops.hclsm_b200.cross_attention_fwd(*leaves, None, None, 0.125)
+        with pytest.raises(NotImplementedError, match="only o has gradients"):
+            use(*out).backward()
+    o, lse, lo = torch.ops.hclsm_b200.cross_attention_fwd(*leaves, None, None, 0.125)
+    lib.calls.clear()
+    (o.float().sum() + lse.detach().sum()).backward()
+    assert [n for n, _ in lib.calls][-1] == "hclsm_xattn_bwd" and all(t.grad.shape == t.shape for t in leaves)
