@@ -57,6 +57,8 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
             raise ValueError(f"{name} without the norm (eps=None)")
         if w.shape != (D,) or w.dtype != torch.float32:
             raise ValueError(f"{name} must be ({D},) float32")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (cos, sin)):
+        raise NotImplementedError("qk_norm_rope has no gradients of cos and sin: detach them")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:

@@ -228,6 +228,8 @@ def _(q, k, q_weight, k_weight, cos, sin, q_pos, k_pos, eps, interleaved, gq, gk
 
 
 def _rope_setup(ctx, inputs, output):
+    if any(ctx.needs_input_grad[4:6]):
+        raise NotImplementedError("qk_norm_rope_fwd has no gradients of cos and sin: detach them")
     ctx.save_for_backward(*inputs[:8])
     ctx.eps, ctx.interleaved = inputs[8:]
 

@@ -230,3 +230,22 @@ def test_gradients_of_lse_and_lo_are_refused_not_dropped(lib):
     lib.calls.clear()
     (o.float().sum() + lse.detach().sum()).backward()
     assert [n for n, _ in lib.calls][-1] == "hclsm_xattn_bwd" and all(t.grad.shape == t.shape for t in leaves)
+
+
+def test_gradients_of_the_rotation_tables_are_refused_not_dropped(lib):
+    x = torch.zeros(2, 3, 1, 32, dtype=torch.bfloat16)
+    xg, cos, sin = x.clone().requires_grad_(), torch.ones(8, 16), torch.zeros(8, 16)
+    cg, op = cos.clone().requires_grad_(), torch.ops.hclsm_b200.qk_norm_rope_fwd
+    for q in (x, xg):
+        for c, s in ((cg, sin), (cos, cg), (cg * 2, sin)):
+            with pytest.raises(NotImplementedError, match="cos and sin"):
+                qk_norm_rope(q, cos=c, sin=s)
+            with pytest.raises(NotImplementedError, match="cos and sin"):
+                op(q, q, None, None, c, s, None, None, 1e-6, False)
+    lib.calls.clear()
+    with torch.no_grad():
+        qk_norm_rope(x, cos=cg, sin=sin)
+        op(x, x, None, None, cg, sin, None, None, 1e-6, False)
+    y, _ = op(xg, x, None, None, cos, sin, None, None, 1e-6, False)
+    y.sum().backward()
+    assert len(lib.calls) == 4
