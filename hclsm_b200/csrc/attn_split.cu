@@ -16,7 +16,8 @@
 // difference).  For fp16's range queries are scaled by a power of two to a largest value
 // below 1 (exact, but for values 2^-14 of the largest and below, which lose what is below
 // 2^-24 of it) and weights to at most 2^12; fp16's 11 bits round them less than bf16's 8.
-// The scale of a block of keys multiplies its scores (K); that of its values, over the largest so far, its weights (V).
+// The scale of a block of keys multiplies its scores (K); that of its values, over the largest of weight times scale so
+// far, its weights (V).
 // fp32 operands are split into three bf16 pieces (8 bits each) and the products
 // of pieces whose order is at most 2 are summed: fp32 accuracy.
 // Bound: HBM (each key and value byte is read once); splits and warps are merged
@@ -189,6 +190,14 @@ struct State {
   float m[2], l[2];
 };
 
+// The 8-bit blocks' O is held over v, times 2^12: a row's largest product so far of a step's largest weight (relative
+// to the row's maximum score, 2^-115 at least, so that no factor overflows) and its block's value scale; at least
+// 2^-110, where the smallest step of an fp16 weight is below bf16's smallest number.
+constexpr float kLeast = 7.703719777548943e-34f, kFaint = 2.407412430484045e-35f;
+struct Ref {
+  float v[2] = {kLeast, kLeast}, inv[2] = {4096.0f / kLeast, 4096.0f / kLeast};  // 2^12 / v
+};
+
 // Blocks an SM: what the registers of a row's accumulators and one step's keys and values leave room for.
 template <typename T, int D> constexpr int kPerSm = sizeof(T) == 4 ? (D <= 64 ? 3 : 2) : (D <= 64 ? 4 : 3);
 
@@ -234,12 +243,11 @@ __device__ __forceinline__ void load_a(const uint32_t* w, uint32_t (&a)[4]) {
 // Steps first, first + stride, ... below last of 16 keys each.  addr_k / addr_v
 // (key) give a row's address; ok(key) says whether the key is allowed (false
 // past the end); nk > 0 keys have memory; all_ok(step) skips the per-key checks.
-// fs, off: factor and offset of rows g and g + 8's raw scores.  vref (F16): the largest value scale so far; O is held
-// over it, times 2^12.
+// fs, off: factor and offset of rows g and g + 8's raw scores.
 template <typename E, int D, int CV, int NQ, int NR, bool F16, typename AddrK, typename AddrV, typename Ok,
           typename AllOk, typename Scale>
 __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const float (&fs)[2], const float (&off)[2],
-                                      float& vref, int first, int last, int stride, int nk,
+                                      Ref& ref, int first, int last, int stride, int nk,
                                       AddrK addr_k, AddrV addr_v, Ok ok, AllOk all_ok, Scale scale) {
   using R = Rows<E, D, CV>;
   // fp32: a product is formed from zero and added here, because the tensor core's own
@@ -304,7 +312,8 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
       for (int t = 0; t < 4; ++t) good[t] = ok(step * 16 + (t >> 1) * 8 + 2 * c + (t & 1));
     }
     const float f[2] = {fs[0] * cur.x, fs[1] * cur.x};
-    float mx[2] = {st.m[0], st.m[1]};
+    float mx[2] = {-INFINITY, -INFINITY};  // of this step alone where F16
+    if constexpr (!F16) mx[0] = st.m[0], mx[1] = st.m[1];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -318,7 +327,38 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
     }
-    if (__any_sync(0xffffffffu, mx[0] != st.m[0] || mx[1] != st.m[1])) {
+    float pv[2] = {cur.y, cur.y};
+    if constexpr (F16) {
+      // Weights are at most 2^12 through the largest weight times scale, not the largest scale: a block of large values
+      // that no weight falls on would take the others' weights below fp16's range.
+      float top[2];
+      bool more = false;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const float m = fmaxf(st.m[r], mx[r]);
+        top[r] = cur.y * fmaxf(ex2(mx[r] - m), kFaint);  // NaN where both are -inf: kFaint
+        mx[r] = m;
+        more |= m != st.m[r] || top[r] > ref.v[r];
+      }
+      if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float w = mx[r] == -INFINITY ? 1.0f : ex2(st.m[r] - mx[r]);
+          st.m[r] = mx[r];
+          st.l[r] *= w;
+          const float old = ref.v[r] * w;  // a new maximum lowers O through it
+          ref.v[r] = fmaxf(fmaxf(old, top[r]), kLeast);
+          ref.inv[r] = 4096.0f / ref.v[r];
+          if (ref.v[r] != old) {
+            const float f = old / ref.v[r];
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) st.o[j][2 * r] *= f, st.o[j][2 * r + 1] *= f;
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) pv[r] *= ref.inv[r];  // a scale of 0 or NaN stays
+    } else if (__any_sync(0xffffffffu, mx[0] != st.m[0] || mx[1] != st.m[1])) {
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         const float w = mx[r] == -INFINITY ? 1.0f : ex2(st.m[r] - mx[r]);
@@ -327,18 +367,6 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) st.o[j][2 * r] *= w, st.o[j][2 * r + 1] *= w;
       }
-    }
-    float pv = cur.y;
-    if constexpr (F16) {
-      if (cur.y > vref) {  // the same for the whole warp
-        const float w = vref / cur.y;
-        vref = cur.y;
-#pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
-      }
-      pv = cur.y > 0.0f ? cur.y / vref * 4096.0f : cur.y;  // 0 or NaN stay
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -351,7 +379,7 @@ __device__ __forceinline__ void sweep(State<D>& st, const uint32_t* qf, const fl
         const float base = st.m[e >> 1] == -INFINITY ? 0.0f : st.m[e >> 1];
         s[t][e] = ex2(s[t][e] - base);
         st.l[e >> 1] += s[t][e];
-        s[t][e] *= pv;
+        s[t][e] *= pv[e >> 1];
         if (!all && !good[2 * t + (e & 1)]) s[t][e] = 0.0f;
       }
     uint32_t pa[NQ][4];
@@ -476,43 +504,42 @@ __global__ void __launch_bounds__(kThreads, kPerSm<T, D>) split_kernel(const __g
 #pragma unroll
       for (int r = 0; r < 2; ++r) fs8[r] = c2 / s_inv[g + 8 * r], off8[r] = 1152.0f * s_sum[g + 8 * r];
     }
-    float vref = 0.0f;
+    Ref ref;
     auto scale = [&](int step) { return make_float2(p.ks[s0 + step / spb], p.vs[s0 + step / spb]); };
     auto key = [&](int j) { return k8 + (int64_t)j * D; };
     auto value = [&](int j) { return v8 + (int64_t)j * D; };
     sweep<int8_t, D, CV, NQ, NR, F16>(
-        st, qh, fs8, off8, vref, first + warp, last, kWarps, n8, key, value, [](int) { return true; },
+        st, qh, fs8, off8, ref, first + warp, last, kWarps, n8, key, value, [](int) { return true; },
         [](int) { return true; }, scale);
     // a length inside a block: a complete one (8 bits), or the one that the tail holds (scale -1)
     const bool more = sp == p.splits - 1 && n > n8;
     const bool tail = more && p.ks[s0 + n8 / p.block] < 0.0f;
     if (more && !tail)
       sweep<int8_t, D, CV, NQ, NR, F16>(
-          st, qh, fs8, off8, vref, steps + warp, (n + 15) / 16, kWarps, n, key, value, [&](int j) { return j < n; },
+          st, qh, fs8, off8, ref, steps + warp, (n + 15) / 16, kWarps, n, key, value, [&](int j) { return j < n; },
           [&](int step) { return step * 16 + 16 <= n; }, scale);
     if constexpr (F16) {
-      const float w = vref * (1.0f / 4096.0f);
 #pragma unroll
       for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-        for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= w;
+        for (int e = 0; e < 2 * NR; ++e) st.o[j][e] *= ref.v[e >> 1] * (1.0f / 4096.0f);
     }
     if (tail) {
       const char* kt = reinterpret_cast<const char*>(static_cast<const T*>(p.kt) + bh * p.block * D);
       const char* vt = reinterpret_cast<const char*>(static_cast<const T*>(p.vt) + bh * p.block * D);
       const int nt = n - n8;
       sweep<T, D, CV, NQ, NR, false>(
-          st, qf, fs, off, vref, warp, (nt + 15) / 16, kWarps, nt, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
+          st, qf, fs, off, ref, warp, (nt + 15) / 16, kWarps, nt, [&](int j) { return kt + j * (int)(D * sizeof(T)); },
           [&](int j) { return vt + j * (int)(D * sizeof(T)); }, [&](int j) { return j < nt; },
           [&](int step) { return step * 16 + 16 <= nt; }, [](int) { return make_float2(1.0f, 1.0f); });
     }
   } else {
-    float vref = 0.0f;
+    Ref ref;
     const char* kb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.k.p) + b * p.x.k.sb + hk * p.x.k.sh);
     const char* vb = reinterpret_cast<const char*>(static_cast<const T*>(p.x.v.p) + b * p.x.v.sb + hk * p.x.v.sh);
     const int64_t kst = p.x.k.st * (int64_t)sizeof(T), vst = p.x.v.st * (int64_t)sizeof(T);
     sweep<T, D, CV, NQ, NR, false>(
-        st, qf, fs, off, vref, first + warp, last, kWarps, n, [&](int j) { return kb + j * kst; },
+        st, qf, fs, off, ref, first + warp, last, kWarps, n, [&](int j) { return kb + j * kst; },
         [&](int j) { return vb + j * vst; }, [&](int j) { return xattn::key_ok(p.x, b, n, j); },
         [&](int step) { return !p.x.mask && step * 16 + 16 <= n; }, [](int) { return make_float2(1.0f, 1.0f); });
   }

@@ -7,8 +7,8 @@ import pytest
 import torch
 
 import hclsm_b200
-from hclsm_b200.kernels import Kv8Cache, cross_attention, kv8_read, kv8_write, qk_norm_rope
-from test_attention_ops_gpu import BF16, F32, U, _allowed, _attn_ref, _err, _gen, _i32, _randn, _rope_ref
+from hclsm_b200.kernels import Kv8Cache, cross_attention, kv8_attention, kv8_read, kv8_write, qk_norm_rope
+from test_attention_ops_gpu import BF16, F32, U, _allowed, _attn_ref, _err, _gen, _i32, _Plain, _randn, _rope_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,26 @@ def test_strides_of_dims_of_one_do_not_count(dtype, L, odd):
         q = _randn(g, 1, Lq, 4, 64, dtype=dtype)
         kd, vd = (t.new_empty(t.shape).copy_(t) for t in (k, v))
         assert torch.equal(cross_attention(q, k, v), cross_attention(q, kd, vd))
+
+
+@pytest.mark.parametrize("far", [0, 5, 15])
+@pytest.mark.parametrize("D,G,block", [(64, 4, 32), (128, 12, 16), (32, 1, 64)])
+def test_cache_blocks_of_large_values_and_no_weight(far, D, G, block):
+    """A block whose values are 1e6 to 1e30 times the others' but whose keys weigh e^-60 and less, or one of zeros whose
+    keys weigh e^25 and more, takes nothing from the precision of the others: 2 u as ever."""
+    g = _gen(D + far)
+    T = 16 * block
+    for size, unit, key in ((1e6, 1.0, -10.0), (1e10, 1.0, -10.0), (1e14, 1.0, -10.0), (1e30, 1.0, -10.0),
+                            (1e30, 1e-35, -10.0), (0.0, 1.0, 4.0), (0.0, 1e-20, 4.0)):
+        k, v = 0.5 * _randn(g, 2, T, 2, D), unit * _randn(g, 2, T, 2, D)
+        k[:, far * block:(far + 1) * block] = key
+        v[:, far * block:(far + 1) * block] *= size
+        q = (1 + 0.3 * _randn(g, 2, 1, 2 * G, D)).to(BF16)
+        k, v = k.to(BF16), v.to(BF16)
+        scale = 7.5 / D  # q . k scale = -75 or 30, +- 15 %, there
+        cache, plain = Kv8Cache.empty(2, T, 2, D, block=block), _Plain(2, T, 2, D, block)
+        kv8_write(cache, k, v, _i32(0, 0))
+        plain.write((k, v), [0, 0], [T, T])
+        for lens in (_i32(T, T), _i32(T, T - block // 2)):
+            got = kv8_attention(q, cache, lens, scale=scale)
+            assert _err(got, _attn_ref(q, *plain.x, _allowed(2, T, lens, None), scale)) < 2 * U, (size, unit)
