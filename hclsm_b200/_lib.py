@@ -134,12 +134,17 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_get_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def stream_ptr(device) -> int:
     """The current stream of a CUDA device as an integer (a tensor's device has an index; the
-    raw query skips the Stream object, about 3 us a call)."""
+    raw query skips the Stream object, about 3 us a call).  Kernels launch on the current
+    device, so it has to be the tensors' one."""
+    if device.index is not None and device.index != _get_device():
+        raise ValueError(f"hclsm_b200: tensors on {device}, current device cuda:{_get_device()}: call "
+                         "torch.cuda.set_device or use torch.cuda.device")
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream

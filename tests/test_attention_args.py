@@ -249,3 +249,12 @@ def test_gradients_of_the_rotation_tables_are_refused_not_dropped(lib):
     y, _ = op(xg, x, None, None, cos, sin, None, None, 1e-6, False)
     y.sum().backward()
     assert len(lib.calls) == 4
+
+
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    """A launch goes to the current device, where the other's addresses mean nothing."""
+    monkeypatch.setattr(_lib, "_get_device", lambda: 0, raising=False)
+    monkeypatch.setattr(_lib, "_raw_stream", lambda index: 1000 + index)
+    assert _lib.stream_ptr(torch.device("cuda", 0)) == 1000
+    with pytest.raises(ValueError, match="current device"):
+        _lib.stream_ptr(torch.device("cuda", 1))
