@@ -8,6 +8,7 @@ import torch
 
 import hclsm_b200
 from hclsm_b200.kernels import Kv8Cache, cross_attention, kv8_attention, kv8_read, kv8_write, qk_norm_rope
+from hclsm_b200.kernels.cross_attn import attention_bwd, attention_fwd
 from test_attention_ops_gpu import BF16, F32, U, _allowed, _attn_ref, _err, _gen, _i32, _Plain, _randn, _rope_ref
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +105,56 @@ def test_cache_blocks_of_large_values_and_no_weight(far, D, G, block):
         for lens in (_i32(T, T), _i32(T, T - block // 2)):
             got = kv8_attention(q, cache, lens, scale=scale)
             assert _err(got, _attn_ref(q, *plain.x, _allowed(2, T, lens, None), scale)) < 2 * U, (size, unit)
+
+
+def _one_rounding(ref):
+    """The error of the 64-bit result rounded to bf16 once: what an output cannot be better than."""
+    return _err(ref.to(BF16), ref)
+
+
+@pytest.mark.parametrize("Lq,Lk,D", [(200, 2000, 64), (200, 2000, 128), (40, 2000, 64), (1, 9000, 128)])
+def test_forward_error_is_that_of_two_roundings(Lq, Lk, D):
+    """Weights are rounded to bf16 once, independently of each other, and so is the output: with random values both errors
+    are of one size, sqrt(2) of one; 10 % for what else there is (exponentials 1e-4, sums in fp32)."""
+    g = _gen(Lq + D)
+    q, k, v = (_randn(g, 2, n, 4, D, dtype=BF16) for n in (Lq, Lk, Lk))
+    ref = _attn_ref(q, k, v, _allowed(2, Lk, None, None))
+    assert _err(cross_attention(q, k, v), ref) < 1.1 * 2 ** 0.5 * _one_rounding(ref)
+
+
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (64, 12)])
+def test_cache_error_is_that_of_one_rounding(D, G):
+    """Weights against the cache are fp16 (3 bits more than the output): the output's rounding is nearly all of the error.
+    bf16 weights would give sqrt(2) of it."""
+    g = _gen(D + G)
+    T = 8192
+    cache, plain = Kv8Cache.empty(2, T, 2, D), _Plain(2, T, 2, D, 32)
+    kv = [_randn(g, 2, T, 2, D, dtype=BF16) for _ in range(2)]
+    kv8_write(cache, *kv, _i32(0, 0))
+    plain.write(kv, [0, 0], [T, T])
+    q = _randn(g, 2, 1, 2 * G, D, dtype=BF16)
+    ref = _attn_ref(q, *plain.x, _allowed(2, T, None, None))
+    assert _err(kv8_attention(q, cache, _i32(T, T)), ref) < 1.15 * _one_rounding(ref)
+
+
+@pytest.mark.parametrize("Lq,D", [(1, 64), (40, 64), (200, 64), (200, 128), (40, 33)])
+def test_what_rounding_took_from_the_output_reaches_the_backward(Lq, D):
+    """With queries of zero the weights of 4 keys are 1/4 exactly, and values of 64 + N(0, 1) make the output's rounding
+    (steps of 0.5) as large as what do . (v - o) is made of: gradients are right only through lo.  o + lo: 16 bits, 2^-16.
+    dq: the weights' gradients and the result rounded once each, and sums of 64 D terms, 2 u and an eighth more."""
+    g = _gen(Lq + D)
+    q = torch.zeros(2, Lq, 2, D, device="cuda", dtype=BF16)
+    k, v, do = (_randn(g, 2, n, 2, D) for n in (4, 4, Lq))
+    k, v, do = k.to(BF16), (64 + v).to(BF16), do.to(BF16)
+    ok = _allowed(2, 4, None, None)
+    o, lse, lo = attention_fwd(q, k, v, None, None, D ** -0.5)
+    ref = [t.double().requires_grad_() for t in (q, k, v)]
+    ro = _attn_ref(*ref, ok)
+    assert _err(o.double() + lo.double(), ro) < 2.0 ** -16 and _err(o, ro) > 2.0 ** -11
+    got = attention_bwd(q, k, v, o, lse, lo, do, None, None, D ** -0.5)
+    want = torch.autograd.grad(ro, ref, do.double())
+    assert _err(got[0], want[0]) < 2.25 * U and _err(got[2], want[2]) < 2.25 * U
+    # the halves are summed: which of the two holds what is nothing to the backward
+    swapped = attention_bwd(q, k, v, lo, lse, o, do, None, None, D ** -0.5)
+    for a, b in zip(got, swapped):
+        assert torch.equal(a, b)
