@@ -142,11 +142,12 @@ def stream_ptr(device) -> int:
     """The current stream of a CUDA device as an integer (a tensor's device has an index; the
     raw query skips the Stream object, about 3 us a call).  Kernels launch on the current
     device, so it has to be the tensors' one."""
-    if device.index is not None and device.index != _get_device():
+    index = device.index
+    if index is not None and index != _get_device():
         raise ValueError(f"hclsm_b200: tensors on {device}, current device cuda:{_get_device()}: call "
                          "torch.cuda.set_device or use torch.cuda.device")
-    if _raw_stream is not None and device.index is not None:
-        return _raw_stream(device.index)
+    if _raw_stream is not None and index is not None:
+        return _raw_stream(index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -222,9 +223,14 @@ def like(t, shape, dtype, name, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def in_dual_level() -> bool:
+    """Whether a tensor can have a forward-mode tangent at all."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def no_tangents(*tensors):
     """A forward-mode derivative (torch.autograd.forward_ad) is refused: the kernels would drop the tangents."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # outside a dual level no tensor has one
+    if not in_dual_level():
         return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:

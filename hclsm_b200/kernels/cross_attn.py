@@ -79,7 +79,8 @@ class _CrossAttention(torch.autograd.Function):
 
 def _prepare(q, k, v, kv_lens, key_mask, scale):
     """The checked arguments of the kernels."""
-    _lib.no_tangents(q, k, v)
+    if _lib.in_dual_level():
+        _lib.no_tangents(q, k, v)
     dev = _lib.require_cuda(q, k, v, kv_lens, key_mask)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError("q must be (B, Lq, H, D); k and v (B, Lk, Hkv, D)")

@@ -36,7 +36,8 @@ def _dense16(t):
 
 
 def _check(q, k, q_weight, k_weight, cos, sin, eps):
-    _lib.no_tangents(q, k, q_weight, k_weight, cos, sin)
+    if _lib.in_dual_level():
+        _lib.no_tangents(q, k, q_weight, k_weight, cos, sin)
     dev = _lib.require_cuda(q, k, q_weight, k_weight, cos, sin)
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q and k must be (batch, tokens, heads, head_dim)")
@@ -57,7 +58,7 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
             raise ValueError(f"{name} without the norm (eps=None)")
         if w.shape != (D,) or w.dtype != torch.float32:
             raise ValueError(f"{name} must be ({D},) float32")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (cos, sin)):
+    if ((cos is not None and cos.requires_grad) or (sin is not None and sin.requires_grad)) and torch.is_grad_enabled():
         raise NotImplementedError("qk_norm_rope has no gradients of cos and sin: detach them")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
@@ -69,8 +70,9 @@ def _check(q, k, q_weight, k_weight, cos, sin, eps):
 
 def _side(x, y, w, pos, dy=None, dw=None):
     sb, st, sh, _ = x.stride()
-    B, L, H, _ = x.shape  # the library wants strides of whole 16 bytes; one of a dim of one is not used
-    sb, st, sh = sb if B > 1 else 0, st if L > 1 else 0, sh if H > 1 else 0
+    B, L, H, _ = x.shape
+    if (sb | st | sh) & 7:  # the library wants strides of whole 16 bytes; one of a dim of one is not used
+        sb, st, sh = sb if B > 1 else 0, st if L > 1 else 0, sh if H > 1 else 0
     return _lib.ROPE_SIDE.pack(x.data_ptr(), 0 if dy is None else dy.data_ptr(), y.data_ptr(),
                                0 if w is None else w.data_ptr(), 0 if pos is None else pos.data_ptr(),
                                0 if dw is None else dw.data_ptr(), sb, st, sh, L, H)
