@@ -15,16 +15,20 @@
 // score.  For V it is taken off (the sum over a long history would lose the
 // difference).  For fp16's range queries are scaled by a power of two to a largest value
 // below 1 (exact, but for values 2^-14 of the largest and below, which lose what is below
-// 2^-24 of it) and weights to at most 2^12; fp16's 11 bits round them less than bf16's 8.
+// 2^-24 of it: a query's channel 2^12 times its others whose keys are nearly zero takes the output from 0.16 to 0.22 %,
+// one of 2^14 times to 0.6 %; bf16 there is exact and costs 18 %, 542 us against 458) and weights to at most 2^12;
+// fp16's 11 bits round them less than bf16's 8.
 // The scale of a block of keys multiplies its scores (K); that of its values, over the largest of weight times scale so
 // far, its weights (V).
 // fp32 operands are split into three bf16 pieces (8 bits each) and the products
 // of pieces whose order is at most 2 are summed: fp32 accuracy.
 // Bound: HBM (each key and value byte is read once); splits and warps are merged
 // in a fixed order.  One query over 8 x 16384 ragged bf16 states, 16 heads over 4 of
-// 128: 48 us (floor 31); over 16 x 65536 cached states, 32 heads over 8 of 128: 371 us,
-// 4.3 TB/s, 41 % of the issue slots (conversions and softmax).  Three blocks an SM: four
-// spill (415 us against 380); four waves of blocks: eight are slower (480 against 450).
+// 128: 50 us (floor 31); over 16 x 65536 cached states, 32 heads over 8 of 128: 459 us,
+// 4.7 TB/s, and 355 us, 4.4 TB/s, where the lengths are ragged (0.72 of the states).  43 % of the
+// issue slots are taken, so loads in flight are the bound: 12 warps an SM, a step each in
+// registers.  Three blocks an SM: four spill (415 us against 380); four waves of blocks: eight are slower (480 against
+// 450).
 #include <cuda_fp16.h>
 
 #include <type_traits>

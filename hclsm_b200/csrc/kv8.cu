@@ -9,8 +9,8 @@
 // not finite gets a NaN scale: what is read from it is NaN, not a wrong number.
 //
 // Both kernels move every byte once: the bound is HBM, at small sizes the launch.
-// 8 x 2048 tokens, 6 heads of 64, bf16 (25 MB of states, 13 MB of integers): about
-// 18 us to write and 10 to read back from L2, one wave of blocks each.
+// 8 x 2048 tokens, 6 heads of 64, bf16 (25 MB of states, 13 MB of integers): 16 to
+// 18 us to write and 10 to 13 to read back from L2, one wave of blocks each.
 #include "xattn.cuh"
 
 namespace hclsm {

@@ -17,9 +17,9 @@
 // the heads of ONE token, 32 / lanes-per-head at a time: the token's cos and
 // sin (64 bytes a lane) are read once and stay in registers for all its heads.
 // Queries and keys go in one launch, the first warps the queries'.
-// 64 x 2048 tokens, 32 + 8 heads of 64, bf16: 293 us forward (4.6 TB/s; 69 % of the
-// issue slots), 487 us backward (4.1 TB/s; 24 warps an SM keep too few loads in
-// flight; 16 warps: 561 us).
+// 64 x 2048 tokens, 32 + 8 heads of 64, bf16: 284 to 293 us forward (4.6 to 4.7 TB/s; 69 %
+// of the issue slots), 474 to 487 us backward (4.1 to 4.2 TB/s; 24 warps an SM keep too few
+// loads in flight; 16 warps: 561 us).
 #include "common.cuh"
 
 namespace hclsm {

@@ -12,7 +12,7 @@
 // are DP + 8 elements, so that ldmatrix reads every bank once.  One pass over the keys
 // with the running maximum and sum of the softmax.  TM 32 where 64 would leave SMs
 // without a block.  Forward and backward in fp32, 3 x 333 over 777 ragged, 6 heads over 2
-// of 64: 181 us, latency-bound (tensor pipe 24 to 32 % busy, 6 to 8 % of the warps).
+// of 64: 172 us, latency-bound (tensor pipe 24 to 32 % busy, 6 to 8 % of the warps).
 #include "xattn.cuh"
 
 namespace hclsm {
@@ -554,7 +554,7 @@ using namespace hclsm;
 // tiles: a start, and a time a tile of keys (128 on the tensor cores, 64 otherwise) of each wave of blocks.  Fitted
 // to 521 shapes (1 to 64 entries, 1 to 64 heads, 1 to 256 queries over 200 to 16384 keys, heads of 64 and 128, both
 // types): picking by it costs 1.7 % over picking the faster one, always the split form for up to 16 rows and never
-// else 46 %.
+// else 46 %.  Heads of 32 take the constants of 64 and heads of 96 those of 128, without a fit of their own.
 static bool use_split(const xattn::Params& p, int dtype, bool tc) {
   const bool f32 = dtype == HCLSM_F32, small = p.D <= 64;
   const int e = f32 ? 4 : 2;

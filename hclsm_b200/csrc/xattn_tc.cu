@@ -11,8 +11,8 @@
 // 8 (in log2): until then the weights are at most 2^8, which fp32 and bf16 hold
 // with the same relative precision, and O is read back and rescaled rarely.
 // The bound is the softmax's issue and its chain with the products: 4 x 2048 queries
-// over 8192 states, 32 heads of 64, 690 us (797 TFLOP/s), 8 x 2048 over 4096, 16 heads
-// of 128, 435 to 462 us (1190 to 1264 TFLOP/s); tensor pipe 28 and 44 % busy (2 x 2048
+// over 8192 states, 32 heads of 64, 690 to 700 us (785 to 797 TFLOP/s), 8 x 2048 over 4096, 16
+// heads of 128, 435 to 474 us (1160 to 1264 TFLOP/s, by the clock); tensor pipe 28 and 44 % busy (2 x 2048
 // over 4096).
 // While one tile takes its softmax the tensor cores run the other's products.
 #include "xattn_tc.cuh"

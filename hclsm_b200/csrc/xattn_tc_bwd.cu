@@ -16,8 +16,9 @@
 // another.  Two buffers of 64 + 64 columns with warpgroups of their own: the tensor
 // cores form one buffer's products while the other's weights are computed.  A tile of
 // 64 and not 128: 2 x (128 + 128) columns and the accumulators (128 or 256) do not fit
-// TMEM's 512.  8 x 2048 queries over 4096 states, 16 heads of 128 over 4: 1525 to
-// 1560 us, of it 46 % for dq (3 products: 1150 TFLOP/s) and 54 % for dk and dv (4: 1300);
+// TMEM's 512.  4 x 2048 queries over 4096 states, 32 heads of 64: 1269 us.
+// 8 x 2048 queries over 4096 states, 16 heads of 128 over 4: 1525 to 1565 us, of it 46 %
+// for dq (3 products: 1150 TFLOP/s) and 54 % for dk and dv (4: 1300);
 // the tensor pipe is 45 and 56 % busy (2 x 2048 over 4096).  What bounds it is the chain
 // of products, weights and products; and in the second kernel 128 x 64 products with both
 // operands in shared memory, 51 cycles a step of 16 instead of 35.

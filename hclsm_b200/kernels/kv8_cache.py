@@ -50,9 +50,9 @@ class Kv8Cache:
         return {**self.__dict__, "_packed": None}  # a copy's tensors are elsewhere
 
     def _args(self):
-        """(hclsm_kv8_cache, (B, Hkv, T, D), dtype, device, its index) for a call.  A tensor that was assigned, copied or
-        given other memory since the last call is checked and its address taken anew: a kernel only ever sees the memory
-        of the present tensors."""
+        """(hclsm_kv8_cache, (B, Hkv, T, D), dtype, device, its index) for a call.  A tensor that was assigned,
+        copied or given other memory since the last call is checked and its address taken anew: a kernel only ever
+        sees the memory of the present tensors."""
         at = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
               self.k_tail.data_ptr(), self.v_tail.data_ptr())
         packed = self._packed
@@ -79,8 +79,8 @@ class Kv8Cache:
                                           (kt, vt, (B, Hkv, block, D), dtype, "_tail")):
             if (one.shape != shape or two.shape != shape or one.dtype != dt or two.dtype != dt
                     or not one.is_contiguous() or not two.is_contiguous()):
-                raise ValueError(f"k{name} and v{name} must be contiguous {shape} {dt}, got {tuple(one.shape)} {one.dtype}"
-                                 f" and {tuple(two.shape)} {two.dtype}")
+                raise ValueError(f"k{name} and v{name} must be contiguous {shape} {dt}, got {tuple(one.shape)} "
+                                 f"{one.dtype} and {tuple(two.shape)} {two.dtype}")
         return _lib.KV8_CACHE.pack(*at, B, Hkv, T, D, block, _lib.dtype_code(dtype)), (B, Hkv, T, D), dtype, dev, index
 
     @classmethod

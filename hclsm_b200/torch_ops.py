@@ -291,7 +291,7 @@ torch.library.register_autograd(f"{_NS}::cross_attention_fwd", _xattn_backward, 
                          mutates_args=("ck", "cv", "k_scale", "v_scale", "k_tail", "v_tail"))
 def kv8_write(ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, k_tail: Tensor, v_tail: Tensor, k: Tensor,
               v: Tensor, start: Tensor, count: Optional[Tensor]) -> None:
-    if k.requires_grad or v.requires_grad:  # an operator that mutates has no autograd formula, and grad mode is off here
+    if k.requires_grad or v.requires_grad:  # an operator that mutates has no autograd formula; grad mode is off here
         raise NotImplementedError("kv8_write has no gradients: detach k and v")
     _kv8.kv8_write(_kv8.Kv8Cache(ck, cv, k_scale, v_scale, k_tail, v_tail), k, v, start, count)
 
