@@ -85,6 +85,17 @@ SIGNATURES = {
     "hclsm_kv8_read": (ctypes.c_int, [_vp] * 5),
     "hclsm_kv8_attn_workspace_size": (_sz, [_vp, _i32, _i32]),
     "hclsm_kv8_attn": (ctypes.c_int, [_vp] * 4 + [_i32, _i32, ctypes.c_float, _vp, _sz, _vp]),
+    "hclsm_decay_attn_fwd_workspace_size": (_sz, [_vp]),
+    "hclsm_decay_attn_fwd": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "hclsm_decay_attn_bwd_workspace_size": (_sz, [_vp]),
+    "hclsm_decay_attn_bwd": (ctypes.c_int, [_vp, _vp, _sz, _vp]),
+    "hclsm_decay_attn_step": (ctypes.c_int, [_vp, _vp, _vp]),
+    "hclsm_kv4_write": (ctypes.c_int, [_vp] * 4 + [_i32, _i32, _vp]),
+    "hclsm_kv4_read": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "hclsm_kv4_attn_workspace_size": (_sz, [_vp, _i32, _i32, _i32, _i32]),
+    "hclsm_kv4_attn": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, ctypes.c_float, _vp, _sz, _vp]),
+    "hclsm_pages_resize": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
+    "hclsm_page_slots": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp]),
     "hclsm_ssm_scan_bwd_noalloc_max_scratch": (_sz, []),
     "hclsm_ssm_scan_bwd_noalloc": (ctypes.c_int, [_vp] * 15 + [_i64, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
@@ -96,6 +107,8 @@ VIEW = struct.Struct("@Pqqq")                     # hclsm_view
 ROPE_SIDE = struct.Struct("@6P3q2i")              # hclsm_rope_side
 XATTN_ARGS = struct.Struct("@" + 4 * "Pqqq" + "8Pq7if")  # hclsm_xattn_args
 KV8_CACHE = struct.Struct("@6P6i")                # hclsm_kv8_cache
+DECAY_ARGS = struct.Struct("@" + 4 * "Pqqq" + "10P6if")  # hclsm_decay_args
+KV4_CACHE = struct.Struct("@4P5i")                # hclsm_kv4_cache
 
 
 class SlotIterWeights(ctypes.Structure):

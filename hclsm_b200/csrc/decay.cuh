@@ -1,0 +1,87 @@
+// Linear attention whose state forgets at a rate of each head.
+//
+//   S_t = g S_{t-1} + k_t^T v_t,   o_t = scale q_t S_t,   g = exp(log_decay) in [0, 1],   S_{-1} the given state or 0
+//
+// Everything is one kind of pass over x, k, v (rows of a head's tokens) in either direction of time:
+//
+//   T <- g T + k_t^T v_t,   y_t = f x_t T      t ascending or, reversed, descending from the last valid token
+//
+//   forward:  (x, k, v) = (q, k, v), ascending from S_{-1}, f = scale; T ends as the new state
+//   dq:       (dO, v, k), ascending from S_{-1}^T
+//   dv:       (k, q, dO), descending from dS / scale, where the first token meets T without a decay, and T
+//             ends as g T = dS_{-1} / scale
+//   dk:       (v, dO, q), descending from dS^T / scale
+//
+// By chunks of C tokens, i and j a token's place among the m valid ones in the pass's order and r = 1 where reversed:
+//
+//   y_i = f [ sum_{j <= i} g^{i-j} (x_i . k_j) v_j  +  g^{i+1-r} x_i T ],   T <- g^m T + sum_j g^{m-1-j+r} k_j^T v_j
+//
+// Chunks lie on multiples of C in memory in both directions, so the incomplete one is the last one.  Where the heads
+// do not fill the GPU their tokens are cut into segments of whole chunks: the segments' own sums (sums pass), their
+// running combination (join kernel), then the segments side by side, each from its own state.
+#pragma once
+#include "xattn.cuh"
+
+namespace hclsm {
+namespace decay {
+
+using xattn::View;
+
+struct Pass {
+  View x, k, v;               // (B, L, H, Dk), (B, L, H, Dk), (B, L, H, Dv), innermost dense
+  void* y;                    // dense (B, L, H, Dv)
+  const float* log_decay;     // (H)
+  const float* init;          // (B, H, Dk, Dv), or transposed, or null
+  float* last;                // the same for the final state
+  const int32_t* lens;        // (B) or null
+  float* part;                // (B * H, segs, Dk, Dv): sums, then the segments' first states
+  int init_t;                 // init is (B, H, Dv, Dk)
+  float init_f, last_f, f;    // factors of init, last and y
+  int rev;
+  int B, L, H, Dk, Dv;
+  int segs, seg_chunks;       // segments a head, chunks of a segment
+  int* err;
+};
+
+// log2 of a head's decay, at most 0 (NaN stays); -inf would be NaN where the exponent is 0.
+__device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
+  float l = log_decay[h] * kLog2e;
+  l = l > 0.0f ? 0.0f : l;
+  return l < -1e30f ? -1e30f : l;
+}
+// g^n.  A chunk's factor meets the state once a chunk, so its error adds up over as many chunks as the head remembers:
+// in 64 bits, as two fp32 parts.
+__device__ __forceinline__ float2 chunk_decay(const float* log_decay, int h, int n) {
+  double l = (double)log_decay[h];
+  l = l > 0.0 ? 0.0 : l;
+  l = l < -1e30 ? -1e30 : l;
+  const double g = exp(l * n);
+  const float hi = (float)g;
+  return make_float2(hi, (float)(g - (double)hi));
+}
+__device__ __forceinline__ int length(const Pass& p, int64_t b) {
+  return p.lens ? min(max(p.lens[b], 0), p.L) : p.L;
+}
+
+// Segments of a head: enough blocks for two a SM, whole chunks of `chunk` tokens, at least four chunks each.
+inline void cut(Pass& p, int chunk, int blocks_per_head) {
+  const int chunks = (p.L + chunk - 1) / chunk;
+  const int64_t have = (int64_t)p.B * p.H * blocks_per_head, want = 2 * (int64_t)num_sms();
+  int64_t segs = have > 0 ? (want + have - 1) / have : 1;
+  const int64_t most = chunks / 4 > 1 ? chunks / 4 : 1;
+  segs = segs < most ? segs : most;
+  p.seg_chunks = (int)((chunks + segs - 1) / segs);
+  if (p.seg_chunks < 1) p.seg_chunks = 1;
+  p.segs = (chunks + p.seg_chunks - 1) / p.seg_chunks;
+  if (p.segs < 1) p.segs = 1;
+}
+
+int join(const Pass& p, int chunk, cudaStream_t st);
+
+// bf16 on the 5th-generation tensor cores (decay_tc.cu), where tc_ok.
+bool tc_ok(const Pass& p);
+size_t tc_part_bytes(Pass p);
+int tc_pass(Pass p, cudaStream_t st);
+
+}  // namespace decay
+}  // namespace hclsm

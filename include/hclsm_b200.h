@@ -436,6 +436,81 @@ size_t hclsm_kv8_attn_workspace_size(const hclsm_kv8_cache* c, int32_t Lq, int32
 int hclsm_kv8_attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const int32_t* lens,
                    int32_t Lq, int32_t H, float scale, void* ws, size_t ws_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Memories of a history of states: linear attention whose state forgets at a
+ * rate of each head, and a 4-bit cache of states in pages that many sequences
+ * share, with the tables of its pages.  The reference has no counterpart.
+ *
+ *   S_t = g S_{t-1} + k_t^T v_t,  o_t = scale q_t S_t,  g = exp(log_decay[h])
+ *
+ * q, k (B, L, H, D), v (B, L, H, Dv), heads dense, D and Dv up to 128; o and the gradients dense.
+ * log_decay (H) fp32 counts as 0 where above.  s0 (B, H, D, Dv) fp32 or NULL (zeros): the state
+ * before the first token; s1 or NULL: the state behind the last.  lens (B) or NULL: an
+ * entry's first lens[b] tokens count; the others are not operands, and their o and
+ * gradients are zeros.  Backward: dout, ds1 (of s1, or NULL) give dq, dk, dv and ds0 (or NULL).
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  hclsm_view q, k, v, dout;
+  void *o, *dq, *dk, *dv;
+  const float* log_decay;
+  const float* s0;
+  float* s1;
+  const float* ds1;
+  float* ds0;
+  const int32_t* lens;
+  int32_t B, L, H, D, Dv, dtype;
+  float scale; /* positive */
+} hclsm_decay_args;
+
+size_t hclsm_decay_attn_fwd_workspace_size(const hclsm_decay_args* a);
+int hclsm_decay_attn_fwd(const hclsm_decay_args* a, void* ws, size_t ws_bytes, void* stream);
+size_t hclsm_decay_attn_bwd_workspace_size(const hclsm_decay_args* a);
+int hclsm_decay_attn_bwd(const hclsm_decay_args* a, void* ws, size_t ws_bytes, void* stream);
+/* One token of each sequence (L 1; the views' st is not used): s1, which may be s0, becomes the
+ * state with the token, o (B, H, Dv) its output.  active (B) or NULL: where 0 the state stays and o is zero. */
+int hclsm_decay_attn_step(const hclsm_decay_args* a, const uint8_t* active, void* stream);
+
+/* The 4-bit state cache: `pages` pages of `page` tokens for every key head.  Groups of 32 dims share a bf16 scale:
+ * the value of largest magnitude (the positive one where both signs have it) over -8; a value is held as
+ * the nearest whole number of value / scale in [-8, 7] (halves to even), plus 8.  A group that is not finite
+ * has scale NaN.  A token's codes are D / 8 words of 32 bits, dims ascending from the low bits in runs
+ * of four: word w of each 64 dims holds dims 4 w to 4 w + 3 and 4 w + 32 to 4 w + 35, 32 dims behind the last 64
+ * follow in order.  D 32, 64, 96 or 128; page 16, 32, 64 or 128; pages * page below 2^31. */
+typedef struct {
+  uint8_t *k, *v;            /* (pages, Hkv, page, D / 2) */
+  uint16_t *k_scale, *v_scale; /* bf16 (pages, Hkv, page, D / 32) */
+  int32_t pages, Hkv, page, D, dtype; /* dtype of the states written and read */
+} hclsm_kv4_cache;
+
+/* Token i of entry b of k, v (B, n, Hkv, D; rows start on 16 bytes) goes to slots[b, i] = page number * page + place;
+ * negative slots are left out, one behind the cache is left out and puts HCLSM_ERR_SHAPE in the error
+ * word.  Slots of one call differ. */
+int hclsm_kv4_write(const hclsm_kv4_cache* c, const hclsm_view* k, const hclsm_view* v, const int32_t* slots,
+                    int32_t B, int32_t n, void* stream);
+/* The first lens[b] tokens (NULL: M * page) of the pages table (B, M) names, dense (B, M * page, Hkv, D), zeros after
+ * them.  A page outside the cache below the length reads as zeros and puts HCLSM_ERR_SHAPE in the error word. */
+int hclsm_kv4_read(const hclsm_kv4_cache* c, const int32_t* table, int32_t B, int32_t M, void* k, void* v,
+                   const int32_t* lens, void* stream);
+/* Attention of q (B, Lq, H, D) over them; o dense; an entry without tokens gives 0, and tokens of pages
+ * outside the cache do not count (HCLSM_ERR_SHAPE in the error word). */
+size_t hclsm_kv4_attn_workspace_size(const hclsm_kv4_cache* c, int32_t B, int32_t M, int32_t Lq, int32_t H);
+int hclsm_kv4_attn(const hclsm_kv4_cache* c, const int32_t* table, int32_t B, int32_t M, const hclsm_view* q, void* o,
+                   const int32_t* lens, int32_t Lq, int32_t H, float scale, void* ws, size_t ws_bytes,
+                   void* stream);
+
+/* Page tables.  table (B, M): the pages of each entry in order, -1 behind them; stack (P): the free pages are its first
+ * *n_free places.  Entries that held old_lens[b] tokens now hold new_lens[b]: the pages this releases go onto the stack,
+ * the first of them (entries, then places ascending) on top; then the pages it wants come off its top. Places that are
+ * taken off or released hold -1.  A request that cannot be met (lengths outside [0, M * page], not
+ * enough free pages, pages outside [0, P)) changes nothing and puts HCLSM_ERR_SHAPE in the error word.
+ * page: a power of two. */
+int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P, int32_t page,
+                       const int32_t* old_lens, const int32_t* new_lens, void* stream);
+/* slots (B, n): of tokens start[b], start[b] + 1, ...; -1 behind the first count[b] (NULL: n) of them and where the
+ * table has no page. */
+int hclsm_page_slots(const int32_t* table, int32_t B, int32_t M, int32_t page, const int32_t* start,
+                     const int32_t* count, int32_t n, int32_t* slots, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
