@@ -411,10 +411,11 @@ Pass grad_k(const hclsm_decay_args* a) {
 }
 
 size_t part_bytes(const Pass& p, int dtype) {
-  return (simt_part_bytes(p) + 15) & ~(size_t)15;
+  return dtype == HCLSM_BF16 && tc_ok(p) ? tc_part_bytes(p) : simt_part_bytes(p);
 }
 int pass(Pass p, int dtype, void* ws, cudaStream_t st) {
   p.part = static_cast<float*>(ws);
+  if (dtype == HCLSM_BF16 && tc_ok(p)) return tc_pass(p, st);
   return dtype == HCLSM_F32 ? simt_pass<float>(p, st) : simt_pass<__nv_bfloat16>(p, st);
 }
 size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
