@@ -281,7 +281,7 @@ int launch_simt(const Pass& p, cudaStream_t st) {
 
 template <typename T>
 int simt_pass(Pass p, cudaStream_t st) {
-  cut(p, kC, (p.Dv + kE - 1) / kE);
+  cut(p, kC, (int64_t)p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
   if (p.segs > 1) {
     if (const int rc = p.Dk <= 64 ? launch_simt<T, 64, true>(p, st) : launch_simt<T, 128, true>(p, st)) return rc;
     if (const int rc = join(p, kC, st)) return rc;
@@ -290,7 +290,7 @@ int simt_pass(Pass p, cudaStream_t st) {
 }
 
 size_t simt_part_bytes(Pass p) {
-  cut(p, kC, (p.Dv + kE - 1) / kE);
+  cut(p, kC, (int64_t)p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
   return p.segs > 1 ? (size_t)p.B * p.H * p.segs * p.Dk * p.Dv * sizeof(float) : 0;
 }
 

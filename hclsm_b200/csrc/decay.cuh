@@ -43,11 +43,12 @@ struct Pass {
   int* err;
 };
 
-// log2 of a head's decay, at most 0 (NaN stays); -inf would be NaN where the exponent is 0.
+// log2 of a head's decay, at most 0 (NaN stays).  Where it is below -200 (-inf, which would be NaN where the exponent is
+// 0) one token forgets all in fp32 either way.
 __device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
   float l = log_decay[h] * kLog2e;
   l = l > 0.0f ? 0.0f : l;
-  return l < -1e30f ? -1e30f : l;
+  return l < -200.0f ? -200.0f : l;
 }
 // g^n.  A chunk's factor meets the state once a chunk, so its error adds up over as many chunks as the head remembers:
 // in 64 bits, as two fp32 parts.
@@ -63,13 +64,13 @@ __device__ __forceinline__ int length(const Pass& p, int64_t b) {
   return p.lens ? min(max(p.lens[b], 0), p.L) : p.L;
 }
 
-// Segments of a head: enough blocks for two a SM, whole chunks of `chunk` tokens, at least four chunks each.
-inline void cut(Pass& p, int chunk, int blocks_per_head) {
+// Segments of a head where the heads would leave more than half of the `room` blocks that run at once idle: whole chunks
+// of `chunk` tokens, at least four each.
+inline void cut(Pass& p, int chunk, int64_t have, int64_t room) {
   const int chunks = (p.L + chunk - 1) / chunk;
-  const int64_t have = (int64_t)p.B * p.H * blocks_per_head, want = 2 * (int64_t)num_sms();
-  int64_t segs = have > 0 ? (want + have - 1) / have : 1;
-  const int64_t most = chunks / 4 > 1 ? chunks / 4 : 1;
-  segs = segs < most ? segs : most;
+  int64_t segs = have > 0 ? room / have : 1;
+  if (segs > chunks / 4) segs = chunks / 4;
+  if (segs < 1) segs = 1;
   p.seg_chunks = (int)((chunks + segs - 1) / segs);
   if (p.seg_chunks < 1) p.seg_chunks = 1;
   p.segs = (chunks + p.seg_chunks - 1) / p.seg_chunks;

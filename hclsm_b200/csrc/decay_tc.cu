@@ -4,11 +4,12 @@
 //   A = x k^T                 128 x 128, fp32 in TMEM
 //   P = A g^|i-j| as bf16 over A (the A operand of the next product), zero outside the pass's past
 //   y = f (P v + g^{i+1-r} x T)   two accumulators, joined by the thread of the row
-//   T = g^m T + k^T (w v)     fp32 in TMEM, w_j = g^{m-1-j+r}
-// The state is returned in fp32, so w v (or w k, whichever is narrower) is not rounded to bf16: it enters as NP = 3
-// bf16 pieces (2 where the state is only read by later chunks), each exact product summed in fp32.  For x T the state
-// is rounded to bf16 once, as P is.
-// Two warps issue: TMA and MMA.  NWG warpgroups do the rest, a thread a row (token, or row of T) and NWG its columns.
+//   T = g^m T + (w k)^T v     the product in TMEM, T in registers in fp32, w_j = g^{m-1-j+r}
+// The state is returned in fp32, so w k is not rounded to bf16: it enters as NP = 3 bf16 pieces (2 where the state is
+// only read by later chunks), smallest first.  The tensor cores cut fp32 sums off instead of rounding them, always
+// towards zero: so only a chunk's sum is theirs, and chunks are added in registers.  For x T the state is rounded
+// to bf16 once, as P is.
+// Warps: TMA, MMA, warpgroups of the state (weighted pieces of k, T) and warpgroups of the rows (P, y).
 #include "decay.cuh"
 #include "xattn_tc.cuh"
 
@@ -25,22 +26,35 @@ constexpr int kTok = 128;                     // tokens of a chunk
 constexpr int kBlock = kTok * (int)kRowBytes; // 64 dims of a staged tile
 
 template <int DX, int DY, int NP> struct Shape {
-  static constexpr bool kScaleV = DY <= DX;   // the operand of the state's update that takes the weights
-  static constexpr int kNwg = DX == 64 && DY == 64 ? 1 : 2;
+  static constexpr bool kSmall = DX == 64 && DY == 64;
+  static constexpr int kWg = kSmall ? 1 : 2;  // warpgroups of each kind: columns are shared out among them
   static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
-  static constexpr int kPiece = kScaleV ? kV : kX;
   static constexpr int kT = DY / 64 * DX * (int)kRowBytes;  // bf16 copy of the state
-  static constexpr int kBars = 10;
-  static constexpr size_t kBytes = 2 * kX + kV + NP * kPiece + kT + 1024;
-  static constexpr int kThreads = kNwg * 128 + 64;
-  static constexpr uint32_t kColY = 128, kColXt = DY == 64 ? 64 : 256, kColT = DY == 64 ? 192 : 384;
-  static constexpr uint32_t kCols = DY == 64 ? 256 : 512;
-  static constexpr int kPerSm = DX == 64 && DY == 64 ? 2 : 1;
+  static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + 1024;
+  static constexpr int kThreads = 2 * kWg * 128 + 64;
+  static constexpr uint32_t kColY = 128, kColXt = kSmall ? 64 : 256, kColT = kSmall ? 192 : 384;
+  static constexpr uint32_t kCols = kSmall ? 256 : 512;
+  static constexpr int kPerSm = kSmall ? 2 : 1;
 };
 
-// Bytes of 16-byte piece c of row r of a tile of `rows` rows, 64 dims (8 pieces) a block, 128-byte swizzle.
-__device__ __forceinline__ int swizzled(int rows, int r, int c) {
-  return ((c >> 3) * rows + r) * (int)kRowBytes + (((c & 7) ^ (r & 7)) << 4);
+// 16-byte piece c of row r of a tile of ROWS rows: 64 dims (8 pieces) a block, 128-byte swizzle.  32-bit addresses that are
+// formed where they are used: as pointers, kept over the loop, they cost the state's threads their registers.
+template <int ROWS> struct RowAt {
+  uint32_t base, turn;
+  __device__ __forceinline__ RowAt(uint32_t tile, int r) : base(tile + (uint32_t)r * kRowBytes), turn((uint32_t)(r & 7) << 4) {
+    asm volatile("" : "+r"(base), "+r"(turn));
+  }
+  __device__ __forceinline__ uint32_t operator()(int c) const {
+    return base + (uint32_t)(c >> 3) * (ROWS * kRowBytes) + (((uint32_t)(c & 7) << 4) ^ turn);
+  }
+};
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 __device__ __forceinline__ void store32(__nv_bfloat16* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
@@ -48,24 +62,73 @@ __device__ __forceinline__ void store32(__nv_bfloat16* p, const uint32_t (&w)[8]
                : "memory");
 }
 
+// 8 columns of this warp's lanes: the state's threads have no registers for more beside T.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(taddr));
+  tmem_wait_ld();
+  tmem_pin<8>(v);
+}
+
+// NP bf16 pieces of w times a row's dims [8 c0, 8 (c0 + N)), to the same place of the tile at `to` and NP - 1 tiles of
+// `step` bytes behind.
+template <int NP, int N>
+__device__ __forceinline__ void weigh_row(uint32_t from, uint32_t to, int step, int row, int c0, float w) {
+  const RowAt<kTok> at(from, row);
+  uint4 raw[N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) raw[c] = ld_shared(at(c0 + c));
+#pragma unroll
+  for (int c = 0; c < N; ++c) {
+    const uint32_t in[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
+    uint32_t q[NP][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float2 v = mul2(make_float2(__uint_as_float(in[e] << 16), __uint_as_float(in[e] & 0xffff0000u)), make_float2(w, w));
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint32_t t = q[i][e] = pack_bf16(v.x, v.y);
+        if (i + 1 < NP)
+          v = fma2(make_float2(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u)), make_float2(-1.0f, -1.0f), v);
+      }
+    }
+    const uint32_t dst = at(c0 + c) + (to - from);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) st_shared(dst + i * step, q[i][0], q[i][1], q[i][2], q[i][3]);
+  }
+}
+// Zeros for a row behind the length, which is no operand whatever it holds: dims [8 c0, 8 c1) of the n tiles from `to`, `step`
+// bytes apart.
+__device__ __forceinline__ void clear_row(uint32_t to, int step, int n, int row, int c0, int c1) {
+#pragma unroll 1
+  for (int i = 0; i < n; ++i)
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) st_shared(RowAt<kTok>(to + i * step, row)(c), 0, 0, 0, 0);
+}
+
 template <int DX, int DY, int NP>
 __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>::kPerSm)
     tc_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mk,
               const __grid_constant__ CUtensorMap mv, const __grid_constant__ Pass p) {
   using Sh = Shape<DX, DY, NP>;
-  constexpr int NWG = Sh::kNwg;
+  constexpr int WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *sX = smem, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sP = sV + Sh::kV, *sT = sP + NP * Sh::kPiece;
+  // with 64 dims the update's products read 64 rows behind a piece of k, for rows of the result that nobody reads: the
+  // pieces come first
+  unsigned char *sP = smem, *sX = sP + NP * Sh::kX, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sT = sV + Sh::kV;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ __align__(16) float s_pow[32];  // g^n
-  __shared__ uint64_t bars[Sh::kBars];
-  uint64_t *xk_full = bars, *v_full = bars + 1, *s_full = bars + 2, *p_ready = bars + 3, *t_ready = bars + 4,
-           *y_done = bars + 5, *x_free = bars + 6, *t_done = bars + 7, *read = bars + 8, *drain = bars + 9;
+  __shared__ __align__(16) float s_pow[32];  // g^(distance of a block's j to its end on the later side)
+  constexpr int kBars = 12;
+  __shared__ uint64_t bars[kBars];
+  uint64_t *x_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_ready = bars + 4,
+           *t_ready = bars + 5, *y_done = bars + 6, *y_free = bars + 7, *x_free = bars + 8, *t_done = bars + 9,
+           *w_ready = bars + 10, *drain = bars + 11;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = NWG * 4, kMmaWarp = NWG * 4 + 1;
+  constexpr int kTmaWarp = WG * 8, kMmaWarp = WG * 8 + 1;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(Sh::kCols)
@@ -74,7 +137,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   }
   if (tid == 0) {
     s_abort = 0;
-    for (uint64_t* b = bars; b < bars + Sh::kBars; ++b) mbar_init(b, b == p_ready || b == t_ready || b == read ? NWG * 128 : 1);
+    for (uint64_t* b = bars; b < bars + kBars; ++b)
+      mbar_init(b, b == p_ready || b == t_ready || b == w_ready || b == y_free ? WG * 128 : 1);
     fence_mbar_init();
   }
   pdl_wait();
@@ -84,7 +148,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   const int h = (int)(bh - b * p.H), r = p.rev ? 1 : 0;
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
-  if (tid < 32) s_pow[tid] = ex2(l2 * (float)tid);
+  if (tid < 32) s_pow[tid] = ex2(l2 * (float)(r ? tid : 31 - tid));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -96,21 +160,23 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
   auto first_token = [&](int it) { return (p.rev ? c_lo + chunks - 1 - it : c_lo + it) * kTok; };
   const bool state_out = p.segs == 1 && p.last;
+  const int64_t sz = (int64_t)p.Dk * p.Dv;
 
-  int asked_xk = 0, asked_v = 0;  // copies (lane 0 of the TMA warp)
+  int asked_x = 0, asked_k = 0, asked_v = 0;  // copies (lane 0 of the TMA warp)
   if (warp == kTmaWarp) {
     if (lane == 0) {
       for (int it = 0; it < chunks; ++it) {
         const int t0 = first_token(it);
+        // in the order in which the chunk before gives them up
+        if (it > 0 && (!wait(s_full, it - 1) || !wait(w_ready, it - 1))) break;
+        mbar_expect_tx(k_full, Sh::kX);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &mk, d * 64, t0, h, (int)b, k_full);
+        asked_k = it + 1;
         if (it > 0 && !wait(x_free, it - 1)) break;
-        mbar_expect_tx(xk_full, 2 * Sh::kX);
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sX + d * kBlock, &mx, d * 64, t0, h, (int)b, xk_full);
-        asked_xk = it + 1;
-        // given up between the two: k is asked for all the same, so that the barrier's bytes arrive
-        const bool ok = it == 0 || wait(t_done, it - 1);
-        if (!ok) mbar_wait(t_done, (it - 1) & 1);
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &mk, d * 64, t0, h, (int)b, xk_full);
-        if (!ok) break;
+        mbar_expect_tx(x_full, Sh::kX);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sX + d * kBlock, &mx, d * 64, t0, h, (int)b, x_full);
+        asked_x = it + 1;
+        if (it > 0 && !wait(y_done, it - 1)) break;  // behind the state's update as well
         mbar_expect_tx(v_full, Sh::kV);
         for (int d = 0; d < DY / 64; ++d) tma_load_4d(sV + d * kBlock, &mv, d * 64, t0, h, (int)b, v_full);
         asked_v = it + 1;
@@ -124,14 +190,11 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
     const uint64_t d_x = smem_desc_sw128(smem_u32(sX), 16, 1024), d_k = smem_desc_sw128(smem_u32(sK), 16, 1024),
                    d_v = smem_desc_sw128(smem_u32(sV), kBlock, 1024),
                    d_t = smem_desc_sw128(smem_u32(sT), DX * kRowBytes, 1024),
-                   d_kt = smem_desc_sw128(smem_u32(sK), kBlock, 1024),
                    d_p = smem_desc_sw128(smem_u32(sP), kBlock, 1024);
     for (int it = 0; it < chunks; ++it) {
-      if (!wait_all(xk_full, it)) break;
-      tc_fence_after();
-      // Over the chunk before's weights (products run in order) and, with 64 value dims, its x T: a row's thread has
-      // read that when it arrives on t_ready.
-      if (DY == 64 && it > 0 && !wait_all(t_ready, it)) break;
+      if (!wait_all(k_full, it) || !wait_all(x_full, it)) break;
+      // over the chunk before's weights (products run in order) and, where TMEM is short, its x T
+      if (Sh::kSmall && it > 0 && !wait_all(y_free, it - 1)) break;
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < DX / 16; ++k) {
@@ -139,224 +202,228 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         if (k < kx) umma_ss(one, tmem, desc_at(d_x, off), desc_at(d_k, off), id_s, k != 0);
       }
       umma_done(one, s_full);
-      if (!wait_all(v_full, it) || !wait_all(t_ready, it) || !wait_all(p_ready, it)) break;
+      auto read_state = [&] {
+#pragma unroll
+        for (int k = 0; k < DX / 16; ++k)
+          if (k < kx)
+            umma_ss(one, tmem + Sh::kColXt, desc_at(d_x, (k >> 2) * kBlock + (k & 3) * 32),
+                    desc_at(d_t, k * 16 * kRowBytes), id_y, k != 0);
+        umma_done(one, x_free);
+      };
+      if constexpr (!Sh::kSmall) {
+        // y_free: the row's threads have read the chunk before's
+        if (!wait_all(t_ready, it) || (it > 0 && !wait_all(y_free, it - 1))) break;
+        tc_fence_after();
+        read_state();
+      }
+      if (!wait_all(w_ready, it) || !wait_all(v_full, it)) break;
       tc_fence_after();
 #pragma unroll
-      for (int k = 0; k < DX / 16; ++k)
-        if (k < kx)
-          umma_ss(one, tmem + Sh::kColXt, desc_at(d_x, (k >> 2) * kBlock + (k & 3) * 32),
-                  desc_at(d_t, k * 16 * kRowBytes), id_y, k != 0);
-      umma_done(one, x_free);
+      for (int i = NP - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = 0; k < kTok / 16; ++k)
+          umma_ss(one, tmem + Sh::kColT, desc_at(d_p, i * Sh::kX + k * 16 * kRowBytes), desc_at(d_v, k * 16 * kRowBytes),
+                  id_t, !(i == NP - 1 && k == 0));
+      umma_done(one, t_done);
+      if (!wait_all(p_ready, it)) break;
+      if (Sh::kSmall && !wait_all(t_ready, it)) break;
+      tc_fence_after();
+      if constexpr (Sh::kSmall) read_state();
 #pragma unroll
       for (int k = 0; k < kTok / 16; ++k)
-        umma_ts(one, tmem + Sh::kColY, tmem + k * 8, desc_at(d_v, k * 16 * kRowBytes), id_y, k != 0);
+        umma_ts(one, tmem + Sh::kColY, tmem + k * 8 + (WG == 2 && k >= 4 ? 32 : 0), desc_at(d_v, k * 16 * kRowBytes), id_y,
+                k != 0);
       umma_done(one, y_done);
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int k = 0; k < kTok / 16; ++k) {
-          const uint64_t pd = desc_at(d_p, i * Sh::kPiece + k * 16 * kRowBytes);
-          umma_ss(one, tmem + Sh::kColT, Sh::kScaleV ? desc_at(d_kt, k * 16 * kRowBytes) : pd,
-                  Sh::kScaleV ? pd : desc_at(d_v, k * 16 * kRowBytes), id_t, 1);
-        }
-      umma_done(one, t_done);
     }
-  } else {
-    const int row = tid & 127, half = tid >> 7;  // token, or row of the state; columns of this warpgroup
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lanes, tY = tS + Sh::kColY, tX = tS + Sh::kColXt, tT = tS + Sh::kColT;
-    constexpr int kYCols = DY / NWG, kPDims = (Sh::kScaleV ? DY : DX) / NWG, kBlocks = 4 / NWG;
-    const int y0 = half * kYCols;
-    const bool holds_t = (warp & 3) * 32 < DX;  // this warp's lanes are rows of the state
-    const float2 whole = chunk_decay(p.log_decay, h, kTok);
-    const int64_t sz = (int64_t)p.Dk * p.Dv;
-    bool ok = true;
-    if (holds_t) {
+  } else if (warp < WG * 4) {
+    // ---- the state --------------------------------------------------------------------------
+    const int row = tid & 127, half = tid >> 7;  // token, or row of T; columns of this warpgroup
+    constexpr int kCols = DY / WG, kDims = DX / WG;
+    const int y0 = half * kCols;
+    const bool holds = (warp & 3) * 32 < DX;  // this warp's lanes are rows of T
+    const uint32_t tT = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::kColT + y0;
+    // of a whole chunk and of the incomplete one (or of no token); not in the loop, where T fills the registers
+    const float2 whole = chunk_decay(p.log_decay, h, kTok), cut_off = chunk_decay(p.log_decay, h, n % kTok);
+    float2 T[kCols / 2];
+#pragma unroll
+    for (int e = 0; e < kCols / 2; ++e) T[e] = make_float2(0.0f, 0.0f);
+    if (holds) {  // the first state as if a chunk's sum
+      const float* from = p.segs > 1 ? p.part + (bh * p.segs + seg) * sz : p.init ? p.init + bh * sz : nullptr;
+      const bool turned = p.segs == 1 && p.init_t;
+      const int64_t at = turned ? row + (int64_t)y0 * p.Dk : (int64_t)row * p.Dv + y0, step = turned ? p.Dk : 1;
+      const float f = p.segs > 1 ? 1.0f : p.init_f;
 #pragma unroll 1
-      for (int c = 0; c < kYCols; c += 16) {
+      for (int c = 0; c < kCols; c += 16) {
         uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = y0 + c + e;
-          float v = 0.0f;
-          if (row < p.Dk && col < p.Dv) {
-            if (p.segs > 1) v = p.part[(bh * p.segs + seg) * sz + (int64_t)row * p.Dv + col];
-            else if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? (int64_t)col * p.Dk + row : (int64_t)row * p.Dv + col)];
-          }
-          w[e] = __float_as_uint(v);
-        }
-        tmem_st16(tT + y0 + c, w);
+        for (int e = 0; e < 16; ++e)
+          w[e] = from && row < p.Dk && y0 + c + e < p.Dv ? __float_as_uint(f * from[at + (c + e) * step]) : 0u;
+        tmem_st16(tT + c, w);
       }
       tmem_wait_st();
     }
-    for (int it = 0; it < chunks && ok; ++it) {
-      const int t0 = first_token(it), m = min(n - t0, kTok);
-      const int place = p.rev ? m - 1 - row : row;
-      // ---- the state: its bf16 copy, then times the chunk's decay
-      if (it > 0) {
-        if (!(ok = wait_all(t_done, it - 1))) break;
-        tc_fence_after();
-      }
-      if (holds_t) {
-        const float2 g = m == kTok ? whole : chunk_decay(p.log_decay, h, m);
-#pragma unroll 1
-        for (int c = 0; c < kYCols; c += 16) {
-          float v[16];
-          tmem_ld16_nowait(tT + y0 + c, v);
-          tmem_wait_ld();
-          tmem_pin<16>(v);
-          uint32_t w[16], q[8];
+    // T behind m more tokens, whose products are complete
+    auto advance = [&](int m) {
+      tc_fence_after();
+      const float2 g = m == kTok ? whole : cut_off;
+      if (!holds) return;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      for (int c = 0; c < kCols; c += 8) {
+        float v[8];
+        tmem_ld8(tT + c, v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(fmaf(v[e], g.x, v[e] * g.y));
-          tmem_st16(tT + y0 + c, w);
-          const int at = (y0 + c) / 8;
-          *reinterpret_cast<uint4*>(sT + swizzled(DX, row, at)) = make_uint4(q[0], q[1], q[2], q[3]);
-          *reinterpret_cast<uint4*>(sT + swizzled(DX, row, at + 1)) = make_uint4(q[4], q[5], q[6], q[7]);
+        for (int e = 0; e < 4; ++e) {
+          float2& t = T[c / 2 + e];
+          t = fma2(t, make_float2(g.x, g.x), fma2(t, make_float2(g.y, g.y), make_float2(v[2 * e], v[2 * e + 1])));
         }
-        tmem_wait_st();
       }
-      // ---- the weighted operand of the state's update; rows behind the length are no operands
-      if (!(ok = wait_all(xk_full, it) && wait_all(v_full, it))) break;
-      if (row >= m) {
-        for (int c = half; c < DX / 8; c += NWG) *reinterpret_cast<uint4*>(sK + swizzled(kTok, row, c)) = make_uint4(0, 0, 0, 0);
-        for (int c = half; c < DY / 8; c += NWG) *reinterpret_cast<uint4*>(sV + swizzled(kTok, row, c)) = make_uint4(0, 0, 0, 0);
-      }
-      {
-        const float w = ex2(l2 * (float)(m - 1 - place + r));
-        const unsigned char* from = Sh::kScaleV ? sV : sK;
-#pragma unroll 2
-        for (int c = half * (kPDims / 8); c < (half + 1) * (kPDims / 8); ++c) {
-          const int at = swizzled(kTok, row, c);
-          uint32_t q[NP][4] = {};
-          if (row < m) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(from + at);
-            const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+    };
+    bool ok = true;
+    int m = kTok;  // tokens of the chunk before (the first state: T is zero)
+    for (int it = 0; it < chunks && ok; ++it) {
+      if (it > 0 && !(ok = wait_all(t_done, it - 1))) break;
+      advance(m);
+      m = min(n - first_token(it), kTok);
+      if (it > 0 && !(ok = wait_all(x_free, it - 1))) break;  // the bf16 copy has been read
+      if (holds) {
+        const RowAt<DX> at(smem_u32(sT), row);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float lo = __uint_as_float(in[e] << 16) * w, hi = __uint_as_float(in[e] & 0xffff0000u) * w;
+        for (int c = 0; c < kCols; c += 8) {
+          uint32_t q[4];
 #pragma unroll
-              for (int i = 0; i < NP; ++i) {
-                q[i][e] = pack_bf16(lo, hi);
-                lo -= __uint_as_float(q[i][e] << 16), hi -= __uint_as_float(q[i][e] & 0xffff0000u);
-              }
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < NP; ++i)
-            *reinterpret_cast<uint4*>(sP + i * Sh::kPiece + at) = make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]);
+          for (int e = 0; e < 4; ++e) q[e] = pack_bf16(T[c / 2 + e].x, T[c / 2 + e].y);
+          st_shared(at(y0 / 8 + c / 8), q[0], q[1], q[2], q[3]);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
       mbar_arrive(t_ready);
-      // ---- P
+      if (!(ok = wait_all(k_full, it))) break;
+      const int c0 = half * (kDims / 8);
+      const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
+#pragma unroll 1
+      for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
+      if (m < kTok) {
+        if (!(ok = wait_all(v_full, it))) break;
+        if (row >= m) {
+          clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
+          clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(w_ready);
+    }
+    if (ok && chunks > 0) {
+      ok = wait_all(t_done, chunks - 1);
+      if (state_out && ok) advance(m);
+    } else if (state_out && ok) {
+      advance(kTok);  // no token: the first state alone
+    }
+    if (state_out && ok && row < p.Dk) {
+      float* to = p.last + bh * sz + (int64_t)row * p.Dv + y0;
+#pragma unroll
+      for (int e = 0; e < kCols; e += 4)
+        if (y0 + e < p.Dv)
+          *reinterpret_cast<float4*>(to + e) =
+              make_float4(p.last_f * T[e / 2].x, p.last_f * T[e / 2].y, p.last_f * T[e / 2 + 1].x, p.last_f * T[e / 2 + 1].y);
+    }
+  } else {
+    // ---- the rows ---------------------------------------------------------------------------
+    const int row = tid & 127, half = (tid >> 7) - WG;  // token; columns of this warpgroup
+    const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16), tY = tS + Sh::kColY, tX = tS + Sh::kColXt;
+    constexpr int kCols = DY / WG, kBlocks = 4 / WG;
+    const int y0 = half * kCols, i0 = (warp & 3) * 32;
+    const bool wide = p.Dv % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 32 == 0;  // rows of whole 32 bytes
+    bool ok = true;
+    for (int it = 0; it < chunks && ok; ++it) {
+      const int t0 = first_token(it), m = min(n - t0, kTok);
+      const int place = p.rev ? m - 1 - row : row;
       if (!(ok = wait_all(s_full, it))) break;
       tc_fence_after();
-      uint32_t pw[kBlocks][16];
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < kBlocks; ++q) {
-        const int j0 = (half * kBlocks + q) * 32, i0 = (warp & 3) * 32;
+        const int j0 = (half * kBlocks + q) * 32;
         const bool past = p.rev ? j0 > i0 : j0 < i0, now = j0 == i0;  // the same for the whole warp
-        if (!past && !now) {
+        uint32_t pw[16];
+        if ((past || now) && j0 < m) {
+          float v[32];
+          tmem_ld32_nowait(tS + j0, v);
+          if (past && j0 + 32 <= m) {
+            // g^|i-j| as the power of i's distance to the block's near end times that of j's
+            const float a = ex2(l2 * (float)(p.rev ? j0 - row : row - j0 - 31));
+            tmem_wait_ld();
+            tmem_pin<32>(v);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pw[q][e] = 0;
-          continue;
-        }
-        float v[32];
-        tmem_ld32_nowait(tS + j0, v);
-        tmem_wait_ld();
-        tmem_pin<32>(v);
-        if (past && j0 + 32 <= m) {
-          // g^|i-j| as the power of i's distance to the block's near end times that of j's
-          const float a = ex2(l2 * (float)(p.rev ? j0 - row : row - j0 - 31));
+            for (int e = 0; e < 8; ++e) {
+              const float4 t = *reinterpret_cast<const float4*>(s_pow + e * 4);
+              float2 lo = mul2(make_float2(v[4 * e], v[4 * e + 1]), make_float2(a, a)),
+                     hi = mul2(make_float2(v[4 * e + 2], v[4 * e + 3]), make_float2(a, a));
+              lo = mul2(lo, make_float2(t.x, t.y));
+              hi = mul2(hi, make_float2(t.z, t.w));
+              pw[2 * e] = pack_bf16(lo.x, lo.y), pw[2 * e + 1] = pack_bf16(hi.x, hi.y);
+            }
+          } else {
+            // the columns [first, last] count; select, not multiply: a later token's score may be NaN
+            const int first = p.rev ? max(row - j0, 0) : 0, last = min(p.rev ? 31 : min(row - j0, 31), m - 1 - j0);
+            const uint32_t on = first <= last && first < 32 ? (0xffffffffu >> (31 - (last - first))) << first : 0u;
+            const float step = p.rev ? l2 : -l2, base = (p.rev ? -l2 : l2) * (float)(row - j0);
+            tmem_wait_ld();
+            tmem_pin<32>(v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 t = *reinterpret_cast<const float4*>(s_pow + (p.rev ? e : 7 - e) * 4);
-            float2 lo = mul2(make_float2(v[4 * e], v[4 * e + 1]), make_float2(a, a)),
-                   hi = mul2(make_float2(v[4 * e + 2], v[4 * e + 3]), make_float2(a, a));
-            lo = mul2(lo, p.rev ? make_float2(t.x, t.y) : make_float2(t.w, t.z));
-            hi = mul2(hi, p.rev ? make_float2(t.z, t.w) : make_float2(t.y, t.x));
-            pw[q][2 * e] = pack_bf16(lo.x, lo.y), pw[q][2 * e + 1] = pack_bf16(hi.x, hi.y);
+            for (int e = 0; e < 32; ++e) {
+              const float w = ex2(fmaf(step, (float)e, base));
+              v[e] = on >> e & 1u ? v[e] * w : 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pw[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int lag = p.rev ? j0 + e - row : row - j0 - e;
-            const bool on = lag >= 0 && j0 + e < m;  // select, not multiply: a later token may be NaN
-            v[e] = on ? v[e] * (now ? s_pow[lag & 31] : ex2(l2 * (float)lag)) : 0.0f;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pw[q][e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+          for (int e = 0; e < 16; ++e) pw[e] = 0;
         }
+        // over scores that this thread has read
+        tmem_st16(tS + half * 64 + q * 16, pw);
       }
-      if constexpr (NWG == 2) {  // all scores are read: P goes over them
-        tc_fence_before();
-        mbar_arrive(read);
-        if (!(ok = wait_all(read, it))) break;
-        tc_fence_after();
-      }
-#pragma unroll
-      for (int q = 0; q < kBlocks; ++q) tmem_st16(tS + (half * kBlocks + q) * 16, pw[q]);
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(p_ready);
-      // ---- y
+      const float lead = ex2(l2 * (float)(place + 1 - r)) * p.f;
+      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t0 + row) * p.H + h) * (int64_t)p.Dv + y0;
       if (!(ok = wait_all(y_done, it))) break;
       tc_fence_after();
-      const float lead = ex2(l2 * (float)(place + 1 - r)) * p.f;
-      __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t0 + row) * p.H + h) * (int64_t)p.Dv;
-      const bool wide = p.Dv % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 32 == 0;  // rows of whole 32 bytes
-#pragma unroll
-      for (int c = 0; c < kYCols; c += 16) {
+#pragma unroll 1
+      for (int c = 0; c < kCols; c += 16) {
         float a[16], x[16];
         tmem_ld16_nowait(tY + y0 + c, a);
         tmem_ld16_nowait(tX + y0 + c, x);
         tmem_wait_ld();
         tmem_pin<16>(a);
         tmem_pin<16>(x);
+        if (c + 16 == kCols) {
+          tc_fence_before();
+          mbar_arrive(y_free);
+        }
         uint32_t q[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          q[e] = pack_bf16(fmaf(lead, x[2 * e], p.f * a[2 * e]), fmaf(lead, x[2 * e + 1], p.f * a[2 * e + 1]));
+        for (int e = 0; e < 8; ++e) {
+          float2 t = mul2(make_float2(a[2 * e], a[2 * e + 1]), make_float2(p.f, p.f));
+          t = fma2(make_float2(x[2 * e], x[2 * e + 1]), make_float2(lead, lead), t);
+          q[e] = pack_bf16(t.x, t.y);
+        }
         if (row < m && y0 + c < p.Dv) {
           if (wide) {
-            store32(out + y0 + c, q);
+            store32(out + c, q);
           } else {
-            *reinterpret_cast<uint4*>(out + y0 + c) = make_uint4(q[0], q[1], q[2], q[3]);
-            if (y0 + c + 8 < p.Dv) *reinterpret_cast<uint4*>(out + y0 + c + 8) = make_uint4(q[4], q[5], q[6], q[7]);
+            *reinterpret_cast<uint4*>(out + c) = make_uint4(q[0], q[1], q[2], q[3]);
+            if (y0 + c + 8 < p.Dv) *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(q[4], q[5], q[6], q[7]);
           }
         }
       }
-      tc_fence_before();
     }
-    // ---- the final state, and zeros behind the length
-    if (state_out && holds_t) {
-      if (ok && chunks > 0) ok = wait_all(t_done, chunks - 1);
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < kYCols && ok; c += 16) {
-        float v[16];
-        tmem_ld16_nowait(tT + y0 + c, v);
-        tmem_wait_ld();
-        tmem_pin<16>(v);
-        if (row < p.Dk) {
-          float* to = p.last + bh * sz + (int64_t)row * p.Dv + y0 + c;
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (y0 + c + e < p.Dv) {
-              float4 t = make_float4(p.last_f * v[e], p.last_f * v[e + 1], p.last_f * v[e + 2], p.last_f * v[e + 3]);
-              *reinterpret_cast<float4*>(to + e) = t;
-            }
-        }
-      }
-    } else if (ok && chunks > 0) {
-      wait_all(t_done, chunks - 1);  // no product is in flight when TMEM is given back
-    }
-    const int e8 = p.Dv / 8;
-    for (int t = max(c_lo * kTok, n) + (tid >> 3); t < min(c_end * kTok, p.L); t += NWG * 16)
-      for (int e = tid & 7; e < e8; e += 8)
+    // zeros behind the length
+    const int e8 = p.Dv / 8, me = tid - WG * 128;
+    for (int t = max(c_lo * kTok, n) + (me >> 3); t < min(c_end * kTok, p.L); t += WG * 16)
+      for (int e = me & 7; e < e8; e += 8)
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t) * p.H + h) * (int64_t)p.Dv + e * 8) =
             make_uint4(0, 0, 0, 0);
   }
@@ -366,7 +433,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   if (s_abort) {  // the same for all: nothing writes it after the barrier
     if (warp == kMmaWarp) drain_umma(drain);
     if (warp == kTmaWarp && lane == 0) {
-      drain_copies(xk_full, asked_xk, 1);
+      drain_copies(x_full, asked_x, 1);
+      drain_copies(k_full, asked_k, 1);
       drain_copies(v_full, asked_v, 1);
     }
     __syncthreads();
@@ -376,51 +444,44 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
 }
 
 // ---- the segments' own sums --------------------------------------------------------------------
-// No x and no y: T = sum over the segment of k_j^T (w_j v_j), w_j to the segment's end, summed in TMEM from its first
-// chunk to its last without being read.  Two stages of k, v and pieces.
+// No x and no y: T = sum over the segment of (w_j k_j)^T v_j, w_j to the segment's end, so T is never scaled.  Stages of
+// k and v; one chunk's sum is added to the registers while the next one's products run.
 template <int DX, int DY> struct SumShape {
-  using Sh = Shape<DX, DY, 3>;
-  static constexpr int kNP = 3;
-  static constexpr int kStages = 2;
-  static constexpr int kIn = Sh::kX + Sh::kV, kStage = kIn;
-  // the pieces of one stage at a time where two do not fit
-  static constexpr int kPieceSets = DX == 128 && DY == 128 ? 1 : 2;
-  // with 64 dims the products read 64 rows behind an operand, for rows of the result that nobody reads
-  static constexpr int kBehind = DX == 64 && !Sh::kScaleV ? kBlock : 0;
-  static constexpr size_t kBytes = kStages * (size_t)kStage + kPieceSets * (size_t)kNP * Sh::kPiece + kBehind + 1024;
-  static constexpr int kThreads = 128 + 64;
-  static constexpr uint32_t kCols = DY;
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 2;
+  static constexpr int kNP = 3, kStages = 2;
+  static constexpr int kWg = DX == 64 && DY == 64 ? 1 : 2;
+  static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock, kStage = kX + kV;
+  static constexpr size_t kBytes = kStages * (size_t)kStage + (size_t)kNP * kX + 1024;
+  static constexpr int kThreads = kWg * 128 + 64;
+  static constexpr uint32_t kCols = 2 * DY;
+  static constexpr int kPerSm = kBytes <= 112 * 1024 ? 2 : 1;
 };
 
 template <int DX, int DY>
-__global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, 1)
+__global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::kPerSm)
     sums_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                 const __grid_constant__ Pass p) {
-  using Ss = SumShape<DX, DY>;
-  using Sh = typename Ss::Sh;
-  constexpr int NP = Ss::kNP, ST = Ss::kStages, PS = Ss::kPieceSets;
+  using Sh = SumShape<DX, DY>;
+  constexpr int NP = Sh::kNP, ST = Sh::kStages, WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *sIn = smem, *sP = smem + ST * Ss::kStage;
+  unsigned char *sP = smem, *sIn = sP + NP * Sh::kX;  // the pieces first, as above
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ uint64_t bars[Ss::kBars];
-  uint64_t *full = bars, *used = bars + ST, *ready = bars + 2 * ST, *taken = ready + 2, *done = taken + 1,
-           *drain = done + 1;
-  // used[s]: the products of stage s's chunk are complete; ready[i]: a chunk's pieces are written
+  constexpr int kBars = ST + 3;
+  __shared__ uint64_t bars[kBars];
+  uint64_t *full = bars, *ready = bars + ST, *done = ready + 1, *drain = done + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = 4, kMmaWarp = 5;
+  constexpr int kTmaWarp = WG * 4, kMmaWarp = WG * 4 + 1;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
-                 "r"(Ss::kCols)
+                 "r"(Sh::kCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 0) {
     s_abort = 0;
-    for (uint64_t* b = bars; b < bars + Ss::kBars; ++b) mbar_init(b, b >= ready && b < ready + 2 ? 128 : 1);
+    for (uint64_t* b = bars; b < bars + kBars; ++b) mbar_init(b, b == ready ? WG * 128 : 1);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -443,9 +504,9 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, 1)
     if (lane == 0)
       for (int it = 0; it < chunks; ++it) {
         const int s = it % ST, t0 = lo + it * kTok;
-        if (it >= ST && !wait(&used[s], it / ST - 1)) break;
-        mbar_expect_tx(&full[s], Ss::kIn);
-        unsigned char* to = sIn + s * Ss::kStage;
+        if (it >= ST && !wait(done, it - ST)) break;
+        mbar_expect_tx(&full[s], Sh::kStage);
+        unsigned char* to = sIn + s * Sh::kStage;
         for (int d = 0; d < DX / 64; ++d) tma_load_4d(to + d * kBlock, &mk, d * 64, t0, h, (int)b, &full[s]);
         for (int d = 0; d < DY / 64; ++d) tma_load_4d(to + Sh::kX + d * kBlock, &mv, d * 64, t0, h, (int)b, &full[s]);
         asked = it + 1;
@@ -453,86 +514,72 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, 1)
   } else if (warp == kMmaWarp) {
     const uint32_t one = elect_one();
     const uint32_t id_t = idesc_bf16(128, (p.Dv + 15) / 16 * 16, true, true);
-    const uint64_t d_k = smem_desc_sw128(smem_u32(sIn), kBlock, 1024),
-                   d_v = smem_desc_sw128(smem_u32(sIn + Sh::kX), kBlock, 1024),
+    const uint64_t d_v = smem_desc_sw128(smem_u32(sIn + Sh::kX), kBlock, 1024),
                    d_p = smem_desc_sw128(smem_u32(sP), kBlock, 1024);
     for (int it = 0; it < chunks; ++it) {
-      const int s = it % ST, ps = it % PS;
-      if (!wait_all(&ready[it & 1], it >> 1)) break;
+      if (!wait_all(ready, it)) break;
       tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
+      for (int i = NP - 1; i >= 0; --i)
 #pragma unroll
-        for (int k = 0; k < kTok / 16; ++k) {
-          const uint64_t pd = desc_at(d_p, (ps * NP + i) * Sh::kPiece + k * 16 * kRowBytes);
-          const uint32_t off = s * Ss::kStage + k * 16 * kRowBytes;
-          umma_ss(one, tmem, Sh::kScaleV ? desc_at(d_k, off) : pd, Sh::kScaleV ? pd : desc_at(d_v, off), id_t,
-                  (it | i | k) != 0);
-        }
-      umma_done(one, &used[s]);
-      if (it == chunks - 1) umma_done(one, done);
+        for (int k = 0; k < kTok / 16; ++k)
+          umma_ss(one, tmem + (it & 1) * DY, desc_at(d_p, i * Sh::kX + k * 16 * kRowBytes),
+                  desc_at(d_v, it % ST * Sh::kStage + k * 16 * kRowBytes), id_t, !(i == NP - 1 && k == 0));
+      umma_done(one, done);
     }
   } else {
-    const int row = tid & 127;
-    constexpr int kPDims = Sh::kScaleV ? DY : DX;
+    const int row = tid & 127, half = tid >> 7;
+    constexpr int kCols = DY / WG, kDims = DX / WG;
+    const int y0 = half * kCols;
+    const bool holds = (warp & 3) * 32 < DX;
+    const uint32_t tT = tmem + ((uint32_t)((warp & 3) * 32) << 16) + y0;
+    float T[kCols];
+#pragma unroll
+    for (int e = 0; e < kCols; ++e) T[e] = 0.0f;
+    auto add = [&](int it) {
+      if (!holds) return;
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        float v[16];
+        tmem_ld16_nowait(tT + (it & 1) * DY + c, v);
+        tmem_wait_ld();
+        tmem_pin<16>(v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) T[c + e] += v[e];
+      }
+    };
     bool ok = true;
     for (int it = 0; it < chunks && ok; ++it) {
       const int s = it % ST, t = lo + it * kTok + row;
-      // the products that read these pieces before
-      if (it >= PS && !(ok = wait_all(&used[(it - PS) % ST], (it - PS) / ST))) break;
       if (!(ok = wait_all(&full[s], it / ST))) break;
-      unsigned char *sK = sIn + s * Ss::kStage, *sV = sK + Sh::kX;
-      if (t >= hi) {
-        unsigned char* other = Sh::kScaleV ? sK : sV;
-        for (int c = 0; c < (Sh::kScaleV ? DX : DY) / 8; ++c)
-          *reinterpret_cast<uint4*>(other + swizzled(kTok, row, c)) = make_uint4(0, 0, 0, 0);
-      }
+      // the products that read the pieces are complete
+      if (it > 0 && !(ok = wait_all(done, it - 1))) break;
+      unsigned char *sK = sIn + s * Sh::kStage, *sV = sK + Sh::kX;
+      const int c0 = half * (kDims / 8);
       const float w = ex2(l2 * (float)(p.rev ? t - lo + 1 : hi - 1 - t));
-      const unsigned char* from = Sh::kScaleV ? sV : sK;
-      unsigned char* to = sP + it % PS * NP * Sh::kPiece;
-#pragma unroll 2
-      for (int c = 0; c < kPDims / 8; ++c) {
-        const int at = swizzled(kTok, row, c);
-        uint32_t q[NP][4] = {};
-        if (t < hi) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(from + at);
-          const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float a = __uint_as_float(in[e] << 16) * w, z = __uint_as_float(in[e] & 0xffff0000u) * w;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-              q[i][e] = pack_bf16(a, z);
-              a -= __uint_as_float(q[i][e] << 16), z -= __uint_as_float(q[i][e] & 0xffff0000u);
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-          *reinterpret_cast<uint4*>(to + i * Sh::kPiece + at) = make_uint4(q[i][0], q[i][1], q[i][2], q[i][3]);
+#pragma unroll 1
+      for (int c = 0; c < kDims / 8; c += 4) weigh_row<NP, 4>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
+      if (t >= hi) {
+        clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
+        clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&ready[it & 1]);
-    }
-    if (ok && chunks > 0) ok = wait_all(done, 0);
-    tc_fence_after();
-    if ((warp & 3) * 32 < DX) {
-      float* to = p.part + (bh * p.segs + seg) * ((int64_t)p.Dk * p.Dv) + (int64_t)row * p.Dv;
-      const uint32_t tT = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-#pragma unroll 1
-      for (int c = 0; c < DY; c += 16) {
-        float v[16] = {};
-        if (chunks > 0) {
-          tmem_ld16_nowait(tT + c, v);
-          tmem_wait_ld();
-          tmem_pin<16>(v);
-        }
-        if (row < p.Dk) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (c + e < p.Dv) *reinterpret_cast<float4*>(to + c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        }
+      tc_fence_before();
+      mbar_arrive(ready);
+      if (it > 0) {
+        tc_fence_after();
+        add(it - 1);
       }
+    }
+    if (ok && chunks > 0 && wait_all(done, chunks - 1)) {
+      tc_fence_after();
+      add(chunks - 1);
+    }
+    if (row < p.Dk) {
+      float* to = p.part + (bh * p.segs + seg) * ((int64_t)p.Dk * p.Dv) + (int64_t)row * p.Dv + y0;
+#pragma unroll
+      for (int e = 0; e < kCols; e += 4)
+        if (y0 + e < p.Dv) *reinterpret_cast<float4*>(to + e) = make_float4(T[e], T[e + 1], T[e + 2], T[e + 3]);
     }
   }
   tc_fence_before();
@@ -544,7 +591,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, 1)
     __syncthreads();
   }
   if (warp == kMmaWarp)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Ss::kCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::kCols) : "memory");
 }
 
 // ---- host ----------------------------------------------------------------------------------
@@ -555,7 +602,7 @@ bool tc_ok(const Pass& p) {
 }
 
 size_t tc_part_bytes(Pass p) {
-  cut(p, kTok, 1);
+  cut(p, kTok, (int64_t)p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
   return p.segs > 1 ? (size_t)p.B * p.H * p.segs * p.Dk * p.Dv * sizeof(float) : 0;
 }
 
@@ -587,7 +634,7 @@ int launch_np(const Pass& p, cudaStream_t st) {
 }
 
 int tc_pass(Pass p, cudaStream_t st) {
-  cut(p, kTok, 1);
+  cut(p, kTok, (int64_t)p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
   if (p.Dk <= 64) return p.Dv <= 64 ? launch_np<64, 64>(p, st) : launch_np<64, 128>(p, st);
   return p.Dv <= 64 ? launch_np<128, 64>(p, st) : launch_np<128, 128>(p, st);
 }
