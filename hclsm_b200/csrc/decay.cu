@@ -240,34 +240,46 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
 }
 
 // The segments' sums become their first states; the state behind the last one (in the pass's order) goes to `last`.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Pass p, int chunk) {
+// Eight sums are asked for at a time, so a thread waits for memory once in eight segments.
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Pass p, int chunk) {
+  __shared__ float2 s_g[2];
   pdl_wait();
   pdl_trigger();
   const int64_t sz = (int64_t)p.Dk * p.Dv;
-  const int64_t per = (sz + 255) / 256;
-  const int64_t bh = blockIdx.x / per, i = blockIdx.x % per * 256 + threadIdx.x;
-  if (i >= sz) return;
+  const int64_t per = (sz + 127) / 128;
+  const int64_t bh = blockIdx.x / per, i = blockIdx.x % per * 128 + threadIdx.x;
   const int64_t b = bh / p.H;
   const int h = (int)(bh - b * p.H), n = length(p, b), span = p.seg_chunks * chunk;
+  // of a whole segment and of the incomplete one
+  if (threadIdx.x < 2) s_g[threadIdx.x] = chunk_decay(p.log_decay, h, threadIdx.x ? n % span : span);
+  __syncthreads();
+  if (i >= sz) return;
   float v = 0.0f;
   if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? i % p.Dv * p.Dk + i / p.Dv : i)];
   float* at = p.part + bh * p.segs * sz + i;
-  const float2 whole = chunk_decay(p.log_decay, h, span);
-  for (int it = 0; it < p.segs; ++it) {
-    const int s = p.rev ? p.segs - 1 - it : it;
-    const int m = min(max(n - s * span, 0), span);
-    const float sum = at[s * sz];
-    at[s * sz] = v;
-    const float2 g = m == span ? whole : chunk_decay(p.log_decay, h, m);
-    v = fmaf(v, g.x, fmaf(v, g.y, sum));
+  const float2 whole = s_g[0], cut_off = s_g[1];
+  for (int it = 0; it < p.segs; it += 8) {
+    float sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (it + k < p.segs) sum[k] = at[(p.rev ? p.segs - 1 - it - k : it + k) * sz];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (it + k >= p.segs) break;
+      const int s = p.rev ? p.segs - 1 - it - k : it + k, m = n - s * span;  // m: tokens from here on
+      at[s * sz] = v;
+      if (m <= 0) continue;  // behind the length
+      const float2 g = m >= span ? whole : cut_off;
+      v = fmaf(v, g.x, fmaf(v, g.y, sum[k]));
+    }
   }
   if (p.last) p.last[bh * sz + i] = p.last_f * v;
 }
 
 int join(const Pass& p, int chunk, cudaStream_t st) {
-  const int64_t grid = (int64_t)p.B * p.H * (((int64_t)p.Dk * p.Dv + 255) / 256);
+  const int64_t grid = (int64_t)p.B * p.H * (((int64_t)p.Dk * p.Dv + 127) / 128);
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  return launch_pdl(join_kernel, (unsigned)grid, 256, 0, st, p, chunk);
+  return launch_pdl(join_kernel, (unsigned)grid, 128, 0, st, p, chunk);
 }
 
 template <typename T, int DP, bool SUMS>

@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ __align__(16) float s_pow[32];  // g^(distance of a block's j to its end on the later side)
+  __shared__ float2 s_g[2];  // decays of a whole chunk and of the incomplete one
   constexpr int kBars = 12;
   __shared__ uint64_t bars[kBars];
   uint64_t *x_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_ready = bars + 4,
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
   if (tid < 32) s_pow[tid] = ex2(l2 * (float)(r ? tid : 31 - tid));
+  if (warp == kTmaWarp && lane < 2) s_g[lane] = chunk_decay(p.log_decay, h, lane ? n % kTok : kTok);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -242,8 +244,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
     const int y0 = half * kCols;
     const bool holds = (warp & 3) * 32 < DX;  // this warp's lanes are rows of T
     const uint32_t tT = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::kColT + y0;
-    // of a whole chunk and of the incomplete one (or of no token); not in the loop, where T fills the registers
-    const float2 whole = chunk_decay(p.log_decay, h, kTok), cut_off = chunk_decay(p.log_decay, h, n % kTok);
+    const float2 whole = s_g[0], cut_off = s_g[1];
     float2 T[kCols / 2];
 #pragma unroll
     for (int e = 0; e < kCols / 2; ++e) T[e] = make_float2(0.0f, 0.0f);
