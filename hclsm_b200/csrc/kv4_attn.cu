@@ -1,46 +1,60 @@
 // Attention of few query rows over the paged 4-bit state cache.
 //
-// The rows that share a key head (tokens x query heads of the group) form the M = 16 side of mma.sync m16n8k16
-// products; a warp takes 32 tokens a step and keeps its own running maximum, sum and output.  Each warp has a
-// ring of stages of its own, filled by bulk copies that its first lane asks for (a page of one head is contiguous):
-// no barrier between warps until the merge.
+// The rows that share a key head (tokens x query heads of the group) are the N = 8 side of mma.sync m16n8k16
+// products, so that few rows waste nothing; a warp takes 32 tokens a step and keeps its own running maximum, sum and
+// output.  Each warp has a ring of stages of its own, filled by bulk copies that four of its lanes ask for (a page of
+// one head is contiguous): no barrier between warps until the merge.
 //
 // A contraction's index can run in any order, so the products take the codes as they lie: two words' halves of the same
 // 32 dims (or of two tokens) side by side, four bits at a time, 0x4300 | code = 128 + code in bf16.
-//   S = Q K^T by groups of 32 dims, each times its key's scale: the 136 = 128 + 8 in every operand is taken off by
+//   S^T = K Q^T by groups of 32 dims, each times its key's scale: the 136 = 128 + 8 in every operand is taken off by
 //   starting the sum at -136 times the row's sum of q in the group (fp32 states: off every operand instead,
 //   their scores would lose 5 bits).
-//   O += P V, P times the value's scale of the group before it is rounded to bf16: the codes are exact, so a weight
-//   is rounded once.  The 136 comes off the operand (summed over a history it would drown the values).
+//   O^T += V^T P^T, P times the value's scale of the group before it is rounded to bf16: the codes are exact, so a weight
+//   is rounded once.  movmatrix turns the scores' fragments into P^T's.  The 136 comes off the operand (summed over a
+//   history it would drown the values).
 // fp32 states: queries and weights as three bf16 pieces, whose products with exact codes are summed in fp32.
 #include "kv4.cuh"
 
 namespace hclsm {
 namespace kv4 {
 
-constexpr int kWarps = 4, kThreads = kWarps * 32, kRows = 16, kUnit = 32;
+constexpr int kWarps = 4, kThreads = kWarps * 32, kUnit = 32;
 constexpr int kWaves = 4, kMinKeys = 1024;
 
-template <typename T, int D> struct Shape {
+// RT: tiles of 8 rows a block.
+template <typename T, int D, int RT> struct Shape {
   static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr int kRows = 8 * RT;
   static constexpr int kNQ = kF32 ? 3 : 1;  // bf16 pieces of a query or weight
   static constexpr int kG = D / kGroup;
   static constexpr int kCodes = kUnit * D / 2, kScales = kUnit * D / 16;  // bytes
   static constexpr int kStage = 2 * (kCodes + kScales);
   static constexpr int kStages = 4;
-  static constexpr int kFrag = kF32 ? kNQ * kG * 2 * 32 * 16 : 0;  // query fragments of fp32 states
+  static constexpr int kFrag = kF32 ? kNQ * kG * 2 * 32 * 8 * RT : 0;  // query fragments of fp32 states
   static constexpr int kMerge = kWarps * kRows * D * 4;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kFrag;
   static constexpr int kPerSm = kF32 ? 2 : D <= 64 ? 4 : 3;
 };
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// d = a b + c: with a sum of its own, the first product of a sum needs no copy of what it starts from.
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
+                                    float c2, float c3) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
-      "%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
+      "%12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  mma(d, a, b0, b1, d[0], d[1], d[2], d[3]);
+}
+// An 8 x 8 matrix of bf16 across the warp (lane 4 g + c: row g, columns 2 c and 2 c + 1), transposed.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -78,11 +92,10 @@ template <int G> __device__ __forceinline__ void scales(const unsigned char* at,
   }
 }
 
-// NR 1: at most 8 rows, the upper half of the products' rows is empty.
-template <typename T, int D, int NR>
-__global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(const __grid_constant__ Attn p) {
-  using Sh = Shape<T, D>;
-  constexpr int G = Sh::kG, NQ = Sh::kNQ, ST = Sh::kStages;
+template <typename T, int D, int RT>
+__global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel(const __grid_constant__ Attn p) {
+  using Sh = Shape<T, D, RT>;
+  constexpr int G = Sh::kG, NQ = Sh::kNQ, ST = Sh::kStages, kRows = Sh::kRows;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t bars[kWarps * ST];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_w[kWarps][kRows];
@@ -100,50 +113,46 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(con
   const int units = (n + kUnit - 1) / kUnit;
   const int u_lo = (int)((int64_t)units * sp / p.splits), u_hi = (int)((int64_t)units * (sp + 1) / p.splits);
 
-  // ---- copies ------------------------------------------------------------------------------
+  // ---- copies: lane 4 h + kind asks for the kind (codes or scales of keys or values) of page h of a unit (two pages
+  // where they have 16 tokens)
   unsigned char* ring = smem + warp * ST * Sh::kStage;
   uint64_t* bar = bars + warp * ST;
   const int32_t* table = p.table + b * p.M;
-  const bool small = p.c.page == 16;  // a unit is two pages
-  uint32_t holes = 0;                 // two bits a stage: halves of a unit that are not there
-  // the page numbers of unit u (loaded by all lanes alike)
-  auto pages_of = [&](int u) {
-    int2 r = make_int2(-1, -1);
-    if (u < u_hi) {
-      const int at = u * kUnit >> p.c.log_page;
-      r.x = table[at];
-      if (small && u * kUnit + 16 < n) r.y = table[at + 1];
-    }
-    return r;
+  const bool small = p.c.page == 16;
+  const int kind = lane & 3, half = lane >> 2 & 1;
+  const int per_token = kind < 2 ? D / 2 : D / 16, tokens = small ? 16 : kUnit;
+  const char* source = reinterpret_cast<const char*>(kind < 2 ? (const void*)p.c.q[kind] : (const void*)p.c.scale[kind & 1]) +
+                       (int64_t)hk * p.c.page * per_token;
+  const int64_t page_step = (int64_t)p.c.Hkv * p.c.page * per_token;
+  const uint32_t to0 = (kind & 1 ? (kind < 2 ? Sh::kCodes : Sh::kScales) : 0) + (kind < 2 ? 0 : 2 * Sh::kCodes) +
+                       half * tokens * per_token;
+  uint32_t holes = 0;  // two bits a stage: halves of a unit that are not there
+  // this lane's page of unit u
+  auto page_of = [&](int u) {
+    const int at = (u * kUnit >> p.c.log_page) + (small ? half : 0);
+    return u < u_hi && u * kUnit + (small ? half * 16 : 0) < n ? table[at] : -1;
   };
-  auto fetch = [&](int u, int s, int2 id) {
+  auto fetch = [&](int u, int s, int id) {
     if (u >= u_hi) return;
-    const bool a = (unsigned)id.x < (unsigned)p.c.pages, z = small && (unsigned)id.y < (unsigned)p.c.pages;
-    if (lane == 0 && (!a || (small && !z && u * kUnit + 16 < n))) record_error(p.err, HCLSM_ERR_SHAPE);
-    const uint32_t hole = a ? (small && !z ? 2u : 0u) : (z ? 1u : 3u);
+    const uint32_t there = __ballot_sync(0xffffffffu, (unsigned)id < (unsigned)p.c.pages);
+    const uint32_t hole = (there & 1u ? 0u : 1u) | (there & 16u ? 0u : 2u);
+    if (hole && lane == 0 && ((hole & 1u) || (small && u * kUnit + 16 < n))) record_error(p.err, HCLSM_ERR_SHAPE);
     holes = (holes & ~(3u << 2 * s)) | hole << 2 * s;
-    if (lane != 0) return;
-    const int half = small ? 2 : 1, tokens = kUnit / half;
-    unsigned char* to = ring + s * Sh::kStage;
-    mbar_expect_tx(&bar[s], (uint32_t)((a ? 1 : 0) + (z ? 1 : 0)) * (Sh::kStage / half));
-    for (int i = 0; i < half; ++i) {
-      if (!(i ? z : a)) continue;
-      const int64_t at = ((int64_t)(i ? id.y : id.x) * p.c.Hkv + hk) * p.c.page + (small ? 0 : u * kUnit & (p.c.page - 1));
-      const int codes = tokens * D / 2, sc = tokens * D / 16;
-      bulk_g2s(to + i * codes, p.c.q[0] + at * (D / 2), codes, &bar[s]);
-      bulk_g2s(to + Sh::kCodes + i * codes, p.c.q[1] + at * (D / 2), codes, &bar[s]);
-      bulk_g2s(to + 2 * Sh::kCodes + i * sc, p.c.scale[0] + at * (D / kGroup), sc, &bar[s]);
-      bulk_g2s(to + 2 * Sh::kCodes + Sh::kScales + i * sc, p.c.scale[1] + at * (D / kGroup), sc, &bar[s]);
-    }
+    if (lane == 0)
+      mbar_expect_tx(&bar[s], small ? (2u - (hole & 1u) - (hole >> 1)) * (Sh::kStage / 2) : hole & 1u ? 0u : Sh::kStage);
+    __syncwarp();
+    if (lane < (small ? 8 : 4) && (there >> lane & 1u))
+      bulk_g2s(ring + s * Sh::kStage + to0,
+               source + id * page_step + (small ? 0 : (u * kUnit & (p.c.page - 1)) * per_token), tokens * per_token, &bar[s]);
   };
   const int u0 = u_lo + warp;
-#pragma unroll
-  for (int i = 0; i < ST - 1; ++i) fetch(u0 + i * kWarps, i, pages_of(u0 + i * kWarps));
-  int2 next = pages_of(u0 + (ST - 1) * kWarps);
+#pragma unroll 1
+  for (int i = 0; i < ST - 1; ++i) fetch(u0 + i * kWarps, i, page_of(u0 + i * kWarps));
+  int next = page_of(u0 + (ST - 1) * kWarps);
 
-  // ---- queries -----------------------------------------------------------------------------
-  uint32_t qa[Sh::kF32 ? 1 : G][2][4];
-  float q136[Sh::kF32 ? 1 : G][NR];  // -136 times the row's sum of a group
+  // ---- queries: fragments of Q^T, row g of each tile, dims 8 c + i and 8 c + 4 + i of a group side by side ----
+  uint32_t qb[Sh::kF32 ? 1 : RT][G][4];
+  float q136[Sh::kF32 ? 1 : RT][G][2];  // -136 times the sum of a group of rows 2 c and 2 c + 1
   uint32_t* frag = reinterpret_cast<uint32_t*>(smem + (Sh::kBytes - Sh::kFrag));
   auto row_at = [&](int r) {  // a row's query, or null
     const int row = rt * kRows + r;
@@ -153,61 +162,63 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(con
   };
   if constexpr (!Sh::kF32) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const T* q = r < NR ? row_at(g + 8 * r) : nullptr;
+    for (int r = 0; r < RT; ++r) {
+      const T* q = row_at(g + 8 * r);
 #pragma unroll
       for (int y = 0; y < G; ++y) {
         uint4 w = make_uint4(0, 0, 0, 0);
         if (q) w = *reinterpret_cast<const uint4*>(q + y * kGroup + 8 * c);
-        qa[y][0][r] = __byte_perm(w.x, w.z, 0x5410), qa[y][0][2 + r] = __byte_perm(w.x, w.z, 0x7632);
-        qa[y][1][r] = __byte_perm(w.y, w.w, 0x5410), qa[y][1][2 + r] = __byte_perm(w.y, w.w, 0x7632);
-        if (r < NR) {
-          float sum = 0.0f;
-          const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+        qb[r][y][0] = __byte_perm(w.x, w.z, 0x5410), qb[r][y][1] = __byte_perm(w.x, w.z, 0x7632);
+        qb[r][y][2] = __byte_perm(w.y, w.w, 0x5410), qb[r][y][3] = __byte_perm(w.y, w.w, 0x7632);
+        float sum = 0.0f;
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xffff0000u);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          q136[y][r] = -136.0f * sum;
-        }
+        for (int i = 0; i < 4; ++i) sum += __uint_as_float(v[i] << 16) + __uint_as_float(v[i] & 0xffff0000u);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        q136[r][y][0] = -136.0f * __shfl_sync(0xffffffffu, sum, 8 * c);
+        q136[r][y][1] = -136.0f * __shfl_sync(0xffffffffu, sum, 8 * c + 4);
       }
     }
   } else {
-    // fragment words [piece][group][step][lane][4]
+    // fragment words [piece][group][step][lane][RT][2]
     for (int i = threadIdx.x; i < G * 2 * 32; i += kThreads) {
       const int l = i & 31, step = i >> 5 & 1, y = i >> 6;
-      uint32_t w[4][NQ];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {  // rows l / 4 and + 8, dims 8 (l % 4) + k and + k + 4, k = 2 step + e / 2
-        const T* q = row_at((l >> 2) + 8 * (e & 1));
-        const int d = y * kGroup + 8 * (l & 3) + 2 * step + (e >> 1);
-        pieces<NQ>(q ? (float)q[d] : 0.0f, q ? (float)q[d + 4] : 0.0f, w[e]);
+      for (int r = 0; r < RT; ++r) {
+        const T* q = row_at((l >> 2) + 8 * r);
+        const int d = y * kGroup + 8 * (l & 3) + 2 * step;
+        uint32_t w[2][NQ];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) pieces<NQ>(q ? (float)q[d + e] : 0.0f, q ? (float)q[d + e + 4] : 0.0f, w[e]);
+#pragma unroll
+        for (int k = 0; k < NQ; ++k)
+          *reinterpret_cast<uint2*>(frag + ((((k * G + y) * 2 + step) * 32 + l) * RT + r) * 2) =
+              make_uint2(w[0][k], w[1][k]);
       }
-#pragma unroll
-      for (int k = 0; k < NQ; ++k)
-        *reinterpret_cast<uint4*>(frag + (((k * G + y) * 2 + step) * 32 + l) * 4) =
-            make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
     }
     __syncthreads();
   }
 
   // ---- tokens ------------------------------------------------------------------------------
-  float o[D / 8][4] = {};
-  float m[NR], l[NR];
+  // o[tile][r]: dims 4 g + 2 (tile % 2) (and + 1) of group tile / 2, rows 2 c and 2 c + 1 of row tile r
+  float o[D / 16][RT][4] = {};
+  float m[RT][2], l[RT][2];
 #pragma unroll
-  for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.0f;
-  // A lane's key of a tile of 8 and its two columns' tokens: an order in which neither keys (four rows a load's half)
-  // nor values (four tokens a load) meet in a bank with 64 dims.
+  for (int r = 0; r < RT; ++r) m[r][0] = m[r][1] = -INFINITY, l[r][0] = l[r][1] = 0.0f;
+  // Of a tile of 8 tokens, the one that is row g of K (and lane g's scores) and columns 2 c and 2 c + 1 of V^T: an order in
+  // which neither keys (four rows a load's half) nor values (four tokens a load) meet in a bank with 64 dims.
   const int key = g & 1 ? (g >> 1) + 2 : (g >> 1) + 2 * (g >> 1 & 2);
   const int tok0 = c + 2 * (c & 2), tok1 = c + 2;
   int s = 0;
   uint32_t phase = 0;
   bool alive = true;
+#pragma unroll 1
   for (int u = u0; u < u_hi; u += kWarps) {
     const int s_new = s == 0 ? ST - 1 : s - 1;
     __syncwarp();  // all lanes have left the stage that is filled now
     fetch(u + (ST - 1) * kWarps, s_new, next);
-    next = pages_of(u + ST * kWarps);
+    next = page_of(u + ST * kWarps);
     if (!__all_sync(0xffffffffu, mbar_wait(&bar[s], phase))) {
       alive = false;
       break;
@@ -218,116 +229,142 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(con
     if (++s == ST) s = 0, phase ^= 1;
     const int left = n - u * kUnit;
     uint32_t valid = left >= kUnit ? 0xffffffffu : (1u << left) - 1u;
-    if (hole) valid &= small ? (hole & 1 ? 0xffff0000u : ~0u) & (hole & 2 ? 0xffffu : ~0u) : 0u;
+    if (hole) valid &= small ? (hole & 1 ? 0xffff0000u : ~0u) & (hole & 2 ? 0xffffu : ~0u) : hole & 1 ? 0u : ~0u;
     if (valid == 0) continue;
 
-    float sc[4][2 * NR];
+    float sc[2][RT][4];  // 16 tokens: lane's tokens key and key + 8, rows 2 c and 2 c + 1
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint32_t* row = reinterpret_cast<const uint32_t*>(kq + (t * 8 + key) * (D / 2));
+    for (int h = 0; h < 2; ++h) {
+      const int t = 16 * h + key;
       float f0[G], f1[G];
-      scales<G>(ks + (t * 8 + tok0) * (D / 16), f0);
-      scales<G>(ks + (t * 8 + tok1) * (D / 16), f1);
-#pragma unroll
-      for (int e = 0; e < 2 * NR; ++e) sc[t][e] = 0.0f;
+      scales<G>(ks + t * (D / 16), f0);
+      scales<G>(ks + (t + 8) * (D / 16), f1);
+      const uint32_t* row0 = reinterpret_cast<const uint32_t*>(kq + t * (D / 2));
+      const uint32_t* row1 = row0 + D;
 #pragma unroll
       for (int y = 0; y < G; ++y) {
-        uint32_t x;  // this lane's eight codes of the group: dims 8 c + i (low half), 8 c + 4 + i
+        uint32_t x0, x1;  // this lane's eight codes of the group: dims 8 c + i (low half), 8 c + 4 + i
         if (y / 2 * 64 + 64 <= D) {
-          const uint2 w = *reinterpret_cast<const uint2*>(row + y / 2 * 8 + 2 * c);
-          x = __byte_perm(w.x, w.y, y & 1 ? 0x7632 : 0x5410);
+          const uint2 w0 = *reinterpret_cast<const uint2*>(row0 + y / 2 * 8 + 2 * c);
+          const uint2 w1 = *reinterpret_cast<const uint2*>(row1 + y / 2 * 8 + 2 * c);
+          x0 = __byte_perm(w0.x, w0.y, y & 1 ? 0x7632 : 0x5410);
+          x1 = __byte_perm(w1.x, w1.y, y & 1 ? 0x7632 : 0x5410);
         } else {
-          x = row[y / 2 * 8 + c];
+          x0 = row0[y / 2 * 8 + c], x1 = row1[y / 2 * 8 + c];
         }
-        float d[4] = {};
-        if constexpr (Sh::kF32) {
+        float d[RT][4];
 #pragma unroll
-          for (int step = 0; step < 2; ++step)
+        for (int step = 0; step < 2; ++step) {
+          const int i = 8 * step;
+          if constexpr (Sh::kF32) {
+            const uint32_t a[4] = {centred(x0 >> i), centred(x1 >> i), centred(x0 >> (i + 4)), centred(x1 >> (i + 4))};
 #pragma unroll
-            for (int k = 0; k < NQ; ++k) {
-              const uint4 w = *reinterpret_cast<const uint4*>(frag + (((k * G + y) * 2 + step) * 32 + lane) * 4);
-              const uint32_t a[4] = {w.x, w.y, w.z, w.w};
-              mma(d, a, centred(x >> 8 * step), centred(x >> (8 * step + 4)));
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+              for (int k = 0; k < NQ; ++k) {
+                const uint2 w = *reinterpret_cast<const uint2*>(frag + ((((k * G + y) * 2 + step) * 32 + lane) * RT + r) * 2);
+                if (step == 0 && k == 0) mma(d[r], a, w.x, w.y, 0.0f, 0.0f, 0.0f, 0.0f);
+                else mma(d[r], a, w.x, w.y);
+              }
+          } else {
+            const uint32_t a[4] = {biased(x0 >> i), biased(x1 >> i), biased(x0 >> (i + 4)), biased(x1 >> (i + 4))};
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              if (step == 0)
+                mma(d[r], a, qb[r][y][0], qb[r][y][1], q136[r][y][0], q136[r][y][1], q136[r][y][0], q136[r][y][1]);
+              else
+                mma(d[r], a, qb[r][y][2], qb[r][y][3]);
             }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 2 * NR; ++e) d[e] = q136[y][e >> 1];
-          mma(d, qa[y][0], biased(x), biased(x >> 4));
-          mma(d, qa[y][1], biased(x >> 8), biased(x >> 12));
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 2 * NR; ++e) sc[t][e] = fmaf(d[e], e & 1 ? f1[y] : f0[y], sc[t][e]);
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = e < 2 ? f0[y] : f1[y];
+            sc[h][r][e] = y == 0 ? d[r][e] * f : fmaf(d[r][e], f, sc[h][r][e]);
+          }
       }
     }
     if (valid != 0xffffffffu) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2 * NR; ++e)
-          if (!(valid >> (t * 8 + (e & 1 ? tok1 : tok0)) & 1u)) sc[t][e] = -INFINITY;
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(valid >> (16 * h + key + (e < 2 ? 0 : 8)) & 1u)) sc[h][r][e] = -INFINITY;
     }
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float top = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-      top = fmaxf(top, fmaxf(fmaxf(sc[2][2 * r], sc[2][2 * r + 1]), fmaxf(sc[3][2 * r], sc[3][2 * r + 1])));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top > m[r])) {
-        const float was = m[r];
-        m[r] = fmaxf(was, top);
-        const float f = was == m[r] ? 1.0f : ex2((was - m[r]) * p.c2);
-        l[r] *= f;
+    for (int r = 0; r < RT; ++r) {
+      float top[2];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][2 * r] *= f, o[j][2 * r + 1] *= f;
+      for (int e = 0; e < 2; ++e) {
+        top[e] = fmaxf(fmaxf(sc[0][r][e], sc[0][r][e + 2]), fmaxf(sc[1][r][e], sc[1][r][e + 2]));
+#pragma unroll
+        for (int x = 4; x <= 16; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
       }
-      const float base = m[r] == -INFINITY ? 0.0f : -m[r] * p.c2;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
+      if (__any_sync(0xffffffffu, top[0] > m[r][0] || top[1] > m[r][1])) {
+        float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          sc[t][2 * r + e] = ex2(fmaf(sc[t][2 * r + e], p.c2, base));
-          l[r] += sc[t][2 * r + e];
+          const float was = m[r][e];
+          m[r][e] = fmaxf(was, top[e]);
+          f[e] = was == m[r][e] ? 1.0f : ex2((was - m[r][e]) * p.c2);
+          l[r][e] *= f[e];
         }
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][r][e] *= f[e & 1];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float base = m[r][e] == -INFINITY ? 0.0f : -m[r][e] * p.c2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            sc[h][r][k + e] = ex2(fmaf(sc[h][r][k + e], p.c2, base));
+            l[r][e] += sc[h][r][k + e];
+          }
+      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // 16 tokens
-      float f[4][G];
-      const int t0 = 16 * h + tok0, t1 = 16 * h + tok1;
-      scales<G>(vs + t0 * (D / 16), f[0]), scales<G>(vs + t1 * (D / 16), f[1]);
-      scales<G>(vs + (t0 + 8) * (D / 16), f[2]), scales<G>(vs + (t1 + 8) * (D / 16), f[3]);
+      float f0[G], f1[G];
+      scales<G>(vs + (16 * h + key) * (D / 16), f0);
+      scales<G>(vs + (16 * h + key + 8) * (D / 16), f1);
       if (valid != 0xffffffffu) {  // what is not there may have any scale, NaN too
+        const bool a = valid >> (16 * h + key) & 1u, z = valid >> (16 * h + key + 8) & 1u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(valid >> ((i & 1 ? t1 : t0) + (i & 2 ? 8 : 0)) & 1u)) {
-#pragma unroll
-            for (int y = 0; y < G; ++y) f[i][y] = 0.0f;
-          }
+        for (int y = 0; y < G; ++y) f0[y] = a ? f0[y] : 0.0f, f1[y] = z ? f1[y] : 0.0f;
       }
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(vq + t0 * (D / 2));
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(vq + t1 * (D / 2));
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(vq + (16 * h + tok0) * (D / 2));
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(vq + (16 * h + tok1) * (D / 2));
 #pragma unroll
       for (int y = 0; y < G; ++y) {
         const bool paired = y / 2 * 64 + 64 <= D;
         const int at = y / 2 * 8 + (paired ? g : g >> 1);
         const uint32_t sel = (paired ? y & 1 : g & 1) ? 0x7632 : 0x5410;
         const uint32_t x0 = __byte_perm(w0[at], w1[at], sel), x1 = __byte_perm(w0[at + D], w1[at + D], sel);
-        uint32_t a[NQ][4];
+        uint32_t pb[RT][NQ][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < RT; ++r) {
+          uint32_t v[2][NQ];
+          pieces<NQ>(sc[h][r][0] * f0[y], sc[h][r][1] * f0[y], v[0]);
+          pieces<NQ>(sc[h][r][2] * f1[y], sc[h][r][3] * f1[y], v[1]);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            uint32_t v[NQ] = {};
-            if (r < NR)
-              pieces<NQ>(sc[2 * h + t][2 * (r < NR ? r : 0)] * f[2 * t][y],
-                         sc[2 * h + t][2 * (r < NR ? r : 0) + 1] * f[2 * t + 1][y], v);
+          for (int k = 0; k < NQ; ++k) pb[r][k][0] = turned(v[0][k]), pb[r][k][1] = turned(v[1][k]);
+        }
 #pragma unroll
-            for (int k = 0; k < NQ; ++k) a[k][2 * t + r] = v[k];
-          }
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t a[4] = {centred(x0 >> 8 * i), centred(x0 >> (8 * i + 4)), centred(x1 >> 8 * i),
+                                 centred(x1 >> (8 * i + 4))};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t b0 = centred(x0 >> 4 * i), b1 = centred(x1 >> 4 * i);
+          for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int k = 0; k < NQ; ++k) mma(o[y * 4 + i], a[k], b0, b1);
+            for (int k = 0; k < NQ; ++k) mma(o[2 * y + i][r], a, pb[r][k][0], pb[r][k][1]);
         }
       }
     }
@@ -339,19 +376,23 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(con
 
   // ---- merge the warps, in order -----------------------------------------------------------
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float sum = r < NR ? l[r < NR ? r : 0] : 0.0f;
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (c == 0) s_m[warp][g + 8 * r] = r < NR ? m[r < NR ? r : 0] : -INFINITY, s_l[warp][g + 8 * r] = sum;
-  }
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float sum = l[r][e];
+#pragma unroll
+      for (int x = 4; x <= 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (g == 0) s_m[warp][8 * r + 2 * c + e] = m[r][e], s_l[warp][8 * r + 2 * c + e] = sum;
+    }
   __syncthreads();  // the rings are done with
   float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j)  // tile j's columns 2 c and 2 c + 1: dims 8 c + j % 4 and + 4 of group j / 4
+  for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      part[(warp * kRows + g + 8 * (e >> 1)) * D + j / 4 * kGroup + 8 * c + 4 * (e & 1) + j % 4] = o[j][e];
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        part[(warp * kRows + 8 * r + 2 * c + (e & 1)) * D + j / 2 * kGroup + 4 * g + 2 * (j & 1) + (e >> 1)] = o[j][r][e];
   if (threadIdx.x < kRows) {
     const int r = threadIdx.x;
     float top = -INFINITY, sum = 0.0f;
@@ -384,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D>::kPerSm) attn_kernel(con
 }
 
 // One warp a row: the splits' parts, in order.
-template <typename T, int D>
+template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Attn p) {
   pdl_wait();
   pdl_trigger();
@@ -415,11 +456,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   for (int i = 0; i < D / 32; ++i) io<T>::st(out + lane + 32 * i, acc[i] * inv);
 }
 
+// Rows a block: 8 where that is all, else 16, which share the work of unpacking the codes.
+int row_tile(const Attn& p) { return (int64_t)p.Lq * (p.H / p.c.Hkv) <= 8 ? 8 : 16; }
+
 // Whole waves of resident blocks; a block's share is its own sequence's, so more waves even unequal lengths out, down
-// to 1024 tokens a block (a block writes up to 16 rows of fp32 for the join).
+// to 1024 tokens a block (a block writes its rows in fp32 for the join).
 void plan(Attn& p, int dtype) {
   const int64_t rows = (int64_t)p.Lq * (p.H / p.c.Hkv), keys = (int64_t)p.M << p.c.log_page;
-  p.rtiles = (int)((rows + kRows - 1) / kRows);
+  p.rtiles = (int)((rows + row_tile(p) - 1) / row_tile(p));
   const int64_t base = (int64_t)p.B * p.c.Hkv * p.rtiles;
   const int per_sm = dtype == HCLSM_F32 ? 2 : p.c.D <= 64 ? 4 : 3;
   int64_t s = 1;
@@ -436,33 +480,38 @@ size_t attn_workspace(const Attn& a, int dtype) {
   Attn p = a;
   plan(p, dtype);
   if (p.splits <= 1) return 0;
-  return (size_t)p.B * p.c.Hkv * p.rtiles * p.splits * kRows * (p.c.D * sizeof(float) + sizeof(float2));
+  return (size_t)p.B * p.c.Hkv * p.rtiles * p.splits * row_tile(p) * (p.c.D * sizeof(float) + sizeof(float2));
 }
 
-template <typename T, int D>
+template <typename T, int D, int RT>
 int launch(Attn& p, void* ws, cudaStream_t st) {
-  using Sh = Shape<T, D>;
+  using Sh = Shape<T, D, RT>;
   const int64_t grid = (int64_t)p.B * p.c.Hkv * p.rtiles * p.splits, rows = (int64_t)p.B * p.H * p.Lq;
   if (grid > 0x7fffffff || rows / kWarps > 0x7ffffff0) return HCLSM_ERR_SHAPE;
   if (p.splits > 1) {
     p.part_ml = static_cast<float2*>(ws);
-    p.part_o = reinterpret_cast<float*>(p.part_ml + grid * kRows);
+    p.part_o = reinterpret_cast<float*>(p.part_ml + grid * Sh::kRows);
   }
-  auto f = (int64_t)p.Lq * (p.H / p.c.Hkv) <= 8 ? attn_kernel<T, D, 1> : attn_kernel<T, D, 2>;
+  auto f = attn_kernel<T, D, RT>;
   if (!set_smem_limit(reinterpret_cast<const void*>(f), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
   if (const int rc = launch_pdl(f, (unsigned)grid, kThreads, Sh::kBytes, st, p)) return rc;
   if (p.splits <= 1) return HCLSM_OK;
-  return launch_pdl(join_kernel<T, D>, (unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st, p);
+  return launch_pdl(join_kernel<T, D, Sh::kRows>, (unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st, p);
+}
+
+template <typename T, int D>
+int launch_rows(Attn& p, void* ws, cudaStream_t st) {
+  return row_tile(p) == 8 ? launch<T, D, 1>(p, ws, st) : launch<T, D, 2>(p, ws, st);
 }
 
 int attn(Attn p, int dtype, void* ws, cudaStream_t st) {
   plan(p, dtype);
   const bool f = dtype == HCLSM_F32;
   switch (p.c.D) {
-    case 32: return f ? launch<float, 32>(p, ws, st) : launch<__nv_bfloat16, 32>(p, ws, st);
-    case 64: return f ? launch<float, 64>(p, ws, st) : launch<__nv_bfloat16, 64>(p, ws, st);
-    case 96: return f ? launch<float, 96>(p, ws, st) : launch<__nv_bfloat16, 96>(p, ws, st);
-    default: return f ? launch<float, 128>(p, ws, st) : launch<__nv_bfloat16, 128>(p, ws, st);
+    case 32: return f ? launch_rows<float, 32>(p, ws, st) : launch_rows<__nv_bfloat16, 32>(p, ws, st);
+    case 64: return f ? launch_rows<float, 64>(p, ws, st) : launch_rows<__nv_bfloat16, 64>(p, ws, st);
+    case 96: return f ? launch_rows<float, 96>(p, ws, st) : launch_rows<__nv_bfloat16, 96>(p, ws, st);
+    default: return f ? launch_rows<float, 128>(p, ws, st) : launch_rows<__nv_bfloat16, 128>(p, ws, st);
   }
 }
 
