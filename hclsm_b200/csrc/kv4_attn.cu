@@ -22,6 +22,8 @@ namespace kv4 {
 constexpr int kWarps = 4, kThreads = kWarps * 32, kUnit = 32;
 constexpr int kWaves = 4, kMinKeys = 1024;
 
+// Resident blocks a SM: what the registers of a block allow.
+constexpr int blocks_per_sm(bool f32, int D, int rt) { return f32 ? (D <= 64 ? 3 : 2) : D <= 64 ? 5 - rt : 4 - (rt > 1); }
 // RT: tiles of 8 rows a block.
 template <typename T, int D, int RT> struct Shape {
   static constexpr bool kF32 = sizeof(T) == 4;
@@ -30,12 +32,13 @@ template <typename T, int D, int RT> struct Shape {
   static constexpr int kG = D / kGroup;
   static constexpr int kCodes = kUnit * D / 2, kScales = kUnit * D / 16;  // bytes
   static constexpr int kStage = 2 * (kCodes + kScales);
-  static constexpr int kStages = 4;
+  static constexpr int kStages = D == 128 ? 2 : 3;
   static constexpr int kFrag = kF32 ? kNQ * kG * 2 * 32 * 8 * RT : 0;  // query fragments of fp32 states
   static constexpr int kMerge = kWarps * kRows * D * 4;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kFrag;
-  static constexpr int kPerSm = kF32 ? 2 : D <= 64 ? 4 : 3;
+  static constexpr int kWide = kWarps * 2 * kUnit * kG * 4;  // a unit's scales in fp32
+  static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge) + kFrag + kWide;
+  static constexpr int kPerSm = blocks_per_sm(kF32, D, RT);
 };
 
 // d = a b + c: with a sum of its own, the first product of a sum needs no copy of what it starts from.
@@ -68,27 +71,30 @@ template <int N> __device__ __forceinline__ void pieces(float lo, float hi, uint
     hi -= __uint_as_float(out[i] & 0xffff0000u);
   }
 }
-// Bits 0-3 and 16-19 as packed bf16: 128 + code, and code - 8.
-__device__ __forceinline__ uint32_t biased(uint32_t x) { return (x & 0x000f000fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t centred(uint32_t x) {
-  const uint32_t b = biased(x), k = 0x43084308u;
+// Bits 0-3 and 16-19 as packed bf16: 128 + code, and code - 8.  One three-input operation with 0x43004300 in a register
+// (an instruction takes one constant).
+__device__ __forceinline__ uint32_t biased(uint32_t x, uint32_t k128) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(y) : "r"(x), "r"(k128));
+  return y;
+}
+__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t k128) {
+  const uint32_t b = biased(x, k128), k = 0x43084308u;
   const __nv_bfloat162 r =
       __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&k));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-// A token's scales of all groups.
-template <int G> __device__ __forceinline__ void scales(const unsigned char* at, float (&s)[G]) {
+// A token's scales of all groups, in fp32.
+template <int G> __device__ __forceinline__ void scales(const float* at, float (&s)[G]) {
   if constexpr (G == 4) {
-    const uint2 w = *reinterpret_cast<const uint2*>(at);
-    s[0] = __uint_as_float(w.x << 16), s[1] = __uint_as_float(w.x & 0xffff0000u);
-    s[2] = __uint_as_float(w.y << 16), s[3] = __uint_as_float(w.y & 0xffff0000u);
+    const float4 w = *reinterpret_cast<const float4*>(at);
+    s[0] = w.x, s[1] = w.y, s[2] = w.z, s[3] = w.w;
   } else if constexpr (G == 2) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(at);
-    s[0] = __uint_as_float(w << 16), s[1] = __uint_as_float(w & 0xffff0000u);
+    const float2 w = *reinterpret_cast<const float2*>(at);
+    s[0] = w.x, s[1] = w.y;
   } else {
 #pragma unroll
-    for (int i = 0; i < G; ++i)
-      s[i] = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(at)[i] << 16);
+    for (int i = 0; i < G; ++i) s[i] = at[i];
   }
 }
 
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   // ---- queries: fragments of Q^T, row g of each tile, dims 8 c + i and 8 c + 4 + i of a group side by side ----
   uint32_t qb[Sh::kF32 ? 1 : RT][G][4];
   float q136[Sh::kF32 ? 1 : RT][G][2];  // -136 times the sum of a group of rows 2 c and 2 c + 1
-  uint32_t* frag = reinterpret_cast<uint32_t*>(smem + (Sh::kBytes - Sh::kFrag));
+  uint32_t* frag = reinterpret_cast<uint32_t*>(smem + (Sh::kBytes - Sh::kFrag - Sh::kWide));
   auto row_at = [&](int r) {  // a row's query, or null
     const int row = rt * kRows + r;
     return row < rows ? static_cast<const T*>(p.q.p) + b * p.q.sb + (int64_t)(row / Gq) * p.q.st +
@@ -210,6 +216,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   // which neither keys (four rows a load's half) nor values (four tokens a load) meet in a bank with 64 dims.
   const int key = g & 1 ? (g >> 1) + 2 : (g >> 1) + 2 * (g >> 1 & 2);
   const int tok0 = c + 2 * (c & 2), tok1 = c + 2;
+  float *ks = reinterpret_cast<float*>(smem + (Sh::kBytes - Sh::kWide)) + warp * 2 * kUnit * G, *vs = ks + kUnit * G;
+  uint32_t k128 = 0x43004300u;
+  asm volatile("" : "+r"(k128));
   int s = 0;
   uint32_t phase = 0;
   bool alive = true;
@@ -224,7 +233,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
       break;
     }
     const unsigned char* kq = ring + s * Sh::kStage;
-    const unsigned char *vq = kq + Sh::kCodes, *ks = vq + Sh::kCodes, *vs = ks + Sh::kScales;
+    const unsigned char* vq = kq + Sh::kCodes;
+    if (lane < 8 * G) {  // the scales of the unit as fp32: eight a lane, keys' and then values'
+      const uint4 w = *reinterpret_cast<const uint4*>(vq + Sh::kCodes + lane * 16);
+      float4* to = reinterpret_cast<float4*>(ks + lane * 8);
+      to[0] = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                          __uint_as_float(w.y & 0xffff0000u));
+      to[1] = make_float4(__uint_as_float(w.z << 16), __uint_as_float(w.z & 0xffff0000u), __uint_as_float(w.w << 16),
+                          __uint_as_float(w.w & 0xffff0000u));
+    }
+    __syncwarp();
     const uint32_t hole = holes >> 2 * s & 3u;
     if (++s == ST) s = 0, phase ^= 1;
     const int left = n - u * kUnit;
@@ -237,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
     for (int h = 0; h < 2; ++h) {
       const int t = 16 * h + key;
       float f0[G], f1[G];
-      scales<G>(ks + t * (D / 16), f0);
-      scales<G>(ks + (t + 8) * (D / 16), f1);
+      scales<G>(ks + t * G, f0);
+      scales<G>(ks + (t + 8) * G, f1);
       const uint32_t* row0 = reinterpret_cast<const uint32_t*>(kq + t * (D / 2));
       const uint32_t* row1 = row0 + D;
 #pragma unroll
@@ -257,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
         for (int step = 0; step < 2; ++step) {
           const int i = 8 * step;
           if constexpr (Sh::kF32) {
-            const uint32_t a[4] = {centred(x0 >> i), centred(x1 >> i), centred(x0 >> (i + 4)), centred(x1 >> (i + 4))};
+            const uint32_t a[4] = {centred(x0 >> i, k128), centred(x1 >> i, k128), centred(x0 >> (i + 4), k128), centred(x1 >> (i + 4), k128)};
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -267,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
                 else mma(d[r], a, w.x, w.y);
               }
           } else {
-            const uint32_t a[4] = {biased(x0 >> i), biased(x1 >> i), biased(x0 >> (i + 4)), biased(x1 >> (i + 4))};
+            const uint32_t a[4] = {biased(x0 >> i, k128), biased(x1 >> i, k128), biased(x0 >> (i + 4), k128), biased(x1 >> (i + 4), k128)};
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               if (step == 0)
@@ -333,8 +351,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
 #pragma unroll
     for (int h = 0; h < 2; ++h) {  // 16 tokens
       float f0[G], f1[G];
-      scales<G>(vs + (16 * h + key) * (D / 16), f0);
-      scales<G>(vs + (16 * h + key + 8) * (D / 16), f1);
+      scales<G>(vs + (16 * h + key) * G, f0);
+      scales<G>(vs + (16 * h + key + 8) * G, f1);
       if (valid != 0xffffffffu) {  // what is not there may have any scale, NaN too
         const bool a = valid >> (16 * h + key) & 1u, z = valid >> (16 * h + key + 8) & 1u;
 #pragma unroll
@@ -359,8 +377,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t a[4] = {centred(x0 >> 8 * i), centred(x0 >> (8 * i + 4)), centred(x1 >> 8 * i),
-                                 centred(x1 >> (8 * i + 4))};
+          const uint32_t a[4] = {centred(x0 >> 8 * i, k128), centred(x0 >> (8 * i + 4), k128), centred(x1 >> 8 * i, k128),
+                                 centred(x1 >> (8 * i + 4), k128)};
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -465,7 +483,7 @@ void plan(Attn& p, int dtype) {
   const int64_t rows = (int64_t)p.Lq * (p.H / p.c.Hkv), keys = (int64_t)p.M << p.c.log_page;
   p.rtiles = (int)((rows + row_tile(p) - 1) / row_tile(p));
   const int64_t base = (int64_t)p.B * p.c.Hkv * p.rtiles;
-  const int per_sm = dtype == HCLSM_F32 ? 2 : p.c.D <= 64 ? 4 : 3;
+  const int per_sm = blocks_per_sm(dtype == HCLSM_F32, p.c.D, row_tile(p) / 8);
   int64_t s = 1;
   for (int waves = 1; waves <= kWaves; ++waves) {
     const int64_t n = base > 0 ? (int64_t)num_sms() * per_sm * waves / base : 1;
