@@ -43,81 +43,108 @@ __device__ __forceinline__ uint32_t code(float x, float s, float inv) {
   const bool above = s < 0.0f ? over < 0.0f : over > 0.0f;
   return (uint32_t)(min(max(i + ((above || (over == 0.0f && (i & 1))) ? 1 : 0), -8), 7) + 8);
 }
+// The codes of eight values, four dims a word: adding 1.5 * 2^23 to the quotient rounds it to a whole number (halves to
+// even), which the low bits then are.
+// bf16 values: x * inv and one correction is the quotient itself where fp32 holds it, halves of whole numbers among
+// them, and a quotient of two 8-bit numbers is no nearer to such a half than 2^-17 of it without being it.
+// fp32 values may be: there x * inv, within 2e-6 of the quotient, decides but for a value within 1e-4 of a half, which
+// goes through code(), as does a group whose scale is too small for a reciprocal.
+template <bool EXACT> __device__ __forceinline__ void codes(const float (&v)[8], float s, uint32_t (&run)[2]) {
+  const float inv = 1.0f / s;
+  int r[8];
+  float far = fabsf(s) < 1e-30f ? 1.0f : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float q = v[e] * inv;
+    if (EXACT) q = fmaf(fmaf(-q, s, v[e]), inv, q);
+    const float t = q + 12582912.0f;
+    if (!EXACT) far = fmaxf(far, fabsf(q + (12582912.0f - t)));
+    r[e] = min(__float_as_int(t), 0x4b400000 + 7);
+  }
+  if (far < 0.4999f) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      uint32_t x = (uint32_t)r[4 * w + 3];
+#pragma unroll
+      for (int e = 2; e >= 0; --e) x = x * 16u + (uint32_t)r[4 * w + e];
+      run[w] = x - 0x4b400000u * 0x1111u + 0x8888u;
+    }
+    return;
+  }
+  const float f = fabsf(s) < 1e-30f ? 0x1p64f : 1.0f, sf = s * f, inv_f = 1.0f / sf;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    run[w] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) run[w] |= code(v[4 * w + e] * f, sf, inv_f) << (4 * e);
+  }
+}
 
 struct Write {
   Cache c;
   xattn::View x[2];
   const int32_t* slots;
-  int B, n;
+  int n;
+  uint32_t total;  // threads with work
   int* err;
 };
 
 // blockIdx.y: keys or values.  Eight lanes hold 64 dims of a token (four the 32 behind them): the largest value of each
 // group by shuffles, and each pair of lanes with the same dims of the two groups makes whole words.
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Write p) {
   pdl_wait();
   pdl_trigger();
-  const int kv = blockIdx.y, lanes = p.c.D / 8;
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t total = (int64_t)p.B * p.n * p.c.Hkv * lanes;
-  const bool in = i < total;
-  const int64_t row = in ? i / lanes : 0;
-  const int part = in ? (int)(i - row * lanes) : 0;
-  const int h = (int)(row % p.c.Hkv);
-  const int64_t token = row / p.c.Hkv, b = token / p.n;
-  const int t = (int)(token - b * p.n);
+  constexpr int lanes = D / 8;
+  const int kv = blockIdx.y;
+  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+  const bool in = i < p.total;
+  const uint32_t row = in ? i / lanes : 0, part = in ? i % lanes : 0;
+  const uint32_t token = row / (uint32_t)p.c.Hkv, h = row - token * (uint32_t)p.c.Hkv;
+  const uint32_t b = token / (uint32_t)p.n, t = token - b * (uint32_t)p.n;
   const int slot = in ? p.slots[token] : -1;
   const bool fits = slot >= 0 && (slot >> p.c.log_page) < p.c.pages;
   if (slot >= 0 && !fits) record_error(p.err, HCLSM_ERR_SHAPE);
   float v[8] = {};
-  if (fits) load8(static_cast<const T*>(p.x[kv].p) + b * p.x[kv].sb + (int64_t)t * p.x[kv].st + h * p.x[kv].sh + part * 8, v);
-  float hi = v[0], lo = v[0];
-  bool finite = true;
+  if (fits)
+    load8(static_cast<const T*>(p.x[kv].p) + (int64_t)b * p.x[kv].sb + (int64_t)t * p.x[kv].st + (int64_t)h * p.x[kv].sh + part * 8,
+          v);
+  float hi = v[0], lo = v[0], finite = 0.0f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     hi = fmaxf(hi, v[e]), lo = fminf(lo, v[e]);
-    finite = finite && fabsf(v[e]) <= 3.402823466e38f;
+    finite = fmaf(v[e], 0.0f, finite);  // NaN where one is not
   }
 #pragma unroll
   for (int o = 1; o <= 2; o <<= 1) {
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
   }
-  const uint32_t votes = __ballot_sync(0xffffffffu, !finite);
+  const uint32_t votes = __ballot_sync(0xffffffffu, finite != 0.0f);
   const int lane = threadIdx.x & 31;
   const bool all_finite = (votes >> (lane & ~3) & 15u) == 0;
   const float top = hi >= -lo ? hi : lo;
   __nv_bfloat16 sb = __float2bfloat16_rn(top * -0.125f);
   if (!all_finite) sb = __ushort_as_bfloat16(0x7fc0);
-  float s = __bfloat162float(sb);
+  const float s = __bfloat162float(sb);
   uint32_t run[2] = {0x8888u, 0x8888u};  // the codes of four dims each
-  if (all_finite && s != 0.0f) {
-    // a tiny group is scaled by a power of two, so that the reciprocal is a normal number
-    const float f = fabsf(s) < 1e-30f ? 0x1p64f : 1.0f;
-    s *= f;
-    const float inv = 1.0f / s;
-#pragma unroll
-    for (int e = 0; e < 8; e += 4)
-      run[e >> 2] = code(v[e] * f, s, inv) | code(v[e + 1] * f, s, inv) << 4 | code(v[e + 2] * f, s, inv) << 8 |
-                    code(v[e + 3] * f, s, inv) << 12;
-  }
+  if (all_finite && s != 0.0f) codes<sizeof(T) == 2>(v, s, run);
   const uint32_t other0 = __shfl_xor_sync(0xffffffffu, run[0], 4), other1 = __shfl_xor_sync(0xffffffffu, run[1], 4);
   if (!fits) return;
   const int page = slot >> p.c.log_page, place = slot & (p.c.page - 1);
   const int64_t at = ((int64_t)page * p.c.Hkv + h) * p.c.page + place;
-  uint32_t* words = reinterpret_cast<uint32_t*>(p.c.q[kv] + at * (p.c.D / 2));
+  uint32_t* words = reinterpret_cast<uint32_t*>(p.c.q[kv] + at * (D / 2));
   const int block = part / 8, l = part % 8;
-  if (p.c.D == 96 && block == 0) {  // its eight lanes may lie in two warps: half words
+  if (D == 96 && block == 0) {  // its eight lanes may lie in two warps: half words
     uint16_t* halves = reinterpret_cast<uint16_t*>(words) + l % 4 * 4 + l / 4;
     halves[0] = (uint16_t)run[0], halves[2] = (uint16_t)run[1];
-  } else if (block * 64 + 64 <= p.c.D) {
+  } else if (block * 64 + 64 <= D) {
     if (l < 4)
       *reinterpret_cast<uint2*>(words + block * 8 + l * 2) = make_uint2(run[0] | other0 << 16, run[1] | other1 << 16);
   } else {
     words[block * 8 + l] = run[0] | run[1] << 16;
   }
-  if (part % 4 == 0) p.c.scale[kv][at * (p.c.D / kGroup) + part / 4] = __bfloat16_as_ushort(sb);
+  if (part % 4 == 0) p.c.scale[kv][at * (D / kGroup) + part / 4] = __bfloat16_as_ushort(sb);
 }
 
 struct Read {
@@ -129,41 +156,59 @@ struct Read {
 };
 
 // Eight dims a thread, in the output's order; blockIdx.y keys or values, blockIdx.z the entry.
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Read p) {
   pdl_wait();
   pdl_trigger();
+  constexpr uint32_t lanes = D / 8;
   const int kv = blockIdx.y;
   const int64_t b = blockIdx.z;
-  const uint32_t lanes = p.c.D / 8, row = lanes * p.c.Hkv;
   const int T_all = p.M << p.c.log_page;
   const int n = p.lens ? min(max(p.lens[b], 0), T_all) : T_all;
-  const uint32_t total = row * (uint32_t)T_all;
+  const uint32_t total = lanes * p.c.Hkv * (uint32_t)T_all;
   T* out = static_cast<T*>(p.out[kv]) + b * (int64_t)total * 8;
   for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
-    const uint32_t t = i / row, h = (i - t * row) / lanes, part = i - t * row - h * lanes;
+    const uint32_t row = i / lanes, part = i % lanes, t = row / (uint32_t)p.c.Hkv, h = row - t * (uint32_t)p.c.Hkv;
     float v[8] = {};
     if ((int)t < n) {
       const int page = p.table[b * p.M + (t >> p.c.log_page)];
       if ((unsigned)page < (unsigned)p.c.pages) {
         const int64_t at = ((int64_t)page * p.c.Hkv + h) * p.c.page + (t & (p.c.page - 1));
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(p.c.q[kv] + at * (p.c.D / 2));
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(p.c.q[kv] + at * (D / 2));
         const uint32_t block = part / 8, l = part % 8;
         uint32_t codes;  // of the eight dims, ascending
-        if (block * 64 + 64 <= (uint32_t)p.c.D) {
+        if (block * 64 + 64 <= D) {
           const uint2 w = *reinterpret_cast<const uint2*>(words + block * 8 + l % 4 * 2);
           codes = __byte_perm(w.x, w.y, l < 4 ? 0x5410 : 0x7632);
         } else {
           codes = words[block * 8 + l];
         }
-        const float s = __uint_as_float((uint32_t)p.c.scale[kv][at * (p.c.D / kGroup) + part / 4] << 16);
+        const float s = __uint_as_float((uint32_t)p.c.scale[kv][at * (D / kGroup) + part / 4] << 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = s * (float)((int)(codes >> (4 * e) & 15u) - 8);
+        for (int e = 0; e < 8; ++e)  // 2^23 + code, less 2^23 + 8
+          v[e] = s * (__uint_as_float(0x4b000000u | (codes >> (4 * e) & 15u)) - 8388616.0f);
       } else {
         record_error(p.err, HCLSM_ERR_SHAPE);
       }
     }
     store8(out + (int64_t)i * 8, v);
+  }
+}
+
+template <typename T> int launch_write(const Write& p, dim3 g, cudaStream_t st) {
+  switch (p.c.D) {
+    case 32: return launch_pdl(write_kernel<T, 32>, g, kThreads, 0, st, p);
+    case 64: return launch_pdl(write_kernel<T, 64>, g, kThreads, 0, st, p);
+    case 96: return launch_pdl(write_kernel<T, 96>, g, kThreads, 0, st, p);
+    default: return launch_pdl(write_kernel<T, 128>, g, kThreads, 0, st, p);
+  }
+}
+template <typename T> int launch_read(const Read& p, dim3 g, cudaStream_t st) {
+  switch (p.c.D) {
+    case 32: return launch_pdl(read_kernel<T, 32>, g, kThreads, 0, st, p);
+    case 64: return launch_pdl(read_kernel<T, 64>, g, kThreads, 0, st, p);
+    case 96: return launch_pdl(read_kernel<T, 96>, g, kThreads, 0, st, p);
+    default: return launch_pdl(read_kernel<T, 128>, g, kThreads, 0, st, p);
   }
 }
 
@@ -214,13 +259,12 @@ extern "C" int hclsm_kv4_write(const hclsm_kv4_cache* c, const hclsm_view* k, co
   p.c = kv4::cache(c);
   p.x[0] = xattn::view(*k, B, n, c->Hkv), p.x[1] = xattn::view(*v, B, n, c->Hkv);
   if (!kv4::row16(p.x[0], c->dtype) || !kv4::row16(p.x[1], c->dtype)) return HCLSM_ERR_ALIGN;
-  p.slots = slots, p.B = B, p.n = n, p.err = device_err_ptr();
-  const int64_t grid = ((int64_t)B * n * c->Hkv * (c->D / 8) + kv4::kThreads - 1) / kv4::kThreads;
-  if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  const int64_t total = (int64_t)B * n * c->Hkv * (c->D / 8), grid = (total + kv4::kThreads - 1) / kv4::kThreads;
+  if (total > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  p.slots = slots, p.n = n, p.total = (uint32_t)total, p.err = device_err_ptr();
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 g((unsigned)grid, 2);
-  return c->dtype == HCLSM_F32 ? launch_pdl(kv4::write_kernel<float>, g, kv4::kThreads, 0, st, p)
-                               : launch_pdl(kv4::write_kernel<__nv_bfloat16>, g, kv4::kThreads, 0, st, p);
+  return c->dtype == HCLSM_F32 ? kv4::launch_write<float>(p, g, st) : kv4::launch_write<__nv_bfloat16>(p, g, st);
 }
 
 extern "C" int hclsm_kv4_read(const hclsm_kv4_cache* c, const int32_t* table, int32_t B, int32_t M, void* k, void* v,
@@ -238,8 +282,7 @@ extern "C" int hclsm_kv4_read(const hclsm_kv4_cache* c, const int32_t* table, in
   const int64_t blocks = (total + kv4::kThreads - 1) / kv4::kThreads, most = (int64_t)num_sms() * 16 / B + 1;
   const dim3 g((unsigned)(blocks < most ? blocks : most), 2, (unsigned)B);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return c->dtype == HCLSM_F32 ? launch_pdl(kv4::read_kernel<float>, g, kv4::kThreads, 0, st, p)
-                               : launch_pdl(kv4::read_kernel<__nv_bfloat16>, g, kv4::kThreads, 0, st, p);
+  return c->dtype == HCLSM_F32 ? kv4::launch_read<float>(p, g, st) : kv4::launch_read<__nv_bfloat16>(p, g, st);
 }
 
 extern "C" size_t hclsm_kv4_attn_workspace_size(const hclsm_kv4_cache* c, int32_t B, int32_t M, int32_t Lq,

@@ -11,7 +11,7 @@ int num_sms();
 
 namespace pages {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kCluster = 8;
+constexpr int kThreads = 1024, kFewThreads = 256, kCluster = 8;
 
 struct Resize {
   int32_t *table, *stack, *n_free;
@@ -20,47 +20,43 @@ struct Resize {
   int* err;
 };
 
-struct Counts {
-  int released, wanted;
-};
-__device__ __forceinline__ Counts add(Counts a, Counts b) {
-  return Counts{a.released + b.released, a.wanted + b.wanted};
-}
-
-// Exclusive sums over the block's threads; `total` the block's.
-__device__ __forceinline__ Counts scan(Counts v, Counts* warp_sum, Counts& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Counts s = v;
+// Exclusive sums of (released, wanted) over the block's threads; total: the block's.
+__device__ __forceinline__ int2 scan(int2 v, int2* warp_sum, int2& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int2 s = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const Counts t{__shfl_up_sync(0xffffffffu, s.released, o), __shfl_up_sync(0xffffffffu, s.wanted, o)};
-    if (lane >= o) s = add(s, t);
+    const int x = __shfl_up_sync(0xffffffffu, s.x, o), y = __shfl_up_sync(0xffffffffu, s.y, o);
+    if (lane >= o) s.x += x, s.y += y;
   }
   __syncthreads();
   if (lane == 31) warp_sum[warp] = s;
   __syncthreads();
-  Counts before{0, 0};
-  total = Counts{0, 0};
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before = add(before, warp_sum[w]);
-    total = add(total, warp_sum[w]);
+  int2 w = lane < warps ? warp_sum[lane] : make_int2(0, 0);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, w.x, o), y = __shfl_up_sync(0xffffffffu, w.y, o);
+    if (lane >= o) w.x += x, w.y += y;
   }
-  return Counts{before.released + s.released - v.released, before.wanted + s.wanted - v.wanted};
+  total = make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
+  const int before = max(warp - 1, 0);
+  const int x = __shfl_sync(0xffffffffu, w.x, before), y = __shfl_sync(0xffffffffu, w.y, before);
+  return make_int2((warp ? x : 0) + s.x - v.x, (warp ? y : 0) + s.y - v.y);
 }
 
-// One cluster.  Each block forms all the sums (entries are few next to their pages); the pages are shared out: a
-// team of warps an entry.
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) resize_kernel(
-    const __grid_constant__ Resize p) {
+// One cluster (of one block where the table is small).  Each block forms all the sums, since entries are few next to
+// their pages; the pages are shared out among all threads by their place in the order, so entries of any size cost
+// the same.  Pages of an order's run: a search in the sums of up to a block's threads of entries.
+__global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant__ Resize p) {
   namespace cg = cooperative_groups;
-  __shared__ Counts warp_sum[kWarps], off[kThreads];
+  __shared__ int2 warp_sum[kThreads / 32], off[kThreads + 1];
   __shared__ int2 span[kThreads];  // pages an entry had, has
   __shared__ int bad;
   pdl_wait();
   pdl_trigger();
   const cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int warp = (int)cluster.block_rank() * kWarps + (tid >> 5);
+  const int tid = threadIdx.x, nt = blockDim.x;
+  const int me = (int)cluster.block_rank() * nt + tid, all = (int)cluster.num_blocks() * nt;
   if (tid == 0) bad = 0;
   __syncthreads();
   const int n = *p.n_free;
@@ -68,68 +64,87 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) res
   // pass 0 counts and checks, 1 releases, 2 takes
   int64_t released = 0, wanted = 0;  // over all entries
   for (int pass = 0; pass < 3; ++pass) {
-    Counts done{0, 0};
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-      const int b = b0 + tid;
-      int2 s = make_int2(0, 0);
-      bool wrong = false;
-      if (b < p.B) {
-        const int from = p.old_lens[b], to = p.new_lens[b];
-        if (from < 0 || to < 0 || from > most || to > most) wrong = true;
-        else s = make_int2((int)(((int64_t)from + (1 << p.shift) - 1) >> p.shift),
-                           (int)(((int64_t)to + (1 << p.shift) - 1) >> p.shift));
+    if (pass == 1 && released == 0) continue;
+    if (pass == 2 && wanted == 0) continue;
+    int2 done = make_int2(0, 0);
+    for (int b0 = 0; b0 < p.B; b0 += nt) {
+      const int b = b0 + tid, entries = min(nt, p.B - b0);
+      if (pass == 0 || p.B > nt) {  // one round of entries stays where it is
+        int2 s = make_int2(0, 0);
+        if (b < p.B) {
+          const int from = p.old_lens[b], to = p.new_lens[b];
+          if (from < 0 || to < 0 || from > most || to > most)
+            bad = 1;
+          else
+            s = make_int2((int)(((int64_t)from + (1 << p.shift) - 1) >> p.shift),
+                          (int)(((int64_t)to + (1 << p.shift) - 1) >> p.shift));
+        }
+        int2 total;
+        const int2 at = scan(make_int2(max(s.x - s.y, 0), max(s.y - s.x, 0)), warp_sum, total);
+        span[tid] = s;
+        off[tid] = at;  // behind the last entry: the total
+        if (tid == 0) off[nt] = total;
+        __syncthreads();
       }
-      if (wrong) bad = 1;
-      Counts total;
-      const Counts at = add(done, scan(Counts{max(s.x - s.y, 0), max(s.y - s.x, 0)}, warp_sum, total));
-      span[tid] = s;
-      off[tid] = at;
-      done = add(done, total);
-      if (pass == 0) released += total.released, wanted += total.wanted;
-      __syncthreads();
-      // Each entry's pages by a team of warps.  Pass 0: all blocks check all of them, so that all decide alike.
-      const int entries = min(kThreads, p.B - b0);
-      const int warps = pass == 0 ? kWarps : kWarps * kCluster, mine = pass == 0 ? tid >> 5 : warp;
-      const int team = max(1, warps / entries), lanes = team * 32;
-      for (int e = mine / team; e < entries && mine / team < warps / team; e += warps / team) {
-        const int2 w = span[e];
-        const Counts o = off[e];
-        int32_t* row = p.table + (int64_t)(b0 + e) * p.M;
-        const int i0 = mine % team * 32 + lane;
-        if (pass == 0) {
-          for (int j = w.y + i0; j < w.x; j += lanes)
-            if ((unsigned)row[j] >= (unsigned)p.P) bad = 1;
-        } else if (pass == 1) {
-          for (int j = w.y + i0; j < w.x; j += lanes) {
-            p.stack[n + (int)released - 1 - (o.released + j - w.y)] = row[j];
-            row[j] = -1;
-          }
-        } else {
-          for (int j = w.x + i0; j < w.y; j += lanes) {
-            int32_t* top = p.stack + n + (int)released - 1 - (o.wanted + j - w.x);
-            row[j] = *top;
-            *top = -1;
+      const int2 total = off[entries];
+      // the pages of these entries, in order
+      const int count = pass == 2 ? total.y : total.x;
+      // four pages at a time: a thread waits for memory once for them
+      for (int i0 = me; i0 < count; i0 += 4 * all) {
+        int32_t* at[4];
+        int32_t page[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = i0 + e * all;
+          at[e] = nullptr;
+          if (i >= count) continue;
+          int lo = 0;  // the last entry that begins at or before i: the one with the page
+#pragma unroll
+          for (int step = kThreads / 2; step > 0; step >>= 1)
+            if (lo + step < entries && (pass == 2 ? off[lo + step].y : off[lo + step].x) <= i) lo += step;
+          at[e] = p.table + (int64_t)(b0 + lo) * p.M + (pass == 2 ? span[lo].x + i - off[lo].y : span[lo].y + i - off[lo].x);
+          page[e] = pass == 2 ? p.stack[n + (int)released - 1 - (done.y + i)] : *at[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!at[e]) continue;
+          const int i = i0 + e * all;
+          if (pass == 0) {
+            if ((unsigned)page[e] >= (unsigned)p.P) bad = 1;
+          } else if (pass == 1) {
+            p.stack[n + (int)released - 1 - (done.x + i)] = page[e];
+            *at[e] = -1;
+          } else {
+            *at[e] = page[e];
+            p.stack[n + (int)released - 1 - (done.y + i)] = -1;
           }
         }
       }
-      __syncthreads();
+      done.x += total.x, done.y += total.y;
+      if (p.B > nt) __syncthreads();
     }
     if (pass == 0) {
+      released = done.x, wanted = done.y;
       if (n < 0 || n > p.P || n + released > p.P || wanted > n + released) {
         if (tid == 0) bad = 1;
       } else {  // the pages that were on the stack before and are taken now
-        for (int i = tid; i < (int)(wanted - released); i += kThreads)
+#pragma unroll 8
+        for (int i = me; i < (int)(wanted - released); i += all)
           if ((unsigned)p.stack[n - 1 - i] >= (unsigned)p.P) bad = 1;
       }
-      __syncthreads();
-      if (bad) {  // the same in every block
-        if (tid == 0) record_error(p.err, HCLSM_ERR_SHAPE);
+      cluster.sync();  // the checks before the first change
+      int any = 0;
+      for (int r = 0; r < (int)cluster.num_blocks(); ++r) any |= *cluster.map_shared_rank(&bad, r);
+      cluster.sync();  // no block leaves while others read its flag
+      if (any) {
+        if (me == 0) record_error(p.err, HCLSM_ERR_SHAPE);
         return;
       }
+    } else {
+      cluster.sync();  // the releases before the first taking
     }
-    cluster.sync();  // the checks before the first change, the releases before the first taking
   }
-  if (warp == 0 && lane == 0) *p.n_free = n + (int)(released - wanted);
+  if (me == 0) *p.n_free = n + (int)(released - wanted);
 }
 
 struct Slots {
@@ -138,19 +153,36 @@ struct Slots {
   int B, M, n, shift;
 };
 
-__global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Slots p) {
+// Four slots a thread, blockIdx.y the entry; `wide`: a row of slots is whole 16 bytes.
+__global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Slots p, int wide) {
   pdl_wait();
   pdl_trigger();
-  const int64_t total = (int64_t)p.B * p.n;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int b = (int)(i / p.n), j = (int)(i - (int64_t)b * p.n);
-    const int64_t at = (int64_t)p.start[b] + j;
-    int slot = -1;
-    if (at >= 0 && at < ((int64_t)p.M << p.shift) && (!p.count || j < p.count[b])) {
-      const int page = p.table[(int64_t)b * p.M + (at >> p.shift)];
-      if (page >= 0) slot = (int)((uint32_t)page << p.shift | ((uint32_t)at & ((1u << p.shift) - 1)));
+  const uint32_t mask = (1u << p.shift) - 1;
+  const int64_t most = (int64_t)p.M << p.shift;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) {
+    const int32_t* row = p.table + (int64_t)b * p.M;
+    int32_t* out = p.slots + (int64_t)b * p.n;
+    const int64_t start = p.start[b];
+    const int count = p.count ? min(p.count[b], p.n) : p.n;
+    for (int64_t j = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; j < p.n; j += (int64_t)gridDim.x * 1024) {
+      int s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t at = start + j + e;
+        s[e] = -1;
+        if (j + e < count && at >= 0 && at < most) {
+          const int page = row[at >> p.shift];
+          if (page >= 0) s[e] = (int)((uint32_t)page << p.shift | ((uint32_t)at & mask));
+        }
+      }
+      if (wide) {
+        *reinterpret_cast<int4*>(out + j) = make_int4(s[0], s[1], s[2], s[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (j + e < p.n) out[j + e] = s[e];
+      }
     }
-    p.slots[i] = slot;
   }
 }
 
@@ -169,11 +201,22 @@ using namespace hclsm;
 extern "C" int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P,
                                   int32_t page, const int32_t* old_lens, const int32_t* new_lens, void* stream) {
   if (B < 0 || M < 0 || P < 0 || !pages::power_of_2(page)) return HCLSM_ERR_SHAPE;
-  if ((int64_t)P * page > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  if ((int64_t)P * page > 0x7fffffff || (int64_t)B * M > 0x7fffffff) return HCLSM_ERR_SHAPE;
   if (B == 0) return HCLSM_OK;
   if ((!table && M) || (!stack && P) || !n_free || !old_lens || !new_lens) return HCLSM_ERR_NULL;
   pages::Resize p = {table, stack, n_free, old_lens, new_lens, B, M, P, pages::log2_of(page), device_err_ptr()};
-  return launch_pdl(pages::resize_kernel, pages::kCluster, pages::kThreads, 0, static_cast<cudaStream_t>(stream), p);
+  // one small block takes a table of a few thousand pages faster than a cluster meets at its barriers
+  const bool few = (int64_t)B * M <= 8192 && B <= pages::kFewThreads;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = few ? 1 : pages::kCluster, cfg.blockDim = few ? pages::kFewThreads : pages::kThreads;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = few ? 1 : pages::kCluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, pages::resize_kernel, p) == cudaSuccess ? HCLSM_OK : HCLSM_ERR_LAUNCH;
 }
 
 extern "C" int hclsm_page_slots(const int32_t* table, int32_t B, int32_t M, int32_t page, const int32_t* start,
@@ -183,7 +226,8 @@ extern "C" int hclsm_page_slots(const int32_t* table, int32_t B, int32_t M, int3
   if (total == 0) return HCLSM_OK;
   if ((!table && M) || !start || !slots) return HCLSM_ERR_NULL;
   pages::Slots p = {table, start, count, slots, B, M, n, pages::log2_of(page)};
-  const int64_t blocks = (total + 255) / 256, most = (int64_t)num_sms() * 32;
-  return launch_pdl(pages::slots_kernel, (unsigned)(blocks < most ? blocks : most), 256, 0,
-                    static_cast<cudaStream_t>(stream), p);
+  const int64_t blocks = ((int64_t)n + 1023) / 1024, most = (int64_t)num_sms() * 8 / B + 1;
+  const int wide = n % 4 == 0 && reinterpret_cast<uintptr_t>(slots) % 16 == 0;
+  return launch_pdl(pages::slots_kernel, dim3((unsigned)(blocks < most ? blocks : most), (unsigned)(B < 65535 ? B : 65535)), 256, 0,
+                    static_cast<cudaStream_t>(stream), p, wide);
 }

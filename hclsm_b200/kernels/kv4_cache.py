@@ -9,7 +9,7 @@ with others.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 from torch import Tensor
@@ -19,7 +19,7 @@ from .. import _lib
 __all__ = ["Kv4Cache", "kv4_write", "kv4_read", "kv4_attention"]
 
 
-@dataclass
+@dataclass(init=False)
 class Kv4Cache:
     """The cache's tensors, all contiguous: k, v (pages, Hkv, page, D / 2) uint8, k_scale, v_scale (pages, Hkv, page,
     D / 32) bfloat16; dtype (float32 or bfloat16) of the states that are written and read.  D is 32, 64, 96 or 128; page
@@ -30,9 +30,31 @@ class Kv4Cache:
     k_scale: Tensor
     v_scale: Tensor
     dtype: torch.dtype = torch.bfloat16
+    # (addresses, what _args returns) of the tensors as last checked, or None
+    _packed: tuple | None = field(init=False, repr=False, compare=False)
+
+    def __init__(self, k, v, k_scale, v_scale, dtype=torch.bfloat16):
+        d = self.__dict__  # past __setattr__: a microsecond less
+        d["k"], d["v"], d["k_scale"], d["v_scale"], d["dtype"], d["_packed"] = k, v, k_scale, v_scale, dtype, None
+
+    def __setattr__(self, name, value):
+        self.__dict__[name] = value
+        self.__dict__["_packed"] = None  # another tensor: checked and packed at the next call
+
+    def __getstate__(self):
+        return {**self.__dict__, "_packed": None}  # a copy's tensors are elsewhere
 
     def _args(self):
-        """(hclsm_kv4_cache, Hkv, D, device) of the present tensors."""
+        """(hclsm_kv4_cache, Hkv, D, device, its index) for a call.  A tensor that was assigned, copied or given other
+        memory since the last call is checked and its address taken anew: a kernel only ever sees the memory of
+        the present tensors."""
+        at = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr())
+        packed = self._packed
+        if packed is None or packed[0] != at:
+            packed = self.__dict__["_packed"] = (at, self._check(at))
+        return packed[1]
+
+    def _check(self, at):
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
         dev = _lib.require_cuda(k, v, ks, vs)
         if k.dim() != 4:
@@ -50,8 +72,7 @@ class Kv4Cache:
         if (ks.shape != shape or vs.shape != shape or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16
                 or not ks.is_contiguous() or not vs.is_contiguous()):
             raise ValueError(f"k_scale and v_scale must be contiguous {shape} bfloat16")
-        return _lib.KV4_CACHE.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), P, Hkv, page, D,
-                                   _lib.dtype_code(self.dtype)), Hkv, D, dev
+        return _lib.KV4_CACHE.pack(*at, P, Hkv, page, D, _lib.dtype_code(self.dtype)), Hkv, D, dev, k.get_device()
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 32, dtype=torch.bfloat16,
@@ -69,7 +90,8 @@ class Kv4Cache:
 
 
 def _no_derivatives(what, cache, *tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (cache.k_scale, cache.v_scale, *tensors)):
+    if torch.is_grad_enabled() and (cache.k_scale.requires_grad or cache.v_scale.requires_grad
+                                    or any(t.requires_grad for t in tensors)):
         raise NotImplementedError(f"{what} has no gradients: call it under torch.no_grad()")
     if _lib.in_dual_level():
         _lib.no_tangents(cache.k_scale, cache.v_scale, *tensors)
@@ -87,8 +109,9 @@ def kv4_write(cache: Kv4Cache, k: Tensor, v: Tensor, slots: Tensor) -> None:
     sets the device error word.  The slots of one call must differ: of tokens that share one, what is kept is
     undefined.  No gradients: k and v that require them are refused."""
     _no_derivatives("kv4_write", cache, k, v)
-    c, Hkv, D, dev = cache._args()
-    _lib.require_cuda(cache.k, k, v)
+    c, Hkv, D, dev, index = cache._args()
+    if k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"k and v must be on {dev}, got {k.device} and {v.device}")
     if k.dim() != 4 or v.shape != k.shape or k.shape[2:] != (Hkv, D):
         raise ValueError(f"k and v must be (B, tokens, {Hkv}, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
@@ -107,7 +130,7 @@ def kv4_read(cache: Kv4Cache, table: Tensor, lens: Tensor | None = None):
     (default all; clamped to [0, T]) of the pages that table (B, T / page) names, as the values they stand for,
     zeros after them.  A page outside the cache below the length reads as zeros and sets the device error word."""
     _no_derivatives("kv4_read", cache)
-    c, Hkv, D, dev = cache._args()
+    c, Hkv, D, dev, _ = cache._args()
     table = _table(table, dev)
     B, M = table.shape
     lens = _lib.index32(lens, (B,), "lens", dev)
@@ -123,8 +146,9 @@ def kv4_attention(q: Tensor, cache: Kv4Cache, table: Tensor, lens: Tensor | None
     clamped to the table's) of the pages that table (B, M) names; H is a multiple of Hkv.  An entry without tokens
     gives zeros; tokens of a page outside the cache do not count and set the device error word.  No gradients."""
     _no_derivatives("kv4_attention", cache, q)
-    c, Hkv, D, dev = cache._args()
-    _lib.require_cuda(cache.k, q)
+    c, Hkv, D, dev, index = cache._args()
+    if q.get_device() != index:
+        raise ValueError(f"q must be on {dev}, got {q.device}")
     table = _table(table, dev)
     B, M = table.shape
     if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
