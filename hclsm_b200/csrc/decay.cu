@@ -53,7 +53,8 @@ __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast
 // The state stays in registers (4 x 4 values a thread and 64 rows) between chunks; shared memory holds the copy that
 // the queries read.
 template <typename T, int DP, bool SUMS>
-__global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ Pass p) {
+__global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ Batch bt) {
+  const Pass& p = bt.p[blockIdx.x % bt.n];
   extern __shared__ __align__(16) unsigned char raw[];
   Smem<DP>& s = *reinterpret_cast<Smem<DP>*>(raw);
   constexpr int kXs = Smem<DP>::kXs, R = DP / 64;
@@ -61,9 +62,10 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
   pdl_trigger();
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int tiles = (p.Dv + kE - 1) / kE;
-  const int e0 = (int)(blockIdx.x % tiles) * kE;
-  const int seg = (int)(blockIdx.x / tiles % p.segs);
-  const int64_t bh = blockIdx.x / tiles / p.segs;
+  const uint32_t block = blockIdx.x / bt.n;
+  const int e0 = (int)(block % tiles) * kE;
+  const int seg = (int)(block / tiles % p.segs);
+  const int64_t bh = block / tiles / p.segs;
   const int64_t b = bh / p.H;
   const int h = (int)(bh - b * p.H), r = p.rev ? 1 : 0;
   const int n = length(p, b);
@@ -241,13 +243,14 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
 
 // The segments' sums become their first states; the state behind the last one (in the pass's order) goes to `last`.
 // Eight sums are asked for at a time, so a thread waits for memory once in eight segments.
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Pass p, int chunk) {
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Batch bt, int chunk) {
+  const Pass& p = bt.p[blockIdx.x % bt.n];
   __shared__ float2 s_g[2];
   pdl_wait();
   pdl_trigger();
   const int64_t sz = (int64_t)p.Dk * p.Dv;
   const int64_t per = (sz + 127) / 128;
-  const int64_t bh = blockIdx.x / per, i = blockIdx.x % per * 128 + threadIdx.x;
+  const int64_t block = blockIdx.x / bt.n, bh = block / per, i = block % per * 128 + threadIdx.x;
   const int64_t b = bh / p.H;
   const int h = (int)(bh - b * p.H), n = length(p, b), span = p.seg_chunks * chunk;
   // of a whole segment and of the incomplete one
@@ -276,34 +279,36 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Pass 
   if (p.last) p.last[bh * sz + i] = p.last_f * v;
 }
 
-int join(const Pass& p, int chunk, cudaStream_t st) {
-  const int64_t grid = (int64_t)p.B * p.H * (((int64_t)p.Dk * p.Dv + 127) / 128);
+int join(const Batch& b, int chunk, cudaStream_t st) {
+  const Pass& p = b.p[0];
+  const int64_t grid = (int64_t)b.n * p.B * p.H * (((int64_t)p.Dk * p.Dv + 127) / 128);
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  return launch_pdl(join_kernel, (unsigned)grid, 128, 0, st, p, chunk);
+  return launch_pdl(join_kernel, (unsigned)grid, 128, 0, st, b, chunk);
 }
 
 template <typename T, int DP, bool SUMS>
-int launch_simt(const Pass& p, cudaStream_t st) {
+int launch_simt(const Batch& b, cudaStream_t st) {
   auto fn = simt_kernel<T, DP, SUMS>;
   if (!set_smem_limit(reinterpret_cast<const void*>(fn), sizeof(Smem<DP>))) return HCLSM_ERR_LAUNCH;
-  const int64_t grid = (int64_t)p.B * p.H * p.segs * ((p.Dv + kE - 1) / kE);
+  const Pass& p = b.p[0];
+  const int64_t grid = (int64_t)b.n * p.B * p.H * p.segs * ((p.Dv + kE - 1) / kE);
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
-  return launch_pdl(fn, (unsigned)grid, kThreads, sizeof(Smem<DP>), st, p);
+  return launch_pdl(fn, (unsigned)grid, kThreads, sizeof(Smem<DP>), st, b);
 }
 
 template <typename T>
-int simt_pass(Pass p, cudaStream_t st) {
-  cut(p, kC, (int64_t)p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
+int simt_run(const Batch& b, cudaStream_t st) {
+  const Pass& p = b.p[0];
   if (p.segs > 1) {
-    if (const int rc = p.Dk <= 64 ? launch_simt<T, 64, true>(p, st) : launch_simt<T, 128, true>(p, st)) return rc;
-    if (const int rc = join(p, kC, st)) return rc;
+    if (const int rc = p.Dk <= 64 ? launch_simt<T, 64, true>(b, st) : launch_simt<T, 128, true>(b, st)) return rc;
+    if (const int rc = join(b, kC, st)) return rc;
   }
-  return p.Dk <= 64 ? launch_simt<T, 64, false>(p, st) : launch_simt<T, 128, false>(p, st);
+  return p.Dk <= 64 ? launch_simt<T, 64, false>(b, st) : launch_simt<T, 128, false>(b, st);
 }
 
-size_t simt_part_bytes(Pass p) {
-  cut(p, kC, (int64_t)p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
-  return p.segs > 1 ? (size_t)p.B * p.H * p.segs * p.Dk * p.Dv * sizeof(float) : 0;
+void simt_cut(Batch& b) {
+  const Pass& p = b.p[0];
+  cut(b, kC, 1, (int64_t)b.n * p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
 }
 
 // ---- one token -------------------------------------------------------------------------------
@@ -422,15 +427,30 @@ Pass grad_k(const hclsm_decay_args* a) {
   return p;
 }
 
-size_t part_bytes(const Pass& p, int dtype) {
-  return dtype == HCLSM_BF16 && tc_ok(p) ? tc_part_bytes(p) : simt_part_bytes(p);
+// The passes of a call, those of the same sizes together.
+Batch forward_batch(const hclsm_decay_args* a) {
+  Batch b = {};
+  b.p[b.n++] = forward(a);
+  return b;
 }
-int pass(Pass p, int dtype, void* ws, cudaStream_t st) {
-  p.part = static_cast<float*>(ws);
-  if (dtype == HCLSM_BF16 && tc_ok(p)) return tc_pass(p, st);
-  return dtype == HCLSM_F32 ? simt_pass<float>(p, st) : simt_pass<__nv_bfloat16>(p, st);
+int backward_batches(const hclsm_decay_args* a, Batch (&b)[2]) {
+  b[0] = b[1] = Batch{};
+  b[0].p[b[0].n++] = grad_k(a);
+  b[0].p[b[0].n++] = grad_q(a);
+  Batch& v = a->D == a->Dv ? b[0] : b[1];
+  v.p[v.n++] = grad_v(a);
+  return b[1].n ? 2 : 1;
 }
-size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
+// Cut into segments; the workspace's bytes, with the parts placed in it.
+size_t plan(Batch& b, int dtype, void* ws) {
+  if (dtype == HCLSM_BF16 && tc_ok(b)) tc_cut(b);
+  else simt_cut(b);
+  return parts(b, ws);
+}
+int run(const Batch& b, int dtype, cudaStream_t st) {
+  if (dtype == HCLSM_BF16 && tc_ok(b)) return tc_run(b, st);
+  return dtype == HCLSM_F32 ? simt_run<float>(b, st) : simt_run<__nv_bfloat16>(b, st);
+}
 
 // Without tokens the state passes through.
 int only_state(float* to, const float* from, size_t n, cudaStream_t st) {
@@ -447,7 +467,8 @@ using namespace hclsm;
 
 extern "C" size_t hclsm_decay_attn_fwd_workspace_size(const hclsm_decay_args* a) {
   if (decay::check(a)) return 0;
-  return decay::part_bytes(decay::forward(a), a->dtype);
+  decay::Batch b = decay::forward_batch(a);
+  return decay::plan(b, a->dtype, nullptr);
 }
 
 extern "C" int hclsm_decay_attn_fwd(const hclsm_decay_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -456,17 +477,23 @@ extern "C" int hclsm_decay_attn_fwd(const hclsm_decay_args* a, void* ws, size_t 
   if (a->B == 0) return HCLSM_OK;
   if (a->L == 0) return decay::only_state(a->s1, a->s0, (size_t)a->B * a->H * a->D * a->Dv, st);
   if (!a->q.p || !a->k.p || !a->v.p || !a->o || !a->log_decay) return HCLSM_ERR_NULL;
-  const decay::Pass p = decay::forward(a);
-  const size_t need = decay::part_bytes(p, a->dtype);
+  decay::Batch b = decay::forward_batch(a);
+  const size_t need = decay::plan(b, a->dtype, ws);
   if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
-  return decay::pass(p, a->dtype, ws, st);
+  return decay::run(b, a->dtype, st);
 }
 
 extern "C" size_t hclsm_decay_attn_bwd_workspace_size(const hclsm_decay_args* a) {
   if (decay::check(a)) return 0;
-  return decay::max3(decay::part_bytes(decay::grad_q(a), a->dtype), decay::part_bytes(decay::grad_v(a), a->dtype),
-                     decay::part_bytes(decay::grad_k(a), a->dtype));
+  decay::Batch b[2];
+  const int n = decay::backward_batches(a, b);
+  size_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    const size_t need = decay::plan(b[i], a->dtype, nullptr);
+    most = need > most ? need : most;
+  }
+  return most;
 }
 
 extern "C" int hclsm_decay_attn_bwd(const hclsm_decay_args* a, void* ws, size_t ws_bytes, void* stream) {
@@ -479,9 +506,13 @@ extern "C" int hclsm_decay_attn_bwd(const hclsm_decay_args* a, void* ws, size_t 
   const size_t need = hclsm_decay_attn_bwd_workspace_size(a);
   if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
-  if (const int rc = decay::pass(decay::grad_q(a), a->dtype, ws, st)) return rc;
-  if (const int rc = decay::pass(decay::grad_v(a), a->dtype, ws, st)) return rc;
-  return decay::pass(decay::grad_k(a), a->dtype, ws, st);
+  decay::Batch b[2];
+  const int n = decay::backward_batches(a, b);
+  for (int i = 0; i < n; ++i) {
+    decay::plan(b[i], a->dtype, ws);
+    if (const int rc = decay::run(b[i], a->dtype, st)) return rc;
+  }
+  return HCLSM_OK;
 }
 
 extern "C" int hclsm_decay_attn_step(const hclsm_decay_args* a, const uint8_t* active, void* stream) {

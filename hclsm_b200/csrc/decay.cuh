@@ -64,25 +64,43 @@ __device__ __forceinline__ int length(const Pass& p, int64_t b) {
   return p.lens ? min(max(p.lens[b], 0), p.L) : p.L;
 }
 
+// Passes over the same sizes that run side by side in one launch: a block's pass is blockIdx.x % n.
+constexpr int kMost = 3;
+struct Batch {
+  Pass p[kMost];
+  int n;
+};
+
 // Segments of a head where the heads would leave more than half of the `room` blocks that run at once idle: whole chunks
-// of `chunk` tokens, at least four each.
-inline void cut(Pass& p, int chunk, int64_t have, int64_t room) {
-  const int chunks = (p.L + chunk - 1) / chunk;
+// of `chunk` tokens, at least `least` each.
+inline void cut(Batch& b, int chunk, int least, int64_t have, int64_t room) {
+  const int chunks = (b.p[0].L + chunk - 1) / chunk;
   int64_t segs = have > 0 ? room / have : 1;
-  if (segs > chunks / 4) segs = chunks / 4;
+  if (segs > chunks / least) segs = chunks / least;
   if (segs < 1) segs = 1;
-  p.seg_chunks = (int)((chunks + segs - 1) / segs);
-  if (p.seg_chunks < 1) p.seg_chunks = 1;
-  p.segs = (chunks + p.seg_chunks - 1) / p.seg_chunks;
-  if (p.segs < 1) p.segs = 1;
+  int each = (int)((chunks + segs - 1) / segs);
+  if (each < 1) each = 1;
+  segs = (chunks + each - 1) / each;
+  if (segs < 1) segs = 1;
+  for (int i = 0; i < b.n; ++i) b.p[i].seg_chunks = each, b.p[i].segs = (int)segs;
+}
+// Bytes of all passes' parts, and where each one's are.
+inline size_t parts(Batch& b, void* ws) {
+  size_t at = 0;
+  for (int i = 0; i < b.n; ++i) {
+    Pass& p = b.p[i];
+    p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + at);
+    if (p.segs > 1) at += ((size_t)p.B * p.H * p.segs * p.Dk * p.Dv * sizeof(float) + 15) & ~(size_t)15;
+  }
+  return at;
 }
 
-int join(const Pass& p, int chunk, cudaStream_t st);
+int join(const Batch& b, int chunk, cudaStream_t st);
 
 // bf16 on the 5th-generation tensor cores (decay_tc.cu), where tc_ok.
-bool tc_ok(const Pass& p);
-size_t tc_part_bytes(Pass p);
-int tc_pass(Pass p, cudaStream_t st);
+bool tc_ok(const Batch& b);
+void tc_cut(Batch& b);
+int tc_run(const Batch& b, cudaStream_t st);
 
 }  // namespace decay
 }  // namespace hclsm

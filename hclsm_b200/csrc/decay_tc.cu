@@ -22,6 +22,10 @@ using xattn::make_map;
 using xattn::mappable;
 using xattn::pack_bf16;
 
+struct Maps {
+  CUtensorMap x[kMost], k[kMost], v[kMost];
+};
+
 constexpr int kTok = 128;                     // tokens of a chunk
 constexpr int kBlock = kTok * (int)kRowBytes; // 64 dims of a staged tile
 
@@ -109,8 +113,9 @@ __device__ __forceinline__ void clear_row(uint32_t to, int step, int n, int row,
 
 template <int DX, int DY, int NP>
 __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>::kPerSm)
-    tc_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mk,
-              const __grid_constant__ CUtensorMap mv, const __grid_constant__ Pass p) {
+    tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Batch bt) {
+  const int which = (int)(blockIdx.x % bt.n);
+  const Pass& p = bt.p[which];
   using Sh = Shape<DX, DY, NP>;
   constexpr int WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
@@ -144,8 +149,9 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   }
   pdl_wait();
   pdl_trigger();
-  const int seg = (int)(blockIdx.x % p.segs);
-  const int64_t bh = blockIdx.x / p.segs, b = bh / p.H;
+  const uint32_t block = blockIdx.x / bt.n;
+  const int seg = (int)(block % p.segs);
+  const int64_t bh = block / p.segs, b = bh / p.H;
   const int h = (int)(bh - b * p.H), r = p.rev ? 1 : 0;
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
@@ -172,15 +178,15 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         // in the order in which the chunk before gives them up
         if (it > 0 && (!wait(s_full, it - 1) || !wait(w_ready, it - 1))) break;
         mbar_expect_tx(k_full, Sh::kX);
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &mk, d * 64, t0, h, (int)b, k_full);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &maps.k[which], d * 64, t0, h, (int)b, k_full);
         asked_k = it + 1;
         if (it > 0 && !wait(x_free, it - 1)) break;
         mbar_expect_tx(x_full, Sh::kX);
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sX + d * kBlock, &mx, d * 64, t0, h, (int)b, x_full);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sX + d * kBlock, &maps.x[which], d * 64, t0, h, (int)b, x_full);
         asked_x = it + 1;
         if (it > 0 && !wait(y_done, it - 1)) break;  // behind the state's update as well
         mbar_expect_tx(v_full, Sh::kV);
-        for (int d = 0; d < DY / 64; ++d) tma_load_4d(sV + d * kBlock, &mv, d * 64, t0, h, (int)b, v_full);
+        for (int d = 0; d < DY / 64; ++d) tma_load_4d(sV + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, v_full);
         asked_v = it + 1;
       }
     }
@@ -459,8 +465,9 @@ template <int DX, int DY> struct SumShape {
 
 template <int DX, int DY>
 __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::kPerSm)
-    sums_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-                const __grid_constant__ Pass p) {
+    sums_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Batch bt) {
+  const int which = (int)(blockIdx.x % bt.n);
+  const Pass& p = bt.p[which];
   using Sh = SumShape<DX, DY>;
   constexpr int NP = Sh::kNP, ST = Sh::kStages, WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
@@ -491,8 +498,9 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   pdl_wait();
   pdl_trigger();
   const uint32_t tmem = s_tmem;
-  const int seg = (int)(blockIdx.x % p.segs);
-  const int64_t bh = blockIdx.x / p.segs, b = bh / p.H;
+  const uint32_t block = blockIdx.x / bt.n;
+  const int seg = (int)(block % p.segs);
+  const int64_t bh = block / p.segs, b = bh / p.H;
   const int h = (int)(bh - b * p.H);
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
@@ -508,8 +516,8 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
         if (it >= ST && !wait(done, it - ST)) break;
         mbar_expect_tx(&full[s], Sh::kStage);
         unsigned char* to = sIn + s * Sh::kStage;
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(to + d * kBlock, &mk, d * 64, t0, h, (int)b, &full[s]);
-        for (int d = 0; d < DY / 64; ++d) tma_load_4d(to + Sh::kX + d * kBlock, &mv, d * 64, t0, h, (int)b, &full[s]);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(to + d * kBlock, &maps.k[which], d * 64, t0, h, (int)b, &full[s]);
+        for (int d = 0; d < DY / 64; ++d) tma_load_4d(to + Sh::kX + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, &full[s]);
         asked = it + 1;
       }
   } else if (warp == kMmaWarp) {
@@ -596,48 +604,59 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
 }
 
 // ---- host ----------------------------------------------------------------------------------
-bool tc_ok(const Pass& p) {
-  return p.Dk % 8 == 0 && p.Dv % 8 == 0 && mappable(p.x, p.L, p.H, p.B) && mappable(p.k, p.L, p.H, p.B) &&
-         mappable(p.v, p.L, p.H, p.B) && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(p.last) % 16 == 0;
+bool tc_ok(const Batch& b) {
+  for (int i = 0; i < b.n; ++i) {
+    const Pass& p = b.p[i];
+    if (!(p.Dk % 8 == 0 && p.Dv % 8 == 0 && mappable(p.x, p.L, p.H, p.B) && mappable(p.k, p.L, p.H, p.B) &&
+          mappable(p.v, p.L, p.H, p.B) && reinterpret_cast<uintptr_t>(p.y) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(p.last) % 16 == 0))
+      return false;
+  }
+  return true;
 }
 
-size_t tc_part_bytes(Pass p) {
-  cut(p, kTok, (int64_t)p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
-  return p.segs > 1 ? (size_t)p.B * p.H * p.segs * p.Dk * p.Dv * sizeof(float) : 0;
+void tc_cut(Batch& b) {
+  const Pass& p = b.p[0];
+  cut(b, kTok, 2, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
 }
 
 template <int DX, int DY, int NP>
-int launch(const Pass& p, cudaStream_t st) {
+int launch(const Batch& b, cudaStream_t st) {
   using Sh = Shape<DX, DY, NP>;
   auto fn = tc_kernel<DX, DY, NP>;
   // before the maps: encoding one needs the device's context, which this call makes current in a new thread
   if (!set_smem_limit(reinterpret_cast<const void*>(fn), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
-  CUtensorMap mx, mk, mv;
-  if (!make_map(&mx, p.x, p.Dk, p.L, p.H, p.B, kTok) || !make_map(&mk, p.k, p.Dk, p.L, p.H, p.B, kTok) ||
-      !make_map(&mv, p.v, p.Dv, p.L, p.H, p.B, kTok))
-    return HCLSM_ERR_UNSUPPORTED;
-  const int64_t grid = (int64_t)p.B * p.H * p.segs;
+  Maps maps;
+  for (int i = 0; i < b.n; ++i) {
+    const Pass& p = b.p[i];
+    if (!make_map(&maps.x[i], p.x, p.Dk, p.L, p.H, p.B, kTok) || !make_map(&maps.k[i], p.k, p.Dk, p.L, p.H, p.B, kTok) ||
+        !make_map(&maps.v[i], p.v, p.Dv, p.L, p.H, p.B, kTok))
+      return HCLSM_ERR_UNSUPPORTED;
+  }
+  const Pass& p = b.p[0];
+  const int64_t grid = (int64_t)b.n * p.B * p.H * p.segs;
   if (grid > 0x7fffffff) return HCLSM_ERR_SHAPE;
   if (p.segs > 1) {
     using Ss = SumShape<DX, DY>;
     auto sums = sums_kernel<DX, DY>;
     if (!set_smem_limit(reinterpret_cast<const void*>(sums), Ss::kBytes)) return HCLSM_ERR_LAUNCH;
-    if (const int rc = launch_pdl(sums, (unsigned)grid, Ss::kThreads, Ss::kBytes, st, mk, mv, p)) return rc;
-    if (const int rc = join(p, kTok, st)) return rc;
+    if (const int rc = launch_pdl(sums, (unsigned)grid, Ss::kThreads, Ss::kBytes, st, maps, b)) return rc;
+    if (const int rc = join(b, kTok, st)) return rc;
   }
-  return launch_pdl(fn, (unsigned)grid, Sh::kThreads, Sh::kBytes, st, mx, mk, mv, p);
+  return launch_pdl(fn, (unsigned)grid, Sh::kThreads, Sh::kBytes, st, maps, b);
 }
 
 template <int DX, int DY>
-int launch_np(const Pass& p, cudaStream_t st) {
-  return p.last && p.segs == 1 ? launch<DX, DY, 3>(p, st) : launch<DX, DY, 2>(p, st);
+int launch_np(const Batch& b, cudaStream_t st) {
+  bool out = false;  // a state that is returned
+  for (int i = 0; i < b.n; ++i) out = out || (b.p[i].last && b.p[i].segs == 1);
+  return out ? launch<DX, DY, 3>(b, st) : launch<DX, DY, 2>(b, st);
 }
 
-int tc_pass(Pass p, cudaStream_t st) {
-  cut(p, kTok, (int64_t)p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
-  if (p.Dk <= 64) return p.Dv <= 64 ? launch_np<64, 64>(p, st) : launch_np<64, 128>(p, st);
-  return p.Dv <= 64 ? launch_np<128, 64>(p, st) : launch_np<128, 128>(p, st);
+int tc_run(const Batch& b, cudaStream_t st) {
+  const Pass& p = b.p[0];
+  if (p.Dk <= 64) return p.Dv <= 64 ? launch_np<64, 64>(b, st) : launch_np<64, 128>(b, st);
+  return p.Dv <= 64 ? launch_np<128, 64>(b, st) : launch_np<128, 128>(b, st);
 }
 
 }  // namespace decay

@@ -14,6 +14,8 @@
 //   is rounded once.  movmatrix turns the scores' fragments into P^T's.  The 136 comes off the operand (summed over a
 //   history it would drown the values).
 // fp32 states: queries and weights as three bf16 pieces, whose products with exact codes are summed in fp32.
+#include <cooperative_groups.h>
+
 #include "kv4.cuh"
 
 namespace hclsm {
@@ -421,7 +423,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
       s_w[w][r] = f;
       sum += f * s_l[w][r];
     }
-    if (p.splits > 1) {
+    if (p.cluster) {
+      s_m[0][r] = top, s_l[0][r] = sum;
+    } else if (p.splits > 1) {
       p.part_ml[((bh * p.rtiles + rt) * p.splits + sp) * kRows + r] = make_float2(top, sum);
     } else {
       const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -429,16 +433,41 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
     }
   }
   __syncthreads();
+  auto row_out = [&](int row) {
+    return static_cast<T*>(p.o) + ((b * p.Lq + row / Gq) * p.H + hk * Gq + row % Gq) * (int64_t)D;
+  };
   for (int i = threadIdx.x; i < kRows * D; i += kThreads) {
     const int r = i / D, d = i % D, row = rt * kRows + r;
     if (row >= rows) break;
     float a = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) a += s_w[w][r] * part[(w * kRows + r) * D + d];
-    if (p.splits > 1)
+    if (p.cluster)
+      part[i] = a;  // over warp 0's, which this thread has read
+    else if (p.splits > 1)
       p.part_o[(((bh * p.rtiles + rt) * p.splits + sp) * kRows + r) * D + d] = a;
     else
-      io<T>::st(static_cast<T*>(p.o) + ((b * p.Lq + row / Gq) * p.H + hk * Gq + row % Gq) * (int64_t)D + d, a);
+      io<T>::st(row_out(row) + d, a);
+  }
+  if (p.cluster) {
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // the cluster's blocks share out the values; each is joined in the order of the splits
+    for (int i = sp * kThreads + threadIdx.x; i < kRows * D; i += p.splits * kThreads) {
+      const int r = i / D, row = rt * kRows + r;
+      if (row >= rows) break;
+      float top = -INFINITY, sum = 0.0f, a = 0.0f;
+      for (int k = 0; k < p.splits; ++k) top = fmaxf(top, cluster.map_shared_rank(&s_m[0][0], k)[r]);
+      for (int k = 0; k < p.splits; ++k) {
+        const float m1 = cluster.map_shared_rank(&s_m[0][0], k)[r];
+        const float f = m1 == -INFINITY ? 1.0f : ex2((m1 - top) * p.c2);
+        sum += f * cluster.map_shared_rank(&s_l[0][0], k)[r];
+        a += f * cluster.map_shared_rank(part, k)[i];
+      }
+      io<T>::st(row_out(row) + i % D, sum == 0.0f ? 0.0f : a * (1.0f / sum));
+    }
+    cluster.sync();  // no block leaves while others read its parts
   }
 }
 
@@ -491,13 +520,17 @@ void plan(Attn& p, int dtype) {
   }
   const int64_t most = (keys + 127) / 128;
   if (s > most) s = most;
+  // Up to eight splits join in their cluster's shared memory.  Up to sixteen are made eight: a second launch costs more than
+  // fewer blocks (slots, write and attention of one token over 8 x 2048, 6 heads of 64: 16.5 us with it, 12.5 without).
+  if (s <= 16) s = s < 8 ? s : 8;
   p.splits = s < 1 ? 1 : (int)s;
+  p.cluster = p.splits > 1 && p.splits <= 8;
 }
 
 size_t attn_workspace(const Attn& a, int dtype) {
   Attn p = a;
   plan(p, dtype);
-  if (p.splits <= 1) return 0;
+  if (p.splits <= 1 || p.cluster) return 0;
   return (size_t)p.B * p.c.Hkv * p.rtiles * p.splits * row_tile(p) * (p.c.D * sizeof(float) + sizeof(float2));
 }
 
@@ -506,12 +539,23 @@ int launch(Attn& p, void* ws, cudaStream_t st) {
   using Sh = Shape<T, D, RT>;
   const int64_t grid = (int64_t)p.B * p.c.Hkv * p.rtiles * p.splits, rows = (int64_t)p.B * p.H * p.Lq;
   if (grid > 0x7fffffff || rows / kWarps > 0x7ffffff0) return HCLSM_ERR_SHAPE;
-  if (p.splits > 1) {
+  if (p.splits > 1 && !p.cluster) {
     p.part_ml = static_cast<float2*>(ws);
     p.part_o = reinterpret_cast<float*>(p.part_ml + grid * Sh::kRows);
   }
   auto f = attn_kernel<T, D, RT>;
   if (!set_smem_limit(reinterpret_cast<const void*>(f), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
+  if (p.cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = (unsigned)grid, cfg.blockDim = kThreads, cfg.dynamicSmemBytes = Sh::kBytes, cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, f, p) == cudaSuccess ? HCLSM_OK : HCLSM_ERR_LAUNCH;
+  }
   if (const int rc = launch_pdl(f, (unsigned)grid, kThreads, Sh::kBytes, st, p)) return rc;
   if (p.splits <= 1) return HCLSM_OK;
   return launch_pdl(join_kernel<T, D, Sh::kRows>, (unsigned)((rows + kWarps - 1) / kWarps), kThreads, 0, st, p);
