@@ -191,6 +191,11 @@ def dense_last(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def empty_like(t):
+    """A dense tensor of t's shape (for a dense t the cheaper of the two calls, by a microsecond)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def rows16(t):
     """The (B, L, H, D) tensor itself if its last dim is dense and every row starts on 16
     bytes, else an aligned contiguous copy.  The stride of a dim of one says nothing (the

@@ -253,27 +253,33 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Batch
   const int64_t block = blockIdx.x / bt.n, bh = block / per, i = block % per * 128 + threadIdx.x;
   const int64_t b = bh / p.H;
   const int h = (int)(bh - b * p.H), n = length(p, b), span = p.seg_chunks * chunk;
-  // of a whole segment and of the incomplete one
-  if (threadIdx.x < 2) s_g[threadIdx.x] = chunk_decay(p.log_decay, h, threadIdx.x ? n % span : span);
-  __syncthreads();
-  if (i >= sz) return;
-  float v = 0.0f;
-  if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? i % p.Dv * p.Dk + i / p.Dv : i)];
-  float* at = p.part + bh * p.segs * sz + i;
-  const float2 whole = s_g[0], cut_off = s_g[1];
-  for (int it = 0; it < p.segs; it += 8) {
-    float sum[8];
+  const bool in = i < sz;
+  const int segs = p.segs, step = p.rev ? -1 : 1, first = p.rev ? segs - 1 : 0;
+  float* at = p.part + (bh * segs + first) * sz + i;
+  const int64_t by = step * sz;
+  float sum[8];
+  auto ask = [&](int it) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (it + k < p.segs) sum[k] = at[(p.rev ? p.segs - 1 - it - k : it + k) * sz];
+      if (in && it + k < segs) sum[k] = at[(it + k) * by];
+  };
+  ask(0);  // on their way while the decays, of a whole segment and of the incomplete one, are formed
+  if (threadIdx.x < 2) s_g[threadIdx.x] = chunk_decay(p.log_decay, h, threadIdx.x ? n % span : span);
+  __syncthreads();
+  if (!in) return;
+  float v = 0.0f;
+  if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? i % p.Dv * p.Dk + i / p.Dv : i)];
+  const float2 whole = s_g[0], cut_off = s_g[1];
+  for (int it = 0; it < segs; it += 8) {
+    if (it > 0) ask(it);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (it + k >= p.segs) break;
-      const int s = p.rev ? p.segs - 1 - it - k : it + k, m = n - s * span;  // m: tokens from here on
-      at[s * sz] = v;
-      if (m <= 0) continue;  // behind the length
-      const float2 g = m >= span ? whole : cut_off;
-      v = fmaf(v, g.x, fmaf(v, g.y, sum[k]));
+      const int m = n - (first + step * (it + k)) * span;  // tokens from this segment on
+      if (it + k < segs) at[(it + k) * by] = v;
+      if (it + k < segs && m > 0) {  // not behind the length
+        const float2 g = m >= span ? whole : cut_off;
+        v = fmaf(v, g.x, fmaf(v, g.y, sum[k]));
+      }
     }
   }
   if (p.last) p.last[bh * sz + i] = p.last_f * v;

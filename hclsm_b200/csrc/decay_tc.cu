@@ -31,11 +31,11 @@ constexpr int kBlock = kTok * (int)kRowBytes; // 64 dims of a staged tile
 
 template <int DX, int DY, int NP> struct Shape {
   static constexpr bool kSmall = DX == 64 && DY == 64;
-  static constexpr int kWg = kSmall ? 1 : 2;  // warpgroups of each kind: columns are shared out among them
+  static constexpr int kWgT = 2, kWg = kSmall ? 1 : 2;  // warpgroups of the state, of the rows: they share out the columns
   static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
   static constexpr int kT = DY / 64 * DX * (int)kRowBytes;  // bf16 copy of the state
   static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + 1024;
-  static constexpr int kThreads = 2 * kWg * 128 + 64;
+  static constexpr int kThreads = (kWgT + kWg) * 128 + 64;
   static constexpr uint32_t kColY = 128, kColXt = kSmall ? 64 : 256, kColT = kSmall ? 192 : 384;
   static constexpr uint32_t kCols = kSmall ? 256 : 512;
   static constexpr int kPerSm = kSmall ? 2 : 1;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   const int which = (int)(blockIdx.x % bt.n);
   const Pass& p = bt.p[which];
   using Sh = Shape<DX, DY, NP>;
-  constexpr int WG = Sh::kWg;
+  constexpr int WGT = Sh::kWgT, WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
            *t_ready = bars + 5, *y_done = bars + 6, *y_free = bars + 7, *x_free = bars + 8, *t_done = bars + 9,
            *w_ready = bars + 10, *drain = bars + 11;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
-  constexpr int kTmaWarp = WG * 8, kMmaWarp = WG * 8 + 1;
+  constexpr int kTmaWarp = (WGT + WG) * 4, kMmaWarp = kTmaWarp + 1;
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(Sh::kCols)
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   if (tid == 0) {
     s_abort = 0;
     for (uint64_t* b = bars; b < bars + kBars; ++b)
-      mbar_init(b, b == p_ready || b == t_ready || b == w_ready || b == y_free ? WG * 128 : 1);
+      mbar_init(b, b == t_ready || b == w_ready ? WGT * 128 : b == p_ready || b == y_free ? WG * 128 : 1);
     fence_mbar_init();
   }
   pdl_wait();
@@ -243,10 +243,10 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
                 k != 0);
       umma_done(one, y_done);
     }
-  } else if (warp < WG * 4) {
+  } else if (warp < WGT * 4) {
     // ---- the state --------------------------------------------------------------------------
     const int row = tid & 127, half = tid >> 7;  // token, or row of T; columns of this warpgroup
-    constexpr int kCols = DY / WG, kDims = DX / WG;
+    constexpr int kCols = DY / WGT, kDims = DX / WGT;
     const int y0 = half * kCols;
     const bool holds = (warp & 3) * 32 < DX;  // this warp's lanes are rows of T
     const uint32_t tT = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::kColT + y0;
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
     }
   } else {
     // ---- the rows ---------------------------------------------------------------------------
-    const int row = tid & 127, half = (tid >> 7) - WG;  // token; columns of this warpgroup
+    const int row = tid & 127, half = (tid >> 7) - WGT;  // token; columns of this warpgroup
     const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16), tY = tS + Sh::kColY, tX = tS + Sh::kColXt;
     constexpr int kCols = DY / WG, kBlocks = 4 / WG;
     const int y0 = half * kCols, i0 = (warp & 3) * 32;
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       }
     }
     // zeros behind the length
-    const int e8 = p.Dv / 8, me = tid - WG * 128;
+    const int e8 = p.Dv / 8, me = tid - WGT * 128;
     for (int t = max(c_lo * kTok, n) + (me >> 3); t < min(c_end * kTok, p.L); t += WG * 16)
       for (int e = me & 7; e < e8; e += 8)
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t) * p.H + h) * (int64_t)p.Dv + e * 8) =
@@ -451,16 +451,17 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
 }
 
 // ---- the segments' own sums --------------------------------------------------------------------
-// No x and no y: T = sum over the segment of (w_j k_j)^T v_j, w_j to the segment's end, so T is never scaled.  Stages of
-// k and v; one chunk's sum is added to the registers while the next one's products run.
+// No x and no y: T = sum over the segment of (w_j k_j)^T v_j, w_j to the segment's end, so T is never scaled.  k is free
+// when its pieces are written, v has two stages; one chunk's sum is added to the registers while the next one's
+// products run.
 template <int DX, int DY> struct SumShape {
   static constexpr int kNP = 3, kStages = 2;
-  static constexpr int kWg = DX == 64 && DY == 64 ? 1 : 2;
-  static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock, kStage = kX + kV;
-  static constexpr size_t kBytes = kStages * (size_t)kStage + (size_t)kNP * kX + 1024;
+  static constexpr int kWg = 2;
+  static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
+  static constexpr size_t kBytes = kX + kStages * (size_t)kV + (size_t)kNP * kX + 1024;
   static constexpr int kThreads = kWg * 128 + 64;
   static constexpr uint32_t kCols = 2 * DY;
-  static constexpr int kPerSm = kBytes <= 112 * 1024 ? 2 : 1;
+  static constexpr int kPerSm = DX == 64 && DY == 64 ? 2 : 1;
 };
 
 template <int DX, int DY>
@@ -473,12 +474,12 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned char *sP = smem, *sIn = sP + NP * Sh::kX;  // the pieces first, as above
+  unsigned char *sP = smem, *sK = sP + NP * Sh::kX, *sV = sK + Sh::kX;  // the pieces first, as above
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  constexpr int kBars = ST + 3;
+  constexpr int kBars = ST + 4;
   __shared__ uint64_t bars[kBars];
-  uint64_t *full = bars, *ready = bars + ST, *done = ready + 1, *drain = done + 1;
+  uint64_t *full = bars, *k_full = bars + ST, *ready = k_full + 1, *done = ready + 1, *drain = done + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = WG * 4, kMmaWarp = WG * 4 + 1;
   if (warp == kMmaWarp) {
@@ -508,32 +509,35 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   const int chunks = hi > lo ? (hi - lo + kTok - 1) / kTok : 0;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, p.err); };
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-  int asked = 0;
+  int asked = 0, asked_k = 0;
   if (warp == kTmaWarp) {
     if (lane == 0)
       for (int it = 0; it < chunks; ++it) {
         const int s = it % ST, t0 = lo + it * kTok;
+        if (it > 0 && !wait(ready, it - 1)) break;
+        mbar_expect_tx(k_full, Sh::kX);
+        for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &maps.k[which], d * 64, t0, h, (int)b, k_full);
+        asked_k = it + 1;
         if (it >= ST && !wait(done, it - ST)) break;
-        mbar_expect_tx(&full[s], Sh::kStage);
-        unsigned char* to = sIn + s * Sh::kStage;
-        for (int d = 0; d < DX / 64; ++d) tma_load_4d(to + d * kBlock, &maps.k[which], d * 64, t0, h, (int)b, &full[s]);
-        for (int d = 0; d < DY / 64; ++d) tma_load_4d(to + Sh::kX + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, &full[s]);
+        mbar_expect_tx(&full[s], Sh::kV);
+        for (int d = 0; d < DY / 64; ++d)
+          tma_load_4d(sV + s * Sh::kV + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, &full[s]);
         asked = it + 1;
       }
   } else if (warp == kMmaWarp) {
     const uint32_t one = elect_one();
     const uint32_t id_t = idesc_bf16(128, (p.Dv + 15) / 16 * 16, true, true);
-    const uint64_t d_v = smem_desc_sw128(smem_u32(sIn + Sh::kX), kBlock, 1024),
+    const uint64_t d_v = smem_desc_sw128(smem_u32(sV), kBlock, 1024),
                    d_p = smem_desc_sw128(smem_u32(sP), kBlock, 1024);
     for (int it = 0; it < chunks; ++it) {
-      if (!wait_all(ready, it)) break;
+      if (!wait_all(ready, it) || !wait_all(&full[it % ST], it / ST)) break;
       tc_fence_after();
 #pragma unroll
       for (int i = NP - 1; i >= 0; --i)
 #pragma unroll
         for (int k = 0; k < kTok / 16; ++k)
           umma_ss(one, tmem + (it & 1) * DY, desc_at(d_p, i * Sh::kX + k * 16 * kRowBytes),
-                  desc_at(d_v, it % ST * Sh::kStage + k * 16 * kRowBytes), id_t, !(i == NP - 1 && k == 0));
+                  desc_at(d_v, it % ST * Sh::kV + k * 16 * kRowBytes), id_t, !(i == NP - 1 && k == 0));
       umma_done(one, done);
     }
   } else {
@@ -560,17 +564,19 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
     bool ok = true;
     for (int it = 0; it < chunks && ok; ++it) {
       const int s = it % ST, t = lo + it * kTok + row;
-      if (!(ok = wait_all(&full[s], it / ST))) break;
+      if (!(ok = wait_all(k_full, it))) break;
       // the products that read the pieces are complete
       if (it > 0 && !(ok = wait_all(done, it - 1))) break;
-      unsigned char *sK = sIn + s * Sh::kStage, *sV = sK + Sh::kX;
       const int c0 = half * (kDims / 8);
       const float w = ex2(l2 * (float)(p.rev ? t - lo + 1 : hi - 1 - t));
 #pragma unroll 1
       for (int c = 0; c < kDims / 8; c += 4) weigh_row<NP, 4>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
-      if (t >= hi) {
-        clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
-        clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
+      if (lo + (it + 1) * kTok > hi) {
+        if (!(ok = wait_all(&full[s], it / ST))) break;
+        if (t >= hi) {
+          clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
+          clear_row(smem_u32(sV + s * Sh::kV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
+        }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc_fence_before();
@@ -596,7 +602,10 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   tc_fence_after();
   if (s_abort) {
     if (warp == kMmaWarp) drain_umma(drain);
-    if (warp == kTmaWarp && lane == 0) drain_copies(full, asked, ST);
+    if (warp == kTmaWarp && lane == 0) {
+      drain_copies(k_full, asked_k, 1);
+      drain_copies(full, asked, ST);
+    }
     __syncthreads();
   }
   if (warp == kMmaWarp)

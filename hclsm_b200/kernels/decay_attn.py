@@ -35,7 +35,7 @@ def _workspace(q, n):
 
 def _forward(q, k, v, decay, s0, lens, scale, want_state):
     B, L, H, D = q.shape
-    o = q.new_empty(v.shape)
+    o = _lib.empty_like(v)
     s1 = q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32) if want_state else None
     a = _args(q, k, v, decay, s0, lens, scale, o, s1)
     lib = _lib.load()
@@ -47,7 +47,7 @@ def _forward(q, k, v, decay, s0, lens, scale, want_state):
 
 def _backward(q, k, v, decay, s0, lens, scale, do, ds1, want_ds0):
     do = _lib.dense_last(do)
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = _lib.empty_like(q), _lib.empty_like(k), _lib.empty_like(v)
     ds0 = torch.empty_like(s0) if want_ds0 else None
     if ds1 is not None:
         ds1 = ds1.contiguous()
@@ -165,15 +165,21 @@ def decay_attention_step(q, k, v, log_decay, state, *, out=None, active=None, sc
         raise NotImplementedError("decay_attention_step has no gradients: call it under torch.no_grad()")
     if _lib.in_dual_level():
         _lib.no_tangents(q, k, v, log_decay, state)
-    dev = _lib.require_cuda(q, k, v, log_decay, state, out, active)
-    if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[:2] != q.shape[:2]:
+    dev, index = _lib.require_cuda(q), q.get_device()
+    if (k.get_device() != index or v.get_device() != index or log_decay.get_device() != index
+            or state.get_device() != index or (out is not None and out.get_device() != index)
+            or (active is not None and active.get_device() != index)):
+        raise ValueError(f"all tensors must be on {dev}")
+    shape_q, shape_v = q.shape, v.shape
+    if len(shape_q) != 3 or k.shape != shape_q or len(shape_v) != 3 or shape_v[:2] != shape_q[:2]:
         raise ValueError(f"q and k must be (B, H, D), v (B, H, Dv), got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
-    B, H, D = q.shape
-    Dv = v.shape[2]
+    B, H, D = shape_q
+    Dv = shape_v[2]
     if H < 1 or not 1 <= D <= 128 or not 1 <= Dv <= 128:
         raise ValueError(f"head dims must be 1 to 128, got {D} and {Dv} of {H} heads")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype:
         raise TypeError(f"q, k and v must share one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
     log_decay = _check_decay(log_decay, H)
     shape = (B, H, D, Dv)
@@ -192,10 +198,13 @@ def decay_attention_step(q, k, v, log_decay, state, *, out=None, active=None, sc
             raise ValueError(f"active must be ({B},) bool")
         active = active.contiguous()
     q, k, v = _lib.dense_last(q), _lib.dense_last(k), _lib.dense_last(v)
-    o = q.new_empty(v.shape)
+    o = _lib.empty_like(v)
+    qb, qh, _ = q.stride()
+    kb, kh, _ = k.stride()
+    vb, vh, _ = v.stride()
     a = _lib.DECAY_ARGS.pack(
-        q.data_ptr(), q.stride(0), 0, q.stride(1), k.data_ptr(), k.stride(0), 0, k.stride(1), v.data_ptr(),
-        v.stride(0), 0, v.stride(1), 0, 0, 0, 0, o.data_ptr(), 0, 0, 0, log_decay.data_ptr(), state.data_ptr(),
-        out.data_ptr(), 0, 0, 0, B, 1, H, D, Dv, _lib.dtype_code(q.dtype), _check_scale(scale, D))
+        q.data_ptr(), qb, 0, qh, k.data_ptr(), kb, 0, kh, v.data_ptr(), vb, 0, vh, 0, 0, 0, 0, o.data_ptr(), 0, 0, 0,
+        log_decay.data_ptr(), state.data_ptr(), out.data_ptr(), 0, 0, 0, B, 1, H, D, Dv, _lib.dtype_code(dtype),
+        _check_scale(scale, D))
     _lib.check(_lib.load().hclsm_decay_attn_step(a, _lib.ptr(active), _lib.stream_ptr(dev)), "hclsm_decay_attn_step")
     return o

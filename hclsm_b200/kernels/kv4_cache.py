@@ -163,7 +163,7 @@ def kv4_attention(q: Tensor, cache: Kv4Cache, table: Tensor, lens: Tensor | None
         raise ValueError(f"scale must be positive and finite, got {scale}")
     lens = _lib.index32(lens, (B,), "lens", dev)
     q = _lib.rows16(q)
-    o = q.new_empty(q.shape)
+    o = _lib.empty_like(q)
     lib, ws = _lib.load(), None
     n = lib.hclsm_kv4_attn_workspace_size(c, B, M, Lq, H)
     if n:
