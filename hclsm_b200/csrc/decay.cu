@@ -314,7 +314,7 @@ int simt_run(const Batch& b, cudaStream_t st) {
 
 void simt_cut(Batch& b) {
   const Pass& p = b.p[0];
-  cut(b, kC, 1, (int64_t)b.n * p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
+  cut(b, kC, 1.0f, 1.1f, (int64_t)b.n * p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
 }
 
 // ---- one token -------------------------------------------------------------------------------
@@ -361,19 +361,33 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
   __syncthreads();
   float acc[V] = {};
   if (g0 < groups) {
-#pragma unroll 8
-    for (int d = g0; d < p.Dk; d += groups) {
-      if constexpr (V == 4) {
-        float4 s = *reinterpret_cast<const float4*>(s0 + d * p.Dv + e);
-        s.x = fmaf(g, s.x, sk[d] * sv[e]), s.y = fmaf(g, s.y, sk[d] * sv[e + 1]);
-        s.z = fmaf(g, s.z, sk[d] * sv[e + 2]), s.w = fmaf(g, s.w, sk[d] * sv[e + 3]);
-        *reinterpret_cast<float4*>(s1 + d * p.Dv + e) = s;
-        acc[0] = fmaf(sq[d], s.x, acc[0]), acc[1] = fmaf(sq[d], s.y, acc[1]);
-        acc[2] = fmaf(sq[d], s.z, acc[2]), acc[3] = fmaf(sq[d], s.w, acc[3]);
-      } else {
-        const float s = fmaf(g, s0[d * p.Dv + e], sk[d] * sv[e]);
-        s1[d * p.Dv + e] = s;
-        acc[0] = fmaf(sq[d], s, acc[0]);
+    // eight rows asked for before the first is written: s1 may be s0, which keeps a load behind a store
+    for (int d0 = g0; d0 < p.Dk; d0 += 8 * groups) {
+      float s[8][V];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i * groups;
+        if (d >= p.Dk) continue;
+        if constexpr (V == 4) {
+          const float4 t = __ldcs(reinterpret_cast<const float4*>(s0 + d * p.Dv + e));
+          s[i][0] = t.x, s[i][1] = t.y, s[i][2] = t.z, s[i][3] = t.w;
+        } else {
+          s[i][0] = s0[d * p.Dv + e];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i * groups;
+        if (d >= p.Dk) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          s[i][k] = fmaf(g, s[i][k], sk[d] * sv[e + k]);
+          acc[k] = fmaf(sq[d], s[i][k], acc[k]);
+        }
+        if constexpr (V == 4)
+          __stcs(reinterpret_cast<float4*>(s1 + d * p.Dv + e), make_float4(s[i][0], s[i][1], s[i][2], s[i][3]));
+        else
+          s1[d * p.Dv + e] = s[i][0];
       }
     }
 #pragma unroll

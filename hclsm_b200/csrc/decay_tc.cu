@@ -291,34 +291,43 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       if (it > 0 && !(ok = wait_all(t_done, it - 1))) break;
       advance(m);
       m = min(n - first_token(it), kTok);
-      if (it > 0 && !(ok = wait_all(x_free, it - 1))) break;  // the bf16 copy has been read
-      if (holds) {
-        const RowAt<DX> at(smem_u32(sT), row);
+      auto copy_state = [&] {  // T in bf16, for x T
+        if (it > 0 && !wait_all(x_free, it - 1)) return false;  // the copy before has been read
+        if (holds) {
+          const RowAt<DX> at(smem_u32(sT), row);
 #pragma unroll
-        for (int c = 0; c < kCols; c += 8) {
-          uint32_t q[4];
+          for (int c = 0; c < kCols; c += 8) {
+            uint32_t q[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q[e] = pack_bf16(T[c / 2 + e].x, T[c / 2 + e].y);
-          st_shared(at(y0 / 8 + c / 8), q[0], q[1], q[2], q[3]);
+            for (int e = 0; e < 4; ++e) q[e] = pack_bf16(T[c / 2 + e].x, T[c / 2 + e].y);
+            st_shared(at(y0 / 8 + c / 8), q[0], q[1], q[2], q[3]);
+          }
         }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc_fence_before();
-      mbar_arrive(t_ready);
-      if (!(ok = wait_all(k_full, it))) break;
-      const int c0 = half * (kDims / 8);
-      const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        mbar_arrive(t_ready);
+        return true;
+      };
+      auto weigh = [&] {  // the pieces of w k
+        if (!wait_all(k_full, it)) return false;
+        const int c0 = half * (kDims / 8);
+        const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
 #pragma unroll 1
-      for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
-      if (m < kTok) {
-        if (!(ok = wait_all(v_full, it))) break;
-        if (row >= m) {
-          clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
-          clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
+        for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
+        if (m < kTok) {
+          if (!wait_all(v_full, it)) return false;
+          if (row >= m) {
+            clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
+            clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
+          }
         }
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(w_ready);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();  // the products' sum has been read
+        mbar_arrive(w_ready);
+        return true;
+      };
+      // x T comes before the update's products, or behind them where it has to wait for P's columns
+      ok = Sh::kSmall ? weigh() && copy_state() : copy_state() && weigh();
     }
     if (ok && chunks > 0) {
       ok = wait_all(t_done, chunks - 1);
@@ -355,8 +364,12 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         if ((past || now) && j0 < m) {
           float v[32];
           tmem_ld32_nowait(tS + j0, v);
-          if (past && j0 + 32 <= m) {
-            // g^|i-j| as the power of i's distance to the block's near end times that of j's
+          // the columns [first, last] count
+          const int first = p.rev ? max(row - j0, 0) : 0, last = min(p.rev ? 31 : min(row - j0, 31), m - 1 - j0);
+          const uint32_t on = first <= last && first < 32 ? (0xffffffffu >> (31 - (last - first))) << first : 0u;
+          if (past || l2 > -4.0f) {
+            // g^|i-j| as the power of i's distance to the block's end on the later side times that of j's; on the
+            // diagonal the first is up to g^-31, which fp32 holds above 2^-4
             const float a = ex2(l2 * (float)(p.rev ? j0 - row : row - j0 - 31));
             tmem_wait_ld();
             tmem_pin<32>(v);
@@ -367,23 +380,21 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
                      hi = mul2(make_float2(v[4 * e + 2], v[4 * e + 3]), make_float2(a, a));
               lo = mul2(lo, make_float2(t.x, t.y));
               hi = mul2(hi, make_float2(t.z, t.w));
-              pw[2 * e] = pack_bf16(lo.x, lo.y), pw[2 * e + 1] = pack_bf16(hi.x, hi.y);
+              v[4 * e] = lo.x, v[4 * e + 1] = lo.y, v[4 * e + 2] = hi.x, v[4 * e + 3] = hi.y;
             }
           } else {
-            // the columns [first, last] count; select, not multiply: a later token's score may be NaN
-            const int first = p.rev ? max(row - j0, 0) : 0, last = min(p.rev ? 31 : min(row - j0, 31), m - 1 - j0);
-            const uint32_t on = first <= last && first < 32 ? (0xffffffffu >> (31 - (last - first))) << first : 0u;
             const float step = p.rev ? l2 : -l2, base = (p.rev ? -l2 : l2) * (float)(row - j0);
             tmem_wait_ld();
             tmem_pin<32>(v);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float w = ex2(fmaf(step, (float)e, base));
-              v[e] = on >> e & 1u ? v[e] * w : 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pw[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+            for (int e = 0; e < 32; ++e) v[e] *= ex2(fmaf(step, (float)e, base));
           }
+          if (!past || j0 + 32 > m) {  // select, not multiply: a later token's score may be NaN, its power inf
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = on >> e & 1u ? v[e] : 0.0f;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pw[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
         } else {
 #pragma unroll
           for (int e = 0; e < 16; ++e) pw[e] = 0;
@@ -626,7 +637,7 @@ bool tc_ok(const Batch& b) {
 
 void tc_cut(Batch& b) {
   const Pass& p = b.p[0];
-  cut(b, kTok, 2, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
+  cut(b, kTok, 5.0f, 1.5f, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
 }
 
 template <int DX, int DY, int NP>
