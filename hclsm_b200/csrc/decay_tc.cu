@@ -23,7 +23,7 @@ using xattn::mappable;
 using xattn::pack_bf16;
 
 struct Maps {
-  CUtensorMap x[kMost], k[kMost], v[kMost];
+  CUtensorMap x[kMost], k[kMost], v[kMost], y[kMost];
 };
 
 constexpr int kTok = 128;                     // tokens of a chunk
@@ -34,7 +34,11 @@ template <int DX, int DY, int NP> struct Shape {
   static constexpr int kWgT = 2, kWg = kSmall ? 1 : 2;  // warpgroups of the state, of the rows: they share out the columns
   static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
   static constexpr int kT = DY / 64 * DX * (int)kRowBytes;  // bf16 copy of the state
-  static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + 1024;
+  // y goes out by way of shared memory where that has room for it: a thread's own row is a line for each store, and those
+  // took a quarter of the L1's cycles
+  static constexpr bool kStaged = NP == 2 && DY / kWg == 64;
+  static constexpr int kY = kStaged ? kV : 0;
+  static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + kY + 1024;
   static constexpr int kThreads = (kWgT + kWg) * 128 + 64;
   static constexpr uint32_t kColY = 128, kColXt = kSmall ? 64 : 256, kColT = kSmall ? 192 : 384;
   static constexpr uint32_t kCols = kSmall ? 256 : 512;
@@ -123,7 +127,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // with 64 dims the update's products read 64 rows behind a piece of k, for rows of the result that nobody reads: the
   // pieces come first
-  unsigned char *sP = smem, *sX = sP + NP * Sh::kX, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sT = sV + Sh::kV;
+  unsigned char *sP = smem, *sX = sP + NP * Sh::kX, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sY = sV + Sh::kV,
+                *sT = sY + Sh::kY;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ __align__(16) float s_pow[32];  // g^(distance of a block's j to its end on the later side)
@@ -409,6 +414,10 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t0 + row) * p.H + h) * (int64_t)p.Dv + y0;
       if (!(ok = wait_all(y_done, it))) break;
       tc_fence_after();
+      if (Sh::kStaged && it > 0) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the rows before have left
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int c = 0; c < kCols; c += 16) {
         float a[16], x[16];
@@ -428,7 +437,12 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
           t = fma2(make_float2(x[2 * e], x[2 * e + 1]), make_float2(lead, lead), t);
           q[e] = pack_bf16(t.x, t.y);
         }
-        if (row < m && y0 + c < p.Dv) {
+        if constexpr (Sh::kStaged) {
+          const RowAt<kTok> at(smem_u32(sY), row);
+          const uint32_t keep = row < m ? 0xffffffffu : 0u;  // zeros behind the length
+          st_shared(at((y0 + c) / 8), q[0] & keep, q[1] & keep, q[2] & keep, q[3] & keep);
+          st_shared(at((y0 + c) / 8 + 1), q[4] & keep, q[5] & keep, q[6] & keep, q[7] & keep);
+        } else if (row < m && y0 + c < p.Dv) {
           if (wide) {
             store32(out + c, q);
           } else {
@@ -437,7 +451,19 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
           }
         }
       }
+      if constexpr (Sh::kStaged) {  // a warp's 32 rows of 64 dims
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0 && t0 + i0 < p.L) {
+          asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                           &maps.y[which]),
+                       "r"(y0), "r"(t0 + i0), "r"(h), "r"((int)b), "r"(smem_u32(sY + y0 / 64 * kBlock + i0 * (int)kRowBytes))
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      }
     }
+    if (Sh::kStaged && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     // zeros behind the length
     const int e8 = p.Dv / 8, me = tid - WGT * 128;
     for (int t = max(c_lo * kTok, n) + (me >> 3); t < min(c_end * kTok, p.L); t += WG * 16)
@@ -652,6 +678,8 @@ int launch(const Batch& b, cudaStream_t st) {
     if (!make_map(&maps.x[i], p.x, p.Dk, p.L, p.H, p.B, kTok) || !make_map(&maps.k[i], p.k, p.Dk, p.L, p.H, p.B, kTok) ||
         !make_map(&maps.v[i], p.v, p.Dv, p.L, p.H, p.B, kTok))
       return HCLSM_ERR_UNSUPPORTED;
+    const View y = xattn::view(hclsm_view{p.y, (int64_t)p.L * p.H * p.Dv, (int64_t)p.H * p.Dv, p.Dv}, p.B, p.L, p.H);
+    if (Sh::kStaged && !make_map(&maps.y[i], y, p.Dv, p.L, p.H, p.B, 32)) return HCLSM_ERR_UNSUPPORTED;
   }
   const Pass& p = b.p[0];
   const int64_t grid = (int64_t)b.n * p.B * p.H * p.segs;
