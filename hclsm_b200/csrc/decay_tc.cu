@@ -34,10 +34,12 @@ template <int DX, int DY, int NP> struct Shape {
   static constexpr int kWgT = 2, kWg = kSmall ? 1 : 2;  // warpgroups of the state, of the rows: they share out the columns
   static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
   static constexpr int kT = DY / 64 * DX * (int)kRowBytes;  // bf16 copy of the state
-  // y goes out by way of shared memory where that has room for it: a thread's own row is a line for each store, and those
-  // took a quarter of the L1's cycles
-  static constexpr bool kStaged = NP == 2 && DY / kWg == 64;
-  static constexpr int kY = kStaged ? kV : 0;
+  // y goes out by way of shared memory: a thread's own row is a line for each store, and those took a quarter of the L1's
+  // cycles.  With three pieces there is no room beside v: with 128 dims y goes over it and the next v waits until y has left
+  // (4 chunks of one head 22.6 -> 20.0 us); with 64, where the wait cost more (128 heads of 2048 tokens 50.7 -> 56.9 us), y
+  // is stored by rows.
+  static constexpr bool kStaged = DY / kWg == 64 && (NP == 2 || !kSmall), kOverV = NP == 3 && DX == 128 && DY == 128;
+  static constexpr int kY = kStaged && !kOverV ? kV : 0;
   static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + kY + 1024;
   static constexpr int kThreads = (kWgT + kWg) * 128 + 64;
   static constexpr uint32_t kColY = 128, kColXt = kSmall ? 64 : 256, kColT = kSmall ? 192 : 384;
@@ -127,17 +129,17 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // with 64 dims the update's products read 64 rows behind a piece of k, for rows of the result that nobody reads: the
   // pieces come first
-  unsigned char *sP = smem, *sX = sP + NP * Sh::kX, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sY = sV + Sh::kV,
-                *sT = sY + Sh::kY;
+  unsigned char *sP = smem, *sX = sP + NP * Sh::kX, *sK = sX + Sh::kX, *sV = sK + Sh::kX, *sY = sV + (Sh::kOverV ? 0 : Sh::kV),
+                *sT = sV + Sh::kV + Sh::kY;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ __align__(16) float s_pow[32];  // g^(distance of a block's j to its end on the later side)
   __shared__ float2 s_g[2];  // decays of a whole chunk and of the incomplete one
-  constexpr int kBars = 12;
+  constexpr int kBars = 13;
   __shared__ uint64_t bars[kBars];
   uint64_t *x_full = bars, *k_full = bars + 1, *v_full = bars + 2, *s_full = bars + 3, *p_ready = bars + 4,
            *t_ready = bars + 5, *y_done = bars + 6, *y_free = bars + 7, *x_free = bars + 8, *t_done = bars + 9,
-           *w_ready = bars + 10, *drain = bars + 11;
+           *w_ready = bars + 10, *y_left = bars + 11, *drain = bars + 12;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = (WGT + WG) * 4, kMmaWarp = kTmaWarp + 1;
   if (warp == kMmaWarp) {
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
   if (tid == 0) {
     s_abort = 0;
     for (uint64_t* b = bars; b < bars + kBars; ++b)
-      mbar_init(b, b == t_ready || b == w_ready ? WGT * 128 : b == p_ready || b == y_free ? WG * 128 : 1);
+      mbar_init(b, b == t_ready || b == w_ready ? WGT * 128 : b == p_ready || b == y_free ? WG * 128 : b == y_left ? WG * 4 : 1);
     fence_mbar_init();
   }
   pdl_wait();
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         mbar_expect_tx(x_full, Sh::kX);
         for (int d = 0; d < DX / 64; ++d) tma_load_4d(sX + d * kBlock, &maps.x[which], d * 64, t0, h, (int)b, x_full);
         asked_x = it + 1;
-        if (it > 0 && !wait(y_done, it - 1)) break;  // behind the state's update as well
+        if (it > 0 && !wait(Sh::kOverV ? y_left : y_done, it - 1)) break;  // behind the state's update as well
         mbar_expect_tx(v_full, Sh::kV);
         for (int d = 0; d < DY / 64; ++d) tma_load_4d(sV + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, v_full);
         asked_v = it + 1;
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t0 + row) * p.H + h) * (int64_t)p.Dv + y0;
       if (!(ok = wait_all(y_done, it))) break;
       tc_fence_after();
-      if (Sh::kStaged && it > 0) {
+      if (Sh::kStaged && !Sh::kOverV && it > 0) {
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the rows before have left
         __syncwarp();
       }
@@ -460,6 +462,10 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
                        "r"(y0), "r"(t0 + i0), "r"(h), "r"((int)b), "r"(smem_u32(sY + y0 / 64 * kBlock + i0 * (int)kRowBytes))
                        : "memory");
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+        if (Sh::kOverV && lane == 0) {
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          mbar_arrive(y_left);
         }
       }
     }
