@@ -25,7 +25,12 @@ CUDA tensors only (no CPU kernel is registered).  Every op has a fake
   ``cross_attention_bwd`` (both forwards with registered autograd formulas; of the
   cross attention's outputs o alone has gradients), and
   ``kv8_write`` / ``kv8_attention`` on the tensors of a ``Kv8Cache``
-  (``kv8_write`` mutates them, and wants detached keys and values).
+  (``kv8_write`` mutates them, and wants detached keys and values);
+* ``decay_attention_fwd`` / ``decay_attention_bwd`` (the forward with a registered autograd
+  formula, of its output and of the final state; none in log_decay) and ``decay_attention_step``
+  (mutates the state), ``kv4_write`` / ``kv4_read`` / ``kv4_attention`` on the tensors of a ``Kv4Cache``
+  (``kv4_write`` mutates them), ``pages_resize`` (mutates a ``PageTable``'s tensors) and ``page_slots``;
+  what mutates wants detached tensors.
 
 Scan inputs must already share one dtype (fp32 or bf16: x, dt, B, C, z) with
 A_log and D in fp32, and be contiguous; ``hclsm_b200.kernels.ssm_scan`` does
@@ -39,7 +44,10 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .kernels import decay_attn as _decay
+from .kernels import kv4_cache as _kv4
 from .kernels import kv8_cache as _kv8
+from .kernels import pages as _pages
 from .kernels import sparse_event_attn as _ev
 from .kernels import ssm_scan_kernel as _scan
 from .kernels.cross_attn import attention_bwd as _xattn_bwd
@@ -50,7 +58,8 @@ from .kernels.slot_attention_kernel import slot_attention_core as _slot_core
 
 __all__ = ["ssm_scan_fwd", "ssm_scan_bwd", "slot_attn_core", "event_compact", "event_gather", "event_scatter",
            "event_mha", "qk_norm_rope_fwd", "qk_norm_rope_bwd", "cross_attention_fwd", "cross_attention_bwd",
-           "kv8_write", "kv8_attention"]
+           "kv8_write", "kv8_attention", "decay_attention_fwd", "decay_attention_bwd", "decay_attention_step",
+           "kv4_write", "kv4_read", "kv4_attention", "pages_resize", "page_slots"]
 
 _NS = "hclsm_b200"
 
@@ -310,3 +319,123 @@ def kv8_attention(q: Tensor, ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: T
 @kv8_attention.register_fake
 def _(q, ck, cv, k_scale, v_scale, k_tail, v_tail, lens, scale):
     return q.new_empty(q.shape)
+
+
+# ---- memories of a history -----------------------------------------------------------------------
+@torch.library.custom_op(f"{_NS}::decay_attention_fwd", mutates_args=())
+def decay_attention_fwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor],
+                        lens: Optional[Tensor], scale: float) -> Tuple[Tensor, Tensor]:
+    return _decay.decay_fwd(q, k, v, log_decay, state, lens, scale)
+
+
+@decay_attention_fwd.register_fake
+def _(q, k, v, log_decay, state, lens, scale):
+    B, _, H, D = q.shape
+    return v.new_empty(v.shape), q.new_empty((B, H, D, v.shape[3]), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::decay_attention_bwd", mutates_args=())
+def decay_attention_bwd(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Optional[Tensor],
+                        lens: Optional[Tensor], scale: float, do: Tensor, dstate: Optional[Tensor]) -> List[Tensor]:
+    g = _decay.decay_bwd(q, k, v, log_decay, state, lens, scale, do, dstate)
+    return [q.new_empty(0, dtype=torch.float32) if t is None else t for t in g]
+
+
+@decay_attention_bwd.register_fake
+def _(q, k, v, log_decay, state, lens, scale, do, dstate):
+    return [t.new_empty(t.shape) for t in (q, k, v)] + [
+        q.new_empty(0 if state is None else state.shape, dtype=torch.float32)]
+
+
+def _decay_setup(ctx, inputs, output):
+    if ctx.needs_input_grad[3]:
+        raise NotImplementedError("decay_attention_fwd has no gradient of log_decay: detach it")
+    ctx.save_for_backward(*inputs[:6])
+    ctx.scale = inputs[6]
+    ctx.set_materialize_grads(False)
+
+
+def _decay_backward(ctx, go, gstate):
+    q, k, v, log_decay, state, lens = ctx.saved_tensors
+    if go is None:
+        if gstate is None:
+            return (None,) * 7
+        go = torch.zeros_like(v)
+    dq, dk, dv, ds = decay_attention_bwd(q, k, v, log_decay, state, lens, ctx.scale, go, gstate)
+    return dq, dk, dv, None, None if state is None else ds, None, None
+
+
+torch.library.register_autograd(f"{_NS}::decay_attention_fwd", _decay_backward, setup_context=_decay_setup)
+
+
+def _detached(what, *tensors):
+    """An operator that mutates has no autograd formula, and grad mode is off inside it."""
+    if any(t.requires_grad for t in tensors):
+        raise NotImplementedError(f"{what} has no gradients: detach its tensors")
+
+
+@torch.library.custom_op(f"{_NS}::decay_attention_step", mutates_args=("state",))
+def decay_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor,
+                         active: Optional[Tensor], scale: float) -> Tensor:
+    _detached("decay_attention_step", q, k, v, log_decay, state)
+    return _decay.decay_attention_step(q, k, v, log_decay, state, active=active, scale=scale)
+
+
+@decay_attention_step.register_fake
+def _(q, k, v, log_decay, state, active, scale):
+    return v.new_empty(v.shape)
+
+
+@torch.library.custom_op(f"{_NS}::kv4_write", mutates_args=("ck", "cv", "k_scale", "v_scale"))
+def kv4_write(ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, k: Tensor, v: Tensor, slots: Tensor) -> None:
+    _detached("kv4_write", k, v)
+    _kv4.kv4_write(_kv4.Kv4Cache(ck, cv, k_scale, v_scale, k.dtype), k, v, slots)
+
+
+@kv4_write.register_fake
+def _(ck, cv, k_scale, v_scale, k, v, slots):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::kv4_read", mutates_args=())
+def kv4_read(ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, table: Tensor, lens: Optional[Tensor],
+             dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    return _kv4.kv4_read(_kv4.Kv4Cache(ck, cv, k_scale, v_scale, dtype), table, lens)
+
+
+@kv4_read.register_fake
+def _(ck, cv, k_scale, v_scale, table, lens, dtype):
+    _, Hkv, page, half = ck.shape
+    B, M = table.shape
+    return tuple(ck.new_empty((B, M * page, Hkv, 2 * half), dtype=dtype) for _ in range(2))
+
+
+@torch.library.custom_op(f"{_NS}::kv4_attention", mutates_args=())
+def kv4_attention(q: Tensor, ck: Tensor, cv: Tensor, k_scale: Tensor, v_scale: Tensor, table: Tensor,
+                  lens: Optional[Tensor], scale: float) -> Tensor:
+    return _kv4.kv4_attention(q, _kv4.Kv4Cache(ck, cv, k_scale, v_scale, q.dtype), table, lens, scale=scale)
+
+
+@kv4_attention.register_fake
+def _(q, ck, cv, k_scale, v_scale, table, lens, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_NS}::pages_resize", mutates_args=("table", "free", "n_free"))
+def pages_resize(table: Tensor, free: Tensor, n_free: Tensor, page: int, old_lens: Tensor, new_lens: Tensor) -> None:
+    _pages.pages_resize(_pages.PageTable(table, free, n_free, page), old_lens, new_lens)
+
+
+@pages_resize.register_fake
+def _(table, free, n_free, page, old_lens, new_lens):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::page_slots", mutates_args=())
+def page_slots(table: Tensor, start: Tensor, n: int, count: Optional[Tensor], page: int) -> Tensor:
+    return _pages.page_slots(table, start, n, count=count, page=page)
+
+
+@page_slots.register_fake
+def _(table, start, n, count, page):
+    return table.new_empty((table.shape[0], n), dtype=torch.int32)

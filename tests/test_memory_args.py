@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import hclsm_b200.torch_ops  # noqa: F401  (registers the ops)
 from hclsm_b200 import _lib
 from hclsm_b200.kernels import (Kv4Cache, PageTable, decay_attention, decay_attention_step, kv4_attention, kv4_read,
                                 kv4_write, page_slots, pages_resize)
@@ -306,3 +307,32 @@ def test_c_entries_refuse_on_the_host():
     assert lib.hclsm_page_slots(None, 1, 1, 32, None, None, 4, None, None) == 8
     assert lib.hclsm_page_slots(None, 1, 1, 31, None, None, 4, None, None) == 1
     assert lib.hclsm_page_slots(None, 1, 1, 32, None, None, 0, None, None) == 0
+
+
+def test_dispatcher_operators_trace_and_refuse(lib):
+    """Shapes under fake tensors; what mutates takes detached tensors; no gradient of log_decay."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    ops, z = torch.ops.hclsm_b200, torch.zeros
+    with FakeTensorMode():
+        q, v = z(2, 5, 3, 64, dtype=BF), z(2, 5, 3, 32, dtype=BF)
+        o, s = ops.decay_attention_fwd(q, q, v, z(3), None, None, 0.125)
+        assert o.shape == v.shape and o.dtype == BF and s.shape == (2, 3, 64, 32) and s.dtype == torch.float32
+        g = ops.decay_attention_bwd(q, q, v, z(3), s, None, 0.125, v, None)
+        assert [t.shape for t in g] == [q.shape, q.shape, v.shape, s.shape]
+        codes, scale = z(7, 3, 16, 32, dtype=torch.uint8), z(7, 3, 16, 2, dtype=BF)
+        table = z(2, 4, dtype=I32)
+        k, _ = ops.kv4_read(codes, codes, scale, scale, table, None, torch.float32)
+        assert k.shape == (2, 64, 3, 64) and k.dtype == torch.float32
+        assert ops.kv4_attention(q, codes, codes, scale, scale, table, None, 0.125).shape == q.shape
+        assert ops.page_slots(table, z(2, dtype=I32), 6, None, 16).shape == (2, 6)
+        assert ops.decay_attention_step(q[:, 0], q[:, 0], v[:, 0], z(3), s, None, 0.125).shape == (2, 3, 32)
+    x = _qkv(q=z(2, 5, 3, 64, dtype=BF, requires_grad=True))
+    with pytest.raises(NotImplementedError):
+        ops.decay_attention_fwd(x["q"], x["k"], x["v"], z(3, requires_grad=True), None, None, 0.125)
+    c = _cache()
+    k = z(3, 4, 2, 64, dtype=BF, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        ops.kv4_write(c.k, c.v, c.k_scale, c.v_scale, k, k, z(3, 4, dtype=I32))
+    with pytest.raises(NotImplementedError):
+        ops.decay_attention_step(z(2, 3, 64, requires_grad=True), z(2, 3, 64), z(2, 3, 32), z(3), z(2, 3, 64, 32), None, 1.0)

@@ -527,3 +527,35 @@ def test_decay_training_step_as_a_graph():
     w.weight.grad.zero_()
     step()
     assert torch.equal(w.weight.grad, want)
+
+
+def test_dispatcher_operators_give_the_functions_results():
+    import hclsm_b200.torch_ops  # noqa: F401
+
+    ops = torch.ops.hclsm_b200
+    x, g = _inputs(2, 150, 3, 64, 32, BF, True), _decays(3)
+    want = [x[n].detach().requires_grad_() for n in ("q", "k", "v", "S0")]
+    o, S = decay_attention(*want[:3], g, state=want[3], return_state=True)
+    grads = torch.autograd.grad((o, S), want, (x["do"], x["dS"]))
+    got = [x[n].detach().requires_grad_() for n in ("q", "k", "v", "S0")]
+    o2, S2 = ops.decay_attention_fwd(*got[:3], g, got[3], None, 0.125)
+    grads2 = torch.autograd.grad((o2, S2), got, (x["do"], x["dS"]))
+    assert torch.equal(o, o2) and torch.equal(S, S2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
+    only = torch.autograd.grad(ops.decay_attention_fwd(*got[:3], g, got[3], None, 0.125)[1], got, x["dS"])
+    ref = decay_grads(x["q"], x["k"], x["v"], g.clamp(min=-1e30), x["S0"], None, 0.125, torch.zeros_like(x["do"]), x["dS"])
+    assert (only[0] == 0).all() and torch.allclose(only[3].double(), ref[3], rtol=1e-5, atol=1e-5)
+    state, other = x["S0"].clone(), x["S0"].clone()
+    a = ops.decay_attention_step(*(x[n][:, 0] for n in ("q", "k", "v")), g, state, None, 0.125)
+    assert torch.equal(a, decay_attention_step(*(x[n][:, 0] for n in ("q", "k", "v")), g, other)) and torch.equal(state, other)
+    pages = PageTable.empty(2, 64, 8)
+    lens = torch.tensor([20, 40], device="cuda", dtype=torch.int32)
+    none = torch.zeros_like(lens)
+    ops.pages_resize(pages.table, pages.free, pages.n_free, 32, none, lens)
+    assert int(pages.n_free) == 5
+    cache = Kv4Cache.empty(8, 3, 64)
+    k = torch.randn(2, 40, 3, 64, device="cuda", dtype=BF)
+    slots = ops.page_slots(pages.table, none, 40, lens, 32)
+    ops.kv4_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, k, slots)
+    parts = (cache.k, cache.v, cache.k_scale, cache.v_scale, pages.table, lens)
+    assert all(torch.equal(a, b) for a, b in zip(ops.kv4_read(*parts, BF), kv4_read(cache, pages.table, lens)))
+    assert torch.equal(ops.kv4_attention(k[:, :1], *parts, 0.125), kv4_attention(k[:, :1], cache, pages.table, lens))
