@@ -94,7 +94,8 @@ SIGNATURES = {
     "hclsm_kv4_read": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
     "hclsm_kv4_attn_workspace_size": (_sz, [_vp, _i32, _i32, _i32, _i32]),
     "hclsm_kv4_attn": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, ctypes.c_float, _vp, _sz, _vp]),
-    "hclsm_pages_resize": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
+    "hclsm_pages_resize_workspace_size": (_sz, [_i32, _i32]),
+    "hclsm_pages_resize": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _sz, _vp]),
     "hclsm_page_slots": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp]),
     "hclsm_ssm_scan_bwd_noalloc_max_scratch": (_sz, []),
     "hclsm_ssm_scan_bwd_noalloc": (ctypes.c_int, [_vp] * 15 + [_i64, _i32, _i32, _i32, _i32, _i32, _vp]),

@@ -1,6 +1,11 @@
 // Page tables of a paged state cache: how many pages each entry's tokens need, kept on the device so that lengths never
 // come to the host.  All work is a prefix sum over the entries and a move of page numbers; the bound is the latency
 // of a handful of dependent loads (resize) and the slots written (slots).
+//
+// Released pages have ranks 0 ... R - 1 (entries, then places ascending), wanted places ranks 0 ... W - 1.  Pushed with the
+// first on top and then popped, the released page of rank r goes to the wanted place of rank r where r < W, else to place
+// n + R - 1 - r of the stack; a wanted place of rank w >= R gets what lay at n - 1 - (w - R).  So, once the request is
+// known to be valid, the pages can move in any order.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -147,6 +152,93 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
   if (me == 0) *p.n_free = n + (int)(released - wanted);
 }
 
+// ---- large tables: a kernel that checks and one that moves, over all SMs ---------------------------------
+// Up to kThreads entries.  131072 pages: 7 us in the two, 22 in one cluster.
+constexpr int kBlocks = 128;
+
+struct Round {
+  int2 off[kThreads + 1];  // released and wanted pages before an entry; behind the last: of all
+  int2 span[kThreads];     // pages an entry had, has
+  int2 warp_sum[kThreads / 32];
+};
+
+// The entries; false where a length lies outside the table.
+__device__ __forceinline__ bool load(const Resize& p, Round& r) {
+  const int b = threadIdx.x;
+  const int64_t most = (int64_t)p.M << p.shift;
+  int2 s = make_int2(0, 0);
+  bool fine = true;
+  if (b < p.B) {
+    const int from = p.old_lens[b], to = p.new_lens[b];
+    fine = from >= 0 && to >= 0 && from <= most && to <= most;
+    if (fine)
+      s = make_int2((int)(((int64_t)from + (1 << p.shift) - 1) >> p.shift),
+                    (int)(((int64_t)to + (1 << p.shift) - 1) >> p.shift));
+  }
+  int2 total;
+  const int2 at = scan(make_int2(max(s.x - s.y, 0), max(s.y - s.x, 0)), r.warp_sum, total);
+  r.span[b] = s;
+  r.off[b] = at;
+  if (b == 0) r.off[kThreads] = total;
+  __syncthreads();
+  return fine;
+}
+// The place in the table of the i-th released or wanted page: a search for the last entry that begins at or before it, which
+// is the one with the page.
+template <bool WANTED> __device__ __forceinline__ int32_t* place(const Resize& p, const Round& r, int i) {
+  int lo = 0;
+#pragma unroll
+  for (int step = kThreads / 2; step > 0; step >>= 1)
+    if (lo + step < p.B && (WANTED ? r.off[lo + step].y : r.off[lo + step].x) <= i) lo += step;
+  return p.table + (int64_t)lo * p.M + (WANTED ? r.span[lo].x + i - r.off[lo].y : r.span[lo].y + i - r.off[lo].x);
+}
+
+// ws: whether each block found a fault, then the free pages.
+__global__ void __launch_bounds__(kThreads) check_kernel(const __grid_constant__ Resize p, int32_t* ws) {
+  __shared__ Round r;
+  pdl_wait();
+  pdl_trigger();
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+  const int n = *p.n_free;
+  bool fine = load(p, r);
+  const int R = r.off[kThreads].x, W = r.off[kThreads].y;
+  fine = fine && n >= 0 && n <= p.P && (int64_t)n + R <= p.P && W <= (int64_t)n + R;
+  if (__syncthreads_and(fine)) {  // else the places below may not exist
+    for (int i = me; i < R; i += all) fine = fine && (unsigned)*place<false>(p, r, i) < (unsigned)p.P;
+    for (int i = me; i < W - R; i += all) fine = fine && (unsigned)p.stack[n - 1 - i] < (unsigned)p.P;
+  }
+  const int all_fine = __syncthreads_and(fine);
+  if (threadIdx.x == 0) ws[blockIdx.x] = !all_fine;
+  if (me == 0) ws[gridDim.x] = n;
+}
+
+__global__ void __launch_bounds__(kThreads) move_kernel(const __grid_constant__ Resize p, const int32_t* ws) {
+  __shared__ Round r;
+  pdl_wait();
+  pdl_trigger();
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+  const int n = ws[gridDim.x];
+  if (__syncthreads_or((int)threadIdx.x < (int)gridDim.x && ws[threadIdx.x])) {
+    if (me == 0) record_error(p.err, HCLSM_ERR_SHAPE);
+    return;
+  }
+  load(p, r);
+  const int R = r.off[kThreads].x, W = r.off[kThreads].y;
+  for (int i = me; i < W; i += all) {
+    int32_t* from = i < R ? place<false>(p, r, i) : p.stack + (n - 1 - (i - R));
+    const int32_t page = *from;
+    *from = -1;
+    *place<true>(p, r, i) = page;
+    if (i < R) p.stack[n + R - 1 - i] = -1;
+  }
+  for (int i = W + me; i < R; i += all) {
+    int32_t* from = place<false>(p, r, i);
+    p.stack[n + R - 1 - i] = *from;
+    *from = -1;
+  }
+  if (me == 0) *p.n_free = n + R - W;
+}
+
 struct Slots {
   const int32_t *table, *start, *count;
   int32_t* slots;
@@ -198,13 +290,30 @@ int log2_of(int n) {
 
 using namespace hclsm;
 
+// Where the two kernels over all SMs pay: more pages than a cluster moves in a few microseconds.
+static bool wide(int32_t B, int32_t M) { return B <= pages::kThreads && (int64_t)B * M > 16384; }
+
+extern "C" size_t hclsm_pages_resize_workspace_size(int32_t B, int32_t M) {
+  return B > 0 && M > 0 && wide(B, M) ? (pages::kBlocks + 1) * sizeof(int32_t) : 0;
+}
+
 extern "C" int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P,
-                                  int32_t page, const int32_t* old_lens, const int32_t* new_lens, void* stream) {
+                                  int32_t page, const int32_t* old_lens, const int32_t* new_lens, void* ws,
+                                  size_t ws_bytes, void* stream) {
   if (B < 0 || M < 0 || P < 0 || !pages::power_of_2(page)) return HCLSM_ERR_SHAPE;
   if ((int64_t)P * page > 0x7fffffff || (int64_t)B * M > 0x7fffffff) return HCLSM_ERR_SHAPE;
   if (B == 0) return HCLSM_OK;
   if ((!table && M) || (!stack && P) || !n_free || !old_lens || !new_lens) return HCLSM_ERR_NULL;
+  const size_t need = hclsm_pages_resize_workspace_size(B, M);
+  if (ws_bytes < need || (need && !ws)) return HCLSM_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return HCLSM_ERR_ALIGN;
   pages::Resize p = {table, stack, n_free, old_lens, new_lens, B, M, P, pages::log2_of(page), device_err_ptr()};
+  if (need) {
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int32_t* flags = static_cast<int32_t*>(ws);
+    if (const int rc = launch_pdl(pages::check_kernel, pages::kBlocks, pages::kThreads, 0, st, p, flags)) return rc;
+    return launch_pdl(pages::move_kernel, pages::kBlocks, pages::kThreads, 0, st, p, flags);
+  }
   // one small block takes a table of a few thousand pages faster than a cluster meets at its barriers
   const bool few = (int64_t)B * M <= 8192 && B <= pages::kFewThreads;
   cudaLaunchConfig_t cfg = {};

@@ -70,8 +70,12 @@ def pages_resize(pages: PageTable, old_lens: Tensor, new_lens: Tensor) -> None:
     new = _lib.index32(new_lens, (B,), "new_lens", dev)
     if old is None or new is None:
         raise ValueError("old_lens and new_lens are required")
-    _lib.check(_lib.load().hclsm_pages_resize(table.data_ptr(), B, M, free.data_ptr(), n_free.data_ptr(), free.numel(),
-                                              pages.page, old.data_ptr(), new.data_ptr(), _lib.stream_ptr(dev)),
+    lib, ws = _lib.load(), None
+    n = lib.hclsm_pages_resize_workspace_size(B, M)
+    if n:
+        ws = table.new_empty(n, dtype=torch.uint8)
+    _lib.check(lib.hclsm_pages_resize(table.data_ptr(), B, M, free.data_ptr(), n_free.data_ptr(), free.numel(), pages.page,
+                                      old.data_ptr(), new.data_ptr(), _lib.ptr(ws), n, _lib.stream_ptr(dev)),
                "hclsm_pages_resize")
 
 

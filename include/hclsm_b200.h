@@ -504,8 +504,9 @@ int hclsm_kv4_attn(const hclsm_kv4_cache* c, const int32_t* table, int32_t B, in
  * taken off or released hold -1.  A request that cannot be met (lengths outside [0, M * page], not
  * enough free pages, pages outside [0, P)) changes nothing and puts HCLSM_ERR_SHAPE in the error word.
  * page: a power of two. */
+size_t hclsm_pages_resize_workspace_size(int32_t B, int32_t M);
 int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P, int32_t page,
-                       const int32_t* old_lens, const int32_t* new_lens, void* stream);
+                       const int32_t* old_lens, const int32_t* new_lens, void* ws, size_t ws_bytes, void* stream);
 /* slots (B, n): of tokens start[b], start[b] + 1, ...; -1 behind the first count[b] (NULL: n) of them and where the
  * table has no page. */
 int hclsm_page_slots(const int32_t* table, int32_t B, int32_t M, int32_t page, const int32_t* start,

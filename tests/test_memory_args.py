@@ -301,9 +301,11 @@ def test_c_entries_refuse_on_the_host():
         assert lib.hclsm_kv4_read(cache(**kw), None, 1, 1, None, None, None, None) == rc, kw
         assert lib.hclsm_kv4_write(cache(**kw), None, None, None, 1, 1, None) == rc, kw
         assert lib.hclsm_kv4_attn(cache(**kw), None, 1, 1, None, None, None, 1, 1, 1.0, None, 0, None) == rc, kw
-    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1, 24, None, None, None) == 1
-    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1, 32, None, None, None) == 8
-    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1 << 27, 32, None, None, None) == 1
+    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1, 24, None, None, None, 0, None) == 1
+    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1, 32, None, None, None, 0, None) == 8
+    assert lib.hclsm_pages_resize(None, 1, 1, None, None, 1 << 27, 32, None, None, None, 0, None) == 1
+    assert lib.hclsm_pages_resize_workspace_size(64, 64) == 0 and lib.hclsm_pages_resize_workspace_size(64, 2048) > 0
+    assert lib.hclsm_pages_resize(16, 64, 2048, 16, 16, 9, 32, 16, 16, None, 0, None) == 4
     assert lib.hclsm_page_slots(None, 1, 1, 32, None, None, 4, None, None) == 8
     assert lib.hclsm_page_slots(None, 1, 1, 31, None, None, 4, None, None) == 1
     assert lib.hclsm_page_slots(None, 1, 1, 32, None, None, 0, None, None) == 0

@@ -402,7 +402,7 @@ def _same(pages, ref):
 
 
 @pytest.mark.parametrize("B,T,page,P", [(1, 100, 16, 7), (5, 300, 32, 40), (64, 2048, 32, 64 * 64), (1500, 200, 16, 9000),
-                                        (300, 1, 128, 300)])
+                                        (300, 1, 128, 300), (50, 9000, 16, 20000), (1024, 700, 32, 17000)])
 def test_pages_resize(B, T, page, P):
     """Random growth and shrinking against lists, requests that cannot be met among them."""
     rng = random.Random(B)
@@ -423,8 +423,9 @@ def test_pages_resize(B, T, page, P):
     assert len(set(held)) == len(held) and sorted(held + ref.free[:ref.n]) == list(range(P))
 
 
-def test_pages_resize_undone_and_refused():
-    pages = PageTable.empty(4, 256, 20, page=32)
+@pytest.mark.parametrize("columns", [256, 8192 * 32])  # a small table, and one whose pages all SMs move
+def test_pages_resize_undone_and_refused(columns):
+    pages = PageTable.empty(4, columns, 20, page=32)
     t = lambda *x: torch.tensor(x, device="cuda", dtype=torch.int32)  # noqa: E731
     pages_resize(pages, t(0, 0, 0, 0), t(100, 0, 33, 64))
     was = [x.clone() for x in (pages.table, pages.free, pages.n_free)]
@@ -432,7 +433,7 @@ def test_pages_resize_undone_and_refused():
     pages_resize(pages, t(256, 32, 33, 65), t(100, 0, 33, 64))
     same = lambda: all(torch.equal(a, b) for a, b in zip(was, (pages.table, pages.free, pages.n_free)))  # noqa: E731
     assert same()
-    for old, new in (((100, 0, 33, 64), (256, 256, 256, 64)), ((100, 0, 33, 64), (257, 0, 0, 0)),
+    for old, new in (((100, 0, 33, 64), (256, 256, 256, 64)), ((100, 0, 33, 64), (columns + 1, 0, 0, 0)),
                      ((100, 0, -1, 64), (0, 0, 0, 0)), ((100, 0, 64, 256), (100, 0, 33, 64))):
         assert hclsm_b200.device_error() == 0
         pages_resize(pages, t(*old), t(*new))  # too many, too long, negative, pages that are not held
