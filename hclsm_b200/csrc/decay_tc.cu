@@ -42,7 +42,8 @@ template <int DX, int DY, int NP> struct Shape {
   static constexpr int kY = kStaged && !kOverV ? kV : 0;
   static constexpr size_t kBytes = 2 * kX + kV + NP * kX + kT + kY + 1024;
   static constexpr int kThreads = (kWgT + kWg) * 128 + 64;
-  static constexpr uint32_t kColY = 128, kColXt = kSmall ? 64 : 256, kColT = kSmall ? 192 : 384;
+  // columns of A and P (0), y, x T (small: y's sum starts from it), the state's products
+  static constexpr uint32_t kColY = 128, kColXt = kSmall ? kColY : 256, kColT = kSmall ? 192 : 384;
   static constexpr uint32_t kCols = kSmall ? 256 : 512;
   static constexpr int kPerSm = kSmall ? 2 : 1;
 };
@@ -208,8 +209,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
                    d_p = smem_desc_sw128(smem_u32(sP), kBlock, 1024);
     for (int it = 0; it < chunks; ++it) {
       if (!wait_all(k_full, it) || !wait_all(x_full, it)) break;
-      // over the chunk before's weights (products run in order) and, where TMEM is short, its x T
-      if (Sh::kSmall && it > 0 && !wait_all(y_free, it - 1)) break;
+      // over the chunk before's weights: products run in order
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < DX / 16; ++k) {
@@ -217,20 +217,15 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         if (k < kx) umma_ss(one, tmem, desc_at(d_x, off), desc_at(d_k, off), id_s, k != 0);
       }
       umma_done(one, s_full);
-      auto read_state = [&] {
+      // y_free: the row's threads have read the chunk before's
+      if (!wait_all(t_ready, it) || (it > 0 && !wait_all(y_free, it - 1))) break;
+      tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < DX / 16; ++k)
-          if (k < kx)
-            umma_ss(one, tmem + Sh::kColXt, desc_at(d_x, (k >> 2) * kBlock + (k & 3) * 32),
-                    desc_at(d_t, k * 16 * kRowBytes), id_y, k != 0);
-        umma_done(one, x_free);
-      };
-      if constexpr (!Sh::kSmall) {
-        // y_free: the row's threads have read the chunk before's
-        if (!wait_all(t_ready, it) || (it > 0 && !wait_all(y_free, it - 1))) break;
-        tc_fence_after();
-        read_state();
-      }
+      for (int k = 0; k < DX / 16; ++k)
+        if (k < kx)
+          umma_ss(one, tmem + Sh::kColXt, desc_at(d_x, (k >> 2) * kBlock + (k & 3) * 32),
+                  desc_at(d_t, k * 16 * kRowBytes), id_y, k != 0);
+      umma_done(one, x_free);
       if (!wait_all(w_ready, it) || !wait_all(v_full, it)) break;
       tc_fence_after();
 #pragma unroll
@@ -241,13 +236,11 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
                   id_t, !(i == NP - 1 && k == 0));
       umma_done(one, t_done);
       if (!wait_all(p_ready, it)) break;
-      if (Sh::kSmall && !wait_all(t_ready, it)) break;
       tc_fence_after();
-      if constexpr (Sh::kSmall) read_state();
 #pragma unroll
       for (int k = 0; k < kTok / 16; ++k)
         umma_ts(one, tmem + Sh::kColY, tmem + k * 8 + (WG == 2 && k >= 4 ? 32 : 0), desc_at(d_v, k * 16 * kRowBytes), id_y,
-                k != 0);
+                Sh::kSmall || k != 0);
       umma_done(one, y_done);
     }
   } else if (warp < WGT * 4) {
@@ -298,43 +291,37 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       if (it > 0 && !(ok = wait_all(t_done, it - 1))) break;
       advance(m);
       m = min(n - first_token(it), kTok);
-      auto copy_state = [&] {  // T in bf16, for x T
-        if (it > 0 && !wait_all(x_free, it - 1)) return false;  // the copy before has been read
-        if (holds) {
-          const RowAt<DX> at(smem_u32(sT), row);
+      // T in bf16, for x T
+      if (it > 0 && !(ok = wait_all(x_free, it - 1))) break;  // the copy before has been read
+      if (holds) {
+        const RowAt<DX> at(smem_u32(sT), row);
 #pragma unroll
-          for (int c = 0; c < kCols; c += 8) {
-            uint32_t q[4];
+        for (int c = 0; c < kCols; c += 8) {
+          uint32_t q[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = pack_bf16(T[c / 2 + e].x, T[c / 2 + e].y);
-            st_shared(at(y0 / 8 + c / 8), q[0], q[1], q[2], q[3]);
-          }
+          for (int e = 0; e < 4; ++e) q[e] = pack_bf16(T[c / 2 + e].x, T[c / 2 + e].y);
+          st_shared(at(y0 / 8 + c / 8), q[0], q[1], q[2], q[3]);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc_fence_before();
-        mbar_arrive(t_ready);
-        return true;
-      };
-      auto weigh = [&] {  // the pieces of w k
-        if (!wait_all(k_full, it)) return false;
-        const int c0 = half * (kDims / 8);
-        const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();
+      mbar_arrive(t_ready);
+      // the pieces of w k
+      if (!(ok = wait_all(k_full, it))) break;
+      const int c0 = half * (kDims / 8);
+      const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
 #pragma unroll 1
-        for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
-        if (m < kTok) {
-          if (!wait_all(v_full, it)) return false;
-          if (row >= m) {
-            clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
-            clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
-          }
+      for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
+      if (m < kTok) {
+        if (!(ok = wait_all(v_full, it))) break;
+        if (row >= m) {
+          clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);
+          clear_row(smem_u32(sV), 0, 1, row, y0 / 8, (y0 + kCols) / 8);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        tc_fence_before();  // the products' sum has been read
-        mbar_arrive(w_ready);
-        return true;
-      };
-      // x T comes before the update's products, or behind them where it has to wait for P's columns
-      ok = Sh::kSmall ? weigh() && copy_state() : copy_state() && weigh();
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc_fence_before();  // the products' sum has been read
+      mbar_arrive(w_ready);
     }
     if (ok && chunks > 0) {
       ok = wait_all(t_done, chunks - 1);
@@ -409,10 +396,25 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         // over scores that this thread has read
         tmem_st16(tS + half * 64 + q * 16, pw);
       }
+      const float lead = ex2(l2 * (float)(place + 1 - r));
+      if constexpr (Sh::kSmall) {  // x T times g^{i+1-r}: what P v is added to
+        if (!(ok = wait_all(x_free, it))) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < kCols; c += 16) {
+          float a[16];
+          tmem_ld16_nowait(tY + y0 + c, a);
+          tmem_wait_ld();
+          tmem_pin<16>(a);
+          uint32_t q[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) q[e] = __float_as_uint(a[e] * lead);
+          tmem_st16(tY + y0 + c, q);
+        }
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(p_ready);
-      const float lead = ex2(l2 * (float)(place + 1 - r)) * p.f;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t0 + row) * p.H + h) * (int64_t)p.Dv + y0;
       if (!(ok = wait_all(y_done, it))) break;
       tc_fence_after();
@@ -424,10 +426,10 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
       for (int c = 0; c < kCols; c += 16) {
         float a[16], x[16];
         tmem_ld16_nowait(tY + y0 + c, a);
-        tmem_ld16_nowait(tX + y0 + c, x);
+        if constexpr (!Sh::kSmall) tmem_ld16_nowait(tX + y0 + c, x);
         tmem_wait_ld();
         tmem_pin<16>(a);
-        tmem_pin<16>(x);
+        if constexpr (!Sh::kSmall) tmem_pin<16>(x);
         if (c + 16 == kCols) {
           tc_fence_before();
           mbar_arrive(y_free);
@@ -435,8 +437,9 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>
         uint32_t q[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          float2 t = mul2(make_float2(a[2 * e], a[2 * e + 1]), make_float2(p.f, p.f));
-          t = fma2(make_float2(x[2 * e], x[2 * e + 1]), make_float2(lead, lead), t);
+          float2 t = make_float2(a[2 * e], a[2 * e + 1]);
+          if constexpr (!Sh::kSmall) t = fma2(make_float2(x[2 * e], x[2 * e + 1]), make_float2(lead, lead), t);
+          t = mul2(t, make_float2(p.f, p.f));
           q[e] = pack_bf16(t.x, t.y);
         }
         if constexpr (Sh::kStaged) {
