@@ -144,7 +144,8 @@ def decay_attention(q, k, v, log_decay, *, state=None, lens=None, scale=None, re
     -inf forgets all).  ``state`` (B, H, D, Dv) fp32: the state before the first token, default zeros;
     with ``return_state`` the result is (o, the state behind the last token).  ``lens`` (B,) int: entry
     b's first lens[b] tokens count (clamped to [0, L]); the others may hold anything, NaN included, and their
-    outputs and gradients are zeros.  ``scale`` > 0, default D ** -0.5.  float32 or bfloat16, head dims up to
+    outputs and gradients are zeros.  A token that counts and is not finite spreads to the
+    tokens of its chunk (128; 64 in fp32), the earlier ones too.  ``scale`` > 0, default D ** -0.5.  float32 or bfloat16, head dims up to
     128; sums and states in fp32.  Differentiable in q, k, v and state, not in log_decay; bit-reproducible.
     """
     args = _prepare(q, k, v, log_decay, state, lens, scale)

@@ -36,6 +36,7 @@ class Kv4Cache:
     def __init__(self, k, v, k_scale, v_scale, dtype=torch.bfloat16):
         d = self.__dict__  # past __setattr__: a microsecond less
         d["k"], d["v"], d["k_scale"], d["v_scale"], d["dtype"], d["_packed"] = k, v, k_scale, v_scale, dtype, None
+        self._args()
 
     def __setattr__(self, name, value):
         self.__dict__[name] = value

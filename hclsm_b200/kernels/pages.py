@@ -30,6 +30,10 @@ class PageTable:
     def empty(cls, batch: int, max_tokens: int, pages: int, *, page: int = 32, device="cuda") -> "PageTable":
         """No entry has a page; room for ``max_tokens`` tokens (rounded up to whole pages) an entry, page 0 on top of
         the stack of all ``pages``."""
+        _check_page(page)
+        if max_tokens < 0 or pages < 0:
+            raise ValueError(f"max_tokens {max_tokens}, pages {pages}")
+
         def full(*shape):
             return torch.full(shape, -1, dtype=torch.int32, device=device)
 

@@ -447,7 +447,7 @@ int hclsm_kv8_attn(const hclsm_kv8_cache* c, const hclsm_view* q, void* o, const
  * log_decay (H) fp32 counts as 0 where above.  s0 (B, H, D, Dv) fp32 or NULL (zeros): the state
  * before the first token; s1 or NULL: the state behind the last.  lens (B) or NULL: an
  * entry's first lens[b] tokens count; the others are not operands, and their o and
- * gradients are zeros.  Backward: dout, ds1 (of s1, or NULL) give dq, dk, dv and ds0 (or NULL).
+ * gradients are zeros (one that counts and is not finite spreads over its chunk of 64 or 128).  Backward: dout, ds1 (of s1, or NULL) give dq, dk, dv and ds0 (or NULL).
  * ------------------------------------------------------------------------- */
 typedef struct {
   hclsm_view q, k, v, dout;

@@ -234,7 +234,11 @@ def test_kv4_refusals(lib):
         for call in (lambda: kv4_write(c, x, x, slots), lambda: kv4_read(c, table), lambda: kv4_attention(x, c, table)):
             _refused(lib, ValueError, call)
     c = _cache()
-    _refused(lib, TypeError, kv4_write, _cache(dtype=torch.float16), x, x, slots)
+    _refused(lib, TypeError, _cache, dtype=torch.float16)
+    for kw in (dict(page=24), dict(head_dim=48), dict(kv_heads=0)):
+        _refused(lib, ValueError, Kv4Cache.empty, **{**dict(pages=3, kv_heads=1, head_dim=64, device="cpu"), **kw})
+    for kw in (dict(page=24), dict(page=0), dict(pages=-1), dict(max_tokens=-1)):
+        _refused(lib, ValueError, PageTable.empty, **{**dict(batch=2, max_tokens=64, pages=4, device="cpu"), **kw})
     for k, s in ((x[:, :, :1], slots), (x[..., :32], slots), (x, slots[:, :3]), (x, None)):
         _refused(lib, ValueError, kv4_write, c, k, k, s)
     _refused(lib, ValueError, kv4_write, c, x, x[:, :3], slots)

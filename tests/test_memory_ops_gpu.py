@@ -211,6 +211,107 @@ def test_decay_attention_step(B, H, D, Dv, dtype):
     assert torch.equal(state[~active], x["S0"][~active])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_decay_attention_broadcast_inputs(dtype):
+    """Dims that are expanded (strides of zero), and their gradients' sums."""
+    B, L, H, D = 2, 140, 3, 64
+    x, g = _inputs(B, L, H, D, D, dtype, False), _decays(H)
+    k1, v1 = x["k"][:, :, :1].clone().requires_grad_(), x["v"][:1].clone().requires_grad_()
+    k, v = k1.expand(B, L, H, D), v1.expand(B, L, H, D)
+    o = decay_attention(x["q"], k, v, g)
+    full = [t.detach().contiguous().requires_grad_() for t in (k, v)]
+    want = decay_attention(x["q"], *full, g)
+    fp32 = (L + 2 * D + 256) * 2.0 ** -24
+    ao = decay_ref(x["q"].abs(), full[0].detach().abs(), full[1].detach().abs(), g.clamp(min=-1e30), scale=D ** -0.5)[0]
+    # expanded bf16 rows go by the fp32 path: each is off the definition by its roundings
+    _near(o.detach(), want.detach().double(), 4 * HALF_STEP[dtype] * (want.detach().double().abs() + ao) + 2 * fp32 * ao, "o")
+    dk, dv = torch.autograd.grad(o, (k1, v1), x["do"])
+    wk, wv = torch.autograd.grad(want, full, x["do"])
+    assert dk.shape == k1.shape and dv.shape == v1.shape
+    for got, ref in ((dk, wk.double().sum(2, keepdim=True)), (dv, wv.double().sum(0, keepdim=True))):
+        assert (got.double() - ref).norm() <= (2.0 ** -6 if dtype == BF else 1e-5) * ref.norm()
+
+
+def test_decay_attention_value_that_is_not_finite():
+    """It reaches its own chunk and what comes behind it, in its entry and head alone."""
+    x, g = _inputs(2, 500, 3, 64, 64, BF, False), torch.full((3,), -0.01, device="cuda")
+    clean = decay_attention(x["q"], x["k"], x["v"], g)
+    x["v"][1, 300, 1, 5] = float("nan")
+    o = decay_attention(x["q"], x["k"], x["v"], g)
+    assert torch.equal(o[0], clean[0]) and torch.equal(o[1, :, 0], clean[1, :, 0]) and torch.equal(o[1, :, 2], clean[1, :, 2])
+    assert torch.equal(o[1, :256, 1], clean[1, :256, 1]) and o[1, 300:, 1, 5].isnan().all()
+
+
+def test_decay_attention_far_offsets():
+    """More than 2^31 elements: the last tokens, whose heads forget within a few, against a call on them alone."""
+    L, H, D, n = 300000, 64, 128, 512
+    g = torch.full((H,), -0.7, device="cuda")
+    q, k, v = (torch.empty(1, L, H, D, device="cuda", dtype=BF).normal_() for _ in range(3))
+    o, S = decay_attention(q, k, v, g, return_state=True)
+    tail = [t[:, L - n:].contiguous() for t in (q, k, v)]
+    ro, rS = decay_ref(*tail, g, scale=D ** -0.5)
+    ao, aS = decay_ref(*(t.abs() for t in tail), g, scale=D ** -0.5)
+    fp32 = (n + 2 * D + 256) * 2.0 ** -24
+    _near(o[:, L - 200:], ro[:, -200:], 2.0 ** -8 * (ro.abs() + ao)[:, -200:] + fp32 * ao[:, -200:], "o")
+    _near(S, rS, fp32 * aS, "state")
+    del o, S
+    v = v.requires_grad_()
+    o = decay_attention(q, k, v, g)
+    dv, = torch.autograd.grad(o, v, q)
+    rv = decay_grads(*tail, g, None, None, D ** -0.5, tail[0], None)[2]
+    av = decay_grads(*(t.abs() for t in tail), g, None, None, D ** -0.5, tail[0].abs(), None)[2]
+    _near(dv[:, L - 200:], rv[:, -200:], 2.0 ** -8 * (rv.abs() + av)[:, -200:] + fp32 * av[:, -200:], "dv")
+
+
+def test_two_streams_at_once():
+    """Calls that run side by side on two streams, each with workspaces of its own, give what they give alone."""
+    x, g = _inputs(1, 6000, 2, 64, 64, BF, False), _decays(2)  # cut into segments
+    cache, table = _pool(2, 40960, 1, 64, 32, BF)
+    cache.k_scale.fill_(0.25), cache.v_scale.fill_(0.5)
+    q = torch.randn(2, 1, 2, 64, device="cuda", dtype=BF)  # more splits than a cluster joins
+    want = decay_attention(x["q"], x["k"], x["v"], g, return_state=True), kv4_attention(q, cache, table)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((decay_attention(x["q"], x["k"], x["v"], g, return_state=True), kv4_attention(q, cache, table)))
+    torch.cuda.synchronize()
+    for (o, S), a in got:
+        assert torch.equal(o, want[0][0]) and torch.equal(S, want[0][1]) and torch.equal(a, want[1])
+
+
+def test_two_graphs_of_the_same_calls():
+    """Two captured graphs, their memory in one pool, replayed in turn."""
+    x, g = _inputs(1, 6000, 2, 64, 64, BF, False), _decays(2)
+    cache, table = _pool(2, 40960, 1, 64, 32, BF)
+    cache.k_scale.fill_(0.25), cache.v_scale.fill_(0.5)
+    q = torch.randn(2, 1, 2, 64, device="cuda", dtype=BF)
+
+    def calls():
+        return decay_attention(x["q"], x["k"], x["v"], g), kv4_attention(q, cache, table)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        calls()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(calls())
+        graphs.append(graph)
+    for _ in range(3):
+        for t in (x["q"], x["v"], q):
+            t.normal_()
+        want = calls()
+        for graph, out in zip(graphs, outs):
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
 def test_decay_attention_empty():
     x, g = _inputs(2, 0, 3, 64, 32, BF, True), _decays(3)
     leaves = [x[n].requires_grad_() for n in ("q", "k", "v", "S0")]
