@@ -34,8 +34,10 @@ struct Maps {
 constexpr int kTok = 128;                     // tokens of a chunk
 constexpr int kBlock = kTok * (int)kRowBytes; // 64 dims of a staged tile
 
-template <int DX, int DY, int NP> struct Shape {
-  static constexpr bool kSmall = DX == 64 && DY == 64;
+// SMALL: heads of 64 with two blocks an SM; without it, where blocks are no more than SMs, a second warpgroup for the
+// rows and TMEM of its own for x T make a chunk's chain shorter.
+template <int DX, int DY, int NP, bool SMALL> struct Shape {
+  static constexpr bool kSmall = SMALL;
   static constexpr int kWgT = 2, kWg = kSmall ? 1 : 2;  // warpgroups of the state, of the rows: they share out the columns
   static constexpr int kX = DX / 64 * kBlock, kV = DY / 64 * kBlock;
   static constexpr int kT = DY / 64 * DX * (int)kRowBytes;  // bf16 copy of the state
@@ -123,12 +125,12 @@ __device__ __forceinline__ void clear_row(uint32_t to, int step, int n, int row,
     for (int c = c0; c < c1; ++c) st_shared(RowAt<kTok>(to + i * step, row)(c), 0, 0, 0, 0);
 }
 
-template <int DX, int DY, int NP>
-__global__ void __launch_bounds__(Shape<DX, DY, NP>::kThreads, Shape<DX, DY, NP>::kPerSm)
+template <int DX, int DY, int NP, bool SMALL>
+__global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, DY, NP, SMALL>::kPerSm)
     tc_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Batch bt) {
   const int which = (int)(blockIdx.x % bt.n);
   const Pass& p = bt.p[which];
-  using Sh = Shape<DX, DY, NP>;
+  using Sh = Shape<DX, DY, NP, SMALL>;
   constexpr int WGT = Sh::kWgT, WG = Sh::kWg;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -680,10 +682,10 @@ void tc_cut(Batch& b) {
   cut(b, kTok, 5.0f, 1.5f, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
 }
 
-template <int DX, int DY, int NP>
+template <int DX, int DY, int NP, bool SMALL>
 int launch(const Batch& b, cudaStream_t st) {
-  using Sh = Shape<DX, DY, NP>;
-  auto fn = tc_kernel<DX, DY, NP>;
+  using Sh = Shape<DX, DY, NP, SMALL>;
+  auto fn = tc_kernel<DX, DY, NP, SMALL>;
   // before the maps: encoding one needs the device's context, which this call makes current in a new thread
   if (!set_smem_limit(reinterpret_cast<const void*>(fn), Sh::kBytes)) return HCLSM_ERR_LAUNCH;
   Maps maps;
@@ -708,17 +710,19 @@ int launch(const Batch& b, cudaStream_t st) {
   return launch_pdl(fn, (unsigned)grid, Sh::kThreads, Sh::kBytes, st, maps, b);
 }
 
-template <int DX, int DY>
+template <int DX, int DY, bool SMALL>
 int launch_np(const Batch& b, cudaStream_t st) {
   bool out = false;  // a state that is returned
   for (int i = 0; i < b.n; ++i) out = out || (b.p[i].last && b.p[i].segs == 1);
-  return out ? launch<DX, DY, 3>(b, st) : launch<DX, DY, 2>(b, st);
+  return out ? launch<DX, DY, 3, SMALL>(b, st) : launch<DX, DY, 2, SMALL>(b, st);
 }
 
 int tc_run(const Batch& b, cudaStream_t st) {
   const Pass& p = b.p[0];
-  if (p.Dk <= 64) return p.Dv <= 64 ? launch_np<64, 64>(b, st) : launch_np<64, 128>(b, st);
-  return p.Dv <= 64 ? launch_np<128, 64>(b, st) : launch_np<128, 128>(b, st);
+  if (p.Dk <= 64 && p.Dv <= 64)
+    return (int64_t)b.n * p.B * p.H * p.segs <= num_sms() ? launch_np<64, 64, false>(b, st) : launch_np<64, 64, true>(b, st);
+  if (p.Dk <= 64) return launch_np<64, 128, false>(b, st);
+  return p.Dv <= 64 ? launch_np<128, 64, false>(b, st) : launch_np<128, 128, false>(b, st);
 }
 
 }  // namespace decay
