@@ -530,9 +530,11 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   unsigned char *sP = smem, *sK = sP + NP * Sh::kX, *sV = sK + Sh::kX;  // the pieces first, as above
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  constexpr int kBars = ST + 4;
+  constexpr int kBars = 2 * ST + 3;
   __shared__ uint64_t bars[kBars];
-  uint64_t *full = bars, *k_full = bars + ST, *ready = k_full + 1, *done = ready + 1, *drain = done + 1;
+  // done: one a stage of v.  The copies wait for products of two chunks ago, and behind one barrier of both stages the
+  // products of the chunk between might have ended as well: a wait for the phase before the last does not return.
+  uint64_t *full = bars, *done = bars + ST, *k_full = bars + 2 * ST, *ready = k_full + 1, *drain = ready + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int kTmaWarp = WG * 4, kMmaWarp = WG * 4 + 1;
   if (warp == kMmaWarp) {
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
         mbar_expect_tx(k_full, Sh::kX);
         for (int d = 0; d < DX / 64; ++d) tma_load_4d(sK + d * kBlock, &maps.k[which], d * 64, t0, h, (int)b, k_full);
         asked_k = it + 1;
-        if (it >= ST && !wait(done, it - ST)) break;
+        if (it >= ST && !wait(&done[s], it / ST - 1)) break;
         mbar_expect_tx(&full[s], Sh::kV);
         for (int d = 0; d < DY / 64; ++d)
           tma_load_4d(sV + s * Sh::kV + d * kBlock, &maps.v[which], d * 64, t0, h, (int)b, &full[s]);
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
         for (int k = 0; k < kTok / 16; ++k)
           umma_ss(one, tmem + (it & 1) * DY, desc_at(d_p, i * Sh::kX + k * 16 * kRowBytes),
                   desc_at(d_v, it % ST * Sh::kV + k * 16 * kRowBytes), id_t, !(i == NP - 1 && k == 0));
-      umma_done(one, done);
+      umma_done(one, &done[it % ST]);
     }
   } else {
     const int row = tid & 127, half = tid >> 7;
@@ -619,7 +621,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
       const int s = it % ST, t = lo + it * kTok + row;
       if (!(ok = wait_all(k_full, it))) break;
       // the products that read the pieces are complete
-      if (it > 0 && !(ok = wait_all(done, it - 1))) break;
+      if (it > 0 && !(ok = wait_all(&done[(it - 1) % ST], (it - 1) / ST))) break;
       const int c0 = half * (kDims / 8);
       const float w = ex2(l2 * (float)(p.rev ? t - lo + 1 : hi - 1 - t));
 #pragma unroll 1
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
         add(it - 1);
       }
     }
-    if (ok && chunks > 0 && wait_all(done, chunks - 1)) {
+    if (ok && chunks > 0 && wait_all(&done[(chunks - 1) % ST], (chunks - 1) / ST)) {
       tc_fence_after();
       add(chunks - 1);
     }

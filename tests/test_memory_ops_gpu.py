@@ -312,6 +312,29 @@ def test_two_graphs_of_the_same_calls():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("B,H,D", [(8, 6, 64), (1, 16, 128)])
+def test_decay_attention_segments_on_busy_multiprocessors(B, H, D):
+    """Segments of many chunks, blocks of several calls side by side: whichever warp is held up, no wait misses its turn."""
+    x, g = _inputs(B, 4096, H, D, D, BF, False), _decays(H)
+
+    def call():
+        leaves = [x[n].detach().requires_grad_() for n in ("q", "k", "v")]
+        o = decay_attention(*leaves, g)
+        return (o, *torch.autograd.grad(o, leaves, x["do"]))
+
+    want = call()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    wrong = []
+    for _ in range(40):
+        for s in streams:
+            with torch.cuda.stream(s):
+                wrong += [(a != b).any() for a, b in zip(call(), want)]
+    torch.cuda.synchronize()
+    assert not torch.stack(wrong).any()
+
+
 def test_decay_attention_empty():
     x, g = _inputs(2, 0, 3, 64, 32, BF, True), _decays(3)
     leaves = [x[n].requires_grad_() for n in ("q", "k", "v", "S0")]
