@@ -315,7 +315,8 @@ int simt_run(const Batch& b, cudaStream_t st) {
 
 void simt_cut(Batch& b) {
   const Pass& p = b.p[0];
-  cut(b, kC, 1.0f, 1.1f, (int64_t)b.n * p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
+  cut(b, kC, 1.6f, 1.1f, 1.0f, 0.0f,
+      (int64_t)b.n * p.B * p.H * ((p.Dv + kE - 1) / kE), (int64_t)num_sms() * (p.Dk <= 64 ? 2 : 1));
 }
 
 // ---- one token -------------------------------------------------------------------------------

@@ -71,18 +71,20 @@ struct Batch {
   int n;
 };
 
-// Segments of a head, as their cost has it, in chunks' times of a block that is alone on its SM: a chunk costs 1.6 with
-// the segments' own sums, `crowd` as much where blocks share an SM, and the sums and the join `fixed` on top.
-// Measured with heads of 64 in bf16 (fixed 5: 13 us, crowd 1.5): 48 heads of 16 chunks 39 us in six segments, 46 whole; of 8 chunks
-// 33 in four, 25 whole; 6 heads of 16 chunks 20 in eight, 46 whole.
-inline void cut(Batch& b, int chunk, float fixed, float crowd, int64_t have, int64_t room) {
+// Segments of a head, as their cost has it, in chunks' times of a block that is alone on its SM: with the segments' own
+// sums a chunk costs `twice`, `crowd` as much where blocks share an SM; the sums' and the join's launches cost `fixed`, and
+// what they move `load` a block of every SM.  Measured in bf16 (1.9, 1.4, 4, 4; us, whole against segments): 6 heads of 64,
+// 8 chunks 20 against 17 in eight, 32 chunks 67 against 24 in sixteen and 31 in 32; 48 heads of 64, 16 chunks 36 against
+// 40 in six, 32 chunks 69 against 58 in six; 16 heads of 128, 8 chunks 27 against 38 in eight, 16 chunks 48 against 43;
+// 64 heads of 128, 128 chunks 348 against 377 in two.
+inline void cut(Batch& b, int chunk, float twice, float crowd, float fixed, float load, int64_t have, int64_t room) {
   const int chunks = (b.p[0].L + chunk - 1) / chunk, sms = num_sms();
   auto shared = [&](int64_t blocks) { return blocks > sms ? crowd : 1.0f; };
   int best = chunks > 1 ? chunks : 1;  // chunks of a segment
   float least = (float)chunks * shared(have);
   for (int64_t s = 2; s <= chunks && s * have <= room; ++s) {
     const int each = (int)((chunks + s - 1) / s);
-    const float cost = fixed + 1.6f * (float)each * shared(s * have);
+    const float cost = fixed + load * (float)(s * have) / (float)sms + twice * (float)each * shared(s * have);
     if (cost < least) least = cost, best = each;
   }
   for (int i = 0; i < b.n; ++i) b.p[i].seg_chunks = best, b.p[i].segs = chunks > 0 ? (chunks + best - 1) / best : 1;

@@ -681,7 +681,7 @@ bool tc_ok(const Batch& b) {
 
 void tc_cut(Batch& b) {
   const Pass& p = b.p[0];
-  cut(b, kTok, 5.0f, 1.5f, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
+  cut(b, kTok, 1.9f, 1.4f, 4.0f, 4.0f, (int64_t)b.n * p.B * p.H, (int64_t)num_sms() * (p.Dk <= 64 && p.Dv <= 64 ? 2 : 1));
 }
 
 template <int DX, int DY, int NP, bool SMALL>
