@@ -211,6 +211,17 @@ def test_decay_attention_step(B, H, D, Dv, dtype):
     assert torch.equal(state[~active], x["S0"][~active])
 
 
+def test_decay_attention_backward_of_a_state_that_has_moved_on():
+    """The step changes its state in place: a backward that needs the state as it was says so."""
+    x, g = _inputs(2, 3, 2, 64, 32, BF, True), _decays(2)
+    o = decay_attention(x["q"].requires_grad_(), x["k"], x["v"], g, state=x["S0"])
+    decay_attention_step(x["k"][:, 0], x["k"][:, 0], x["v"][:, 0], g, x["S0"], out=torch.empty_like(x["S0"]))
+    torch.autograd.grad(o, x["q"], x["do"], retain_graph=True)
+    decay_attention_step(x["k"][:, 0], x["k"][:, 0], x["v"][:, 0], g, x["S0"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(o, x["q"], x["do"])
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_decay_attention_broadcast_inputs(dtype):
     """Dims that are expanded (strides of zero), and their gradients' sums."""
