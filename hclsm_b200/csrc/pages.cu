@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(256) slots_kernel(const __grid_constant__ Slot
         s[e] = -1;
         if (j + e < count && at >= 0 && at < most) {
           const int page = row[at >> p.shift];
-          if (page >= 0) s[e] = (int)((uint32_t)page << p.shift | ((uint32_t)at & mask));
+          // a number that no slot of 31 bits holds: the last slot, which is behind every cache
+          if (page >= 0) s[e] = page >> (31 - p.shift) ? 0x7fffffff : (int)((uint32_t)page << p.shift | ((uint32_t)at & mask));
         }
       }
       if (wide) {

@@ -85,7 +85,8 @@ def pages_resize(pages: PageTable, old_lens: Tensor, new_lens: Tensor) -> None:
 
 def page_slots(table: Tensor, start: Tensor, n: int, *, count: Tensor | None = None, page: int = 32) -> Tensor:
     """Slots (B, n) int32 of tokens start[b], start[b] + 1, ...: page number * page + place in the page; -1
-    behind the first ``count[b]`` (default n) of them and where the table (B, M) has no page."""
+    behind the first ``count[b]`` (default n) of them and where the table (B, M) has no page; 2^31 - 1, behind every cache,
+    for a page number that no slot holds."""
     dev = _lib.require_cuda(table)
     if table.dim() != 2:
         raise ValueError("table must be (B, M)")

@@ -508,7 +508,7 @@ size_t hclsm_pages_resize_workspace_size(int32_t B, int32_t M);
 int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P, int32_t page,
                        const int32_t* old_lens, const int32_t* new_lens, void* ws, size_t ws_bytes, void* stream);
 /* slots (B, n): of tokens start[b], start[b] + 1, ...; -1 behind the first count[b] (NULL: n) of them and where the
- * table has no page. */
+ * table has no page; 2^31 - 1 for a page number that no slot holds. */
 int hclsm_page_slots(const int32_t* table, int32_t B, int32_t M, int32_t page, const int32_t* start,
                      const int32_t* count, int32_t n, int32_t* slots, void* stream);
 

@@ -592,6 +592,20 @@ def test_page_slots(n):
 
 
 # ---- together ------------------------------------------------------------------------------------
+def test_page_slots_of_a_page_number_that_no_slot_holds():
+    """Shifted it would be some other page's slot; so it names none, and the write that is given it sets the error word."""
+    table = torch.tensor([[1, (1 << 26) + 1, (1 << 26) - 1, -1]], dtype=torch.int32, device="cuda")
+    slots = page_slots(table, torch.tensor([31], device="cuda"), 66, page=32)
+    want = [63] + [2 ** 31 - 1] * 32 + list(range(2 ** 31 - 32, 2 ** 31)) + [-1]
+    assert slots.tolist() == [want]
+    assert page_slots(table, torch.tensor([0], device="cuda"), 4, page=1).tolist() == [[1, (1 << 26) + 1, (1 << 26) - 1, -1]]
+    cache = Kv4Cache.empty(4, 1, 32, page=32)
+    before = cache.k.clone()
+    kv = torch.randn(1, 32, 1, 32, device="cuda", dtype=BF)
+    kv4_write(cache, kv, kv, slots[:, 1:33])
+    assert hclsm_b200.device_error() != 0 and torch.equal(cache.k, before)
+
+
 def test_rollout_with_pages_cache_and_state_as_a_graph():
     """A rollout step (pages, slots, write, attention, decaying state) captured once and replayed as histories grow gives what
     eager calls give, and the values of a plain attention over what was written."""
