@@ -302,7 +302,8 @@ extern "C" int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t*
                                   int32_t page, const int32_t* old_lens, const int32_t* new_lens, void* ws,
                                   size_t ws_bytes, void* stream) {
   if (B < 0 || M < 0 || P < 0 || !pages::power_of_2(page)) return HCLSM_ERR_SHAPE;
-  if ((int64_t)P * page > 0x7fffffff || (int64_t)B * M > 0x7fffffff) return HCLSM_ERR_SHAPE;
+  // the kernels' indices go past the last page by their stride, at most 2^18
+  if ((int64_t)P * page > 0x7fffffff || (int64_t)B * M > 0x7fffffff - (1 << 18)) return HCLSM_ERR_SHAPE;
   if (B == 0) return HCLSM_OK;
   if ((!table && M) || (!stack && P) || !n_free || !old_lens || !new_lens) return HCLSM_ERR_NULL;
   const size_t need = hclsm_pages_resize_workspace_size(B, M);
