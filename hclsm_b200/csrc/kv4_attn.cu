@@ -21,6 +21,7 @@
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
+#include "tcgen05.cuh"
 
 namespace hclsm {
 namespace kv4 {
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t bars[kWarps * ST];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_w[kWarps][kRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, c = lane & 3;
   if (lane == 0)
     for (int i = 0; i < ST; ++i) mbar_init(&bars[warp * ST + i], 1);
   fence_mbar_init();
@@ -125,37 +126,42 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   const int units = (n + kUnit - 1) / kUnit;
   const int u_lo = (int)((int64_t)units * sp / p.splits), u_hi = (int)((int64_t)units * (sp + 1) / p.splits);
 
-  // ---- copies: lane 4 h + kind asks for the kind (codes or scales of keys or values) of page h of a unit (two pages
-  // where they have 16 tokens)
+  // ---- copies: one elected lane asks for the codes and scales of a unit (of two pages where they have 16 tokens) ----
   unsigned char* ring = smem + warp * ST * Sh::kStage;
   uint64_t* bar = bars + warp * ST;
   const int32_t* table = p.table + b * p.M;
   const bool small = p.c.page == 16;
-  const int kind = lane & 3, half = lane >> 2 & 1;
-  const int per_token = kind < 2 ? D / 2 : D / 16, tokens = small ? 16 : kUnit;
-  const char* source = reinterpret_cast<const char*>(kind < 2 ? (const void*)p.c.q[kind] : (const void*)p.c.scale[kind & 1]) +
-                       (int64_t)hk * p.c.page * per_token;
-  const int64_t page_step = (int64_t)p.c.Hkv * p.c.page * per_token;
-  const uint32_t to0 = (kind & 1 ? (kind < 2 ? Sh::kCodes : Sh::kScales) : 0) + (kind < 2 ? 0 : 2 * Sh::kCodes) +
-                       half * tokens * per_token;
+  const int half = lane >> 2 & 1;
   uint32_t holes = 0;  // two bits a stage: halves of a unit that are not there
   // this lane's page of unit u
   auto page_of = [&](int u) {
     const int at = (u * kUnit >> p.c.log_page) + (small ? half : 0);
     return u < u_hi && u * kUnit + (small ? half * 16 : 0) < n ? table[at] : -1;
   };
+  auto ask = [&](int s, int64_t token, auto tokens, int to) {  // from the page's token on, to the stage's
+    unsigned char* dst = ring + s * Sh::kStage;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      bulk_g2s(dst + kv * Sh::kCodes + to * (D / 2), p.c.q[kv] + token * (D / 2), tokens * (D / 2), &bar[s]);
+      bulk_g2s(dst + 2 * Sh::kCodes + kv * Sh::kScales + to * (D / 16),
+               reinterpret_cast<const unsigned char*>(p.c.scale[kv]) + token * (D / 16), tokens * (D / 16), &bar[s]);
+    }
+  };
   auto fetch = [&](int u, int s, int id) {
     if (u >= u_hi) return;
-    const uint32_t there = __ballot_sync(0xffffffffu, (unsigned)id < (unsigned)p.c.pages);
-    const uint32_t hole = (there & 1u ? 0u : 1u) | (there & 16u ? 0u : 2u);
-    if (hole && lane == 0 && ((hole & 1u) || (small && u * kUnit + 16 < n))) record_error(p.err, HCLSM_ERR_SHAPE);
-    holes = (holes & ~(3u << 2 * s)) | hole << 2 * s;
-    if (lane == 0)
-      mbar_expect_tx(&bar[s], small ? (2u - (hole & 1u) - (hole >> 1)) * (Sh::kStage / 2) : hole & 1u ? 0u : Sh::kStage);
-    __syncwarp();
-    if (lane < (small ? 8 : 4) && (there >> lane & 1u))
-      bulk_g2s(ring + s * Sh::kStage + to0,
-               source + id * page_step + (small ? 0 : (u * kUnit & (p.c.page - 1)) * per_token), tokens * per_token, &bar[s]);
+    const int id0 = __shfl_sync(0xffffffffu, id, 0), id1 = small ? __shfl_sync(0xffffffffu, id, 4) : id0;
+    const bool hole0 = (unsigned)id0 >= (unsigned)p.c.pages, hole1 = (unsigned)id1 >= (unsigned)p.c.pages;
+    if ((hole0 || (hole1 && u * kUnit + 16 < n)) && lane == 0) record_error(p.err, HCLSM_ERR_SHAPE);
+    holes = (holes & ~(3u << 2 * s)) | ((hole0 ? 1u : 0u) | (hole1 ? 2u : 0u)) << 2 * s;
+    if (!tc::elect_one()) return;
+    if (!small) {
+      mbar_expect_tx(&bar[s], hole0 ? 0u : Sh::kStage);
+      if (!hole0) ask(s, ((int64_t)id0 * p.c.Hkv + hk) * p.c.page + (u * kUnit & (p.c.page - 1)), kUnit, 0);
+    } else {
+      mbar_expect_tx(&bar[s], (hole0 ? 0u : Sh::kStage / 2) + (hole1 ? 0u : Sh::kStage / 2));
+      if (!hole0) ask(s, ((int64_t)id0 * p.c.Hkv + hk) * 16, 16, 0);
+      if (!hole1) ask(s, ((int64_t)id1 * p.c.Hkv + hk) * 16, 16, 16);
+    }
   };
   const int u0 = u_lo + warp;
 #pragma unroll 1
