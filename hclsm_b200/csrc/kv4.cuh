@@ -33,6 +33,7 @@ struct Attn {
   int B, M, Lq, H;
   int splits, rtiles;
   int cluster;        // the splits of a row are one cluster, whose blocks join them
+  int longest_first;  // entries in the order of their lengths
   float* part_o;      // (B * Hkv * rtiles, splits, 16, D)
   float2* part_ml;    // (B * Hkv * rtiles, splits, 16): max, sum
   float c2;           // scale * log2 e

@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   constexpr int G = Sh::kG, NQ = Sh::kNQ, ST = Sh::kStages, kRows = Sh::kRows;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t bars[kWarps * ST];
+  __shared__ int s_len[kThreads], s_entry;
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_w[kWarps][kRows];
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), g = lane >> 2, c = lane & 3;
   if (lane == 0)
@@ -120,9 +121,19 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   pdl_wait();
   pdl_trigger();
   const int sp = (int)(blockIdx.x % p.splits), rt = (int)(blockIdx.x / p.splits % p.rtiles);
-  const int64_t bh = blockIdx.x / p.splits / p.rtiles, b = bh / p.c.Hkv;
+  int64_t bh = blockIdx.x / p.splits / p.rtiles, b = bh / p.c.Hkv;
   const int hk = (int)(bh - b * p.c.Hkv), Gq = p.H / p.c.Hkv, rows = p.Lq * Gq;
-  const int n = p.lens ? min(max(p.lens[b], 0), p.M << p.c.log_page) : p.M << p.c.log_page;
+  const int most = p.M << p.c.log_page;
+  if (p.longest_first) {  // the entry that has b longer ones before it
+    int len = 0, before = 0;
+    if (threadIdx.x < p.B) s_len[threadIdx.x] = len = min(max(p.lens[threadIdx.x], 0), most);
+    __syncthreads();
+    for (int i = 0; i < p.B; ++i) before += s_len[i] > len || (s_len[i] == len && i < threadIdx.x);
+    if (threadIdx.x < p.B && before == b) s_entry = threadIdx.x;
+    __syncthreads();
+    b = __shfl_sync(0xffffffffu, s_entry, 0), bh = b * p.c.Hkv + hk;
+  }
+  const int n = p.lens ? min(max(p.lens[b], 0), most) : most;
   const int units = (n + kUnit - 1) / kUnit;
   const int u_lo = (int)((int64_t)units * sp / p.splits), u_hi = (int)((int64_t)units * (sp + 1) / p.splits);
 
@@ -535,6 +546,8 @@ void plan(Attn& p, int dtype) {
   if (s <= 16) s = s < 8 ? s : 8;
   p.splits = s < 1 ? 1 : (int)s;
   p.cluster = p.splits > 1 && p.splits <= 8;
+  // Blocks of unequal lengths in several waves: the long ones first, so that the last to run are short.
+  p.longest_first = p.lens && p.B > 1 && p.B <= kThreads && base * p.splits > (int64_t)num_sms() * per_sm;
 }
 
 size_t attn_workspace(const Attn& a, int dtype) {
