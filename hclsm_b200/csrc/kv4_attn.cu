@@ -240,6 +240,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   const int key = g & 1 ? (g >> 1) + 2 : (g >> 1) + 2 * (g >> 1 & 2);
   const int tok0 = c + 2 * (c & 2), tok1 = c + 2;
   float *ks = reinterpret_cast<float*>(smem + (Sh::kBytes - Sh::kWide)) + warp * 2 * kUnit * G, *vs = ks + kUnit * G;
+  // a maximum stays while no score is 2^8 above it in its power: nothing overflows, and no lane asks the others each step
+  const float slack = fminf(8.0f / p.c2, 3.0e38f);
   uint32_t k128 = 0x43004300u;
   asm volatile("" : "+r"(k128));
   int s = 0;
@@ -340,15 +342,14 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
     for (int r = 0; r < RT; ++r) {
       float top[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e)
         top[e] = fmaxf(fmaxf(sc[0][r][e], sc[0][r][e + 2]), fmaxf(sc[1][r][e], sc[1][r][e + 2]));
-#pragma unroll
-        for (int x = 4; x <= 16; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[r][0] || top[1] > m[r][1])) {
+      if (__any_sync(0xffffffffu, top[0] > m[r][0] + slack || top[1] > m[r][1] + slack)) {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x <= 16; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
           const float was = m[r][e];
           m[r][e] = fmaxf(was, top[e]);
           f[e] = was == m[r][e] ? 1.0f : ex2((was - m[r][e]) * p.c2);
