@@ -2,7 +2,7 @@
 //
 // The rows that share a key head (tokens x query heads of the group) are the N = 8 side of mma.sync m16n8k16
 // products, so that few rows waste nothing; a warp takes 32 tokens a step and keeps its own running maximum, sum and
-// output.  Each warp has a ring of stages of its own, filled by bulk copies that four of its lanes ask for (a page of
+// output.  Each warp has a ring of stages of its own, filled by bulk copies that one elected lane asks for (a page of
 // one head is contiguous): no barrier between warps until the merge.
 //
 // A contraction's index can run in any order, so the products take the codes as they lie: two words' halves of the same
@@ -14,10 +14,13 @@
 //   is rounded once.  movmatrix turns the scores' fragments into P^T's.  The 136 comes off the operand (summed over a
 //   history it would drown the values).
 // fp32 states: queries and weights as three bf16 pieces, whose products with exact codes are summed in fp32.
-// The bound is issue, above all the integer pipe that unpacks the codes (63 %; issue slots 65 %, tensor pipe 19 %, 16 warps an
-// SM): one query over 16 x 65536 ragged tokens, 32 heads over 8 of 128, 268 us, 3.4 TB/s.  From 450: the rows as N = 8
+// The bound is issue, above all the integer pipe that unpacks the codes (60 %; issue slots 69 %, tensor pipe 23 %, 16 warps an
+// SM): one query over 16 x 65536 ragged tokens, 32 heads over 8 of 128, 224 us, 4.0 TB/s.  From 450: the rows as N = 8
 // instead of M = 16 (323), one operation a pair of codes (284), scales widened to fp32 once a step and four blocks an SM of
-// two stages (268).  Not kept: shifts as the upper half of products (317), 1, 2, 3 or 6 waves of blocks (383, 318, 313, 277).
+// two stages (268), one elected lane for the copies and a uniform warp index, whose addresses then cost no vector
+// instructions (232), long histories first (226), a maximum that may lag behind (224).  Not kept: shifts as the upper half of
+// products (317), queries and codes as e4m3 (318; its products convert them), codes as tiny bf16 numbers, which need no shift
+// but a sum of their own to take off the 8 (244), 2, 3, 5, 6 or 8 waves of blocks (237, 238, 230, 238, 250).
 #include <cooperative_groups.h>
 
 #include "kv4.cuh"
@@ -300,7 +303,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
         for (int step = 0; step < 2; ++step) {
           const int i = 8 * step;
           if constexpr (Sh::kF32) {
-            const uint32_t a[4] = {centred(x0 >> i, k128), centred(x1 >> i, k128), centred(x0 >> (i + 4), k128), centred(x1 >> (i + 4), k128)};
+            const uint32_t a[4] = {centred(x0 >> i, k128), centred(x1 >> i, k128), centred(x0 >> (i + 4), k128),
+                                   centred(x1 >> (i + 4), k128)};
 #pragma unroll
             for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -310,7 +314,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
                 else mma(d[r], a, w.x, w.y);
               }
           } else {
-            const uint32_t a[4] = {biased(x0 >> i, k128), biased(x1 >> i, k128), biased(x0 >> (i + 4), k128), biased(x1 >> (i + 4), k128)};
+            const uint32_t a[4] = {biased(x0 >> i, k128), biased(x1 >> i, k128), biased(x0 >> (i + 4), k128),
+                                   biased(x1 >> (i + 4), k128)};
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               if (step == 0)
