@@ -452,7 +452,8 @@ def _attention_ref(q, k, v, lens, scale):
     (1, 32, 1, 1, 1, 64, 32), (3, 256, 1, 6, 6, 64, 32), (2, 160, 1, 8, 2, 128, 16), (2, 192, 3, 5, 1, 96, 64),
     (2, 4096, 1, 4, 1, 64, 16), (2, 2560, 32, 6, 3, 32, 128), (1, 8192, 7, 8, 2, 128, 32), (5, 384, 1, 10, 2, 32, 32),
     (2, 1024, 17, 12, 12, 96, 16),
-    (128, 96, 1, 16, 8, 32, 32), (129, 64, 1, 8, 8, 64, 16)])  # several waves of blocks, equal lengths among them
+    (128, 96, 1, 16, 8, 32, 32), (129, 64, 1, 8, 8, 64, 16),  # several waves of blocks, equal lengths among them
+    *((2, 128, Lq, 9, 3, D, 32) for D in (32, 64, 96, 128) for Lq in (1, 3))])  # each kernel: up to 8 rows, and more
 def test_kv4_attention(B, T, Lq, H, Hkv, D, page, dtype):
     cache, table = _pool(B, T, Hkv, D, page, dtype)
     lens = torch.randint(0, T + 1, (B,), device="cuda", dtype=torch.int32)
