@@ -371,17 +371,16 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
           const uint32_t on = first <= last && first < 32 ? (0xffffffffu >> (31 - (last - first))) << first : 0u;
           if (past || l2 > -4.0f) {
             // g^|i-j| as the power of i's distance to the block's end on the later side times that of j's; on the
-            // diagonal the first is up to g^-31, which fp32 holds above 2^-4
+            // diagonal the first is up to g^-31, which fp32 holds above 2^-4: so the score comes last
             const float a = ex2(l2 * (float)(p.rev ? j0 - row : row - j0 - 31));
             tmem_wait_ld();
             tmem_pin<32>(v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float4 t = *reinterpret_cast<const float4*>(s_pow + e * 4);
-              float2 lo = mul2(make_float2(v[4 * e], v[4 * e + 1]), make_float2(a, a)),
-                     hi = mul2(make_float2(v[4 * e + 2], v[4 * e + 3]), make_float2(a, a));
-              lo = mul2(lo, make_float2(t.x, t.y));
-              hi = mul2(hi, make_float2(t.z, t.w));
+              float2 lo = mul2(make_float2(t.x, t.y), make_float2(a, a)), hi = mul2(make_float2(t.z, t.w), make_float2(a, a));
+              lo = mul2(lo, make_float2(v[4 * e], v[4 * e + 1]));
+              hi = mul2(hi, make_float2(v[4 * e + 2], v[4 * e + 3]));
               v[4 * e] = lo.x, v[4 * e + 1] = lo.y, v[4 * e + 2] = hi.x, v[4 * e + 3] = hi.y;
             }
           } else {

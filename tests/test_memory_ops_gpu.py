@@ -150,6 +150,19 @@ def test_decay_attention_strides_and_streams(dtype):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("L", [1, 70, 300])
+def test_decay_attention_fast_decays_and_large_scores(L, dtype):
+    """A token's weight is no larger than its score, whatever powers of the decay it is formed from."""
+    x = _inputs(2, L, 6, 128, 128, dtype, True)
+    for n in ("q", "k", "v", "do"):
+        x[n] *= 64
+    g = torch.tensor([-2.6, -2.7, -2.75, -2.77, -2.78, -20.0], device="cuda")
+    _check_decay(x, g, None, dtype, 128 ** -0.5)
+    x["S0"] = x["dS"] = None
+    _check_decay(x, g, torch.tensor([L, L // 2], device="cuda", dtype=torch.int32), dtype, 128 ** -0.5)
+
+
 def test_decay_attention_is_linear_in_each_argument():
     """Differences: o and the state are linear in v, so <do, o(v = u)> + <dS, S(v = u)> is the gradient in v times u, exactly but
     for rounding; likewise k and the state, and o in q."""
