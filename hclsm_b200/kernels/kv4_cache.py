@@ -9,7 +9,7 @@ with others.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 from torch import Tensor
@@ -30,50 +30,36 @@ class Kv4Cache:
     k_scale: Tensor
     v_scale: Tensor
     dtype: torch.dtype = torch.bfloat16
-    # (addresses, what _args returns) of the tensors as last checked, or None
-    _packed: tuple | None = field(init=False, repr=False, compare=False)
 
     def __init__(self, k, v, k_scale, v_scale, dtype=torch.bfloat16):
-        d = self.__dict__  # past __setattr__: a microsecond less
-        d["k"], d["v"], d["k_scale"], d["v_scale"], d["dtype"], d["_packed"] = k, v, k_scale, v_scale, dtype, None
+        self.k, self.v, self.k_scale, self.v_scale, self.dtype = k, v, k_scale, v_scale, dtype
         self._args()
 
-    def __setattr__(self, name, value):
-        self.__dict__[name] = value
-        self.__dict__["_packed"] = None  # another tensor: checked and packed at the next call
-
-    def __getstate__(self):
-        return {**self.__dict__, "_packed": None}  # a copy's tensors are elsewhere
-
     def _args(self):
-        """(hclsm_kv4_cache, Hkv, D, device, its index) for a call.  A tensor that was assigned, copied or given other
-        memory since the last call is checked and its address taken anew: a kernel only ever sees the memory of
-        the present tensors."""
-        at = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr())
-        packed = self._packed
-        if packed is None or packed[0] != at:
-            packed = self.__dict__["_packed"] = (at, self._check(at))
-        return packed[1]
-
-    def _check(self, at):
+        """(hclsm_kv4_cache, Hkv, page, D, device, its index) for a call, from the tensors as they are now: nothing is kept,
+        since a tensor that is changed in place (resize_, transpose_, its data) may stay at its address."""
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
-        dev = _lib.require_cuda(k, v, ks, vs)
-        if k.dim() != 4:
+        dev, index = _lib.require_cuda(k), k.get_device()
+        if v.get_device() != index or ks.get_device() != index or vs.get_device() != index:
+            _lib.require_cuda(k, v, ks, vs)
+        whole = k.shape
+        if len(whole) != 4:
             raise ValueError("k must be (pages, Hkv, page, D / 2)")
-        P, Hkv, page, half = k.shape
+        P, Hkv, page, half = whole
         D = 2 * half
         if page not in (16, 32, 64, 128) or D not in (32, 64, 96, 128) or Hkv < 1:
             raise ValueError(f"page must be 16, 32, 64 or 128 and head_dim 32, 64, 96 or 128, got {page} and {D}")
         if P * page >= 1 << 31:
             raise ValueError(f"{P} pages of {page} tokens pass 31 bits")
         shape = (P, Hkv, page, D // 32)
-        if (v.shape != k.shape or k.dtype != torch.uint8 or v.dtype != torch.uint8 or not k.is_contiguous()
+        if (v.shape != whole or k.dtype != torch.uint8 or v.dtype != torch.uint8 or not k.is_contiguous()
                 or not v.is_contiguous()):
-            raise ValueError(f"k and v must be contiguous {tuple(k.shape)} uint8")
+            raise ValueError(f"k and v must be contiguous {tuple(whole)} uint8")
         if (ks.shape != shape or vs.shape != shape or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16
                 or not ks.is_contiguous() or not vs.is_contiguous()):
             raise ValueError(f"k_scale and v_scale must be contiguous {shape} bfloat16")
-        return _lib.KV4_CACHE.pack(*at, P, Hkv, page, D, _lib.dtype_code(self.dtype)), Hkv, D, dev, k.get_device()
+        return (_lib.KV4_CACHE.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), P, Hkv, page, D,
+                                    _lib.dtype_code(self.dtype)), Hkv, page, D, dev, index)
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, head_dim: int, *, page: int = 32, dtype=torch.bfloat16,
@@ -110,7 +96,7 @@ def kv4_write(cache: Kv4Cache, k: Tensor, v: Tensor, slots: Tensor) -> None:
     sets the device error word.  The slots of one call must differ: of tokens that share one, what is kept is
     undefined.  No gradients: k and v that require them are refused."""
     _no_derivatives("kv4_write", cache, k, v)
-    c, Hkv, D, dev, index = cache._args()
+    c, Hkv, _, D, dev, index = cache._args()
     if k.get_device() != index or v.get_device() != index:
         raise ValueError(f"k and v must be on {dev}, got {k.device} and {v.device}")
     if k.dim() != 4 or v.shape != k.shape or k.shape[2:] != (Hkv, D):
@@ -131,11 +117,11 @@ def kv4_read(cache: Kv4Cache, table: Tensor, lens: Tensor | None = None):
     (default all; clamped to [0, T]) of the pages that table (B, T / page) names, as the values they stand for,
     zeros after them.  A page outside the cache below the length reads as zeros and sets the device error word."""
     _no_derivatives("kv4_read", cache)
-    c, Hkv, D, dev, _ = cache._args()
+    c, Hkv, page, D, dev, _ = cache._args()
     table = _table(table, dev)
     B, M = table.shape
     lens = _lib.index32(lens, (B,), "lens", dev)
-    k, v = (torch.empty(B, M * cache.page, Hkv, D, dtype=cache.dtype, device=dev) for _ in range(2))
+    k, v = (torch.empty(B, M * page, Hkv, D, dtype=cache.dtype, device=dev) for _ in range(2))
     _lib.check(_lib.load().hclsm_kv4_read(c, table.data_ptr(), B, M, k.data_ptr(), v.data_ptr(), _lib.ptr(lens),
                                           _lib.stream_ptr(dev)), "hclsm_kv4_read")
     return k, v
@@ -147,7 +133,7 @@ def kv4_attention(q: Tensor, cache: Kv4Cache, table: Tensor, lens: Tensor | None
     clamped to the table's) of the pages that table (B, M) names; H is a multiple of Hkv.  An entry without tokens
     gives zeros; tokens of a page outside the cache do not count and set the device error word.  No gradients."""
     _no_derivatives("kv4_attention", cache, q)
-    c, Hkv, D, dev, index = cache._args()
+    c, Hkv, _, D, dev, index = cache._args()
     if q.get_device() != index:
         raise ValueError(f"q must be on {dev}, got {q.device}")
     table = _table(table, dev)

@@ -1,0 +1,64 @@
+"""The operators that remember a history, on the CPU: calls and tables at the edges of what they are documented to take."""
+import pytest
+import torch
+
+from hclsm_b200 import _lib
+from hclsm_b200.kernels import Kv4Cache, kv4_attention, kv4_read, kv4_write
+
+BF, I32 = torch.bfloat16, torch.int32
+
+
+class _Library:
+    """Records each call's arguments; workspace queries give 0."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+
+        return call
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    rec = _Library()
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cpu"))
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda dev: 0)
+    return rec
+
+
+def test_kv4_tensors_that_were_changed_where_they_are(lib):
+    """A tensor changed in place may keep its address: the call takes its present shape, or refuses it."""
+    c = Kv4Cache.empty(4, 1, 32, page=32, device="cpu")
+    at = c.k.data_ptr()
+    for t in (c.k, c.v):
+        t.resize_(8, 1, 16, 16)
+    table, x, slots = torch.zeros(1, 3, dtype=I32), torch.zeros(1, 2, 1, 32, dtype=BF), torch.zeros(1, 2, dtype=I32)
+    calls = (lambda: kv4_read(c, table), lambda: kv4_write(c, x, x, slots), lambda: kv4_attention(x, c, table))
+    for call in calls:  # the scales are those of pages of 32
+        with pytest.raises(ValueError):
+            call()
+    for t in (c.k_scale, c.v_scale):
+        t.resize_(8, 1, 16, 1)
+    assert c.k.data_ptr() == at
+    for call in calls:
+        lib.calls.clear()
+        call()
+        assert _lib.KV4_CACHE.unpack(lib.calls[-1][1][0])[4:8] == (8, 1, 16, 32)
+    assert calls[0]()[0].shape == (1, 48, 1, 32)
+    c.k.transpose_(0, 2), c.v.transpose_(0, 2)  # 16 pages of 8 tokens
+    d = Kv4Cache.empty(32, 1, 32, page=32, device="cpu")
+    d.k.transpose_(0, 2)  # the same shape, in another order
+    e = Kv4Cache.empty(4, 1, 32, page=32, device="cpu")
+    e.k_scale.data = e.k_scale.data.view(torch.float16)
+    lib.calls.clear()
+    for cache in (c, d, e):
+        for call in (lambda: kv4_read(cache, table), lambda: kv4_write(cache, x, x, slots),
+                     lambda: kv4_attention(x, cache, table)):
+            with pytest.raises(ValueError):
+                call()
+    assert not lib.calls
