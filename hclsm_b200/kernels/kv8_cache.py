@@ -11,7 +11,7 @@ replayed with other positions.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 from torch import Tensor
@@ -33,55 +33,41 @@ class Kv8Cache:
     v_scale: Tensor
     k_tail: Tensor
     v_tail: Tensor
-    # (addresses, what _args returns) of the tensors as last checked, or None
-    _packed: tuple | None = field(init=False, repr=False, compare=False)
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
-        d = self.__dict__  # past __setattr__: a microsecond less
-        d["k"], d["v"], d["k_scale"], d["v_scale"], d["k_tail"], d["v_tail"] = k, v, k_scale, v_scale, k_tail, v_tail
-        d["_packed"] = None
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
         self._args()
 
-    def __setattr__(self, name, value):
-        self.__dict__[name] = value
-        self.__dict__["_packed"] = None  # another tensor: checked and packed at the next call
-
-    def __getstate__(self):
-        return {**self.__dict__, "_packed": None}  # a copy's tensors are elsewhere
-
     def _args(self):
-        """(hclsm_kv8_cache, (B, Hkv, T, D), dtype, device, its index) for a call.  A tensor that was assigned,
-        copied or given other memory since the last call is checked and its address taken anew: a kernel only ever
-        sees the memory of the present tensors."""
-        at = (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-              self.k_tail.data_ptr(), self.v_tail.data_ptr())
-        packed = self._packed
-        if packed is None or packed[0] != at:
-            packed = self.__dict__["_packed"] = (at, self._check(at))
-        return packed[1]
-
-    def _check(self, at):
-        k, v, ks, vs, kt, vt = tensors = self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail
+        """(hclsm_kv8_cache, (B, Hkv, T, D), dtype, device, its index) for a call, from the tensors as they are now: nothing
+        is kept, since a tensor that is changed in place (resize_, transpose_, its data) may stay at its address."""
+        k, v, ks, vs, kt, vt = self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail
         dev, index = _lib.require_cuda(k), k.get_device()
-        for t in tensors:
-            if t.get_device() != index:
-                _lib.require_cuda(*tensors)
-        if k.dim() != 4 or kt.dim() != 4:
+        if (v.get_device() != index or ks.get_device() != index or vs.get_device() != index or kt.get_device() != index
+                or vt.get_device() != index):
+            _lib.require_cuda(k, v, ks, vs, kt, vt)
+        whole, tail, dtype = k.shape, kt.shape, kt.dtype
+        if len(whole) != 4 or len(tail) != 4:
             raise ValueError("k must be (B, Hkv, T, D), k_tail (B, Hkv, block, D)")
-        B, Hkv, T, D = k.shape
-        block, dtype = kt.shape[2], kt.dtype
+        B, Hkv, T, D = whole
+        block = tail[2]
         if block not in (16, 32, 64, 128) or T % block:
             raise ValueError(f"block must be 16, 32, 64 or 128 and divide the capacity {T}, got {block}")
         if D not in (32, 64, 96, 128):
             raise ValueError(f"head_dim must be 32, 64, 96 or 128, got {D}")
-        for one, two, shape, dt, name in ((k, v, (B, Hkv, T, D), torch.int8, ""),
-                                          (ks, vs, (B, Hkv, T // block), torch.float32, "_scale"),
-                                          (kt, vt, (B, Hkv, block, D), dtype, "_tail")):
-            if (one.shape != shape or two.shape != shape or one.dtype != dt or two.dtype != dt
-                    or not one.is_contiguous() or not two.is_contiguous()):
-                raise ValueError(f"k{name} and v{name} must be contiguous {shape} {dt}, got {tuple(one.shape)} "
-                                 f"{one.dtype} and {tuple(two.shape)} {two.dtype}")
-        return _lib.KV8_CACHE.pack(*at, B, Hkv, T, D, block, _lib.dtype_code(dtype)), (B, Hkv, T, D), dtype, dev, index
+        if (v.shape != whole or k.dtype != torch.int8 or v.dtype != torch.int8 or not k.is_contiguous()
+                or not v.is_contiguous()):
+            raise ValueError(f"k and v must be contiguous {tuple(whole)} int8")
+        shape = (B, Hkv, T // block)
+        if (ks.shape != shape or vs.shape != shape or ks.dtype != torch.float32 or vs.dtype != torch.float32
+                or not ks.is_contiguous() or not vs.is_contiguous()):
+            raise ValueError(f"k_scale and v_scale must be contiguous {shape} float32")
+        shape = (B, Hkv, block, D)
+        if (tail != shape or vt.shape != shape or vt.dtype != dtype or not kt.is_contiguous()
+                or not vt.is_contiguous()):
+            raise ValueError(f"k_tail and v_tail must be contiguous {shape} of one dtype")
+        return (_lib.KV8_CACHE.pack(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(), vt.data_ptr(), B,
+                                    Hkv, T, D, block, _lib.dtype_code(dtype)), (B, Hkv, T, D), dtype, dev, index)
 
     @classmethod
     def empty(cls, batch: int, capacity: int, kv_heads: int, head_dim: int, *, block: int = 32, dtype=torch.bfloat16,

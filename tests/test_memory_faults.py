@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from hclsm_b200 import _lib
-from hclsm_b200.kernels import Kv4Cache, kv4_attention, kv4_read, kv4_write
+from hclsm_b200.kernels import (Kv4Cache, Kv8Cache, kv4_attention, kv4_read, kv4_write, kv8_attention, kv8_read,
+                                kv8_write)
 
 BF, I32 = torch.bfloat16, torch.int32
 
@@ -62,3 +63,31 @@ def test_kv4_tensors_that_were_changed_where_they_are(lib):
             with pytest.raises(ValueError):
                 call()
     assert not lib.calls
+
+
+def test_kv8_tensors_that_were_changed_where_they_are(lib):
+    c = Kv8Cache.empty(2, 64, 2, 32, device="cpu")
+    at = c.k.data_ptr()
+    c.k.resize_(2, 1, 64, 32), c.v.resize_(2, 1, 64, 32)
+    x, start = torch.zeros(2, 3, 1, 32, dtype=BF), torch.zeros(2, dtype=I32)
+    calls = (lambda: kv8_read(c, start), lambda: kv8_write(c, x, x, start), lambda: kv8_attention(x, c, start))
+    for call in calls:  # the scales and tails are those of two heads
+        with pytest.raises(ValueError):
+            call()
+    c.k_scale.resize_(2, 1, 2), c.v_scale.resize_(2, 1, 2)
+    c.k_tail.resize_(2, 1, 32, 32), c.v_tail.resize_(2, 1, 32, 32)
+    assert c.k.data_ptr() == at
+    for call in calls:
+        lib.calls.clear()
+        call()
+        assert _lib.KV8_CACHE.unpack(lib.calls[-1][1][0])[6:11] == (2, 1, 64, 32, 32)
+    assert calls[0]()[0].shape == (2, 64, 1, 32)
+    for name in ("k", "k_scale", "k_tail"):
+        d = Kv8Cache.empty(2, 64, 2, 32, device="cpu")
+        getattr(d, name).transpose_(0, 1)  # the same shape, in another order
+        lib.calls.clear()
+        y = torch.zeros(2, 3, 2, 32, dtype=BF)
+        for call in (lambda: kv8_read(d, start), lambda: kv8_write(d, y, y, start), lambda: kv8_attention(y, d, start)):
+            with pytest.raises(ValueError):
+                call()
+        assert not lib.calls
