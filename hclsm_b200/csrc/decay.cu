@@ -72,8 +72,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
   const float2 whole = chunk_decay(p.log_decay, h, kC);
-  const int c_lo = seg * p.seg_chunks, c_end = min(c_lo + p.seg_chunks, (p.L + kC - 1) / kC);
-  const int c_hi = min(c_end, (n + kC - 1) / kC);  // chunks with valid tokens
+  const int c_lo = seg * p.seg_chunks, c_end = min(c_lo + p.seg_chunks, chunks_of(p.L, kC));
+  const int c_hi = min(c_end, chunks_of(n, kC));  // chunks with valid tokens
   const int64_t xb = b * p.x.sb + h * p.x.sh, kb = b * p.k.sb + h * p.k.sh, vb = b * p.v.sb + h * p.v.sh;
   T* y = static_cast<T*>(p.y) + (b * p.L * p.H + h) * (int64_t)p.Dv;
 
@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
         }
   }
   if (!SUMS)  // rows behind the length
-    for (int t = max(c_lo * kC, n) + ty; t < min(c_end * kC, p.L); t += 16)
-      for (int e = tx; e < min(kE, p.Dv - e0); e += 16) io<T>::st(y + (int64_t)t * p.H * p.Dv + e0 + e, 0.0f);
+    for (int64_t t = max(c_lo * kC, n) + (int64_t)ty, end = min((int64_t)c_end * kC, (int64_t)p.L); t < end; t += 16)
+      for (int e = tx; e < min(kE, p.Dv - e0); e += 16) io<T>::st(y + t * p.H * p.Dv + e0 + e, 0.0f);
 }
 
 // The segments' sums become their first states; the state behind the last one (in the pass's order) goes to `last`.
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Batch
     if (it > 0) ask(it);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int m = n - (first + step * (it + k)) * span;  // tokens from this segment on
+      const int64_t m = n - (int64_t)(first + step * (it + k)) * span;  // tokens from this segment on
       if (it + k < segs) at[(it + k) * by] = v;
       if (it + k < segs && m > 0) {  // not behind the length
         const float2 g = m >= span ? whole : cut_off;

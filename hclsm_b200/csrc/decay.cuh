@@ -60,6 +60,8 @@ __device__ __forceinline__ float2 chunk_decay(const float* log_decay, int h, int
   const float hi = (float)g;
   return make_float2(hi, (float)(g - (double)hi));
 }
+// Chunks of n tokens; n + chunk - 1 may pass 31 bits.
+__host__ __device__ __forceinline__ int chunks_of(int n, int chunk) { return n / chunk + (n % chunk != 0); }
 __device__ __forceinline__ int length(const Pass& p, int64_t b) {
   return p.lens ? min(max(p.lens[b], 0), p.L) : p.L;
 }
@@ -78,7 +80,7 @@ struct Batch {
 // 40 in six, 32 chunks 69 against 58 in six; 16 heads of 128, 8 chunks 27 against 38 in eight, 16 chunks 48 against 43;
 // 64 heads of 128, 128 chunks 348 against 377 in two.
 inline void cut(Batch& b, int chunk, float twice, float crowd, float fixed, float load, int64_t have, int64_t room) {
-  const int chunks = (b.p[0].L + chunk - 1) / chunk, sms = num_sms();
+  const int chunks = chunks_of(b.p[0].L, chunk), sms = num_sms();
   auto shared = [&](int64_t blocks) { return blocks > sms ? crowd : 1.0f; };
   int best = chunks > 1 ? chunks : 1;  // chunks of a segment
   float least = (float)chunks * shared(have);

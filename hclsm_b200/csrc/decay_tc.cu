@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const int c_lo = seg * p.seg_chunks, c_end = min(c_lo + p.seg_chunks, (p.L + kTok - 1) / kTok);
-  const int chunks = max(min(c_end, (n + kTok - 1) / kTok) - c_lo, 0);  // with valid tokens
+  const int c_lo = seg * p.seg_chunks, c_end = min(c_lo + p.seg_chunks, chunks_of(p.L, kTok));
+  const int chunks = max(min(c_end, chunks_of(n, kTok)) - c_lo, 0);  // with valid tokens
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, p.err); };
   // the whole warp goes on or gives up together
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
@@ -482,7 +482,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
     if (Sh::kStaged && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     // zeros behind the length
     const int e8 = p.Dv / 8, me = tid - WGT * 128;
-    for (int t = max(c_lo * kTok, n) + (me >> 3); t < min(c_end * kTok, p.L); t += WG * 16)
+    for (int64_t t = max(c_lo * kTok, n) + (int64_t)(me >> 3), end = min((int64_t)c_end * kTok, (int64_t)p.L); t < end;
+         t += WG * 16)
       for (int e = me & 7; e < e8; e += 8)
         *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.y) + ((b * p.L + t) * p.H + h) * (int64_t)p.Dv + e * 8) =
             make_uint4(0, 0, 0, 0);
@@ -560,8 +561,9 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
   const int h = (int)(bh - b * p.H);
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
-  const int lo = seg * p.seg_chunks * kTok, hi = min(min(lo + p.seg_chunks * kTok, p.L), n);
-  const int chunks = hi > lo ? (hi - lo + kTok - 1) / kTok : 0;
+  const int lo = seg * p.seg_chunks * kTok;
+  const int hi = (int)min((int64_t)lo + p.seg_chunks * kTok, (int64_t)n);  // the segment's end may lie past 31 bits
+  const int chunks = hi > lo ? chunks_of(hi - lo, kTok) : 0;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_or(bar, parity & 1, &s_abort, p.err); };
   auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
   int asked = 0, asked_k = 0;
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
       const float w = ex2(l2 * (float)(p.rev ? t - lo + 1 : hi - 1 - t));
 #pragma unroll 1
       for (int c = 0; c < kDims / 8; c += 4) weigh_row<NP, 4>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
-      if (lo + (it + 1) * kTok > hi) {
+      if (hi - lo - it * kTok < kTok) {
         if (!(ok = wait_all(&full[s], it / ST))) break;
         if (t >= hi) {
           clear_row(smem_u32(sP), Sh::kX, NP, row, c0, c0 + kDims / 8);

@@ -91,3 +91,21 @@ def test_kv8_tensors_that_were_changed_where_they_are(lib):
             with pytest.raises(ValueError):
                 call()
         assert not lib.calls
+
+
+# ---- lengths next to 2^31 -------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16])
+@pytest.mark.parametrize("D", [1, 8, 64, 128])
+def test_decay_plans_of_lengths_up_to_31_bits(dtype, D):
+    """A long history is cut into segments, the longest ones as those a little shorter: their parts' bytes are the same."""
+    lib, some = _lib.load(), 1 << 20  # an aligned address that no query looks at
+
+    def bytes_of(query, L, H=1):
+        view = (some, L * H * D, H * D, D)
+        return query(_lib.DECAY_ARGS.pack(*view * 4, *(some,) * 4, some, 0, 0, 0, 0, 0, 1, L, H, D, D, dtype, 1.0))
+
+    for query in (lib.hclsm_decay_attn_fwd_workspace_size, lib.hclsm_decay_attn_bwd_workspace_size):
+        want = bytes_of(query, (1 << 31) - 1000)
+        assert want > 0
+        for L in (1 << 31) - 200, (1 << 31) - 128, (1 << 31) - 127, (1 << 31) - 64, (1 << 31) - 63, (1 << 31) - 1:
+            assert bytes_of(query, L) == want, L

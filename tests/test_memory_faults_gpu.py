@@ -1,0 +1,65 @@
+"""The operators that remember a history on the GPU: calls at the edges of what they are documented to take, against plain
+definitions in 64 bits.  Tolerances count roundings as test_memory_ops_gpu.py does."""
+import pytest
+import torch
+
+import hclsm_b200
+from hclsm_b200.kernels import decay_attention
+from hclsm_b200.kernels.decay_attn import decay_bwd
+from memory_ref import decay_grads, decay_ref
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+HALF_STEP = {BF: 2.0 ** -8, F32: 2.0 ** -24}  # eps / 2
+
+
+@pytest.fixture(autouse=True)
+def no_device_error():
+    hclsm_b200.device_error()
+    yield
+    assert hclsm_b200.device_error() == 0
+
+
+def _near(got, want, tol, name):
+    assert got.shape == want.shape, name
+    over = ((got.double() - want).abs() - tol).max()
+    assert over <= 0, f"{name}: {float(over)} over its tolerance"
+    assert torch.isfinite(got).all(), name
+
+
+# ---- lengths next to 2^31 -------------------------------------------------------------------------
+def test_decay_attention_of_31_bits_of_tokens():
+    """One number a token, fp32: what the last tokens see is the sum over all before, and what is behind the length is zero.
+    Heads that forget: a token sees no more than some 60 others, in chunks of 64 by n = 400 terms' rounding."""
+    L, n, g = (1 << 31) - 1, 1000, torch.tensor([-0.7], device="cuda")
+    q, k, v = (torch.full((1, 1, 1, 1), x, device="cuda").expand(1, L, 1, 1) for x in (2.0, 0.5, 3.0))
+    tail = [t[:, :n] for t in (q, k, v)]
+    ro, rS = decay_ref(*tail, g, scale=0.25)
+    tol = 400 * 2.0 ** -24
+    lens = torch.tensor([L - 5], device="cuda")
+    o, S = decay_attention(q, k, v, g, scale=0.25, lens=lens, return_state=True)
+    _near(o[:, L - 305:L - 5], ro[:, -300:], tol * ro[:, -300:], "o")
+    assert (o[:, L - 5:] == 0).all()
+    _near(S, rS, tol * rS, "state")
+    del o
+    want = decay_grads(*tail, g, None, None, 0.25, tail[2], None)
+    got = decay_bwd(q, k, v, g, None, None, 0.25, v, None)
+    for a, w, name in zip(got, want, ("dq", "dk", "dv")):
+        _near(a[:, L - 300:], w[:, -300:], tol * w[:, -300:], name)
+        first = w[:, :300] if name == "dq" else w[:, 300:600]  # dq looks back, the others ahead
+        _near(a[:, :300], first, tol * first, name)
+
+
+def test_decay_attention_of_31_bits_of_tokens_on_the_tensor_cores():
+    """Rows of 16 bytes, bf16, all but the last zeros: the last chunks and the state behind them."""
+    L, n, g = (1 << 31) - 1, 5000, torch.tensor([-0.01], device="cuda")
+    x = torch.zeros(1, L, 1, 8, device="cuda", dtype=BF)
+    x[:, L - n:].normal_()
+    tail = x[:, L - n:].clone()
+    o, S = decay_attention(x, x, x, g, return_state=True)
+    ro, rS = decay_ref(tail, tail, tail, g, scale=8 ** -0.5)
+    ao, aS = decay_ref(*(tail.abs(),) * 3, g, scale=8 ** -0.5)
+    fp32 = (n + 2 * 8 + 256) * 2.0 ** -24
+    _near(o[:, L - n:], ro, 2.0 ** -8 * (ro.abs() + ao) + fp32 * ao, "o")
+    _near(S, rS, fp32 * aS, "state")
+    assert (o[:, :L - n] == 0).all()
