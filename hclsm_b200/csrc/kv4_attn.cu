@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
     b = __shfl_sync(0xffffffffu, s_entry, 0), bh = b * p.c.Hkv + hk;
   }
   const int n = p.lens ? min(max(p.lens[b], 0), most) : most;
-  const int units = (n + kUnit - 1) / kUnit;
+  const int units = n / kUnit + (n % kUnit != 0);  // n + kUnit - 1 may pass 31 bits
   const int u_lo = (int)((int64_t)units * sp / p.splits), u_hi = (int)((int64_t)units * (sp + 1) / p.splits);
 
   // ---- copies: one elected lane asks for the codes and scales of a unit (of two pages where they have 16 tokens) ----
@@ -149,8 +149,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, RT>::kPerSm) attn_kernel
   uint32_t holes = 0;  // two bits a stage: halves of a unit that are not there
   // this lane's page of unit u
   auto page_of = [&](int u) {
-    const int at = (u * kUnit >> p.c.log_page) + (small ? half : 0);
-    return u < u_hi && u * kUnit + (small ? half * 16 : 0) < n ? table[at] : -1;
+    return u < u_hi && u * kUnit + (small ? half * 16 : 0) < n ? table[(u * kUnit >> p.c.log_page) + (small ? half : 0)] : -1;
   };
   auto ask = [&](int s, int64_t token, auto tokens, int to) {  // from the page's token on, to the stage's
     unsigned char* dst = ring + s * Sh::kStage;

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import hclsm_b200
-from hclsm_b200.kernels import decay_attention
+from hclsm_b200.kernels import Kv4Cache, decay_attention, kv4_attention, kv4_write
 from hclsm_b200.kernels.decay_attn import decay_bwd
 from memory_ref import decay_grads, decay_ref
 
@@ -63,3 +63,24 @@ def test_decay_attention_of_31_bits_of_tokens_on_the_tensor_cores():
     _near(o[:, L - n:], ro, 2.0 ** -8 * (ro.abs() + ao) + fp32 * ao, "o")
     _near(S, rS, fp32 * aS, "state")
     assert (o[:, :L - n] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_kv4_attention_of_31_bits_of_tokens(dtype):
+    """Pages of 16 that repeat, 2^31 - 16 tokens: all scores are zero but those of the last page, whose tokens weigh as much as
+    all others.  The sums of these weights and values are exact in fp32; e^18.75 is off by 2^-20 of it."""
+    M = (1 << 27) - 1
+    cache = Kv4Cache.empty(2, 1, 32, page=16, dtype=dtype)
+    k, v = (torch.zeros(1, 32, 1, 32, device="cuda", dtype=dtype) for _ in range(2))
+    k[:, 16:, :, 0], v[:, :16], v[:, 16:] = 8.0, 1.0, 3.0  # held exactly
+    kv4_write(cache, k, v, torch.arange(32, device="cuda", dtype=torch.int32)[None])
+    table = torch.zeros(1, M, device="cuda", dtype=torch.int32)
+    table[0, -1] = 1
+    q = torch.zeros(1, 1, 1, 32, device="cuda", dtype=dtype)
+    q[..., 0] = 18.75 / 8
+    for lens in (None, torch.tensor([16 * M - 1], device="cuda")):
+        last = 16 if lens is None else 15
+        e = last * torch.tensor(18.75, dtype=torch.float64).exp()
+        want = ((M - 1) * 16 + 3 * e) / ((M - 1) * 16 + e)
+        got = kv4_attention(q, cache, table, lens, scale=1.0)
+        assert (got.double() - want.cuda()).abs().max() <= (2 * HALF_STEP[dtype] + 2.0 ** -18) * want
