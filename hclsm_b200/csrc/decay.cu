@@ -321,7 +321,8 @@ void simt_cut(Batch& b) {
 
 // ---- one token -------------------------------------------------------------------------------
 // A block a head: V = 4 (or 1) value dims and every kThreads / (Dv / V)-th row of the state a thread.
-// Each value of the state is read and written once; the bound is memory: 256 x 16 states of 128 x 128 in 84 us, 6.4 TB/s.
+// The decay is in two fp32 parts, as the chunks' are: one fp32 number is up to 2^-25 off it, at every token the same way, so that
+// e^-1e-6 a token would forget 1.3 % too slowly.  Each value of the state is read and written once; the bound is memory: 256 x 16 states of 128 x 128 in 84 us, 6.4 TB/s.
 struct Step {
   const void *q, *k, *v;
   void* o;
@@ -338,6 +339,7 @@ constexpr int kStepThreads = 256;
 template <typename T, int V>
 __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ Step p) {
   __shared__ float sq[128], sk[128], sv[128], red[kStepThreads * V];
+  __shared__ float2 s_g;
   pdl_wait();
   pdl_trigger();
   const int64_t bh = blockIdx.x, b = bh / p.H;
@@ -359,8 +361,9 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
     sk[tid] = io<T>::ld(static_cast<const T*>(p.k) + b * p.kb + h * p.kh + tid);
   }
   if (tid < p.Dv) sv[tid] = io<T>::ld(static_cast<const T*>(p.v) + b * p.vb + h * p.vh + tid);
-  const float g = exp2f(log2_decay(p.log_decay, h));
+  if (tid == kStepThreads - 1) s_g = chunk_decay(p.log_decay, h, 1);
   __syncthreads();
+  const float2 g = s_g;
   float acc[V] = {};
   if (g0 < groups) {
     // eight rows asked for before the first is written: s1 may be s0, which keeps a load behind a store
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
         if (d >= p.Dk) continue;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          s[i][k] = fmaf(g, s[i][k], sk[d] * sv[e + k]);
+          s[i][k] = fmaf(s[i][k], g.x, fmaf(s[i][k], g.y, sk[d] * sv[e + k]));
           acc[k] = fmaf(sq[d], s[i][k], acc[k]);
         }
         if constexpr (V == 4)

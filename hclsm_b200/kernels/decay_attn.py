@@ -160,7 +160,8 @@ def decay_attention(q, k, v, log_decay, *, state=None, lens=None, scale=None, re
 def decay_attention_step(q, k, v, log_decay, state, *, out=None, active=None, scale=None):
     """One token: o (B, H, Dv) of q, k (B, H, D) and v (B, H, Dv); ``state`` (B, H, D, Dv) fp32 takes it in, in place, or
     ``out`` gets the new state and ``state`` stays.  ``active`` (B,) bool: an entry that is not keeps its state and gives
-    zeros.  No gradients."""
+    zeros.  The state is rounded to fp32 once a token: a head that forgets less than 2^-25 of it a token keeps a value to which
+    nothing is added.  No gradients."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad
                                     or (out is not None and out.requires_grad)):
         raise NotImplementedError("decay_attention_step has no gradients: call it under torch.no_grad()")

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import hclsm_b200
-from hclsm_b200.kernels import Kv4Cache, decay_attention, kv4_attention, kv4_write
+from hclsm_b200.kernels import Kv4Cache, decay_attention, decay_attention_step, kv4_attention, kv4_write
 from hclsm_b200.kernels.decay_attn import decay_bwd
 from memory_ref import decay_grads, decay_ref
 
@@ -25,6 +25,42 @@ def _near(got, want, tol, name):
     over = ((got.double() - want).abs() - tol).max()
     assert over <= 0, f"{name}: {float(over)} over its tolerance"
     assert torch.isfinite(got).all(), name
+
+
+# ---- one token after another ----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_decay_attention_step_forgets_at_the_rate_it_is_given(dtype):
+    """Slow heads over 4096 tokens against the recurrence in 64 bits.  A token rounds each value of the state once, by at most
+    2^-24 of it and on either side alike: over n tokens the roundings' sum is some sqrt(n / 3) 2^-24 and, over a few
+    thousand values, hardly ever above six times that.  A decay of one fp32 number is up to n 2^-25 off, always the same way."""
+    n, H, D = 4096, 6, 16
+    g = torch.tensor([-1e-3, -2.0 ** -12, -1e-5, -1e-6, -3e-7, 0.0], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q, k, v = (torch.randn(n, 1, H, D, generator=gen, device="cuda").to(dtype) for _ in range(3))
+    k *= 1e-3  # the first state is most of what is there
+    state = torch.rand(1, H, D, D, generator=gen, device="cuda") + 1
+    want, decay, most = state.double(), g.double().exp().view(1, H, 1, 1), state.double()
+    for t in range(n):
+        want = decay * want + k[t].double()[..., None] * v[t].double()[..., None, :]
+        most = torch.maximum(most, want.abs())
+        o = decay_attention_step(q[t], k[t], v[t], g, state, scale=1.0)
+    tol = 6 * (n / 3) ** 0.5 * 2.0 ** -24
+    assert tol < 1.4e-5
+    # bf16: a product's last bit may be 2^-24, half the state's.  Of a head that loses less than a bit of what it loses a token
+    # over the whole run (1e-6: 8 to 16 bits a token, 4096 1e-6 of that over the run) the rest is then the same at every
+    # token and so is its rounding: such heads are compared in fp32 alone.
+    heads = [0, 1, 2, 5] if dtype == BF else list(range(H))
+    _near(state[:, heads], want[:, heads], tol * most[:, heads], "state")
+    o, want, most, q = o[:, heads], want[:, heads], most[:, heads], q[:, :, heads]
+    terms = torch.einsum("bhi,bhij->bhj", q[-1].double().abs(), most)
+    _near(o, torch.einsum("bhi,bhij->bhj", q[-1].double(), want), (tol + (D + 16) * 2.0 ** -24 + HALF_STEP[dtype]) * terms, "o")
+    # with next to nothing added a whole history of tokens is one factor
+    state = torch.rand(1, H, D, D, generator=gen, device="cuda") + 1
+    first, none = state.double(), torch.zeros_like(k[0])
+    for t in range(n):
+        decay_attention_step(none, none, none, g, state)
+    want = (g.double() * n).exp().view(1, H, 1, 1) * first
+    _near(state[:, [0, 1, 5]], want[:, [0, 1, 5]], tol * want[:, [0, 1, 5]], "state")
 
 
 # ---- lengths next to 2^31 -------------------------------------------------------------------------
