@@ -49,6 +49,15 @@ __device__ __forceinline__ int2 scan(int2 v, int2* warp_sum, int2& total) {
   return make_int2((warp ? x : 0) + s.x - v.x, (warp ? y : 0) + s.y - v.y);
 }
 
+// The entry with the i-th released or wanted page: the last one that begins at or before it.
+template <bool WANTED> __device__ __forceinline__ int entry_of(const int2* off, int entries, int i) {
+  int lo = 0;
+#pragma unroll
+  for (int step = kThreads / 2; step > 0; step >>= 1)
+    if (lo + step < entries && (WANTED ? off[lo + step].y : off[lo + step].x) <= i) lo += step;
+  return lo;
+}
+
 // One cluster (of one block where the table is small).  Each block forms all the sums, since entries are few next to
 // their pages; the pages are shared out among all threads by their place in the order, so entries of any size cost
 // the same.  Pages of an order's run: a search in the sums of up to a block's threads of entries.
@@ -56,13 +65,13 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
   namespace cg = cooperative_groups;
   __shared__ int2 warp_sum[kThreads / 32], off[kThreads + 1];
   __shared__ int2 span[kThreads];  // pages an entry had, has
-  __shared__ int bad;
+  __shared__ int bad, many;
   pdl_wait();
   pdl_trigger();
   const cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, nt = blockDim.x;
   const int me = (int)cluster.block_rank() * nt + tid, all = (int)cluster.num_blocks() * nt;
-  if (tid == 0) bad = 0;
+  if (tid == 0) bad = many = 0;
   __syncthreads();
   const int n = *p.n_free;
   const int64_t most = (int64_t)p.M << p.shift;
@@ -74,6 +83,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
     int2 done = make_int2(0, 0);
     for (int b0 = 0; b0 < p.B; b0 += nt) {
       const int b = b0 + tid, entries = min(nt, p.B - b0);
+      int32_t first = -1;  // what this thread's entry has at the first place that it wants: asked for before the sums
       if (pass == 0 || p.B > nt) {  // one round of entries stays where it is
         int2 s = make_int2(0, 0);
         if (b < p.B) {
@@ -83,6 +93,10 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
           else
             s = make_int2((int)(((int64_t)from + (1 << p.shift) - 1) >> p.shift),
                           (int)(((int64_t)to + (1 << p.shift) - 1) >> p.shift));
+          if (pass == 0 && s.y > s.x) {
+            first = p.table[(int64_t)b * p.M + s.x];
+            if (s.y > s.x + 1) many = 1;
+          }
         }
         int2 total;
         const int2 at = scan(make_int2(max(s.x - s.y, 0), max(s.y - s.x, 0)), warp_sum, total);
@@ -103,10 +117,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
           const int i = i0 + e * all;
           at[e] = nullptr;
           if (i >= count) continue;
-          int lo = 0;  // the last entry that begins at or before i: the one with the page
-#pragma unroll
-          for (int step = kThreads / 2; step > 0; step >>= 1)
-            if (lo + step < entries && (pass == 2 ? off[lo + step].y : off[lo + step].x) <= i) lo += step;
+          const int lo = pass == 2 ? entry_of<true>(off, entries, i) : entry_of<false>(off, entries, i);
           at[e] = p.table + (int64_t)(b0 + lo) * p.M + (pass == 2 ? span[lo].x + i - off[lo].y : span[lo].y + i - off[lo].x);
           page[e] = pass == 2 ? p.stack[n + (int)released - 1 - (done.y + i)] : *at[e];
         }
@@ -122,6 +133,16 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
           } else {
             *at[e] = page[e];
             p.stack[n + (int)released - 1 - (done.y + i)] = -1;
+          }
+        }
+      }
+      if (pass == 0) {  // a wanted place that holds a page: the page would be lost
+        if (first >= 0) bad = 1;
+        if (many) {
+#pragma unroll 4
+          for (int i = me; i < total.y; i += all) {
+            const int lo = entry_of<true>(off, entries, i);
+            if (p.table[(int64_t)(b0 + lo) * p.M + span[lo].x + i - off[lo].y] >= 0) bad = 1;
           }
         }
       }
@@ -183,13 +204,9 @@ __device__ __forceinline__ bool load(const Resize& p, Round& r) {
   __syncthreads();
   return fine;
 }
-// The place in the table of the i-th released or wanted page: a search for the last entry that begins at or before it, which
-// is the one with the page.
+// The place in the table of the i-th released or wanted page.
 template <bool WANTED> __device__ __forceinline__ int32_t* place(const Resize& p, const Round& r, int i) {
-  int lo = 0;
-#pragma unroll
-  for (int step = kThreads / 2; step > 0; step >>= 1)
-    if (lo + step < p.B && (WANTED ? r.off[lo + step].y : r.off[lo + step].x) <= i) lo += step;
+  const int lo = entry_of<WANTED>(r.off, p.B, i);
   return p.table + (int64_t)lo * p.M + (WANTED ? r.span[lo].x + i - r.off[lo].y : r.span[lo].y + i - r.off[lo].x);
 }
 
@@ -205,6 +222,7 @@ __global__ void __launch_bounds__(kThreads) check_kernel(const __grid_constant__
   fine = fine && n >= 0 && n <= p.P && (int64_t)n + R <= p.P && W <= (int64_t)n + R;
   if (__syncthreads_and(fine)) {  // else the places below may not exist
     for (int i = me; i < R; i += all) fine = fine && (unsigned)*place<false>(p, r, i) < (unsigned)p.P;
+    for (int i = me; i < W; i += all) fine = fine && *place<true>(p, r, i) < 0;  // a page there would be lost
     for (int i = me; i < W - R; i += all) fine = fine && (unsigned)p.stack[n - 1 - i] < (unsigned)p.P;
   }
   const int all_fine = __syncthreads_and(fine);

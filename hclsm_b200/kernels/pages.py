@@ -62,7 +62,8 @@ def pages_resize(pages: PageTable, old_lens: Tensor, new_lens: Tensor) -> None:
     The pages this releases go onto the stack, the first (entries, then places ascending) on top; then the pages that
     are wanted come off its top in the same order, so giving up what was just taken puts all back as it was.
     A request that cannot be met (a length outside the table, too few free pages, a page outside the
-    pool) changes nothing and sets the device error word."""
+    pool, a wanted place that holds a page already, as where ``old_lens`` is not what an entry has) changes nothing and
+    sets the device error word."""
     dev = _lib.require_cuda(pages.table)
     table, free = _state(pages.table, 2, "table", dev), _state(pages.free, 1, "free", dev)
     n_free = _state(pages.n_free, 1, "n_free", dev)

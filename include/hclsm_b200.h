@@ -502,7 +502,7 @@ int hclsm_kv4_attn(const hclsm_kv4_cache* c, const int32_t* table, int32_t B, in
  * *n_free places.  Entries that held old_lens[b] tokens now hold new_lens[b]: the pages this releases go onto the stack,
  * the first of them (entries, then places ascending) on top; then the pages it wants come off its top. Places that are
  * taken off or released hold -1.  A request that cannot be met (lengths outside [0, M * page], not
- * enough free pages, pages outside [0, P)) changes nothing and puts HCLSM_ERR_SHAPE in the error word.
+ * enough free pages, pages outside [0, P), wanted places that hold a page number, 0 or above) changes nothing and puts HCLSM_ERR_SHAPE in the error word.
  * page: a power of two. */
 size_t hclsm_pages_resize_workspace_size(int32_t B, int32_t M);
 int hclsm_pages_resize(int32_t* table, int32_t B, int32_t M, int32_t* stack, int32_t* n_free, int32_t P, int32_t page,

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import hclsm_b200
-from hclsm_b200.kernels import Kv4Cache, decay_attention, decay_attention_step, kv4_attention, kv4_write
+from hclsm_b200.kernels import (Kv4Cache, PageTable, decay_attention, decay_attention_step, kv4_attention, kv4_write,
+                                pages_resize)
 from hclsm_b200.kernels.decay_attn import decay_bwd
 from memory_ref import decay_grads, decay_ref
 
@@ -120,3 +121,35 @@ def test_kv4_attention_of_31_bits_of_tokens(dtype):
         want = ((M - 1) * 16 + 3 * e) / ((M - 1) * 16 + e)
         got = kv4_attention(q, cache, table, lens, scale=1.0)
         assert (got.double() - want.cuda()).abs().max() <= (2 * HALF_STEP[dtype] + 2.0 ** -18) * want
+
+
+# ---- page tables ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,columns", [(1, 256), (4, 256), (300, 64), (2000, 64), (4, 8192 * 32), (1024, 1024)])
+def test_pages_are_not_lost_where_the_old_lengths_fall_short(B, columns):
+    """A growth that is asked for again with the lengths from before it, or with lengths that understate one entry, changes
+    nothing and sets the error word, in each of the kernels (one block, a cluster, several rounds of entries, all SMs)."""
+    pages = PageTable.empty(B, columns, 5 * B + 7, page=32)
+    gen = torch.Generator(device="cuda").manual_seed(B)
+    old = torch.randint(0, 33, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    pages_resize(pages, torch.zeros_like(old), old)
+    new = old + 33 if columns > 64 else torch.full_like(old, 64)
+    pages_resize(pages, old, new)
+    assert hclsm_b200.device_error() == 0
+    parts = pages.table, pages.free, pages.n_free
+    was = [t.clone() for t in parts]
+
+    def refused(a, b):
+        pages_resize(pages, a, b)
+        assert hclsm_b200.device_error() == 1
+        assert all(torch.equal(x, y) for x, y in zip(was, parts))
+
+    refused(old, new)  # the same call again
+    last = new.clone()
+    last[B - 1] = 0  # one entry that has pages is said to have none, the others give theirs up
+    refused(last, torch.where(torch.arange(B, device="cuda") == B - 1, 40, 0))
+    pages_resize(pages, new, old)  # the lengths as they are
+    pages_resize(pages, old, new)
+    assert hclsm_b200.device_error() == 0
+    assert all(torch.equal(x, y) for x, y in zip(was, parts))
+    held = torch.cat((pages.table[pages.table >= 0], pages.free[:int(pages.n_free)]))
+    assert torch.equal(held.sort().values, torch.arange(5 * B + 7, device="cuda", dtype=torch.int32))
