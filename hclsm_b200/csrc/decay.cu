@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
   const float2 whole = chunk_decay(p.log_decay, h, kC);
+  const float factor = p.w;
   const int c_lo = seg * p.seg_chunks, c_end = min(c_lo + p.seg_chunks, chunks_of(p.L, kC));
   const int c_hi = min(c_end, chunks_of(n, kC));  // chunks with valid tokens
   const int64_t xb = b * p.x.sb + h * p.x.sh, kb = b * p.k.sb + h * p.k.sh, vb = b * p.v.sb + h * p.v.sh;
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
         float v = 0.0f;
         if (!SUMS && d < p.Dk && c < p.Dv) {
           if (p.segs > 1) v = p.part[(bh * p.segs + seg) * sz + (int64_t)d * p.Dv + c];
-          else if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? (int64_t)c * p.Dk + d : (int64_t)d * p.Dv + c)];
+          else if (p.init) v = p.init[bh * sz + (p.init_t ? (int64_t)c * p.Dk + d : (int64_t)d * p.Dv + c)];
         }
         S[q][i][e] = v;
       }
@@ -111,11 +112,11 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
     }
     if (tid < kC) {
       const int place = p.rev ? m - 1 - tid : tid;
-      s.w[tid] = tid < m ? exp2f(l2 * (float)(m - 1 - place + r)) : 0.0f;
+      s.w[tid] = tid < m ? factor * exp2f(l2 * (float)(m - 1 - place + r)) : 0.0f;
     }
     __syncthreads();
     if (!SUMS) {
-      {  // P = (X K^T) g^|i - j|: rows 4 ty + i, columns tx + 16 j
+      {  // P = (X K^T) w g^|i - j|: rows 4 ty + i, columns tx + 16 j
         float a[4][4] = {};
 #pragma unroll 4
         for (int d = 0; d < DP; d += 4) {
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int row = ty * 4 + i, col = tx + 16 * j, lag = p.rev ? col - row : row - col;
-            s.p[row * kPs + col] = lag >= 0 ? a[i][j] * exp2f(l2 * (float)lag) : 0.0f;
+            s.p[row * kPs + col] = lag >= 0 ? a[i][j] * (factor * exp2f(l2 * (float)lag)) : 0.0f;
           }
       }
       __syncthreads();
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int d = q * 64 + ty * 4 + i, c = e0 + tx * 4 + e;
-          if (d < p.Dk && c < p.Dv) out[(int64_t)d * p.Dv + c] = SUMS ? S[q][i][e] : p.last_f * S[q][i][e];
+          if (d < p.Dk && c < p.Dv) out[(int64_t)d * p.Dv + c] = S[q][i][e];
         }
   }
   if (!SUMS)  // rows behind the length
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Batch
   __syncthreads();
   if (!in) return;
   float v = 0.0f;
-  if (p.init) v = p.init_f * p.init[bh * sz + (p.init_t ? i % p.Dv * p.Dk + i / p.Dv : i)];
+  if (p.init) v = p.init[bh * sz + (p.init_t ? i % p.Dv * p.Dk + i / p.Dv : i)];
   const float2 whole = s_g[0], cut_off = s_g[1];
   for (int it = 0; it < segs; it += 8) {
     if (it > 0) ask(it);
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Batch
       }
     }
   }
-  if (p.last) p.last[bh * sz + i] = p.last_f * v;
+  if (p.last) p.last[bh * sz + i] = v;
 }
 
 int join(const Batch& b, int chunk, cudaStream_t st) {
@@ -419,7 +420,7 @@ Pass base(const hclsm_decay_args* a) {
   Pass p = {};
   p.log_decay = a->log_decay, p.lens = a->lens;
   p.B = a->B, p.L = a->L, p.H = a->H;
-  p.f = a->scale, p.init_f = p.last_f = 1.0f;
+  p.w = 1.0f, p.f = a->scale;
   p.err = device_err_ptr();
   return p;
 }
@@ -441,14 +442,14 @@ Pass grad_v(const hclsm_decay_args* a) {
   Pass p = base(a);
   p.x = view(a, a->k), p.k = view(a, a->q), p.v = view(a, a->dout), p.y = a->dv;
   p.Dk = a->D, p.Dv = a->Dv, p.rev = 1;
-  p.init = a->ds1, p.init_f = 1.0f / a->scale, p.last = a->ds0, p.last_f = a->scale;
+  p.init = a->ds1, p.last = a->ds0, p.w = a->scale, p.f = 1.0f;
   return p;
 }
 Pass grad_k(const hclsm_decay_args* a) {
   Pass p = base(a);
   p.x = view(a, a->v), p.k = view(a, a->dout), p.v = view(a, a->q), p.y = a->dk;
   p.Dk = a->Dv, p.Dv = a->D, p.rev = 1;
-  p.init = a->ds1, p.init_t = 1, p.init_f = 1.0f / a->scale;
+  p.init = a->ds1, p.init_t = 1, p.w = a->scale, p.f = 1.0f;
   return p;
 }
 

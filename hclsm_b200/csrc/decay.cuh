@@ -4,17 +4,19 @@
 //
 // Everything is one kind of pass over x, k, v (rows of a head's tokens) in either direction of time:
 //
-//   T <- g T + k_t^T v_t,   y_t = f x_t T      t ascending or, reversed, descending from the last valid token
+//   T <- g T + w k_t^T v_t,   y_t = f x_t T      t ascending or, reversed, descending from the last valid token
 //
-//   forward:  (x, k, v) = (q, k, v), ascending from S_{-1}, f = scale; T ends as the new state
-//   dq:       (dO, v, k), ascending from S_{-1}^T
-//   dv:       (k, q, dO), descending from dS / scale, where the first token meets T without a decay, and T
-//             ends as g T = dS_{-1} / scale
-//   dk:       (v, dO, q), descending from dS^T / scale
+//   forward:  (x, k, v) = (q, k, v), ascending from S_{-1}, w = 1, f = scale; T ends as the new state
+//   dq:       (dO, v, k), ascending from S_{-1}^T, w = 1, f = scale
+//   dv:       (k, q, dO), descending from dS, w = scale, f = 1, where the first token meets T without a decay, and T
+//             ends as g T = dS_{-1}
+//   dk:       (v, dO, q), descending from dS^T, w = scale, f = 1
+//
+// (dS knows no scale: a T that is multiplied by it at the end would have to start from dS / scale, which may overflow.)
 //
 // By chunks of C tokens, i and j a token's place among the m valid ones in the pass's order and r = 1 where reversed:
 //
-//   y_i = f [ sum_{j <= i} g^{i-j} (x_i . k_j) v_j  +  g^{i+1-r} x_i T ],   T <- g^m T + sum_j g^{m-1-j+r} k_j^T v_j
+//   y_i = f [ sum_{j <= i} w g^{i-j} (x_i . k_j) v_j  +  g^{i+1-r} x_i T ],   T <- g^m T + sum_j w g^{m-1-j+r} k_j^T v_j
 //
 // Chunks lie on multiples of C in memory in both directions, so the incomplete one is the last one.  Where the heads
 // do not fill the GPU their tokens are cut into segments of whole chunks: the segments' own sums (sums pass), their
@@ -36,7 +38,7 @@ struct Pass {
   const int32_t* lens;        // (B) or null
   float* part;                // (B * H, segs, Dk, Dv): sums, then the segments' first states
   int init_t;                 // init is (B, H, Dv, Dk)
-  float init_f, last_f, f;    // factors of init, last and y
+  float w, f;                 // factors of the tokens' weights and of y
   int rev;
   int B, L, H, Dk, Dv;
   int segs, seg_chunks;       // segments a head, chunks of a segment

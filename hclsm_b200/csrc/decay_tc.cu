@@ -2,9 +2,9 @@
 //
 // A block takes one segment of one head, chunk after chunk of 128 tokens:
 //   A = x k^T                 128 x 128, fp32 in TMEM
-//   P = A g^|i-j| as bf16 over A (the A operand of the next product), zero outside the pass's past
+//   P = A w g^|i-j| as bf16 over A (the A operand of the next product), zero outside the pass's past
 //   y = f (P v + g^{i+1-r} x T)   two accumulators, joined by the thread of the row
-//   T = g^m T + (w k)^T v     the product in TMEM, T in registers in fp32, w_j = g^{m-1-j+r}
+//   T = g^m T + (w k)^T v     the product in TMEM, T in registers in fp32, w_j = w g^{m-1-j+r}
 // The state is returned in fp32, so w k is not rounded to bf16: it enters as NP = 3 bf16 pieces (2 where the state is
 // only read by later chunks), smallest first.  The tensor cores cut fp32 sums off instead of rounding them, always
 // towards zero: so only a chunk's sum is theirs, and chunks are added in registers.  For x T the state is rounded
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
                 *sT = sV + Sh::kV + Sh::kY;
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ __align__(16) float s_pow[32];  // g^(distance of a block's j to its end on the later side)
+  __shared__ __align__(16) float s_pow[32];  // w g^(distance of a block's j to its end on the later side)
   __shared__ float2 s_g[2];  // decays of a whole chunk and of the incomplete one
   constexpr int kBars = 13;
   __shared__ uint64_t bars[kBars];
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
   const int h = (int)(bh - b * p.H), r = p.rev ? 1 : 0;
   const int n = length(p, b);
   const float l2 = log2_decay(p.log_decay, h);
-  if (tid < 32) s_pow[tid] = ex2(l2 * (float)(r ? tid : 31 - tid));
+  if (tid < 32) s_pow[tid] = p.w * ex2(l2 * (float)(r ? tid : 31 - tid));
   if (warp == kTmaWarp && lane < 2) s_g[lane] = chunk_decay(p.log_decay, h, lane ? n % kTok : kTok);
   tc_fence_before();
   __syncthreads();
@@ -266,13 +266,12 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
       const float* from = p.segs > 1 ? p.part + (bh * p.segs + seg) * sz : p.init ? p.init + bh * sz : nullptr;
       const bool turned = p.segs == 1 && p.init_t;
       const int64_t at = turned ? row + (int64_t)y0 * p.Dk : (int64_t)row * p.Dv + y0, step = turned ? p.Dk : 1;
-      const float f = p.segs > 1 ? 1.0f : p.init_f;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += 16) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          w[e] = from && row < p.Dk && y0 + c + e < p.Dv ? __float_as_uint(f * from[at + (c + e) * step]) : 0u;
+          w[e] = from && row < p.Dk && y0 + c + e < p.Dv ? __float_as_uint(from[at + (c + e) * step]) : 0u;
         tmem_st16(tT + c, w);
       }
       tmem_wait_st();
@@ -317,7 +316,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
       // the pieces of w k
       if (!(ok = wait_all(k_full, it))) break;
       const int c0 = half * (kDims / 8);
-      const float w = ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
+      const float w = p.w * ex2(l2 * (float)(p.rev ? row + 1 : m - 1 - row));
 #pragma unroll 1
       for (int c = 0; c < kDims / 8; c += 2) weigh_row<NP, 2>(smem_u32(sK), smem_u32(sP), Sh::kX, row, c0 + c, w);
       if (m < kTok) {
@@ -343,7 +342,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
       for (int e = 0; e < kCols; e += 4)
         if (y0 + e < p.Dv)
           *reinterpret_cast<float4*>(to + e) =
-              make_float4(p.last_f * T[e / 2].x, p.last_f * T[e / 2].y, p.last_f * T[e / 2 + 1].x, p.last_f * T[e / 2 + 1].y);
+              make_float4(T[e / 2].x, T[e / 2].y, T[e / 2 + 1].x, T[e / 2 + 1].y);
     }
   } else {
     // ---- the rows ---------------------------------------------------------------------------
@@ -352,6 +351,8 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
     constexpr int kCols = DY / WG, kBlocks = 4 / WG;
     const int y0 = half * kCols, i0 = (warp & 3) * 32;
     const bool wide = p.Dv % 16 == 0 && reinterpret_cast<uintptr_t>(p.y) % 32 == 0;  // rows of whole 32 bytes
+    // the log2 of a decay above which g^-31 stays below 2^125 and w g^31 above 2^-125
+    const float near = fminf(-4.0f - fminf(__log2f(p.w), 0.0f) * (1.0f / 31.0f), 0.0f);
     bool ok = true;
     for (int it = 0; it < chunks && ok; ++it) {
       const int t0 = first_token(it), m = min(n - t0, kTok);
@@ -369,9 +370,10 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
           // the columns [first, last] count
           const int first = p.rev ? max(row - j0, 0) : 0, last = min(p.rev ? 31 : min(row - j0, 31), m - 1 - j0);
           const uint32_t on = first <= last && first < 32 ? (0xffffffffu >> (31 - (last - first))) << first : 0u;
-          if (past || l2 > -4.0f) {
+          if (past || l2 > near) {
             // g^|i-j| as the power of i's distance to the block's end on the later side times that of j's; on the
-            // diagonal the first is up to g^-31, which fp32 holds above 2^-4: so the score comes last
+            // diagonal the first is up to g^-31 and the second, with w, down to w g^31, which fp32 holds above `near`: so the
+            // score comes last
             const float a = ex2(l2 * (float)(p.rev ? j0 - row : row - j0 - 31));
             tmem_wait_ld();
             tmem_pin<32>(v);
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(Shape<DX, DY, NP, SMALL>::kThreads, Shape<DX, 
             tmem_wait_ld();
             tmem_pin<32>(v);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] *= ex2(fmaf(step, (float)e, base));
+            for (int e = 0; e < 32; ++e) v[e] *= p.w * ex2(fmaf(step, (float)e, base));
           }
           if (!past || j0 + 32 > m) {  // select, not multiply: a later token's score may be NaN, its power inf
 #pragma unroll
@@ -651,7 +653,8 @@ __global__ void __launch_bounds__(SumShape<DX, DY>::kThreads, SumShape<DX, DY>::
       float* to = p.part + (bh * p.segs + seg) * ((int64_t)p.Dk * p.Dv) + (int64_t)row * p.Dv + y0;
 #pragma unroll
       for (int e = 0; e < kCols; e += 4)
-        if (y0 + e < p.Dv) *reinterpret_cast<float4*>(to + e) = make_float4(T[e], T[e + 1], T[e + 2], T[e + 3]);
+        if (y0 + e < p.Dv)
+          *reinterpret_cast<float4*>(to + e) = make_float4(p.w * T[e], p.w * T[e + 1], p.w * T[e + 2], p.w * T[e + 3]);
     }
   }
   tc_fence_before();

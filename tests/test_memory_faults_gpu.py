@@ -28,6 +28,37 @@ def _near(got, want, tol, name):
     assert torch.isfinite(got).all(), name
 
 
+# ---- scales -----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,L,H,D,Dv", [(2, 150, 6, 64, 64), (1, 2500, 6, 64, 64), (40, 200, 6, 64, 64), (1, 1700, 6, 128, 128),
+                                        (2, 150, 6, 20, 8)])
+@pytest.mark.parametrize("scale,up,dstate", [(1e-39, 1.0, 1.0), (1e-20, 1.0, 1e30), (64.0, 1.0, 1.0), (1e20, 1e-20, 1.0)])
+def test_decay_attention_gradients_of_any_scale(B, L, H, D, Dv, scale, up, dstate, dtype):
+    """The final state's gradient reaches k, v and the first state without the scale, however small that is; the other
+    terms have it.  Decays on both sides of where the powers on the diagonal are formed in two ways."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+
+    def r(*s, f=1.0):
+        return torch.randn(*s, generator=gen, device="cuda") * f
+
+    q, k, v = r(B, L, H, D).to(dtype), r(B, L, H, D, f=D ** -0.5).to(dtype), r(B, L, H, Dv).to(dtype)
+    do, S0, dS = r(B, L, H, Dv, f=up).to(dtype), r(B, H, D, Dv), r(B, H, D, Dv, f=dstate)
+    g = torch.tensor([-0.01, -2.6, -2.65, -2.75, -2.78, -20.0], device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v, S0)]
+    o, S = decay_attention(q, k, v, g, state=S0, scale=scale, return_state=True)
+    grads = torch.autograd.grad((o, S), leaves, (do, dS))
+    q, k, v, S0 = (t.detach() for t in leaves)
+    fp32, e = (L + D + Dv + 256) * 2.0 ** -24, HALF_STEP[dtype]
+    want = decay_grads(q, k, v, g, S0, None, scale, do, dS)
+    most = decay_grads(q.abs(), k.abs(), v.abs(), g, S0.abs(), None, scale, do.abs(), dS.abs())
+    # a power of a decay below 2^-126 is zero, times the product of a row (entries below 8) and the gradient of the state; and
+    # each bf16 weight below 2^-126 (of 128 in a chunk, or of the state) is off by 2^-134, times a row's entry, which is less
+    low = 2.0 ** -126 * 128 * 8 * max(8.0, float(dS.abs().max()))
+    for n, got, w, m in zip(("dq", "dk", "dv", "dS0"), grads, want, most):
+        half = e if n != "dS0" else 0.0
+        _near(got, w, half * w.abs() + (half + fp32) * m + low, n)
+
+
 # ---- one token after another ----------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_decay_attention_step_forgets_at_the_rate_it_is_given(dtype):
