@@ -242,6 +242,11 @@ def like(t, shape, dtype, name, device):
     return t if t.is_contiguous() else t.contiguous()
 
 
+def changed(*tensors):
+    """A kernel has changed these in place: a backward that saved one of them refuses, as after any such change."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def in_dual_level() -> bool:
     """Whether a tensor can have a forward-mode tangent at all."""
     return getattr(forward_ad, "_current_level", 0) >= 0

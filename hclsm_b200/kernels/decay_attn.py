@@ -209,5 +209,5 @@ def decay_attention_step(q, k, v, log_decay, state, *, out=None, active=None, sc
         log_decay.data_ptr(), state.data_ptr(), out.data_ptr(), 0, 0, 0, B, 1, H, D, Dv, _lib.dtype_code(dtype),
         _check_scale(scale, D))
     _lib.check(_lib.load().hclsm_decay_attn_step(a, _lib.ptr(active), _lib.stream_ptr(dev)), "hclsm_decay_attn_step")
-    torch.autograd.graph.increment_version(out)  # a backward that saved it refuses, as after any change in place
+    _lib.changed(out)
     return o

@@ -110,6 +110,7 @@ def kv4_write(cache: Kv4Cache, k: Tensor, v: Tensor, slots: Tensor) -> None:
     k, v = _lib.rows16(k), _lib.rows16(v)
     _lib.check(_lib.load().hclsm_kv4_write(c, _lib.VIEW.pack(*_lib.view_args(k)), _lib.VIEW.pack(*_lib.view_args(v)),
                                            slots.data_ptr(), B, n, _lib.stream_ptr(dev)), "hclsm_kv4_write")
+    _lib.changed(cache.k, cache.v, cache.k_scale, cache.v_scale)
 
 
 def kv4_read(cache: Kv4Cache, table: Tensor, lens: Tensor | None = None):

@@ -123,6 +123,7 @@ def kv8_write(cache: Kv8Cache, k: Tensor, v: Tensor, start: Tensor, count: Tenso
     _lib.check(_lib.load().hclsm_kv8_write(c, _lib.VIEW.pack(*_lib.view_args(k)),
                                            _lib.VIEW.pack(*_lib.view_args(v)), k.shape[1], start.data_ptr(),
                                            _lib.ptr(count), _lib.stream_ptr(dev)), "hclsm_kv8_write")
+    _lib.changed(cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_tail, cache.v_tail)
 
 
 def kv8_read(cache: Kv8Cache, lens: Tensor | None = None):

@@ -82,6 +82,7 @@ def pages_resize(pages: PageTable, old_lens: Tensor, new_lens: Tensor) -> None:
     _lib.check(lib.hclsm_pages_resize(table.data_ptr(), B, M, free.data_ptr(), n_free.data_ptr(), free.numel(), pages.page,
                                       old.data_ptr(), new.data_ptr(), _lib.ptr(ws), n, _lib.stream_ptr(dev)),
                "hclsm_pages_resize")
+    _lib.changed(table, free, n_free)
 
 
 def page_slots(table: Tensor, start: Tensor, n: int, *, count: Tensor | None = None, page: int = 32) -> Tensor:

@@ -3,8 +3,8 @@ import pytest
 import torch
 
 from hclsm_b200 import _lib
-from hclsm_b200.kernels import (Kv4Cache, Kv8Cache, kv4_attention, kv4_read, kv4_write, kv8_attention, kv8_read,
-                                kv8_write)
+from hclsm_b200.kernels import (Kv4Cache, Kv8Cache, PageTable, decay_attention_step, kv4_attention, kv4_read, kv4_write,
+                                kv8_attention, kv8_read, kv8_write, pages_resize)
 
 BF, I32 = torch.bfloat16, torch.int32
 
@@ -91,6 +91,34 @@ def test_kv8_tensors_that_were_changed_where_they_are(lib):
             with pytest.raises(ValueError):
                 call()
         assert not lib.calls
+
+
+def test_changes_in_place_move_the_versions(lib):
+    """A backward that saved a tensor which a call has changed since says so."""
+    c4, c8 = Kv4Cache.empty(4, 1, 32, page=32, device="cpu"), Kv8Cache.empty(2, 64, 1, 32, device="cpu")
+    x, state = torch.zeros(2, 3, 1, 32, dtype=BF), torch.zeros(2, 1, 32, 32)
+    at, slots = torch.zeros(2, dtype=I32), torch.zeros(2, 3, dtype=I32)
+    pages = PageTable.empty(2, 64, 8, device="cpu")
+    step, out = x[:, 0].float(), state.clone()
+    for call, changed, kept in (
+            (lambda: kv4_write(c4, x, x, slots), (c4.k, c4.v, c4.k_scale, c4.v_scale), (x, slots)),
+            (lambda: kv8_write(c8, x, x, at), (c8.k, c8.v, c8.k_scale, c8.v_scale, c8.k_tail, c8.v_tail), (x, at)),
+            (lambda: pages_resize(pages, at, at), (pages.table, pages.free, pages.n_free), (at,)),
+            (lambda: decay_attention_step(step, step, step, torch.zeros(1), state), (state,), (step,)),
+            (lambda: decay_attention_step(step, step, step, torch.zeros(1), state, out=out), (out,), (step, state))):
+        before, others = [t._version for t in changed], [t._version for t in kept]
+        call()
+        assert all(t._version > n for t, n in zip(changed, before))
+        assert [t._version for t in kept] == others
+        with torch.inference_mode():
+            call()
+    w = torch.ones(1, requires_grad=True, dtype=BF)
+    y = (w * c4.k_scale).sum()
+    kv4_read(c4, slots), kv4_attention(x, c4, slots)
+    y.backward(retain_graph=True)
+    kv4_write(c4, x, x, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 # ---- lengths next to 2^31 -------------------------------------------------------------------------
