@@ -52,7 +52,7 @@ __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast
 // One block: 64 value dims of one segment of one head.  SUMS: the segment's own sum of k^T v alone.
 // The state stays in registers (4 x 4 values a thread and 64 rows) between chunks; shared memory holds the copy that
 // the queries read.  A chunk is 1.05 M multiplications of 8192 cycles at full rate, so the FMA pipe is the bound, and
-// latency where blocks are few: 3 x 333 ragged tokens, 6 heads of 64, forward + backward 82 us (239 without segments).
+// latency where blocks are few: 3 x 333 ragged tokens, 6 heads of 64, forward + backward 84 us (239 without segments).
 template <typename T, int DP, bool SUMS>
 __global__ void __launch_bounds__(kThreads) simt_kernel(const __grid_constant__ Batch bt) {
   const Pass& p = bt.p[blockIdx.x % bt.n];

@@ -546,8 +546,9 @@ void plan(Attn& p, int dtype) {
   }
   const int64_t most = (keys + 127) / 128;
   if (s > most) s = most;
-  // Up to eight splits join in their cluster's shared memory.  Up to sixteen are made eight: a second launch costs more than
-  // fewer blocks (slots, write and attention of one token over 8 x 2048, 6 heads of 64: 16.5 us with it, 12.5 without).
+  // Up to eight splits join in their cluster's shared memory.  Nine to sixteen are made eight, fewer waves than above: up to
+  // some 16384 tokens a second launch costs more (slots, write and attention of one token over 8 x 2048, 6 heads of 64: 16.5 us
+  // with it, 12.5 without; 20 x 16384, 8 key heads of 128: 91 and 86), for longer ones less (20 x 65536: 258 and 271).
   if (s <= 16) s = s < 8 ? s : 8;
   p.splits = s < 1 ? 1 : (int)s;
   p.cluster = p.splits > 1 && p.splits <= 8;

@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(const __grid_constant_
 }
 
 // ---- large tables: a kernel that checks and one that moves, over all SMs ---------------------------------
-// Up to kThreads entries.  131072 pages: 7 us in the two, 22 in one cluster.
+// Up to kThreads entries.  131072 pages: 6 to 7 us in the two, 22 in one cluster.
 constexpr int kBlocks = 128;
 
 struct Round {

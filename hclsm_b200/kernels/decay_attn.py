@@ -146,7 +146,9 @@ def decay_attention(q, k, v, log_decay, *, state=None, lens=None, scale=None, re
     b's first lens[b] tokens count (clamped to [0, L]); the others may hold anything, NaN included, and their
     outputs and gradients are zeros.  A token that counts and is not finite spreads to the
     tokens of its chunk (128; 64 in fp32), the earlier ones too.  ``scale`` > 0, default D ** -0.5.  float32 or bfloat16, head dims up to
-    128; sums and states in fp32.  Differentiable in q, k, v and state, not in log_decay; bit-reproducible.
+    128; sums and states in fp32.  bfloat16 runs on the tensor cores where dims, strides and addresses are
+    whole 16 bytes and no dim of more than one is expanded (in the backward those of o's gradient too), else on the
+    much slower FMA pipe.  Differentiable in q, k, v and state, not in log_decay; bit-reproducible.
     """
     args = _prepare(q, k, v, log_decay, state, lens, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
