@@ -132,7 +132,9 @@ def kv4_attention(q: Tensor, cache: Kv4Cache, table: Tensor, lens: Tensor | None
                   scale: float | None = None) -> Tensor:
     """softmax(scale q k^T) v of q (B, Lq, H, D), in the cache's dtype, over the first ``lens[b]`` tokens (default all;
     clamped to the table's) of the pages that table (B, M) names; H is a multiple of Hkv.  An entry without tokens
-    gives zeros; tokens of a page outside the cache do not count and set the device error word.  No gradients."""
+    gives zeros; tokens of a page outside the cache do not count and set the device error word.
+    Weights of up to 2^8 times values are summed in fp32 before they are divided by the weights' sum: values
+    above some 2^119 over the number of tokens overflow.  No gradients."""
     _no_derivatives("kv4_attention", cache, q)
     c, Hkv, _, D, dev, index = cache._args()
     if q.get_device() != index:
